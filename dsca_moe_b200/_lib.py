@@ -97,6 +97,29 @@ class QosArgs(ctypes.Structure):
                 ("first_counts", _vp), ("partial", _vp), ("done_counter", _vp)]
 
 
+# ---- include/dsca_b200_block.h
+NORM_Q_NONE, NORM_Q_E4M3, NORM_Q_SPLIT = range(3)
+NORM_MAX_D = 32768
+FEW_TOKENS = 32
+FEW_COUNTER_BYTES = 256
+_i64 = ctypes.c_int64
+
+
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("residual", _vp), ("weight", _vp), ("rows", _i), ("d", _i), ("dtype", _i),
+                ("weight_dtype", _i), ("ld_x", _i64), ("ld_residual", _i64), ("ld_y", _i64), ("ld_residual_out", _i64),
+                ("eps", ctypes.c_float), ("quant", _i), ("y", _vp), ("residual_out", _vp), ("q", _vp), ("scale", _vp)]
+
+
+class FewArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("w_router", _vp), ("w_shared_gate", _vp), ("T", _i), ("d", _i), ("E", _i), ("top_k", _i),
+                ("weights", _i), ("mode", _i), ("norm_topk", _i), ("act", _i), ("inter", _i), ("n1p", _i), ("ip", _i),
+                ("dp", _i), ("shared_inter", _i), ("shared_n1p", _i), ("shared_ip", _i), ("w1", _vp), ("w2", _vp),
+                ("ws1", _vp), ("ws2", _vp), ("w1_scale", _vp), ("w2_scale", _vp), ("ws1_scale", _vp),
+                ("ws2_scale", _vp), ("out", _vp), ("logits", _vp), ("topk_ids", _vp), ("topk_w", _vp),
+                ("expert_index", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
+
+
 # every symbol include/dsca_b200.h declares
 EXPORTED = ["dsca_version", "dsca_status_string", "dsca_device_info", "dsca_router_topk",
             "dsca_dispatch_scan", "dsca_permute", "dsca_grouped_ffn", "dsca_combine",
@@ -105,6 +128,8 @@ EXPORTED = ["dsca_version", "dsca_status_string", "dsca_device_info", "dsca_rout
             "dsca_ep_plan", "dsca_ep_plan_counts", "dsca_ep_priority", "dsca_ep_group_order", "dsca_ep_dispatch", "dsca_ep_wait", "dsca_ep_plan_eval", "dsca_ipc_export",
             "dsca_ipc_import", "dsca_ipc_close", "dsca_ep_read_plan", "dsca_ep_region_alloc",
             "dsca_ep_region_free", "dsca_ep_return", "dsca_qos_priority", "dsca_router_pack_i8", "dsca_split_rows"]
+# every symbol include/dsca_b200_block.h declares
+EXPORTED_BLOCK = ["dsca_rms_norm", "dsca_few_workspace_bytes", "dsca_moe_few"]
 STATIC_SCRATCH_BYTES = 16 << 20
 
 _LIB = None
@@ -164,7 +189,11 @@ def load():
     lib.dsca_plan_layout.argtypes = [_vp, _i, _i, _i, p(_i), _vp, _vp, _vp, _vp, _vp, _vp, _vp]
     lib.dsca_check_error.argtypes = [_vp, _vp]
     lib.dsca_exp_neg_eval.argtypes = [_vp, _vp, _i, _vp]
-    for name in EXPORTED:
+    lib.dsca_rms_norm.argtypes = [p(RmsNormArgs), _vp]
+    lib.dsca_few_workspace_bytes.restype = ctypes.c_size_t
+    lib.dsca_few_workspace_bytes.argtypes = [_i, _i, _i, _i]
+    lib.dsca_moe_few.argtypes = [p(FewArgs), _vp]
+    for name in EXPORTED + EXPORTED_BLOCK:
         getattr(lib, name).restype = getattr(lib, name).restype or _i
     lib.dsca_version.restype = ctypes.c_char_p
     lib.dsca_status_string.restype = ctypes.c_char_p

@@ -26,7 +26,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
               "--expt-relaxed-constexpr", "-I" + INCLUDE] + ARCH
 CU_SOURCES = ["router.cu", "router_tc.cu", "dispatch.cu", "gemm_sm100.cu", "gemm_sm100_pair.cu", "gemm_sm100_fp8.cu", "gemm_sm100_fp8t.cu", "gemm_simt.cu", "abi.cu",
-              "ffn_static_scratch.cu", "ep.cu", "qos.cu"]
+              "ffn_static_scratch.cu", "ep.cu", "qos.cu", "norm.cu", "moe_few.cu"]
 CXX_SOURCES = ["plan.cpp"]
 
 
@@ -42,7 +42,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     # every header of the package (a change to any of them rebuilds every object)
     headers = sorted(os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith((".cuh", ".h")))
-    headers.append(os.path.join(INCLUDE, "dsca_b200.h"))
+    headers += [os.path.join(INCLUDE, h) for h in ("dsca_b200.h", "dsca_b200_block.h")]
     objs = []
     for src in CU_SOURCES:
         s = os.path.join(CSRC, src)

@@ -63,6 +63,7 @@ class QoSMoEConfig:
     shared_expert: object = None   # module with gate_proj / up_proj / down_proj, or None
     shared_expert_gate: object = None  # Linear(d, 1) or None
     process_group: object = None   # torch.distributed group for world_size > 1
+    few_tokens: int = 0            # calls of at most this many tokens run as one kernel (0 = never)
     collect_stats: bool = False    # per-forward latency / token statistics (host syncs)
     # forward returns (h, (router_logits, expert_index)) — the reference contract, which
     # transformers-4.x SwitchTransformersLayerFF unpacks — or h alone (transformers-5.x callers);

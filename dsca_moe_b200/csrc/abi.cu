@@ -1,8 +1,10 @@
 // extern "C" entry points: argument validation, then the kernel launches in router.cu,
-// dispatch.cu, gemm_sm100.cu and gemm_simt.cu.  No entry point allocates device memory.
+// dispatch.cu, gemm_sm100.cu, gemm_simt.cu, norm.cu and moe_few.cu.  No entry point allocates
+// device memory.
 #include <stdio.h>
 
 #include "common.cuh"
+#include "dsca_b200_block.h"
 
 namespace dsca {
 int launch_router(const dsca_router_args* p, cudaStream_t stream, const float* logits_in = nullptr);
@@ -21,6 +23,9 @@ int launch_grouped_ffn_fp8_tmem(const dsca_ffn_args* f, int num_sms, cudaStream_
 int launch_grouped_ffn_f8_split(const dsca_ffn_args* f, int num_sms, cudaStream_t stream);
 int launch_split_rows(const void* src, int ld, int rows, const int32_t* rows_dev, int K, void* dst, float* inv_scale,
                       cudaStream_t stream);
+int launch_rms_norm(const dsca_rms_norm_args* a, cudaStream_t stream);
+int launch_moe_few(const dsca_few_args* a, int num_sms, cudaStream_t stream);
+size_t few_workspace_bytes(int T, int k, int inter, int shared_inter);
 }  // namespace dsca
 
 namespace {
@@ -243,6 +248,76 @@ int dsca_qos_priority(const dsca_qos_args* a, dsca_stream_t stream) {
   if ((a->partial == nullptr) != (a->done_counter == nullptr)) return DSCA_ERR_BAD_ARG;
   if (a->top_k > DSCA_MAX_TOPK) return DSCA_ERR_BAD_ARG;
   return dsca::launch_qos(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream) {
+  if (a == nullptr || a->rows < 0 || a->d <= 0) return DSCA_ERR_BAD_ARG;
+  if (a->dtype != DSCA_BF16 && a->dtype != DSCA_F32) return DSCA_ERR_BAD_ARG;
+  if (a->weight_dtype != a->dtype && a->weight_dtype != DSCA_F32) return DSCA_ERR_BAD_ARG;
+  if (a->quant != DSCA_NORM_Q_NONE && a->quant != DSCA_NORM_Q_E4M3 && a->quant != DSCA_NORM_Q_SPLIT)
+    return DSCA_ERR_BAD_ARG;
+  if (!(a->eps >= 0.0f)) return DSCA_ERR_BAD_ARG;
+  if (a->d > DSCA_NORM_MAX_D) return DSCA_ERR_CAPACITY;
+  const bool quant = a->quant != DSCA_NORM_Q_NONE;
+  if (a->quant == DSCA_NORM_Q_SPLIT && (a->dtype != DSCA_BF16 || a->d % 8 != 0)) return DSCA_ERR_BAD_ARG;
+  if (a->rows == 0) return DSCA_OK;
+  if (a->x == nullptr || a->weight == nullptr || (a->y == nullptr && !quant)) return DSCA_ERR_BAD_ARG;
+  if (quant && (a->q == nullptr || a->scale == nullptr)) return DSCA_ERR_BAD_ARG;
+  if (a->ld_x < a->d || (a->residual && a->ld_residual < a->d) || (a->y && a->ld_y < a->d) ||
+      (a->residual_out && a->ld_residual_out < a->d))
+    return DSCA_ERR_BAD_ARG;
+  const uintptr_t esz = a->dtype == DSCA_BF16 ? 2 : 4, wsz = a->weight_dtype == DSCA_BF16 ? 2 : 4;
+  const void* ptrs[] = {a->x, a->residual, a->y, a->residual_out};
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % esz != 0) return DSCA_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(a->weight) % wsz != 0 || reinterpret_cast<uintptr_t>(a->scale) % 4 != 0)
+    return DSCA_ERR_BAD_ARG;
+  return dsca::launch_rms_norm(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t dsca_few_workspace_bytes(int T, int top_k, int inter, int shared_inter) {
+  if (T < 0 || T > DSCA_FEW_TOKENS || top_k <= 0 || top_k > DSCA_MAX_TOPK || inter <= 0 || shared_inter < 0) return 0;
+  return dsca::few_workspace_bytes(T, top_k, inter, shared_inter);
+}
+
+int dsca_moe_few(const dsca_few_args* a, dsca_stream_t stream) {
+  if (a == nullptr || a->T < 0 || a->d <= 0 || a->E <= 0 || a->inter <= 0) return DSCA_ERR_BAD_ARG;
+  if (a->weights != DSCA_BF16 && a->weights != DSCA_F32 && a->weights != DSCA_F8E4M3) return DSCA_ERR_BAD_ARG;
+  if (a->mode != DSCA_ROUTE_SWITCH_TOP1 && a->mode != DSCA_ROUTE_SOFTMAX_TOPK) return DSCA_ERR_BAD_ARG;
+  if (a->act != DSCA_ACT_RELU && a->act != DSCA_ACT_SWIGLU) return DSCA_ERR_BAD_ARG;
+  const int k = a->mode == DSCA_ROUTE_SWITCH_TOP1 ? 1 : a->top_k;
+  if (k <= 0 || k > DSCA_MAX_TOPK || k > a->E) return DSCA_ERR_BAD_ARG;
+  const bool shared = a->w_shared_gate != nullptr;
+  if (a->T > DSCA_FEW_TOKENS || a->E + (shared ? 1 : 0) > DSCA_MAX_EXPERTS) return DSCA_ERR_CAPACITY;
+  // the packing of dsca_ffn_args
+  const bool glu = a->act == DSCA_ACT_SWIGLU, fp8 = a->weights == DSCA_F8E4M3;
+  if (a->n1p <= 0 || a->n1p % 256 != 0 || a->ip != (glu ? a->n1p / 2 : a->n1p) || a->inter > a->ip || a->dp < a->d)
+    return DSCA_ERR_BAD_ARG;
+  if (shared && (a->shared_inter <= 0 || a->shared_n1p <= 0 || a->shared_n1p % 256 != 0 ||
+                 a->shared_ip != (glu ? a->shared_n1p / 2 : a->shared_n1p) || a->shared_inter > a->shared_ip))
+    return DSCA_ERR_BAD_ARG;
+  // 16-byte copies of weight rows and vector loads of token rows
+  const int wsz = fp8 ? 1 : (a->weights == DSCA_BF16 ? 2 : 4), xsz = a->weights == DSCA_F32 ? 4 : 2;
+  if (((size_t)a->d * wsz) % 16 != 0 || ((size_t)a->d * xsz) % 16 != 0) return DSCA_ERR_BAD_ARG;
+  if (a->T == 0) return DSCA_OK;
+  const void* need[] = {a->x, a->w_router, a->w1, a->w2, a->out, a->logits, a->topk_ids, a->topk_w, a->workspace};
+  for (const void* p : need)
+    if (p == nullptr) return DSCA_ERR_BAD_ARG;
+  const void* al[] = {a->x, a->w_router, a->w_shared_gate, a->w1, a->w2, a->ws1, a->ws2, a->out, a->workspace};
+  for (const void* p : al)
+    if (!aligned16(p)) return DSCA_ERR_BAD_ARG;
+  if (shared && (a->ws1 == nullptr || a->ws2 == nullptr)) return DSCA_ERR_BAD_ARG;
+  if (fp8 && (a->w1_scale == nullptr || a->w2_scale == nullptr ||
+              (shared && (a->ws1_scale == nullptr || a->ws2_scale == nullptr))))
+    return DSCA_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return DSCA_ERR_BAD_ARG;
+  if (a->workspace_bytes < dsca::few_workspace_bytes(a->T, k, a->inter, shared ? a->shared_inter : 0))
+    return DSCA_ERR_CAPACITY;
+  int num_sms = 0, major = 0;
+  int rc = device_info(&num_sms, &major);
+  if (rc) return rc;
+  if (major != 10) return DSCA_ERR_UNSUPPORTED;
+  return dsca::launch_moe_few(a, num_sms, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int dsca_check_error(int32_t* err_dev, dsca_stream_t stream) {

@@ -10,6 +10,10 @@ G GPUs:    (exchange="p2p", the default) router -> counts pushed to every peer a
            graph (MoEEngine.capture).  exchange="nccl": counts all-gather -> host plan -> NCCL
            grouped send/recv of the chunks, kept as the library-collective baseline.
 
+Few tokens (decode, at most 32): forward_few runs the whole block in one kernel (dsca_moe_few);
+           forward() takes it for calls of at most few_tokens tokens (0, the default: never).
+           forward_normed puts the residual's addition and the norm (add_rms_norm) in front.
+
 Reference hot path: QoSMoELayer.forward (src/qosmoe/moe_layer.py:271-459) and
 ShardedQwenMoE.forward (qwen_ep_adapter/qwen_ep.py:44-97).  Every expert's weights are
 resident on every GPU (B200 HBM holds a whole layer), so tokens that the harmony plan migrates
@@ -25,6 +29,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
+from .norm import add_rms_norm
 from .qos import ExpertCache, QoSInputs, build_exec_plan, match_token_length
 
 __all__ = ["PackedExperts", "pack_swiglu", "pack_relu", "MoEEngine", "ForwardGraph", "HostPipeline", "plan_harmony",
@@ -418,6 +423,12 @@ class MoEEngine:
         self.shared_handoff = True
         self._qos_done = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._ws = {}
+        # forward() runs calls of at most this many tokens through the one-kernel form where that
+        # supports the block (forward_few); 0 = never.  Results then differ from the other path's by
+        # its roundings (the intermediates and expert outputs are not rounded to bf16 here)
+        self.few_tokens = 0
+        self._few_ws = {}
+        self._few_args = None
         self.last_plan = None
         self.last_layout = None
         # when a list, forward() appends (name, cuda.Event) markers between its kernel launches
@@ -662,6 +673,8 @@ class MoEEngine:
             raise ValueError(f"expected [T, {self.d}] input, got {tuple(x.shape)}")
         x = x.to(dtype=self.dtype).contiguous()
         T = x.shape[0]
+        if 0 < T <= self.few_tokens and self.markers is None and self._few_unsupported(T) is None:
+            return self.forward_few(x)
         ws = dict(self._workspace(T))
         dev, k = self.device, self.top_k
         # results are fresh tensors (the caller keeps them); scratch above is reused
@@ -685,6 +698,93 @@ class MoEEngine:
             self._mark("combine")
             return ws
         return self._forward_ep(x, ws, qos)
+
+    # -------------------------------------------------------------- few tokens: one kernel
+    def _few_unsupported(self, T: int) -> str | None:
+        """Why forward_few cannot run T tokens through this block (None: it can)."""
+        if T > L.FEW_TOKENS:
+            return f"{T} tokens exceed {L.FEW_TOKENS}"
+        if self.world > 1 or self.ep_loopback:
+            return "it runs on one GPU"
+        if self.cache is not None:
+            return "the experts must be resident"
+        esz = 1 if self.experts.fp8 else (2 if self.dtype == torch.bfloat16 else 4)
+        if self.d * esz % 16:
+            return f"a weight row of {self.d} values is not a multiple of 16 bytes"
+        return None
+
+    def _few_workspace(self):
+        """Scratch of dsca_moe_few: one per stream, because calls that may overlap must not share it.
+        A call that is being captured gets one of its own from the graph's memory, with its
+        counters zeroed by the graph."""
+        n = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.top_k, self.experts.inter, self.experts.s_inter)
+        if torch.cuda.is_current_stream_capturing():
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+            ws[:L.FEW_COUNTER_BYTES].zero_()
+            return ws
+        key = torch.cuda.current_stream(self.device).cuda_stream
+        ws = self._few_ws.get(key)
+        if ws is None:
+            ws = self._few_ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return ws
+
+    def _few_struct(self):
+        """dsca_few_args with everything that does not change from call to call."""
+        if self._few_args is None:
+            pe, a = self.experts, L.FewArgs()
+            a.w_router, a.w_shared_gate = _ptr(self.router_weight), _ptr(self.shared_gate_weight)
+            a.d, a.E, a.top_k = self.d, self.E, self.top_k
+            a.weights = L.F8E4M3 if pe.fp8 else _dt(self.dtype)
+            a.mode, a.norm_topk, a.act = self.route_mode, int(self.norm_topk), pe.act
+            a.inter, a.n1p, a.ip, a.dp = pe.inter, pe.n1p, pe.ip, pe.dp
+            a.shared_inter, a.shared_n1p, a.shared_ip = pe.s_inter, pe.s_n1p, pe.s_ip
+            a.w1, a.w2, a.ws1, a.ws2 = _ptr(pe.w1), _ptr(pe.w2), _ptr(pe.ws1), _ptr(pe.ws2)
+            a.w1_scale, a.w2_scale = _ptr(pe.w1_scale), _ptr(pe.w2_scale)
+            a.ws1_scale, a.ws2_scale = _ptr(pe.ws1_scale), _ptr(pe.ws2_scale)
+            a.err = _ptr(self.err)
+            self._few_args = a
+        return L.FewArgs.from_buffer_copy(self._few_args)
+
+    def forward_few(self, x: torch.Tensor) -> dict:
+        """The whole block for at most 32 tokens in one kernel (dsca_moe_few): x [T, d] on this
+        engine's device -> fresh out [T, d], logits [T, E], topk_ids [T, k], topk_w [T, k] and
+        expert_index [T], with forward()'s meaning.  One GPU, resident experts, any of the engine's
+        weight types; ValueError otherwise.  Runs on the current stream; can be captured."""
+        if x.dim() != 2 or x.shape[1] != self.d:
+            raise ValueError(f"expected [T, {self.d}] input, got {tuple(x.shape)}")
+        if x.device != self.router_weight.device:
+            raise ValueError(f"x is on {x.device}, the engine on {self.router_weight.device}")
+        T, k, dev = x.shape[0], self.top_k, self.router_weight.device
+        why = self._few_unsupported(T)
+        if why is not None:
+            raise ValueError(f"forward_few: {why}")
+        x = x.to(dtype=self.dtype).contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+        r = dict(out=torch.empty(T, self.d, dtype=self.dtype, device=dev),
+                 logits=torch.empty(T, self.E, dtype=self.dtype, device=dev),
+                 topk_ids=torch.empty(T, k, dtype=torch.int32, device=dev),
+                 topk_w=torch.empty(T, k, dtype=torch.float32, device=dev),
+                 expert_index=torch.empty(T, dtype=torch.int64, device=dev))
+        if T == 0:
+            return r
+        with torch.cuda.device(dev):
+            ws = self._few_workspace()
+            a = self._few_struct()
+            a.T, a.x, a.out, a.logits = T, x.data_ptr(), r["out"].data_ptr(), r["logits"].data_ptr()
+            a.topk_ids, a.topk_w = r["topk_ids"].data_ptr(), r["topk_w"].data_ptr()
+            a.expert_index, a.workspace, a.workspace_bytes = r["expert_index"].data_ptr(), ws.data_ptr(), ws.numel()
+            L.call("dsca_moe_few", ctypes.byref(a), _stream())
+        return r
+
+    def forward_normed(self, x: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6,
+                       residual: torch.Tensor | None = None, qos: QoSInputs | None = None) -> dict:
+        """add_rms_norm and the block behind it: the result of forward(y) plus residual = x + residual
+        (what the caller adds `out` to, or hands to the next add_rms_norm) and normed = y."""
+        n = add_rms_norm(x, norm_weight, eps, residual)
+        r = self.forward(n.y, qos)
+        r["residual"], r["normed"] = n.residual, n.y
+        return r
 
     # -------------------------------------------------------------- expert cache path
     def _qos(self, x, ws, qos: QoSInputs | None):
@@ -1102,7 +1202,10 @@ class MoEEngine:
 
     def check(self):
         """Synchronise and raise if a kernel recorded an error."""
-        L.check(L.load().dsca_check_error(_ptr(self.err), _stream()), "device error word")
+        rc = L.load().dsca_check_error(_ptr(self.err), _stream())
+        if rc != L.OK:
+            self._few_ws = {}  # a call that gave up leaves its counters as they were
+        L.check(rc, "device error word")
 
     # -------------------------------------------------------------- CUDA graphs
     def capture(self, x: torch.Tensor) -> "ForwardGraph":

@@ -127,6 +127,7 @@ class QoSMoELayer(nn.Module):
                                 shared_gate_weight=sg_w, rank=config.rank, world=config.world_size,
                                 group=getattr(config, "process_group", None), expert_to_gpu=e2g,
                                 eq_tokens=config.eq_tokens, cache_slots=cache_slots, device=dev)
+        self.engine.few_tokens = int(getattr(config, "few_tokens", 0) or 0)
         for k in ("alpha", "beta", "delta", "target_batch", "epsilon"):
             self.engine.qos_params[k] = float(getattr(config, "qos_" + k, self.engine.qos_params[k]))
         self.engine.qos_params["attention_mode"] = 0 if getattr(config, "qos_attention_mode", "router_var") == "router_var" else 1
@@ -214,7 +215,10 @@ class QoSMoELayer(nn.Module):
             ev1.record()
             ev1.synchronize()
             self.latencies.append(ev0.elapsed_time(ev1))
-            self.expert_freqs.append(r["counts"].tolist())
+            counts = r.get("counts")
+            if counts is None:  # the one-kernel form keeps no histogram
+                counts = torch.bincount(r["topk_ids"].reshape(-1), minlength=self.num_experts)
+            self.expert_freqs.append(counts.tolist())
             self.expert_swaps.append(self.engine.last_loads)
             lay = self.engine.last_layout
             T = r["out"].shape[0] * self.engine.top_k
@@ -232,10 +236,11 @@ class ShardedQwenMoE(nn.Module):
     Placement: contiguous blocks (E % world need not be 0) or `expert_to_gpu`; `eq_tokens` >= 0
     turns on harmony rebalancing (the reference block uses fixed ownership: eq_tokens = -1).
     forward returns `(h, router_logits)` (the reference contract) or, with
-    `return_logits=False`, `h` alone for transformers-5.x decoder layers."""
+    `return_logits=False`, `h` alone for transformers-5.x decoder layers.  `few_tokens`: calls of at
+    most this many tokens run as one kernel (MoEEngine.few_tokens)."""
 
     def __init__(self, old, rank, world, policy="fifo", group=None, expert_to_gpu=None, eq_tokens=-1,
-                 return_logits=True):
+                 return_logits=True, few_tokens=0):
         super().__init__()
         self.rank, self.world, self.policy = rank, world, policy
         # transformers 4.x keeps num_experts / top_k / norm_topk_prob on the block, 5.x on its router
@@ -255,6 +260,7 @@ class ShardedQwenMoE(nn.Module):
                                 route_mode=L.ROUTE_SOFTMAX_TOPK, norm_topk=self.norm_topk_prob,
                                 shared_gate_weight=old.shared_expert_gate.weight.detach(), rank=rank,
                                 world=world, group=group, expert_to_gpu=expert_to_gpu, eq_tokens=eq_tokens)
+        self.engine.few_tokens = int(few_tokens)
         self.route_calls = 0
 
     @torch.no_grad()
@@ -267,14 +273,15 @@ class ShardedQwenMoE(nn.Module):
         return r["out"].view(b, s, d), r["logits"]
 
 
-def patch(model, rank, world, policy="fifo"):
+def patch(model, rank, world, policy="fifo", few_tokens=0):
     """qwen_ep_adapter/qwen_ep.py:100-109: swap every Qwen2MoeSparseMoeBlock of model.model.layers.
     The swapped blocks return what the installed transformers' Qwen2MoeDecoderLayer expects."""
     changed = 0
     tuple_out = hf_callers_unpack_tuples()
     for layer in model.model.layers:
         if layer.mlp.__class__.__name__ == "Qwen2MoeSparseMoeBlock":
-            layer.mlp = ShardedQwenMoE(layer.mlp, rank, world, policy, return_logits=tuple_out)
+            layer.mlp = ShardedQwenMoE(layer.mlp, rank, world, policy, return_logits=tuple_out,
+                                       few_tokens=few_tokens)
             changed += 1
     if not changed:
         raise RuntimeError("No Qwen2MoeSparseMoeBlock found: wrong checkpoint/model version")

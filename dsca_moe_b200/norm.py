@@ -1,0 +1,108 @@
+"""Root-mean-square norm in front of an MoE block (dsca_rms_norm, include/dsca_b200_block.h).
+
+add_rms_norm(x, weight, eps, residual, quant) adds the block's input to the residual stream,
+normalises the sum and, on request, writes the normed rows in 8 bits as well: what a decoder layer
+runs between its attention and its MoE block (Qwen2MoeDecoderLayer.post_attention_layernorm,
+SwitchTransformersLayerFF.layer_norm).  MoEEngine.forward_normed runs it with the block behind it.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+
+__all__ = ["RmsNormOutput", "add_rms_norm"]
+
+_QUANT = {None: L.NORM_Q_NONE, "e4m3": L.NORM_Q_E4M3, "split": L.NORM_Q_SPLIT}
+_DTYPES = {torch.bfloat16: L.BF16, torch.float32: L.F32}
+
+
+class RmsNormOutput(NamedTuple):
+    """y: the normed rows, shaped like x (None when not asked for); residual: the residual stream h
+    (x itself without a residual); q, scale: the 8-bit rows [rows, ...] e4m3 and their fp32 scales
+    [rows] (None without quant)."""
+    y: torch.Tensor | None
+    residual: torch.Tensor
+    q: torch.Tensor | None
+    scale: torch.Tensor | None
+
+
+def _rows(t: torch.Tensor, name: str):
+    """(t as rows, their stride in elements): the leading dimensions must lie one stride apart."""
+    d = t.shape[-1]
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    elif t.dim() > 2:
+        try:
+            t = t.view(-1, d)
+        except RuntimeError:
+            raise ValueError(f"{name}: the rows of {tuple(t.shape)} with strides {t.stride()} are not evenly "
+                             "spaced (call contiguous())") from None
+    if d > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    ld = t.stride(0) if t.shape[0] > 1 else max(d, t.stride(0))
+    if ld < d:
+        raise ValueError(f"{name}: rows overlap (stride {ld}, width {d})")
+    return t, ld
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                 quant: str | None = None, write_y: bool = True) -> RmsNormOutput:
+    """h = x + residual (rounded to x's type), y = weight * h / sqrt(mean(h^2) + eps) over the last
+    dimension, summed in fp32 and rounded once.
+
+    x [..., d] bf16 or fp32 (rows may lie in a wider buffer), residual the same shape and type,
+    weight [d] of x's type or fp32.  quant "e4m3": q [rows, d] with scale = max|y| / 448 a row, from
+    the unrounded y (the row format of the fp8 expert weights); "split" (bf16, d % 8 == 0): q
+    [rows, 2 * ceil(d / 128) * 128], the two-term rows of dsca_split_rows with scale = 1 / s, the token
+    operand of the fp8-weight experts.  write_y=False leaves y out when only the 8-bit rows are
+    wanted.  Runs on x's device, on its current stream."""
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if quant not in _QUANT:
+        raise ValueError(f"quant must be None, 'e4m3' or 'split', not {quant!r}")
+    if not x.is_cuda:
+        raise ValueError("x must be on a GPU")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"expected [..., d] rows, got {tuple(x.shape)}")
+    d = x.shape[-1]
+    if tuple(weight.shape) != (d,) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device \
+            or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous [{d}] tensor of x's type or float32 on x's device")
+    if quant == "split" and (dt != L.BF16 or d % 8):
+        raise ValueError("quant='split' takes bf16 rows with d % 8 == 0")
+    if not write_y and quant is None:
+        raise ValueError("write_y=False needs a quant")
+    if d > L.NORM_MAX_D:
+        raise ValueError(f"rows of {d} values exceed {L.NORM_MAX_D}")
+    a = L.RmsNormArgs()
+    xr, a.ld_x = _rows(x, "x")
+    rows = xr.shape[0]
+    a.x, a.weight, a.rows, a.d, a.dtype, a.eps = x.data_ptr(), weight.data_ptr(), rows, d, dt, eps
+    a.weight_dtype = _DTYPES[weight.dtype]
+    h = x
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("residual must have x's shape, type and device")
+        _, a.ld_residual = _rows(residual, "residual")
+        a.residual = residual.data_ptr()
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a.residual_out, a.ld_residual_out = h.data_ptr(), d
+    y = q = scale = None
+    if write_y:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a.y, a.ld_y = y.data_ptr(), d
+    if quant is not None:
+        a.quant = _QUANT[quant]
+        width = d if quant == "e4m3" else 2 * ((d + 127) // 128 * 128)
+        q = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        a.q, a.scale = q.data_ptr(), scale.data_ptr()
+    if rows:
+        with torch.cuda.device(x.device):
+            L.call("dsca_rms_norm", ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    return RmsNormOutput(y, h, q, scale)
