@@ -6,9 +6,12 @@
 // Such a call's time is the reading of the chosen experts' weights (17 MB an expert of the Qwen block
 // in bf16, 69 MB for its shared expert, against 4 KB a token), so everything here serves one
 // uninterrupted stream of weight bytes:
-//  - one persistent CTA per SM; each of its 8 warps keeps its own ring of asynchronous bulk copies
-//    (16 weight rows x up to 512 bytes a stage) and multiplies what has arrived, so no warp waits
-//    for another one's data and a stage is refilled as soon as it is read;
+//  - one persistent CTA per SM.  A producer warp copies pieces of 16 weight rows x up to 2 KB into a
+//    ring of shared-memory stages (asynchronous bulk copies, 16 a piece); eight compute warps split
+//    each piece along k, keep their sums in registers and hand them over at the end of a unit (16
+//    rows of a matrix); three service warps add the eight parts, apply the activation and store, and
+//    run the router at the start.  No role waits for another one's latency: the stream stalls only
+//    when the whole ring is full;
 //  - the weights are cut 16 rows at a time (8 gate + 8 up rows, or 16 rows of any other matrix), fine
 //    enough that 148 SMs get nearly equal shares, where a 128-row tensor-memory tile would leave
 //    two fifths of them idle at one token.  16 rows x 8 tokens is the shape of mma.sync, which
@@ -33,10 +36,13 @@
 namespace dsca {
 namespace few {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kMaxStages = 8;
-constexpr int kPiece = 512;               // bytes of one weight row in a stage, at most
+constexpr int kWarps = 8;                 // compute warps (0 .. 7)
+constexpr int kProducer = kWarps;         // the warp that issues the copies
+constexpr int kService = kProducer + 1;   // first of the service warps
+constexpr int kServices = 3;
+constexpr int kThreads = (kService + kServices) * 32;
+constexpr int kMaxStages = 16;
+constexpr int kPiece = 2048;              // bytes of one weight row in a stage, at most
 constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
 constexpr int kLgPitch = 64;              // logits scratch: E + 1 <= 64 per token
 
@@ -64,9 +70,9 @@ struct Args {
   int hp, hsp;            // row pitch of h / hs in values
   int upe, ups;           // units (16 weight rows of GEMM1) per routed expert / of the shared expert
   int k2, k2s;            // values of a row of w2 / ws2 that are read
-  int kc1;                // values of a GEMM1 row that one warp reads
+  int p1, p2, p2s;        // values of a row that one piece of GEMM1 / routed / shared GEMM2 holds
   int rt, tiles;          // rows of a GEMM2 tile, tiles
-  int pitch, stages;      // bytes of a stage row, stages of a warp's ring
+  int pitch, stages;      // bytes of a stage row, stages of the ring
 };
 
 struct Bf16 {
@@ -130,16 +136,24 @@ __device__ __forceinline__ bool ctr_wait(const uint32_t* p, uint32_t target, vol
     }
   }
 }
-__device__ __forceinline__ void ctr_add(uint32_t* p) {
+__device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n) {
   __threadfence();
-  atomicAdd(p, 1u);
+  atomicAdd(p, n);
 }
 
 // ---------------------------------------------------------------- shared memory
+// Units whose parts may wait for a service warp: as many as leave the ring five or six full stages.
+// At least kServices, so that a service warp that has seen one unit's parts knows every earlier use of
+// the buffer it waits for next to be complete (a parity wait cannot look two phases ahead).
+constexpr int parts_of(int nt) { return nt == 1 ? 4 : 3; }
+static_assert(parts_of(1) >= kServices && parts_of(4) >= kServices, "parity waits");
 template <int NT>
 struct Smem {
-  float part[2][kWarps][NT][32][4];         // partial sums of a unit or tile, double buffered
-  uint64_t bar[kWarps][kMaxStages];
+  static constexpr int kParts = parts_of(NT);
+  float part[kParts][kWarps][NT][32][4];    // the compute warps' sums of a unit
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t part_full[kParts], part_empty[kParts];
+  uint64_t routed;
   float wt[8 * NT][DSCA_MAX_TOPK];          // routing weights
   float sg[8 * NT];                         // shared-expert gate
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
@@ -274,19 +288,18 @@ __device__ __forceinline__ uint4 ld_b(const uint8_t* p, bool live, bool coherent
   return coherent ? __ldcg(q) : *q;
 }
 
-// acc += 16 weight rows x (up to 8 NT tokens) over one stage of bf16 or e4m3 weights.
-//   stage: shared address of the stage, len: bytes of its rows, k0: first k, klim: first k without a
-//   token value, ntu: token tiles in use (bit nt of ntm).  wait(): until the stage has arrived.
+// acc += 16 weight rows x (up to 8 NT tokens) over the 64-byte blocks [kb0, kb1) of a piece of bf16 or
+// e4m3 weights.
+//   stage: shared address of the stage, len: bytes of its rows, k0: k of its first value, klim: first k
+//   without a token value, ntm: token tiles in use.  wait(): until the stage has arrived.
 template <typename W, int NT, int kTerms, typename Wait>
-__device__ __forceinline__ void stage_mma(float (&acc)[NT][4], uint32_t stage, int pitch, int len, int k0, int klim,
-                                          const Rows<NT>& b, size_t lo, uint32_t ntm, int lane, Wait wait) {
-  constexpr int kPer = W::kBlock / 32;                  // 16-byte token vectors per lane and 64-byte block
-  constexpr int kGroupRaw = 8 / (NT * kTerms * kPer);   // 64-byte blocks whose token values are loaded together
-  constexpr int kGroup = kGroupRaw < 1 ? 1 : kGroupRaw;
+__device__ __forceinline__ void piece_mma(float (&acc)[NT][4], uint32_t stage, int pitch, int len, int kb0, int kb1, int k0,
+                                          int klim, const Rows<NT>& b, size_t lo, uint32_t ntm, int lane, Wait wait) {
+  constexpr int kPer = W::kBlock / 32;             // 16-byte token vectors per lane and 64-byte block
+  constexpr int kGroup = NT == 1 ? 4 : (NT == 2 ? 2 : 1);  // blocks whose token values are loaded together
   const int g = lane >> 2, t = lane & 3;
-  const int nkb = (len + 63) >> 6;
   bool waited = false;
-  for (int kb0 = 0; kb0 < nkb; kb0 += kGroup) {
+  for (int kg = kb0; kg < kb1; kg += kGroup) {
     uint4 bv[kGroup][NT][kTerms][kPer];
 #pragma unroll
     for (int i = 0; i < kGroup; ++i)
@@ -295,8 +308,8 @@ __device__ __forceinline__ void stage_mma(float (&acc)[NT][4], uint32_t stage, i
         if (!((ntm >> nt) & 1u)) continue;
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
-          const int k = k0 + (kb0 + i) * W::kBlock + t * 8 * kPer + q * 8;
-          const bool live = kb0 + i < nkb && k < klim && b.p[nt] != nullptr;
+          const int k = k0 + (kg + i) * W::kBlock + t * 8 * kPer + q * 8;
+          const bool live = kg + i < kb1 && k < klim && b.p[nt] != nullptr;
 #pragma unroll
           for (int m = 0; m < kTerms; ++m)
             bv[i][nt][m][q] = ld_b(b.p[nt] + (size_t)k * 2 + (m ? lo : 0), live, kTerms == 2);
@@ -308,9 +321,8 @@ __device__ __forceinline__ void stage_mma(float (&acc)[NT][4], uint32_t stage, i
     }
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
-      const int kb = kb0 + i;
-      if (kb >= nkb) break;
-      const int off = kb * 64 + t * 16;
+      if (kg + i >= kb1) break;
+      const int off = (kg + i) * 64 + t * 16;
       uint4 a0 = make_uint4(0u, 0u, 0u, 0u), a1 = a0;
       if (off < len) {  // behind the row's end the stage holds other rows' bytes
         a0 = lds128(stage + g * pitch + off);
@@ -354,10 +366,9 @@ __device__ __forceinline__ void stage_mma(float (&acc)[NT][4], uint32_t stage, i
 // eight tokens of a tile; f32_fold() adds the four lanes of a row and leaves the layout of the
 // tensor-core accumulators.  row(nt, n): token row (or null), the same on all lanes.
 template <int NT, bool kCoherent, typename Row, typename Wait>
-__device__ __forceinline__ void stage_fma(float (&acc)[NT][16], uint32_t stage, int pitch, int len, int k0, int klim, Row row,
-                                          uint32_t ntm, int lane, Wait wait) {
+__device__ __forceinline__ void piece_fma(float (&acc)[NT][16], uint32_t stage, int pitch, int len, int kb0, int kb1, int k0,
+                                          int klim, Row row, uint32_t ntm, int lane, Wait wait) {
   const int g = lane >> 2, t = lane & 3;
-  const int nkb = (len + 63) >> 6;
   wait();
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -366,7 +377,7 @@ __device__ __forceinline__ void stage_fma(float (&acc)[NT][16], uint32_t stage, 
 #pragma unroll
     for (int n = 0; n < 8; ++n) rp[n] = row(nt, n);
 #pragma unroll 2
-    for (int kb = 0; kb < nkb; ++kb) {
+    for (int kb = kb0; kb < kb1; ++kb) {
       const int off = kb * 64 + t * 16;
       const int k = k0 + kb * 16 + t * 4;
       if (off >= len || k >= klim) continue;
@@ -401,102 +412,29 @@ __device__ __forceinline__ void f32_fold(const float (&a)[NT][16], float (&acc)[
 }
 
 // ---------------------------------------------------------------- the kernel
-template <typename W, int NT>
-__global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
-  using X = typename W::X;
-  constexpr bool kF32 = W::kSize == 4;
-  constexpr int kKC = kPiece / W::kSize;  // values of a full stage row
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  Smem<NT>& s = *reinterpret_cast<Smem<NT>*>(smem_raw);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+__device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+
+// Router: fp64 dot products spread over the grid, then softmax, selection and the expert lists in every
+// CTA for itself.  Warp wi of the nw warps that take part (they share named barrier 1).
+template <typename X, int NT>
+__device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
-  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)((sizeof(Smem<NT>) + 127) / 128 * 128) +
-                        (uint32_t)(warp * a.stages * 16 * a.pitch);
-  const uint32_t bars = smem_u32(&s.bar[warp][0]);
-  volatile int* abort_flag = &s.abort;
-
-  if (lane < a.stages) mbar_init(bars + 8 * lane, 1);
-  fence_mbar_init();
-  for (int i = threadIdx.x; i < DSCA_MAX_EXPERTS; i += kThreads) s.emask[i] = 0u;
-  if (threadIdx.x == 0) {
-    s.abort = 0;
-    s.n_act = 0;
+  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), nd = a.T * R;
+  for (int q = cta + wi * G; q < nd; q += nw * G) {
+    const int t = q / R, r = q % R;
+    const X* w = r < a.E ? reinterpret_cast<const X*>(a.w_router) + (size_t)r * a.d : reinterpret_cast<const X*>(a.w_gate);
+    const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, lane);
+    if (lane == 0) a.lg[t * kLgPitch + r] = round_to<X>(v);
   }
-  __syncthreads();
-
-  // ---- this warp's list of stages.  GEMM1: units cta, cta + G, ... of the shared expert, then of
-  // the routed experts (the first of them on the CTA behind the last shared unit's); of every unit
-  // the warp has its own range of k.  GEMM2: tiles cta, cta + G, ...; the pieces of the shared row,
-  // then of the active experts' rows, go round the warps.
-  const int k1a = min(a.d, warp * a.kc1), k1b = min(a.d, k1a + a.kc1);
-  const int ppu = (k1b - k1a + kKC - 1) / kKC;  // stages a unit (0: this warp has no share of d)
-  const int nu_s = a.ups > cta ? (a.ups - cta + G - 1) / G : 0;
-  const int r_first = (cta + G - a.ups % G) % G;
-  const int n2s = (a.k2s + kKC - 1) / kKC, n2r = (a.k2 + kKC - 1) / kKC;
-  int nu_r = 0, n2w = 0, n1 = nu_s * ppu, total = n1;  // until the routing is known
-
-  auto issue = [&](int i) {
-    const int st = i % a.stages;
-    const uint32_t bar = bars + 8 * st, dst = ring + (uint32_t)(st * 16 + (lane & 15)) * a.pitch;
-    const uint8_t* src;
-    int rows = 16, len;
-    if (i < n1) {
-      const int ul = i / ppu, kb = k1a + (i % ppu) * kKC;
-      const bool sh = ul < nu_s;
-      const int r = sh ? cta + ul * G : r_first + (ul - nu_s) * G;
-      const int u = sh ? r : r % a.upe, e = sh ? 0 : s.act[r / a.upe];
-      const int l = lane & 15;
-      const int ch = 8 * u + (l & 7);
-      const int row = a.glu ? (ch >> 7) * 256 + (ch & 127) + (l >> 3) * 128 : 16 * u + l;
-      len = min(kKC, k1b - kb) * W::kSize;
-      src = (sh ? a.ws1 : a.w1) + (((size_t)e * a.n1p + row) * a.d + kb) * W::kSize;
-    } else {
-      const int j = i - n1, tile = cta + (j / n2w) * G, q = warp + kWarps * (j % n2w);
-      const int r0 = tile * a.rt;
-      rows = min(a.rt, a.d - r0);
-      const bool sh = q < n2s;
-      const int e = sh ? 0 : s.act[(q - n2s) / n2r], kb = (sh ? q : (q - n2s) % n2r) * kKC;
-      const int row = r0 + min(lane & 15, rows - 1);
-      len = (min(kKC, (sh ? a.k2s : a.k2) - kb) * W::kSize + 15) & ~15;
-      src = sh ? a.ws2 + ((size_t)row * a.s_ip + kb) * W::kSize
-               : a.w2 + (((size_t)e * a.dp + row) * a.ip + kb) * W::kSize;
-    }
-    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(rows * len));
-    __syncwarp();
-    if (lane < rows) bulk_load(dst, src, (uint32_t)len, bar);
-  };
-  int issued = 0, done = 0;
-  // every lane has read stage `done`: refill it with the stage that follows the last one issued
-  // (none after an abort, so that the copies in flight can be waited for at the end)
-  auto release = [&]() {
-    const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
-    ++done;
-    if (issued < total && !stop) issue(issued++);
-  };
-  auto wait_stage = [&]() {
-    mbar_wait(bars + 8 * (done % a.stages), (uint32_t)(done / a.stages) & 1u, abort_flag, a.err);
-  };
-  while (issued < min(a.stages, total)) issue(issued++);
-
-  // ---- router: one warp a dot product, spread over the grid
-  {
-    const int R = a.E + (a.w_gate != nullptr ? 1 : 0), nd = a.T * R;
-    for (int q = cta + warp * G; q < nd; q += kWarps * G) {
-      const int t = q / R, r = q % R;
-      const X* w = r < a.E ? reinterpret_cast<const X*>(a.w_router) + (size_t)r * a.d : reinterpret_cast<const X*>(a.w_gate);
-      const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, lane);
-      if (lane == 0) a.lg[t * kLgPitch + r] = round_to<X>(v);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      if (cta < nd) ctr_add(a.ctr + kCtrLogits);
-      ctr_wait(a.ctr + kCtrLogits, (uint32_t)min(nd, G), abort_flag, a.err);
-    }
-    __syncthreads();
+  group_sync(nw * 32);
+  if (wi == 0 && lane == 0) {
+    if (cta < nd) ctr_add(a.ctr + kCtrLogits, 1u);
+    ctr_wait(a.ctr + kCtrLogits, (uint32_t)min(nd, G), &s.abort, a.err);
   }
-  for (int t = warp; t < a.T; t += kWarps) select_token<X, NT>(a, s, t, lane);
-  __syncthreads();
-  if (warp == 0) {
+  group_sync(nw * 32);
+  for (int t = wi; t < a.T; t += nw) select_token<X, NT>(a, s, t, lane);
+  group_sync(nw * 32);
+  if (wi == 0) {
     const uint32_t m0 = s.emask[lane], m1 = s.emask[lane + 32];
     const uint32_t b0 = __ballot_sync(0xffffffffu, m0 != 0u), b1 = __ballot_sync(0xffffffffu, m1 != 0u);
     const uint32_t below = (1u << lane) - 1u;
@@ -504,226 +442,370 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
     if (m1) s.act[__popc(b0) + __popc(b1 & below)] = (uint8_t)(lane + 32);
     if (lane == 0) s.n_act = __popc(b0) + __popc(b1);
   }
-  for (int i = threadIdx.x; i < DSCA_MAX_EXPERTS * 8 * NT; i += kThreads) {
+  for (int i = wi * 32 + lane; i < DSCA_MAX_EXPERTS * 8 * NT; i += nw * 32) {
     const int e = i / (8 * NT), t = i % (8 * NT);
     const uint32_t m = s.emask[e];
     if ((m >> t) & 1u) s.tok[e][__popc(m & ((1u << t) - 1u))] = (uint8_t)t;
   }
+  group_sync(nw * 32);
+  if (wi == 0 && lane == 0) mbar_arrive(smem_u32(&s.routed));
+}
+
+template <typename W, int NT>
+__global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
+  using X = typename W::X;
+  constexpr bool kF32 = W::kSize == 4;
+  constexpr int kParts = Smem<NT>::kParts;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  Smem<NT>& s = *reinterpret_cast<Smem<NT>*>(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int G = gridDim.x, cta = blockIdx.x;
+  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)((sizeof(Smem<NT>) + 127) / 128 * 128);
+  const uint32_t stage_bytes = 16u * (uint32_t)a.pitch;
+  volatile int* abort_flag = &s.abort;
+
+  if (threadIdx.x < (unsigned)a.stages) {
+    mbar_init(smem_u32(&s.full[threadIdx.x]), 1);
+    mbar_init(smem_u32(&s.empty[threadIdx.x]), kWarps);
+  }
+  if (threadIdx.x < kParts) {
+    mbar_init(smem_u32(&s.part_full[threadIdx.x]), kWarps);
+    mbar_init(smem_u32(&s.part_empty[threadIdx.x]), 1);
+  }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + DSCA_MAX_EXPERTS) s.emask[threadIdx.x - 64] = 0u;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&s.routed), 1);
+    s.abort = 0;
+    s.n_act = 0;
+  }
+  fence_mbar_init();
   __syncthreads();
-  const int n_act = s.n_act;
-  {
+
+  // ---- this CTA's work.  GEMM1: units cta, cta + G, ... of the shared expert, then of the routed
+  // experts (the first of them on the CTA behind the last shared unit's).  GEMM2: tiles cta, cta + G,
+  // ... of the output's rows; the pieces of the shared expert's row, then of the active experts'.
+  const int nu_s = a.ups > cta ? (a.ups - cta + G - 1) / G : 0;
+  const int r_first = (cta + G - a.ups % G) % G;
+  auto routed_units = [&](int n_act) {
     const int units = n_act * a.upe;
-    nu_r = units > r_first ? (units - r_first + G - 1) / G : 0;
-    const int n2 = n2s + n_act * n2r;
-    n2w = n2 > warp ? (n2 - warp + kWarps - 1) / kWarps : 0;
-    const int tl = a.tiles > cta ? (a.tiles - cta + G - 1) / G : 0;
-    n1 = (nu_s + nu_r) * ppu;
-    total = n1 + tl * n2w;
-  }
-  while (issued < min(a.stages, total)) issue(issued++);
+    return units > r_first ? (units - r_first + G - 1) / G : 0;
+  };
+  auto wait_routed = [&]() { mbar_wait(smem_u32(&s.routed), 0u, abort_flag, a.err); };
+  // The router runs on the service warps while the compute warps begin with the shared expert; on all
+  // of them where there is no shared expert to begin with, or where the tokens are more than three
+  // warps would do in the time of the first stages.
+  const bool all_route = a.ups == 0 || a.T > 4;
+  const int route_warps = all_route ? kWarps + kServices : kServices;
 
-  // ---- GEMM1
-  const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
-  const int nw1 = (a.d + a.kc1 - 1) / a.kc1;  // warps with a share of d
-  for (int ul = 0; ul < nu_s + nu_r; ++ul) {
-    const bool sh = ul < nu_s;
-    const int r = sh ? cta + ul * G : r_first + (ul - nu_s) * G;
-    const int u = sh ? r : r % a.upe, e = sh ? 0 : s.act[r / a.upe];
-    const int n_tok = sh ? a.T : __popc(s.emask[e]);
-    const uint32_t ntm = (1u << ((n_tok + 7) / 8)) - 1u;
-    float acc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
-    auto token = [&](int n) { return sh ? n : (int)s.tok[e][n]; };
-    if constexpr (kF32) {
-      float big[NT][16];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) big[nt][i] = 0.0f;
-      auto row = [&](int nt, int n) {
-        return 8 * nt + n < n_tok ? reinterpret_cast<const float*>(a.x) + (size_t)token(8 * nt + n) * a.d : nullptr;
-      };
-      for (int p = 0; p < ppu; ++p) {
-        const int kb = k1a + p * kKC, len = min(kKC, k1b - kb) * W::kSize;
-        stage_fma<NT, false>(big, ring + (uint32_t)((done % a.stages) * 16) * a.pitch, a.pitch, len, kb, a.d, row, ntm, lane,
-                             wait_stage);
-        release();
-      }
-      f32_fold<NT>(big, acc, lane);
-    } else {
-      Rows<NT> b;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        b.p[nt] = 8 * nt + g < n_tok ? reinterpret_cast<const uint8_t*>(a.x) + (size_t)token(8 * nt + g) * a.d * 2 : nullptr;
-      for (int p = 0; p < ppu; ++p) {
-        const int kb = k1a + p * kKC, len = min(kKC, k1b - kb) * W::kSize;
-        stage_mma<W, NT, 1>(acc, ring + (uint32_t)((done % a.stages) * 16) * a.pitch, a.pitch, len, kb, a.d, b, 0, ntm, lane,
-                            wait_stage);
-        release();
-      }
-    }
-    float(*part)[NT][32][4] = s.part[ul & 1];
-    if (ppu > 0) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        if ((ntm >> nt) & 1u) *reinterpret_cast<float4*>(part[warp][nt][lane]) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-    }
-    // double buffered: this buffer is written again two units on, behind the next unit's barrier,
-    // which the finishing warp reaches only after it has read it
-    __syncthreads();
-    if (warp == (ul & (kWarps - 1))) {
-      for (int nt = 0; nt * 8 < n_tok; ++nt) {
-        float4 v = *reinterpret_cast<const float4*>(part[0][nt][lane]);
-        for (int w = 1; w < nw1; ++w) {
-          const float4 o = *reinterpret_cast<const float4*>(part[w][nt][lane]);
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        float c[4] = {v.x, v.y, v.z, v.w};
-        if constexpr (W::kSize == 1) {
-          const int ch = 8 * u + g;
-          const int r0 = a.glu ? (ch >> 7) * 256 + (ch & 127) : 16 * u + g, r1 = a.glu ? r0 + 128 : r0 + 8;
-          const float* sc = sh ? a.ws1s : a.w1s + (size_t)e * a.n1p;
-          const float s0 = sc[r0], s1 = sc[r1];
-          c[0] *= s0; c[1] *= s0; c[2] *= s1; c[3] *= s1;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = nt * 8 + 2 * t4 + i;
-          if (n >= n_tok) continue;
-          const int tk = token(n), j = sh ? 0 : s.slot[e][tk];
-          const float w = sh ? s.sg[tk] : s.wt[tk][j];
-          const size_t at = sh ? (size_t)tk * a.hsp : ((size_t)tk * a.k + j) * a.hp;
-          uint8_t* base = sh ? a.hs : a.h;
-          auto put = [&](int ch, float val) {
-            if constexpr (kF32) {
-              reinterpret_cast<float*>(base)[at + ch] = val;
-            } else {
-              const __nv_bfloat16 hi = __float2bfloat16_rn(val);
-              const float rest = val - __bfloat162float(hi);
-              __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at + ch;
-              o[0] = hi;
-              // an infinite or NaN value is the high term alone
-              o[(sh ? hs_lo : h_lo) / 2] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
-            }
-          };
-          if (a.glu) {
-            put(8 * u + g, w * (c[i] / (1.0f + expf(-c[i])) * c[2 + i]));
-          } else {
-            put(16 * u + g, w * fmaxf(c[i], 0.0f));
-            put(16 * u + g + 8, w * fmaxf(c[2 + i], 0.0f));
-          }
-        }
-      }
+  if (warp == kProducer) {
+    // ================================================================ producer
+    int it = 0;
+    auto piece = [&](const uint8_t* src, int rows, int len) {
+      const int st = it % a.stages;
+      if (it >= a.stages) mbar_wait(smem_u32(&s.empty[st]), (uint32_t)(it / a.stages - 1) & 1u, abort_flag, a.err);
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) return;
+      const uint32_t bar = smem_u32(&s.full[st]);
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(rows * len));
       __syncwarp();
-      if (lane == 0) ctr_add(a.ctr + (sh ? kCtrShared : kCtrRouted));
+      if (lane < rows) bulk_load(ring + (uint32_t)st * stage_bytes + (uint32_t)(lane * a.pitch), src, (uint32_t)len, bar);
+      ++it;
+    };
+    const int l = lane & 15;
+    int nu_r = 0;
+    for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
+      const bool sh = ul < nu_s;
+      if (ul == nu_s) {
+        wait_routed();
+        nu_r = routed_units(s.n_act);
+        if (nu_r == 0) break;
+      }
+      const int r = sh ? cta + ul * G : r_first + (ul - nu_s) * G;
+      const int u = sh ? r : r % a.upe, e = sh ? 0 : s.act[r / a.upe];
+      const int ch = 8 * u + (l & 7);
+      const int row = a.glu ? (ch >> 7) * 256 + (ch & 127) + (l >> 3) * 128 : 16 * u + l;
+      const uint8_t* src = (sh ? a.ws1 : a.w1) + ((size_t)e * a.n1p + row) * a.d * W::kSize;
+      for (int k = 0; k < a.d; k += a.p1) piece(src + (size_t)k * W::kSize, 16, min(a.p1, a.d - k) * W::kSize);
     }
-  }
-
-  // ---- GEMM2
-  bool have_s = n2s == 0, have_r = false;
-  for (int tile = cta, tn = 0; tile < a.tiles; tile += G, ++tn) {
-    const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
-    float acc[NT][4];
-    float big[kF32 ? NT : 1][16];
+    const int n_act = s.n_act;
+    for (int tile = cta; tile < a.tiles; tile += G) {
+      const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0), row = r0 + min(l, rows - 1);
+      for (int k = 0; k < a.k2s; k += a.p2s)
+        piece(a.ws2 + ((size_t)row * a.s_ip + k) * W::kSize, rows, (min(a.p2s, a.k2s - k) * W::kSize + 15) & ~15);
+      for (int i = 0; i < n_act; ++i) {
+        const uint8_t* src = a.w2 + ((size_t)s.act[i] * a.dp + row) * a.ip * W::kSize;
+        for (int k = 0; k < a.k2; k += a.p2)
+          piece(src + (size_t)k * W::kSize, rows, (min(a.p2, a.k2 - k) * W::kSize + 15) & ~15);
+      }
+    }
+    // after an abort copies may still be on their way into this CTA's shared memory
+    if (*abort_flag) {
+      for (int i = max(0, it - a.stages); i < it; ++i) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(smem_u32(&s.full[i % a.stages]), (uint32_t)(i / a.stages) & 1u) &&
+               globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+    }
+  } else if (warp < kWarps) {
+    // ================================================================ compute
+    if (all_route) route<X, NT>(a, s, kServices + warp, route_warps, lane);
+    int it = 0, un = 0;  // pieces read, units handed over
+    uint32_t st = ring;
+    int len = 0, kb0 = 0, kb1 = 0;
+    auto begin = [&](int bytes) {
+      len = bytes;
+      st = ring + (uint32_t)(it % a.stages) * stage_bytes;
+      const int nkb = (len + 63) >> 6;
+      kb0 = nkb * warp / kWarps;
+      kb1 = nkb * (warp + 1) / kWarps;
+    };
+    auto arrived = [&]() { mbar_wait(smem_u32(&s.full[it % a.stages]), (uint32_t)(it / a.stages) & 1u, abort_flag, a.err); };
+    auto release = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s.empty[it % a.stages]));
+      ++it;
+    };
+    auto hand_over = [&](const float (&acc)[NT][4]) {
+      const int b = un % kParts;
+      if (un >= kParts) mbar_wait(smem_u32(&s.part_empty[b]), (uint32_t)(un / kParts - 1) & 1u, abort_flag, a.err);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
-    if constexpr (kF32) {
+      for (int nt = 0; nt < NT; ++nt)
+        *reinterpret_cast<float4*>(s.part[b][warp][nt][lane]) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s.part_full[b]));
+      ++un;
+    };
+    int nu_r = 0;
+    for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
+      const bool sh = ul < nu_s;
+      if (ul == nu_s) {
+        wait_routed();
+        nu_r = routed_units(s.n_act);
+        if (nu_r == 0) break;
+      }
+      const int r = sh ? 0 : r_first + (ul - nu_s) * G;
+      const int e = sh ? 0 : s.act[r / a.upe];
+      const int n_tok = sh ? a.T : __popc(s.emask[e]);
+      const uint32_t ntm = (1u << ((n_tok + 7) / 8)) - 1u;
+      float acc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) big[nt][i] = 0.0f;
-    }
-    for (int jj = 0; jj < n2w; ++jj) {
-      const int q = warp + kWarps * jj;
-      const bool sh = q < n2s;
-      if (sh ? !have_s : !have_r) {
-        // the intermediates come from every CTA's finishing warps
-        if (lane == 0) {
-          if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
-          else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
-        }
-        __syncwarp();
-        if (sh) have_s = true; else have_r = true;
-      }
-      const int e = sh ? 0 : s.act[(q - n2s) / n2r], kb = (sh ? q : (q - n2s) % n2r) * kKC;
-      const int kend = sh ? a.k2s : a.k2;
-      const int len = (min(kKC, kend - kb) * W::kSize + 15) & ~15;
-      const uint32_t mask = sh ? (a.T >= 32 ? 0xffffffffu : (1u << a.T) - 1u) : s.emask[e];
-      uint32_t ntm = 0u;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) ntm |= ((mask >> (8 * nt)) & 0xffu) ? 1u << nt : 0u;
-      const uint32_t st = ring + (uint32_t)((done % a.stages) * 16) * a.pitch;
-      auto at = [&](int tk) { return sh ? (size_t)tk * a.hsp : ((size_t)tk * a.k + s.slot[e][tk]) * a.hp; };
-      const uint8_t* base = sh ? a.hs : a.h;
+        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
+      auto token = [&](int n) { return sh ? n : (int)s.tok[e][n]; };
       if constexpr (kF32) {
+        float big[NT][16];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) big[nt][i] = 0.0f;
         auto row = [&](int nt, int n) {
-          return (mask >> (8 * nt + n)) & 1u ? reinterpret_cast<const float*>(base) + at(8 * nt + n) : nullptr;
+          return 8 * nt + n < n_tok ? reinterpret_cast<const float*>(a.x) + (size_t)token(8 * nt + n) * a.d : nullptr;
         };
-        stage_fma<NT, true>(big, st, a.pitch, len, kb, kend, row, ntm, lane, wait_stage);
+        for (int k = 0; k < a.d; k += a.p1) {
+          begin(min(a.p1, a.d - k) * W::kSize);
+          piece_fma<NT, false>(big, st, a.pitch, len, kb0, kb1, k, a.d, row, ntm, lane, arrived);
+          release();
+        }
+        f32_fold<NT>(big, acc, lane);
       } else {
         Rows<NT> b;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) b.p[nt] = (mask >> (8 * nt + g)) & 1u ? base + at(8 * nt + g) * 2 : nullptr;
-        if constexpr (W::kSize == 1) {
-          // every (expert, row) has its own scale: this stage's sums are scaled before they join
-          float part[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[nt][i] = 0.0f;
-          const float* sc = sh ? a.ws2s : a.w2s + (size_t)e * a.dp;
-          const float s0 = sc[r0 + min(g, rows - 1)], s1 = sc[r0 + min(g + 8, rows - 1)];
-          stage_mma<W, NT, 2>(part, st, a.pitch, len, kb, kend, b, sh ? hs_lo : h_lo, ntm, lane, wait_stage);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = fmaf(part[nt][0], s0, acc[nt][0]);
-            acc[nt][1] = fmaf(part[nt][1], s0, acc[nt][1]);
-            acc[nt][2] = fmaf(part[nt][2], s1, acc[nt][2]);
-            acc[nt][3] = fmaf(part[nt][3], s1, acc[nt][3]);
-          }
-        } else {
-          stage_mma<W, NT, 2>(acc, st, a.pitch, len, kb, kend, b, sh ? hs_lo : h_lo, ntm, lane, wait_stage);
+        for (int nt = 0; nt < NT; ++nt)
+          b.p[nt] = 8 * nt + g < n_tok ? reinterpret_cast<const uint8_t*>(a.x) + (size_t)token(8 * nt + g) * a.d * 2 : nullptr;
+        for (int k = 0; k < a.d; k += a.p1) {
+          begin(min(a.p1, a.d - k) * W::kSize);
+          piece_mma<W, NT, 1>(acc, st, a.pitch, len, kb0, kb1, k, a.d, b, 0, ntm, lane, arrived);
+          release();
         }
       }
-      release();
+      hand_over(acc);
     }
-    if constexpr (kF32) f32_fold<NT>(big, acc, lane);
-    float(*part)[NT][32][4] = s.part[tn & 1];
-    if (tn == 0) __syncthreads();  // the last units' finishing warps may still read the buffers
+    // ---- GEMM2
+    const int n_act = s.n_act;
+    const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
+    bool have_s = false, have_r = false;
+    for (int tile = cta; tile < a.tiles; tile += G) {
+      const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
+      float acc[NT][4];
+      float big[kF32 ? NT : 1][16];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      *reinterpret_cast<float4*>(part[warp][nt][lane]) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-    __syncthreads();
-    if (warp < NT) {
-      float4 v = *reinterpret_cast<const float4*>(part[0][warp][lane]);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
-        const float4 o = *reinterpret_cast<const float4*>(part[w][warp][lane]);
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
+      if constexpr (kF32) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) big[nt][i] = 0.0f;
       }
-      const float c[4] = {v.x, v.y, v.z, v.w};
-      X* out = reinterpret_cast<X*>(a.out);
+      // segment -1: the shared expert; i: active expert i
+      for (int i = a.k2s ? -1 : 0; i < n_act; ++i) {
+        const bool sh = i < 0;
+        if (sh ? !have_s : !have_r) {
+          // the intermediates come from every CTA's service warps
+          if (lane == 0) {
+            if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
+            else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
+          }
+          __syncwarp();
+          if (sh) have_s = true; else have_r = true;
+        }
+        const int e = sh ? 0 : s.act[i], kend = sh ? a.k2s : a.k2, pk = sh ? a.p2s : a.p2;
+        const uint32_t mask = sh ? (a.T >= 32 ? 0xffffffffu : (1u << a.T) - 1u) : s.emask[e];
+        uint32_t ntm = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tk = warp * 8 + 2 * t4 + (i & 1), r = g + (i >> 1) * 8;
-        if (tk < a.T && r < rows) out[(size_t)tk * a.d + r0 + r] = X(c[i]);
+        for (int nt = 0; nt < NT; ++nt) ntm |= ((mask >> (8 * nt)) & 0xffu) ? 1u << nt : 0u;
+        auto at = [&](int tk) { return sh ? (size_t)tk * a.hsp : ((size_t)tk * a.k + s.slot[e][tk]) * a.hp; };
+        const uint8_t* base = sh ? a.hs : a.h;
+        if constexpr (kF32) {
+          auto row = [&](int nt, int n) {
+            return (mask >> (8 * nt + n)) & 1u ? reinterpret_cast<const float*>(base) + at(8 * nt + n) : nullptr;
+          };
+          for (int k = 0; k < kend; k += pk) {
+            begin((min(pk, kend - k) * W::kSize + 15) & ~15);
+            piece_fma<NT, true>(big, st, a.pitch, len, kb0, kb1, k, kend, row, ntm, lane, arrived);
+            release();
+          }
+        } else {
+          Rows<NT> b;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) b.p[nt] = (mask >> (8 * nt + g)) & 1u ? base + at(8 * nt + g) * 2 : nullptr;
+          const size_t lo = sh ? hs_lo : h_lo;
+          if constexpr (W::kSize == 1) {
+            // every (expert, row) has its own scale: an expert's sums are scaled before they join
+            float part[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) part[nt][q] = 0.0f;
+            const float* sc = sh ? a.ws2s : a.w2s + (size_t)e * a.dp;
+            const float s0 = sc[r0 + min(g, rows - 1)], s1 = sc[r0 + min(g + 8, rows - 1)];
+            for (int k = 0; k < kend; k += pk) {
+              begin((min(pk, kend - k) * W::kSize + 15) & ~15);
+              piece_mma<W, NT, 2>(part, st, a.pitch, len, kb0, kb1, k, kend, b, lo, ntm, lane, arrived);
+              release();
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              acc[nt][0] = fmaf(part[nt][0], s0, acc[nt][0]);
+              acc[nt][1] = fmaf(part[nt][1], s0, acc[nt][1]);
+              acc[nt][2] = fmaf(part[nt][2], s1, acc[nt][2]);
+              acc[nt][3] = fmaf(part[nt][3], s1, acc[nt][3]);
+            }
+          } else {
+            for (int k = 0; k < kend; k += pk) {
+              begin((min(pk, kend - k) * W::kSize + 15) & ~15);
+              piece_mma<W, NT, 2>(acc, st, a.pitch, len, kb0, kb1, k, kend, b, lo, ntm, lane, arrived);
+              release();
+            }
+          }
+        }
+      }
+      if constexpr (kF32) f32_fold<NT>(big, acc, lane);
+      hand_over(acc);
+    }
+  } else {
+    // ================================================================ service
+    const int sw = warp - kService;
+    route<X, NT>(a, s, sw, route_warps, lane);
+    wait_routed();
+    const int n_act = s.n_act, n1 = nu_s + routed_units(n_act);
+    const int n2 = a.tiles > cta ? (a.tiles - cta + G - 1) / G : 0;
+    const size_t h_lo = (size_t)a.T * a.k * a.hp, hs_lo = (size_t)a.T * a.hsp;
+    uint32_t owed[2] = {0u, 0u};  // stored units of the shared expert / the routed experts not yet announced
+    auto announce = [&](int which, uint32_t* ctr) {
+      if (owed[which] == 0u) return;
+      __syncwarp();
+      if (lane == 0) ctr_add(ctr, owed[which]);
+      owed[which] = 0u;
+    };
+    for (int un = sw; un < n1 + n2; un += kServices) {
+      const int b = un % kParts;
+      // ---- where this unit's sums go, looked up before they are there
+      const bool g1 = un < n1, sh = un < nu_s;
+      if (!sh) announce(0, a.ctr + kCtrShared);
+      if (!g1) announce(1, a.ctr + kCtrRouted);
+      const int r = sh ? cta + un * G : r_first + (un - nu_s) * G;
+      const int u = sh ? r : r % a.upe, e = (g1 && !sh) ? s.act[r / a.upe] : 0;
+      const int n_tok = (sh || !g1) ? a.T : __popc(s.emask[e]);
+      float s0 = 1.0f, s1 = 1.0f;
+      if constexpr (W::kSize == 1) {
+        if (g1) {
+          const int ch = 8 * u + g;
+          const int r0 = a.glu ? (ch >> 7) * 256 + (ch & 127) : 16 * u + g, r1 = a.glu ? r0 + 128 : r0 + 8;
+          const float* sc = sh ? a.ws1s : a.w1s + (size_t)e * a.n1p;
+          s0 = __ldg(sc + r0);
+          s1 = __ldg(sc + r1);
+        }
+      }
+      mbar_wait(smem_u32(&s.part_full[b]), (uint32_t)(un / kParts) & 1u, abort_flag, a.err);
+      float c[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (nt * 8 >= n_tok) break;
+        float4 v = *reinterpret_cast<const float4*>(s.part[b][0][nt][lane]);
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+          const float4 o = *reinterpret_cast<const float4*>(s.part[b][w][nt][lane]);
+          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        c[nt][0] = v.x; c[nt][1] = v.y; c[nt][2] = v.z; c[nt][3] = v.w;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[b]));
+      if (g1) {
+        // activation, routing weight, and the intermediate to where GEMM2 reads it
+        uint8_t* base = sh ? a.hs : a.h;
+        const size_t lo = sh ? hs_lo : h_lo;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (nt * 8 >= n_tok) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = nt * 8 + 2 * t4 + i;
+            if (n >= n_tok) continue;
+            const int tk = sh ? n : s.tok[e][n], j = sh ? 0 : s.slot[e][tk];
+            const float w = sh ? s.sg[tk] : s.wt[tk][j];
+            const size_t at = sh ? (size_t)tk * a.hsp : ((size_t)tk * a.k + j) * a.hp;
+            auto put = [&](int ch, float val) {
+              if constexpr (kF32) {
+                reinterpret_cast<float*>(base)[at + ch] = val;
+              } else {
+                const __nv_bfloat16 hi = __float2bfloat16_rn(val);
+                const float rest = val - __bfloat162float(hi);
+                __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at + ch;
+                o[0] = hi;
+                // an infinite or NaN value is the high term alone
+                o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
+              }
+            };
+            const float c0 = c[nt][i] * s0, c1 = c[nt][2 + i] * s1;
+            if (a.glu) {
+              put(8 * u + g, w * (c0 / (1.0f + expf(-c0)) * c1));
+            } else {
+              put(16 * u + g, w * fmaxf(c0, 0.0f));
+              put(16 * u + g + 8, w * fmaxf(c1, 0.0f));
+            }
+          }
+        }
+        ++owed[sh ? 0 : 1];
+      } else {
+        const int r0 = (cta + (un - n1) * G) * a.rt, rows = min(a.rt, a.d - r0);
+        X* out = reinterpret_cast<X*>(a.out);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tk = nt * 8 + 2 * t4 + (i & 1), rr = g + (i >> 1) * 8;
+            if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(c[nt][i]);
+          }
       }
     }
+    announce(0, a.ctr + kCtrShared);
+    announce(1, a.ctr + kCtrRouted);
   }
 
-  // ---- after an abort stages may still be on their way into this CTA's shared memory
-  if (*abort_flag) {
-    for (int i = max(0, issued - a.stages); i < issued; ++i) {
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(bars + 8 * (i % a.stages), (uint32_t)(i / a.stages) & 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
-      }
-    }
-  }
   // ---- the last CTA to leave zeroes the counters for the next call
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -745,13 +827,18 @@ int launch(Args a, int sms, cudaStream_t stream) {
       }) != cudaSuccess)
     return DSCA_ERR_CUDA;
   constexpr int kFixed = (int)((sizeof(Smem<NT>) + 127) / 128 * 128);
-  // a warp's share of a GEMM1 row, and the bytes of a stage row: rows 64 bytes apart modulo 128, so
-  // that the eight lanes of a shared-memory access phase (two rows) meet different banks
-  a.kc1 = round_up((a.d + kWarps - 1) / kWarps, W::kBlock);
-  const int widest = max(a.kc1, max(a.k2, a.k2s)) * W::kSize;
-  a.pitch = round_up(min(kPiece, widest), 64);
+  // a row in even pieces of whole 64-byte blocks; stage rows lie 64 bytes apart modulo 128, so that the
+  // eight lanes of a shared-memory access phase (two rows) meet different banks
+  auto piece = [](int k) {
+    const int n = (k * W::kSize + kPiece - 1) / kPiece;
+    return n ? round_up((k + n - 1) / n, W::kBlock) : 0;
+  };
+  a.p1 = piece(a.d);
+  a.p2 = piece(a.k2);
+  a.p2s = piece(a.k2s);
+  a.pitch = max(a.p1, max(a.p2, a.p2s)) * W::kSize;
   if (a.pitch % 128 == 0) a.pitch += 64;
-  a.stages = min(kMaxStages, (kSmem - kFixed) / (kWarps * 16 * a.pitch));
+  a.stages = min(kMaxStages, (kSmem - kFixed) / (16 * a.pitch));
   // output rows in tiles of at most 16, as even as they come over the SMs
   const int per = (a.d + sms - 1) / sms, nt = (per + 15) / 16;
   a.rt = (a.d + sms * nt - 1) / (sms * nt);
@@ -759,7 +846,7 @@ int launch(Args a, int sms, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)sms);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(kFixed + kWarps * a.stages * 16 * a.pitch);
+  cfg.dynamicSmemBytes = (size_t)(kFixed + a.stages * 16 * a.pitch);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeCooperative;
