@@ -6,12 +6,12 @@
 // Such a call's time is the reading of the chosen experts' weights (17 MB an expert of the Qwen block
 // in bf16, 69 MB for its shared expert, against 4 KB a token), so everything here serves one
 // uninterrupted stream of weight bytes:
-//  - one persistent CTA per SM.  A producer warp copies pieces of 16 weight rows x up to 2 KB into a
-//    ring of shared-memory stages (asynchronous bulk copies, 16 a piece); eight compute warps split
-//    each piece along k, keep their sums in registers and hand them over at the end of a unit (16
-//    rows of a matrix); three service warps add the eight parts, apply the activation and store, and
-//    run the router at the start.  No role waits for another one's latency: the stream stalls only
-//    when the whole ring is full;
+//  - one persistent CTA per SM.  Two producer warps copy boxes of 16 weight rows x 64 to 320 bytes into
+//    shared memory by TMA (plain bulk copies, one a row, cost 60 ns of issue each: 16 times as much
+//    per byte); each of twelve compute warps has its own ring of boxes, its share of k, and its sums in
+//    registers, so that one warp's wait for its tokens' values (L2) passes under the others' products.
+//    Two service warps run the router at the start; then one of them, the finisher, adds the twelve
+//    parts of each unit (16 rows of a matrix), applies the activation and stores;
 //  - the weights are cut 16 rows at a time (8 gate + 8 up rows, or 16 rows of any other matrix), fine
 //    enough that 148 SMs get nearly equal shares, where a 128-row tensor-memory tile would leave
 //    two fifths of them idle at one token.  16 rows x 8 tokens is the shape of mma.sync, which
@@ -36,13 +36,14 @@
 namespace dsca {
 namespace few {
 
-constexpr int kWarps = 8;                 // compute warps (0 .. 7)
-constexpr int kProducer = kWarps;         // the warp that issues the copies
-constexpr int kService = kProducer + 1;   // first of the service warps
-constexpr int kServices = 3;
+constexpr int kCompute = 12;              // compute warps 0 .. 11: they split every row along k
+constexpr int kProducer = kCompute;       // first of the producer warps
+constexpr int kProducers = 2;
+constexpr int kService = kProducer + kProducers;  // first of the service warps
+constexpr int kServices = 2;              // both run the router; the first one finishes the units
 constexpr int kThreads = (kService + kServices) * 32;
-constexpr int kMaxStages = 16;
-constexpr int kPiece = 2048;              // bytes of one weight row in a stage, at most
+constexpr int kMaxStages = 8;             // boxes of a compute warp's ring, at most
+constexpr int kMaxBox = 320;              // bytes of a weight row in a box, at most
 constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
 constexpr int kLgPitch = 64;              // logits scratch: E + 1 <= 64 per token
 
@@ -70,9 +71,10 @@ struct Args {
   int hp, hsp;            // row pitch of h / hs in values
   int upe, ups;           // units (16 weight rows of GEMM1) per routed expert / of the shared expert
   int k2, k2s;            // values of a row of w2 / ws2 that are read
-  int p1, p2, p2s;        // values of a row that one piece of GEMM1 / routed / shared GEMM2 holds
+  int b1, b2, b2s;        // values of a row in a box: GEMM1, routed and shared GEMM2
+  int n1, n2, n2s;        // boxes of a row
   int rt, tiles;          // rows of a GEMM2 tile, tiles
-  int pitch, stages;      // bytes of a stage row, stages of the ring
+  int stage, stages;      // bytes of a stage, stages of a warp's ring
 };
 
 struct Bf16 {
@@ -88,10 +90,12 @@ struct Fp8 {
   static constexpr int kSize = 1, kBlock = 64;
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+// One box of a tensor map (weights of this GPU) into this CTA's shared memory.
+__device__ __forceinline__ void box_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -142,24 +146,23 @@ __device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n) {
 }
 
 // ---------------------------------------------------------------- shared memory
-// Units whose parts may wait for a service warp: as many as leave the ring five or six full stages.
-// At least kServices, so that a service warp that has seen one unit's parts knows every earlier use of
-// the buffer it waits for next to be complete (a parity wait cannot look two phases ahead).
-constexpr int parts_of(int nt) { return nt == 1 ? 4 : 3; }
-static_assert(parts_of(1) >= kServices && parts_of(4) >= kServices, "parity waits");
+// Sums of a unit wait for the finisher in one of kParts buffers; all compute warps and the finisher go
+// through the units in order.
+constexpr int kParts = 2;
 template <int NT>
 struct Smem {
-  static constexpr int kParts = parts_of(NT);
-  float part[kParts][kWarps][NT][32][4];    // the compute warps' sums of a unit
-  uint64_t full[kMaxStages], empty[kMaxStages];
+  float part[kParts][kCompute][NT][32][4];
+  uint64_t full[kCompute][kMaxStages], empty[kCompute][kMaxStages];
   uint64_t part_full[kParts], part_empty[kParts];
   uint64_t routed;
-  float wt[8 * NT][DSCA_MAX_TOPK];          // routing weights
+  float wt[8 * NT * DSCA_MAX_TOPK];         // routing weights by assignment
   float sg[8 * NT];                         // shared-expert gate
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
-  uint8_t act[DSCA_MAX_EXPERTS];            // experts with tokens, ascending
-  uint8_t tok[DSCA_MAX_EXPERTS][8 * NT];    // n-th token of an expert
-  uint8_t slot[DSCA_MAX_EXPERTS][8 * NT];   // choice j of (expert, token)
+  uint8_t act[DSCA_MAX_EXPERTS];            // experts with tokens ("active"), ascending
+  uint8_t cnt[DSCA_MAX_EXPERTS];            // tokens of active expert i
+  uint8_t tok[DSCA_MAX_EXPERTS][8 * NT];    // its n-th token
+  uint8_t asg[DSCA_MAX_EXPERTS][8 * NT];    // and that assignment: token * k + choice, the row of h
+  uint8_t slot[DSCA_MAX_EXPERTS][8 * NT];   // choice of (expert, token)
   int n_act;
   int abort;
 };
@@ -263,7 +266,7 @@ __device__ __forceinline__ void select_token(const Args& a, Smem<NT>& s, int t, 
       if (a.norm_topk) w = __fdiv_rn(my_p, sum);
       if (sizeof(X) == 2) w = round_bf16(w);
     }
-    s.wt[t][lane] = w;
+    s.wt[t * a.k + lane] = w;
     s.slot[my_id][t] = (uint8_t)lane;
     atomicOr(&s.emask[my_id], 1u << t);
     if (first) {
@@ -275,45 +278,36 @@ __device__ __forceinline__ void select_token(const Args& a, Smem<NT>& s, int t, 
 }
 
 // ---------------------------------------------------------------- products of one stage
-// B operand of GEMM1 / GEMM2: the tokens' rows.  p[nt] = this lane's row (token 8 nt + g) or null;
-// lo = byte distance to the low terms (GEMM2).  kTerms 1: x; 2: the intermediate.
-template <int NT>
-struct Rows {
-  const uint8_t* p[NT];
-};
-
 __device__ __forceinline__ uint4 ld_b(const uint8_t* p, bool live, bool coherent) {
   if (!live) return make_uint4(0u, 0u, 0u, 0u);
   const uint4* q = reinterpret_cast<const uint4*>(p);
   return coherent ? __ldcg(q) : *q;
 }
 
-// acc += 16 weight rows x (up to 8 NT tokens) over the 64-byte blocks [kb0, kb1) of a piece of bf16 or
-// e4m3 weights.
-//   stage: shared address of the stage, len: bytes of its rows, k0: k of its first value, klim: first k
-//   without a token value, ntm: token tiles in use.  wait(): until the stage has arrived.
-template <typename W, int NT, int kTerms, typename Wait>
-__device__ __forceinline__ void piece_mma(float (&acc)[NT][4], uint32_t stage, int pitch, int len, int kb0, int kb1, int k0,
-                                          int klim, const Rows<NT>& b, size_t lo, uint32_t ntm, int lane, Wait wait) {
-  constexpr int kPer = W::kBlock / 32;             // 16-byte token vectors per lane and 64-byte block
-  constexpr int kGroup = NT == 1 ? 4 : (NT == 2 ? 2 : 1);  // blocks whose token values are loaded together
-  const int g = lane >> 2, t = lane & 3;
+// acc += 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box of bf16 or e4m3 weights.
+//   box: this lane's place in its row g in shared memory, up: bytes from there to row g + 8,
+//   row: this lane's token row (token g) at the box's first k, lo: byte distance to its low terms,
+//   live: values of that row that are there (0: no such token).  kTerms 1: x; 2: the intermediate.
+//   wait(): until the box has arrived.
+template <typename W, int kTerms, typename Wait>
+__device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, int nkb, const uint8_t* row, size_t lo, int live,
+                                        int lane, Wait wait) {
+  constexpr int kPer = W::kBlock / 32;            // 16-byte token vectors per lane and 64-byte block
+  constexpr int kGroup = kPer == 1 ? 5 : 3;       // blocks whose token values are loaded together
+  const int t = lane & 3;
+  live = min(live, nkb * W::kBlock) - t * 8 * kPer;
+  const uint8_t* p = row + t * 16 * kPer;
+  const uint8_t* pl = p + lo;
   bool waited = false;
-  for (int kg = kb0; kg < kb1; kg += kGroup) {
-    uint4 bv[kGroup][NT][kTerms][kPer];
+  for (int kg = 0; kg < nkb; kg += kGroup) {
+    uint4 bv[kGroup][kTerms][kPer];
 #pragma unroll
     for (int i = 0; i < kGroup; ++i)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (!((ntm >> nt) & 1u)) continue;
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-          const int k = k0 + (kg + i) * W::kBlock + t * 8 * kPer + q * 8;
-          const bool live = kg + i < kb1 && k < klim && b.p[nt] != nullptr;
-#pragma unroll
-          for (int m = 0; m < kTerms; ++m)
-            bv[i][nt][m][q] = ld_b(b.p[nt] + (size_t)k * 2 + (m ? lo : 0), live, kTerms == 2);
-        }
+      for (int q = 0; q < kPer; ++q) {
+        const bool there = i * W::kBlock + q * 8 < live;
+        bv[i][0][q] = ld_b(p + i * W::kBlock * 2 + q * 16, there, kTerms == 2);
+        if constexpr (kTerms == 2) bv[i][1][q] = ld_b(pl + i * W::kBlock * 2 + q * 16, there, true);
       }
     if (!waited) {
       wait();
@@ -321,23 +315,14 @@ __device__ __forceinline__ void piece_mma(float (&acc)[NT][4], uint32_t stage, i
     }
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
-      if (kg + i >= kb1) break;
-      const int off = (kg + i) * 64 + t * 16;
-      uint4 a0 = make_uint4(0u, 0u, 0u, 0u), a1 = a0;
-      if (off < len) {  // behind the row's end the stage holds other rows' bytes
-        a0 = lds128(stage + g * pitch + off);
-        a1 = lds128(stage + (g + 8) * pitch + off);
-      }
+      if (kg + i >= nkb) break;
+      const uint4 a0 = lds128(box + i * 64), a1 = lds128(box + up + i * 64);
       if constexpr (W::kBlock == 32) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (!((ntm >> nt) & 1u)) continue;
-#pragma unroll
-          for (int m = 0; m < kTerms; ++m) {
-            const uint4 v = bv[i][nt][m][0];
-            mma_bf16(acc[nt], a0.x, a1.x, a0.y, a1.y, v.x, v.y);
-            mma_bf16(acc[nt], a0.z, a1.z, a0.w, a1.w, v.z, v.w);
-          }
+        for (int m = 0; m < kTerms; ++m) {
+          const uint4 v = bv[i][m][0];
+          mma_bf16(acc, a0.x, a1.x, a0.y, a1.y, v.x, v.y);
+          mma_bf16(acc, a0.z, a1.z, a0.w, a1.w, v.z, v.w);
         }
       } else {
         const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
@@ -347,68 +332,59 @@ __device__ __forceinline__ void piece_mma(float (&acc)[NT][4], uint32_t stage, i
           e4m3x4_to_bf16(w0[j], p0, p1);
           e4m3x4_to_bf16(w1[j], q0, q1);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (!((ntm >> nt) & 1u)) continue;
-#pragma unroll
-            for (int m = 0; m < kTerms; ++m) {
-              const uint4 v = bv[i][nt][m][j / 2];
-              mma_bf16(acc[nt], p0, q0, p1, q1, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
-            }
+          for (int m = 0; m < kTerms; ++m) {
+            const uint4 v = bv[i][m][j / 2];
+            mma_bf16(acc, p0, q0, p1, q1, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
           }
         }
       }
     }
+    box += kGroup * 64;
+    p += kGroup * W::kBlock * 2;
+    pl += kGroup * W::kBlock * 2;
+    live -= kGroup * W::kBlock;
   }
-  if (!waited) wait();
 }
 
 // The same for fp32 weights on the CUDA cores: lane (g, t) sums rows g and g + 8 over its k for all
-// eight tokens of a tile; f32_fold() adds the four lanes of a row and leaves the layout of the
-// tensor-core accumulators.  row(nt, n): token row (or null), the same on all lanes.
-template <int NT, bool kCoherent, typename Row, typename Wait>
-__device__ __forceinline__ void piece_fma(float (&acc)[NT][16], uint32_t stage, int pitch, int len, int kb0, int kb1, int k0,
-                                          int klim, Row row, uint32_t ntm, int lane, Wait wait) {
-  const int g = lane >> 2, t = lane & 3;
+// eight tokens, then the four lanes of a row are added into the layout of the tensor-core
+// accumulators.  row(n): token row n at the box's first k (or null), the same on all lanes.
+template <bool kCoherent, typename Row, typename Wait>
+__device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, int nkb, Row row, int live, int lane, Wait wait) {
+  const int t = lane & 3;
+  const float* rp[8];
+  float s[16];
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    rp[n] = row(n);
+    if (rp[n] != nullptr) rp[n] += t * 4;
+    s[2 * n] = s[2 * n + 1] = 0.0f;
+  }
   wait();
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    if (!((ntm >> nt) & 1u)) continue;
-    const float* rp[8];
-#pragma unroll
-    for (int n = 0; n < 8; ++n) rp[n] = row(nt, n);
 #pragma unroll 2
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int off = kb * 64 + t * 16;
-      const int k = k0 + kb * 16 + t * 4;
-      if (off >= len || k >= klim) continue;
-      const uint4 u0 = lds128(stage + g * pitch + off), u1 = lds128(stage + (g + 8) * pitch + off);
-      const float a0[4] = {__uint_as_float(u0.x), __uint_as_float(u0.y), __uint_as_float(u0.z), __uint_as_float(u0.w)};
-      const float a1[4] = {__uint_as_float(u1.x), __uint_as_float(u1.y), __uint_as_float(u1.z), __uint_as_float(u1.w)};
+  for (int kb = 0; kb < nkb; ++kb) {
+    if (kb * 16 + t * 4 >= live) continue;
+    const uint4 u0 = lds128(box + kb * 64), u1 = lds128(box + up + kb * 64);
+    const float a0[4] = {__uint_as_float(u0.x), __uint_as_float(u0.y), __uint_as_float(u0.z), __uint_as_float(u0.w)};
+    const float a1[4] = {__uint_as_float(u1.x), __uint_as_float(u1.y), __uint_as_float(u1.z), __uint_as_float(u1.w)};
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        if (rp[n] == nullptr) continue;
-        const float4* q = reinterpret_cast<const float4*>(rp[n] + k);
-        const float4 v = kCoherent ? __ldcg(q) : *q;
-        acc[nt][2 * n] = fmaf(a0[3], v.w, fmaf(a0[2], v.z, fmaf(a0[1], v.y, fmaf(a0[0], v.x, acc[nt][2 * n]))));
-        acc[nt][2 * n + 1] = fmaf(a1[3], v.w, fmaf(a1[2], v.z, fmaf(a1[1], v.y, fmaf(a1[0], v.x, acc[nt][2 * n + 1]))));
-      }
+    for (int n = 0; n < 8; ++n) {
+      if (rp[n] == nullptr) continue;
+      const float4* q = reinterpret_cast<const float4*>(rp[n] + kb * 16);
+      const float4 v = kCoherent ? __ldcg(q) : *q;
+      s[2 * n] = fmaf(a0[3], v.w, fmaf(a0[2], v.z, fmaf(a0[1], v.y, fmaf(a0[0], v.x, s[2 * n]))));
+      s[2 * n + 1] = fmaf(a1[3], v.w, fmaf(a1[2], v.z, fmaf(a1[1], v.y, fmaf(a1[0], v.x, s[2 * n + 1]))));
     }
   }
-}
-template <int NT>
-__device__ __forceinline__ void f32_fold(const float (&a)[NT][16], float (&acc)[NT][4], int lane) {
-  const int t = lane & 3;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int n = 0; n < 8; ++n)
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float v = a[nt][2 * n + r];
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        if (t == n / 2) acc[nt][2 * r + (n & 1)] = v;
-      }
+    for (int r = 0; r < 2; ++r) {
+      float v = s[2 * n + r];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (t == n / 2) acc[2 * r + (n & 1)] += v;
+    }
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -442,37 +418,43 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
     if (m1) s.act[__popc(b0) + __popc(b1 & below)] = (uint8_t)(lane + 32);
     if (lane == 0) s.n_act = __popc(b0) + __popc(b1);
   }
-  for (int i = wi * 32 + lane; i < DSCA_MAX_EXPERTS * 8 * NT; i += nw * 32) {
-    const int e = i / (8 * NT), t = i % (8 * NT);
+  group_sync(nw * 32);
+  for (int i = wi; i < s.n_act; i += nw) {
+    const int e = s.act[i];
     const uint32_t m = s.emask[e];
-    if ((m >> t) & 1u) s.tok[e][__popc(m & ((1u << t) - 1u))] = (uint8_t)t;
+    if (lane == 0) s.cnt[i] = (uint8_t)__popc(m);
+    if ((m >> lane) & 1u) {
+      const int n = __popc(m & ((1u << lane) - 1u));
+      s.tok[i][n] = (uint8_t)lane;
+      s.asg[i][n] = (uint8_t)(lane * a.k + s.slot[e][lane]);
+    }
   }
   group_sync(nw * 32);
   if (wi == 0 && lane == 0) mbar_arrive(smem_u32(&s.routed));
 }
 
 template <typename W, int NT>
-__global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    moe_few_kernel(const Args a, const __grid_constant__ CUtensorMap m1, const __grid_constant__ CUtensorMap m2,
+                   const __grid_constant__ CUtensorMap ms1, const __grid_constant__ CUtensorMap ms2) {
   using X = typename W::X;
   constexpr bool kF32 = W::kSize == 4;
-  constexpr int kParts = Smem<NT>::kParts;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<NT>& s = *reinterpret_cast<Smem<NT>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int G = gridDim.x, cta = blockIdx.x;
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)((sizeof(Smem<NT>) + 127) / 128 * 128);
-  const uint32_t stage_bytes = 16u * (uint32_t)a.pitch;
   volatile int* abort_flag = &s.abort;
 
-  if (threadIdx.x < (unsigned)a.stages) {
-    mbar_init(smem_u32(&s.full[threadIdx.x]), 1);
-    mbar_init(smem_u32(&s.empty[threadIdx.x]), kWarps);
+  if (threadIdx.x < kCompute * kMaxStages) {
+    mbar_init(smem_u32(&s.full[0][0] + threadIdx.x), 1);
+    mbar_init(smem_u32(&s.empty[0][0] + threadIdx.x), 1);
   }
   if (threadIdx.x < kParts) {
-    mbar_init(smem_u32(&s.part_full[threadIdx.x]), kWarps);
+    mbar_init(smem_u32(&s.part_full[threadIdx.x]), kCompute);
     mbar_init(smem_u32(&s.part_empty[threadIdx.x]), 1);
   }
-  if (threadIdx.x >= 64 && threadIdx.x < 64 + DSCA_MAX_EXPERTS) s.emask[threadIdx.x - 64] = 0u;
+  if (threadIdx.x >= 128 && threadIdx.x < 128 + DSCA_MAX_EXPERTS) s.emask[threadIdx.x - 128] = 0u;
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&s.routed), 1);
     s.abort = 0;
@@ -483,7 +465,9 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
 
   // ---- this CTA's work.  GEMM1: units cta, cta + G, ... of the shared expert, then of the routed
   // experts (the first of them on the CTA behind the last shared unit's).  GEMM2: tiles cta, cta + G,
-  // ... of the output's rows; the pieces of the shared expert's row, then of the active experts'.
+  // ... of the output's rows, for each the shared expert's row and then the active experts'.  Box j of
+  // a row goes to compute warp j mod 12; in the routed GEMM2 j counts on from expert to expert (all
+  // experts, active or not: a token's sums do not depend on the other tokens of the call).
   const int nu_s = a.ups > cta ? (a.ups - cta + G - 1) / G : 0;
   const int r_first = (cta + G - a.ups % G) % G;
   auto routed_units = [&](int n_act) {
@@ -495,87 +479,120 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
   // of them where there is no shared expert to begin with, or where the tokens are more than three
   // warps would do in the time of the first stages.
   const bool all_route = a.ups == 0 || a.T > 4;
-  const int route_warps = all_route ? kWarps + kServices : kServices;
+  const int route_warps = all_route ? kCompute + kServices : kServices;
+  auto first_box = [&](int w, int e) { return (w + kCompute - (e * a.n2) % kCompute) % kCompute; };
 
-  if (warp == kProducer) {
-    // ================================================================ producer
-    int it = 0;
-    auto piece = [&](const uint8_t* src, int rows, int len) {
-      const int st = it % a.stages;
-      if (it >= a.stages) mbar_wait(smem_u32(&s.empty[st]), (uint32_t)(it / a.stages - 1) & 1u, abort_flag, a.err);
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) return;
-      const uint32_t bar = smem_u32(&s.full[st]);
-      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(rows * len));
-      __syncwarp();
-      if (lane < rows) bulk_load(ring + (uint32_t)st * stage_bytes + (uint32_t)(lane * a.pitch), src, (uint32_t)len, bar);
-      ++it;
-    };
-    const int l = lane & 15;
-    int nu_r = 0;
-    for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
-      const bool sh = ul < nu_s;
-      if (ul == nu_s) {
-        wait_routed();
-        nu_r = routed_units(s.n_act);
-        if (nu_r == 0) break;
+  if (warp >= kProducer && warp < kService) {
+    // ================================================================ producers: one lane a ring
+    constexpr int kLanes = kCompute / kProducers;
+    if (lane < kLanes) {
+      const int w = (warp - kProducer) * kLanes + lane;
+      const uint32_t base = ring + (uint32_t)(w * a.stages * a.stage);
+      int st = 0, last = -1;  // next stage, stage before it
+      uint32_t phase = 0u;    // parity of the next stage's copy
+      bool shallow = true, wrapped = false;
+      // the next stage's barrier, its slot free and the box's bytes announced (0: abort)
+      auto slot = [&](int bytes) -> uint32_t {
+        if (wrapped) mbar_wait(smem_u32(&s.empty[w][st]), phase ^ 1u, abort_flag, a.err);
+        // Until the routing is known, one box a ring in flight: the router's loads queue behind them in DRAM
+        if (shallow && last >= 0)
+          mbar_wait(smem_u32(&s.full[w][last]), st == 0 ? phase ^ 1u : phase, abort_flag, a.err);
+        if (*abort_flag) return 0u;
+        const uint32_t bar = smem_u32(&s.full[w][st]);
+        mbar_arrive_expect_tx(bar, (uint32_t)bytes);
+        return bar;
+      };
+      auto dst = [&]() { return base + (uint32_t)(st * a.stage); };
+      auto next = [&]() {
+        last = st;
+        if (++st == a.stages) {
+          st = 0;
+          phase ^= 1u;
+          wrapped = true;
+        }
+      };
+      int nu_r = 0, r = r_first, ai = 0, first = 0;
+      for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
+        const bool sh = ul < nu_s;
+        if (ul == nu_s) {
+          wait_routed();
+          shallow = false;
+          nu_r = routed_units(s.n_act);
+          if (nu_r == 0) break;
+        }
+        if (!sh) {
+          if (ul > nu_s) r += G;
+          while (r >= first + a.upe) {
+            first += a.upe;
+            ++ai;
+          }
+        }
+        const int u = sh ? cta + ul * G : r - first, e = sh ? 0 : s.act[ai];
+        const CUtensorMap* m = sh ? &ms1 : &m1;
+        for (int j = w; j < a.n1; j += kCompute) {
+          const uint32_t bar = slot(16 * a.b1 * W::kSize);
+          if (bar == 0u) continue;
+          if (a.glu) box_load_4d(dst(), m, bar, j * a.b1, 8 * u % 128, 0, e * (a.n1p / 256) + 8 * u / 128);
+          else tma_load_2d(dst(), m, bar, j * a.b1, e * a.n1p + 16 * u);
+          next();
+        }
       }
-      const int r = sh ? cta + ul * G : r_first + (ul - nu_s) * G;
-      const int u = sh ? r : r % a.upe, e = sh ? 0 : s.act[r / a.upe];
-      const int ch = 8 * u + (l & 7);
-      const int row = a.glu ? (ch >> 7) * 256 + (ch & 127) + (l >> 3) * 128 : 16 * u + l;
-      const uint8_t* src = (sh ? a.ws1 : a.w1) + ((size_t)e * a.n1p + row) * a.d * W::kSize;
-      for (int k = 0; k < a.d; k += a.p1) piece(src + (size_t)k * W::kSize, 16, min(a.p1, a.d - k) * W::kSize);
-    }
-    const int n_act = s.n_act;
-    for (int tile = cta; tile < a.tiles; tile += G) {
-      const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0), row = r0 + min(l, rows - 1);
-      for (int k = 0; k < a.k2s; k += a.p2s)
-        piece(a.ws2 + ((size_t)row * a.s_ip + k) * W::kSize, rows, (min(a.p2s, a.k2s - k) * W::kSize + 15) & ~15);
-      for (int i = 0; i < n_act; ++i) {
-        const uint8_t* src = a.w2 + ((size_t)s.act[i] * a.dp + row) * a.ip * W::kSize;
-        for (int k = 0; k < a.k2; k += a.p2)
-          piece(src + (size_t)k * W::kSize, rows, (min(a.p2, a.k2 - k) * W::kSize + 15) & ~15);
+      const int n_act = s.n_act;
+      for (int tile = cta; tile < a.tiles; tile += G) {
+        for (int j = w; j < a.n2s; j += kCompute) {
+          const uint32_t bar = slot(a.rt * a.b2s * W::kSize);
+          if (bar == 0u) continue;
+          tma_load_2d(dst(), &ms2, bar, j * a.b2s, tile * a.rt);
+          next();
+        }
+        for (int i = 0; i < n_act; ++i) {
+          const int e = s.act[i];
+          for (int j = first_box(w, e); j < a.n2; j += kCompute) {
+            const uint32_t bar = slot(a.rt * a.b2 * W::kSize);
+            if (bar == 0u) continue;
+            tma_load_2d(dst(), &m2, bar, j * a.b2, e * a.dp + tile * a.rt);
+            next();
+          }
+        }
       }
-    }
-    // after an abort copies may still be on their way into this CTA's shared memory
-    if (*abort_flag) {
-      for (int i = max(0, it - a.stages); i < it; ++i) {
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(smem_u32(&s.full[i % a.stages]), (uint32_t)(i / a.stages) & 1u) &&
-               globaltimer_ns() - t0 < kWaitLimitNs) {
+      // after an abort copies may still be on their way into this CTA's shared memory
+      if (*abort_flag) {
+        for (int q = 0; q < (wrapped ? a.stages : st); ++q) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(smem_u32(&s.full[w][q]), q < st ? phase : phase ^ 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
+          }
         }
       }
     }
-  } else if (warp < kWarps) {
+  } else if (warp < kCompute) {
     // ================================================================ compute
     if (all_route) route<X, NT>(a, s, kServices + warp, route_warps, lane);
-    int it = 0, un = 0;  // pieces read, units handed over
-    uint32_t st = ring;
-    int len = 0, kb0 = 0, kb1 = 0;
-    auto begin = [&](int bytes) {
-      len = bytes;
-      st = ring + (uint32_t)(it % a.stages) * stage_bytes;
-      const int nkb = (len + 63) >> 6;
-      kb0 = nkb * warp / kWarps;
-      kb1 = nkb * (warp + 1) / kWarps;
-    };
-    auto arrived = [&]() { mbar_wait(smem_u32(&s.full[it % a.stages]), (uint32_t)(it / a.stages) & 1u, abort_flag, a.err); };
+    const uint32_t base = ring + (uint32_t)(warp * a.stages * a.stage);
+    int st = 0, given = 0;  // next stage, sums handed over
+    uint32_t phase = 0u;    // parity of the next stage's copy
+    auto box = [&](int pitch) { return base + (uint32_t)(st * a.stage + g * pitch + t4 * 16); };
+    auto arrived = [&]() { mbar_wait(smem_u32(&s.full[warp][st]), phase, abort_flag, a.err); };
     auto release = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.empty[it % a.stages]));
-      ++it;
+      if (lane == 0) mbar_arrive(smem_u32(&s.empty[warp][st]));
+      if (++st == a.stages) {
+        st = 0;
+        phase ^= 1u;
+      }
     };
-    auto hand_over = [&](const float (&acc)[NT][4]) {
-      const int b = un % kParts;
-      if (un >= kParts) mbar_wait(smem_u32(&s.part_empty[b]), (uint32_t)(un / kParts - 1) & 1u, abort_flag, a.err);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        *reinterpret_cast<float4*>(s.part[b][warp][nt][lane]) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+    // this warp's part of the next buffer, free to be written
+    auto buffer = [&]() {
+      const int b = given % kParts;
+      if (given >= kParts) mbar_wait(smem_u32(&s.part_empty[b]), (uint32_t)(given / kParts - 1) & 1u, abort_flag, a.err);
+      return &s.part[b][warp][0][0][0];
+    };
+    auto hand_over = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.part_full[b]));
-      ++un;
+      if (lane == 0) mbar_arrive(smem_u32(&s.part_full[given % kParts]));
+      ++given;
     };
-    int nu_r = 0;
+    const int pitch1 = a.b1 * W::kSize, blk1 = a.b1 / W::kBlock, blk2 = a.b2 / W::kBlock, blk2s = a.b2s / W::kBlock;
+    int nu_r = 0, ai = 0, r = r_first;  // routed units of this CTA; active expert and number of the next one
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
       const bool sh = ul < nu_s;
       if (ul == nu_s) {
@@ -583,127 +600,108 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
         nu_r = routed_units(s.n_act);
         if (nu_r == 0) break;
       }
-      const int r = sh ? 0 : r_first + (ul - nu_s) * G;
-      const int e = sh ? 0 : s.act[r / a.upe];
-      const int n_tok = sh ? a.T : __popc(s.emask[e]);
-      const uint32_t ntm = (1u << ((n_tok + 7) / 8)) - 1u;
+      if (!sh) {
+        if (ul > nu_s) r += G;
+        while (r >= (ai + 1) * a.upe) ++ai;
+      }
+      const int n_tok = sh ? a.T : s.cnt[ai];
       float acc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
-      auto token = [&](int n) { return sh ? n : (int)s.tok[e][n]; };
-      if constexpr (kF32) {
-        float big[NT][16];
+      for (int j = warp; j < a.n1; j += kCompute) {
+        const int k = j * a.b1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) big[nt][i] = 0.0f;
-        auto row = [&](int nt, int n) {
-          return 8 * nt + n < n_tok ? reinterpret_cast<const float*>(a.x) + (size_t)token(8 * nt + n) * a.d : nullptr;
-        };
-        for (int k = 0; k < a.d; k += a.p1) {
-          begin(min(a.p1, a.d - k) * W::kSize);
-          piece_fma<NT, false>(big, st, a.pitch, len, kb0, kb1, k, a.d, row, ntm, lane, arrived);
-          release();
+        for (int nt = 0; nt < NT; ++nt) {
+          if (nt * 8 >= n_tok) break;
+          auto row = [&](int n) -> const uint8_t* {
+            n += nt * 8;
+            if (n >= n_tok) return nullptr;
+            return reinterpret_cast<const uint8_t*>(a.x) + ((size_t)(sh ? n : (int)s.tok[ai][n]) * a.d + k) * sizeof(X);
+          };
+          if constexpr (kF32) {
+            auto frow = [&](int n) { return reinterpret_cast<const float*>(row(n)); };
+            box_fma<false>(acc[nt], box(pitch1), 8 * pitch1, blk1, frow, a.d - k, lane, arrived);
+          } else {
+            const uint8_t* p = row(g);
+            box_mma<W, 1>(acc[nt], box(pitch1), 8 * pitch1, blk1, p, 0, p != nullptr ? a.d - k : 0, lane, arrived);
+          }
         }
-        f32_fold<NT>(big, acc, lane);
-      } else {
-        Rows<NT> b;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          b.p[nt] = 8 * nt + g < n_tok ? reinterpret_cast<const uint8_t*>(a.x) + (size_t)token(8 * nt + g) * a.d * 2 : nullptr;
-        for (int k = 0; k < a.d; k += a.p1) {
-          begin(min(a.p1, a.d - k) * W::kSize);
-          piece_mma<W, NT, 1>(acc, st, a.pitch, len, kb0, kb1, k, a.d, b, 0, ntm, lane, arrived);
-          release();
-        }
+        release();
       }
-      hand_over(acc);
+      float* p = buffer();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        if (nt * 8 < n_tok && warp < a.n1)
+          *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+      hand_over();
     }
-    // ---- GEMM2
+    // ---- GEMM2: a box's sums, for the tokens of its expert, join the warp's sums of all tokens in
+    // its part buffer (a lane's four values have places of their own)
     const int n_act = s.n_act;
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;
     for (int tile = cta; tile < a.tiles; tile += G) {
       const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
-      float acc[NT][4];
-      float big[kF32 ? NT : 1][16];
+      float* p = buffer();
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
-      if constexpr (kF32) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) big[nt][i] = 0.0f;
-      }
+      for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      __syncwarp();
       // segment -1: the shared expert; i: active expert i
-      for (int i = a.k2s ? -1 : 0; i < n_act; ++i) {
+      for (int i = a.n2s ? -1 : 0; i < n_act; ++i) {
         const bool sh = i < 0;
-        if (sh ? !have_s : !have_r) {
-          // the intermediates come from every CTA's service warps
-          if (lane == 0) {
-            if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
-            else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
+        const int e = sh ? 0 : s.act[i], kend = sh ? a.k2s : a.k2, bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize;
+        const int nb = sh ? a.n2s : a.n2, blk = sh ? blk2s : blk2;
+        const int n_tok = sh ? a.T : s.cnt[i];
+        const uint8_t* hbase = sh ? a.hs : a.h;
+        const size_t lo = sh ? hs_lo : h_lo;
+        for (int j = sh ? warp : first_box(warp, e); j < nb; j += kCompute) {
+          const int k = j * bk;
+          if (sh ? !have_s : !have_r) {
+            // the intermediates come from every CTA's service warps
+            if (lane == 0) {
+              if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
+              else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
+            }
+            __syncwarp();
+            if (sh) have_s = true; else have_r = true;
           }
-          __syncwarp();
-          if (sh) have_s = true; else have_r = true;
-        }
-        const int e = sh ? 0 : s.act[i], kend = sh ? a.k2s : a.k2, pk = sh ? a.p2s : a.p2;
-        const uint32_t mask = sh ? (a.T >= 32 ? 0xffffffffu : (1u << a.T) - 1u) : s.emask[e];
-        uint32_t ntm = 0u;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) ntm |= ((mask >> (8 * nt)) & 0xffu) ? 1u << nt : 0u;
-        auto at = [&](int tk) { return sh ? (size_t)tk * a.hsp : ((size_t)tk * a.k + s.slot[e][tk]) * a.hp; };
-        const uint8_t* base = sh ? a.hs : a.h;
-        if constexpr (kF32) {
-          auto row = [&](int nt, int n) {
-            return (mask >> (8 * nt + n)) & 1u ? reinterpret_cast<const float*>(base) + at(8 * nt + n) : nullptr;
-          };
-          for (int k = 0; k < kend; k += pk) {
-            begin((min(pk, kend - k) * W::kSize + 15) & ~15);
-            piece_fma<NT, true>(big, st, a.pitch, len, kb0, kb1, k, kend, row, ntm, lane, arrived);
-            release();
-          }
-        } else {
-          Rows<NT> b;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) b.p[nt] = (mask >> (8 * nt + g)) & 1u ? base + at(8 * nt + g) * 2 : nullptr;
-          const size_t lo = sh ? hs_lo : h_lo;
+          float s0 = 1.0f, s1 = 1.0f;
           if constexpr (W::kSize == 1) {
-            // every (expert, row) has its own scale: an expert's sums are scaled before they join
-            float part[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) part[nt][q] = 0.0f;
-            const float* sc = sh ? a.ws2s : a.w2s + (size_t)e * a.dp;
-            const float s0 = sc[r0 + min(g, rows - 1)], s1 = sc[r0 + min(g + 8, rows - 1)];
-            for (int k = 0; k < kend; k += pk) {
-              begin((min(pk, kend - k) * W::kSize + 15) & ~15);
-              piece_mma<W, NT, 2>(part, st, a.pitch, len, kb0, kb1, k, kend, b, lo, ntm, lane, arrived);
-              release();
+            const float* sc = (sh ? a.ws2s : a.w2s + (size_t)e * a.dp) + r0;
+            s0 = __ldg(sc + min(g, rows - 1));
+            s1 = __ldg(sc + min(g + 8, rows - 1));
+          }
+          for (int n0 = 0; n0 < n_tok; n0 += 8) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            auto row = [&](int n) -> const uint8_t* {
+              n += n0;
+              if (n >= n_tok) return nullptr;
+              return hbase + ((size_t)(sh ? n : (int)s.asg[i][n]) * (sh ? a.hsp : a.hp) + k) * (kF32 ? 4 : 2);
+            };
+            if constexpr (kF32) {
+              auto frow = [&](int n) { return reinterpret_cast<const float*>(row(n)); };
+              box_fma<true>(acc, box(pitch), 8 * pitch, blk, frow, kend - k, lane, arrived);
+            } else {
+              const uint8_t* b = row(g);
+              box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, b, lo, b != nullptr ? kend - k : 0, lane, arrived);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[nt][0] = fmaf(part[nt][0], s0, acc[nt][0]);
-              acc[nt][1] = fmaf(part[nt][1], s0, acc[nt][1]);
-              acc[nt][2] = fmaf(part[nt][2], s1, acc[nt][2]);
-              acc[nt][3] = fmaf(part[nt][3], s1, acc[nt][3]);
-            }
-          } else {
-            for (int k = 0; k < kend; k += pk) {
-              begin((min(pk, kend - k) * W::kSize + 15) & ~15);
-              piece_mma<W, NT, 2>(acc, st, a.pitch, len, kb0, kb1, k, kend, b, lo, ntm, lane, arrived);
-              release();
+            for (int q = 0; q < 2; ++q) {
+              const int n = n0 + 2 * t4 + q;
+              if (n < n_tok) {
+                const int tk = sh ? n : (int)s.tok[i][n];
+                float* o = p + ((tk >> 3) * 32 + g * 4 + ((tk & 7) >> 1)) * 4 + (tk & 1);
+                o[0] = fmaf(acc[q], s0, o[0]);
+                o[2] = fmaf(acc[2 + q], s1, o[2]);
+              }
             }
           }
+          release();
         }
       }
-      if constexpr (kF32) f32_fold<NT>(big, acc, lane);
-      hand_over(acc);
+      hand_over();
     }
   } else {
     // ================================================================ service
@@ -720,90 +718,103 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
       if (lane == 0) ctr_add(ctr, owed[which]);
       owed[which] = 0u;
     };
-    for (int un = sw; un < n1 + n2; un += kServices) {
-      const int b = un % kParts;
-      // ---- where this unit's sums go, looked up before they are there
-      const bool g1 = un < n1, sh = un < nu_s;
-      if (!sh) announce(0, a.ctr + kCtrShared);
-      if (!g1) announce(1, a.ctr + kCtrRouted);
-      const int r = sh ? cta + un * G : r_first + (un - nu_s) * G;
-      const int u = sh ? r : r % a.upe, e = (g1 && !sh) ? s.act[r / a.upe] : 0;
-      const int n_tok = (sh || !g1) ? a.T : __popc(s.emask[e]);
+    int seen = 0;
+    auto wait_parts = [&]() {
+      mbar_wait(smem_u32(&s.part_full[seen % kParts]), (uint32_t)(seen / kParts) & 1u, abort_flag, a.err);
+    };
+    // tile nt of the sums of the first n compute warps
+    auto sum = [&](int n, int nt, float (&c)[4]) {
+      c[0] = c[1] = c[2] = c[3] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kCompute; ++w) {
+        if (w >= n) break;
+        const float4 o = *reinterpret_cast<const float4*>(s.part[seen % kParts][w][nt][lane]);
+        c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
+      }
+    };
+    auto free_parts = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[seen % kParts]));
+      ++seen;
+    };
+    int r = r_first, ai = 0, first = 0;  // number, active expert and that expert's first unit of the next routed unit
+    for (int un = 0; sw == 0 && un < n1; ++un) {
+      const bool sh = un < nu_s;
+      if (un == nu_s) announce(0, a.ctr + kCtrShared);
+      if (!sh) {
+        if (un > nu_s) r += G;
+        while (r >= first + a.upe) {
+          first += a.upe;
+          ++ai;
+        }
+      }
+      const int u = sh ? cta + un * G : r - first, e = sh ? 0 : s.act[ai];
+      const int n_tok = sh ? a.T : s.cnt[ai];
+      // where this unit's sums go is looked up before they are there
       float s0 = 1.0f, s1 = 1.0f;
       if constexpr (W::kSize == 1) {
-        if (g1) {
-          const int ch = 8 * u + g;
-          const int r0 = a.glu ? (ch >> 7) * 256 + (ch & 127) : 16 * u + g, r1 = a.glu ? r0 + 128 : r0 + 8;
-          const float* sc = sh ? a.ws1s : a.w1s + (size_t)e * a.n1p;
-          s0 = __ldg(sc + r0);
-          s1 = __ldg(sc + r1);
-        }
+        const int ch = 8 * u + g;
+        const int r0 = a.glu ? (ch >> 7) * 256 + (ch & 127) : 16 * u + g, r1 = a.glu ? r0 + 128 : r0 + 8;
+        const float* sc = sh ? a.ws1s : a.w1s + (size_t)e * a.n1p;
+        s0 = __ldg(sc + r0);
+        s1 = __ldg(sc + r1);
       }
-      mbar_wait(smem_u32(&s.part_full[b]), (uint32_t)(un / kParts) & 1u, abort_flag, a.err);
-      float c[NT][4];
+      wait_parts();
+      // activation, routing weight, and the intermediate to where GEMM2 reads it
+      uint8_t* base = sh ? a.hs : a.h;
+      const size_t lo = sh ? hs_lo : h_lo;
+      for (int nt = 0; nt * 8 < n_tok; ++nt) {
+        float c[4];
+        sum(a.n1, nt, c);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (nt * 8 >= n_tok) break;
-        float4 v = *reinterpret_cast<const float4*>(s.part[b][0][nt][lane]);
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) {
-          const float4 o = *reinterpret_cast<const float4*>(s.part[b][w][nt][lane]);
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        c[nt][0] = v.x; c[nt][1] = v.y; c[nt][2] = v.z; c[nt][3] = v.w;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[b]));
-      if (g1) {
-        // activation, routing weight, and the intermediate to where GEMM2 reads it
-        uint8_t* base = sh ? a.hs : a.h;
-        const size_t lo = sh ? hs_lo : h_lo;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt * 8 >= n_tok) break;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int n = nt * 8 + 2 * t4 + i;
-            if (n >= n_tok) continue;
-            const int tk = sh ? n : s.tok[e][n], j = sh ? 0 : s.slot[e][tk];
-            const float w = sh ? s.sg[tk] : s.wt[tk][j];
-            const size_t at = sh ? (size_t)tk * a.hsp : ((size_t)tk * a.k + j) * a.hp;
-            auto put = [&](int ch, float val) {
-              if constexpr (kF32) {
-                reinterpret_cast<float*>(base)[at + ch] = val;
-              } else {
-                const __nv_bfloat16 hi = __float2bfloat16_rn(val);
-                const float rest = val - __bfloat162float(hi);
-                __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at + ch;
-                o[0] = hi;
-                // an infinite or NaN value is the high term alone
-                o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
-              }
-            };
-            const float c0 = c[nt][i] * s0, c1 = c[nt][2 + i] * s1;
-            if (a.glu) {
-              put(8 * u + g, w * (c0 / (1.0f + expf(-c0)) * c1));
+        for (int i = 0; i < 2; ++i) {
+          const int n = nt * 8 + 2 * t4 + i;
+          if (n >= n_tok) continue;
+          const float w = sh ? s.sg[n] : s.wt[s.asg[ai][n]];
+          const size_t at = sh ? (size_t)n * a.hsp : (size_t)s.asg[ai][n] * a.hp;
+          auto put = [&](int ch, float val) {
+            if constexpr (kF32) {
+              reinterpret_cast<float*>(base)[at + ch] = val;
             } else {
-              put(16 * u + g, w * fmaxf(c0, 0.0f));
-              put(16 * u + g + 8, w * fmaxf(c1, 0.0f));
+              const __nv_bfloat16 hi = __float2bfloat16_rn(val);
+              const float rest = val - __bfloat162float(hi);
+              __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at + ch;
+              o[0] = hi;
+              // an infinite or NaN value is the high term alone
+              o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
             }
+          };
+          const float c0 = c[i] * s0, c1 = c[2 + i] * s1;
+          if (a.glu) {
+            put(8 * u + g, w * (c0 / (1.0f + expf(-c0)) * c1));
+          } else {
+            put(16 * u + g, w * fmaxf(c0, 0.0f));
+            put(16 * u + g + 8, w * fmaxf(c1, 0.0f));
           }
         }
-        ++owed[sh ? 0 : 1];
-      } else {
-        const int r0 = (cta + (un - n1) * G) * a.rt, rows = min(a.rt, a.d - r0);
-        X* out = reinterpret_cast<X*>(a.out);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tk = nt * 8 + 2 * t4 + (i & 1), rr = g + (i >> 1) * 8;
-            if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(c[nt][i]);
-          }
       }
+      free_parts();
+      ++owed[sh ? 0 : 1];
     }
     announce(0, a.ctr + kCtrShared);
     announce(1, a.ctr + kCtrRouted);
+    // ---- the output's rows
+    for (int n = 0; sw == 0 && n < n2; ++n) {
+      const int r0 = (cta + n * G) * a.rt, rows = min(a.rt, a.d - r0);
+      wait_parts();
+      X* out = reinterpret_cast<X*>(a.out);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float c[4];
+        sum(kCompute, nt, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tk = nt * 8 + 2 * t4 + (i & 1), rr = g + (i >> 1) * 8;
+          if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(c[i]);
+        }
+      }
+      free_parts();
+    }
   }
 
   // ---- the last CTA to leave zeroes the counters for the next call
@@ -819,48 +830,105 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_kernel(const Args a) {
 
 inline int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_fn() {
+  static EncodeTiled fn = nullptr;
+  if (fn == nullptr) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(ptr);
+  }
+  return fn;
+}
+
+// Boxes of `rows` rows x `box` values of a row-major matrix [n, width]; glu: of 8 gate and the matching 8
+// up rows of its 256-row blocks.  Values behind the row's end are filled with zeros.
+template <typename W>
+int make_map(CUtensorMap* m, const void* base, uint64_t n, int width, int box, int rows, bool glu) {
+  EncodeTiled enc = encode_fn();
+  if (enc == nullptr) return DSCA_ERR_CUDA;
+  const CUtensorMapDataType type = W::kSize == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : W::kSize == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const cuuint64_t row = (cuuint64_t)width * W::kSize;
+  const cuuint64_t dims[4] = {(cuuint64_t)width, glu ? 128u : n, 2, n / 256}, strides[3] = {row, row * 128, row * 256};
+  const cuuint32_t boxes[4] = {(cuuint32_t)box, (cuuint32_t)(glu ? 8 : rows), 2, 1}, one[4] = {1, 1, 1, 1};
+  return enc(m, type, glu ? 4 : 2, const_cast<void*>(base), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? DSCA_OK
+             : DSCA_ERR_CUDA;
+}
+
+// Bytes of a row of `bytes` in a box: the twelve warps take the boxes in turn, and a warp's time for one
+// is about that of 256 bytes for the tokens' values from L2 plus that of the box itself.  Tensor maps
+// take at most 256 values.
+template <typename W>
+int box_of(int bytes) {
+  int best = 64, cost = 1 << 30;
+  for (int b = 64; b <= kMaxBox && b <= 256 * W::kSize; b += 64) {
+    const int n = (bytes + b - 1) / b, c = (n + kCompute - 1) / kCompute * (b + 256);
+    if (c < cost) {
+      best = b;
+      cost = c;
+    }
+  }
+  return best;
+}
+
 template <typename W, int NT>
-int launch(Args a, int sms, cudaStream_t stream) {
+int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   static PerDeviceOnce once;
   if (once.run([] {
         return cudaFuncSetAttribute(moe_few_kernel<W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
       }) != cudaSuccess)
     return DSCA_ERR_CUDA;
   constexpr int kFixed = (int)((sizeof(Smem<NT>) + 127) / 128 * 128);
-  // a row in even pieces of whole 64-byte blocks; stage rows lie 64 bytes apart modulo 128, so that the
-  // eight lanes of a shared-memory access phase (two rows) meet different banks
-  auto piece = [](int k) {
-    const int n = (k * W::kSize + kPiece - 1) / kPiece;
-    return n ? round_up((k + n - 1) / n, W::kBlock) : 0;
+  static_assert((kSmem - kFixed) / (kCompute * 16 * kMaxBox) >= 2, "two boxes a ring");
+  auto boxes = [](int k, int* b, int* n) {
+    *b = box_of<W>(k * W::kSize) / W::kSize;
+    *n = (k + *b - 1) / *b;
   };
-  a.p1 = piece(a.d);
-  a.p2 = piece(a.k2);
-  a.p2s = piece(a.k2s);
-  a.pitch = max(a.p1, max(a.p2, a.p2s)) * W::kSize;
-  if (a.pitch % 128 == 0) a.pitch += 64;
-  a.stages = min(kMaxStages, (kSmem - kFixed) / (16 * a.pitch));
+  boxes(a.d, &a.b1, &a.n1);
+  boxes(a.k2, &a.b2, &a.n2);
+  boxes(a.k2s, &a.b2s, &a.n2s);
+  a.stage = 16 * max(a.b1, max(a.b2, a.n2s ? a.b2s : 0)) * W::kSize;
+  a.stages = min(kMaxStages, (kSmem - kFixed) / (kCompute * a.stage));
   // output rows in tiles of at most 16, as even as they come over the SMs
   const int per = (a.d + sms - 1) / sms, nt = (per + 15) / 16;
   a.rt = (a.d + sms * nt - 1) / (sms * nt);
   a.tiles = (a.d + a.rt - 1) / a.rt;
+  CUtensorMap m1, m2, ms1, ms2;
+  int rc;
+  if ((rc = make_map<W>(&m1, a.w1, (uint64_t)a.E * a.n1p, a.d, a.b1, 16, a.glu))) return rc;
+  if ((rc = make_map<W>(&m2, a.w2, (uint64_t)a.E * a.dp, a.ip, a.b2, a.rt, false))) return rc;
+  ms1 = m1;
+  ms2 = m2;
+  if (a.ups) {
+    if ((rc = make_map<W>(&ms1, a.ws1, (uint64_t)p->shared_n1p, a.d, a.b1, 16, a.glu))) return rc;
+    if ((rc = make_map<W>(&ms2, a.ws2, (uint64_t)a.dp, a.s_ip, a.b2s, a.rt, false))) return rc;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)sms);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(kFixed + a.stages * 16 * a.pitch);
+  cfg.dynamicSmemBytes = (size_t)(kFixed + kCompute * a.stages * a.stage);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeCooperative;
   at[0].val.cooperative = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, moe_few_kernel<W, NT>, (const Args)a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, moe_few_kernel<W, NT>, (const Args)a, m1, m2, ms1, ms2) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
 template <typename W>
-int launch_t(const Args& a, int sms, cudaStream_t stream) {
-  if (a.T <= 8) return launch<W, 1>(a, sms, stream);
-  if (a.T <= 16) return launch<W, 2>(a, sms, stream);
-  return launch<W, 4>(a, sms, stream);
+int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream) {
+  if (a.T <= 8) return launch<W, 1>(a, p, sms, stream);
+  if (a.T <= 16) return launch<W, 2>(a, p, sms, stream);
+  return launch<W, 4>(a, p, sms, stream);
 }
 
 }  // namespace few
@@ -895,9 +963,9 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.lg = (float*)(w + DSCA_FEW_COUNTER_BYTES);
   a.h = w + DSCA_FEW_COUNTER_BYTES + (size_t)a.T * few::kLgPitch * 4;
   a.hs = a.h + (size_t)a.T * a.k * a.hp * 4;
-  if (p->weights == DSCA_BF16) return few::launch_t<few::Bf16>(a, num_sms, stream);
-  if (p->weights == DSCA_F32) return few::launch_t<few::F32>(a, num_sms, stream);
-  return few::launch_t<few::Fp8>(a, num_sms, stream);
+  if (p->weights == DSCA_BF16) return few::launch_t<few::Bf16>(a, p, num_sms, stream);
+  if (p->weights == DSCA_F32) return few::launch_t<few::F32>(a, p, num_sms, stream);
+  return few::launch_t<few::Fp8>(a, p, num_sms, stream);
 }
 
 }  // namespace dsca
