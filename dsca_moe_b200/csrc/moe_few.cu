@@ -10,8 +10,9 @@
 //    shared memory by TMA (plain bulk copies, one a row, cost 60 ns of issue each: 16 times as much
 //    per byte); each of twelve compute warps has its own ring of boxes, its share of k, and its sums in
 //    registers, so that one warp's wait for its tokens' values (L2) passes under the others' products.
-//    Two service warps run the router at the start; then one of them, the finisher, adds the twelve
-//    parts of each unit (16 rows of a matrix), applies the activation and stores;
+//    The values for the next box are asked for before the present one is multiplied.  Two service
+//    warps run the router at the start; then, in turn, they add the twelve parts of each unit (16
+//    rows of a matrix), apply the activation and store;
 //  - the weights are cut 16 rows at a time (8 gate + 8 up rows, or 16 rows of any other matrix), fine
 //    enough that 148 SMs get nearly equal shares, where a 128-row tensor-memory tile would leave
 //    two fifths of them idle at one token.  16 rows x 8 tokens is the shape of mma.sync, which
@@ -40,10 +41,11 @@ constexpr int kCompute = 12;              // compute warps 0 .. 11: they split e
 constexpr int kProducer = kCompute;       // first of the producer warps
 constexpr int kProducers = 2;
 constexpr int kService = kProducer + kProducers;  // first of the service warps
-constexpr int kServices = 2;              // both run the router; the first one finishes the units
+constexpr int kServices = 2;              // they run the router, then finish the units in turn
 constexpr int kThreads = (kService + kServices) * 32;
 constexpr int kMaxStages = 8;             // boxes of a compute warp's ring, at most
-constexpr int kMaxBox = 320;              // bytes of a weight row in a box, at most
+constexpr int kMaxBox = 256;              // bytes of a weight row in a box, at most
+constexpr int kVals = 8;                  // 16-byte vectors of token values that a lane holds for a box
 constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
 constexpr int kLgPitch = 64;              // logits scratch: E + 1 <= 64 per token
 
@@ -146,9 +148,10 @@ __device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n) {
 }
 
 // ---------------------------------------------------------------- shared memory
-// Sums of a unit wait for the finisher in one of kParts buffers; all compute warps and the finisher go
-// through the units in order.
-constexpr int kParts = 2;
+// Sums of a unit wait for their service warp in one of kParts buffers, one for each service warp: all
+// compute warps take part in every unit, so a warp that has finished unit n knows the buffer's use before
+// unit n + kParts to be complete (a parity wait cannot look two phases ahead).
+constexpr int kParts = kServices;
 template <int NT>
 struct Smem {
   float part[kParts][kCompute][NT][32][4];
@@ -284,73 +287,70 @@ __device__ __forceinline__ uint4 ld_b(const uint8_t* p, bool live, bool coherent
   return coherent ? __ldcg(q) : *q;
 }
 
-// acc += 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box of bf16 or e4m3 weights.
-//   box: this lane's place in its row g in shared memory, up: bytes from there to row g + 8,
+// A lane's token values for a box of bf16 or e4m3 weights: vector (i, m, q) holds eight values of 64-byte
+// block i, term m (0: x or the high term, 1: the low term), part q.
 //   row: this lane's token row (token g) at the box's first k, lo: byte distance to its low terms,
-//   live: values of that row that are there (0: no such token).  kTerms 1: x; 2: the intermediate.
-//   wait(): until the box has arrived.
-template <typename W, int kTerms, typename Wait>
-__device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, int nkb, const uint8_t* row, size_t lo, int live,
-                                        int lane, Wait wait) {
-  constexpr int kPer = W::kBlock / 32;            // 16-byte token vectors per lane and 64-byte block
-  constexpr int kGroup = kPer == 1 ? 5 : 3;       // blocks whose token values are loaded together
-  const int t = lane & 3;
-  live = min(live, nkb * W::kBlock) - t * 8 * kPer;
-  const uint8_t* p = row + t * 16 * kPer;
+//   live: values of that row that are there (0: no such token).
+template <typename W, int kTerms>
+struct Layout {
+  static constexpr int kPer = W::kBlock < 32 ? 1 : W::kBlock / 32;  // vectors of a block and term
+  static constexpr int kBlocks = kVals / (kPer * kTerms);           // blocks of a box, at most
+  static __device__ __forceinline__ int at(int i, int m, int q) { return (i * kTerms + m) * kPer + q; }
+};
+template <typename W, int kTerms>
+__device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row, size_t lo, int live, int lane) {
+  using L = Layout<W, kTerms>;
+  const int t8 = (lane & 3) * 8 * L::kPer;
+  live -= t8;
+  const uint8_t* p = row + t8 * 2;
   const uint8_t* pl = p + lo;
-  bool waited = false;
-  for (int kg = 0; kg < nkb; kg += kGroup) {
-    uint4 bv[kGroup][kTerms][kPer];
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i)
+  for (int i = 0; i < L::kBlocks; ++i)
 #pragma unroll
-      for (int q = 0; q < kPer; ++q) {
-        const bool there = i * W::kBlock + q * 8 < live;
-        bv[i][0][q] = ld_b(p + i * W::kBlock * 2 + q * 16, there, kTerms == 2);
-        if constexpr (kTerms == 2) bv[i][1][q] = ld_b(pl + i * W::kBlock * 2 + q * 16, there, true);
-      }
-    if (!waited) {
-      wait();
-      waited = true;
+    for (int q = 0; q < L::kPer; ++q) {
+      const int k = i * W::kBlock + q * 8;
+      v[L::at(i, 0, q)] = ld_b(p + k * 2, k < live, kTerms == 2);
+      if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, k < live, true);
     }
+}
+// acc += 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box.  box: this lane's place in its
+// row g in shared memory, up: bytes from there to row g + 8.
+template <typename W, int kTerms>
+__device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, int nkb, const uint4 (&v)[kVals]) {
+  using L = Layout<W, kTerms>;
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-      if (kg + i >= nkb) break;
-      const uint4 a0 = lds128(box + i * 64), a1 = lds128(box + up + i * 64);
-      if constexpr (W::kBlock == 32) {
+  for (int i = 0; i < L::kBlocks; ++i) {
+    if (i >= nkb) break;
+    const uint4 a0 = lds128(box + i * 64), a1 = lds128(box + up + i * 64);
+    if constexpr (W::kBlock == 32) {
+#pragma unroll
+      for (int m = 0; m < kTerms; ++m) {
+        const uint4 b = v[L::at(i, m, 0)];
+        mma_bf16(acc, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+        mma_bf16(acc, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+      }
+    } else {
+      const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t p0, p1, q0, q1;
+        e4m3x4_to_bf16(w0[j], p0, p1);
+        e4m3x4_to_bf16(w1[j], q0, q1);
 #pragma unroll
         for (int m = 0; m < kTerms; ++m) {
-          const uint4 v = bv[i][m][0];
-          mma_bf16(acc, a0.x, a1.x, a0.y, a1.y, v.x, v.y);
-          mma_bf16(acc, a0.z, a1.z, a0.w, a1.w, v.z, v.w);
-        }
-      } else {
-        const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t p0, p1, q0, q1;
-          e4m3x4_to_bf16(w0[j], p0, p1);
-          e4m3x4_to_bf16(w1[j], q0, q1);
-#pragma unroll
-          for (int m = 0; m < kTerms; ++m) {
-            const uint4 v = bv[i][m][j / 2];
-            mma_bf16(acc, p0, q0, p1, q1, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
-          }
+          const uint4 b = v[L::at(i, m, j / 2)];
+          mma_bf16(acc, p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
         }
       }
     }
-    box += kGroup * 64;
-    p += kGroup * W::kBlock * 2;
-    pl += kGroup * W::kBlock * 2;
-    live -= kGroup * W::kBlock;
   }
 }
 
 // The same for fp32 weights on the CUDA cores: lane (g, t) sums rows g and g + 8 over its k for all
 // eight tokens, then the four lanes of a row are added into the layout of the tensor-core
 // accumulators.  row(n): token row n at the box's first k (or null), the same on all lanes.
-template <bool kCoherent, typename Row, typename Wait>
-__device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, int nkb, Row row, int live, int lane, Wait wait) {
+template <bool kCoherent, typename Row>
+__device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, int nkb, Row row, int live, int lane) {
   const int t = lane & 3;
   const float* rp[8];
   float s[16];
@@ -360,7 +360,6 @@ __device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, i
     if (rp[n] != nullptr) rp[n] += t * 4;
     s[2 * n] = s[2 * n + 1] = 0.0f;
   }
-  wait();
 #pragma unroll 2
   for (int kb = 0; kb < nkb; ++kb) {
     if (kb * 16 + t * 4 >= live) continue;
@@ -484,83 +483,94 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= kProducer && warp < kService) {
     // ================================================================ producers: one lane a ring
+    // The lanes stay together (a lane that waits alone holds up the others of its warp), so a ring gets
+    // its next box when the rings of all six have room.
     constexpr int kLanes = kCompute / kProducers;
-    if (lane < kLanes) {
-      const int w = (warp - kProducer) * kLanes + lane;
-      const uint32_t base = ring + (uint32_t)(w * a.stages * a.stage);
-      int st = 0, last = -1;  // next stage, stage before it
-      uint32_t phase = 0u;    // parity of the next stage's copy
-      bool shallow = true, wrapped = false;
-      // the next stage's barrier, its slot free and the box's bytes announced (0: abort)
-      auto slot = [&](int bytes) -> uint32_t {
-        if (wrapped) mbar_wait(smem_u32(&s.empty[w][st]), phase ^ 1u, abort_flag, a.err);
-        // Until the routing is known, one box a ring in flight: the router's loads queue behind them in DRAM
-        if (shallow && last >= 0)
-          mbar_wait(smem_u32(&s.full[w][last]), st == 0 ? phase ^ 1u : phase, abort_flag, a.err);
-        if (*abort_flag) return 0u;
+    const bool on = lane < kLanes;
+    const int w = (warp - kProducer) * kLanes + (on ? lane : 0);
+    const uint32_t base = ring + (uint32_t)(w * a.stages * a.stage);
+    int st = 0, last = -1;  // next stage, stage before it
+    uint32_t phase = 0u;    // parity of the next stage's copy
+    bool shallow = true, wrapped = false, stop = false;
+    // Box j of this lane's row, if there is one: load(bar, dst) once its stage is free.
+    auto box = [&](bool there, int bytes, auto load) {
+      const uint32_t e = smem_u32(&s.empty[w][st]), f = smem_u32(&s.full[w][max(last, 0)]);
+      // Until the routing is known, one box a ring in flight: the router's loads queue behind them in DRAM
+      const bool we = there && wrapped, wf = there && shallow && last >= 0;
+      const uint64_t t0 = globaltimer_ns();
+      for (uint32_t it = 0;; ++it) {
+        const bool ok = (!we || mbar_try_wait(e, phase ^ 1u)) && (!wf || mbar_try_wait(f, st == 0 ? phase ^ 1u : phase));
+        if (__all_sync(0xffffffffu, ok)) break;
+        if ((it & 63u) == 63u) {
+          if (lane == 0 && globaltimer_ns() - t0 > kWaitLimitNs) {
+            record_error(a.err, kErrWaitTimeout);
+            *abort_flag = 1;
+          }
+          __syncwarp();
+          if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+        }
+      }
+      stop = stop || __any_sync(0xffffffffu, *abort_flag != 0);
+      if (there && !stop) {
         const uint32_t bar = smem_u32(&s.full[w][st]);
         mbar_arrive_expect_tx(bar, (uint32_t)bytes);
-        return bar;
-      };
-      auto dst = [&]() { return base + (uint32_t)(st * a.stage); };
-      auto next = [&]() {
+        load(bar, base + (uint32_t)(st * a.stage));
         last = st;
         if (++st == a.stages) {
           st = 0;
           phase ^= 1u;
           wrapped = true;
         }
-      };
-      int nu_r = 0, r = r_first, ai = 0, first = 0;
-      for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
-        const bool sh = ul < nu_s;
-        if (ul == nu_s) {
-          wait_routed();
-          shallow = false;
-          nu_r = routed_units(s.n_act);
-          if (nu_r == 0) break;
-        }
-        if (!sh) {
-          if (ul > nu_s) r += G;
-          while (r >= first + a.upe) {
-            first += a.upe;
-            ++ai;
-          }
-        }
-        const int u = sh ? cta + ul * G : r - first, e = sh ? 0 : s.act[ai];
-        const CUtensorMap* m = sh ? &ms1 : &m1;
-        for (int j = w; j < a.n1; j += kCompute) {
-          const uint32_t bar = slot(16 * a.b1 * W::kSize);
-          if (bar == 0u) continue;
-          if (a.glu) box_load_4d(dst(), m, bar, j * a.b1, 8 * u % 128, 0, e * (a.n1p / 256) + 8 * u / 128);
-          else tma_load_2d(dst(), m, bar, j * a.b1, e * a.n1p + 16 * u);
-          next();
+      }
+      __syncwarp();
+    };
+    int nu_r = 0, r = r_first, ai = 0, first = 0;
+    for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
+      const bool sh = ul < nu_s;
+      if (ul == nu_s) {
+        wait_routed();
+        shallow = false;
+        nu_r = routed_units(s.n_act);
+        if (nu_r == 0) break;
+      }
+      if (!sh) {
+        if (ul > nu_s) r += G;
+        while (r >= first + a.upe) {
+          first += a.upe;
+          ++ai;
         }
       }
-      const int n_act = s.n_act;
-      for (int tile = cta; tile < a.tiles; tile += G) {
-        for (int j = w; j < a.n2s; j += kCompute) {
-          const uint32_t bar = slot(a.rt * a.b2s * W::kSize);
-          if (bar == 0u) continue;
-          tma_load_2d(dst(), &ms2, bar, j * a.b2s, tile * a.rt);
-          next();
-        }
-        for (int i = 0; i < n_act; ++i) {
-          const int e = s.act[i];
-          for (int j = first_box(w, e); j < a.n2; j += kCompute) {
-            const uint32_t bar = slot(a.rt * a.b2 * W::kSize);
-            if (bar == 0u) continue;
-            tma_load_2d(dst(), &m2, bar, j * a.b2, e * a.dp + tile * a.rt);
-            next();
-          }
+      const int u = sh ? cta + ul * G : r - first, e = sh ? 0 : s.act[ai];
+      const CUtensorMap* m = sh ? &ms1 : &m1;
+      for (int j0 = 0; j0 < a.n1; j0 += kCompute) {
+        const int j = j0 + w;
+        box(on && j < a.n1, 16 * a.b1 * W::kSize, [&](uint32_t bar, uint32_t dst) {
+          if (a.glu) box_load_4d(dst, m, bar, j * a.b1, 8 * u % 128, 0, e * (a.n1p / 256) + 8 * u / 128);
+          else tma_load_2d(dst, m, bar, j * a.b1, e * a.n1p + 16 * u);
+        });
+      }
+    }
+    const int n_act = s.n_act;
+    for (int tile = cta; tile < a.tiles; tile += G) {
+      for (int j0 = 0; j0 < a.n2s; j0 += kCompute) {
+        const int j = j0 + w;
+        box(on && j < a.n2s, a.rt * a.b2s * W::kSize,
+            [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &ms2, bar, j * a.b2s, tile * a.rt); });
+      }
+      for (int i = 0; i < n_act; ++i) {
+        const int e = s.act[i], fb = first_box(w, e);
+        for (int j0 = 0; j0 < a.n2; j0 += kCompute) {
+          const int j = j0 + fb;
+          box(on && j < a.n2, a.rt * a.b2 * W::kSize,
+              [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &m2, bar, j * a.b2, e * a.dp + tile * a.rt); });
         }
       }
-      // after an abort copies may still be on their way into this CTA's shared memory
-      if (*abort_flag) {
-        for (int q = 0; q < (wrapped ? a.stages : st); ++q) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(smem_u32(&s.full[w][q]), q < st ? phase : phase ^ 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
-          }
+    }
+    // after an abort copies may still be on their way into this CTA's shared memory
+    if (on && *abort_flag) {
+      for (int q = 0; q < (wrapped ? a.stages : st); ++q) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(smem_u32(&s.full[w][q]), q < st ? phase : phase ^ 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
         }
       }
     }
@@ -592,19 +602,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++given;
     };
     const int pitch1 = a.b1 * W::kSize, blk1 = a.b1 / W::kBlock, blk2 = a.b2 / W::kBlock, blk2s = a.b2s / W::kBlock;
-    int nu_r = 0, ai = 0, r = r_first;  // routed units of this CTA; active expert and number of the next one
+    // ---- GEMM1
+    uint4 cur[kVals], nxt[kVals];  // token values of the present and the next box
+    bool ready = false;            // whether cur already holds the next box's
+    // row n of active expert i's tokens (i < 0: of all), from k on
+    auto x_row = [&](int i, int n_tok, int n, int k) -> const uint8_t* {
+      if (n >= n_tok) return nullptr;
+      return reinterpret_cast<const uint8_t*>(a.x) + ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
+    };
+    auto load_x = [&](uint4 (&v)[kVals], int i, int n_tok, int n, int k) {
+      const uint8_t* row = x_row(i, n_tok, n + g, k);
+      load_vals<W, 1>(v, row, 0, row != nullptr ? min(a.d - k, a.b1) : 0, lane);
+    };
+    int nu_r = 0, ai = -1, r = r_first;  // routed units of this CTA; active expert and number of the present one
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
-      const bool sh = ul < nu_s;
       if (ul == nu_s) {
         wait_routed();
         nu_r = routed_units(s.n_act);
         if (nu_r == 0) break;
-      }
-      if (!sh) {
-        if (ul > nu_s) r += G;
+        ai = r / a.upe;
+        ready = false;
+      } else if (ul > nu_s) {
+        r += G;
         while (r >= (ai + 1) * a.upe) ++ai;
       }
-      const int n_tok = sh ? a.T : s.cnt[ai];
+      const int n_tok = ai < 0 ? a.T : s.cnt[ai];
       float acc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -612,21 +634,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
       for (int j = warp; j < a.n1; j += kCompute) {
         const int k = j * a.b1;
+        if constexpr (kF32) {
+          arrived();
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt * 8 >= n_tok) break;
-          auto row = [&](int n) -> const uint8_t* {
-            n += nt * 8;
-            if (n >= n_tok) return nullptr;
-            return reinterpret_cast<const uint8_t*>(a.x) + ((size_t)(sh ? n : (int)s.tok[ai][n]) * a.d + k) * sizeof(X);
-          };
-          if constexpr (kF32) {
-            auto frow = [&](int n) { return reinterpret_cast<const float*>(row(n)); };
-            box_fma<false>(acc[nt], box(pitch1), 8 * pitch1, blk1, frow, a.d - k, lane, arrived);
-          } else {
-            const uint8_t* p = row(g);
-            box_mma<W, 1>(acc[nt], box(pitch1), 8 * pitch1, blk1, p, 0, p != nullptr ? a.d - k : 0, lane, arrived);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (nt * 8 >= n_tok) break;
+            auto row = [&](int n) { return reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)); };
+            box_fma<false>(acc[nt], box(pitch1), 8 * pitch1, blk1, row, a.d - k, lane);
           }
+        } else {
+          if (!ready) load_x(cur, ai, n_tok, 0, k);
+          ready = false;
+          if (j + kCompute < a.n1) {
+            load_x(nxt, ai, n_tok, 0, k + kCompute * a.b1);
+            ready = true;
+          } else if (ul + 1 < (ai < 0 ? nu_s : nu_s + nu_r)) {
+            int i = ai;
+            if (i >= 0)
+              while (r + G >= (i + 1) * a.upe) ++i;
+            load_x(nxt, i, i < 0 ? a.T : s.cnt[i], 0, warp * a.b1);
+            ready = true;
+          }
+          arrived();
+          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, cur);
+#pragma unroll
+          for (int nt = 1; nt < NT; ++nt) {
+            if (nt * 8 >= n_tok) break;
+            load_x(cur, ai, n_tok, nt * 8, k);
+            box_mma<W, 1>(acc[nt], box(pitch1), 8 * pitch1, blk1, cur);
+          }
+#pragma unroll
+          for (int i = 0; i < kVals; ++i) cur[i] = nxt[i];
         }
         release();
       }
@@ -638,68 +676,93 @@ __global__ void __launch_bounds__(kThreads, 1)
       hand_over();
     }
     // ---- GEMM2: a box's sums, for the tokens of its expert, join the warp's sums of all tokens in
-    // its part buffer (a lane's four values have places of their own)
+    // its part buffer (a lane's four values have places of their own).  Segment -1 of a tile is the
+    // shared expert's row, segment i active expert i's.
     const int n_act = s.n_act;
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
-    bool have_s = false, have_r = false;
+    bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
+    auto h_row = [&](int i, int n_tok, int n, int k) -> const uint8_t* {
+      if (n >= n_tok) return nullptr;
+      return i < 0 ? a.hs + ((size_t)n * a.hsp + k) * (kF32 ? 4 : 2) : a.h + ((size_t)s.asg[i][n] * a.hp + k) * (kF32 ? 4 : 2);
+    };
+    auto load_h = [&](uint4 (&v)[kVals], int i, int n, int k) {
+      const uint8_t* row = h_row(i, i < 0 ? a.T : s.cnt[i], n + g, k);
+      const int live = i < 0 ? min(a.k2s - k, a.b2s) : min(a.k2 - k, a.b2);
+      load_vals<W, 2>(v, row, i < 0 ? hs_lo : h_lo, row != nullptr ? live : 0, lane);
+    };
+    // this warp's first box at or behind (segment i, box j)
+    auto seek = [&](int& i, int& j) {
+      while (i < n_act && j >= (i < 0 ? a.n2s : a.n2)) {
+        ++i;
+        if (i < n_act) j = first_box(warp, s.act[i]);
+      }
+    };
     for (int tile = cta; tile < a.tiles; tile += G) {
       const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
       float* p = buffer();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       __syncwarp();
-      // segment -1: the shared expert; i: active expert i
-      for (int i = a.n2s ? -1 : 0; i < n_act; ++i) {
+      ready = false;
+      int i = -1, j = warp;
+      seek(i, j);
+      while (i < n_act) {
         const bool sh = i < 0;
-        const int e = sh ? 0 : s.act[i], kend = sh ? a.k2s : a.k2, bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize;
-        const int nb = sh ? a.n2s : a.n2, blk = sh ? blk2s : blk2;
+        if (sh ? !have_s : !have_r) {
+          if (lane == 0) {
+            if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
+            else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
+          }
+          __syncwarp();
+          if (sh) have_s = true; else have_r = true;
+        }
+        const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
         const int n_tok = sh ? a.T : s.cnt[i];
-        const uint8_t* hbase = sh ? a.hs : a.h;
-        const size_t lo = sh ? hs_lo : h_lo;
-        for (int j = sh ? warp : first_box(warp, e); j < nb; j += kCompute) {
-          const int k = j * bk;
-          if (sh ? !have_s : !have_r) {
-            // the intermediates come from every CTA's service warps
-            if (lane == 0) {
-              if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
-              else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
+        int ni = i, nj = j + kCompute;
+        seek(ni, nj);
+        float s0 = 1.0f, s1 = 1.0f;
+        if constexpr (W::kSize == 1) {
+          const float* sc = (sh ? a.ws2s : a.w2s + (size_t)s.act[i] * a.dp) + r0;
+          s0 = __ldg(sc + min(g, rows - 1));
+          s1 = __ldg(sc + min(g + 8, rows - 1));
+        }
+        auto join = [&](const float (&acc)[4], int n0) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int n = n0 + 2 * t4 + q;
+            if (n < n_tok) {
+              const int tk = sh ? n : (int)s.tok[i][n];
+              float* o = p + ((tk >> 3) * 32 + g * 4 + ((tk & 7) >> 1)) * 4 + (tk & 1);
+              o[0] = fmaf(acc[q], s0, o[0]);
+              o[2] = fmaf(acc[2 + q], s1, o[2]);
             }
-            __syncwarp();
-            if (sh) have_s = true; else have_r = true;
           }
-          float s0 = 1.0f, s1 = 1.0f;
-          if constexpr (W::kSize == 1) {
-            const float* sc = (sh ? a.ws2s : a.w2s + (size_t)e * a.dp) + r0;
-            s0 = __ldg(sc + min(g, rows - 1));
-            s1 = __ldg(sc + min(g + 8, rows - 1));
-          }
+        };
+        if constexpr (kF32) {
+          arrived();
           for (int n0 = 0; n0 < n_tok; n0 += 8) {
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            auto row = [&](int n) -> const uint8_t* {
-              n += n0;
-              if (n >= n_tok) return nullptr;
-              return hbase + ((size_t)(sh ? n : (int)s.asg[i][n]) * (sh ? a.hsp : a.hp) + k) * (kF32 ? 4 : 2);
-            };
-            if constexpr (kF32) {
-              auto frow = [&](int n) { return reinterpret_cast<const float*>(row(n)); };
-              box_fma<true>(acc, box(pitch), 8 * pitch, blk, frow, kend - k, lane, arrived);
-            } else {
-              const uint8_t* b = row(g);
-              box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, b, lo, b != nullptr ? kend - k : 0, lane, arrived);
-            }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int n = n0 + 2 * t4 + q;
-              if (n < n_tok) {
-                const int tk = sh ? n : (int)s.tok[i][n];
-                float* o = p + ((tk >> 3) * 32 + g * 4 + ((tk & 7) >> 1)) * 4 + (tk & 1);
-                o[0] = fmaf(acc[q], s0, o[0]);
-                o[2] = fmaf(acc[2 + q], s1, o[2]);
-              }
-            }
+            auto row = [&](int n) { return reinterpret_cast<const float*>(h_row(i, n_tok, n0 + n, k)); };
+            box_fma<true>(acc, box(pitch), 8 * pitch, blk, row, (sh ? a.k2s : a.k2) - k, lane);
+            join(acc, n0);
           }
-          release();
+        } else {
+          if (!ready) load_h(cur, i, 0, k);
+          ready = ni < n_act && (ni < 0 || have_r);
+          if (ready) load_h(nxt, ni, 0, nj * (ni < 0 ? a.b2s : a.b2));
+          arrived();
+          for (int n0 = 0; n0 < n_tok; n0 += 8) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (n0 > 0) load_h(cur, i, n0, k);
+            box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, cur);
+            join(acc, n0);
+          }
+#pragma unroll
+          for (int q = 0; q < kVals; ++q) cur[q] = nxt[q];
         }
+        release();
+        i = ni;
+        j = nj;
       }
       hand_over();
     }
@@ -718,9 +781,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) ctr_add(ctr, owed[which]);
       owed[which] = 0u;
     };
-    int seen = 0;
+    int seen = sw;  // units and tiles of the CTA in order, every second one
     auto wait_parts = [&]() {
-      mbar_wait(smem_u32(&s.part_full[seen % kParts]), (uint32_t)(seen / kParts) & 1u, abort_flag, a.err);
+      mbar_wait(smem_u32(&s.part_full[sw]), (uint32_t)(seen / kParts) & 1u, abort_flag, a.err);
     };
     // tile nt of the sums of the first n compute warps
     auto sum = [&](int n, int nt, float (&c)[4]) {
@@ -728,26 +791,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int w = 0; w < kCompute; ++w) {
         if (w >= n) break;
-        const float4 o = *reinterpret_cast<const float4*>(s.part[seen % kParts][w][nt][lane]);
+        const float4 o = *reinterpret_cast<const float4*>(s.part[sw][w][nt][lane]);
         c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
       }
     };
     auto free_parts = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[seen % kParts]));
-      ++seen;
+      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[sw]));
+      seen += kServices;
     };
-    int r = r_first, ai = 0, first = 0;  // number, active expert and that expert's first unit of the next routed unit
-    for (int un = 0; sw == 0 && un < n1; ++un) {
+    int ai = 0, first = 0;  // active expert of the next routed unit, and that expert's first one
+    for (; seen < n1;) {
+      const int un = seen;
       const bool sh = un < nu_s;
-      if (un == nu_s) announce(0, a.ctr + kCtrShared);
-      if (!sh) {
-        if (un > nu_s) r += G;
+      if (!sh) announce(0, a.ctr + kCtrShared);
+      const int r = r_first + (un - nu_s) * G;
+      if (!sh)
         while (r >= first + a.upe) {
           first += a.upe;
           ++ai;
         }
-      }
       const int u = sh ? cta + un * G : r - first, e = sh ? 0 : s.act[ai];
       const int n_tok = sh ? a.T : s.cnt[ai];
       // where this unit's sums go is looked up before they are there
@@ -799,7 +862,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     announce(0, a.ctr + kCtrShared);
     announce(1, a.ctr + kCtrRouted);
     // ---- the output's rows
-    for (int n = 0; sw == 0 && n < n2; ++n) {
+    while (seen < n1 + n2) {
+      const int n = seen - n1;
       const int r0 = (cta + n * G) * a.rt, rows = min(a.rt, a.d - r0);
       wait_parts();
       X* out = reinterpret_cast<X*>(a.out);
@@ -864,12 +928,13 @@ int make_map(CUtensorMap* m, const void* base, uint64_t n, int width, int box, i
 }
 
 // Bytes of a row of `bytes` in a box: the twelve warps take the boxes in turn, and a warp's time for one
-// is about that of 256 bytes for the tokens' values from L2 plus that of the box itself.  Tensor maps
-// take at most 256 values.
-template <typename W>
+// is about that of 256 bytes for the tokens' values from L2 plus that of the box itself.  At most the
+// blocks whose token values a lane holds; tensor maps take at most 256 values.
+template <typename W, int kTerms>
 int box_of(int bytes) {
+  const int most = W::kSize == 4 ? kMaxBox : min(kMaxBox, Layout<W, kTerms>::kBlocks * 64);
   int best = 64, cost = 1 << 30;
-  for (int b = 64; b <= kMaxBox && b <= 256 * W::kSize; b += 64) {
+  for (int b = 64; b <= most && b <= 256 * W::kSize; b += 64) {
     const int n = (bytes + b - 1) / b, c = (n + kCompute - 1) / kCompute * (b + 256);
     if (c < cost) {
       best = b;
@@ -888,13 +953,12 @@ int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
     return DSCA_ERR_CUDA;
   constexpr int kFixed = (int)((sizeof(Smem<NT>) + 127) / 128 * 128);
   static_assert((kSmem - kFixed) / (kCompute * 16 * kMaxBox) >= 2, "two boxes a ring");
-  auto boxes = [](int k, int* b, int* n) {
-    *b = box_of<W>(k * W::kSize) / W::kSize;
-    *n = (k + *b - 1) / *b;
-  };
-  boxes(a.d, &a.b1, &a.n1);
-  boxes(a.k2, &a.b2, &a.n2);
-  boxes(a.k2s, &a.b2s, &a.n2s);
+  a.b1 = box_of<W, 1>(a.d * W::kSize) / W::kSize;
+  a.b2 = box_of<W, 2>(a.k2 * W::kSize) / W::kSize;
+  a.b2s = box_of<W, 2>(a.k2s * W::kSize) / W::kSize;
+  a.n1 = (a.d + a.b1 - 1) / a.b1;
+  a.n2 = (a.k2 + a.b2 - 1) / a.b2;
+  a.n2s = (a.k2s + a.b2s - 1) / a.b2s;
   a.stage = 16 * max(a.b1, max(a.b2, a.n2s ? a.b2s : 0)) * W::kSize;
   a.stages = min(kMaxStages, (kSmem - kFixed) / (kCompute * a.stage));
   // output rows in tiles of at most 16, as even as they come over the SMs
