@@ -101,7 +101,7 @@ class QosArgs(ctypes.Structure):
 NORM_Q_NONE, NORM_Q_E4M3, NORM_Q_SPLIT = range(3)
 NORM_MAX_D = 32768
 FEW_TOKENS = 32
-FEW_COUNTER_BYTES = 256
+FEW_ZERO_BYTES = 1024
 _i64 = ctypes.c_int64
 
 

@@ -163,6 +163,8 @@ struct Smem {
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
   uint8_t act[DSCA_MAX_EXPERTS];            // experts with tokens ("active"), ascending
   uint8_t cnt[DSCA_MAX_EXPERTS];            // tokens of active expert i
+  uint32_t mask[DSCA_MAX_EXPERTS];          // and which
+  uint8_t turn[DSCA_MAX_EXPERTS];           // the compute warp that its first box of GEMM2 goes to
   uint8_t tok[DSCA_MAX_EXPERTS][8 * NT];    // its n-th token
   uint8_t asg[DSCA_MAX_EXPERTS][8 * NT];    // and that assignment: token * k + choice, the row of h
   uint8_t slot[DSCA_MAX_EXPERTS][8 * NT];   // choice of (expert, token)
@@ -290,28 +292,43 @@ __device__ __forceinline__ uint4 ld_b(const uint8_t* p, bool live, bool coherent
 // A lane's token values for a box of bf16 or e4m3 weights: vector (i, m, q) holds eight values of 64-byte
 // block i, term m (0: x or the high term, 1: the low term), part q.
 //   row: this lane's token row (token g) at the box's first k, lo: byte distance to its low terms,
-//   live: values of that row that are there (0: no such token).
+//   live: values of that row from there on.
 template <typename W, int kTerms>
 struct Layout {
   static constexpr int kPer = W::kBlock < 32 ? 1 : W::kBlock / 32;  // vectors of a block and term
   static constexpr int kBlocks = kVals / (kPer * kTerms);           // blocks of a box, at most
   static __device__ __forceinline__ int at(int i, int m, int q) { return (i * kTerms + m) * kPer + q; }
 };
+// full: all nkb blocks of the box lie inside the row (the same on all lanes); a lane without a token is
+// given some row whose values it may read.
 template <typename W, int kTerms>
-__device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row, size_t lo, int live, int lane) {
+__device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row, size_t lo, bool full, int nkb, int live, int lane) {
   using L = Layout<W, kTerms>;
   const int t8 = (lane & 3) * 8 * L::kPer;
   live -= t8;
   const uint8_t* p = row + t8 * 2;
   const uint8_t* pl = p + lo;
+  if (full) {
 #pragma unroll
-  for (int i = 0; i < L::kBlocks; ++i)
+    for (int i = 0; i < L::kBlocks; ++i) {
+      if (i >= nkb) break;
 #pragma unroll
-    for (int q = 0; q < L::kPer; ++q) {
-      const int k = i * W::kBlock + q * 8;
-      v[L::at(i, 0, q)] = ld_b(p + k * 2, k < live, kTerms == 2);
-      if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, k < live, true);
+      for (int q = 0; q < L::kPer; ++q) {
+        const int k = i * W::kBlock + q * 8;
+        v[L::at(i, 0, q)] = ld_b(p + k * 2, true, kTerms == 2);
+        if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, true, true);
+      }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < L::kBlocks; ++i)
+#pragma unroll
+      for (int q = 0; q < L::kPer; ++q) {
+        const int k = i * W::kBlock + q * 8;
+        v[L::at(i, 0, q)] = ld_b(p + k * 2, k < live, kTerms == 2);
+        if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, k < live, true);
+      }
+  }
 }
 // acc += 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box.  box: this lane's place in its
 // row g in shared memory, up: bytes from there to row g + 8.
@@ -421,7 +438,11 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
   for (int i = wi; i < s.n_act; i += nw) {
     const int e = s.act[i];
     const uint32_t m = s.emask[e];
-    if (lane == 0) s.cnt[i] = (uint8_t)__popc(m);
+    if (lane == 0) {
+      s.cnt[i] = (uint8_t)__popc(m);
+      s.mask[i] = m;
+      s.turn[i] = (uint8_t)(e * a.n2 % kCompute);
+    }
     if ((m >> lane) & 1u) {
       const int n = __popc(m & ((1u << lane) - 1u));
       s.tok[i][n] = (uint8_t)lane;
@@ -479,7 +500,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // warps would do in the time of the first stages.
   const bool all_route = a.ups == 0 || a.T > 4;
   const int route_warps = all_route ? kCompute + kServices : kServices;
-  auto first_box = [&](int w, int e) { return (w + kCompute - (e * a.n2) % kCompute) % kCompute; };
+  // warp w's first box of active expert i
+  auto first_box = [&](int w, int i) { return w - s.turn[i] + (w < s.turn[i] ? kCompute : 0); };
 
   if (warp >= kProducer && warp < kService) {
     // ================================================================ producers: one lane a ring
@@ -558,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &ms2, bar, j * a.b2s, tile * a.rt); });
       }
       for (int i = 0; i < n_act; ++i) {
-        const int e = s.act[i], fb = first_box(w, e);
+        const int e = s.act[i], fb = first_box(w, i);
         for (int j0 = 0; j0 < a.n2; j0 += kCompute) {
           const int j = j0 + fb;
           box(on && j < a.n2, a.rt * a.b2 * W::kSize,
@@ -603,16 +625,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     const int pitch1 = a.b1 * W::kSize, blk1 = a.b1 / W::kBlock, blk2 = a.b2 / W::kBlock, blk2s = a.b2s / W::kBlock;
     // ---- GEMM1
-    uint4 cur[kVals], nxt[kVals];  // token values of the present and the next box
-    bool ready = false;            // whether cur already holds the next box's
-    // row n of active expert i's tokens (i < 0: of all), from k on
-    auto x_row = [&](int i, int n_tok, int n, int k) -> const uint8_t* {
-      if (n >= n_tok) return nullptr;
+    uint4 va[kVals], vb[kVals];  // token values of the present and the next box, in turn
+    bool ready = false;          // whether the next box's are on their way
+    bool flip = false;           // and whether they are in vb
+    // row n of active expert i's tokens (i < 0: of all) from k on; one of them where there is no such token
+    auto x_row = [&](int i, int n_tok, int n, int k) {
+      n = n < n_tok ? n : 0;
       return reinterpret_cast<const uint8_t*>(a.x) + ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
     };
     auto load_x = [&](uint4 (&v)[kVals], int i, int n_tok, int n, int k) {
-      const uint8_t* row = x_row(i, n_tok, n + g, k);
-      load_vals<W, 1>(v, row, 0, row != nullptr ? min(a.d - k, a.b1) : 0, lane);
+      load_vals<W, 1>(v, x_row(i, n_tok, n + g, k), 0, k + a.b1 <= a.d, blk1, a.d - k, lane);
     };
     int nu_r = 0, ai = -1, r = r_first;  // routed units of this CTA; active expert and number of the present one
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
@@ -632,41 +654,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
-      for (int j = warp; j < a.n1; j += kCompute) {
+      // box j, whose token values are in v (or not yet asked for); the next box's go to w
+      auto step = [&](int j, uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const int k = j * a.b1;
         if constexpr (kF32) {
           arrived();
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             if (nt * 8 >= n_tok) break;
-            auto row = [&](int n) { return reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)); };
+            auto row = [&](int n) {
+              return nt * 8 + n < n_tok ? reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)) : nullptr;
+            };
             box_fma<false>(acc[nt], box(pitch1), 8 * pitch1, blk1, row, a.d - k, lane);
           }
         } else {
-          if (!ready) load_x(cur, ai, n_tok, 0, k);
+          if (!ready) load_x(v, ai, n_tok, 0, k);
           ready = false;
           if (j + kCompute < a.n1) {
-            load_x(nxt, ai, n_tok, 0, k + kCompute * a.b1);
+            load_x(w, ai, n_tok, 0, k + kCompute * a.b1);
             ready = true;
           } else if (ul + 1 < (ai < 0 ? nu_s : nu_s + nu_r)) {
             int i = ai;
             if (i >= 0)
               while (r + G >= (i + 1) * a.upe) ++i;
-            load_x(nxt, i, i < 0 ? a.T : s.cnt[i], 0, warp * a.b1);
+            load_x(w, i, i < 0 ? a.T : s.cnt[i], 0, warp * a.b1);
             ready = true;
           }
           arrived();
-          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, cur);
+          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, v);
 #pragma unroll
           for (int nt = 1; nt < NT; ++nt) {
             if (nt * 8 >= n_tok) break;
-            load_x(cur, ai, n_tok, nt * 8, k);
-            box_mma<W, 1>(acc[nt], box(pitch1), 8 * pitch1, blk1, cur);
+            load_x(v, ai, n_tok, nt * 8, k);
+            box_mma<W, 1>(acc[nt], box(pitch1), 8 * pitch1, blk1, v);
           }
-#pragma unroll
-          for (int i = 0; i < kVals; ++i) cur[i] = nxt[i];
         }
         release();
+      };
+      for (int j = warp; j < a.n1; j += kCompute) {
+        if (flip) step(j, vb, va);
+        else step(j, va, vb);
+        flip = !flip;
       }
       float* p = buffer();
 #pragma unroll
@@ -675,38 +703,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
       hand_over();
     }
-    // ---- GEMM2: a box's sums, for the tokens of its expert, join the warp's sums of all tokens in
-    // its part buffer (a lane's four values have places of their own).  Segment -1 of a tile is the
-    // shared expert's row, segment i active expert i's.
+    // ---- GEMM2: segment -1 of a tile is the shared expert's row, segment i active expert i's.  Up to
+    // eight tokens: the tensor core's columns are the tokens of the call (a token without this expert
+    // reads another one's row and its column is dropped), and the sums of all experts stay in
+    // registers.  More tokens, and fp32: the columns are the expert's own tokens, and a box's sums join the warp's sums of all tokens in its
+    // part buffer (a lane's four values have places of their own).
+    constexpr bool kDirect = NT == 1 && !kF32;
     const int n_act = s.n_act;
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
-    auto h_row = [&](int i, int n_tok, int n, int k) -> const uint8_t* {
-      if (n >= n_tok) return nullptr;
+    auto h_at = [&](int i, int n, int k) {
       return i < 0 ? a.hs + ((size_t)n * a.hsp + k) * (kF32 ? 4 : 2) : a.h + ((size_t)s.asg[i][n] * a.hp + k) * (kF32 ? 4 : 2);
     };
     auto load_h = [&](uint4 (&v)[kVals], int i, int n, int k) {
-      const uint8_t* row = h_row(i, i < 0 ? a.T : s.cnt[i], n + g, k);
-      const int live = i < 0 ? min(a.k2s - k, a.b2s) : min(a.k2 - k, a.b2);
-      load_vals<W, 2>(v, row, i < 0 ? hs_lo : h_lo, row != nullptr ? live : 0, lane);
+      const int kend = i < 0 ? a.k2s : a.k2, bk = i < 0 ? a.b2s : a.b2;
+      // token g's place among the expert's tokens
+      if constexpr (kDirect) n = i < 0 ? g : __popc(s.mask[i] & ((1u << g) - 1u));
+      else n += g;
+      const uint8_t* row = h_at(i, n < (i < 0 ? a.T : s.cnt[i]) ? n : 0, k);
+      load_vals<W, 2>(v, row, i < 0 ? hs_lo : h_lo, k + bk <= kend, i < 0 ? blk2s : blk2, kend - k, lane);
     };
     // this warp's first box at or behind (segment i, box j)
     auto seek = [&](int& i, int& j) {
       while (i < n_act && j >= (i < 0 ? a.n2s : a.n2)) {
         ++i;
-        if (i < n_act) j = first_box(warp, s.act[i]);
+        if (i < n_act) j = first_box(warp, i);
       }
     };
     for (int tile = cta; tile < a.tiles; tile += G) {
       const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
       float* p = buffer();
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (!kDirect) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      __syncwarp();
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        __syncwarp();
+      }
       ready = false;
       int i = -1, j = warp;
       seek(i, j);
-      while (i < n_act) {
+      auto step = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const bool sh = i < 0;
         if (sh ? !have_s : !have_r) {
           if (lane == 0) {
@@ -720,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n_tok = sh ? a.T : s.cnt[i];
         int ni = i, nj = j + kCompute;
         seek(ni, nj);
-        float s0 = 1.0f, s1 = 1.0f;
+        float s0 = 1.0f, s1 = 1.0f;  // fp8: every (expert, row) has its own scale
         if constexpr (W::kSize == 1) {
           const float* sc = (sh ? a.ws2s : a.w2s + (size_t)s.act[i] * a.dp) + r0;
           s0 = __ldg(sc + min(g, rows - 1));
@@ -742,28 +779,48 @@ __global__ void __launch_bounds__(kThreads, 1)
           arrived();
           for (int n0 = 0; n0 < n_tok; n0 += 8) {
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            auto row = [&](int n) { return reinterpret_cast<const float*>(h_row(i, n_tok, n0 + n, k)); };
+            auto row = [&](int n) { return n0 + n < n_tok ? reinterpret_cast<const float*>(h_at(i, n0 + n, k)) : nullptr; };
             box_fma<true>(acc, box(pitch), 8 * pitch, blk, row, (sh ? a.k2s : a.k2) - k, lane);
             join(acc, n0);
           }
         } else {
-          if (!ready) load_h(cur, i, 0, k);
+          if (!ready) load_h(v, i, 0, k);
           ready = ni < n_act && (ni < 0 || have_r);
-          if (ready) load_h(nxt, ni, 0, nj * (ni < 0 ? a.b2s : a.b2));
+          if (ready) load_h(w, ni, 0, nj * (ni < 0 ? a.b2s : a.b2));
           arrived();
-          for (int n0 = 0; n0 < n_tok; n0 += 8) {
+          if constexpr (kDirect) {
+            // a box's sums join by the same operations in both forms: a token's result does not depend
+            // on how many others there are
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (n0 > 0) load_h(cur, i, n0, k);
-            box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, cur);
-            join(acc, n0);
+            box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, v);
+            const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
+            if (m & 1u) {
+              sum[0] = fmaf(acc[0], s0, sum[0]);
+              sum[2] = fmaf(acc[2], s1, sum[2]);
+            }
+            if (m & 2u) {
+              sum[1] = fmaf(acc[1], s0, sum[1]);
+              sum[3] = fmaf(acc[3], s1, sum[3]);
+            }
+          } else {
+            for (int n0 = 0; n0 < n_tok; n0 += 8) {
+              float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              if (n0 > 0) load_h(v, i, n0, k);
+              box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, v);
+              join(acc, n0);
+            }
           }
-#pragma unroll
-          for (int q = 0; q < kVals; ++q) cur[q] = nxt[q];
         }
         release();
         i = ni;
         j = nj;
+      };
+      while (i < n_act) {
+        step(va, vb);
+        if (i >= n_act) break;
+        step(vb, va);
       }
+      if constexpr (kDirect) *reinterpret_cast<float4*>(p + lane * 4) = make_float4(sum[0], sum[1], sum[2], sum[3]);
       hand_over();
     }
   } else {
@@ -999,7 +1056,7 @@ int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream
 
 size_t few_workspace_bytes(int T, int k, int inter, int shared_inter) {
   const size_t hp = few::round_up(inter, 64), hsp = few::round_up(shared_inter, 64);
-  return DSCA_FEW_COUNTER_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4;
+  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4;
 }
 
 int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
@@ -1024,8 +1081,8 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.k2s = a.ups * unit;
   uint8_t* w = (uint8_t*)p->workspace;
   a.ctr = (uint32_t*)w;
-  a.lg = (float*)(w + DSCA_FEW_COUNTER_BYTES);
-  a.h = w + DSCA_FEW_COUNTER_BYTES + (size_t)a.T * few::kLgPitch * 4;
+  a.lg = (float*)(w + DSCA_FEW_ZERO_BYTES);
+  a.h = w + DSCA_FEW_ZERO_BYTES + (size_t)a.T * few::kLgPitch * 4;
   a.hs = a.h + (size_t)a.T * a.k * a.hp * 4;
   if (p->weights == DSCA_BF16) return few::launch_t<few::Bf16>(a, p, num_sms, stream);
   if (p->weights == DSCA_F32) return few::launch_t<few::F32>(a, p, num_sms, stream);

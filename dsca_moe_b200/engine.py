@@ -720,7 +720,7 @@ class MoEEngine:
         n = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.top_k, self.experts.inter, self.experts.s_inter)
         if torch.cuda.is_current_stream_capturing():
             ws = torch.empty(n, dtype=torch.uint8, device=self.device)
-            ws[:L.FEW_COUNTER_BYTES].zero_()
+            ws[:L.FEW_ZERO_BYTES].zero_()
             return ws
         key = torch.cuda.current_stream(self.device).cuda_stream
         ws = self._few_ws.get(key)

@@ -52,8 +52,8 @@ DSCA_API int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream);
 
 /* Tokens one dsca_moe_few call takes at most. */
 #define DSCA_FEW_TOKENS 32
-/* Bytes at the start of its workspace that hold the counters of its waits. */
-#define DSCA_FEW_COUNTER_BYTES 256
+/* Bytes at the start of its workspace that are zero between calls (counters). */
+#define DSCA_FEW_ZERO_BYTES 1024
 
 /*
  * The whole MoE block for a few tokens, one kernel: router, softmax, top-k, the chosen experts'
@@ -65,7 +65,7 @@ DSCA_API int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream);
  * Weights in the packing of dsca_ffn_args.  weights: DSCA_BF16 or DSCA_F32 (x, router and out in the
  * same type), or DSCA_F8E4M3 with the four scale arrays (x, router and out bf16).
  * d * (bytes of a weight) must be a multiple of 16 and every weight matrix 16-byte aligned.
- * workspace: dsca_few_workspace_bytes() bytes, 256-byte aligned, the first DSCA_FEW_COUNTER_BYTES zero
+ * workspace: dsca_few_workspace_bytes() bytes, 256-byte aligned, the first DSCA_FEW_ZERO_BYTES zero
  * before the first call; every call leaves them zero.  Calls that may overlap on the GPU must not
  * share a workspace.  After a call whose waits timed out (dsca_check_error on err) zero them again.
  * The kernel's CTAs wait for one another (bounded), so it is launched cooperatively, one CTA per SM.

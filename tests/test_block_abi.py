@@ -25,7 +25,7 @@ def test_symbols_and_constants(lib):
     for name in L.EXPORTED_BLOCK:
         assert hasattr(lib, name), name
     for c, v in (("DSCA_NORM_MAX_D", L.NORM_MAX_D), ("DSCA_FEW_TOKENS", L.FEW_TOKENS),
-                 ("DSCA_FEW_COUNTER_BYTES", L.FEW_COUNTER_BYTES)):
+                 ("DSCA_FEW_ZERO_BYTES", L.FEW_ZERO_BYTES)):
         assert int(re.search(rf"#define {c} (\d+)", src).group(1)) == v
     assert set(re.findall(r"\}\s*(dsca_[a-z0-9_]+)\s*;", src)) == set(STRUCTS)
 
@@ -134,7 +134,7 @@ def test_few_limits(lib):
     assert lib.dsca_moe_few(ctypes.byref(a), None) == L.OK
     assert lib.dsca_few_workspace_bytes(33, 4, 64, 0) == 0 and lib.dsca_few_workspace_bytes(4, 9, 64, 0) == 0
     n = lib.dsca_few_workspace_bytes(32, 4, 1408, 5632)
-    assert n >= 256 + 4 * 32 * (4 * 1408 + 5632) and n % 256 == 0
+    assert n >= 1024 + 4 * 32 * (4 * 1408 + 5632) and n % 256 == 0
 
 
 def test_norm_python_refusals(lib):
