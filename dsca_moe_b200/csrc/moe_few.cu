@@ -44,7 +44,7 @@ constexpr int kService = kProducer + kProducers;  // first of the service warps
 constexpr int kServices = 2;              // they run the router, then finish the units in turn
 constexpr int kThreads = (kService + kServices) * 32;
 constexpr int kMaxStages = 8;             // boxes of a compute warp's ring, at most
-constexpr int kMaxBox = 256;              // bytes of a weight row in a box, at most
+constexpr int kMaxBox = 384;              // bytes of a weight row in a box, at most
 constexpr int kVals = 8;                  // 16-byte vectors of token values that a lane holds for a box
 constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
 constexpr int kLgPitch = 64;              // logits scratch: E + 1 <= 64 per token
@@ -331,10 +331,16 @@ __device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row,
   }
 }
 // acc += 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box.  box: this lane's place in its
-// row g in shared memory, up: bytes from there to row g + 8.
+// row g in shared memory, up: bytes from there to row g + 8.  Four chains of products (a tensor-core
+// product waits some 30 clocks for the one whose sum it adds to), added at the end.
 template <typename W, int kTerms>
 __device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, int nkb, const uint4 (&v)[kVals]) {
   using L = Layout<W, kTerms>;
+  float c[4][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[q][i] = 0.0f;
 #pragma unroll
   for (int i = 0; i < L::kBlocks; ++i) {
     if (i >= nkb) break;
@@ -343,8 +349,9 @@ __device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, i
 #pragma unroll
       for (int m = 0; m < kTerms; ++m) {
         const uint4 b = v[L::at(i, m, 0)];
-        mma_bf16(acc, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
-        mma_bf16(acc, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+        const int q = kTerms == 1 ? (i & 1) * 2 : m * 2;
+        mma_bf16(c[q], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+        mma_bf16(c[q + 1], a0.z, a1.z, a0.w, a1.w, b.z, b.w);
       }
     } else {
       const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
@@ -356,11 +363,13 @@ __device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, i
 #pragma unroll
         for (int m = 0; m < kTerms; ++m) {
           const uint4 b = v[L::at(i, m, j / 2)];
-          mma_bf16(acc, p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
+          mma_bf16(c[kTerms == 1 ? j : m * 2 + (j & 1)], p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
         }
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += (c[0][i] + c[1][i]) + (c[2][i] + c[3][i]);
 }
 
 // The same for fp32 weights on the CUDA cores: lane (g, t) sums rows g and g + 8 over its k for all
@@ -628,14 +637,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint4 va[kVals], vb[kVals];  // token values of the present and the next box, in turn
     bool ready = false;          // whether the next box's are on their way
     bool flip = false;           // and whether they are in vb
+    // Up to eight tokens: the tensor core's columns are the tokens of the call.  A warp whose boxes of a
+    // row are one or two then multiplies the same values in every unit and keeps them.
+    constexpr bool kDirect = NT == 1 && !kF32;
+    const bool keep = kDirect && a.n1 <= 2 * kCompute;
     // row n of active expert i's tokens (i < 0: of all) from k on; one of them where there is no such token
     auto x_row = [&](int i, int n_tok, int n, int k) {
       n = n < n_tok ? n : 0;
       return reinterpret_cast<const uint8_t*>(a.x) + ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
     };
     auto load_x = [&](uint4 (&v)[kVals], int i, int n_tok, int n, int k) {
+      if constexpr (kDirect) {
+        i = -1;
+        n_tok = a.T;
+      }
       load_vals<W, 1>(v, x_row(i, n_tok, n + g, k), 0, k + a.b1 <= a.d, blk1, a.d - k, lane);
     };
+    if constexpr (kDirect) {
+      if (keep) {
+        if (warp < a.n1) load_x(va, -1, a.T, 0, warp * a.b1);
+        if (warp + kCompute < a.n1) load_x(vb, -1, a.T, 0, (warp + kCompute) * a.b1);
+      }
+    }
     int nu_r = 0, ai = -1, r = r_first;  // routed units of this CTA; active expert and number of the present one
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
       if (ul == nu_s) {
@@ -691,10 +714,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         release();
       };
-      for (int j = warp; j < a.n1; j += kCompute) {
-        if (flip) step(j, vb, va);
-        else step(j, va, vb);
-        flip = !flip;
+      if (keep) {
+        if (warp < a.n1) {
+          arrived();
+          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, va);
+          release();
+        }
+        if (warp + kCompute < a.n1) {
+          arrived();
+          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, vb);
+          release();
+        }
+      } else {
+        for (int j = warp; j < a.n1; j += kCompute) {
+          if (flip) step(j, vb, va);
+          else step(j, va, vb);
+          flip = !flip;
+        }
       }
       float* p = buffer();
 #pragma unroll
@@ -704,11 +740,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       hand_over();
     }
     // ---- GEMM2: segment -1 of a tile is the shared expert's row, segment i active expert i's.  Up to
-    // eight tokens: the tensor core's columns are the tokens of the call (a token without this expert
-    // reads another one's row and its column is dropped), and the sums of all experts stay in
-    // registers.  More tokens, and fp32: the columns are the expert's own tokens, and a box's sums join the warp's sums of all tokens in its
+    // eight tokens: the columns are the tokens of the call (one without this expert reads another one's
+    // row and its column is dropped), and the sums of all experts stay in registers.  More tokens, and fp32: the columns are the expert's own tokens, and a box's sums join the warp's sums of all tokens in its
     // part buffer (a lane's four values have places of their own).
-    constexpr bool kDirect = NT == 1 && !kF32;
     const int n_act = s.n_act;
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
@@ -826,6 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================================================ service
     const int sw = warp - kService;
+    constexpr bool kDirect = NT == 1 && !kF32;  // GEMM1's columns, as in the compute warps
     route<X, NT>(a, s, sw, route_warps, lane);
     wait_routed();
     const int n_act = s.n_act, n1 = nu_s + routed_units(n_act);
@@ -879,26 +914,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         s0 = __ldg(sc + r0);
         s1 = __ldg(sc + r1);
       }
-      wait_parts();
       // activation, routing weight, and the intermediate to where GEMM2 reads it
       uint8_t* base = sh ? a.hs : a.h;
       const size_t lo = sh ? hs_lo : h_lo;
-      for (int nt = 0; nt * 8 < n_tok; ++nt) {
+      const uint32_t mask = sh ? 0xffffffffu : s.mask[ai];
+      for (int nt = 0; nt * 8 < (kDirect ? a.T : n_tok); ++nt) {
+        float wt[2];
+        size_t at[2];
+        bool on[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          int n = nt * 8 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
+          on[i] = n < (kDirect ? a.T : n_tok);
+          if constexpr (kDirect) {
+            on[i] = on[i] && ((mask >> n) & 1u);
+            if (!sh) n = __popc(mask & ((1u << n) - 1u));
+          }
+          const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
+          wt[i] = sh ? s.sg[row] : s.wt[row];
+          at[i] = (size_t)row * (sh ? a.hsp : a.hp);
+        }
+        if (nt == 0) wait_parts();
         float c[4];
         sum(a.n1, nt, c);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int n = nt * 8 + 2 * t4 + i;
-          if (n >= n_tok) continue;
-          const float w = sh ? s.sg[n] : s.wt[s.asg[ai][n]];
-          const size_t at = sh ? (size_t)n * a.hsp : (size_t)s.asg[ai][n] * a.hp;
+          if (!on[i]) continue;
           auto put = [&](int ch, float val) {
             if constexpr (kF32) {
-              reinterpret_cast<float*>(base)[at + ch] = val;
+              reinterpret_cast<float*>(base)[at[i] + ch] = val;
             } else {
               const __nv_bfloat16 hi = __float2bfloat16_rn(val);
               const float rest = val - __bfloat162float(hi);
-              __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at + ch;
+              __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at[i] + ch;
               o[0] = hi;
               // an infinite or NaN value is the high term alone
               o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
@@ -906,10 +954,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           };
           const float c0 = c[i] * s0, c1 = c[2 + i] * s1;
           if (a.glu) {
-            put(8 * u + g, w * (c0 / (1.0f + expf(-c0)) * c1));
+            put(8 * u + g, wt[i] * (c0 / (1.0f + expf(-c0)) * c1));
           } else {
-            put(16 * u + g, w * fmaxf(c0, 0.0f));
-            put(16 * u + g + 8, w * fmaxf(c1, 0.0f));
+            put(16 * u + g, wt[i] * fmaxf(c0, 0.0f));
+            put(16 * u + g + 8, wt[i] * fmaxf(c1, 0.0f));
           }
         }
       }
