@@ -181,32 +181,38 @@ __device__ __forceinline__ float round_to<__nv_bfloat16>(double v) { return roun
 template <>
 __device__ __forceinline__ float round_to<float>(double v) { return (float)v; }
 
-// x . w over one warp in fp64, the same on every lane
-__device__ __forceinline__ double dot64(const __nv_bfloat16* x, const __nv_bfloat16* w, int d, int lane) {
-  double s[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int c = lane * 8; c < d; c += 256) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(x + c)), b = __ldg(reinterpret_cast<const uint4*>(w + c));
-    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+// x . w over one warp in fp64, the same on every lane.  Rows come from DRAM behind the stream of weights,
+// so eight vectors of each are asked for at once.
+__device__ __forceinline__ void dot_add(double (&s)[4], uint4 a, uint4 b, const __nv_bfloat16*) {
+  const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // products of two 8-bit significands are exact in fp32
-      s[i] += (double)(__uint_as_float(av[i] << 16) * __uint_as_float(bv[i] << 16));
-      s[i] += (double)(__uint_as_float(av[i] & 0xffff0000u) * __uint_as_float(bv[i] & 0xffff0000u));
-    }
+  for (int i = 0; i < 4; ++i) {
+    // products of two 8-bit significands are exact in fp32
+    s[i] += (double)(__uint_as_float(av[i] << 16) * __uint_as_float(bv[i] << 16));
+    s[i] += (double)(__uint_as_float(av[i] & 0xffff0000u) * __uint_as_float(bv[i] & 0xffff0000u));
   }
-  double r = (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
-  return r;
 }
-__device__ __forceinline__ double dot64(const float* x, const float* w, int d, int lane) {
+__device__ __forceinline__ void dot_add(double (&s)[4], uint4 a, uint4 b, const float*) {
+  s[0] = fma((double)__uint_as_float(a.x), (double)__uint_as_float(b.x), s[0]);
+  s[1] = fma((double)__uint_as_float(a.y), (double)__uint_as_float(b.y), s[1]);
+  s[2] = fma((double)__uint_as_float(a.z), (double)__uint_as_float(b.z), s[2]);
+  s[3] = fma((double)__uint_as_float(a.w), (double)__uint_as_float(b.w), s[3]);
+}
+template <typename X>
+__device__ __forceinline__ double dot64(const X* x, const X* w, int d, int lane) {
+  constexpr int kVec = 16 / sizeof(X), kAhead = 8;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   double s[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int c = lane * 4; c < d; c += 128) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(x + c)), b = __ldg(reinterpret_cast<const float4*>(w + c));
-    s[0] = fma((double)a.x, (double)b.x, s[0]);
-    s[1] = fma((double)a.y, (double)b.y, s[1]);
-    s[2] = fma((double)a.z, (double)b.z, s[2]);
-    s[3] = fma((double)a.w, (double)b.w, s[3]);
+  for (int c = lane * kVec; c < d; c += 32 * kVec * kAhead) {
+    uint4 a[kAhead], b[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = c + i * 32 * kVec;
+      a[i] = k < d ? __ldg(reinterpret_cast<const uint4*>(x + k)) : zero;
+      b[i] = k < d ? __ldg(reinterpret_cast<const uint4*>(w + k)) : zero;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) dot_add(s, a[i], b[i], x);
   }
   double r = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
