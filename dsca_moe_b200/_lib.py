@@ -215,3 +215,24 @@ def check(code: int, where: str):
 
 def call(name: str, *args):
     check(getattr(load(), name)(*args), name)
+
+
+_torch = None
+
+
+def call_on(device, name: str, *args):
+    """`name` on the current stream of torch device `device`, made the current one for the call."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+        load()
+    cuda, index = _torch.cuda, device.index
+    cur = cuda.current_device()
+    if index is None or index == cur:
+        rc = getattr(_LIB, name)(*args, _torch._C._cuda_getCurrentRawStream(cur))
+    else:
+        with cuda.device(index):
+            rc = getattr(_LIB, name)(*args, _torch._C._cuda_getCurrentRawStream(index))
+    if rc != OK:
+        raise DscaError(rc, name)

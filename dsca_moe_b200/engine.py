@@ -714,18 +714,17 @@ class MoEEngine:
         return None
 
     def _few_workspace(self):
-        """Scratch of dsca_moe_few: one per stream, because calls that may overlap must not share it.
-        A call that is being captured gets one of its own from the graph's memory, with its
-        counters zeroed by the graph."""
-        n = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.top_k, self.experts.inter, self.experts.s_inter)
+        """Scratch of dsca_moe_few (the current device is the engine's): one per stream, because calls
+        that may overlap must not share it.  A call that is being captured gets one of its own from the
+        graph's memory, with the part that must be zero zeroed by the graph."""
         if torch.cuda.is_current_stream_capturing():
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+            ws = torch.empty(self._few_bytes, dtype=torch.uint8, device=self.device)
             ws[:L.FEW_ZERO_BYTES].zero_()
             return ws
-        key = torch.cuda.current_stream(self.device).cuda_stream
+        key = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
         ws = self._few_ws.get(key)
         if ws is None:
-            ws = self._few_ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            ws = self._few_ws[key] = torch.zeros(self._few_bytes, dtype=torch.uint8, device=self.device)
         return ws
 
     def _few_struct(self):
@@ -742,6 +741,7 @@ class MoEEngine:
             a.w1_scale, a.w2_scale = _ptr(pe.w1_scale), _ptr(pe.w2_scale)
             a.ws1_scale, a.ws2_scale = _ptr(pe.ws1_scale), _ptr(pe.ws2_scale)
             a.err = _ptr(self.err)
+            self._few_bytes = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.top_k, pe.inter, pe.s_inter)
             self._few_args = a
         return L.FewArgs.from_buffer_copy(self._few_args)
 
@@ -750,31 +750,35 @@ class MoEEngine:
         engine's device -> fresh out [T, d], logits [T, E], topk_ids [T, k], topk_w [T, k] and
         expert_index [T], with forward()'s meaning.  One GPU, resident experts, any of the engine's
         weight types; ValueError otherwise.  Runs on the current stream; can be captured."""
+        w = self.router_weight
+        dev, k = w.device, self.top_k
         if x.dim() != 2 or x.shape[1] != self.d:
             raise ValueError(f"expected [T, {self.d}] input, got {tuple(x.shape)}")
-        if x.device != self.router_weight.device:
-            raise ValueError(f"x is on {x.device}, the engine on {self.router_weight.device}")
-        T, k, dev = x.shape[0], self.top_k, self.router_weight.device
+        if x.device != dev:
+            raise ValueError(f"x is on {x.device}, the engine on {dev}")
+        T = x.shape[0]
         why = self._few_unsupported(T)
         if why is not None:
             raise ValueError(f"forward_few: {why}")
-        x = x.to(dtype=self.dtype).contiguous()
+        if x.dtype != self.dtype or not x.is_contiguous():
+            x = x.to(dtype=self.dtype).contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-        r = dict(out=torch.empty(T, self.d, dtype=self.dtype, device=dev),
-                 logits=torch.empty(T, self.E, dtype=self.dtype, device=dev),
-                 topk_ids=torch.empty(T, k, dtype=torch.int32, device=dev),
-                 topk_w=torch.empty(T, k, dtype=torch.float32, device=dev),
-                 expert_index=torch.empty(T, dtype=torch.int64, device=dev))
+        r = dict(out=torch.empty_like(x), logits=x.new_empty((T, self.E)),
+                 topk_ids=x.new_empty((T, k), dtype=torch.int32), topk_w=x.new_empty((T, k), dtype=torch.float32),
+                 expert_index=x.new_empty(T, dtype=torch.int64))
         if T == 0:
             return r
-        with torch.cuda.device(dev):
+        a = self._few_struct()
+        if dev.index == torch.cuda.current_device():
             ws = self._few_workspace()
-            a = self._few_struct()
-            a.T, a.x, a.out, a.logits = T, x.data_ptr(), r["out"].data_ptr(), r["logits"].data_ptr()
-            a.topk_ids, a.topk_w = r["topk_ids"].data_ptr(), r["topk_w"].data_ptr()
-            a.expert_index, a.workspace, a.workspace_bytes = r["expert_index"].data_ptr(), ws.data_ptr(), ws.numel()
-            L.call("dsca_moe_few", ctypes.byref(a), _stream())
+        else:
+            with torch.cuda.device(dev):
+                ws = self._few_workspace()
+        a.T, a.x, a.out, a.logits = T, x.data_ptr(), r["out"].data_ptr(), r["logits"].data_ptr()
+        a.topk_ids, a.topk_w = r["topk_ids"].data_ptr(), r["topk_w"].data_ptr()
+        a.expert_index, a.workspace, a.workspace_bytes = r["expert_index"].data_ptr(), ws.data_ptr(), self._few_bytes
+        L.call_on(dev, "dsca_moe_few", ctypes.byref(a))
         return r
 
     def forward_normed(self, x: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6,

@@ -30,23 +30,22 @@ class RmsNormOutput(NamedTuple):
     scale: torch.Tensor | None
 
 
-def _rows(t: torch.Tensor, name: str):
-    """(t as rows, their stride in elements): the leading dimensions must lie one stride apart."""
-    d = t.shape[-1]
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    elif t.dim() > 2:
+def _stride(t: torch.Tensor, name: str, d: int) -> int:
+    """Distance of t's rows in elements: the leading dimensions must lie one stride apart."""
+    if t.is_contiguous():
+        return d
+    if t.dim() > 2:
         try:
             t = t.view(-1, d)
         except RuntimeError:
             raise ValueError(f"{name}: the rows of {tuple(t.shape)} with strides {t.stride()} are not evenly "
                              "spaced (call contiguous())") from None
-    if d > 1 and t.stride(1) != 1:
+    if d > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    ld = t.stride(0) if t.shape[0] > 1 else max(d, t.stride(0))
+    ld = t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else d
     if ld < d:
         raise ValueError(f"{name}: rows overlap (stride {ld}, width {d})")
-    return t, ld
+    return ld
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -60,18 +59,19 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     [rows, 2 * ceil(d / 128) * 128], the two-term rows of dsca_split_rows with scale = 1 / s, the token
     operand of the fp8-weight experts.  write_y=False leaves y out when only the 8-bit rows are
     wanted.  Runs on x's device, on its current stream."""
-    dt = _DTYPES.get(x.dtype)
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    dt, q_mode = _DTYPES.get(dtype), _QUANT.get(quant)
     if dt is None:
-        raise ValueError(f"unsupported dtype {x.dtype}")
-    if quant not in _QUANT:
+        raise ValueError(f"unsupported dtype {dtype}")
+    if q_mode is None:
         raise ValueError(f"quant must be None, 'e4m3' or 'split', not {quant!r}")
-    if not x.is_cuda:
+    if dev.type != "cuda":
         raise ValueError("x must be on a GPU")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"expected [..., d] rows, got {tuple(x.shape)}")
-    d = x.shape[-1]
-    if tuple(weight.shape) != (d,) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device \
-            or not weight.is_contiguous():
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"expected [..., d] rows, got {tuple(shape)}")
+    d = shape[-1]
+    w_dt = _DTYPES.get(weight.dtype)
+    if weight.dim() != 1 or weight.shape[0] != d or (w_dt != dt and w_dt != L.F32) or weight.device != dev or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous [{d}] tensor of x's type or float32 on x's device")
     if quant == "split" and (dt != L.BF16 or d % 8):
         raise ValueError("quant='split' takes bf16 rows with d % 8 == 0")
@@ -79,30 +79,27 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
         raise ValueError("write_y=False needs a quant")
     if d > L.NORM_MAX_D:
         raise ValueError(f"rows of {d} values exceed {L.NORM_MAX_D}")
-    a = L.RmsNormArgs()
-    xr, a.ld_x = _rows(x, "x")
-    rows = xr.shape[0]
-    a.x, a.weight, a.rows, a.d, a.dtype, a.eps = x.data_ptr(), weight.data_ptr(), rows, d, dt, eps
-    a.weight_dtype = _DTYPES[weight.dtype]
-    h = x
+    dense = x.is_contiguous()
+    ld = d if dense else _stride(x, "x", d)
+    rows = x.numel() // d
+    h, r_ptr, h_ptr, ld_r = x, None, None, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
             raise ValueError("residual must have x's shape, type and device")
-        _, a.ld_residual = _rows(residual, "residual")
-        a.residual = residual.data_ptr()
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        a.residual_out, a.ld_residual_out = h.data_ptr(), d
-    y = q = scale = None
+        ld_r = _stride(residual, "residual", d)
+        h = torch.empty_like(x) if dense else x.new_empty(shape)
+        r_ptr, h_ptr = residual.data_ptr(), h.data_ptr()
+    y = q = scale = y_ptr = q_ptr = s_ptr = None
     if write_y:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        a.y, a.ld_y = y.data_ptr(), d
+        y = torch.empty_like(x) if dense else x.new_empty(shape)
+        y_ptr = y.data_ptr()
     if quant is not None:
-        a.quant = _QUANT[quant]
         width = d if quant == "e4m3" else 2 * ((d + 127) // 128 * 128)
-        q = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-        a.q, a.scale = q.data_ptr(), scale.data_ptr()
+        q = x.new_empty((rows, width), dtype=torch.float8_e4m3fn)
+        scale = x.new_empty(rows, dtype=torch.float32)
+        q_ptr, s_ptr = q.data_ptr(), scale.data_ptr()
     if rows:
-        with torch.cuda.device(x.device):
-            L.call("dsca_rms_norm", ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        a = L.RmsNormArgs(x.data_ptr(), r_ptr, weight.data_ptr(), rows, d, dt, w_dt, ld, ld_r, d, d, eps, q_mode, y_ptr,
+                          h_ptr, q_ptr, s_ptr)
+        L.call_on(dev, "dsca_rms_norm", ctypes.byref(a))
     return RmsNormOutput(y, h, q, scale)
