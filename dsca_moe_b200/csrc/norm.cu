@@ -41,55 +41,97 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// Eight consecutive values as they lie in memory: h of a bf16 row takes half the registers of its
+// floats, and the loads of x, residual and weight are all on their way before the first is used.
 template <typename T>
-__device__ __forceinline__ float to_f(T v);
+struct Chunk;
 template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+struct Chunk<__nv_bfloat16> {
+  uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    u = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+};
 template <>
-__device__ __forceinline__ float to_f(float v) { return v; }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ float from_f(float v) { return v; }
+struct Chunk<float> {
+  float4 a, b;
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    reinterpret_cast<float4*>(p)[0] = a;
+    reinterpret_cast<float4*>(p)[1] = b;
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    a = make_float4(v[0], v[1], v[2], v[3]);
+    b = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
 
-// Eight consecutive values from a 16-byte aligned place.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+__device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float one(const float* p) { return *p; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+// Thread tid's chunk i of a row.  kVec (d % 8 == 0): eight consecutive values, loaded one by one where
+// the row is not aligned (a warp's eight loads cover the same lines, so all but the first find them
+// in L1).  Otherwise single values TPR apart, so that loads and stores stay coalesced at any width.
+template <bool kVec, int TPR>
+__device__ __forceinline__ int column(int i, int j, int tid) {
+  return kVec ? (i * TPR + tid) * 8 + j : (i * 8 + j) * TPR + tid;
+}
+template <typename T, bool kVec, int TPR>
+__device__ __forceinline__ void read(Chunk<T>& c, const T* row, bool aligned, int i, int tid, int d) {
+  if constexpr (kVec) {
+    const int k = column<true, TPR>(i, 0, tid);
+    if (k >= d) {
+      c.zero();
+      return;
+    }
+    if (aligned) {
+      c.load(row + k);
+      return;
+    }
   }
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int k = column<kVec, TPR>(i, j, tid);
+    v[j] = k < d ? one(row + k) : 0.0f;
+  }
+  c.set(v);
 }
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-// Eight consecutive values, one by one where they are not aligned (a warp's eight loads cover the
-// same lines, so all but the first find them in L1).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool aligned, float (&v)[8]) {
-  if (aligned) {
-    load8(p, v);
+template <typename T, bool kVec, int TPR>
+__device__ __forceinline__ void write(const Chunk<T>& c, T* row, int i, int tid, int d) {
+  if constexpr (kVec) {
+    const int k = column<true, TPR>(i, 0, tid);
+    if (k < d) c.store(row + k);
   } else {
+    float v[8];
+    c.get(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f<T>(p[j]);
+    for (int j = 0; j < 8; ++j) {
+      const int k = column<false, TPR>(i, j, tid);
+      if (k < d) put(row + k, v[j]);
+    }
   }
-}
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                    pack_bf16x2(v[6], v[7]));
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = pack8(v);
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
 // Sum / max over the TPR threads of a row, the same value on every thread; the order of the
@@ -112,126 +154,139 @@ __device__ __forceinline__ float row_reduce(float v, float* sm) {
   return v;
 }
 
-// VEC: d % 8 == 0 and every output row 16-byte aligned; thread i of a row holds chunks i, i + TPR, ...
-// of eight values.  Otherwise the thread holds single values TPR apart, so that loads and stores
-// stay coalesced at any width and alignment.
-template <typename T, bool VEC, int VPT, int TPR, int THREADS>
+template <typename T, bool kVec, int VPT, int TPR, int THREADS, int QUANT>
 __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
   __shared__ float sm[THREADS / 32];
   const int tid = threadIdx.x % TPR;
   const long long row = (long long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
   const bool live = row < a.rows;
+  const int d = live ? a.d : 0;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
+  // residual and weight in registers too, unless the row alone fills them (fp32, eight chunks)
+  constexpr bool kHold = VPT * sizeof(T) <= 16;
+  constexpr int kN = kHold ? VPT : 1;
+  const bool w_held = kHold && !a.w_f32;
   const T* res = a.res ? reinterpret_cast<const T*>(a.res) + row * a.ld_res : nullptr;
-  T* ho = a.h ? reinterpret_cast<T*>(a.h) + row * a.ld_h : nullptr;
-  float v[VPT][8];
+  const T* wt = reinterpret_cast<const T*>(a.w);
+  Chunk<T> h[VPT], w[kN];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(h[i], x, a.vx, i, tid, d);
+  auto add = [&](Chunk<T>& c, const Chunk<T>& r) {
+    float v[8], u[8];
+    c.get(v);
+    r.get(u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += u[j];
+    c.set(v);  // rounded: this is the stream
+  };
+  if (res != nullptr) {
+    Chunk<T> r[kN];
+    if constexpr (kHold) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(r[i], res, a.vres, i, tid, d);
+      if (w_held) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(w[i], wt, a.vw, i, tid, a.d);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if constexpr (!kHold) read<T, kVec, TPR>(r[0], res, a.vres, i, tid, d);
+      add(h[i], r[kHold ? i : 0]);
+    }
+  } else if (w_held) {
+    if constexpr (kHold) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(w[i], wt, a.vw, i, tid, a.d);
+    }
+  }
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if constexpr (VEC) {
-      const int c = (i * TPR + tid) * 8;
-      if (live && c < a.d) {
-        load8<T>(x + c, a.vx, v[i]);
-      } else {
+    float v[8];
+    h[i].get(v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = (i * 8 + j) * TPR + tid;
-        v[i][j] = live && c < a.d ? to_f<T>(x[c]) : 0.0f;
-      }
-    }
+    for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
   }
-  if (res != nullptr) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      if constexpr (VEC) {
-        const int c = (i * TPR + tid) * 8;
-        if (live && c < a.d) {
-          float r[8];
-          load8<T>(res + c, a.vres, r);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = to_f<T>(from_f<T>(v[i][j] + r[j]));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = (i * 8 + j) * TPR + tid;
-          if (live && c < a.d) v[i][j] = to_f<T>(from_f<T>(v[i][j] + to_f<T>(res[c])));
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
   ss = row_reduce<TPR, false>(ss, sm);
   // every thread of the row has read its inputs by now: the outputs may lie over them
   const float inv = __frsqrt_rn(__fdiv_rn(ss, (float)a.d) + a.eps);
-  T* y = a.y ? reinterpret_cast<T*>(a.y) + row * a.ld_y : nullptr;
+  // chunk i of the unrounded y
+  auto normed = [&](int i, float (&v)[8]) {
+    float f[8];
+    h[i].get(v);
+    if (w_held) {
+      w[kHold ? i : 0].get(f);
+    } else if (!a.w_f32) {
+      Chunk<T> c;
+      read<T, kVec, TPR>(c, wt, a.vw, i, tid, a.d);
+      c.get(f);
+    } else {
+      Chunk<float> c;
+      read<float, kVec, TPR>(c, reinterpret_cast<const float*>(a.w), a.vw, i, tid, a.d);
+      c.get(f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * f[j];
+  };
+  T* ho = a.h ? reinterpret_cast<T*>(a.h) + row * a.ld_h : nullptr;
+  T* yo = a.y ? reinterpret_cast<T*>(a.y) + row * a.ld_y : nullptr;
   float mx = 0.0f;
   uint32_t mbits = 0u;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if constexpr (VEC) {
-      const int c = (i * TPR + tid) * 8;
-      if (live && c < a.d) {
-        if (ho != nullptr) store8(ho + c, v[i]);
-        float w[8];
-        if (a.w_f32) load8<float>(reinterpret_cast<const float*>(a.w) + c, a.vw, w);
-        else load8<T>(reinterpret_cast<const T*>(a.w) + c, a.vw, w);
+    if (ho != nullptr) write<T, kVec, TPR>(h[i], ho, i, tid, d);
+    float v[8];
+    normed(i, v);
+    Chunk<T> y;
+    y.set(v);
+    if (yo != nullptr) write<T, kVec, TPR>(y, yo, i, tid, d);
+    if constexpr (QUANT == DSCA_NORM_Q_E4M3) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * w[j];
-        if (y != nullptr) store8(y + c, v[i]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = (i * 8 + j) * TPR + tid;
-        if (live && c < a.d) {
-          if (ho != nullptr) ho[c] = from_f<T>(v[i][j]);
-          const float w = a.w_f32 ? reinterpret_cast<const float*>(a.w)[c] : to_f<T>(reinterpret_cast<const T*>(a.w)[c]);
-          v[i][j] = v[i][j] * inv * w;
-          if (y != nullptr) y[c] = from_f<T>(v[i][j]);
-        }
-      }
+      for (int j = 0; j < 8; ++j) mx = max_nan(mx, fabsf(v[j]));
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      mx = max_nan(mx, fabsf(v[i][j]));
-      if constexpr (sizeof(T) == 2) mbits = max(mbits, (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v[i][j])) & 0x7fffu);
+    if constexpr (QUANT == DSCA_NORM_Q_SPLIT) {
+      const uint32_t q = __vmaxu2(__vmaxu2(y.u.x & 0x7fff7fffu, y.u.y & 0x7fff7fffu), __vmaxu2(y.u.z & 0x7fff7fffu, y.u.w & 0x7fff7fffu));
+      mbits = max(mbits, max(q & 0xffffu, q >> 16));
+      h[i] = y;  // the rounded row, which the two terms stand for
     }
   }
-  if (a.quant == DSCA_NORM_Q_NONE) return;
-  if (a.quant == DSCA_NORM_Q_E4M3) {
+  if constexpr (QUANT == DSCA_NORM_Q_E4M3) {
     mx = row_reduce<TPR, true>(mx, sm);
     const float s = (mx > 0.0f || mx != mx) ? __fdiv_rn(mx, 448.0f) : 1.0f;
     if (live && tid == 0) a.scale[row] = s;
+    // y / s as y times the rounded 1 / s, an fp32 rounding more than the quotient (a division an element
+    // took twice the kernel's time); rows so small that 1 / s leaves fp32's normal range do divide
+    const bool tiny = s < 1e-37f;
+    const float rs = tiny ? 0.0f : __frcp_rn(s);
     uint8_t* q = a.q + row * a.d;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if constexpr (VEC) {
-        const int c = (i * TPR + tid) * 8;
-        if (live && c < a.d) {
-          uint32_t b[4];
+      float v[8];
+      normed(i, v);
+      uint32_t b[4];
+      if (tiny) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = f8s::e4m3x2_rn(__fdiv_rn(v[i][2 * j], s), __fdiv_rn(v[i][2 * j + 1], s));
-          *reinterpret_cast<uint2*>(q + c) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
-        }
+        for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(v[j], s);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= rs;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = f8s::e4m3x2_rn(v[2 * j], v[2 * j + 1]);
+      if constexpr (kVec) {
+        const int k = column<true, TPR>(i, 0, tid);
+        if (k < d) *reinterpret_cast<uint2*>(q + k) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int c = (i * 8 + j) * TPR + tid;
-          if (live && c < a.d) q[c] = (uint8_t)f8s::e4m3x2_rn(__fdiv_rn(v[i][j], s), 0.0f);
+          const int k = column<false, TPR>(i, j, tid);
+          if (k < d) q[k] = (uint8_t)(b[j / 2] >> (8 * (j & 1)));
         }
       }
     }
-    return;
   }
-  if constexpr (VEC && sizeof(T) == 2) {
+  if constexpr (QUANT == DSCA_NORM_Q_SPLIT) {
     // bf16 bits without the sign order like integers, and are exact as fp32 integers
     mbits = (uint32_t)row_reduce<TPR, true>((float)mbits, sm);
     float s, is;
@@ -242,8 +297,8 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
     uint8_t* q = a.q + row * 2 * kp;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (i * TPR + tid) * 8;
-      if (c < a.d) f8s::store_split(q, nullptr, kp, c / 8, pack8(v[i]), s);
+      const int c = i * TPR + tid;
+      if (c * 8 < a.d) f8s::store_split(q, nullptr, kp, c, h[i].u, s);
     }
     for (int c = a.d + 8 * tid; c < kp; c += 8 * TPR) {
       *reinterpret_cast<uint2*>(q + c) = make_uint2(0u, 0u);
@@ -252,25 +307,41 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
   }
 }
 
-template <typename T, bool VEC, int VPT, int TPR>
+template <typename T, bool kVec, int VPT, int TPR, int QUANT>
 int launch(const Args& a, cudaStream_t stream) {
   constexpr int kThreads = TPR > 256 ? TPR : 256;
   constexpr int kRows = kThreads / TPR;
   const unsigned grid = (unsigned)(((long long)a.rows + kRows - 1) / kRows);
-  rms_norm_kernel<T, VEC, VPT, TPR, kThreads><<<grid, kThreads, 0, stream>>>(a);
+  rms_norm_kernel<T, kVec, VPT, TPR, kThreads, QUANT><<<grid, kThreads, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
-template <typename T, bool VEC>
+// A warp a row needs no barrier and keeps most rows in flight; with few rows, or rows wider than a
+// warp's registers (32 chunks of eight values a lane's eighth of bf16, half of that of fp32), a whole CTA
+// takes one.
+template <typename T, bool kVec, int QUANT>
 int dispatch(const Args& a, cudaStream_t stream) {
+  constexpr int kWide = 16 / sizeof(T);  // chunks a lane holds with residual and weight
   const int chunks = (a.d + 7) / 8;
-  if (chunks <= 32) return launch<T, VEC, 1, 32>(a, stream);
-  if (chunks <= 64) return launch<T, VEC, 2, 32>(a, stream);
-  if (chunks <= 128) return launch<T, VEC, 4, 32>(a, stream);
-  if (chunks <= 256) return launch<T, VEC, 8, 32>(a, stream);
-  if (chunks <= 1024) return launch<T, VEC, 4, 256>(a, stream);
-  if (chunks <= 2048) return launch<T, VEC, 8, 256>(a, stream);
-  return launch<T, VEC, 8, 512>(a, stream);
+  if (a.rows > 2 * current_device_sms() && chunks <= 32 * kWide) {
+    if (chunks <= 32) return launch<T, kVec, 1, 32, QUANT>(a, stream);
+    if (chunks <= 64) return launch<T, kVec, 2, 32, QUANT>(a, stream);
+    if (chunks <= 128) return launch<T, kVec, 4, 32, QUANT>(a, stream);
+    return launch<T, kVec, kWide, 32, QUANT>(a, stream);
+  }
+  if (chunks <= 256) return launch<T, kVec, 1, 256, QUANT>(a, stream);
+  if (chunks <= 512) return launch<T, kVec, 2, 256, QUANT>(a, stream);
+  if (chunks <= 1024) return launch<T, kVec, 4, 256, QUANT>(a, stream);
+  return launch<T, kVec, 8, 512, QUANT>(a, stream);
+}
+
+template <typename T>
+int run(const Args& a, bool vec, cudaStream_t stream) {
+  if (a.quant == DSCA_NORM_Q_E4M3)
+    return vec ? dispatch<T, true, DSCA_NORM_Q_E4M3>(a, stream) : dispatch<T, false, DSCA_NORM_Q_E4M3>(a, stream);
+  if constexpr (sizeof(T) == 2)
+    if (a.quant == DSCA_NORM_Q_SPLIT) return vec ? dispatch<T, true, DSCA_NORM_Q_SPLIT>(a, stream) : DSCA_ERR_BAD_ARG;
+  return vec ? dispatch<T, true, DSCA_NORM_Q_NONE>(a, stream) : dispatch<T, false, DSCA_NORM_Q_NONE>(a, stream);
 }
 
 }  // namespace norm
@@ -289,10 +360,7 @@ int launch_rms_norm(const dsca_rms_norm_args* p, cudaStream_t stream) {
   a.vres = ok(a.res, a.ld_res);
   a.vw = ok(a.w, 0);
   const bool vec = p->d % 8 == 0 && reinterpret_cast<uintptr_t>(p->q) % 8 == 0 && ok(a.y, a.ld_y) && ok(a.h, a.ld_h);
-  if (p->quant == DSCA_NORM_Q_SPLIT && !vec) return DSCA_ERR_BAD_ARG;
-  if (p->dtype == DSCA_BF16)
-    return vec ? norm::dispatch<__nv_bfloat16, true>(a, stream) : norm::dispatch<__nv_bfloat16, false>(a, stream);
-  return vec ? norm::dispatch<float, true>(a, stream) : norm::dispatch<float, false>(a, stream);
+  return p->dtype == DSCA_BF16 ? norm::run<__nv_bfloat16>(a, vec, stream) : norm::run<float>(a, vec, stream);
 }
 
 }  // namespace dsca
