@@ -97,26 +97,33 @@ template <bool kVec, int TPR>
 __device__ __forceinline__ int column(int i, int j, int tid) {
   return kVec ? (i * TPR + tid) * 8 + j : (i * 8 + j) * TPR + tid;
 }
-template <typename T, bool kVec, int TPR>
-__device__ __forceinline__ void read(Chunk<T>& c, const T* row, bool aligned, int i, int tid, int d) {
-  if constexpr (kVec) {
-    const int k = column<true, TPR>(i, 0, tid);
-    if (k >= d) {
-      c.zero();
-      return;
-    }
-    if (aligned) {
-      c.load(row + k);
-      return;
-    }
-  }
-  float v[8];
+// Reads chunks i0 .. i0 + N - 1 of a row: every load is issued before the first value is packed.
+template <typename T, bool kVec, int TPR, int N>
+__device__ __forceinline__ void read(Chunk<T> (&c)[N], const T* row, bool aligned, int i0, int tid, int d) {
+  if (kVec && aligned) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int k = column<kVec, TPR>(i, j, tid);
-    v[j] = k < d ? one(row + k) : 0.0f;
+    for (int i = 0; i < N; ++i) {
+      const int k = column<true, TPR>(i0 + i, 0, tid);
+      if (k < d) c[i].load(row + k);
+      else c[i].zero();
+    }
+    return;
   }
-  c.set(v);
+  T raw[N][8];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = column<kVec, TPR>(i0 + i, j, tid);
+      raw[i][j] = k < d ? row[k] : T(0.0f);
+    }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = one(&raw[i][j]);
+    c[i].set(v);
+  }
 }
 template <typename T, bool kVec, int TPR>
 __device__ __forceinline__ void write(const Chunk<T>& c, T* row, int i, int tid, int d) {
@@ -169,8 +176,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
   const T* res = a.res ? reinterpret_cast<const T*>(a.res) + row * a.ld_res : nullptr;
   const T* wt = reinterpret_cast<const T*>(a.w);
   Chunk<T> h[VPT], w[kN];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(h[i], x, a.vx, i, tid, d);
+  read<T, kVec, TPR>(h, x, a.vx, 0, tid, d);
   auto add = [&](Chunk<T>& c, const Chunk<T>& r) {
     float v[8], u[8];
     c.get(v);
@@ -182,23 +188,16 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
   if (res != nullptr) {
     Chunk<T> r[kN];
     if constexpr (kHold) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(r[i], res, a.vres, i, tid, d);
-      if (w_held) {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(w[i], wt, a.vw, i, tid, a.d);
-      }
+      read<T, kVec, TPR>(r, res, a.vres, 0, tid, d);
+      if (w_held) read<T, kVec, TPR>(w, wt, a.vw, 0, tid, a.d);
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if constexpr (!kHold) read<T, kVec, TPR>(r[0], res, a.vres, i, tid, d);
+      if constexpr (!kHold) read<T, kVec, TPR>(r, res, a.vres, i, tid, d);
       add(h[i], r[kHold ? i : 0]);
     }
   } else if (w_held) {
-    if constexpr (kHold) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) read<T, kVec, TPR>(w[i], wt, a.vw, i, tid, a.d);
-    }
+    if constexpr (kHold) read<T, kVec, TPR>(w, wt, a.vw, 0, tid, a.d);
   }
   float ss = 0.0f;
 #pragma unroll
@@ -218,13 +217,13 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
     if (w_held) {
       w[kHold ? i : 0].get(f);
     } else if (!a.w_f32) {
-      Chunk<T> c;
+      Chunk<T> c[1];
       read<T, kVec, TPR>(c, wt, a.vw, i, tid, a.d);
-      c.get(f);
+      c[0].get(f);
     } else {
-      Chunk<float> c;
+      Chunk<float> c[1];
       read<float, kVec, TPR>(c, reinterpret_cast<const float*>(a.w), a.vw, i, tid, a.d);
-      c.get(f);
+      c[0].get(f);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * f[j];
@@ -316,18 +315,23 @@ int launch(const Args& a, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
-// A warp a row needs no barrier and keeps most rows in flight; with few rows, or rows wider than a
-// warp's registers (32 chunks of eight values a lane's eighth of bf16, half of that of fp32), a whole CTA
-// takes one.
+// Threads a row: with many rows as few as hold it in two or three chunks each (fp32: one), so that a
+// row's reduction passes under the loads of the other rows on the SM; with few rows a whole CTA.
+// 4096 x 2048 bf16: 128 threads with 2 chunks 10.4 us, 256 with 1 11.1 us, a warp with 8 12.9 us.
 template <typename T, bool kVec, int QUANT>
 int dispatch(const Args& a, cudaStream_t stream) {
-  constexpr int kWide = 16 / sizeof(T);  // chunks a lane holds with residual and weight
   const int chunks = (a.d + 7) / 8;
-  if (a.rows > 2 * current_device_sms() && chunks <= 32 * kWide) {
+  if (a.rows > 2 * current_device_sms() && chunks <= 256) {
     if (chunks <= 32) return launch<T, kVec, 1, 32, QUANT>(a, stream);
-    if (chunks <= 64) return launch<T, kVec, 2, 32, QUANT>(a, stream);
-    if (chunks <= 128) return launch<T, kVec, 4, 32, QUANT>(a, stream);
-    return launch<T, kVec, kWide, 32, QUANT>(a, stream);
+    if constexpr (sizeof(T) == 2) {
+      if (chunks <= 64) return launch<T, kVec, 2, 32, QUANT>(a, stream);
+      if (chunks <= 96) return launch<T, kVec, 3, 32, QUANT>(a, stream);
+      if (chunks <= 128) return launch<T, kVec, 2, 64, QUANT>(a, stream);
+      return launch<T, kVec, 2, 128, QUANT>(a, stream);
+    } else {
+      if (chunks <= 64) return launch<T, kVec, 1, 64, QUANT>(a, stream);
+      if (chunks <= 128) return launch<T, kVec, 1, 128, QUANT>(a, stream);
+    }
   }
   if (chunks <= 256) return launch<T, kVec, 1, 256, QUANT>(a, stream);
   if (chunks <= 512) return launch<T, kVec, 2, 256, QUANT>(a, stream);
