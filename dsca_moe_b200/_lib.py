@@ -116,7 +116,7 @@ class FewArgs(ctypes.Structure):
                 ("weights", _i), ("mode", _i), ("norm_topk", _i), ("act", _i), ("inter", _i), ("n1p", _i), ("ip", _i),
                 ("dp", _i), ("shared_inter", _i), ("shared_n1p", _i), ("shared_ip", _i), ("w1", _vp), ("w2", _vp),
                 ("ws1", _vp), ("ws2", _vp), ("w1_scale", _vp), ("w2_scale", _vp), ("ws1_scale", _vp),
-                ("ws2_scale", _vp), ("out", _vp), ("logits", _vp), ("topk_ids", _vp), ("topk_w", _vp),
+                ("ws2_scale", _vp), ("w1_max", ctypes.c_float), ("out", _vp), ("logits", _vp), ("topk_ids", _vp), ("topk_w", _vp),
                 ("expert_index", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
 
 
@@ -191,7 +191,7 @@ def load():
     lib.dsca_exp_neg_eval.argtypes = [_vp, _vp, _i, _vp]
     lib.dsca_rms_norm.argtypes = [p(RmsNormArgs), _vp]
     lib.dsca_few_workspace_bytes.restype = ctypes.c_size_t
-    lib.dsca_few_workspace_bytes.argtypes = [_i, _i, _i, _i]
+    lib.dsca_few_workspace_bytes.argtypes = [_i, _i, _i, _i, _i]
     lib.dsca_moe_few.argtypes = [p(FewArgs), _vp]
     for name in EXPORTED + EXPORTED_BLOCK:
         getattr(lib, name).restype = getattr(lib, name).restype or _i

@@ -25,7 +25,7 @@ int launch_split_rows(const void* src, int ld, int rows, const int32_t* rows_dev
                       cudaStream_t stream);
 int launch_rms_norm(const dsca_rms_norm_args* a, cudaStream_t stream);
 int launch_moe_few(const dsca_few_args* a, int num_sms, cudaStream_t stream);
-size_t few_workspace_bytes(int T, int k, int inter, int shared_inter);
+size_t few_workspace_bytes(int T, int d, int k, int inter, int shared_inter);
 }  // namespace dsca
 
 namespace {
@@ -275,9 +275,9 @@ int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream) {
   return dsca::launch_rms_norm(a, reinterpret_cast<cudaStream_t>(stream));
 }
 
-size_t dsca_few_workspace_bytes(int T, int top_k, int inter, int shared_inter) {
-  if (T < 0 || T > DSCA_FEW_TOKENS || top_k <= 0 || top_k > DSCA_MAX_TOPK || inter <= 0 || shared_inter < 0) return 0;
-  return dsca::few_workspace_bytes(T, top_k, inter, shared_inter);
+size_t dsca_few_workspace_bytes(int T, int d, int top_k, int inter, int shared_inter) {
+  if (T < 0 || T > DSCA_FEW_TOKENS || d <= 0 || top_k <= 0 || top_k > DSCA_MAX_TOPK || inter <= 0 || shared_inter < 0) return 0;
+  return dsca::few_workspace_bytes(T, d, top_k, inter, shared_inter);
 }
 
 int dsca_moe_few(const dsca_few_args* a, dsca_stream_t stream) {
@@ -310,8 +310,9 @@ int dsca_moe_few(const dsca_few_args* a, dsca_stream_t stream) {
   if (fp8 && (a->w1_scale == nullptr || a->w2_scale == nullptr ||
               (shared && (a->ws1_scale == nullptr || a->ws2_scale == nullptr))))
     return DSCA_ERR_BAD_ARG;
+  if (fp8 && !(a->w1_max >= 0.0f && a->w1_max < 3.0e38f)) return DSCA_ERR_BAD_ARG;
   if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return DSCA_ERR_BAD_ARG;
-  if (a->workspace_bytes < dsca::few_workspace_bytes(a->T, k, a->inter, shared ? a->shared_inter : 0))
+  if (a->workspace_bytes < dsca::few_workspace_bytes(a->T, a->d, k, a->inter, shared ? a->shared_inter : 0))
     return DSCA_ERR_CAPACITY;
   int num_sms = 0, major = 0;
   int rc = device_info(&num_sms, &major);

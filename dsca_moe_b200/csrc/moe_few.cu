@@ -31,6 +31,15 @@
 //
 // The intermediate is kept as two bf16 terms (16 significant bits); everything is summed in fp32,
 // the router in fp64 (bf16 products are exact in fp32, so the logits round correctly).
+//
+// fp8 weights go through f16: e4m3 converts to it exactly with one instruction a pair (to bf16 it
+// takes four, which alone cost more than the weights' DRAM time).  A token row times a power of two
+// that takes its largest value to [2^14, 2^15) is exact in f16 down to 2^-29 of that value.  The
+// intermediate (two f16 terms) needs a scale before it is known: |h| <= B^2 (SwiGLU; B with ReLU), B =
+// max|w1| sum|x|, so 2^14 / B^2 rounded down to a power of two cannot overflow, and typical values, some
+// 2^20 below the bound, still lie 2^18 above the smallest f16.
+#include <math.h>
+
 #include "common.cuh"
 #include "dsca_b200_block.h"
 
@@ -64,12 +73,15 @@ struct Args {
   float* topk_w;
   int64_t* expert_index;
   float* lg;        // [T][64] logits as fp32 (rounded to the router's type), column E = shared gate
-  uint8_t* h;       // [T * k][hp] intermediate: bf16 high terms, then the low terms; or fp32
+  uint8_t* x16;     // fp8 weights, more than eight tokens: [T][d] token rows in f16
+  float* xmeta;     // and [T][2]: 1 / their scale, the largest power of two below sum|x|
+  uint8_t* h;       // [T * k][hp] intermediate: high terms, then the low terms; or fp32
   uint8_t* hs;      // [T][hsp] the shared expert's
   uint32_t* ctr;
   int32_t* err;
   int T, d, E, k, mode, norm_topk, glu;
   int n1p, ip, dp, s_ip;
+  int w1_exp;             // fp8: max|w1| < 2^w1_exp
   int hp, hsp;            // row pitch of h / hs in values
   int upe, ups;           // units (16 weight rows of GEMM1) per routed expert / of the shared expert
   int k2, k2s;            // values of a row of w2 / ws2 that are read
@@ -111,14 +123,50 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// four e4m3 values -> two bf16 pairs, exact
-__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t v, uint32_t& lo, uint32_t& hi) {
-  uint32_t a, b;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"((uint16_t)v));
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(v >> 16)));
-  const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a)), fb = __half22float2(*reinterpret_cast<__half2*>(&b));
-  lo = pack_bf16x2(fa.x, fa.y);
-  hi = pack_bf16x2(fb.x, fb.y);
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four e4m3 values -> two f16 pairs, exact
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)v));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(v >> 16)));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 2^e
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// Exponent of the scale that takes a row whose largest magnitude has these bf16 bits to [2^14, 2^15),
+// within what fp32 holds together with its inverse.
+__device__ __forceinline__ int x_scale_exp(uint32_t max_bits) { return 141 - max(15, min(254, (int)(max_bits >> 7))); }
+// The intermediate's scale (see the top): sum|x| < 2^(e + 1), max|w1| < 2^w.
+__device__ __forceinline__ int h_scale_exp(int e, int w, bool glu) {
+  const int b = e + 1 + w;
+  return max(-126, min(126, 14 - (glu ? 2 * b : b)));
+}
+// the exponent of a non-negative float
+__device__ __forceinline__ int exp_of(float v) { return (int)(__float_as_uint(v) >> 23) - 127; }
+// eight bf16 values times s -> f16
+__device__ __forceinline__ uint4 to_f16(uint4 u, float s) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = pack_f16x2(__uint_as_float(w[i] << 16) * s, __uint_as_float(w[i] & 0xffff0000u) * s);
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// the largest magnitude bits and the magnitudes' sum of eight bf16 values, joined to (m, l1)
+__device__ __forceinline__ void magnitudes(uint4 u, uint32_t& m, float& l1) {
+  const uint32_t w[4] = {u.x & 0x7fff7fffu, u.y & 0x7fff7fffu, u.z & 0x7fff7fffu, u.w & 0x7fff7fffu};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m = max(m, max(w[i] & 0xffffu, w[i] >> 16));
+    l1 += __uint_as_float(w[i] << 16) + __uint_as_float(w[i] & 0xffff0000u);
+  }
 }
 
 __device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
@@ -160,6 +208,9 @@ struct Smem {
   uint64_t routed;
   float wt[8 * NT * DSCA_MAX_TOPK];         // routing weights by assignment
   float sg[8 * NT];                         // shared-expert gate
+  float xinv[8 * NT], hscale[8 * NT];       // fp8: 1 / scale of a token's row, scale of its intermediate
+  uint32_t xmax[kCompute][8];               // fp8, up to eight tokens: a warp's share of a row
+  float xsum[kCompute][8];
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
   uint8_t act[DSCA_MAX_EXPERTS];            // experts with tokens ("active"), ascending
   uint8_t cnt[DSCA_MAX_EXPERTS];            // tokens of active expert i
@@ -235,6 +286,10 @@ __device__ __forceinline__ void select_token(const Args& a, Smem<NT>& s, int t, 
   const int E = a.E, e0 = lane, e1 = lane + 32;
   const float l0 = __ldcg(a.lg + t * kLgPitch + e0), l1 = __ldcg(a.lg + t * kLgPitch + e1);
   const bool v0 = e0 < E, v1 = e1 < E, first = blockIdx.x == 0;
+  if (a.x16 != nullptr && lane == 0) {
+    s.xinv[t] = __ldcg(a.xmeta + 2 * t);
+    s.hscale[t] = pow2(h_scale_exp(exp_of(__ldcg(a.xmeta + 2 * t + 1)), a.w1_exp, a.glu));
+  }
   if (a.w_gate != nullptr && (e0 == E || e1 == E)) s.sg[t] = 1.0f / (1.0f + expf(-(e0 == E ? l0 : l1)));
   if (first) {
     X* lo = reinterpret_cast<X*>(a.logits) + (size_t)t * E;
@@ -364,12 +419,12 @@ __device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, i
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t p0, p1, q0, q1;
-        e4m3x4_to_bf16(w0[j], p0, p1);
-        e4m3x4_to_bf16(w1[j], q0, q1);
+        e4m3x4_to_f16(w0[j], p0, p1);
+        e4m3x4_to_f16(w1[j], q0, q1);
 #pragma unroll
         for (int m = 0; m < kTerms; ++m) {
           const uint4 b = v[L::at(i, m, j / 2)];
-          mma_bf16(c[kTerms == 1 ? j : m * 2 + (j & 1)], p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
+          mma_f16(c[kTerms == 1 ? j : m * 2 + (j & 1)], p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
         }
       }
     }
@@ -432,6 +487,26 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
     const X* w = r < a.E ? reinterpret_cast<const X*>(a.w_router) + (size_t)r * a.d : reinterpret_cast<const X*>(a.w_gate);
     const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, lane);
     if (lane == 0) a.lg[t * kLgPitch + r] = round_to<X>(v);
+  }
+  // fp8 weights, more than eight tokens: CTA t writes token t's row in f16 (eight or less: the compute
+  // warps convert what they keep of it)
+  if (a.x16 != nullptr && cta < a.T && wi == nw - 1) {
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const X*>(a.x) + (size_t)cta * a.d);
+    uint4* dst = reinterpret_cast<uint4*>(a.x16) + (size_t)cta * (a.d / 8);
+    uint32_t m = 0u;
+    float l1 = 0.0f;
+#pragma unroll 4
+    for (int c = lane; c < a.d / 8; c += 32) magnitudes(__ldg(src + c), m, l1);
+    m = __reduce_max_sync(0xffffffffu, m);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+    const int e = x_scale_exp(m);
+#pragma unroll 4
+    for (int c = lane; c < a.d / 8; c += 32) dst[c] = to_f16(__ldg(src + c), pow2(e));
+    if (lane == 0) {
+      a.xmeta[2 * cta] = pow2(-e);
+      a.xmeta[2 * cta + 1] = l1;
+    }
   }
   group_sync(nw * 32);
   if (wi == 0 && lane == 0) {
@@ -640,17 +715,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     const int pitch1 = a.b1 * W::kSize, blk1 = a.b1 / W::kBlock, blk2 = a.b2 / W::kBlock, blk2s = a.b2s / W::kBlock;
     // ---- GEMM1
-    uint4 va[kVals], vb[kVals];  // token values of the present and the next box, in turn
-    bool ready = false;          // whether the next box's are on their way
-    bool flip = false;           // and whether they are in vb
+    constexpr bool kHalf = W::kSize == 1;  // fp8 weights: f16 products
     // Up to eight tokens: the tensor core's columns are the tokens of the call.  A warp whose boxes of a
     // row are one or two then multiplies the same values in every unit and keeps them.
     constexpr bool kDirect = NT == 1 && !kF32;
     const bool keep = kDirect && a.n1 <= 2 * kCompute;
+    uint4 va[kVals], vb[kVals];  // token values of the present and the next box, in turn
+    bool ready = false;          // whether the next box's are on their way
+    bool flip = false;           // and whether they are in vb
     // row n of active expert i's tokens (i < 0: of all) from k on; one of them where there is no such token
     auto x_row = [&](int i, int n_tok, int n, int k) {
       n = n < n_tok ? n : 0;
-      return reinterpret_cast<const uint8_t*>(a.x) + ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
+      return reinterpret_cast<const uint8_t*>(kHalf && !kDirect ? a.x16 : a.x) + ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
     };
     auto load_x = [&](uint4 (&v)[kVals], int i, int n_tok, int n, int k) {
       if constexpr (kDirect) {
@@ -663,6 +739,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (keep) {
         if (warp < a.n1) load_x(va, -1, a.T, 0, warp * a.b1);
         if (warp + kCompute < a.n1) load_x(vb, -1, a.T, 0, (warp + kCompute) * a.b1);
+      }
+    }
+    float xs = 1.0f;  // the scale of token g's row
+    auto halve = [&](uint4 (&v)[kVals]) {
+#pragma unroll
+      for (int i = 0; i < kVals; ++i) v[i] = to_f16(v[i], xs);
+    };
+    if constexpr (kDirect && kHalf) {
+      // largest magnitude and sum of the magnitudes of token g's row: this warp's boxes, then all warps'
+      uint32_t m = 0u;
+      float l1 = 0.0f;
+      for (int j = warp; j < a.n1; j += kCompute) {
+        auto join = [&](const uint4 (&v)[kVals]) {
+#pragma unroll
+          for (int i = 0; i < kVals; ++i)
+            if (i / 2 < blk1) magnitudes(v[i], m, l1);
+        };
+        if (keep) {
+          if (j == warp) join(va);
+          else join(vb);
+        } else {
+          uint4 v[kVals];
+          load_x(v, -1, a.T, 0, j * a.b1);
+          join(v);
+        }
+      }
+#pragma unroll
+      for (int off = 1; off <= 2; off <<= 1) {
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+      }
+      if (t4 == 0) {
+        s.xmax[warp][g] = m;
+        s.xsum[warp][g] = l1;
+      }
+      asm volatile("bar.sync 2, %0;" ::"r"(kCompute * 32) : "memory");
+      m = 0u;
+      l1 = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kCompute; ++w) {
+        m = max(m, s.xmax[w][g]);
+        l1 += s.xsum[w][g];
+      }
+      const int e = x_scale_exp(m);
+      xs = pow2(e);
+      if (warp == 0 && t4 == 0) {
+        s.xinv[g] = pow2(-e);
+        s.hscale[g] = pow2(h_scale_exp(exp_of(l1), a.w1_exp, a.glu));
+      }
+      if (keep) {
+        halve(va);
+        halve(vb);
       }
     }
     int nu_r = 0, ai = -1, r = r_first;  // routed units of this CTA; active expert and number of the present one
@@ -710,6 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ready = true;
           }
           arrived();
+          if constexpr (kDirect && kHalf) halve(v);
           box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, v);
 #pragma unroll
           for (int nt = 1; nt < NT; ++nt) {
@@ -866,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================================================ service
     const int sw = warp - kService;
-    constexpr bool kDirect = NT == 1 && !kF32;  // GEMM1's columns, as in the compute warps
+    constexpr bool kDirect = NT == 1 && !kF32, kHalf = W::kSize == 1;  // as in the compute warps
     route<X, NT>(a, s, sw, route_warps, lane);
     wait_routed();
     const int n_act = s.n_act, n1 = nu_s + routed_units(n_act);
@@ -925,9 +1054,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const size_t lo = sh ? hs_lo : h_lo;
       const uint32_t mask = sh ? 0xffffffffu : s.mask[ai];
       for (int nt = 0; nt * 8 < (kDirect ? a.T : n_tok); ++nt) {
-        float wt[2];
+        float wt[2], xi[2], hs[2];
         size_t at[2];
         bool on[2];
+        int tok[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           int n = nt * 8 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
@@ -938,6 +1068,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
           wt[i] = sh ? s.sg[row] : s.wt[row];
+          tok[i] = sh ? n : (on[i] ? (int)s.tok[ai][n] : 0);
           at[i] = (size_t)row * (sh ? a.hsp : a.hp);
         }
         if (nt == 0) wait_parts();
@@ -945,10 +1076,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum(a.n1, nt, c);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          xi[i] = kHalf ? s.xinv[tok[i]] : 1.0f;
+          hs[i] = kHalf ? s.hscale[tok[i]] : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           if (!on[i]) continue;
           auto put = [&](int ch, float val) {
             if constexpr (kF32) {
               reinterpret_cast<float*>(base)[at[i] + ch] = val;
+            } else if constexpr (kHalf) {
+              const __half hi = __float2half_rn(val);
+              __half* o = reinterpret_cast<__half*>(base) + at[i] + ch;
+              o[0] = hi;
+              const float rest = val - __half2float(hi);
+              o[lo] = __float2half_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
             } else {
               const __nv_bfloat16 hi = __float2bfloat16_rn(val);
               const float rest = val - __bfloat162float(hi);
@@ -958,12 +1100,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
             }
           };
-          const float c0 = c[i] * s0, c1 = c[2 + i] * s1;
+          const float c0 = c[i] * xi[i] * s0, c1 = c[2 + i] * xi[i] * s1, f = wt[i] * hs[i];
           if (a.glu) {
-            put(8 * u + g, wt[i] * (c0 / (1.0f + expf(-c0)) * c1));
+            // the scale joins one factor first: their product may leave fp32 where the scaled one does not
+            put(8 * u + g, c0 / (1.0f + expf(-c0)) * f * c1);
           } else {
-            put(16 * u + g, wt[i] * fmaxf(c0, 0.0f));
-            put(16 * u + g + 8, wt[i] * fmaxf(c1, 0.0f));
+            put(16 * u + g, f * fmaxf(c0, 0.0f));
+            put(16 * u + g + 8, f * fmaxf(c1, 0.0f));
           }
         }
       }
@@ -985,7 +1128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tk = nt * 8 + 2 * t4 + (i & 1), rr = g + (i >> 1) * 8;
-          if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(c[i]);
+          if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(kHalf ? c[i] / s.hscale[tk] : c[i]);
         }
       }
       free_parts();
@@ -1108,9 +1251,10 @@ int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream
 
 }  // namespace few
 
-size_t few_workspace_bytes(int T, int k, int inter, int shared_inter) {
+size_t few_workspace_bytes(int T, int d, int k, int inter, int shared_inter) {
   const size_t hp = few::round_up(inter, 64), hsp = few::round_up(shared_inter, 64);
-  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4;
+  const size_t x16 = T > 8 ? (size_t)T * (d * 2 + 8) : 0;  // fp8 weights
+  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4 + (x16 + 255) / 256 * 256;
 }
 
 int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
@@ -1138,6 +1282,15 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.lg = (float*)(w + DSCA_FEW_ZERO_BYTES);
   a.h = w + DSCA_FEW_ZERO_BYTES + (size_t)a.T * few::kLgPitch * 4;
   a.hs = a.h + (size_t)a.T * a.k * a.hp * 4;
+  if (p->weights == DSCA_F8E4M3) {
+    if (a.T > 8) {
+      a.x16 = a.hs + (size_t)a.T * a.hsp * 4;
+      a.xmeta = (float*)(a.x16 + (size_t)a.T * a.d * 2);
+    }
+    int e = 0;
+    frexpf(p->w1_max, &e);  // w1_max < 2^e
+    a.w1_exp = max(-200, min(200, e));
+  }
   if (p->weights == DSCA_BF16) return few::launch_t<few::Bf16>(a, p, num_sms, stream);
   if (p->weights == DSCA_F32) return few::launch_t<few::F32>(a, p, num_sms, stream);
   return few::launch_t<few::Fp8>(a, p, num_sms, stream);

@@ -110,7 +110,9 @@ def _few_args():
     dict(T=-1), dict(d=0), dict(d=60), dict(E=0), dict(top_k=0), dict(top_k=9), dict(E=1), dict(weights=3), dict(mode=2),
     dict(act=2), dict(inter=0), dict(inter=129), dict(n1p=255), dict(ip=256), dict(dp=32), dict(shared_inter=0),
     dict(shared_inter=129), dict(shared_ip=64), dict(ws1=None), dict(x=4104), dict(workspace=4112),
-    dict(weights=2), dict(weights=2, w1_scale=4096, w2_scale=4096), dict(weights=2, d=72)])
+    dict(weights=2), dict(weights=2, w1_scale=4096, w2_scale=4096),
+    dict(weights=2, w1_scale=4096, w2_scale=4096, ws1_scale=4096, ws2_scale=4096, w1_max=-1.0),
+    dict(weights=2, w1_scale=4096, w2_scale=4096, ws1_scale=4096, ws2_scale=4096, w1_max=float("inf")), dict(weights=2, d=72)])
 def test_few_bad_arguments(lib, change):
     from dsca_moe_b200 import _lib as L
 
@@ -132,8 +134,8 @@ def test_few_limits(lib):
     a = _few_args()
     a.T, a.x = 0, None
     assert lib.dsca_moe_few(ctypes.byref(a), None) == L.OK
-    assert lib.dsca_few_workspace_bytes(33, 4, 64, 0) == 0 and lib.dsca_few_workspace_bytes(4, 9, 64, 0) == 0
-    n = lib.dsca_few_workspace_bytes(32, 4, 1408, 5632)
+    assert lib.dsca_few_workspace_bytes(33, 64, 4, 64, 0) == 0 and lib.dsca_few_workspace_bytes(4, 64, 9, 64, 0) == 0
+    n = lib.dsca_few_workspace_bytes(32, 2048, 4, 1408, 5632)
     assert n >= 1024 + 4 * 32 * (4 * 1408 + 5632) and n % 256 == 0
 
 

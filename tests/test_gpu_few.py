@@ -159,31 +159,35 @@ def test_ties_take_the_lowest_ids(cuda):
         _check(_run(eng, x), x, w, eng.router_weight, gate, 4)
 
 
-@pytest.mark.parametrize("kind", ["bf16", "f32"])
-def test_bad_values_stay_in_their_row(cuda, kind):
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
+@pytest.mark.parametrize("T", [6, 18])
+def test_bad_values_stay_in_their_row(cuda, kind, T):
     eng, w, router, gate, n = _engine(cuda, 256, 12, 2, 100, 72, kind=kind, seed=5)
-    x = n(6, 256, std=1.0)
+    x = n(T, 256, std=1.0)
     want = _run(eng, x)["out"].clone()
     x[1, 3], x[4, 200] = float("nan"), float("inf")
     r = _run(eng, x)
-    keep = [0, 2, 3, 5]
+    keep = [0, 2, 3, 5] + list(range(6, T))
     assert torch.equal(r["out"][keep], want[keep])
     assert not torch.isfinite(r["out"][[1, 4]]).all(-1).any()
     assert ((r["topk_ids"] >= 0) & (r["topk_ids"] < 12)).all()
 
 
-def test_large_and_small_magnitudes(cuda):
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
+@pytest.mark.parametrize("T", [8, 24])
+def test_large_and_small_magnitudes(cuda, kind, T):
     """Rows from 2^-30 to 2^30: each is held to its own size."""
-    eng, w, router, gate, n = _engine(cuda, 256, 12, 2, 100, 72, seed=6)
-    x = n(8, 256, std=1.0) * torch.exp2(torch.arange(-30, 31, 8, device=cuda).float())[:8, None]
-    x = x.to(torch.bfloat16)
+    eng, w, router, gate, n = _engine(cuda, 256, 12, 2, 100, 72, kind=kind, seed=6)
+    x = n(T, 256, std=1.0) * torch.exp2(torch.arange(-30, 31, 8, device=cuda).float()).repeat(3)[:T, None]
+    x = x.to(eng.dtype)
     _check(_run(eng, x), x, w, router, gate, 2)
 
 
-def test_agrees_with_forward_and_is_repeatable(cuda):
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
+def test_agrees_with_forward_and_is_repeatable(cuda, kind):
     """The same routing as the block's other path where the logits are not on a rounding border, outputs
     within the bf16 tolerance of the block's other tests; bit-equal from call to call."""
-    eng, w, router, gate, n = _engine(cuda, 512, 60, 4, 384, 768, seed=7)
+    eng, w, router, gate, n = _engine(cuda, 512, 60, 4, 384, 768, kind=kind, seed=7)
     x = n(32, 512, std=1.0)
     a, b = _run(eng, x), eng.forward(x)
     same = (a["topk_ids"] == b["topk_ids"]).all(-1)
