@@ -21,7 +21,17 @@
 //    routing, so its weights are on their way while the router runs, and by the time a CTA needs
 //    the intermediates of another one they have mostly been published.
 //  - the routing weight is multiplied into the intermediate, so GEMM2 adds every expert's part into
-//    the same fp32 registers and a CTA owns its rows of the output: no atomics, no second pass.
+//    the same fp32 sums and a CTA owns its rows of the output.  Where that would leave a CTA few rows
+//    (a narrow model, or more than eight tokens, whose boxes are 32 rows high), several CTAs share a
+//    tile of rows, each with its share of every row's boxes, and the last one to finish adds their
+//    sums in order.
+//
+// A warp spends some 150 instructions on a box whatever its size, at one in eight clocks (three or four
+// warps a scheduler, each waiting for its own last result); this, not the products, is what keeps it
+// from DRAM speed.  So the boxes are as large as the shares allow; up to eight tokens, whose rows every
+// unit multiplies in full, x stays in registers through GEMM1 and the sums through GEMM2; with more,
+// an expert's few tokens are gathered for it, and units and tiles are 32 rows high where the rows are
+// short enough, so that 32 rows share one gathering.
 //
 // Lane layout: lane (g, t) = (lane / 4, lane % 4) reads 16 bytes of weight rows g and g + 8 at offset
 // 16 t of each 64-byte block, and the same positions of token g.  A dot product does not mind in
@@ -59,7 +69,7 @@ constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
 constexpr int kLgPitch = 64;              // logits scratch: E + 1 <= 64 per token
 
 // words of the counter block
-enum { kCtrLogits = 0, kCtrShared = 1, kCtrRouted = 2, kCtrExit = 3 };
+enum { kCtrLogits = 0, kCtrShared = 1, kCtrRouted = 2, kCtrExit = 3, kCtrTiles = 8 };
 
 struct Args {
   const void* x;
@@ -83,11 +93,12 @@ struct Args {
   int n1p, ip, dp, s_ip;
   int w1_exp;             // fp8: max|w1| < 2^w1_exp
   int hp, hsp;            // row pitch of h / hs in values
-  int upe, ups;           // units (16 weight rows of GEMM1) per routed expert / of the shared expert
+  int upe, ups;           // units (16 or 32 weight rows of GEMM1) per routed expert / of the shared expert
   int k2, k2s;            // values of a row of w2 / ws2 that are read
   int b1, b2, b2s;        // values of a row in a box: GEMM1, routed and shared GEMM2
   int n1, n2, n2s;        // boxes of a row
-  int rt, tiles;          // rows of a GEMM2 tile, tiles
+  int rt, tiles, splits;  // rows of a GEMM2 tile, tiles, CTAs that share one
+  float* partial;         // their sums: [tiles * splits][tokens in eights][kSub2][32][4]
   int stage, stages;      // bytes of a stage, stages of a warp's ring
 };
 
@@ -196,13 +207,28 @@ __device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n) {
 }
 
 // ---------------------------------------------------------------- shared memory
-// Sums of a unit wait for their service warp in one of kParts buffers, one for each service warp: all
-// compute warps take part in every unit, so a warp that has finished unit n knows the buffer's use before
-// unit n + kParts to be complete (a parity wait cannot look two phases ahead).
+// What a kernel for up to 8 NT tokens does.  SUB: 16-row tiles of a GEMM1 unit.
+template <typename W, int NT, int SUB>
+struct Form {
+  static constexpr bool kF32 = W::kSize == 4, kHalf = W::kSize == 1;
+  // the tensor core's columns are the tokens of the call (else the tokens of the expert at hand)
+  static constexpr bool kDirect = NT == 1 && !kF32;
+  static constexpr int kSub2 = kDirect || kF32 ? 1 : 2;  // 16-row tiles of a GEMM2 tile
+  // tiles of eight tokens that a unit's sums are handed over in at a time
+  static constexpr int kHand = SUB == 2 ? 1 : NT;
+};
+
+// Sums wait for their service warp in one of kParts buffers, one for each service warp: all compute warps
+// take part in every handing over, so a warp that has seen number n knows the buffer's use before
+// n + kParts to be complete (a parity wait cannot look two phases ahead).
 constexpr int kParts = kServices;
-template <int NT>
+template <typename W, int NT, int SUB>
 struct Smem {
-  float part[kParts][kCompute][NT][32][4];
+  using F = Form<W, NT, SUB>;
+  union {
+    float part[kParts][kCompute][F::kHand][SUB][32][4];
+    float sums[F::kDirect ? 1 : kCompute][NT][F::kSub2][32][4];  // GEMM2, all tokens (not kDirect)
+  };
   uint64_t full[kCompute][kMaxStages], empty[kCompute][kMaxStages];
   uint64_t part_full[kParts], part_empty[kParts];
   uint64_t routed;
@@ -220,6 +246,7 @@ struct Smem {
   uint8_t asg[DSCA_MAX_EXPERTS][8 * NT];    // and that assignment: token * k + choice, the row of h
   uint8_t slot[DSCA_MAX_EXPERTS][8 * NT];   // choice of (expert, token)
   int n_act;
+  uint32_t handed;                          // routed units' handings over, all CTAs'
   int abort;
 };
 
@@ -281,8 +308,8 @@ __device__ __forceinline__ float ord_val(uint32_t k) {
 
 // Softmax and selection of one token by one warp (lane holds experts lane and lane + 32), with the
 // arithmetic and the tie rule of dsca_router_topk.  Every CTA does it for itself; CTA 0 writes the results.
-template <typename X, int NT>
-__device__ __forceinline__ void select_token(const Args& a, Smem<NT>& s, int t, int lane) {
+template <typename X, typename S>
+__device__ __forceinline__ void select_token(const Args& a, S& s, int t, int lane) {
   const int E = a.E, e0 = lane, e1 = lane + 32;
   const float l0 = __ldcg(a.lg + t * kLgPitch + e0), l1 = __ldcg(a.lg + t * kLgPitch + e1);
   const bool v0 = e0 < E, v1 = e1 < E, first = blockIdx.x == 0;
@@ -391,46 +418,58 @@ __device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row,
       }
   }
 }
-// acc += 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box.  box: this lane's place in its
-// row g in shared memory, up: bytes from there to row g + 8.  Four chains of products (a tensor-core
-// product waits some 30 clocks for the one whose sum it adds to), added at the end.
-template <typename W, int kTerms>
-__device__ __forceinline__ void box_mma(float (&acc)[4], uint32_t box, int up, int nkb, const uint4 (&v)[kVals]) {
+// acc += SUB x 16 weight rows x 8 tokens over the nkb 64-byte blocks of a box.  box: this lane's place in
+// its row g of the first 16 in shared memory, up: bytes from there to row g + 8, sub: to the next 16
+// rows.  Four chains of products (a tensor-core product waits some 30 clocks for the one whose sum
+// it adds to), added at the end.
+template <typename W, int kTerms, int SUB>
+__device__ __forceinline__ void box_mma(float (&acc)[SUB][4], uint32_t box, int up, int sub, int nkb, const uint4 (&v)[kVals]) {
   using L = Layout<W, kTerms>;
-  float c[4][4];
+  constexpr int kCh = 4 / SUB;  // chains of a 16-row tile
+  float c[SUB][kCh][4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
+  for (int r = 0; r < SUB; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[q][i] = 0.0f;
+    for (int q = 0; q < kCh; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[r][q][i] = 0.0f;
 #pragma unroll
   for (int i = 0; i < L::kBlocks; ++i) {
     if (i >= nkb) break;
-    const uint4 a0 = lds128(box + i * 64), a1 = lds128(box + up + i * 64);
-    if constexpr (W::kBlock == 32) {
 #pragma unroll
-      for (int m = 0; m < kTerms; ++m) {
-        const uint4 b = v[L::at(i, m, 0)];
-        const int q = kTerms == 1 ? (i & 1) * 2 : m * 2;
-        mma_bf16(c[q], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
-        mma_bf16(c[q + 1], a0.z, a1.z, a0.w, a1.w, b.z, b.w);
-      }
-    } else {
-      const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t p0, p1, q0, q1;
-        e4m3x4_to_f16(w0[j], p0, p1);
-        e4m3x4_to_f16(w1[j], q0, q1);
+    for (int r = 0; r < SUB; ++r) {
+      const uint4 a0 = lds128(box + r * sub + i * 64), a1 = lds128(box + r * sub + up + i * 64);
+      if constexpr (W::kBlock == 32) {
 #pragma unroll
         for (int m = 0; m < kTerms; ++m) {
-          const uint4 b = v[L::at(i, m, j / 2)];
-          mma_f16(c[kTerms == 1 ? j : m * 2 + (j & 1)], p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
+          const uint4 b = v[L::at(i, m, 0)];
+          const int q = (kTerms == 1 ? (i & 1) * 2 : m * 2);
+          mma_bf16(c[r][q % kCh], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+          mma_bf16(c[r][(q + 1) % kCh], a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+        }
+      } else {
+        const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p0, p1, q0, q1;
+          e4m3x4_to_f16(w0[j], p0, p1);
+          e4m3x4_to_f16(w1[j], q0, q1);
+#pragma unroll
+          for (int m = 0; m < kTerms; ++m) {
+            const uint4 b = v[L::at(i, m, j / 2)];
+            mma_f16(c[r][(kTerms == 1 ? j : m * 2 + (j & 1)) % kCh], p0, q0, p1, q1, (j & 1) ? b.z : b.x, (j & 1) ? b.w : b.y);
+          }
         }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] += (c[0][i] + c[1][i]) + (c[2][i] + c[3][i]);
+  for (int r = 0; r < SUB; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kCh == 4) acc[r][i] += (c[r][0][i] + c[r][1][i]) + (c[r][2][i] + c[r][3][i]);
+      else acc[r][i] += c[r][0][i] + c[r][1][i];
+    }
 }
 
 // The same for fp32 weights on the CUDA cores: lane (g, t) sums rows g and g + 8 over its k for all
@@ -478,8 +517,8 @@ __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync
 
 // Router: fp64 dot products spread over the grid, then softmax, selection and the expert lists in every
 // CTA for itself.  Warp wi of the nw warps that take part (they share named barrier 1).
-template <typename X, int NT>
-__device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw, int lane) {
+template <typename X, int SUB, typename S>
+__device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
   const int R = a.E + (a.w_gate != nullptr ? 1 : 0), nd = a.T * R;
   for (int q = cta + wi * G; q < nd; q += nw * G) {
@@ -514,7 +553,7 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
     ctr_wait(a.ctr + kCtrLogits, (uint32_t)min(nd, G), &s.abort, a.err);
   }
   group_sync(nw * 32);
-  for (int t = wi; t < a.T; t += nw) select_token<X, NT>(a, s, t, lane);
+  for (int t = wi; t < a.T; t += nw) select_token<X>(a, s, t, lane);
   group_sync(nw * 32);
   if (wi == 0) {
     const uint32_t m0 = s.emask[lane], m1 = s.emask[lane + 32];
@@ -522,7 +561,14 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
     const uint32_t below = (1u << lane) - 1u;
     if (m0) s.act[__popc(b0 & below)] = (uint8_t)lane;
     if (m1) s.act[__popc(b0) + __popc(b1 & below)] = (uint8_t)(lane + 32);
-    if (lane == 0) s.n_act = __popc(b0) + __popc(b1);
+    // handings over of an expert's unit: one, or one for each eight of its tokens
+    const uint32_t h0 = m0 == 0u ? 0u : (SUB == 2 ? (__popc(m0) + 7u) / 8u : 1u);
+    const uint32_t h1 = m1 == 0u ? 0u : (SUB == 2 ? (__popc(m1) + 7u) / 8u : 1u);
+    const uint32_t handed = __reduce_add_sync(0xffffffffu, h0 + h1) * (uint32_t)a.upe;
+    if (lane == 0) {
+      s.n_act = __popc(b0) + __popc(b1);
+      s.handed = handed;
+    }
   }
   group_sync(nw * 32);
   for (int i = wi; i < s.n_act; i += nw) {
@@ -531,7 +577,7 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
     if (lane == 0) {
       s.cnt[i] = (uint8_t)__popc(m);
       s.mask[i] = m;
-      s.turn[i] = (uint8_t)(e * a.n2 % kCompute);
+      s.turn[i] = (uint8_t)(e * ((a.n2 + a.splits - 1) / a.splits) % kCompute);
     }
     if ((m >> lane) & 1u) {
       const int n = __popc(m & ((1u << lane) - 1u));
@@ -543,17 +589,21 @@ __device__ __forceinline__ void route(const Args& a, Smem<NT>& s, int wi, int nw
   if (wi == 0 && lane == 0) mbar_arrive(smem_u32(&s.routed));
 }
 
-template <typename W, int NT>
+template <typename W, int NT, int SUB>
 __global__ void __launch_bounds__(kThreads, 1)
     moe_few_kernel(const Args a, const __grid_constant__ CUtensorMap m1, const __grid_constant__ CUtensorMap m2,
                    const __grid_constant__ CUtensorMap ms1, const __grid_constant__ CUtensorMap ms2) {
   using X = typename W::X;
-  constexpr bool kF32 = W::kSize == 4;
+  using F = Form<W, NT, SUB>;
+  constexpr bool kF32 = F::kF32, kHalf = F::kHalf, kDirect = F::kDirect;
+  constexpr int kSub2 = F::kSub2, kHand = F::kHand;
+  static_assert(SUB == 1 || !kDirect, "units of 32 rows are for gathered tokens");
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  Smem<NT>& s = *reinterpret_cast<Smem<NT>*>(smem_raw);
+  using S = Smem<W, NT, SUB>;
+  S& s = *reinterpret_cast<S*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int G = gridDim.x, cta = blockIdx.x;
-  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)((sizeof(Smem<NT>) + 127) / 128 * 128);
+  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)((sizeof(S) + 127) / 128 * 128);
   volatile int* abort_flag = &s.abort;
 
   if (threadIdx.x < kCompute * kMaxStages) {
@@ -574,24 +624,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
 
   // ---- this CTA's work.  GEMM1: units cta, cta + G, ... of the shared expert, then of the routed
-  // experts (the first of them on the CTA behind the last shared unit's).  GEMM2: tiles cta, cta + G,
-  // ... of the output's rows, for each the shared expert's row and then the active experts'.  Box j of
-  // a row goes to compute warp j mod 12; in the routed GEMM2 j counts on from expert to expert (all
-  // experts, active or not: a token's sums do not depend on the other tokens of the call).
+  // experts (the first of them on the CTA behind the last shared unit's).  GEMM2: items cta, cta + G,
+  // ... : tile item / splits of the output's rows, and of each of its rows the boxes j with j mod splits =
+  // item mod splits, first the shared expert's row, then the active experts'.  In GEMM1 box j goes to
+  // compute warp j mod 12; in GEMM2 they count on from expert to expert (all experts, active or not: a
+  // token's sums do not depend on the other tokens of the call).
   const int nu_s = a.ups > cta ? (a.ups - cta + G - 1) / G : 0;
   const int r_first = (cta + G - a.ups % G) % G;
+  const int items = a.tiles * a.splits;
   auto routed_units = [&](int n_act) {
     const int units = n_act * a.upe;
     return units > r_first ? (units - r_first + G - 1) / G : 0;
   };
   auto wait_routed = [&]() { mbar_wait(smem_u32(&s.routed), 0u, abort_flag, a.err); };
+  // warp w's first box (of this item's) of active expert i
+  auto first_box = [&](int w, int i) { return w - s.turn[i] + (w < s.turn[i] ? kCompute : 0); };
   // The router runs on the service warps while the compute warps begin with the shared expert; on all
-  // of them where there is no shared expert to begin with, or where the tokens are more than three
-  // warps would do in the time of the first stages.
+  // of them where there is no shared expert to begin with, or where the tokens are more than two
+  // warps would do in the time of the first boxes.
   const bool all_route = a.ups == 0 || a.T > 4;
   const int route_warps = all_route ? kCompute + kServices : kServices;
-  // warp w's first box of active expert i
-  auto first_box = [&](int w, int i) { return w - s.turn[i] + (w < s.turn[i] ? kCompute : 0); };
 
   if (warp >= kProducer && warp < kService) {
     // ================================================================ producers: one lane a ring
@@ -604,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int st = 0, last = -1;  // next stage, stage before it
     uint32_t phase = 0u;    // parity of the next stage's copy
     bool shallow = true, wrapped = false, stop = false;
-    // Box j of this lane's row, if there is one: load(bar, dst) once its stage is free.
+    // A box for this lane's ring, if there is one: load(bar, dst) once its stage is free.
     auto box = [&](bool there, int bytes, auto load) {
       const uint32_t e = smem_u32(&s.empty[w][st]), f = smem_u32(&s.full[w][max(last, 0)]);
       // Until the routing is known, one box a ring in flight: the router's loads queue behind them in DRAM
@@ -656,23 +708,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       const CUtensorMap* m = sh ? &ms1 : &m1;
       for (int j0 = 0; j0 < a.n1; j0 += kCompute) {
         const int j = j0 + w;
-        box(on && j < a.n1, 16 * a.b1 * W::kSize, [&](uint32_t bar, uint32_t dst) {
-          if (a.glu) box_load_4d(dst, m, bar, j * a.b1, 8 * u % 128, 0, e * (a.n1p / 256) + 8 * u / 128);
-          else tma_load_2d(dst, m, bar, j * a.b1, e * a.n1p + 16 * u);
+        box(on && j < a.n1, 16 * SUB * a.b1 * W::kSize, [&](uint32_t bar, uint32_t dst) {
+          if (a.glu) box_load_4d(dst, m, bar, j * a.b1, 8 * SUB * u % 128, 0, e * (a.n1p / 256) + 8 * SUB * u / 128);
+          else tma_load_2d(dst, m, bar, j * a.b1, e * a.n1p + 16 * SUB * u);
         });
       }
     }
     const int n_act = s.n_act;
-    for (int tile = cta; tile < a.tiles; tile += G) {
-      for (int j0 = 0; j0 < a.n2s; j0 += kCompute) {
-        const int j = j0 + w;
+    for (int item = cta; item < items; item += G) {
+      const int tile = item / a.splits, split = item % a.splits, per = kCompute * a.splits;
+      for (int j0 = 0; j0 < a.n2s; j0 += per) {
+        const int j = j0 + w * a.splits + split;
         box(on && j < a.n2s, a.rt * a.b2s * W::kSize,
             [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &ms2, bar, j * a.b2s, tile * a.rt); });
       }
       for (int i = 0; i < n_act; ++i) {
         const int e = s.act[i], fb = first_box(w, i);
-        for (int j0 = 0; j0 < a.n2; j0 += kCompute) {
-          const int j = j0 + fb;
+        for (int j0 = 0; j0 < a.n2; j0 += per) {
+          const int j = j0 + fb * a.splits + split;
           box(on && j < a.n2, a.rt * a.b2 * W::kSize,
               [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &m2, bar, j * a.b2, e * a.dp + tile * a.rt); });
         }
@@ -688,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < kCompute) {
     // ================================================================ compute
-    if (all_route) route<X, NT>(a, s, kServices + warp, route_warps, lane);
+    if (all_route) route<X, SUB>(a, s, kServices + warp, route_warps, lane);
     const uint32_t base = ring + (uint32_t)(warp * a.stages * a.stage);
     int st = 0, given = 0;  // next stage, sums handed over
     uint32_t phase = 0u;    // parity of the next stage's copy
@@ -702,11 +755,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= 1u;
       }
     };
+    // until the sums handed over as number n have been read
+    auto wait_read = [&](int n) { mbar_wait(smem_u32(&s.part_empty[n % kParts]), (uint32_t)(n / kParts) & 1u, abort_flag, a.err); };
     // this warp's part of the next buffer, free to be written
     auto buffer = [&]() {
-      const int b = given % kParts;
-      if (given >= kParts) mbar_wait(smem_u32(&s.part_empty[b]), (uint32_t)(given / kParts - 1) & 1u, abort_flag, a.err);
-      return &s.part[b][warp][0][0][0];
+      if (given >= kParts) wait_read(given - kParts);
+      return &s.part[given % kParts][warp][0][0][0][0];
     };
     auto hand_over = [&]() {
       __syncwarp();
@@ -714,11 +768,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++given;
     };
     const int pitch1 = a.b1 * W::kSize, blk1 = a.b1 / W::kBlock, blk2 = a.b2 / W::kBlock, blk2s = a.b2s / W::kBlock;
+    // GEMM1: from weight row g of a 16-row tile to row g + 8, and to the next tile
+    const int up1 = (a.glu ? 8 * SUB : 8) * pitch1, sub1 = (a.glu ? 8 : 16) * pitch1;
+
     // ---- GEMM1
-    constexpr bool kHalf = W::kSize == 1;  // fp8 weights: f16 products
-    // Up to eight tokens: the tensor core's columns are the tokens of the call.  A warp whose boxes of a
-    // row are one or two then multiplies the same values in every unit and keeps them.
-    constexpr bool kDirect = NT == 1 && !kF32;
+    // With kDirect a warp whose boxes of a row are one or two multiplies the same values in every unit
+    // and keeps them.
     const bool keep = kDirect && a.n1 <= 2 * kCompute;
     uint4 va[kVals], vb[kVals];  // token values of the present and the next box, in turn
     bool ready = false;          // whether the next box's are on their way
@@ -726,7 +781,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // row n of active expert i's tokens (i < 0: of all) from k on; one of them where there is no such token
     auto x_row = [&](int i, int n_tok, int n, int k) {
       n = n < n_tok ? n : 0;
-      return reinterpret_cast<const uint8_t*>(kHalf && !kDirect ? a.x16 : a.x) + ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
+      return reinterpret_cast<const uint8_t*>(kHalf && !kDirect ? a.x16 : a.x) +
+             ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
     };
     auto load_x = [&](uint4 (&v)[kVals], int i, int n_tok, int n, int k) {
       if constexpr (kDirect) {
@@ -806,78 +862,120 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (r >= (ai + 1) * a.upe) ++ai;
       }
       const int n_tok = ai < 0 ? a.T : s.cnt[ai];
-      float acc[NT][4];
+      // asks for the values of the next unit's first box of this warp, if that unit is known
+      auto ahead = [&](uint4 (&w)[kVals]) {
+        if (ul + 1 < (ai < 0 ? nu_s : nu_s + nu_r)) {
+          int i = ai;
+          if (i >= 0)
+            while (r + G >= (i + 1) * a.upe) ++i;
+          load_x(w, i, i < 0 ? a.T : s.cnt[i], 0, warp * a.b1);
+          ready = true;
+        }
+      };
+      if constexpr (SUB == 2) {
+        // one box a warp and unit; the expert's tokens eight at a time
+        auto unit = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
+          const bool has = warp < a.n1;
+          for (int n0 = 0; n0 < n_tok; n0 += 8) {
+            float acc[SUB][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+            for (int q = 0; q < SUB; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.0f;
-      // box j, whose token values are in v (or not yet asked for); the next box's go to w
-      auto step = [&](int j, uint4 (&v)[kVals], uint4 (&w)[kVals]) {
-        const int k = j * a.b1;
-        if constexpr (kF32) {
-          arrived();
+              for (int i = 0; i < 4; ++i) acc[q][i] = 0.0f;
+            if (has) {
+              if (n0 > 0 || !ready) load_x(v, ai, n_tok, n0, warp * a.b1);
+              if (n0 == 0) {
+                ready = false;
+                ahead(w);
+                arrived();
+              }
+              box_mma<W, 1, SUB>(acc, box(pitch1), up1, sub1, blk1, v);
+              if (n0 + 8 >= n_tok) release();
+            }
+            float* p = buffer();
+            if (has) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (nt * 8 >= n_tok) break;
-            auto row = [&](int n) {
-              return nt * 8 + n < n_tok ? reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)) : nullptr;
-            };
-            box_fma<false>(acc[nt], box(pitch1), 8 * pitch1, blk1, row, a.d - k, lane);
+              for (int q = 0; q < SUB; ++q)
+                *reinterpret_cast<float4*>(p + (q * 32 + lane) * 4) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+            }
+            hand_over();
+          }
+        };
+        if (flip) unit(vb, va);
+        else unit(va, vb);
+        flip = !flip;
+      } else {
+        float acc[NT][1][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[nt][0][i] = 0.0f;
+        // box j, whose token values are in v (or not yet asked for); the next box's go to w
+        auto step = [&](int j, uint4 (&v)[kVals], uint4 (&w)[kVals]) {
+          const int k = j * a.b1;
+          if constexpr (kF32) {
+            arrived();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (nt * 8 >= n_tok) break;
+              auto row = [&](int n) {
+                return nt * 8 + n < n_tok ? reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)) : nullptr;
+              };
+              box_fma<false>(acc[nt][0], box(pitch1), up1, blk1, row, a.d - k, lane);
+            }
+          } else {
+            if (!ready) load_x(v, ai, n_tok, 0, k);
+            ready = false;
+            if (j + kCompute < a.n1) {
+              load_x(w, ai, n_tok, 0, k + kCompute * a.b1);
+              ready = true;
+            } else {
+              ahead(w);
+            }
+            arrived();
+            if constexpr (kDirect && kHalf) halve(v);
+            box_mma<W, 1, 1>(acc[0], box(pitch1), up1, 0, blk1, v);
+#pragma unroll
+            for (int nt = 1; nt < NT; ++nt) {
+              if (nt * 8 >= n_tok) break;
+              load_x(v, ai, n_tok, nt * 8, k);
+              box_mma<W, 1, 1>(acc[nt], box(pitch1), up1, 0, blk1, v);
+            }
+          }
+          release();
+        };
+        if (keep) {
+          if (warp < a.n1) {
+            arrived();
+            box_mma<W, 1, 1>(acc[0], box(pitch1), up1, 0, blk1, va);
+            release();
+          }
+          if (warp + kCompute < a.n1) {
+            arrived();
+            box_mma<W, 1, 1>(acc[0], box(pitch1), up1, 0, blk1, vb);
+            release();
           }
         } else {
-          if (!ready) load_x(v, ai, n_tok, 0, k);
-          ready = false;
-          if (j + kCompute < a.n1) {
-            load_x(w, ai, n_tok, 0, k + kCompute * a.b1);
-            ready = true;
-          } else if (ul + 1 < (ai < 0 ? nu_s : nu_s + nu_r)) {
-            int i = ai;
-            if (i >= 0)
-              while (r + G >= (i + 1) * a.upe) ++i;
-            load_x(w, i, i < 0 ? a.T : s.cnt[i], 0, warp * a.b1);
-            ready = true;
+          for (int j = warp; j < a.n1; j += kCompute) {
+            if (flip) step(j, vb, va);
+            else step(j, va, vb);
+            flip = !flip;
           }
-          arrived();
-          if constexpr (kDirect && kHalf) halve(v);
-          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, v);
+        }
+        float* p = buffer();
 #pragma unroll
-          for (int nt = 1; nt < NT; ++nt) {
-            if (nt * 8 >= n_tok) break;
-            load_x(v, ai, n_tok, nt * 8, k);
-            box_mma<W, 1>(acc[nt], box(pitch1), 8 * pitch1, blk1, v);
-          }
-        }
-        release();
-      };
-      if (keep) {
-        if (warp < a.n1) {
-          arrived();
-          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, va);
-          release();
-        }
-        if (warp + kCompute < a.n1) {
-          arrived();
-          box_mma<W, 1>(acc[0], box(pitch1), 8 * pitch1, blk1, vb);
-          release();
-        }
-      } else {
-        for (int j = warp; j < a.n1; j += kCompute) {
-          if (flip) step(j, vb, va);
-          else step(j, va, vb);
-          flip = !flip;
-        }
+        for (int nt = 0; nt < NT; ++nt)
+          if ((kDirect || nt * 8 < n_tok) && warp < a.n1)
+            *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) =
+                make_float4(acc[nt][0][0], acc[nt][0][1], acc[nt][0][2], acc[nt][0][3]);
+        hand_over();
       }
-      float* p = buffer();
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        if (nt * 8 < n_tok && warp < a.n1)
-          *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-      hand_over();
     }
-    // ---- GEMM2: segment -1 of a tile is the shared expert's row, segment i active expert i's.  Up to
-    // eight tokens: the columns are the tokens of the call (one without this expert reads another one's
-    // row and its column is dropped), and the sums of all experts stay in registers.  More tokens, and fp32: the columns are the expert's own tokens, and a box's sums join the warp's sums of all tokens in its
-    // part buffer (a lane's four values have places of their own).
+
+    // ---- GEMM2: segment -1 of an item is the shared expert's row, segment i active expert i's.  With
+    // kDirect a token without the expert reads another one's row and its column is dropped, and the sums
+    // of all experts stay in registers.  Else the columns are the expert's own tokens, and a box's sums
+    // join the warp's sums of all tokens in shared memory (a lane's values have places of their own).
     const int n_act = s.n_act;
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
@@ -892,64 +990,77 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint8_t* row = h_at(i, n < (i < 0 ? a.T : s.cnt[i]) ? n : 0, k);
       load_vals<W, 2>(v, row, i < 0 ? hs_lo : h_lo, k + bk <= kend, i < 0 ? blk2s : blk2, kend - k, lane);
     };
-    // this warp's first box at or behind (segment i, box j)
-    auto seek = [&](int& i, int& j) {
-      while (i < n_act && j >= (i < 0 ? a.n2s : a.n2)) {
-        ++i;
-        if (i < n_act) j = first_box(warp, i);
-      }
-    };
-    for (int tile = cta; tile < a.tiles; tile += G) {
+    for (int item = cta; item < items; item += G) {
+      const int tile = item / a.splits, split = item % a.splits, per = kCompute * a.splits;
+      // this warp's first box at or behind (segment i, box j)
+      auto seek = [&](int& i, int& j) {
+        while (i < n_act && j >= (i < 0 ? a.n2s : a.n2)) {
+          ++i;
+          if (i < n_act) j = first_box(warp, i) * a.splits + split;
+        }
+      };
       const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
-      float* p = buffer();
+      float* p;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (!kDirect) {
+      if constexpr (kDirect) {
+        p = buffer();
+      } else {
+        // the sums lie over all the buffers
+        p = &s.sums[warp][0][0][0][0];
+        for (int n = max(0, given - kParts); n < given; ++n) wait_read(n);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          *reinterpret_cast<float4*>(p + (nt * 32 + lane) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int q = 0; q < NT * kSub2; ++q)
+          *reinterpret_cast<float4*>(p + (q * 32 + lane) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         __syncwarp();
       }
       ready = false;
-      int i = -1, j = warp;
+      int i = -1, j = warp * a.splits + split;
       seek(i, j);
       auto step = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const bool sh = i < 0;
         if (sh ? !have_s : !have_r) {
           if (lane == 0) {
-            if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)a.ups, abort_flag, a.err);
-            else ctr_wait(a.ctr + kCtrRouted, (uint32_t)(n_act * a.upe), abort_flag, a.err);
+            if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)(a.ups * (SUB == 2 ? (a.T + 7) / 8 : 1)), abort_flag, a.err);
+            else ctr_wait(a.ctr + kCtrRouted, s.handed, abort_flag, a.err);
           }
           __syncwarp();
           if (sh) have_s = true; else have_r = true;
         }
         const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
         const int n_tok = sh ? a.T : s.cnt[i];
-        int ni = i, nj = j + kCompute;
+        int ni = i, nj = j + per;
         seek(ni, nj);
-        float s0 = 1.0f, s1 = 1.0f;  // fp8: every (expert, row) has its own scale
-        if constexpr (W::kSize == 1) {
-          const float* sc = (sh ? a.ws2s : a.w2s + (size_t)s.act[i] * a.dp) + r0;
-          s0 = __ldg(sc + min(g, rows - 1));
-          s1 = __ldg(sc + min(g + 8, rows - 1));
-        }
-        auto join = [&](const float (&acc)[4], int n0) {
+        float sc[kSub2][2];  // fp8: every (expert, row) has its own scale
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int n = n0 + 2 * t4 + q;
+        for (int q = 0; q < kSub2; ++q) {
+          sc[q][0] = sc[q][1] = 1.0f;
+          if constexpr (kHalf) {
+            const float* f = (sh ? a.ws2s : a.w2s + (size_t)s.act[i] * a.dp) + r0;
+            sc[q][0] = __ldg(f + min(16 * q + g, rows - 1));
+            sc[q][1] = __ldg(f + min(16 * q + g + 8, rows - 1));
+          }
+        }
+        auto join = [&](const float (&acc)[kSub2][4], int n0) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int n = n0 + 2 * t4 + c;
             if (n < n_tok) {
               const int tk = sh ? n : (int)s.tok[i][n];
-              float* o = p + ((tk >> 3) * 32 + g * 4 + ((tk & 7) >> 1)) * 4 + (tk & 1);
-              o[0] = fmaf(acc[q], s0, o[0]);
-              o[2] = fmaf(acc[2 + q], s1, o[2]);
+              float* o = p + ((tk >> 3) * kSub2 * 32 + g * 4 + ((tk & 7) >> 1)) * 4 + (tk & 1);
+#pragma unroll
+              for (int q = 0; q < kSub2; ++q) {
+                o[q * 128] = fmaf(acc[q][c], sc[q][0], o[q * 128]);
+                o[q * 128 + 2] = fmaf(acc[q][2 + c], sc[q][1], o[q * 128 + 2]);
+              }
             }
           }
         };
         if constexpr (kF32) {
           arrived();
           for (int n0 = 0; n0 < n_tok; n0 += 8) {
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float acc[1][4] = {{0.0f, 0.0f, 0.0f, 0.0f}};
             auto row = [&](int n) { return n0 + n < n_tok ? reinterpret_cast<const float*>(h_at(i, n0 + n, k)) : nullptr; };
-            box_fma<true>(acc, box(pitch), 8 * pitch, blk, row, (sh ? a.k2s : a.k2) - k, lane);
+            box_fma<true>(acc[0], box(pitch), 8 * pitch, blk, row, (sh ? a.k2s : a.k2) - k, lane);
             join(acc, n0);
           }
         } else {
@@ -957,25 +1068,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           ready = ni < n_act && (ni < 0 || have_r);
           if (ready) load_h(w, ni, 0, nj * (ni < 0 ? a.b2s : a.b2));
           arrived();
-          if constexpr (kDirect) {
-            // a box's sums join by the same operations in both forms: a token's result does not depend
-            // on how many others there are
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, v);
-            const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
-            if (m & 1u) {
-              sum[0] = fmaf(acc[0], s0, sum[0]);
-              sum[2] = fmaf(acc[2], s1, sum[2]);
-            }
-            if (m & 2u) {
-              sum[1] = fmaf(acc[1], s0, sum[1]);
-              sum[3] = fmaf(acc[3], s1, sum[3]);
-            }
-          } else {
-            for (int n0 = 0; n0 < n_tok; n0 += 8) {
-              float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              if (n0 > 0) load_h(v, i, n0, k);
-              box_mma<W, 2>(acc, box(pitch), 8 * pitch, blk, v);
+          for (int n0 = 0; n0 < n_tok; n0 += 8) {
+            // a box's sums join by the same operations in both forms: a token's result does not depend on
+            // how many others there are
+            float acc[kSub2][4];
+#pragma unroll
+            for (int q = 0; q < kSub2; ++q)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[q][c] = 0.0f;
+            if (n0 > 0) load_h(v, i, n0, k);
+            box_mma<W, 2, kSub2>(acc, box(pitch), 8 * pitch, 16 * pitch, blk, v);
+            if constexpr (kDirect) {
+              const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
+              if (m & 1u) {
+                sum[0] = fmaf(acc[0][0], sc[0][0], sum[0]);
+                sum[2] = fmaf(acc[0][2], sc[0][1], sum[2]);
+              }
+              if (m & 2u) {
+                sum[1] = fmaf(acc[0][1], sc[0][0], sum[1]);
+                sum[3] = fmaf(acc[0][3], sc[0][1], sum[3]);
+              }
+            } else {
               join(acc, n0);
             }
           }
@@ -995,43 +1108,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================================================ service
     const int sw = warp - kService;
-    constexpr bool kDirect = NT == 1 && !kF32, kHalf = W::kSize == 1;  // as in the compute warps
-    route<X, NT>(a, s, sw, route_warps, lane);
+    route<X, SUB>(a, s, sw, route_warps, lane);
     wait_routed();
-    const int n_act = s.n_act, n1 = nu_s + routed_units(n_act);
-    const int n2 = a.tiles > cta ? (a.tiles - cta + G - 1) / G : 0;
+    const int n_act = s.n_act, nu = nu_s + routed_units(n_act);
     const size_t h_lo = (size_t)a.T * a.k * a.hp, hs_lo = (size_t)a.T * a.hsp;
-    uint32_t owed[2] = {0u, 0u};  // stored units of the shared expert / the routed experts not yet announced
+    uint32_t owed[2] = {0u, 0u};  // handings over of the shared expert / the routed experts stored, not announced
     auto announce = [&](int which, uint32_t* ctr) {
       if (owed[which] == 0u) return;
       __syncwarp();
       if (lane == 0) ctr_add(ctr, owed[which]);
       owed[which] = 0u;
     };
-    int seen = sw;  // units and tiles of the CTA in order, every second one
+    // Every second handing over is this warp's.
+    int seq = 0;
+    auto mine = [&]() { return seq % kServices == sw; };
     auto wait_parts = [&]() {
-      mbar_wait(smem_u32(&s.part_full[sw]), (uint32_t)(seen / kParts) & 1u, abort_flag, a.err);
-    };
-    // tile nt of the sums of the first n compute warps
-    auto sum = [&](int n, int nt, float (&c)[4]) {
-      c[0] = c[1] = c[2] = c[3] = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kCompute; ++w) {
-        if (w >= n) break;
-        const float4 o = *reinterpret_cast<const float4*>(s.part[sw][w][nt][lane]);
-        c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
-      }
+      mbar_wait(smem_u32(&s.part_full[seq % kParts]), (uint32_t)(seq / kParts) & 1u, abort_flag, a.err);
     };
     auto free_parts = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[sw]));
-      seen += kServices;
+      if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[seq % kParts]));
     };
-    int ai = 0, first = 0;  // active expert of the next routed unit, and that expert's first one
-    for (; seen < n1;) {
-      const int un = seen;
+    int ai = 0, first = 0;  // active expert of the present routed unit, and that expert's first one
+    for (int un = 0; un < nu; ++un) {
       const bool sh = un < nu_s;
-      if (!sh) announce(0, a.ctr + kCtrShared);
+      if (un == nu_s) announce(0, a.ctr + kCtrShared);
       const int r = r_first + (un - nu_s) * G;
       if (!sh)
         while (r >= first + a.upe) {
@@ -1040,98 +1141,163 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       const int u = sh ? cta + un * G : r - first, e = sh ? 0 : s.act[ai];
       const int n_tok = sh ? a.T : s.cnt[ai];
-      // where this unit's sums go is looked up before they are there
-      float s0 = 1.0f, s1 = 1.0f;
-      if constexpr (W::kSize == 1) {
-        const int ch = 8 * u + g;
-        const int r0 = a.glu ? (ch >> 7) * 256 + (ch & 127) : 16 * u + g, r1 = a.glu ? r0 + 128 : r0 + 8;
-        const float* sc = sh ? a.ws1s : a.w1s + (size_t)e * a.n1p;
-        s0 = __ldg(sc + r0);
-        s1 = __ldg(sc + r1);
-      }
-      // activation, routing weight, and the intermediate to where GEMM2 reads it
-      uint8_t* base = sh ? a.hs : a.h;
-      const size_t lo = sh ? hs_lo : h_lo;
-      const uint32_t mask = sh ? 0xffffffffu : s.mask[ai];
-      for (int nt = 0; nt * 8 < (kDirect ? a.T : n_tok); ++nt) {
-        float wt[2], xi[2], hs[2];
-        size_t at[2];
-        bool on[2];
-        int tok[2];
+      for (int h0 = 0; h0 < (kHand < NT ? n_tok : 1); h0 += 8, ++seq) {
+        if (!mine()) continue;
+        // where these sums go is looked up before they are there
+        float s0[SUB], s1[SUB];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          int n = nt * 8 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
-          on[i] = n < (kDirect ? a.T : n_tok);
-          if constexpr (kDirect) {
-            on[i] = on[i] && ((mask >> n) & 1u);
-            if (!sh) n = __popc(mask & ((1u << n) - 1u));
+        for (int q = 0; q < SUB; ++q) {
+          s0[q] = s1[q] = 1.0f;
+          if constexpr (kHalf) {
+            const int ch = 8 * SUB * u + 8 * q + g;
+            const int row0 = a.glu ? (ch >> 7) * 256 + (ch & 127) : 16 * SUB * u + 16 * q + g, row1 = a.glu ? row0 + 128 : row0 + 8;
+            const float* sc = sh ? a.ws1s : a.w1s + (size_t)e * a.n1p;
+            s0[q] = __ldg(sc + row0);
+            s1[q] = __ldg(sc + row1);
           }
-          const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
-          wt[i] = sh ? s.sg[row] : s.wt[row];
-          tok[i] = sh ? n : (on[i] ? (int)s.tok[ai][n] : 0);
-          at[i] = (size_t)row * (sh ? a.hsp : a.hp);
         }
-        if (nt == 0) wait_parts();
-        float c[4];
-        sum(a.n1, nt, c);
+        // activation, routing weight, and the intermediate to where GEMM2 reads it
+        uint8_t* base = sh ? a.hs : a.h;
+        const size_t lo = sh ? hs_lo : h_lo;
+        const uint32_t mask = sh ? 0xffffffffu : s.mask[ai];
+        bool waited = false;
+        for (int nt = 0; nt < kHand; ++nt) {
+          const int n0 = kHand < NT ? h0 : nt * 8;
+          if (n0 >= (kDirect ? a.T : n_tok)) break;
+          float wt[2];
+          size_t at[2];
+          bool on[2];
+          int tok[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          xi[i] = kHalf ? s.xinv[tok[i]] : 1.0f;
-          hs[i] = kHalf ? s.hscale[tok[i]] : 1.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!on[i]) continue;
-          auto put = [&](int ch, float val) {
-            if constexpr (kF32) {
-              reinterpret_cast<float*>(base)[at[i] + ch] = val;
-            } else if constexpr (kHalf) {
-              const __half hi = __float2half_rn(val);
-              __half* o = reinterpret_cast<__half*>(base) + at[i] + ch;
-              o[0] = hi;
-              const float rest = val - __half2float(hi);
-              o[lo] = __float2half_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
-            } else {
-              const __nv_bfloat16 hi = __float2bfloat16_rn(val);
-              const float rest = val - __bfloat162float(hi);
-              __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at[i] + ch;
-              o[0] = hi;
-              // an infinite or NaN value is the high term alone
-              o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
+          for (int i = 0; i < 2; ++i) {
+            int n = n0 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
+            on[i] = n < (kDirect ? a.T : n_tok);
+            if constexpr (kDirect) {
+              on[i] = on[i] && ((mask >> n) & 1u);
+              if (!sh) n = __popc(mask & ((1u << n) - 1u));
             }
-          };
-          const float c0 = c[i] * xi[i] * s0, c1 = c[2 + i] * xi[i] * s1, f = wt[i] * hs[i];
-          if (a.glu) {
-            // the scale joins one factor first: their product may leave fp32 where the scaled one does not
-            put(8 * u + g, c0 / (1.0f + expf(-c0)) * f * c1);
-          } else {
-            put(16 * u + g, f * fmaxf(c0, 0.0f));
-            put(16 * u + g + 8, f * fmaxf(c1, 0.0f));
+            const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
+            tok[i] = on[i] ? (sh ? n : (int)s.tok[ai][n]) : 0;
+            wt[i] = sh ? s.sg[row] : s.wt[row];
+            at[i] = (size_t)row * (sh ? a.hsp : a.hp);
+          }
+          if (!waited) wait_parts();
+          waited = true;
+          float c[SUB][4];
+#pragma unroll
+          for (int q = 0; q < SUB; ++q) c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kCompute; ++w) {
+            if (w >= a.n1) break;
+#pragma unroll
+            for (int q = 0; q < SUB; ++q) {
+              const float4 o = *reinterpret_cast<const float4*>(s.part[seq % kParts][w][nt][q][lane]);
+              c[q][0] += o.x; c[q][1] += o.y; c[q][2] += o.z; c[q][3] += o.w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!on[i]) continue;
+            const float xi = kHalf ? s.xinv[tok[i]] : 1.0f, f = kHalf ? wt[i] * s.hscale[tok[i]] : wt[i];
+            auto put = [&](int ch, float val) {
+              if constexpr (kF32) {
+                reinterpret_cast<float*>(base)[at[i] + ch] = val;
+              } else if constexpr (kHalf) {
+                const __half hi = __float2half_rn(val);
+                __half* o = reinterpret_cast<__half*>(base) + at[i] + ch;
+                o[0] = hi;
+                const float rest = val - __half2float(hi);
+                o[lo] = __float2half_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
+              } else {
+                const __nv_bfloat16 hi = __float2bfloat16_rn(val);
+                const float rest = val - __bfloat162float(hi);
+                __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + at[i] + ch;
+                o[0] = hi;
+                // an infinite or NaN value is the high term alone
+                o[lo] = __float2bfloat16_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
+              }
+            };
+#pragma unroll
+            for (int q = 0; q < SUB; ++q) {
+              const float c0 = c[q][i] * xi * s0[q], c1 = c[q][2 + i] * xi * s1[q];
+              if (a.glu) {
+                // the factor joins one side first: the product alone may leave fp32 where the scaled one does not
+                put(8 * SUB * u + 8 * q + g, c0 / (1.0f + expf(-c0)) * f * c1);
+              } else {
+                put(16 * SUB * u + 16 * q + g, f * fmaxf(c0, 0.0f));
+                put(16 * SUB * u + 16 * q + g + 8, f * fmaxf(c1, 0.0f));
+              }
+            }
           }
         }
+        free_parts();
+        ++owed[sh ? 0 : 1];
       }
-      free_parts();
-      ++owed[sh ? 0 : 1];
     }
     announce(0, a.ctr + kCtrShared);
     announce(1, a.ctr + kCtrRouted);
     // ---- the output's rows
-    while (seen < n1 + n2) {
-      const int n = seen - n1;
-      const int r0 = (cta + n * G) * a.rt, rows = min(a.rt, a.d - r0);
+    for (int item = cta; item < items; item += G, ++seq) {
+      if (!mine()) continue;
+      const int tile = item / a.splits, r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
       wait_parts();
       X* out = reinterpret_cast<X*>(a.out);
+      auto sums = [&](int nt, int q, float (&c)[4]) {
+        c[0] = c[1] = c[2] = c[3] = 0.0f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float c[4];
-        sum(kCompute, nt, c);
+        for (int w = 0; w < kCompute; ++w) {
+          const float4 o = *reinterpret_cast<const float4*>(kDirect ? s.part[seq % kParts][w][0][0][lane] : s.sums[kDirect ? 0 : w][nt][q][lane]);
+          c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
+        }
+      };
+      auto store = [&](int nt, int q, const float (&c)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int tk = nt * 8 + 2 * t4 + (i & 1), rr = g + (i >> 1) * 8;
+          const int tk = nt * 8 + 2 * t4 + (i & 1), rr = 16 * q + g + (i >> 1) * 8;
           if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(kHalf ? c[i] / s.hscale[tk] : c[i]);
         }
+      };
+      if (a.splits == 1) {
+        for (int nt = 0; nt < NT; ++nt)
+          for (int q = 0; q < kSub2; ++q) {
+            float c[4];
+            sums(nt, q, c);
+            store(nt, q, c);
+          }
+        free_parts();
+      } else {
+        constexpr int kTile = NT * kSub2 * 128;
+        float* mine_at = a.partial + (size_t)item * kTile;
+        for (int nt = 0; nt < NT; ++nt)
+          for (int q = 0; q < kSub2; ++q) {
+            float c[4];
+            sums(nt, q, c);
+            *reinterpret_cast<float4*>(mine_at + (nt * kSub2 + q) * 128 + lane * 4) = make_float4(c[0], c[1], c[2], c[3]);
+          }
+        free_parts();
+        // the last of the CTAs that share the tile adds their sums, in order
+        uint32_t before = 0u;
+        if (lane == 0) {
+          __threadfence();
+          before = atomicAdd(a.ctr + kCtrTiles + tile, 1u);
+          __threadfence();
+        }
+        before = __shfl_sync(0xffffffffu, before, 0);
+        if (before == (uint32_t)a.splits - 1u) {
+          const float* all = a.partial + (size_t)tile * a.splits * kTile;
+          for (int nt = 0; nt < NT; ++nt)
+            for (int q = 0; q < kSub2; ++q) {
+              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+              for (int v = 0; v < a.splits; ++v) {
+                const float4 o = __ldcg(reinterpret_cast<const float4*>(all + (size_t)v * kTile + (nt * kSub2 + q) * 128 + lane * 4));
+                c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
+              }
+              store(nt, q, c);
+            }
+          if (lane == 0) a.ctr[kCtrTiles + tile] = 0u;
+        }
       }
-      free_parts();
     }
   }
 
@@ -1145,6 +1311,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 }
+
+constexpr int kMaxItems = 256;  // items whose sums the workspace holds, 32 rows x 32 tokens each
+constexpr size_t kPartialBytes = (size_t)kMaxItems * 4 * 2 * 512;
 
 inline int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
@@ -1163,8 +1332,8 @@ EncodeTiled encode_fn() {
   return fn;
 }
 
-// Boxes of `rows` rows x `box` values of a row-major matrix [n, width]; glu: of 8 gate and the matching 8
-// up rows of its 256-row blocks.  Values behind the row's end are filled with zeros.
+// Boxes of `rows` rows x `box` values of a row-major matrix [n, width]; glu: half of them gate rows, half the
+// matching up rows of its 256-row blocks.  Values behind the row's end are filled with zeros.
 template <typename W>
 int make_map(CUtensorMap* m, const void* base, uint64_t n, int width, int box, int rows, bool glu) {
   EncodeTiled enc = encode_fn();
@@ -1174,22 +1343,23 @@ int make_map(CUtensorMap* m, const void* base, uint64_t n, int width, int box, i
                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const cuuint64_t row = (cuuint64_t)width * W::kSize;
   const cuuint64_t dims[4] = {(cuuint64_t)width, glu ? 128u : n, 2, n / 256}, strides[3] = {row, row * 128, row * 256};
-  const cuuint32_t boxes[4] = {(cuuint32_t)box, (cuuint32_t)(glu ? 8 : rows), 2, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t boxes[4] = {(cuuint32_t)box, (cuuint32_t)(glu ? rows / 2 : rows), 2, 1}, one[4] = {1, 1, 1, 1};
   return enc(m, type, glu ? 4 : 2, const_cast<void*>(base), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? DSCA_OK
              : DSCA_ERR_CUDA;
 }
 
-// Bytes of a row of `bytes` in a box: the twelve warps take the boxes in turn, and a warp's time for one
-// is about that of 256 bytes for the tokens' values from L2 plus that of the box itself.  At most the
-// blocks whose token values a lane holds; tensor maps take at most 256 values.
+// Bytes of a row of `bytes` in a box: `warps` warps take a row's boxes in turn (GEMM2, where they go round from
+// expert to expert: as one), and a warp's time for one is about that of 256 bytes for its instructions
+// plus that of the box itself.  At most `most`, and the blocks whose
+// token values a lane holds; tensor maps take at most 256 values.
 template <typename W, int kTerms>
-int box_of(int bytes) {
-  const int most = W::kSize == 4 ? kMaxBox : min(kMaxBox, Layout<W, kTerms>::kBlocks * 64);
+int box_of(int bytes, int warps, int most) {
+  if (W::kSize != 4) most = min(most, Layout<W, kTerms>::kBlocks * 64);
   int best = 64, cost = 1 << 30;
   for (int b = 64; b <= most && b <= 256 * W::kSize; b += 64) {
-    const int n = (bytes + b - 1) / b, c = (n + kCompute - 1) / kCompute * (b + 256);
+    const int n = (bytes + b - 1) / b, c = (n + warps - 1) / warps * (b + 256);
     if (c < cost) {
       best = b;
       cost = c;
@@ -1198,35 +1368,54 @@ int box_of(int bytes) {
   return best;
 }
 
-template <typename W, int NT>
+// Output rows of a tile and CTAs that share one (see the top): CTAs of their own for at least nine rows
+// (gathered tokens: 24) each, else tiles of 16 (32) rows and as many CTAs to each as there are.
+// Gathered tokens, 28 rows by 2 CTAs against 14 by one: 32 tokens of the Qwen block with fp8 weights.
+inline void plan_tiles(int d, int sms, int high, int* rt, int* tiles, int* splits) {
+  const int per = (d + sms - 1) / sms, full = (d + high - 1) / high;
+  *splits = per * 4 > high * 2 + high ? 1 : max(1, sms / full);
+  const int ctas = sms / *splits, nt = ((d + ctas - 1) / ctas + high - 1) / high;
+  *rt = (d + ctas * nt - 1) / (ctas * nt);
+  *tiles = (d + *rt - 1) / *rt;
+}
+
+template <typename W, int NT, int SUB>
 int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
+  using F = Form<W, NT, SUB>;
   static PerDeviceOnce once;
   if (once.run([] {
-        return cudaFuncSetAttribute(moe_few_kernel<W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        return cudaFuncSetAttribute(moe_few_kernel<W, NT, SUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
       }) != cudaSuccess)
     return DSCA_ERR_CUDA;
-  constexpr int kFixed = (int)((sizeof(Smem<NT>) + 127) / 128 * 128);
-  static_assert((kSmem - kFixed) / (kCompute * 16 * kMaxBox) >= 2, "two boxes a ring");
-  a.b1 = box_of<W, 1>(a.d * W::kSize) / W::kSize;
-  a.b2 = box_of<W, 2>(a.k2 * W::kSize) / W::kSize;
-  a.b2s = box_of<W, 2>(a.k2s * W::kSize) / W::kSize;
+  constexpr int kFixed = (int)((sizeof(Smem<W, NT, SUB>) + 127) / 128 * 128);
+  const int unit = (a.glu ? 8 : 16) * SUB, shared = p->w_shared_gate != nullptr ? p->shared_inter : 0;
+  a.upe = (p->inter + unit - 1) / unit;
+  a.ups = (shared + unit - 1) / unit;
+  // GEMM2 reads whole 16-byte vectors: the channels behind the last are zero in both operands
+  a.k2 = a.upe * unit;
+  a.k2s = a.ups * unit;
+  plan_tiles(a.d, sms, 16 * F::kSub2, &a.rt, &a.tiles, &a.splits);
+  if (a.splits > 1 && (kCtrTiles + a.tiles > DSCA_FEW_ZERO_BYTES / 4 || a.tiles * a.splits > kMaxItems)) return DSCA_ERR_CAPACITY;
+  // a stage holds whole 16-row tiles: the rows behind a tile's last are read, and dropped
+  const int rows = 16 * max(SUB, F::kSub2), most = min(kMaxBox, (kSmem - kFixed) / (2 * kCompute * rows) / 64 * 64);
+  a.b1 = box_of<W, 1>(a.d * W::kSize, kCompute, most) / W::kSize;
+  a.b2 = box_of<W, 2>(a.k2 * W::kSize, 1, most) / W::kSize;
+  a.b2s = box_of<W, 2>(a.k2s * W::kSize, 1, most) / W::kSize;
   a.n1 = (a.d + a.b1 - 1) / a.b1;
   a.n2 = (a.k2 + a.b2 - 1) / a.b2;
   a.n2s = (a.k2s + a.b2s - 1) / a.b2s;
-  a.stage = 16 * max(a.b1, max(a.b2, a.n2s ? a.b2s : 0)) * W::kSize;
+  if (SUB == 2 && a.n1 > kCompute) return DSCA_ERR_CAPACITY;
+  const int bytes = max(16 * SUB * a.b1, 16 * F::kSub2 * max(a.b2, a.n2s ? a.b2s : 0)) * W::kSize;
+  a.stage = (bytes + 127) / 128 * 128;
   a.stages = min(kMaxStages, (kSmem - kFixed) / (kCompute * a.stage));
-  // output rows in tiles of at most 16, as even as they come over the SMs
-  const int per = (a.d + sms - 1) / sms, nt = (per + 15) / 16;
-  a.rt = (a.d + sms * nt - 1) / (sms * nt);
-  a.tiles = (a.d + a.rt - 1) / a.rt;
   CUtensorMap m1, m2, ms1, ms2;
   int rc;
-  if ((rc = make_map<W>(&m1, a.w1, (uint64_t)a.E * a.n1p, a.d, a.b1, 16, a.glu))) return rc;
+  if ((rc = make_map<W>(&m1, a.w1, (uint64_t)a.E * a.n1p, a.d, a.b1, 16 * SUB, a.glu))) return rc;
   if ((rc = make_map<W>(&m2, a.w2, (uint64_t)a.E * a.dp, a.ip, a.b2, a.rt, false))) return rc;
   ms1 = m1;
   ms2 = m2;
   if (a.ups) {
-    if ((rc = make_map<W>(&ms1, a.ws1, (uint64_t)p->shared_n1p, a.d, a.b1, 16, a.glu))) return rc;
+    if ((rc = make_map<W>(&ms1, a.ws1, (uint64_t)p->shared_n1p, a.d, a.b1, 16 * SUB, a.glu))) return rc;
     if ((rc = make_map<W>(&ms2, a.ws2, (uint64_t)a.dp, a.s_ip, a.b2s, a.rt, false))) return rc;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1239,14 +1428,22 @@ int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   at[0].val.cooperative = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, moe_few_kernel<W, NT>, (const Args)a, m1, m2, ms1, ms2) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, moe_few_kernel<W, NT, SUB>, (const Args)a, m1, m2, ms1, ms2) == cudaSuccess ? DSCA_OK
+                                                                                                             : DSCA_ERR_CUDA;
 }
 
 template <typename W>
 int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream) {
-  if (a.T <= 8) return launch<W, 1>(a, p, sms, stream);
-  if (a.T <= 16) return launch<W, 2>(a, p, sms, stream);
-  return launch<W, 4>(a, p, sms, stream);
+  if (a.T <= 8) return launch<W, 1, 1>(a, p, sms, stream);
+  if constexpr (W::kSize != 4) {
+    // units of 32 rows: one box of at most 192 bytes a warp
+    if (a.d * W::kSize <= 192 * kCompute) {
+      if (a.T <= 16) return launch<W, 2, 2>(a, p, sms, stream);
+      return launch<W, 4, 2>(a, p, sms, stream);
+    }
+  }
+  if (a.T <= 16) return launch<W, 2, 1>(a, p, sms, stream);
+  return launch<W, 4, 1>(a, p, sms, stream);
 }
 
 }  // namespace few
@@ -1254,7 +1451,8 @@ int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream
 size_t few_workspace_bytes(int T, int d, int k, int inter, int shared_inter) {
   const size_t hp = few::round_up(inter, 64), hsp = few::round_up(shared_inter, 64);
   const size_t x16 = T > 8 ? (size_t)T * (d * 2 + 8) : 0;  // fp8 weights
-  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4 + (x16 + 255) / 256 * 256;
+  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4 +
+         (x16 + 255) / 256 * 256 + few::kPartialBytes;
 }
 
 int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
@@ -1269,19 +1467,15 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.k = p->mode == DSCA_ROUTE_SWITCH_TOP1 ? 1 : p->top_k;
   a.glu = p->act == DSCA_ACT_SWIGLU;
   a.n1p = p->n1p; a.ip = p->ip; a.dp = p->dp; a.s_ip = p->shared_ip;
-  const int shared = p->w_shared_gate != nullptr ? p->shared_inter : 0, unit = a.glu ? 8 : 16;
+  const int shared = p->w_shared_gate != nullptr ? p->shared_inter : 0;
   a.hp = few::round_up(p->inter, 64);
   a.hsp = few::round_up(shared, 64);
-  a.upe = (p->inter + unit - 1) / unit;
-  a.ups = (shared + unit - 1) / unit;
-  // GEMM2 reads whole 16-byte vectors: the channels behind the last are zero in both operands
-  a.k2 = a.upe * unit;
-  a.k2s = a.ups * unit;
   uint8_t* w = (uint8_t*)p->workspace;
   a.ctr = (uint32_t*)w;
   a.lg = (float*)(w + DSCA_FEW_ZERO_BYTES);
   a.h = w + DSCA_FEW_ZERO_BYTES + (size_t)a.T * few::kLgPitch * 4;
   a.hs = a.h + (size_t)a.T * a.k * a.hp * 4;
+  a.partial = (float*)(w + few_workspace_bytes(a.T, a.d, a.k, p->inter, shared) - few::kPartialBytes);
   if (p->weights == DSCA_F8E4M3) {
     if (a.T > 8) {
       a.x16 = a.hs + (size_t)a.T * a.hsp * 4;

@@ -194,11 +194,19 @@ def test_agrees_with_forward_and_is_repeatable(cuda, kind):
     assert same.sum() >= 31
     ao, bo = a["out"][same].float(), b["out"][same].float()
     assert ((ao - bo).abs().max() / bo.abs().max()) < 2e-2
-    for T in (32, 9, 1):
+    c = _run(eng, x)
+    for key in ("out", "topk_w", "topk_ids", "logits"):
+        assert torch.equal(c[key], a[key])
+    # the choice of experts does not depend on how many tokens a call has, nor a token's result on the
+    # others' values
+    for T in (9, 1):
         c = _run(eng, x[:T])
-        # a token's result does not depend on the other tokens of the call
-        for key in ("out", "topk_w", "topk_ids", "logits"):
+        _check(c, x[:T], w, router, gate, 4)
+        for key in ("topk_w", "topk_ids", "logits"):
             assert torch.equal(c[key], a[key][:T])
+    y = n(32, 512, std=1.0)
+    y[5] = x[5]
+    assert torch.equal(_run(eng, y)["out"][5], a["out"][5])
 
 
 def test_input_forms(cuda):
