@@ -66,7 +66,8 @@ constexpr int kMaxStages = 8;             // boxes of a compute warp's ring, at 
 constexpr int kMaxBox = 384;              // bytes of a weight row in a box, at most
 constexpr int kVals = 8;                  // 16-byte vectors of token values that a lane holds for a box
 constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
-constexpr int kLgPitch = 64;              // logits scratch: E + 1 <= 64 per token
+constexpr int kLgPitch = 64;              // logits of a token in the scratch: E + 1 <= 64
+constexpr int kDotParts = 4;              // warps that share a logit's dot product
 
 // words of the counter block
 enum { kCtrLogits = 0, kCtrShared = 1, kCtrRouted = 2, kCtrExit = 3, kCtrTiles = 8 };
@@ -82,7 +83,7 @@ struct Args {
   int32_t* topk_ids;
   float* topk_w;
   int64_t* expert_index;
-  float* lg;        // [T][64] logits as fp32 (rounded to the router's type), column E = shared gate
+  double* lg;       // [T][64][4] parts of the logits, column E = shared gate
   uint8_t* x16;     // fp8 weights, more than eight tokens: [T][d] token rows in f16
   float* xmeta;     // and [T][2]: 1 / their scale, the largest power of two below sum|x|
   uint8_t* h;       // [T * k][hp] intermediate: high terms, then the low terms; or fp32
@@ -259,8 +260,9 @@ __device__ __forceinline__ float round_to<__nv_bfloat16>(double v) { return roun
 template <>
 __device__ __forceinline__ float round_to<float>(double v) { return (float)v; }
 
-// x . w over one warp in fp64, the same on every lane.  Rows come from DRAM behind the stream of weights,
-// so eight vectors of each are asked for at once.
+// Part `part` of x . w over one warp in fp64, the same on every lane.  The code is short and the parts are
+// small because a call runs it cold: instructions come from L2 at some 75 ns for eight of them, so 64
+// products unrolled took 2.5 us where 16 take 0.7.
 __device__ __forceinline__ void dot_add(double (&s)[4], uint4 a, uint4 b, const __nv_bfloat16*) {
   const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -277,23 +279,21 @@ __device__ __forceinline__ void dot_add(double (&s)[4], uint4 a, uint4 b, const 
   s[3] = fma((double)__uint_as_float(a.w), (double)__uint_as_float(b.w), s[3]);
 }
 template <typename X>
-__device__ __forceinline__ double dot64(const X* x, const X* w, int d, int lane) {
-  constexpr int kVec = 16 / sizeof(X), kAhead = 8;
+__device__ __forceinline__ double dot64(const X* x, const X* w, int d, int part, int lane) {
+  constexpr int kVec = 16 / sizeof(X), kStep = 32 * kDotParts * kVec;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   double s[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int c = lane * kVec; c < d; c += 32 * kVec * kAhead) {
-    uint4 a[kAhead], b[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int k = c + i * 32 * kVec;
-      a[i] = k < d ? __ldg(reinterpret_cast<const uint4*>(x + k)) : zero;
-      b[i] = k < d ? __ldg(reinterpret_cast<const uint4*>(w + k)) : zero;
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) dot_add(s, a[i], b[i], x);
+#pragma unroll 1
+  for (int k = (part * 32 + lane) * kVec; k < d; k += 2 * kStep) {
+    const bool more = k + kStep < d;
+    const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(x + k)), b0 = __ldg(reinterpret_cast<const uint4*>(w + k));
+    const uint4 a1 = more ? __ldg(reinterpret_cast<const uint4*>(x + k + kStep)) : zero;
+    const uint4 b1 = more ? __ldg(reinterpret_cast<const uint4*>(w + k + kStep)) : zero;
+    dot_add(s, a0, b0, x);
+    dot_add(s, a1, b1, x);
   }
   double r = (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
+#pragma unroll 1
   for (int off = 16; off >= 1; off >>= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
   return r;
 }
@@ -307,17 +307,25 @@ __device__ __forceinline__ float ord_val(uint32_t k) {
 }
 
 // Softmax and selection of one token by one warp (lane holds experts lane and lane + 32), with the
-// arithmetic and the tie rule of dsca_router_topk.  Every CTA does it for itself; CTA 0 writes the results.
+// arithmetic and the tie rule of dsca_router_topk.  Every CTA does it for itself; CTA 0 writes the
+// results.  dry: nothing is read or written (the code only comes into the instruction cache, in the
+// time that the logits of other CTAs take: see dot64).
 template <typename X, typename S>
-__device__ __forceinline__ void select_token(const Args& a, S& s, int t, int lane) {
+__device__ __forceinline__ void select_token(const Args& a, S& s, int t, bool dry, int lane) {
   const int E = a.E, e0 = lane, e1 = lane + 32;
-  const float l0 = __ldcg(a.lg + t * kLgPitch + e0), l1 = __ldcg(a.lg + t * kLgPitch + e1);
-  const bool v0 = e0 < E, v1 = e1 < E, first = blockIdx.x == 0;
-  if (a.x16 != nullptr && lane == 0) {
+  auto logit = [&](int e) {
+    if (dry) return 0.0f;
+    const double2* p = reinterpret_cast<const double2*>(a.lg + (size_t)(t * kLgPitch + e) * kDotParts);
+    const double2 u = __ldcg(p), v = __ldcg(p + 1);
+    return round_to<X>((u.x + u.y) + (v.x + v.y));
+  };
+  const float l0 = logit(e0), l1 = logit(e1);
+  const bool v0 = e0 < E, v1 = e1 < E, first = blockIdx.x == 0 && !dry;
+  if (a.x16 != nullptr && lane == 0 && !dry) {
     s.xinv[t] = __ldcg(a.xmeta + 2 * t);
     s.hscale[t] = pow2(h_scale_exp(exp_of(__ldcg(a.xmeta + 2 * t + 1)), a.w1_exp, a.glu));
   }
-  if (a.w_gate != nullptr && (e0 == E || e1 == E)) s.sg[t] = 1.0f / (1.0f + expf(-(e0 == E ? l0 : l1)));
+  if (a.w_gate != nullptr && (e0 == E || e1 == E) && !dry) s.sg[t] = 1.0f / (1.0f + expf(-(e0 == E ? l0 : l1)));
   if (first) {
     X* lo = reinterpret_cast<X*>(a.logits) + (size_t)t * E;
     if (v0) lo[e0] = X(l0);
@@ -353,7 +361,7 @@ __device__ __forceinline__ void select_token(const Args& a, S& s, int t, int lan
     }
     sum = __fadd_rn(sum, bv);
   }
-  if (lane < a.k) {
+  if (lane < a.k && !dry) {
     float w = my_p;
     if (!top1) {
       if (a.norm_topk) w = __fdiv_rn(my_p, sum);
@@ -520,12 +528,13 @@ __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync
 template <typename X, int SUB, typename S>
 __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
-  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), nd = a.T * R;
+  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), nd = a.T * R * kDotParts;
+#pragma unroll 1
   for (int q = cta + wi * G; q < nd; q += nw * G) {
-    const int t = q / R, r = q % R;
+    const int part = q % kDotParts, t = q / kDotParts / R, r = q / kDotParts % R;
     const X* w = r < a.E ? reinterpret_cast<const X*>(a.w_router) + (size_t)r * a.d : reinterpret_cast<const X*>(a.w_gate);
-    const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, lane);
-    if (lane == 0) a.lg[t * kLgPitch + r] = round_to<X>(v);
+    const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, part, lane);
+    if (lane == 0) a.lg[(size_t)(t * kLgPitch + r) * kDotParts + part] = v;
   }
   // fp8 weights, more than eight tokens: CTA t writes token t's row in f16 (eight or less: the compute
   // warps convert what they keep of it)
@@ -548,12 +557,19 @@ __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int l
     }
   }
   group_sync(nw * 32);
-  if (wi == 0 && lane == 0) {
-    if (cta < nd) ctr_add(a.ctr + kCtrLogits, 1u);
-    ctr_wait(a.ctr + kCtrLogits, (uint32_t)min(nd, G), &s.abort, a.err);
+  if (wi == 0 && lane == 0 && cta < nd) ctr_add(a.ctr + kCtrLogits, 1u);
+  __syncwarp();
+  for (int t = wi - nw; t < a.T; t += nw) {
+    if (t >= 0 && t < nw) {
+      if (wi == 0 && lane == 0) ctr_wait(a.ctr + kCtrLogits, (uint32_t)min(nd, G), &s.abort, a.err);
+      __syncwarp();
+      group_sync(nw * 32);
+    }
+    select_token<X>(a, s, max(t, 0), t < 0, lane);
   }
-  group_sync(nw * 32);
-  for (int t = wi; t < a.T; t += nw) select_token<X>(a, s, t, lane);
+  if (wi >= a.T) {  // no token for this warp: the same barrier
+    group_sync(nw * 32);
+  }
   group_sync(nw * 32);
   if (wi == 0) {
     const uint32_t m0 = s.emask[lane], m1 = s.emask[lane + 32];
@@ -1451,7 +1467,7 @@ int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream
 size_t few_workspace_bytes(int T, int d, int k, int inter, int shared_inter) {
   const size_t hp = few::round_up(inter, 64), hsp = few::round_up(shared_inter, 64);
   const size_t x16 = T > 8 ? (size_t)T * (d * 2 + 8) : 0;  // fp8 weights
-  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * 4 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4 +
+  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * few::kDotParts * 8 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4 +
          (x16 + 255) / 256 * 256 + few::kPartialBytes;
 }
 
@@ -1472,8 +1488,8 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.hsp = few::round_up(shared, 64);
   uint8_t* w = (uint8_t*)p->workspace;
   a.ctr = (uint32_t*)w;
-  a.lg = (float*)(w + DSCA_FEW_ZERO_BYTES);
-  a.h = w + DSCA_FEW_ZERO_BYTES + (size_t)a.T * few::kLgPitch * 4;
+  a.lg = (double*)(w + DSCA_FEW_ZERO_BYTES);
+  a.h = w + DSCA_FEW_ZERO_BYTES + (size_t)a.T * few::kLgPitch * few::kDotParts * 8;
   a.hs = a.h + (size_t)a.T * a.k * a.hp * 4;
   a.partial = (float*)(w + few_workspace_bytes(a.T, a.d, a.k, p->inter, shared) - few::kPartialBytes);
   if (p->weights == DSCA_F8E4M3) {
