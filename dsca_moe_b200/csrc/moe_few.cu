@@ -39,13 +39,16 @@
 // are: the k index that the instruction thinks it sees is a permutation of the real one, the same
 // for both operands.
 //
-// The intermediate is kept as two bf16 terms (16 significant bits); everything is summed in fp32,
+// The intermediate is kept as two bf16 terms (16 significant bits; with fp32 weights in fp32, with fp8 weights
+// as one f16 term); everything is summed in fp32,
 // the router in fp64 (bf16 products are exact in fp32, so the logits round correctly).
 //
 // fp8 weights go through f16: e4m3 converts to it exactly with one instruction a pair (to bf16 it
 // takes four, which alone cost more than the weights' DRAM time).  A token row times a power of two
 // that takes its largest value to [2^14, 2^15) is exact in f16 down to 2^-29 of that value.  The
-// intermediate (two f16 terms) needs a scale before it is known: |h| <= B^2 (SwiGLU; B with ReLU), B =
+// intermediate (one f16 term: it is off by 2^-11 at most where the output's bf16 is by 2^-8 and the weights'
+// own rounding by 2^-4; with a second one, twice the loads and products of
+// GEMM2, 32 tokens took 183 us instead of 153 and one took 31 instead of 27) needs a scale before it is known: |h| <= B^2 (SwiGLU; B with ReLU), B =
 // max|w1| sum|x|, so 2^14 / B^2 rounded down to a power of two cannot overflow, and typical values, some
 // 2^20 below the bound, still lie 2^18 above the smallest f16.
 #include <math.h>
@@ -215,6 +218,7 @@ struct Form {
   // the tensor core's columns are the tokens of the call (else the tokens of the expert at hand)
   static constexpr bool kDirect = NT == 1 && !kF32;
   static constexpr int kSub2 = kDirect || kF32 ? 1 : 2;  // 16-row tiles of a GEMM2 tile
+  static constexpr int kTerms = kHalf ? 1 : 2;           // of the intermediate (see the top)
   // tiles of eight tokens that a unit's sums are handed over in at a time
   static constexpr int kHand = SUB == 2 ? 1 : NT;
 };
@@ -279,16 +283,17 @@ __device__ __forceinline__ void dot_add(double (&s)[4], uint4 a, uint4 b, const 
   s[3] = fma((double)__uint_as_float(a.w), (double)__uint_as_float(b.w), s[3]);
 }
 template <typename X>
-__device__ __forceinline__ double dot64(const X* x, const X* w, int d, int part, int lane) {
-  constexpr int kVec = 16 / sizeof(X), kStep = 32 * kDotParts * kVec;
+__device__ __forceinline__ double dot64(const X* x, const X* w, int d, int part, int parts, int lane) {
+  constexpr int kVec = 16 / sizeof(X);
+  const int step = 32 * parts * kVec;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 1
-  for (int k = (part * 32 + lane) * kVec; k < d; k += 2 * kStep) {
-    const bool more = k + kStep < d;
+  for (int k = (part * 32 + lane) * kVec; k < d; k += 2 * step) {
+    const bool more = k + step < d;
     const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(x + k)), b0 = __ldg(reinterpret_cast<const uint4*>(w + k));
-    const uint4 a1 = more ? __ldg(reinterpret_cast<const uint4*>(x + k + kStep)) : zero;
-    const uint4 b1 = more ? __ldg(reinterpret_cast<const uint4*>(w + k + kStep)) : zero;
+    const uint4 a1 = more ? __ldg(reinterpret_cast<const uint4*>(x + k + step)) : zero;
+    const uint4 b1 = more ? __ldg(reinterpret_cast<const uint4*>(w + k + step)) : zero;
     dot_add(s, a0, b0, x);
     dot_add(s, a1, b1, x);
   }
@@ -397,7 +402,7 @@ struct Layout {
 };
 // full: all nkb blocks of the box lie inside the row (the same on all lanes); a lane without a token is
 // given some row whose values it may read.
-template <typename W, int kTerms>
+template <typename W, int kTerms, bool kCoherent>
 __device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row, size_t lo, bool full, int nkb, int live, int lane) {
   using L = Layout<W, kTerms>;
   const int t8 = (lane & 3) * 8 * L::kPer;
@@ -411,8 +416,8 @@ __device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row,
 #pragma unroll
       for (int q = 0; q < L::kPer; ++q) {
         const int k = i * W::kBlock + q * 8;
-        v[L::at(i, 0, q)] = ld_b(p + k * 2, true, kTerms == 2);
-        if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, true, true);
+        v[L::at(i, 0, q)] = ld_b(p + k * 2, true, kCoherent);
+        if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, true, kCoherent);
       }
     }
   } else {
@@ -421,8 +426,8 @@ __device__ __forceinline__ void load_vals(uint4 (&v)[kVals], const uint8_t* row,
 #pragma unroll
       for (int q = 0; q < L::kPer; ++q) {
         const int k = i * W::kBlock + q * 8;
-        v[L::at(i, 0, q)] = ld_b(p + k * 2, k < live, kTerms == 2);
-        if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, k < live, true);
+        v[L::at(i, 0, q)] = ld_b(p + k * 2, k < live, kCoherent);
+        if constexpr (kTerms == 2) v[L::at(i, 1, q)] = ld_b(pl + k * 2, k < live, kCoherent);
       }
   }
 }
@@ -528,13 +533,18 @@ __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync
 template <typename X, int SUB, typename S>
 __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
-  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), nd = a.T * R * kDotParts;
+  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), parts = a.T * R * kDotParts <= nw * G ? kDotParts : 1, nd = a.T * R * parts;
 #pragma unroll 1
   for (int q = cta + wi * G; q < nd; q += nw * G) {
-    const int part = q % kDotParts, t = q / kDotParts / R, r = q / kDotParts % R;
+    const int part = q % parts, t = q / parts / R, r = q / parts % R;
     const X* w = r < a.E ? reinterpret_cast<const X*>(a.w_router) + (size_t)r * a.d : reinterpret_cast<const X*>(a.w_gate);
-    const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, part, lane);
-    if (lane == 0) a.lg[(size_t)(t * kLgPitch + r) * kDotParts + part] = v;
+    const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, part, parts, lane);
+    double* o = a.lg + (size_t)(t * kLgPitch + r) * kDotParts;
+    if (parts != 1) {
+      if (lane == 0) o[part] = v;
+    } else if (lane < kDotParts) {
+      o[lane] = lane == 0 ? v : 0.0;
+    }
   }
   // fp8 weights, more than eight tokens: CTA t writes token t's row in f16 (eight or less: the compute
   // warps convert what they keep of it)
@@ -612,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using X = typename W::X;
   using F = Form<W, NT, SUB>;
   constexpr bool kF32 = F::kF32, kHalf = F::kHalf, kDirect = F::kDirect;
-  constexpr int kSub2 = F::kSub2, kHand = F::kHand;
+  constexpr int kSub2 = F::kSub2, kHand = F::kHand, kTerms = F::kTerms;
   static_assert(SUB == 1 || !kDirect, "units of 32 rows are for gathered tokens");
   extern __shared__ __align__(128) uint8_t smem_raw[];
   using S = Smem<W, NT, SUB>;
@@ -805,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         i = -1;
         n_tok = a.T;
       }
-      load_vals<W, 1>(v, x_row(i, n_tok, n + g, k), 0, k + a.b1 <= a.d, blk1, a.d - k, lane);
+      load_vals<W, 1, false>(v, x_row(i, n_tok, n + g, k), 0, k + a.b1 <= a.d, blk1, a.d - k, lane);
     };
     if constexpr (kDirect) {
       if (keep) {
@@ -1004,7 +1014,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (kDirect) n = i < 0 ? g : __popc(s.mask[i] & ((1u << g) - 1u));
       else n += g;
       const uint8_t* row = h_at(i, n < (i < 0 ? a.T : s.cnt[i]) ? n : 0, k);
-      load_vals<W, 2>(v, row, i < 0 ? hs_lo : h_lo, k + bk <= kend, i < 0 ? blk2s : blk2, kend - k, lane);
+      load_vals<W, kTerms, true>(v, row, i < 0 ? hs_lo : h_lo, k + bk <= kend, i < 0 ? blk2s : blk2, kend - k, lane);
     };
     for (int item = cta; item < items; item += G) {
       const int tile = item / a.splits, split = item % a.splits, per = kCompute * a.splits;
@@ -1093,7 +1103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int c = 0; c < 4; ++c) acc[q][c] = 0.0f;
             if (n0 > 0) load_h(v, i, n0, k);
-            box_mma<W, 2, kSub2>(acc, box(pitch), 8 * pitch, 16 * pitch, blk, v);
+            box_mma<W, kTerms, kSub2>(acc, box(pitch), 8 * pitch, 16 * pitch, blk, v);
             if constexpr (kDirect) {
               const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
               if (m & 1u) {
@@ -1219,11 +1229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if constexpr (kF32) {
                 reinterpret_cast<float*>(base)[at[i] + ch] = val;
               } else if constexpr (kHalf) {
-                const __half hi = __float2half_rn(val);
-                __half* o = reinterpret_cast<__half*>(base) + at[i] + ch;
-                o[0] = hi;
-                const float rest = val - __half2float(hi);
-                o[lo] = __float2half_rn(fabsf(val) <= 3.38e38f ? rest : 0.0f);
+                reinterpret_cast<__half*>(base)[at[i] + ch] = __float2half_rn(val);
               } else {
                 const __nv_bfloat16 hi = __float2bfloat16_rn(val);
                 const float rest = val - __bfloat162float(hi);
@@ -1415,8 +1421,8 @@ int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   // a stage holds whole 16-row tiles: the rows behind a tile's last are read, and dropped
   const int rows = 16 * max(SUB, F::kSub2), most = min(kMaxBox, (kSmem - kFixed) / (2 * kCompute * rows) / 64 * 64);
   a.b1 = box_of<W, 1>(a.d * W::kSize, kCompute, most) / W::kSize;
-  a.b2 = box_of<W, 2>(a.k2 * W::kSize, 1, most) / W::kSize;
-  a.b2s = box_of<W, 2>(a.k2s * W::kSize, 1, most) / W::kSize;
+  a.b2 = box_of<W, F::kTerms>(a.k2 * W::kSize, 1, most) / W::kSize;
+  a.b2s = box_of<W, F::kTerms>(a.k2s * W::kSize, 1, most) / W::kSize;
   a.n1 = (a.d + a.b1 - 1) / a.b1;
   a.n2 = (a.k2 + a.b2 - 1) / a.b2;
   a.n2s = (a.k2s + a.b2s - 1) / a.b2s;

@@ -4,14 +4,18 @@ Logits, expert ids and weights are compared bit for bit: the kernel sums the rou
 and its softmax, ties and weights are those of the block's routing oracle.  Tolerance of out, propagated from the inputs' magnitudes: a product sum of K terms is off by at most
 c * sum|terms|, c = (K / 8 + 32) * 2^-23 (a warp's chain is K / 8 / 16 tensor-core steps or K / 32 fused
 multiply-adds, then 8 partial sums and the activation's few operations; 2^-23 a step covers an
-accumulator that truncates).  The intermediate is held to 2^-17 of itself, |silu'| <= 1.1, the gate and
-the weighted products are off by 2^-19, and out is rounded once: eps / 2 of its type, relative."""
+accumulator that truncates).  The intermediate is held to 2^-17 of itself (two bf16
+terms, 2^-9 * 2^-9 and the first's sign; with fp8 weights one f16 term: half a step of 11 significant bits is
+2^-11 of the value), |silu'| <= 1.1, the gate and the weighted products are off by 2^-19, and out is
+rounded once: eps / 2 of its type, relative."""
 import pytest
 import torch
 
 from oracle import oracle as O
 
 pytestmark = pytest.mark.gpu
+
+H_EPS = {"bf16": 2.0 ** -17, "f32": 2.0 ** -17, "fp8": torch.finfo(torch.float16).eps / 2}
 
 
 def _weights(dev, d, E, I, Is, act, dtype, seed, std=0.03):
@@ -43,6 +47,7 @@ def _engine(dev, d, E, k, I, Is=0, act="swiglu", kind="bf16", norm=False, seed=1
     else:
         pe = pack_relu(w["gate"], w["down"], dtype=dtype, device=dev)
     w64 = {key: v.double() for key, v in w.items()}
+    w64["h_eps"] = H_EPS[kind]
     if kind == "fp8":
         pe = quantize_fp8(pe)
         for key, v in w.items():
@@ -66,7 +71,7 @@ def _route(x, router, k, top1, norm):
     return lg, torch.from_numpy(ids).long().to(x.device), torch.from_numpy(p).to(x.device)
 
 
-def _ffn(x, gate, up, down):
+def _ffn(x, gate, up, down, h_eps):
     """(result, its error bound before the last rounding) of one expert on rows x, in 64 bits."""
     d, I = gate.shape[1], gate.shape[0]
     c1, c2 = (d / 8 + 32) * 2.0 ** -23, (I / 8 + 32) * 2.0 ** -23
@@ -77,7 +82,7 @@ def _ffn(x, gate, up, down):
         u, eu = x @ up.T, c1 * (x.abs() @ up.abs().T)
         s = g * torch.sigmoid(g)
         h, eh = s * u, 1.1 * eg * (u.abs() + eu) + s.abs() * eu
-    eh = eh + 2.0 ** -17 * h.abs()
+    eh = eh + h_eps * h.abs()
     return h @ down.T, eh @ down.abs().T + c2 * (h.abs() @ down.abs().T)
 
 
@@ -91,12 +96,12 @@ def _check(r, x, w, router, gate, k, top1=False, norm=False):
     y, err = torch.zeros_like(xd), torch.zeros_like(xd)
     for e in ids.unique().tolist():
         t, j = (ids == e).nonzero(as_tuple=True)
-        o, eo = _ffn(xd[t], w["gate"][e], w["up"][e] if "up" in w else None, w["down"][e])
+        o, eo = _ffn(xd[t], w["gate"][e], w["up"][e] if "up" in w else None, w["down"][e], w["h_eps"])
         y.index_add_(0, t, p[t, j, None] * o)
         err.index_add_(0, t, p[t, j, None] * (eo + 2.0 ** -19 * o.abs()))
     if gate is not None:
         sg = torch.sigmoid((xd @ gate.double()).to(x.dtype).double())[:, None]
-        o, eo = _ffn(xd, w["s_gate"], w["s_up"], w["s_down"])
+        o, eo = _ffn(xd, w["s_gate"], w["s_up"], w["s_down"], w["h_eps"])
         y += sg * o
         err += sg * (eo + 2.0 ** -19 * o.abs())
     tol = torch.finfo(x.dtype).eps / 2 * (y.abs() + err) + err + 1e-30
