@@ -237,6 +237,7 @@ struct Smem {
   uint64_t full[kCompute][kMaxStages], empty[kCompute][kMaxStages];
   uint64_t part_full[kParts], part_empty[kParts];
   uint64_t routed;
+  bool last;                                // this CTA's sums of a tile were the last to come
   float wt[8 * NT * DSCA_MAX_TOPK];         // routing weights by assignment
   float sg[8 * NT];                         // shared-expert gate
   float xinv[8 * NT], hscale[8 * NT];       // fp8: 1 / scale of a token's row, scale of its intermediate
@@ -527,6 +528,32 @@ __device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, i
 
 // ---------------------------------------------------------------- the kernel
 __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kCompute * 32) : "memory"); }
+
+__device__ __forceinline__ void add(float4& c, float4 o) {
+  c.x += o.x; c.y += o.y; c.z += o.z; c.w += o.w;
+}
+// A lane's sums of a tile, the parts of its `splits` CTAs added in order.
+__device__ __forceinline__ float4 tile_sum(const float* all, int splits, int pitch) {
+  float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int v = 0; v < splits; ++v) add(r, __ldcg(reinterpret_cast<const float4*>(all + (size_t)v * pitch)));
+  return r;
+}
+// A lane's sums of 16-row tile q and token tile nt of an output tile.
+template <typename W, typename S>
+__device__ __forceinline__ void store_out(const Args& a, S& s, float4 v, int tile, int nt, int q, int lane) {
+  using X = typename W::X;
+  const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
+  X* out = reinterpret_cast<X*>(a.out);
+  const float c[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tk = nt * 8 + 2 * (lane & 3) + (i & 1), rr = 16 * q + (lane >> 2) + (i >> 1) * 8;
+    if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(W::kSize == 1 ? c[i] / s.hscale[tk] : c[i]);
+  }
+}
 
 // Router: fp64 dot products spread over the grid, then softmax, selection and the expert lists in every
 // CTA for itself.  Warp wi of the nw warps that take part (they share named barrier 1).
@@ -856,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         s.xmax[warp][g] = m;
         s.xsum[warp][g] = l1;
       }
-      asm volatile("bar.sync 2, %0;" ::"r"(kCompute * 32) : "memory");
+      compute_sync();
       m = 0u;
       l1 = 0.0f;
 #pragma unroll
@@ -1128,8 +1155,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i >= n_act) break;
         step(vb, va);
       }
-      if constexpr (kDirect) *reinterpret_cast<float4*>(p + lane * 4) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-      hand_over();
+      if constexpr (kDirect) {
+        *reinterpret_cast<float4*>(p + lane * 4) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        hand_over();
+      } else {
+        // The twelve warps' sums, a 16 x 8 tile a warp; no other work of this CTA is left to overlap with (few
+        // CTAs have a second item), and one finishing warp took 6 us longer over 32 tokens' eight tiles.
+        constexpr int kTiles = NT * kSub2;
+        float* all = a.partial + (size_t)tile * a.splits * kTiles * 128 + lane * 4;
+        compute_sync();
+        for (int q = warp; q < kTiles; q += kCompute) {
+          float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int w = 0; w < kCompute; ++w) add(c, *reinterpret_cast<const float4*>(s.sums[w][q / kSub2][q % kSub2][lane]));
+          if (a.splits == 1) store_out<W>(a, s, c, tile, q / kSub2, q % kSub2, lane);
+          else *reinterpret_cast<float4*>(all + (split * kTiles + q) * 128) = c;
+        }
+        if (a.splits > 1) {
+          __threadfence();
+          compute_sync();
+          if (threadIdx.x == 0) {
+            s.last = atomicAdd(a.ctr + kCtrTiles + tile, 1u) == (uint32_t)a.splits - 1u;
+            if (s.last) a.ctr[kCtrTiles + tile] = 0u;
+            __threadfence();
+          }
+          compute_sync();
+          if (s.last)
+            for (int q = warp; q < kTiles; q += kCompute)
+              store_out<W>(a, s, tile_sum(all + q * 128, a.splits, kTiles * 128), tile, q / kSub2, q % kSub2, lane);
+        }
+        compute_sync();
+      }
     }
   } else {
     // ================================================================ service
@@ -1258,66 +1314,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     announce(0, a.ctr + kCtrShared);
     announce(1, a.ctr + kCtrRouted);
-    // ---- the output's rows
-    for (int item = cta; item < items; item += G, ++seq) {
-      if (!mine()) continue;
-      const int tile = item / a.splits, r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
-      wait_parts();
-      X* out = reinterpret_cast<X*>(a.out);
-      auto sums = [&](int nt, int q, float (&c)[4]) {
-        c[0] = c[1] = c[2] = c[3] = 0.0f;
+    // ---- the output's rows, one 16 x 8 tile an item (else the compute warps store them)
+    if constexpr (kDirect) {
+      for (int item = cta; item < items; item += G, ++seq) {
+        if (!mine()) continue;
+        const int tile = item / a.splits;
+        wait_parts();
+        float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < kCompute; ++w) {
-          const float4 o = *reinterpret_cast<const float4*>(kDirect ? s.part[seq % kParts][w][0][0][lane] : s.sums[kDirect ? 0 : w][nt][q][lane]);
-          c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
-        }
-      };
-      auto store = [&](int nt, int q, const float (&c)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tk = nt * 8 + 2 * t4 + (i & 1), rr = 16 * q + g + (i >> 1) * 8;
-          if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(kHalf ? c[i] / s.hscale[tk] : c[i]);
-        }
-      };
-      if (a.splits == 1) {
-        for (int nt = 0; nt < NT; ++nt)
-          for (int q = 0; q < kSub2; ++q) {
-            float c[4];
-            sums(nt, q, c);
-            store(nt, q, c);
-          }
-        free_parts();
-      } else {
-        constexpr int kTile = NT * kSub2 * 128;
-        float* mine_at = a.partial + (size_t)item * kTile;
-        for (int nt = 0; nt < NT; ++nt)
-          for (int q = 0; q < kSub2; ++q) {
-            float c[4];
-            sums(nt, q, c);
-            *reinterpret_cast<float4*>(mine_at + (nt * kSub2 + q) * 128 + lane * 4) = make_float4(c[0], c[1], c[2], c[3]);
-          }
-        free_parts();
-        // the last of the CTAs that share the tile adds their sums, in order
-        uint32_t before = 0u;
-        if (lane == 0) {
+        for (int w = 0; w < kCompute; ++w) add(c, *reinterpret_cast<const float4*>(s.part[seq % kParts][w][0][0][lane]));
+        if (a.splits == 1) {
+          store_out<W>(a, s, c, tile, 0, 0, lane);
+          free_parts();
+        } else {
+          float* all = a.partial + (size_t)tile * a.splits * 128 + lane * 4;
+          *reinterpret_cast<float4*>(all + item % a.splits * 128) = c;
+          free_parts();
           __threadfence();
-          before = atomicAdd(a.ctr + kCtrTiles + tile, 1u);
-          __threadfence();
-        }
-        before = __shfl_sync(0xffffffffu, before, 0);
-        if (before == (uint32_t)a.splits - 1u) {
-          const float* all = a.partial + (size_t)tile * a.splits * kTile;
-          for (int nt = 0; nt < NT; ++nt)
-            for (int q = 0; q < kSub2; ++q) {
-              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-              for (int v = 0; v < a.splits; ++v) {
-                const float4 o = __ldcg(reinterpret_cast<const float4*>(all + (size_t)v * kTile + (nt * kSub2 + q) * 128 + lane * 4));
-                c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
-              }
-              store(nt, q, c);
-            }
-          if (lane == 0) a.ctr[kCtrTiles + tile] = 0u;
+          __syncwarp();
+          uint32_t before = 0u;
+          if (lane == 0) before = atomicAdd(a.ctr + kCtrTiles + tile, 1u);
+          before = __shfl_sync(0xffffffffu, before, 0);
+          if (before == (uint32_t)a.splits - 1u) {
+            __threadfence();
+            store_out<W>(a, s, tile_sum(all, a.splits, 128), tile, 0, 0, lane);
+            if (lane == 0) a.ctr[kCtrTiles + tile] = 0u;
+          }
         }
       }
     }
