@@ -905,6 +905,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         halve(vb);
       }
     }
+    int holds = -1;  // active expert whose values are in va and vb
     int nu_r = 0, ai = -1, r = 0;  // routed units of this CTA; active expert and number of the present one
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
       if (ul == nu_s) {
@@ -931,37 +932,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (SUB == 2) {
         // one box a warp and unit; the expert's tokens eight at a time
         const bool stay = n_tok <= 8 && ai >= 0 && ul + 1 < nu_s + nu_r && r + 1 < (ai + 1) * a.upe;
-        auto unit = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
-          const bool has = warp < a.n1;
-          for (int n0 = 0; n0 < n_tok; n0 += 8) {
-            float acc[SUB][4];
+        const bool has = warp < a.n1;
+        auto group = [&](int n0, uint4 (&v)[kVals], uint4 (&w)[kVals]) {
+          const bool last = n0 + 8 >= n_tok;
+          float acc[SUB][4];
+#pragma unroll
+          for (int q = 0; q < SUB; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[q][i] = 0.0f;
+          if (has) {
+            if (!ready) load_x(v, ai, n_tok, n0, warp * a.b1);
+            // the same values again, if the next unit is of the same expert
+            ready = !last || stay;
+            if (!last) load_x(w, ai, n_tok, n0 + 8, warp * a.b1);
+            else if (!stay) ahead(w);
+            if (n0 == 0) arrived();
+            box_mma<W, 1, SUB>(acc, box(pitch1), up1, sub1, blk1, v);
+            if (last) release();
+          }
+          float* p = buffer();
+          if (has) {
 #pragma unroll
             for (int q = 0; q < SUB; ++q)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[q][i] = 0.0f;
-            if (has) {
-              if (n0 > 0 || !ready) load_x(v, ai, n_tok, n0, warp * a.b1);
-              if (n0 == 0) {
-                // the same values again, if the next unit is of the same expert
-                ready = stay;
-                if (!stay) ahead(w);
-                arrived();
-              }
-              box_mma<W, 1, SUB>(acc, box(pitch1), up1, sub1, blk1, v);
-              if (n0 + 8 >= n_tok) release();
-            }
-            float* p = buffer();
-            if (has) {
-#pragma unroll
-              for (int q = 0; q < SUB; ++q)
-                *reinterpret_cast<float4*>(p + (q * 32 + lane) * 4) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
-            }
-            hand_over();
+              *reinterpret_cast<float4*>(p + (q * 32 + lane) * 4) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
           }
+          hand_over();
+          if (!last || !stay) flip = !flip;
         };
-        if (flip) unit(vb, va);
-        else unit(va, vb);
-        if (!stay) flip = !flip;
+        for (int n0 = 0; n0 < n_tok; n0 += 8) {
+          if (flip) group(n0, vb, va);
+          else group(n0, va, vb);
+        }
       } else {
         float acc[NT][1][4];
 #pragma unroll
@@ -984,25 +985,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             if (!ready) load_x(v, ai, n_tok, 0, k);
             ready = false;
-            if (j + kCompute < a.n1) {
-              load_x(w, ai, n_tok, 0, k + kCompute * a.b1);
-              ready = true;
-            } else {
-              ahead(w);
-            }
-            arrived();
-            if constexpr (kDirect && kHalf) halve(v);
-            box_mma<W, 1, 1>(acc[0], box(pitch1), up1, 0, blk1, v);
 #pragma unroll
-            for (int nt = 1; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt) {
               if (nt * 8 >= n_tok) break;
-              load_x(v, ai, n_tok, nt * 8, k);
-              box_mma<W, 1, 1>(acc[nt], box(pitch1), up1, 0, blk1, v);
+              uint4(&now)[kVals] = nt % 2 == 0 ? v : w;
+              uint4(&then)[kVals] = nt % 2 == 0 ? w : v;
+              if (nt * 8 + 8 < n_tok) {
+                load_x(then, ai, n_tok, nt * 8 + 8, k);
+              } else if (j + kCompute < a.n1) {
+                load_x(then, ai, n_tok, 0, k + kCompute * a.b1);
+                ready = true;
+              } else {
+                ahead(then);
+              }
+              if (nt == 0) arrived();
+              if constexpr (kDirect && kHalf) halve(now);
+              box_mma<W, 1, 1>(acc[nt], box(pitch1), up1, 0, blk1, now);
+              flip = !flip;
             }
           }
           release();
         };
-        if (keep) {
+        // the boxes of an expert's unit, the same values again in the next one
+        bool held = keep;
+        if constexpr (!kDirect && !kF32) {
+          held = ai >= 0 && n_tok <= 8 && a.n1 <= 2 * kCompute;
+          if (held && ai != holds) {
+            if (warp < a.n1) load_x(va, ai, n_tok, 0, warp * a.b1);
+            if (warp + kCompute < a.n1) load_x(vb, ai, n_tok, 0, (warp + kCompute) * a.b1);
+          }
+          holds = held ? ai : -1;
+          ready = ready && !held;
+        }
+        if (held) {
           if (warp < a.n1) {
             arrived();
             box_mma<W, 1, 1>(acc[0], box(pitch1), up1, 0, blk1, va);
@@ -1017,7 +1032,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = warp; j < a.n1; j += kCompute) {
             if (flip) step(j, vb, va);
             else step(j, va, vb);
-            flip = !flip;
           }
         }
         float* p = buffer();
@@ -1072,7 +1086,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       ready = false;
-      int i = -1, j = warp * a.splits + split;
+      int i = -1, j = warp * a.splits + split, n0 = 0;  // the tokens eight at a time
       seek(i, j);
       auto step = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const bool sh = i < 0;
@@ -1086,8 +1100,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
         const int n_tok = sh ? a.T : s.cnt[i];
-        int ni = i, nj = j + per;
-        seek(ni, nj);
+        const bool last = kF32 || n0 + 8 >= n_tok;
+        int ni = i, nj = j, nn = n0 + 8;
+        if (last) {
+          nn = 0;
+          nj += per;
+          seek(ni, nj);
+        }
         float sc[kSub2][2];  // fp8: every (expert, row) has its own scale
 #pragma unroll
         for (int q = 0; q < kSub2; ++q) {
@@ -1122,38 +1141,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             join(acc, n0);
           }
         } else {
-          if (!ready) load_h(v, i, 0, k);
+          if (!ready) load_h(v, i, n0, k);
           ready = ni < n_act && (ni < 0 || have_r);
-          if (ready) load_h(w, ni, 0, nj * (ni < 0 ? a.b2s : a.b2));
-          arrived();
-          for (int n0 = 0; n0 < n_tok; n0 += 8) {
-            // a box's sums join by the same operations in both forms: a token's result does not depend on
-            // how many others there are
-            float acc[kSub2][4];
+          if (ready) load_h(w, ni, nn, nj * (ni < 0 ? a.b2s : a.b2));
+          if (n0 == 0) arrived();
+          // a box's sums join by the same operations in both forms: a token's result does not depend on
+          // how many others there are
+          float acc[kSub2][4];
 #pragma unroll
-            for (int q = 0; q < kSub2; ++q)
+          for (int q = 0; q < kSub2; ++q)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) acc[q][c] = 0.0f;
-            if (n0 > 0) load_h(v, i, n0, k);
-            box_mma<W, kTerms, kSub2>(acc, box(pitch), 8 * pitch, 16 * pitch, blk, v);
-            if constexpr (kDirect) {
-              const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
-              if (m & 1u) {
-                sum[0] = fmaf(acc[0][0], sc[0][0], sum[0]);
-                sum[2] = fmaf(acc[0][2], sc[0][1], sum[2]);
-              }
-              if (m & 2u) {
-                sum[1] = fmaf(acc[0][1], sc[0][0], sum[1]);
-                sum[3] = fmaf(acc[0][3], sc[0][1], sum[3]);
-              }
-            } else {
-              join(acc, n0);
+            for (int c = 0; c < 4; ++c) acc[q][c] = 0.0f;
+          box_mma<W, kTerms, kSub2>(acc, box(pitch), 8 * pitch, 16 * pitch, blk, v);
+          if constexpr (kDirect) {
+            const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
+            if (m & 1u) {
+              sum[0] = fmaf(acc[0][0], sc[0][0], sum[0]);
+              sum[2] = fmaf(acc[0][2], sc[0][1], sum[2]);
             }
+            if (m & 2u) {
+              sum[1] = fmaf(acc[0][1], sc[0][0], sum[1]);
+              sum[3] = fmaf(acc[0][3], sc[0][1], sum[3]);
+            }
+          } else {
+            join(acc, n0);
           }
         }
-        release();
+        if (last) release();
         i = ni;
         j = nj;
+        n0 = nn;
       };
       while (i < n_act) {
         step(va, vb);
