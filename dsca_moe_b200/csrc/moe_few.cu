@@ -245,11 +245,14 @@ struct Smem {
   float xsum[kCompute][8];
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
   uint8_t act[DSCA_MAX_EXPERTS];            // experts with tokens ("active"), ascending
-  uint8_t cnt[DSCA_MAX_EXPERTS];            // tokens of active expert i
+  // active expert i: its number, how many tokens it has (bits 8 ..), the compute warp that its first box
+  // of GEMM2 goes to (bits 16 ..)
+  uint32_t info[DSCA_MAX_EXPERTS];
   uint32_t mask[DSCA_MAX_EXPERTS];          // and which
-  uint8_t turn[DSCA_MAX_EXPERTS];           // the compute warp that its first box of GEMM2 goes to
-  uint8_t tok[DSCA_MAX_EXPERTS][8 * NT];    // its n-th token
-  uint8_t asg[DSCA_MAX_EXPERTS][8 * NT];    // and that assignment: token * k + choice, the row of h
+  // Its n-th token, and that assignment: token * k + choice, the row of h (kDirect: that of token n).  Where there
+  // is none, the first's: what is read for it is dropped.
+  uint8_t tok[DSCA_MAX_EXPERTS][8 * NT];
+  uint8_t asg[DSCA_MAX_EXPERTS][8 * NT];
   uint8_t slot[DSCA_MAX_EXPERTS][8 * NT];   // choice of (expert, token)
   int n_act;
   uint32_t handed;                          // routed units' handings over, all CTAs'
@@ -557,7 +560,7 @@ __device__ __forceinline__ void store_out(const Args& a, S& s, float4 v, int til
 
 // Router: fp64 dot products spread over the grid, then softmax, selection and the expert lists in every
 // CTA for itself.  Warp wi of the nw warps that take part (they share named barrier 1).
-template <typename X, int SUB, typename S>
+template <typename X, int SUB, int kTokens, bool kDirect, typename S>
 __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
   const int R = a.E + (a.w_gate != nullptr ? 1 : 0), parts = a.T * R * kDotParts <= nw * G ? kDotParts : 1, nd = a.T * R * parts;
@@ -628,14 +631,16 @@ __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int l
     const int e = s.act[i];
     const uint32_t m = s.emask[e];
     if (lane == 0) {
-      s.cnt[i] = (uint8_t)__popc(m);
       s.mask[i] = m;
-      s.turn[i] = (uint8_t)(e * ((a.n2 + a.splits - 1) / a.splits) % kCompute);
+      s.info[i] = (uint32_t)e | (uint32_t)__popc(m) << 8 | (uint32_t)(e * ((a.n2 + a.splits - 1) / a.splits) % kCompute) << 16;
     }
-    if ((m >> lane) & 1u) {
-      const int n = __popc(m & ((1u << lane) - 1u));
-      s.tok[i][n] = (uint8_t)lane;
-      s.asg[i][n] = (uint8_t)(lane * a.k + s.slot[e][lane]);
+    const uint32_t below = (1u << lane) - 1u;
+    const bool on = (m >> lane) & 1u;
+    const int t = on ? lane : __ffs(m) - 1;
+    const int n = kDirect ? lane : (on ? __popc(m & below) : __popc(m) + __popc(~m & below));
+    if (n < kTokens) {
+      s.tok[i][n] = (uint8_t)t;
+      s.asg[i][n] = (uint8_t)(t * a.k + s.slot[e][t]);
     }
   }
   group_sync(nw * 32);
@@ -691,8 +696,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     return int2{cta * (units / G) + max(0, more), units / G + (more >= 0)};  // the first of them, and how many
   };
   auto wait_routed = [&]() { mbar_wait(smem_u32(&s.routed), 0u, abort_flag, a.err); };
-  // warp w's first box (of this item's) of active expert i
-  auto first_box = [&](int w, int i) { return w - s.turn[i] + (w < s.turn[i] ? kCompute : 0); };
+  // warp w's first box (of this item's) of an active expert
+  auto first_box = [&](int w, uint32_t info) {
+    const int b = w - (int)(info >> 16);
+    return b < 0 ? b + kCompute : b;
+  };
   // The router runs on the service warps while the compute warps begin with the shared expert; on all
   // of them where there is no shared expert to begin with, or where the tokens are more than two
   // warps would do in the time of the first boxes.
@@ -779,7 +787,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &ms2, bar, j * a.b2s, tile * a.rt); });
       }
       for (int i = 0; i < n_act; ++i) {
-        const int e = s.act[i], fb = first_box(w, i);
+        const uint32_t info = s.info[i];
+        const int e = info & 255u, fb = first_box(w, info);
         for (int j0 = 0; j0 < a.n2; j0 += per) {
           const int j = j0 + fb * a.splits + split;
           box(on && j < a.n2, a.rt * a.b2 * W::kSize,
@@ -797,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < kCompute) {
     // ================================================================ compute
-    if (all_route) route<X, SUB>(a, s, kServices + warp, route_warps, lane);
+    if (all_route) route<X, SUB, 8 * NT, kDirect>(a, s, kServices + warp, route_warps, lane);
     const uint32_t base = ring + (uint32_t)(warp * a.stages * a.stage);
     int st = 0, given = 0;  // next stage, sums handed over
     uint32_t phase = 0u;    // parity of the next stage's copy
@@ -836,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool flip = false;           // and whether they are in vb
     // row n of active expert i's tokens (i < 0: of all) from k on; one of them where there is no such token
     auto x_row = [&](int i, int n_tok, int n, int k) {
-      n = n < n_tok ? n : 0;
+      if (i < 0) n = min(n, n_tok - 1);
       return reinterpret_cast<const uint8_t*>(kHalf && !kDirect ? a.x16 : a.x) +
              ((size_t)(i < 0 ? n : (int)s.tok[i][n]) * a.d + k) * sizeof(X);
     };
@@ -920,12 +929,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++r;
         if (r == (ai + 1) * a.upe) ++ai;
       }
-      const int n_tok = ai < 0 ? a.T : s.cnt[ai];
+      const int n_tok = ai < 0 ? a.T : (int)(s.info[ai] >> 8 & 255u);
       // asks for the values of the next unit's first box of this warp, if that unit is known
       auto ahead = [&](uint4 (&w)[kVals]) {
         if (ul + 1 < (ai < 0 ? nu_s : nu_s + nu_r)) {
           const int i = ai >= 0 && r + 1 == (ai + 1) * a.upe ? ai + 1 : ai;
-          load_x(w, i, i < 0 ? a.T : s.cnt[i], 0, warp * a.b1);
+          load_x(w, i, i < 0 ? a.T : (int)(s.info[i] >> 8 & 255u), 0, warp * a.b1);
           ready = true;
         }
       };
@@ -1056,19 +1065,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto load_h = [&](uint4 (&v)[kVals], int i, int n, int k) {
       const int kend = i < 0 ? a.k2s : a.k2, bk = i < 0 ? a.b2s : a.b2;
-      // token g's place among the expert's tokens
-      if constexpr (kDirect) n = i < 0 ? g : __popc(s.mask[i] & ((1u << g) - 1u));
-      else n += g;
-      const uint8_t* row = h_at(i, n < (i < 0 ? a.T : s.cnt[i]) ? n : 0, k);
+      const uint8_t* row = h_at(i, i < 0 ? min(n + g, a.T - 1) : n + g, k);
       load_vals<W, kTerms, true>(v, row, i < 0 ? hs_lo : h_lo, k + bk <= kend, i < 0 ? blk2s : blk2, kend - k, lane);
     };
     for (int item = cta; item < items; item += G) {
       const int tile = item / a.splits, split = item % a.splits, per = kCompute * a.splits;
       // this warp's first box at or behind (segment i, box j)
-      auto seek = [&](int& i, int& j) {
+      auto seek = [&](int& i, int& j, uint32_t& info) {
         while (i < n_act && j >= (i < 0 ? a.n2s : a.n2)) {
           ++i;
-          if (i < n_act) j = first_box(warp, i) * a.splits + split;
+          if (i < n_act) {
+            info = s.info[i];
+            j = first_box(warp, info) * a.splits + split;
+          }
         }
       };
       const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
@@ -1087,7 +1096,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ready = false;
       int i = -1, j = warp * a.splits + split, n0 = 0;  // the tokens eight at a time
-      seek(i, j);
+      uint32_t info = 0u;
+      seek(i, j, info);
       auto step = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const bool sh = i < 0;
         if (sh ? !have_s : !have_r) {
@@ -1099,20 +1109,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (sh) have_s = true; else have_r = true;
         }
         const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
-        const int n_tok = sh ? a.T : s.cnt[i];
+        const int n_tok = sh ? a.T : (int)(info >> 8 & 255u);
+        uint32_t next = info;
         const bool last = kF32 || n0 + 8 >= n_tok;
         int ni = i, nj = j, nn = n0 + 8;
         if (last) {
           nn = 0;
           nj += per;
-          seek(ni, nj);
+          seek(ni, nj, next);
         }
         float sc[kSub2][2];  // fp8: every (expert, row) has its own scale
 #pragma unroll
         for (int q = 0; q < kSub2; ++q) {
           sc[q][0] = sc[q][1] = 1.0f;
           if constexpr (kHalf) {
-            const float* f = (sh ? a.ws2s : a.w2s + (size_t)s.act[i] * a.dp) + r0;
+            const float* f = (sh ? a.ws2s : a.w2s + (size_t)(info & 255u) * a.dp) + r0;
             sc[q][0] = __ldg(f + min(16 * q + g, rows - 1));
             sc[q][1] = __ldg(f + min(16 * q + g + 8, rows - 1));
           }
@@ -1171,6 +1182,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         i = ni;
         j = nj;
         n0 = nn;
+        info = next;
       };
       while (i < n_act) {
         step(va, vb);
@@ -1212,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================================================ service
     const int sw = warp - kService;
-    route<X, SUB>(a, s, sw, route_warps, lane);
+    route<X, SUB, 8 * NT, kDirect>(a, s, sw, route_warps, lane);
     wait_routed();
     const int2 ru = routed_units(s.n_act);
     const int nu = nu_s + ru.y;
@@ -1245,7 +1257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++ai;
         }
       const int u = sh ? cta + un * G : r - first, e = sh ? 0 : s.act[ai];
-      const int n_tok = sh ? a.T : s.cnt[ai];
+      const int n_tok = sh ? a.T : (int)(s.info[ai] >> 8 & 255u);
       for (int h0 = 0; h0 < (kHand < NT ? n_tok : 1); h0 += 8, ++seq) {
         if (!mine()) continue;
         // where these sums go is looked up before they are there
@@ -1275,14 +1287,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           int tok[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            int n = n0 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
+            const int n = n0 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
             on[i] = n < (kDirect ? a.T : n_tok);
-            if constexpr (kDirect) {
-              on[i] = on[i] && ((mask >> n) & 1u);
-              if (!sh) n = __popc(mask & ((1u << n) - 1u));
-            }
+            if constexpr (kDirect) on[i] = on[i] && ((mask >> n) & 1u);
             const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
-            tok[i] = on[i] ? (sh ? n : (int)s.tok[ai][n]) : 0;
+            tok[i] = on[i] ? (sh || kDirect ? n : (int)s.tok[ai][n]) : 0;
             wt[i] = sh ? s.sg[row] : s.wt[row];
             at[i] = (size_t)row * (sh ? a.hsp : a.hp);
           }
