@@ -101,6 +101,7 @@ struct Args {
   int k2, k2s;            // values of a row of w2 / ws2 that are read
   int b1, b2, b2s;        // values of a row in a box: GEMM1, routed and shared GEMM2
   int n1, n2, n2s;        // boxes of a row
+  int n2_cta;             // boxes of a row of w2 for one of the CTAs that share a tile, rounded up
   int rt, tiles, splits;  // rows of a GEMM2 tile, tiles, CTAs that share one
   float* partial;         // their sums: [tiles * splits][tokens in eights][kSub2][32][4]
   int stage, stages;      // bytes of a stage, stages of a warp's ring
@@ -320,11 +321,13 @@ __device__ __forceinline__ float ord_val(uint32_t k) {
 // results.  dry: nothing is read or written (the code only comes into the instruction cache, in the
 // time that the logits of other CTAs take: see dot64).
 template <typename X, typename S>
-__device__ __forceinline__ void select_token(const Args& a, S& s, int t, bool dry, int lane) {
+__device__ __forceinline__ void select_token(const Args& a, S& s, int t, int parts, bool dry, int lane) {
   const int E = a.E, e0 = lane, e1 = lane + 32;
   auto logit = [&](int e) {
     if (dry) return 0.0f;
-    const double2* p = reinterpret_cast<const double2*>(a.lg + (size_t)(t * kLgPitch + e) * kDotParts);
+    const double* q = a.lg + (size_t)(t * kLgPitch + e) * parts;
+    if (parts == 1) return round_to<X>(__ldcg(q));
+    const double2* p = reinterpret_cast<const double2*>(q);
     const double2 u = __ldcg(p), v = __ldcg(p + 1);
     return round_to<X>((u.x + u.y) + (v.x + v.y));
   };
@@ -569,18 +572,14 @@ __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int l
     const int part = q % parts, t = q / parts / R, r = q / parts % R;
     const X* w = r < a.E ? reinterpret_cast<const X*>(a.w_router) + (size_t)r * a.d : reinterpret_cast<const X*>(a.w_gate);
     const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, part, parts, lane);
-    double* o = a.lg + (size_t)(t * kLgPitch + r) * kDotParts;
-    if (parts != 1) {
-      if (lane == 0) o[part] = v;
-    } else if (lane < kDotParts) {
-      o[lane] = lane == 0 ? v : 0.0;
-    }
+    if (lane == 0) a.lg[(size_t)(t * kLgPitch + r) * parts + part] = v;
   }
-  // fp8 weights, more than eight tokens: CTA t writes token t's row in f16 (eight or less: the compute
-  // warps convert what they keep of it)
-  if (a.x16 != nullptr && cta < a.T && wi == nw - 1) {
-    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const X*>(a.x) + (size_t)cta * a.d);
-    uint4* dst = reinterpret_cast<uint4*>(a.x16) + (size_t)cta * (a.d / 8);
+  // fp8 weights, more than eight tokens: the t-th last CTA (the first have one dot product
+  // more) writes token t's row in f16 (eight or less: the compute warps convert what they keep of it)
+  const int counted = a.x16 != nullptr ? G : min(nd, G);  // CTAs that have a part in this
+  for (int tc = G - 1 - cta; a.x16 != nullptr && wi == nw - 1 && tc < a.T; tc += G) {
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const X*>(a.x) + (size_t)tc * a.d);
+    uint4* dst = reinterpret_cast<uint4*>(a.x16) + (size_t)tc * (a.d / 8);
     uint32_t m = 0u;
     float l1 = 0.0f;
 #pragma unroll 4
@@ -592,20 +591,20 @@ __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int l
 #pragma unroll 4
     for (int c = lane; c < a.d / 8; c += 32) dst[c] = to_f16(__ldg(src + c), pow2(e));
     if (lane == 0) {
-      a.xmeta[2 * cta] = pow2(-e);
-      a.xmeta[2 * cta + 1] = l1;
+      a.xmeta[2 * tc] = pow2(-e);
+      a.xmeta[2 * tc + 1] = l1;
     }
   }
   group_sync(nw * 32);
-  if (wi == 0 && lane == 0 && cta < nd) ctr_add(a.ctr + kCtrLogits, 1u);
+  if (wi == 0 && lane == 0 && cta < counted) ctr_add(a.ctr + kCtrLogits, 1u);
   __syncwarp();
   for (int t = wi - nw; t < a.T; t += nw) {
     if (t >= 0 && t < nw) {
-      if (wi == 0 && lane == 0) ctr_wait(a.ctr + kCtrLogits, (uint32_t)min(nd, G), &s.abort, a.err);
+      if (wi == 0 && lane == 0) ctr_wait(a.ctr + kCtrLogits, (uint32_t)counted, &s.abort, a.err);
       __syncwarp();
       group_sync(nw * 32);
     }
-    select_token<X>(a, s, max(t, 0), t < 0, lane);
+    select_token<X>(a, s, max(t, 0), parts, t < 0, lane);
   }
   if (wi >= a.T) {  // no token for this warp: the same barrier
     group_sync(nw * 32);
@@ -632,7 +631,7 @@ __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int l
     const uint32_t m = s.emask[e];
     if (lane == 0) {
       s.mask[i] = m;
-      s.info[i] = (uint32_t)e | (uint32_t)__popc(m) << 8 | (uint32_t)(e * ((a.n2 + a.splits - 1) / a.splits) % kCompute) << 16;
+      s.info[i] = (uint32_t)e | (uint32_t)__popc(m) << 8 | (uint32_t)(e * a.n2_cta % kCompute) << 16;
     }
     const uint32_t below = (1u << lane) - 1u;
     const bool on = (m >> lane) & 1u;
@@ -1480,6 +1479,7 @@ int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   a.n1 = (a.d + a.b1 - 1) / a.b1;
   a.n2 = (a.k2 + a.b2 - 1) / a.b2;
   a.n2s = (a.k2s + a.b2s - 1) / a.b2s;
+  a.n2_cta = (a.n2 + a.splits - 1) / a.splits;
   if (SUB == 2 && a.n1 > kCompute) return DSCA_ERR_CAPACITY;
   const int bytes = max(16 * SUB * a.b1, 16 * F::kSub2 * max(a.b2, a.n2s ? a.b2s : 0)) * W::kSize;
   a.stage = (bytes + 127) / 128 * 128;
