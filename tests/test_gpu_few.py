@@ -129,6 +129,17 @@ def test_swiglu(cuda, T, d, E, k, I, Is, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
+@pytest.mark.parametrize("T,d,E,k,I,Is", [(3, 5120, 6, 2, 72, 40), (12, 5120, 6, 2, 72, 40), (24, 8192, 4, 2, 40, 16),
+                                          (16, 256, 2, 1, 4096, 0), (32, 512, 3, 2, 3000, 1000), (20, 1152, 40, 3, 500, 0)])
+def test_swiglu_long_rows_and_many_units(cuda, T, d, E, k, I, Is, kind):
+    """Rows of more boxes than a warp keeps values of; consecutive units of one expert, with at most eight
+    tokens and with more, and of the next one."""
+    eng, w, router, gate, n = _engine(cuda, d, E, k, I, Is, kind=kind, seed=T + d)
+    x = n(T, d, std=1.0)
+    _check(_run(eng, x), x, w, router, gate, k)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
 @pytest.mark.parametrize("T,d,E,F", [(1, 768, 64, 512), (6, 64, 3, 17), (16, 768, 64, 1000), (32, 272, 10, 2048)])
 def test_switch(cuda, T, d, E, F, kind):
     eng, w, router, gate, n = _engine(cuda, d, E, 1, F, act="relu", kind=kind, seed=T + d)
