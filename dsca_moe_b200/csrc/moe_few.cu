@@ -134,14 +134,14 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -566,7 +566,10 @@ __device__ __forceinline__ void store_out(const Args& a, S& s, float4 v, int til
 template <typename X, int SUB, int kTokens, bool kDirect, typename S>
 __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
-  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), parts = a.T * R * kDotParts <= nw * G ? kDotParts : 1, nd = a.T * R * parts;
+  // a logit's product in four parts while that leaves a warp one (one token of the Qwen block 32.7 us, whole
+  // 34.6), else whole (32 tokens with fp8 weights 130 us, four parts 133)
+  const int R = a.E + (a.w_gate != nullptr ? 1 : 0), parts = a.T * R * kDotParts <= nw * G ? kDotParts : 1;
+  const int nd = a.T * R * parts;
 #pragma unroll 1
   for (int q = cta + wi * G; q < nd; q += nw * G) {
     const int part = q % parts, t = q / parts / R, r = q / parts % R;
@@ -702,7 +705,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // The router runs on the service warps while the compute warps begin with the shared expert; on all
   // of them where there is no shared expert to begin with, or where the tokens are more than two
-  // warps would do in the time of the first boxes.
+  // warps would do in the time of the first boxes (two warps, all: one token 32.7 us, 35.6; eight 103.6, 97.1;
+  // 32 with fp8 weights 167, 132).
   const bool all_route = a.ups == 0 || a.T > 4;
   const int route_warps = all_route ? kCompute + kServices : kServices;
 
@@ -1014,7 +1018,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           release();
         };
-        // the boxes of an expert's unit, the same values again in the next one
+        // the boxes of an expert's unit, the same values again in the next one (20 tokens of the Qwen block in
+        // bf16: 216 us; asked for anew 232)
         bool held = keep;
         if constexpr (!kDirect && !kF32) {
           held = ai >= 0 && n_tok <= 8 && a.n1 <= 2 * kCompute;
@@ -1443,12 +1448,13 @@ int box_of(int bytes, int warps, int most) {
   return best;
 }
 
-// Output rows of a tile and CTAs that share one (see the top): CTAs of their own for at least nine rows
-// (gathered tokens: 24) each, else tiles of 16 (32) rows and as many CTAs to each as there are.
-// Gathered tokens, 28 rows by 2 CTAs against 14 by one: 32 tokens of the Qwen block with fp8 weights.
+// Output rows of a tile and CTAs that share one (see the top): tiles of `high` rows at most, as many CTAs to
+// each as there are.  Against tiles for one CTA each: 32 tokens of the Qwen block with fp8 weights (28 rows
+// by 2 CTAs, not 14 by one) 132 us, 165; 16 tokens of a Switch block of 768 (32 rows by 6, not 6 by one)
+// 37 us, 58; one token of it 15.4 us, 15.9.
 inline void plan_tiles(int d, int sms, int high, int* rt, int* tiles, int* splits) {
-  const int per = (d + sms - 1) / sms, full = (d + high - 1) / high;
-  *splits = per * 4 > high * 2 + high ? 1 : max(1, sms / full);
+  const int full = (d + high - 1) / high;
+  *splits = max(1, sms / full);
   const int ctas = sms / *splits, nt = ((d + ctas - 1) / ctas + high - 1) / high;
   *rt = (d + ctas * nt - 1) / (ctas * nt);
   *tiles = (d + *rt - 1) / *rt;
@@ -1512,7 +1518,8 @@ template <typename W>
 int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   if (a.T <= 8) return launch<W, 1, 1>(a, p, sms, stream);
   if constexpr (W::kSize != 4) {
-    // units of 32 rows: one box of at most 192 bytes a warp
+    // units of 32 rows: one box of at most 192 bytes a warp (against 16 rows: 32 tokens of the Qwen block with
+    // fp8 weights 132 us, 165; 16 of the Switch block of 768 36.5 us, 40.4)
     if (a.d * W::kSize <= 192 * kCompute) {
       if (a.T <= 16) return launch<W, 2, 2>(a, p, sms, stream);
       return launch<W, 4, 2>(a, p, sms, stream);

@@ -433,7 +433,8 @@ class MoEEngine:
         self._ws = {}
         # forward() runs calls of at most this many tokens through the one-kernel form where that
         # supports the block (forward_few); 0 = never.  Results then differ from the other path's by
-        # its roundings (the intermediates and expert outputs are not rounded to bf16 here)
+        # its roundings (the intermediates and expert outputs are not rounded to bf16 here) and hold no
+        # counts, token_row or other views of the scratch
         self.few_tokens = 0
         self._few_ws = {}
         self._few_args = None
@@ -720,6 +721,8 @@ class MoEEngine:
             return "it runs on one GPU"
         if self.cache is not None:
             return "the experts must be resident"
+        if self.E + (self.shared_gate_weight is not None) > L.MAX_EXPERTS:
+            return f"more than {L.MAX_EXPERTS} logits, the shared expert's gate among them"
         esz = 1 if self.experts.fp8 else (2 if self.dtype == torch.bfloat16 else 4)
         if self.d * esz % 16:
             return f"a weight row of {self.d} values is not a multiple of 16 bytes"

@@ -58,7 +58,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     the unrounded y (the row format of the fp8 expert weights); "split" (bf16, d % 8 == 0): q
     [rows, 2 * ceil(d / 128) * 128], the two-term rows of dsca_split_rows with scale = 1 / s, the token
     operand of the fp8-weight experts.  write_y=False leaves y out when only the 8-bit rows are
-    wanted.  Runs on x's device, on its current stream."""
+    wanted.  Runs on x's device, on its current stream.  Inference only: the results carry no
+    gradient."""
     dtype, dev, shape = x.dtype, x.device, x.shape
     dt, q_mode = _DTYPES.get(dtype), _QUANT.get(quant)
     if dt is None:

@@ -61,7 +61,7 @@ DSCA_API int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream);
  * dsca_grouped_ffn and dsca_combine in one, for a call whose time is the reading of the weights).
  *   logits = round(x W_r^T), summed in 64 bits and rounded to fp32, then to the type; probabilities, ties and weights as dsca_router_topk
  *   out    = round(sum_j w_j down(act(up x)) + sigmoid(round(x . g)) shared(x)), summed in fp32;
- *            the activated intermediate is held to 16 significant bits or more (fp32 for DSCA_F32)
+ *            the activated intermediate is held to 16 significant bits (DSCA_F8E4M3: 11; DSCA_F32: fp32)
  * Weights in the packing of dsca_ffn_args.  weights: DSCA_BF16 or DSCA_F32 (x, router and out in the
  * same type), or DSCA_F8E4M3 with the four scale arrays (x, router and out bf16).
  * d * (bytes of a weight) must be a multiple of 16 and every weight matrix 16-byte aligned.
@@ -91,7 +91,7 @@ typedef struct {
   const float* ws2_scale;
   float w1_max;               /* DSCA_F8E4M3: the largest magnitude among the (scaled) weights of w1 and ws1; it
                                  bounds the intermediate, whose f16 scale comes from it.  A bound up to
-                                 64 times too large costs no accuracy */
+                                 64 times too large costs typical values no accuracy */
   void* out;                  /* [T, d] */
   void* logits;               /* [T, E] */
   int32_t* topk_ids;          /* [T, top_k] */

@@ -295,6 +295,13 @@ def test_streams_and_graphs(cuda):
         assert all(torch.equal(o, v) for o, v in zip(outs, want))
 
 
+def test_64_experts_and_a_shared_one_are_refused(cuda):
+    """One logit more than the router holds."""
+    eng, w, router, gate, n = _engine(cuda, 128, 64, 4, 64, 64, seed=13)
+    with pytest.raises(ValueError):
+        eng.forward_few(n(4, 128))
+
+
 def test_forward_takes_it_below_few_tokens(cuda):
     """few_tokens switches forward(), capture() and the layers over; forward_normed is the norm and then
     the block."""
