@@ -228,7 +228,7 @@ def call_on(device, name: str, *args):
         _torch = torch
         load()
     cuda, index = _torch.cuda, device.index
-    cur = cuda.current_device()
+    cur = _torch._C._cuda_getDevice()  # device's tensors exist, so CUDA is initialised
     if index is None or index == cur:
         rc = getattr(_LIB, name)(*args, _torch._C._cuda_getCurrentRawStream(cur))
     else:

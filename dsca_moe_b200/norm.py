@@ -96,8 +96,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
         y_ptr = y.data_ptr()
     if quant is not None:
         width = d if quant == "e4m3" else 2 * ((d + 127) // 128 * 128)
-        q = x.new_empty((rows, width), dtype=torch.float8_e4m3fn)
-        scale = x.new_empty(rows, dtype=torch.float32)
+        q = torch.empty_strided((rows, width), (width, 1), dtype=torch.float8_e4m3fn, device=dev)
+        scale = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=dev)
         q_ptr, s_ptr = q.data_ptr(), scale.data_ptr()
     if rows:
         a = L.RmsNormArgs(x.data_ptr(), r_ptr, weight.data_ptr(), rows, d, dt, w_dt, ld, ld_r, d, d, eps, q_mode, y_ptr,
