@@ -813,8 +813,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t base = ring + (uint32_t)(warp * a.stages * a.stage);
     int st = 0, given = 0;  // next stage, sums handed over
     uint32_t phase = 0u;    // parity of the next stage's copy
-    auto box = [&](int pitch) { return base + (uint32_t)(st * a.stage + g * pitch + t4 * 16); };
-    auto arrived = [&]() { mbar_wait(smem_u32(&s.full[warp][st]), phase, abort_flag, a.err); };
+    // the next box (then = 0) or the one behind it
+    auto stage_of = [&](int then) { return st + then < a.stages ? st + then : 0; };
+    auto box = [&](int pitch, int then = 0) { return base + (uint32_t)(stage_of(then) * a.stage + g * pitch + t4 * 16); };
+    auto arrived = [&](int then = 0) {
+      mbar_wait(smem_u32(&s.full[warp][stage_of(then)]), st + then < a.stages ? phase : phase ^ 1u, abort_flag, a.err);
+    };
     auto release = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s.empty[warp][st]));
@@ -971,9 +975,48 @@ __global__ void __launch_bounds__(kThreads, 1)
           hand_over();
           if (!last || !stay) flip = !flip;
         };
-        for (int n0 = 0; n0 < n_tok; n0 += 8) {
-          if (flip) group(n0, vb, va);
-          else group(n0, va, vb);
+        // two boxes a warp and unit, values of the first in va and of the second in vb: either's next ones are
+        // asked for as soon as it is multiplied
+        auto pair = [&](int n0) {
+          const bool last = n0 + 8 >= n_tok, two = warp + kCompute < a.n1;
+          const int i2 = last && ai >= 0 && r + 1 == (ai + 1) * a.upe ? ai + 1 : ai, n2 = last ? 0 : n0 + 8;
+          const bool more = !last || ul + 1 < (ai < 0 ? nu_s : nu_s + nu_r), same = last && stay;
+          const int tok2 = !more || i2 < 0 ? a.T : (int)(s.info[i2] >> 8 & 255u);
+          float acc[SUB][4];
+#pragma unroll
+          for (int q = 0; q < SUB; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[q][i] = 0.0f;
+          if (!ready) {
+            load_x(va, ai, n_tok, n0, warp * a.b1);
+            if (two) load_x(vb, ai, n_tok, n0, (warp + kCompute) * a.b1);
+          }
+          if (n0 == 0) arrived();
+          box_mma<W, 1, SUB>(acc, box(pitch1), up1, sub1, blk1, va);
+          if (more && !same) load_x(va, i2, tok2, n2, warp * a.b1);
+          if (two) {
+            if (n0 == 0) arrived(1);
+            box_mma<W, 1, SUB>(acc, box(pitch1, 1), up1, sub1, blk1, vb);
+            if (more && !same) load_x(vb, i2, tok2, n2, (warp + kCompute) * a.b1);
+          }
+          ready = more;
+          if (last) {
+            release();
+            if (two) release();
+          }
+          float* p = buffer();
+#pragma unroll
+          for (int q = 0; q < SUB; ++q)
+            *reinterpret_cast<float4*>(p + (q * 32 + lane) * 4) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+          hand_over();
+        };
+        if (a.n1 > kCompute) {
+          for (int n0 = 0; n0 < n_tok; n0 += 8) pair(n0);
+        } else {
+          for (int n0 = 0; n0 < n_tok; n0 += 8) {
+            if (flip) group(n0, vb, va);
+            else group(n0, va, vb);
+          }
         }
       } else {
         float acc[NT][1][4];
@@ -1486,7 +1529,7 @@ int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   a.n2 = (a.k2 + a.b2 - 1) / a.b2;
   a.n2s = (a.k2s + a.b2s - 1) / a.b2s;
   a.n2_cta = (a.n2 + a.splits - 1) / a.splits;
-  if (SUB == 2 && a.n1 > kCompute) return DSCA_ERR_CAPACITY;
+  if (SUB == 2 && a.n1 > 2 * kCompute) return DSCA_ERR_CAPACITY;
   const int bytes = max(16 * SUB * a.b1, 16 * F::kSub2 * max(a.b2, a.n2s ? a.b2s : 0)) * W::kSize;
   a.stage = (bytes + 127) / 128 * 128;
   a.stages = min(kMaxStages, (kSmem - kFixed) / (kCompute * a.stage));
@@ -1518,9 +1561,9 @@ template <typename W>
 int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   if (a.T <= 8) return launch<W, 1, 1>(a, p, sms, stream);
   if constexpr (W::kSize != 4) {
-    // units of 32 rows: one box of at most 192 bytes a warp (against 16 rows: 32 tokens of the Qwen block with
-    // fp8 weights 132 us, 165; 16 of the Switch block of 768 36.5 us, 40.4)
-    if (a.d * W::kSize <= 192 * kCompute) {
+    // units of 32 rows: one or two boxes of at most 192 bytes a warp (against 16 rows: of the Qwen
+    // block 20 tokens in bf16 187 us, 216, 32 with fp8 weights 132 us, 165; 16 of the Switch block of 768 36.5 us, 40.4)
+    if (a.d * W::kSize <= 2 * 192 * kCompute) {
       if (a.T <= 16) return launch<W, 2, 2>(a, p, sms, stream);
       return launch<W, 4, 2>(a, p, sms, stream);
     }
