@@ -6,13 +6,14 @@
 // Such a call's time is the reading of the chosen experts' weights (17 MB an expert of the Qwen block
 // in bf16, 69 MB for its shared expert, against 4 KB a token), so everything here serves one
 // uninterrupted stream of weight bytes:
-//  - one persistent CTA per SM.  Two producer warps copy boxes of 16 weight rows x 64 to 320 bytes into
+//  - one persistent CTA per SM.  Two producer warps copy boxes of 16 weight rows x 64 to 384 bytes into
 //    shared memory by TMA (plain bulk copies, one a row, cost 60 ns of issue each: 16 times as much
 //    per byte); each of twelve compute warps has its own ring of boxes, its share of k, and its sums in
 //    registers, so that one warp's wait for its tokens' values (L2) passes under the others' products.
 //    The values for the next box are asked for before the present one is multiplied.  Two service
 //    warps run the router at the start; then, in turn, they add the twelve parts of each unit (16
-//    rows of a matrix), apply the activation and store;
+//    rows of a matrix), apply the activation and store (in the warp that is the last with its part this
+//    stood in the way of its next box: one token 43 us instead of 35);
 //  - the weights are cut 16 rows at a time (8 gate + 8 up rows, or 16 rows of any other matrix), fine
 //    enough that 148 SMs get nearly equal shares, where a 128-row tensor-memory tile would leave
 //    two fifths of them idle at one token.  16 rows x 8 tokens is the shape of mma.sync, which
@@ -25,6 +26,13 @@
 //    (a narrow model, or more than eight tokens, whose boxes are 32 rows high), several CTAs share a
 //    tile of rows, each with its share of every row's boxes, and the last one to finish adds their
 //    sums in order.
+//
+// Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
+// a token, a shared one of 5632) 1 token in bf16 32.6 us (4.3 TB/s, 65%), with fp8 weights 26.4 us (40%),
+// 8 tokens in bf16 97 us (80%), 20 tokens 187 us, 32 tokens with fp8 weights 132 us (58%); a Switch block (d 768, 64
+// experts of 2048) 16 tokens 36.5 us (38%); fp32 33 us where the bytes take 5.3.  At one token some 13 us
+// are not the stream's: launch (3), router (7, half of it under the shared expert's weights), the two
+// GEMMs' border (3), the last rows (2).
 //
 // A warp spends some 150 instructions on a box whatever its size, at one in eight clocks (three or four
 // warps a scheduler, each waiting for its own last result); this, not the products, is what keeps it
@@ -1061,8 +1069,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           release();
         };
-        // the boxes of an expert's unit, the same values again in the next one (20 tokens of the Qwen block in
-        // bf16: 216 us; asked for anew 232)
+        // the boxes of an expert's unit, the same values again in the next one (16 tokens of a
+        // block of 2560 in bf16 171 us; asked for anew 180)
         bool held = keep;
         if constexpr (!kDirect && !kF32) {
           held = ai >= 0 && n_tok <= 8 && a.n1 <= 2 * kCompute;

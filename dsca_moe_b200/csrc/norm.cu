@@ -12,7 +12,10 @@
 // scale (fp8_split.cuh), the token operand of the fp8-weight GEMMs.
 //
 // One pass over the data: a row lives in the registers of its TPR threads (up to 64 values each)
-// between the sum and the stores, so DRAM sees every input and output once.
+// between the sum and the stores, so DRAM sees every input and output once: it is bound by DRAM from a few
+// thousand rows on (with residual 16384 x 2048 bf16 41.5 us, 99% of a copy's 6.5 TB/s; 20000 x 768 with split
+// rows 26.7 us, 88%; 4096 x 2048 with e4m3 rows 14.2 us, 82%), below that by the launch and two trips to
+// memory (1 x 2048 2.1 us).
 #include "common.cuh"
 #include "dsca_b200_block.h"
 #include "fp8_split.cuh"
@@ -318,10 +321,12 @@ int launch(const Args& a, cudaStream_t stream) {
 // Threads a row: with many rows as few as hold it in two or three chunks each (fp32: one), so that a
 // row's reduction passes under the loads of the other rows on the SM; with few rows a whole CTA.
 // 4096 x 2048 bf16: 128 threads with 2 chunks 10.4 us, 256 with 1 11.1 us, a warp with 8 12.9 us.
+// Few threads against a whole CTA, bf16 with residual: 32 x 768 2.5 us, 2.1; 400 x 2048 3.0 us, 2.8; 600 x 768
+// 2.9 us both; 1200 x 768 3.3 us, 3.9; 1200 x 2048 4.3 us, 4.7.
 template <typename T, bool kVec, int QUANT>
 int dispatch(const Args& a, cudaStream_t stream) {
   const int chunks = (a.d + 7) / 8;
-  if (a.rows > 2 * current_device_sms() && chunks <= 256) {
+  if (a.rows > 4 * current_device_sms() && chunks <= 256) {
     if (chunks <= 32) return launch<T, kVec, 1, 32, QUANT>(a, stream);
     if constexpr (sizeof(T) == 2) {
       if (chunks <= 64) return launch<T, kVec, 2, 32, QUANT>(a, stream);
