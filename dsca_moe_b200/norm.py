@@ -83,6 +83,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     dense = x.is_contiguous()
     ld = d if dense else _stride(x, "x", d)
     rows = x.numel() // d
+    if rows > 0x7FFFFFFF:
+        raise ValueError(f"{rows} rows exceed 2^31 - 1")
     h, r_ptr, h_ptr, ld_r = x, None, None, 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != dtype or residual.device != dev:

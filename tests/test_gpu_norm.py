@@ -164,6 +164,40 @@ def test_norm_shapes_weights_and_places(cuda):
     assert torch.equal(y[:24], want.y) and (y[24] == 7).all()
 
 
+def test_norm_offsets_beyond_32_bits(cuda):
+    """Rows more than 2^31 elements apart, and dense rows with as many in front of them."""
+    from dsca_moe_b200 import add_rms_norm
+
+    ld, d = 2 ** 31 + 8, 64
+    x, r, w = _inputs(cuda, 3, d, torch.bfloat16, 21)
+    far = torch.empty(2 * ld + 2 * d, dtype=torch.bfloat16, device=cuda)
+    xs, rs = far.as_strided((3, d), (ld, 1)), far.as_strided((3, d), (ld, 1), d)
+    xs.copy_(x)
+    rs.copy_(r)
+    got, want = add_rms_norm(xs, w, residual=rs, quant="split"), add_rms_norm(x, w, residual=r, quant="split")
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    del far, xs, rs
+    rows, d = 2 ** 20 + 4096, 2048
+    x, w = torch.zeros(rows, d, dtype=torch.bfloat16, device=cuda), _inputs(cuda, 1, d, torch.bfloat16, 22)[2]
+    last = torch.randn(5, d, device=cuda).bfloat16()
+    x[-5:] = last
+    got = add_rms_norm(x, w, quant="e4m3")
+    assert not got.y[:-5].any() and (got.scale[:-5] == 1).all()
+    _close(got.y[-5:], _exact(last, None, w)[1])
+    assert torch.equal(got.residual, x)
+    want = add_rms_norm(last, w, quant="e4m3")
+    assert ((got.scale[-5:] - want.scale).abs() <= 2 * F32 * want.scale).all()
+
+
+def test_norm_rows_beyond_32_bits_are_refused(cuda):
+    from dsca_moe_b200 import add_rms_norm
+
+    w = torch.ones(1, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError):
+        add_rms_norm(torch.empty(2 ** 31, 1, dtype=torch.bfloat16, device=cuda), w)
+
+
 def test_norm_refusals(cuda):
     from dsca_moe_b200 import add_rms_norm
 
