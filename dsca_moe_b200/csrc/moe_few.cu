@@ -30,7 +30,8 @@
 // Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
 // a token, a shared one of 5632) 1 token in bf16 32.6 us (4.3 TB/s, 65%), with fp8 weights 26.4 us (40%),
 // 8 tokens in bf16 97 us (80%), 20 tokens 187 us, 32 tokens with fp8 weights 132 us (58%); a Switch block (d 768, 64
-// experts of 2048) 16 tokens 36.5 us (38%); fp32 33 us where the bytes take 5.3.  At one token some 13 us
+// experts of 2048) 16 tokens 36.5 us (38%); fp32 (d 712, 13 experts of 333) 5 tokens
+// 28.5 us where the bytes take 5.3.  At one token some 13 us
 // are not the stream's: launch (3), router (7, half of it under the shared expert's weights), the two
 // GEMMs' border (3), the last rows (2).
 //
@@ -500,44 +501,50 @@ __device__ __forceinline__ void box_mma(float (&acc)[SUB][4], uint32_t box, int 
     }
 }
 
-// The same for fp32 weights on the CUDA cores: lane (g, t) sums rows g and g + 8 over its k for all
-// eight tokens, then the four lanes of a row are added into the layout of the tensor-core
-// accumulators.  row(n): token row n at the box's first k (or null), the same on all lanes.
+// The same for fp32 weights on the CUDA cores, a token at a time: lane (g, t) sums rows g and g + 8 over its k,
+// then the four lanes of a row are added into the layout of the tensor-core accumulators.  row(n): token
+// row n at the box's first k, n < tokens; the next token's values are on their way under the present one's sums.
+// Few instructions count for more than few reads of the box: a warp has a handful of boxes, and with eight
+// tokens' sums side by side it waited for the code (d 712, one token 21.2 us, so 16.6; 5 tokens 32, 28.5; 32
+// tokens 103, 95).
 template <bool kCoherent, typename Row>
-__device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, int nkb, Row row, int live, int lane) {
+__device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, int nkb, Row row, int tokens, int live, int lane) {
+  constexpr int kMost = kMaxBox / 64;
   const int t = lane & 3;
-  const float* rp[8];
-  float s[16];
+  nkb = min(nkb, max(0, (live - t * 4 + 15) / 16));
+  float4 v[kMost], w[kMost];  // the token's values and the next one's
+  auto load = [&](int n) {
+    const float4* x = reinterpret_cast<const float4*>(row(n) + t * 4);
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    rp[n] = row(n);
-    if (rp[n] != nullptr) rp[n] += t * 4;
-    s[2 * n] = s[2 * n + 1] = 0.0f;
-  }
-#pragma unroll 2
-  for (int kb = 0; kb < nkb; ++kb) {
-    if (kb * 16 + t * 4 >= live) continue;
-    const uint4 u0 = lds128(box + kb * 64), u1 = lds128(box + up + kb * 64);
-    const float a0[4] = {__uint_as_float(u0.x), __uint_as_float(u0.y), __uint_as_float(u0.z), __uint_as_float(u0.w)};
-    const float a1[4] = {__uint_as_float(u1.x), __uint_as_float(u1.y), __uint_as_float(u1.z), __uint_as_float(u1.w)};
+    for (int kb = 0; kb < kMost; ++kb)
+      if (kb < nkb) w[kb] = kCoherent ? __ldcg(x + kb * 4) : x[kb * 4];
+  };
+  load(0);
+#pragma unroll 1
+  for (int n = 0; n < tokens; ++n) {
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      if (rp[n] == nullptr) continue;
-      const float4* q = reinterpret_cast<const float4*>(rp[n] + kb * 16);
-      const float4 v = kCoherent ? __ldcg(q) : *q;
-      s[2 * n] = fmaf(a0[3], v.w, fmaf(a0[2], v.z, fmaf(a0[1], v.y, fmaf(a0[0], v.x, s[2 * n]))));
-      s[2 * n + 1] = fmaf(a1[3], v.w, fmaf(a1[2], v.z, fmaf(a1[1], v.y, fmaf(a1[0], v.x, s[2 * n + 1]))));
+    for (int kb = 0; kb < kMost; ++kb) v[kb] = w[kb];
+    if (n + 1 < tokens) load(n + 1);
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int kb = 0; kb < kMost; ++kb) {
+      if (kb >= nkb) break;
+      const uint4 u0 = lds128(box + kb * 64), u1 = lds128(box + up + kb * 64);
+      const float4 x = v[kb];
+      s[0] = fmaf(__uint_as_float(u0.w), x.w, fmaf(__uint_as_float(u0.z), x.z, fmaf(__uint_as_float(u0.y), x.y, fmaf(__uint_as_float(u0.x), x.x, s[0]))));
+      s[1] = fmaf(__uint_as_float(u1.w), x.w, fmaf(__uint_as_float(u1.z), x.z, fmaf(__uint_as_float(u1.y), x.y, fmaf(__uint_as_float(u1.x), x.x, s[1]))));
     }
-  }
-#pragma unroll
-  for (int n = 0; n < 8; ++n)
+    __syncwarp();
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float v = s[2 * n + r];
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      if (t == n / 2) acc[2 * r + (n & 1)] += v;
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+      if (t == n / 2) {
+        if (n & 1) acc[2 * r + 1] += s[r];
+        else acc[2 * r] += s[r];
+      }
     }
+  }
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -1040,10 +1047,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               if (nt * 8 >= n_tok) break;
-              auto row = [&](int n) {
-                return nt * 8 + n < n_tok ? reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)) : nullptr;
-              };
-              box_fma<false>(acc[nt][0], box(pitch1), up1, blk1, row, a.d - k, lane);
+              auto row = [&](int n) { return reinterpret_cast<const float*>(x_row(ai, n_tok, nt * 8 + n, k)); };
+              box_fma<false>(acc[nt][0], box(pitch1), up1, blk1, row, min(8, n_tok - nt * 8), a.d - k, lane);
             }
           } else {
             if (!ready) load_x(v, ai, n_tok, 0, k);
@@ -1202,8 +1207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           arrived();
           for (int n0 = 0; n0 < n_tok; n0 += 8) {
             float acc[1][4] = {{0.0f, 0.0f, 0.0f, 0.0f}};
-            auto row = [&](int n) { return n0 + n < n_tok ? reinterpret_cast<const float*>(h_at(i, n0 + n, k)) : nullptr; };
-            box_fma<true>(acc[0], box(pitch), 8 * pitch, blk, row, (sh ? a.k2s : a.k2) - k, lane);
+            auto row = [&](int n) { return reinterpret_cast<const float*>(h_at(i, n0 + n, k)); };
+            box_fma<true>(acc[0], box(pitch), 8 * pitch, blk, row, min(8, n_tok - n0), (sh ? a.k2s : a.k2) - k, lane);
             join(acc, n0);
           }
         } else {
