@@ -30,14 +30,12 @@
 // Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
 // a token, a shared one of 5632) 1 token in bf16 32.6 us (4.3 TB/s, 65%), with fp8 weights 26.4 us (40%),
 // 8 tokens in bf16 97 us (80%), 20 tokens 187 us, 32 tokens with fp8 weights 132 us (58%); a Switch block (d 768, 64
-// experts of 2048) 16 tokens 36.5 us (38%); fp32 (d 712, 13 experts of 333) 5 tokens
-// 28.5 us where the bytes take 5.3.  At one token some 13 us
-// are not the stream's: launch (3), router (7, half of it under the shared expert's weights), the two
-// GEMMs' border (3), the last rows (2).
+// experts of 2048) 16 tokens 36.5 us (38%); fp32 (d 712, 13 experts of 333) 5 tokens 28.5 us where the bytes
+// take 5.3.  At one token some 13 us are not the stream's: launch (3), router (7, half of it under the
+// shared expert's weights), the two GEMMs' border (3), the last rows (2).
 //
-// A warp spends some 150 instructions on a box whatever its size, at one in eight clocks (three or four
-// warps a scheduler, each waiting for its own last result); this, not the products, is what keeps it
-// from DRAM speed.  So the boxes are as large as the shares allow; up to eight tokens, whose rows every
+// A warp spends 150 to 400 instructions on a box, at one in eight clocks (three or four warps a scheduler,
+// each waiting for its own last result); this, not the products, is what keeps it from DRAM speed.  So the boxes are as large as the shares allow; up to eight tokens, whose rows every
 // unit multiplies in full, x stays in registers through GEMM1 and the sums through GEMM2; with more,
 // an expert's few tokens are gathered for it, and units and tiles are 32 rows high where the rows are
 // short enough, so that 32 rows share one gathering.
@@ -49,8 +47,8 @@
 // for both operands.
 //
 // The intermediate is kept as two bf16 terms (16 significant bits; with fp32 weights in fp32, with fp8 weights
-// as one f16 term); everything is summed in fp32,
-// the router in fp64 (bf16 products are exact in fp32, so the logits round correctly).
+// as one f16 term); everything is summed in fp32, the router in fp64 (bf16 products are exact in fp32, so
+// the logits round correctly).
 //
 // fp8 weights go through f16: e4m3 converts to it exactly with one instruction a pair (to bf16 it
 // takes four, which alone cost more than the weights' DRAM time).  A token row times a power of two
