@@ -28,9 +28,9 @@
 //    sums in order.
 //
 // Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
-// a token, a shared one of 5632) 1 token in bf16 32.6 us (4.3 TB/s, 65%), with fp8 weights 26.4 us (40%),
-// 8 tokens in bf16 97 us (80%), 20 tokens 187 us, 32 tokens with fp8 weights 132 us (58%); a Switch block (d 768, 64
-// experts of 2048) 16 tokens 36.5 us (38%); fp32 (d 712, 13 experts of 333) 5 tokens 28.5 us where the bytes
+// a token, a shared one of 5632) 1 token in bf16 31.3 us (4.4 TB/s, 68%), with fp8 weights 26.0 us (41%),
+// 8 tokens in bf16 92 us (84%), 20 tokens 179 us, 32 tokens with fp8 weights 131 us (58%); a Switch block (d 768, 64
+// experts of 2048) 16 tokens 35.4 us (39%); fp32 (d 712, 13 experts of 333) 5 tokens 28.5 us where the bytes
 // take 5.3.  At one token some 13 us are not the stream's: launch (3), router (7, half of it under the
 // shared expert's weights), the two GEMMs' border (3), the last rows (2).
 //
@@ -128,10 +128,12 @@ struct Fp8 {
 };
 
 // One box of a tensor map (weights of this GPU) into this CTA's shared memory.
-__device__ __forceinline__ void box_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+__device__ __forceinline__ void box_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3,
+                                            uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
       : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -728,6 +730,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The lanes stay together (a lane that waits alone holds up the others of its warp), so a ring gets
     // its next box when the rings of all six have room.
     constexpr int kLanes = kCompute / kProducers;
+    // every weight is read once, and leaves room in L2 for the code, the intermediates and the rows that are read
+    // again (Qwen block, 8 tokens in bf16 97.5 us, so 92.3; 32 with fp8 weights 136.5, 131)
+    const uint64_t once = l2_policy_evict_first();
     const bool on = lane < kLanes;
     const int w = (warp - kProducer) * kLanes + (on ? lane : 0);
     const uint32_t base = ring + (uint32_t)(w * a.stages * a.stage);
@@ -789,8 +794,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j0 = 0; j0 < a.n1; j0 += kCompute) {
         const int j = j0 + w;
         box(on && j < a.n1, 16 * SUB * a.b1 * W::kSize, [&](uint32_t bar, uint32_t dst) {
-          if (a.glu) box_load_4d(dst, m, bar, j * a.b1, 8 * SUB * u % 128, 0, e * (a.n1p / 256) + 8 * SUB * u / 128);
-          else tma_load_2d(dst, m, bar, j * a.b1, e * a.n1p + 16 * SUB * u);
+          if (a.glu) box_load_4d(dst, m, bar, j * a.b1, 8 * SUB * u % 128, 0, e * (a.n1p / 256) + 8 * SUB * u / 128, once);
+          else tma_load_2d_hint(dst, m, bar, j * a.b1, e * a.n1p + 16 * SUB * u, once);
         });
       }
     }
@@ -800,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j0 = 0; j0 < a.n2s; j0 += per) {
         const int j = j0 + w * a.splits + split;
         box(on && j < a.n2s, a.rt * a.b2s * W::kSize,
-            [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &ms2, bar, j * a.b2s, tile * a.rt); });
+            [&](uint32_t bar, uint32_t dst) { tma_load_2d_hint(dst, &ms2, bar, j * a.b2s, tile * a.rt, once); });
       }
       for (int i = 0; i < n_act; ++i) {
         const uint32_t info = s.info[i];
@@ -808,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j0 = 0; j0 < a.n2; j0 += per) {
           const int j = j0 + fb * a.splits + split;
           box(on && j < a.n2, a.rt * a.b2 * W::kSize,
-              [&](uint32_t bar, uint32_t dst) { tma_load_2d(dst, &m2, bar, j * a.b2, e * a.dp + tile * a.rt); });
+              [&](uint32_t bar, uint32_t dst) { tma_load_2d_hint(dst, &m2, bar, j * a.b2, e * a.dp + tile * a.rt, once); });
         }
       }
     }
