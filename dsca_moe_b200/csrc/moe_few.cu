@@ -29,7 +29,7 @@
 //
 // Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
 // a token, a shared one of 5632) 1 token in bf16 31.3 us (4.4 TB/s, 68%), with fp8 weights 26.0 us (41%),
-// 8 tokens in bf16 92 us (84%), 20 tokens 179 us, 32 tokens with fp8 weights 131 us (58%); a Switch block (d 768, 64
+// 8 tokens in bf16 92-96 us (84%), 20 tokens 177 us, 32 tokens with fp8 weights 131 us (58%); a Switch block (d 768, 64
 // experts of 2048) 16 tokens 35.4 us (39%); fp32 (d 712, 13 experts of 333) 5 tokens 28.5 us where the bytes
 // take 5.3.  At one token some 13 us are not the stream's: launch (3), router (7, half of it under the
 // shared expert's weights), the two GEMMs' border (3), the last rows (2).
@@ -59,6 +59,8 @@
 // max|w1| sum|x|, so 2^14 / B^2 rounded down to a power of two cannot overflow, and typical values, some
 // 2^20 below the bound, still lie 2^18 above the smallest f16.
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "dsca_b200_block.h"
@@ -738,26 +740,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t base = ring + (uint32_t)(w * a.stages * a.stage);
     int st = 0, last = -1;  // next stage, stage before it
     uint32_t phase = 0u;    // parity of the next stage's copy
-    bool shallow = true, wrapped = false, stop = false;
-    // A box for this lane's ring, if there is one: load(bar, dst) once its stage is free.
-    auto box = [&](bool there, int bytes, auto load) {
+    // While two warps route, one box a ring in flight: the router's loads queue behind them in DRAM (one token in
+    // bf16 31.5 us, full rings 32.5).  Where all warps do, the rings fill at once.
+    bool shallow = !all_route, wrapped = false, stop = false;
+    // A box for this lane's ring, if there is one: load(bar, dst) once its stage is free.  one (only before
+    // the routing is known, a constant elsewhere): not before the last one has come.
+    auto box = [&](auto one, bool there, int bytes, auto load) {
       const uint32_t e = smem_u32(&s.empty[w][st]), f = smem_u32(&s.full[w][max(last, 0)]);
-      // Until the routing is known, one box a ring in flight: the router's loads queue behind them in DRAM
-      const bool we = there && wrapped, wf = there && shallow && last >= 0;
-      const uint64_t t0 = globaltimer_ns();
+      const bool we = there && wrapped, wf = there && one && last >= 0;
+      uint64_t since = 0u;
       for (uint32_t it = 0;; ++it) {
         const bool ok = (!we || mbar_try_wait(e, phase ^ 1u)) && (!wf || mbar_try_wait(f, st == 0 ? phase ^ 1u : phase));
-        if (__all_sync(0xffffffffu, ok)) break;
-        if ((it & 63u) == 63u) {
-          if (lane == 0 && globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (__all_sync(0xffffffffu, ok && *abort_flag == 0)) break;
+        if (lane == 0 && (it & 63u) == 63u) {
+          const uint64_t now = globaltimer_ns();
+          if (since == 0u) since = now;
+          if (now - since > kWaitLimitNs) {
             record_error(a.err, kErrWaitTimeout);
             *abort_flag = 1;
           }
-          __syncwarp();
-          if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+        }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) {
+          stop = true;
+          break;
         }
       }
-      stop = stop || __any_sync(0xffffffffu, *abort_flag != 0);
       if (there && !stop) {
         const uint32_t bar = smem_u32(&s.full[w][st]);
         mbar_arrive_expect_tx(bar, (uint32_t)bytes);
@@ -793,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const CUtensorMap* m = sh ? &ms1 : &m1;
       for (int j0 = 0; j0 < a.n1; j0 += kCompute) {
         const int j = j0 + w;
-        box(on && j < a.n1, 16 * SUB * a.b1 * W::kSize, [&](uint32_t bar, uint32_t dst) {
+        box(shallow, on && j < a.n1, 16 * SUB * a.b1 * W::kSize, [&](uint32_t bar, uint32_t dst) {
           if (a.glu) box_load_4d(dst, m, bar, j * a.b1, 8 * SUB * u % 128, 0, e * (a.n1p / 256) + 8 * SUB * u / 128, once);
           else tma_load_2d_hint(dst, m, bar, j * a.b1, e * a.n1p + 16 * SUB * u, once);
         });
@@ -804,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tile = item / a.splits, split = item % a.splits, per = kCompute * a.splits;
       for (int j0 = 0; j0 < a.n2s; j0 += per) {
         const int j = j0 + w * a.splits + split;
-        box(on && j < a.n2s, a.rt * a.b2s * W::kSize,
+        box(std::false_type{}, on && j < a.n2s, a.rt * a.b2s * W::kSize,
             [&](uint32_t bar, uint32_t dst) { tma_load_2d_hint(dst, &ms2, bar, j * a.b2s, tile * a.rt, once); });
       }
       for (int i = 0; i < n_act; ++i) {
@@ -812,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = info & 255u, fb = first_box(w, info);
         for (int j0 = 0; j0 < a.n2; j0 += per) {
           const int j = j0 + fb * a.splits + split;
-          box(on && j < a.n2, a.rt * a.b2 * W::kSize,
+          box(std::false_type{}, on && j < a.n2, a.rt * a.b2 * W::kSize,
               [&](uint32_t bar, uint32_t dst) { tma_load_2d_hint(dst, &m2, bar, j * a.b2, e * a.dp + tile * a.rt, once); });
         }
       }
