@@ -131,7 +131,8 @@ def test_swiglu(cuda, T, d, E, k, I, Is, kind):
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
 @pytest.mark.parametrize("T,d,E,k,I,Is", [(3, 5120, 6, 2, 72, 40), (12, 5120, 6, 2, 72, 40), (24, 8192, 4, 2, 40, 16),
                                           (16, 256, 2, 1, 4096, 0), (32, 512, 3, 2, 3000, 1000), (20, 1152, 40, 3, 500, 0), (9, 2304, 5, 2, 300, 100),
-                                          (32, 1200, 2, 1, 900, 300), (28, 4096, 12, 4, 150, 70)])
+                                          (32, 1200, 2, 1, 900, 300), (28, 4096, 12, 4, 150, 70),
+                                          (2, 16384, 3, 2, 24, 8), (11, 16384, 3, 1, 24, 0), (4, 64, 4, 2, 20000, 9000)])
 def test_swiglu_long_rows_and_many_units(cuda, T, d, E, k, I, Is, kind):
     """Rows of more boxes than a warp keeps values of; consecutive units of one expert, with at most eight
     tokens and with more, and of the next one."""

@@ -71,6 +71,7 @@ def test_norm(cuda, dtype, rows, d, gap):
 @pytest.mark.parametrize("rows,d,gap,dtype", [(1, 2048, 0, torch.bfloat16), (37, 768, 0, torch.bfloat16),
                                               (5, 1021, 2, torch.bfloat16), (40, 2048, 0, torch.float32),
                                               (3, 8192, 0, torch.bfloat16), (2, 20000, 0, torch.float32),
+                                              (2, 32768, 0, torch.float32),
                                               (11, 96, 5, torch.float32)])
 def test_norm_e4m3(cuda, rows, d, gap, dtype):
     from dsca_moe_b200 import add_rms_norm
@@ -90,7 +91,8 @@ def test_norm_e4m3(cuda, rows, d, gap, dtype):
     assert only.y is None and torch.equal(only.q.view(torch.uint8), out.q.view(torch.uint8))
 
 
-@pytest.mark.parametrize("rows,d,gap", [(1, 2048, 0), (50, 768, 0), (7, 264, 5), (3, 8192, 0), (2, 16384, 3), (4, 8, 0)])
+@pytest.mark.parametrize("rows,d,gap", [(1, 2048, 0), (50, 768, 0), (7, 264, 5), (3, 8192, 0), (2, 16384, 3), (4, 8, 0),
+                                        (2, 32768, 0)])
 def test_norm_split_rows(cuda, rows, d, gap):
     """The two-term rows are those of dsca_split_rows on y, bit for bit, padding included."""
     from dsca_moe_b200 import add_rms_norm
