@@ -30,7 +30,7 @@
 // Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
 // a token, a shared one of 5632) 1 token in bf16 31.3 us (4.4 TB/s, 68%), with fp8 weights 26.0 us (41%),
 // 8 tokens in bf16 92-96 us (84%), 20 tokens 177 us, 32 tokens with fp8 weights 131 us (58%); a Switch block (d 768, 64
-// experts of 2048) 16 tokens 35.4 us (39%); fp32 (d 712, 13 experts of 333) 5 tokens 28.5 us where the bytes
+// experts of 2048) 16 tokens 35.4 us (39%); fp32 (d 712, 13 experts of 333) 5 tokens 27.3 us where the bytes
 // take 5.3.  At one token some 13 us are not the stream's: launch (3), router (7, half of it under the
 // shared expert's weights), the two GEMMs' border (3), the last rows (2).
 //
@@ -503,49 +503,50 @@ __device__ __forceinline__ void box_mma(float (&acc)[SUB][4], uint32_t box, int 
     }
 }
 
-// The same for fp32 weights on the CUDA cores, a token at a time: lane (g, t) sums rows g and g + 8 over its k,
+// The same for fp32 weights on the CUDA cores, two tokens at a time: lane (g, t) sums rows g and g + 8 over its k,
 // then the four lanes of a row are added into the layout of the tensor-core accumulators.  row(n): token
-// row n at the box's first k, n < tokens; the next token's values are on their way under the present one's sums.
-// Few instructions count for more than few reads of the box: a warp has a handful of boxes, and with eight
-// tokens' sums side by side it waited for the code (d 712, one token 21.2 us, so 16.6; 5 tokens 32, 28.5; 32
-// tokens 103, 95).
+// row n at the box's first k, n < tokens.  Few instructions count for more than few reads of the box: a warp
+// has a handful of boxes, and with eight tokens' sums side by side it waited for the code.  d 712, 1 / 5 / 8 /
+// 32 tokens: eight side by side 21.2 / 32 / 38 / 103 us, one at a time 17.2 / 27.8 / 38.2 / 94, two 17.9 /
+// 27.3 / 33.2 / 79, two with code of its own for an odd last one 19.0 / 28.6 / 34.6 / 84.
 template <bool kCoherent, typename Row>
 __device__ __forceinline__ void box_fma(float (&acc)[4], uint32_t box, int up, int nkb, Row row, int tokens, int live, int lane) {
   constexpr int kMost = kMaxBox / 64;
   const int t = lane & 3;
   nkb = min(nkb, max(0, (live - t * 4 + 15) / 16));
-  float4 v[kMost], w[kMost];  // the token's values and the next one's
-  auto load = [&](int n) {
-    const float4* x = reinterpret_cast<const float4*>(row(n) + t * 4);
-#pragma unroll
-    for (int kb = 0; kb < kMost; ++kb)
-      if (kb < nkb) w[kb] = kCoherent ? __ldcg(x + kb * 4) : x[kb * 4];
-  };
-  load(0);
 #pragma unroll 1
-  for (int n = 0; n < tokens; ++n) {
+  for (int n = 0; n < tokens; n += 2) {
+    float4 v[2][kMost];
+    float s[2][2];
 #pragma unroll
-    for (int kb = 0; kb < kMost; ++kb) v[kb] = w[kb];
-    if (n + 1 < tokens) load(n + 1);
-    float s[2] = {0.0f, 0.0f};
+    for (int i = 0; i < 2; ++i) {
+      // an odd last token twice: the column behind it is dropped
+      const float4* x = reinterpret_cast<const float4*>(row(min(n + i, tokens - 1)) + t * 4);
+#pragma unroll
+      for (int kb = 0; kb < kMost; ++kb)
+        if (kb < nkb) v[i][kb] = kCoherent ? __ldcg(x + kb * 4) : x[kb * 4];
+      s[i][0] = s[i][1] = 0.0f;
+    }
 #pragma unroll
     for (int kb = 0; kb < kMost; ++kb) {
       if (kb >= nkb) break;
-      const uint4 u0 = lds128(box + kb * 64), u1 = lds128(box + up + kb * 64);
-      const float4 x = v[kb];
-      s[0] = fmaf(__uint_as_float(u0.w), x.w, fmaf(__uint_as_float(u0.z), x.z, fmaf(__uint_as_float(u0.y), x.y, fmaf(__uint_as_float(u0.x), x.x, s[0]))));
-      s[1] = fmaf(__uint_as_float(u1.w), x.w, fmaf(__uint_as_float(u1.z), x.z, fmaf(__uint_as_float(u1.y), x.y, fmaf(__uint_as_float(u1.x), x.x, s[1]))));
+      const uint4 u[2] = {lds128(box + kb * 64), lds128(box + up + kb * 64)};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          s[i][r] = fmaf(__uint_as_float(u[r].w), v[i][kb].w, fmaf(__uint_as_float(u[r].z), v[i][kb].z,
+                    fmaf(__uint_as_float(u[r].y), v[i][kb].y, fmaf(__uint_as_float(u[r].x), v[i][kb].x, s[i][r]))));
     }
     __syncwarp();
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
-      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
-      if (t == n / 2) {
-        if (n & 1) acc[2 * r + 1] += s[r];
-        else acc[2 * r] += s[r];
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        s[i][r] += __shfl_xor_sync(0xffffffffu, s[i][r], 1);
+        s[i][r] += __shfl_xor_sync(0xffffffffu, s[i][r], 2);
+        if (t == n / 2) acc[2 * r + i] += s[i][r];
       }
-    }
   }
 }
 
