@@ -117,7 +117,8 @@ class FewArgs(ctypes.Structure):
                 ("dp", _i), ("shared_inter", _i), ("shared_n1p", _i), ("shared_ip", _i), ("w1", _vp), ("w2", _vp),
                 ("ws1", _vp), ("ws2", _vp), ("w1_scale", _vp), ("w2_scale", _vp), ("ws1_scale", _vp),
                 ("ws2_scale", _vp), ("w1_max", ctypes.c_float), ("out", _vp), ("logits", _vp), ("topk_ids", _vp), ("topk_w", _vp),
-                ("expert_index", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
+                ("expert_index", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp),
+                ("wait_limit_ns", ctypes.c_uint64)]
 
 
 # every symbol include/dsca_b200.h declares

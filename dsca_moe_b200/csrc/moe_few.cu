@@ -114,6 +114,7 @@ struct Args {
   int rt, tiles, splits;  // rows of a GEMM2 tile, tiles, CTAs that share one
   float* partial;         // their sums: [tiles * splits][tokens in eights][kSub2][32][4]
   int stage, stages;      // bytes of a stage, stages of a warp's ring
+  uint64_t wait_ns;       // limit of every wait
 };
 
 struct Bf16 {
@@ -196,27 +197,57 @@ __device__ __forceinline__ void magnitudes(uint4 u, uint32_t& m, float& l1) {
   }
 }
 
+// whether the phase of this parity is complete, without waiting
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
   uint32_t v;
   asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-// Bounded wait until *p reaches `target` (one thread; the counters only grow during a call).
-__device__ __forceinline__ bool ctr_wait(const uint32_t* p, uint32_t target, volatile int* abort_flag, int32_t* err) {
-  if (ld_acquire(p) >= target) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (ld_acquire(p) >= target) return true;
-    if ((it & 63u) == 0u) {
-      if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        record_error(err, kErrWaitTimeout);
-        *abort_flag = 1;
-        return false;
-      }
+// The kernel's waits, every one bounded.  One that has run out records the error and raises the CTA's flag,
+// after which every other wait of the CTA returns at its first look (false, unless what it waits for has come):
+// each role then runs to its end on whatever it has, without another copy, and takes part in every barrier.
+struct Waits {
+  volatile int* abort;
+  int32_t* err;
+  uint64_t limit;  // nanoseconds
+  __device__ __forceinline__ bool over(uint64_t t0) const {
+    if (globaltimer_ns() - t0 <= limit) return false;
+    record_error(err, kErrWaitTimeout);
+    *abort = 1;
+    return true;
+  }
+  // the phase of this parity of an mbarrier
+  __device__ __forceinline__ bool bar(uint32_t b, uint32_t parity) const {
+    if (mbar_test_wait(b, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+      if (*abort) return false;
+      if (mbar_try_wait(b, parity)) return true;
+      if ((it & 15u) == 0u && over(t0)) return false;
     }
   }
-}
+  // until *p has reached `target` (one thread; the counters only grow during a call).  As a signed distance:
+  // a workspace whose counter starts too low makes the wait run out.
+  __device__ __forceinline__ bool counter(const uint32_t* p, uint32_t target) const {
+    if ((int32_t)(ld_acquire(p) - target) >= 0) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+      if ((int32_t)(ld_acquire(p) - target) >= 0) return true;
+      if ((it & 15u) == 0u && (*abort || over(t0))) return false;
+    }
+  }
+};
 __device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n) {
   __threadfence();
   atomicAdd(p, n);
@@ -268,6 +299,7 @@ struct Smem {
   uint8_t slot[DSCA_MAX_EXPERTS][8 * NT];   // choice of (expert, token)
   int n_act;
   uint32_t handed;                          // routed units' handings over, all CTAs'
+  uint32_t left[kCompute];                  // where a ring's producer ended: stage, its parity (bit 8), gone round (bit 9)
   int abort;
 };
 
@@ -582,7 +614,7 @@ __device__ __forceinline__ void store_out(const Args& a, S& s, float4 v, int til
 // Router: fp64 dot products spread over the grid, then softmax, selection and the expert lists in every
 // CTA for itself.  Warp wi of the nw warps that take part (they share named barrier 1).
 template <typename X, int SUB, int kTokens, bool kDirect, typename S>
-__device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int lane) {
+__device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
   // a logit's product in four parts while that leaves a warp one (one token of the Qwen block 32.7 us, whole
   // 34.6), else whole (32 tokens with fp8 weights 130 us, four parts 133)
@@ -621,7 +653,7 @@ __device__ __forceinline__ void route(const Args& a, S& s, int wi, int nw, int l
   __syncwarp();
   for (int t = wi - nw; t < a.T; t += nw) {
     if (t >= 0 && t < nw) {
-      if (wi == 0 && lane == 0) ctr_wait(a.ctr + kCtrLogits, (uint32_t)counted, &s.abort, a.err);
+      if (wi == 0 && lane == 0) waits.counter(a.ctr + kCtrLogits, (uint32_t)counted);
       __syncwarp();
       group_sync(nw * 32);
     }
@@ -683,6 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int G = gridDim.x, cta = blockIdx.x;
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)((sizeof(S) + 127) / 128 * 128);
   volatile int* abort_flag = &s.abort;
+  const Waits waits{abort_flag, a.err, a.wait_ns};
 
   if (threadIdx.x < kCompute * kMaxStages) {
     mbar_init(smem_u32(&s.full[0][0] + threadIdx.x), 1);
@@ -715,7 +748,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int units = n_act * a.upe, more = cta - (G - units % G);
     return int2{cta * (units / G) + max(0, more), units / G + (more >= 0)};  // the first of them, and how many
   };
-  auto wait_routed = [&]() { mbar_wait(smem_u32(&s.routed), 0u, abort_flag, a.err); };
+  // Waits for the lists of experts (a whole warp); how many experts have tokens.  None where a lane's wait was given
+  // up: nothing of the lists is read then, as they may not be there.
+  auto wait_routed = [&]() {
+    const bool there = waits.bar(smem_u32(&s.routed), 0u);
+    return __all_sync(0xffffffffu, there) ? s.n_act : 0;
+  };
   // warp w's first box (of this item's) of an active expert
   auto first_box = [&](int w, uint32_t info) {
     const int b = w - (int)(info >> 16);
@@ -747,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A box for this lane's ring, if there is one: load(bar, dst) once its stage is free.  one (only before
     // the routing is known, a constant elsewhere): not before the last one has come.
     auto box = [&](auto one, bool there, int bytes, auto load) {
+      if (stop) return;
       const uint32_t e = smem_u32(&s.empty[w][st]), f = smem_u32(&s.full[w][max(last, 0)]);
       const bool we = there && wrapped, wf = there && one && last >= 0;
       uint64_t since = 0u;
@@ -756,10 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && (it & 63u) == 63u) {
           const uint64_t now = globaltimer_ns();
           if (since == 0u) since = now;
-          if (now - since > kWaitLimitNs) {
-            record_error(a.err, kErrWaitTimeout);
-            *abort_flag = 1;
-          }
+          waits.over(since);
         }
         __syncwarp();
         if (__any_sync(0xffffffffu, *abort_flag != 0)) {
@@ -780,13 +816,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     };
-    int nu_r = 0, r = 0, ai = 0, first = 0;
+    int n_act = 0, nu_r = 0, r = 0, ai = 0, first = 0;
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
       const bool sh = ul < nu_s;
       if (ul == nu_s) {
-        wait_routed();
+        n_act = wait_routed();
         shallow = false;
-        const int2 ru = routed_units(s.n_act);
+        const int2 ru = routed_units(n_act);
         r = ru.x;
         nu_r = ru.y;
         if (nu_r == 0) break;
@@ -808,7 +844,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         });
       }
     }
-    const int n_act = s.n_act;
     for (int item = cta; item < items; item += G) {
       const int tile = item / a.splits, split = item % a.splits, per = kCompute * a.splits;
       for (int j0 = 0; j0 < a.n2s; j0 += per) {
@@ -826,17 +861,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    // after an abort copies may still be on their way into this CTA's shared memory
-    if (on && *abort_flag) {
-      for (int q = 0; q < (wrapped ? a.stages : st); ++q) {
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(smem_u32(&s.full[w][q]), q < st ? phase : phase ^ 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
-        }
-      }
-    }
+    if (on) s.left[w] = (uint32_t)st | phase << 8 | (uint32_t)wrapped << 9;
   } else if (warp < kCompute) {
     // ================================================================ compute
-    if (all_route) route<X, SUB, 8 * NT, kDirect>(a, s, kServices + warp, route_warps, lane);
+    if (all_route) route<X, SUB, 8 * NT, kDirect>(a, s, waits, kServices + warp, route_warps, lane);
     const uint32_t base = ring + (uint32_t)(warp * a.stages * a.stage);
     int st = 0, given = 0;  // next stage, sums handed over
     uint32_t phase = 0u;    // parity of the next stage's copy
@@ -844,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto stage_of = [&](int then) { return st + then < a.stages ? st + then : 0; };
     auto box = [&](int pitch, int then = 0) { return base + (uint32_t)(stage_of(then) * a.stage + g * pitch + t4 * 16); };
     auto arrived = [&](int then = 0) {
-      mbar_wait(smem_u32(&s.full[warp][stage_of(then)]), st + then < a.stages ? phase : phase ^ 1u, abort_flag, a.err);
+      waits.bar(smem_u32(&s.full[warp][stage_of(then)]), st + then < a.stages ? phase : phase ^ 1u);
     };
     auto release = [&]() {
       __syncwarp();
@@ -855,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     // until the sums handed over as number n have been read
-    auto wait_read = [&](int n) { mbar_wait(smem_u32(&s.part_empty[n % kParts]), (uint32_t)(n / kParts) & 1u, abort_flag, a.err); };
+    auto wait_read = [&](int n) { waits.bar(smem_u32(&s.part_empty[n % kParts]), (uint32_t)(n / kParts) & 1u); };
     // this warp's part of the next buffer, free to be written
     auto buffer = [&]() {
       if (given >= kParts) wait_read(given - kParts);
@@ -949,11 +977,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     int holds = -1;  // active expert whose values are in va and vb
+    int n_act = 0;                 // active experts
     int nu_r = 0, ai = -1, r = 0;  // routed units of this CTA; active expert and number of the present one
     for (int ul = 0; ul < nu_s + nu_r || ul == nu_s; ++ul) {
       if (ul == nu_s) {
-        wait_routed();
-        const int2 ru = routed_units(s.n_act);
+        n_act = wait_routed();
+        const int2 ru = routed_units(n_act);
         r = ru.x;
         nu_r = ru.y;
         if (nu_r == 0) break;
@@ -1129,7 +1158,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // kDirect a token without the expert reads another one's row and its column is dropped, and the sums
     // of all experts stay in registers.  Else the columns are the expert's own tokens, and a box's sums
     // join the warp's sums of all tokens in shared memory (a lane's values have places of their own).
-    const int n_act = s.n_act;
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
     auto h_at = [&](int i, int n, int k) {
@@ -1174,8 +1202,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool sh = i < 0;
         if (sh ? !have_s : !have_r) {
           if (lane == 0) {
-            if (sh) ctr_wait(a.ctr + kCtrShared, (uint32_t)(a.ups * (SUB == 2 ? (a.T + 7) / 8 : 1)), abort_flag, a.err);
-            else ctr_wait(a.ctr + kCtrRouted, s.handed, abort_flag, a.err);
+            if (sh) waits.counter(a.ctr + kCtrShared, (uint32_t)(a.ups * (SUB == 2 ? (a.T + 7) / 8 : 1)));
+            else waits.counter(a.ctr + kCtrRouted, s.handed);
           }
           __syncwarp();
           if (sh) have_s = true; else have_r = true;
@@ -1296,9 +1324,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================================================ service
     const int sw = warp - kService;
-    route<X, SUB, 8 * NT, kDirect>(a, s, sw, route_warps, lane);
-    wait_routed();
-    const int2 ru = routed_units(s.n_act);
+    route<X, SUB, 8 * NT, kDirect>(a, s, waits, sw, route_warps, lane);
+    const int2 ru = routed_units(wait_routed());
     const int nu = nu_s + ru.y;
     const size_t h_lo = (size_t)a.T * a.k * a.hp, hs_lo = (size_t)a.T * a.hsp;
     uint32_t owed[2] = {0u, 0u};  // handings over of the shared expert / the routed experts stored, not announced
@@ -1311,9 +1338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Every second handing over is this warp's.
     int seq = 0;
     auto mine = [&]() { return seq % kServices == sw; };
-    auto wait_parts = [&]() {
-      mbar_wait(smem_u32(&s.part_full[seq % kParts]), (uint32_t)(seq / kParts) & 1u, abort_flag, a.err);
-    };
+    auto wait_parts = [&]() { waits.bar(smem_u32(&s.part_full[seq % kParts]), (uint32_t)(seq / kParts) & 1u); };
     auto free_parts = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[seq % kParts]));
@@ -1449,8 +1474,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  // ---- the last CTA to leave zeroes the counters for the next call
   __syncthreads();
+  // After an abort copies may still be on their way into this CTA's shared memory.  They come whatever the caller's
+  // limit is, so it does not count here.
+  if (*abort_flag) {
+    if (threadIdx.x < kCompute) {
+      const uint32_t left = s.left[threadIdx.x];
+      const int st = (int)(left & 255u);
+      const uint32_t phase = left >> 8 & 1u;
+      for (int q = 0; q < ((left >> 9) ? a.stages : st); ++q) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(smem_u32(&s.full[threadIdx.x][q]), q < st ? phase : phase ^ 1u) &&
+               globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+    }
+    __syncthreads();
+  }
+  // ---- the last CTA to leave zeroes the counters for the next call
   if (threadIdx.x == 0) {
     __threadfence();
     if (atomicAdd(a.ctr + kCtrExit, 1u) == (uint32_t)G - 1u) {
@@ -1614,6 +1655,7 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.w1s = p->w1_scale; a.w2s = p->w2_scale; a.ws1s = p->ws1_scale; a.ws2s = p->ws2_scale;
   a.out = p->out; a.logits = p->logits; a.topk_ids = p->topk_ids; a.topk_w = p->topk_w;
   a.expert_index = p->expert_index; a.err = p->err;
+  a.wait_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
   a.T = p->T; a.d = p->d; a.E = p->E; a.mode = p->mode; a.norm_topk = p->norm_topk;
   a.k = p->mode == DSCA_ROUTE_SWITCH_TOP1 ? 1 : p->top_k;
   a.glu = p->act == DSCA_ACT_SWIGLU;

@@ -755,7 +755,7 @@ class MoEEngine:
             a.w1, a.w2, a.ws1, a.ws2 = _ptr(pe.w1), _ptr(pe.w2), _ptr(pe.ws1), _ptr(pe.ws2)
             a.w1_scale, a.w2_scale = _ptr(pe.w1_scale), _ptr(pe.w2_scale)
             a.ws1_scale, a.ws2_scale = _ptr(pe.ws1_scale), _ptr(pe.ws2_scale)
-            a.w1_max, a.err = self._w1_max, _ptr(self.err)
+            a.w1_max, a.err, a.wait_limit_ns = self._w1_max, _ptr(self.err), self.wait_limit_ns
             self._few_bytes = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.d, self.top_k, pe.inter,
                                                                    pe.s_inter)
             self._few_args = a

@@ -67,8 +67,10 @@ DSCA_API int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream);
  * d * (bytes of a weight) must be a multiple of 16 and every weight matrix 16-byte aligned.
  * workspace: dsca_few_workspace_bytes() bytes, 256-byte aligned, the first DSCA_FEW_ZERO_BYTES zero
  * before the first call; every call leaves them zero.  Calls that may overlap on the GPU must not
- * share a workspace.  After a call whose waits timed out (dsca_check_error on err) zero them again.
- * The kernel's CTAs wait for one another (bounded), so it is launched cooperatively, one CTA per SM.
+ * share a workspace.
+ * The kernel's CTAs wait for one another, so it is launched cooperatively, one CTA per SM.  Each wait ends after
+ * wait_limit_ns: the call then ends too, with DSCA_ERR_WAIT_TIMEOUT in err (dsca_check_error) and results of no
+ * meaning, and the bytes above have to be zeroed again.
  */
 typedef struct {
   const void* x;              /* [T, d] contiguous, 16-byte aligned */
@@ -100,6 +102,7 @@ typedef struct {
   void* workspace;
   size_t workspace_bytes;
   int32_t* err;               /* device error word */
+  uint64_t wait_limit_ns;     /* limit of each of the kernel's waits; 0: 2 s */
 } dsca_few_args;
 DSCA_API size_t dsca_few_workspace_bytes(int T, int d, int top_k, int inter, int shared_inter);
 DSCA_API int dsca_moe_few(const dsca_few_args* a, dsca_stream_t stream);
