@@ -47,7 +47,7 @@
 // for both operands.
 //
 // The intermediate is kept as two bf16 terms (16 significant bits; with fp32 weights in fp32, with fp8 weights
-// as one f16 term); everything is summed in fp32, the router in fp64 (bf16 products are exact in fp32, so
+// as one f16 term, see below); everything is summed in fp32, the router in fp64 (bf16 products are exact in fp32, so
 // the logits round correctly).
 //
 // fp8 weights go through f16: e4m3 converts to it exactly with one instruction a pair (to bf16 it
@@ -56,8 +56,12 @@
 // intermediate (one f16 term: it is off by 2^-11 at most where the output's bf16 is by 2^-8 and the weights'
 // own rounding by 2^-4; with a second one, twice the loads and products of
 // GEMM2, 32 tokens took 183 us instead of 153 and one took 31 instead of 27) needs a scale before it is known: |h| <= B^2 (SwiGLU; B with ReLU), B =
-// max|w1| sum|x|, so 2^14 / B^2 rounded down to a power of two cannot overflow, and typical values, some
-// 2^20 below the bound, still lie 2^18 above the smallest f16.
+// max|w1| sum|x|, so 2^14 / B^2 rounded down to a power of two cannot overflow.  How far below the bound a row's
+// values are depends on the weights (some 2^20 where all are alike, 2^30 and more where a few rows or one expert
+// are much larger than the rest), so the intermediate is stored three times, each copy 2^20 times the one before
+// (infinite where it overflows), and the largest magnitude of each row is kept along: GEMM2 reads the first copy in
+// which that is at least 2^-5, where every value has 11 significant bits or is off by 2^-20 of the row's largest,
+// as long as that largest value is not below 2^-59 of the bound.
 #include <math.h>
 
 #include <type_traits>
@@ -80,6 +84,8 @@ constexpr int kVals = 8;                  // 16-byte vectors of token values tha
 constexpr int kSmem = 227 * 1024;         // shared memory of a CTA
 constexpr int kLgPitch = 64;              // logits of a token in the scratch: E + 1 <= 64
 constexpr int kDotParts = 4;              // warps that share a logit's dot product
+constexpr int kCopies = 3;                // of the intermediate, fp8 weights
+constexpr int kCopyExp = 20;              // each is 2^20 times the one before
 
 // words of the counter block
 enum { kCtrLogits = 0, kCtrShared = 1, kCtrRouted = 2, kCtrExit = 3, kCtrTiles = 8 };
@@ -98,13 +104,15 @@ struct Args {
   double* lg;       // [T][64][4] parts of the logits, column E = shared gate
   uint8_t* x16;     // fp8 weights, more than eight tokens: [T][d] token rows in f16
   float* xmeta;     // and [T][2]: 1 / their scale, the largest power of two below sum|x|
-  uint8_t* h;       // [T * k][hp] intermediate: high terms, then the low terms; or fp32
+  uint32_t* hmax;   // fp8 weights: [T * k], then [T]: largest magnitude of a row of h / hs (float bits of the first copy)
+  uint8_t* h;       // [T * k][hp] intermediate: high terms, then the low terms; or fp32; or the f16 copies
   uint8_t* hs;      // [T][hsp] the shared expert's
   uint32_t* ctr;
   int32_t* err;
   int T, d, E, k, mode, norm_topk, glu;
   int n1p, ip, dp, s_ip;
   int w1_exp;             // fp8: max|w1| < 2^w1_exp
+  int inv_k;              // 2^16 / k + 1
   int hp, hsp;            // row pitch of h / hs in values
   int upe, ups;           // units (16 or 32 weight rows of GEMM1) per routed expert / of the shared expert
   int k2, k2s;            // values of a row of w2 / ws2 that are read
@@ -172,10 +180,15 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // Exponent of the scale that takes a row whose largest magnitude has these bf16 bits to [2^14, 2^15),
 // within what fp32 holds together with its inverse.
 __device__ __forceinline__ int x_scale_exp(uint32_t max_bits) { return 141 - max(15, min(254, (int)(max_bits >> 7))); }
-// The intermediate's scale (see the top): sum|x| < 2^(e + 1), max|w1| < 2^w.
+// Exponent of the scale of the intermediate's first copy (see the top): sum|x| < 2^(e + 1), max|w1| < 2^w.  At most
+// 80, so that the last copy's inverse is a normal float.
 __device__ __forceinline__ int h_scale_exp(int e, int w, bool glu) {
   const int b = e + 1 + w;
-  return max(-126, min(126, 14 - (glu ? 2 * b : b)));
+  return max(-126, min(80, 14 - (glu ? 2 * b : b)));
+}
+// the copy to read of a row whose largest magnitude has these bits (an infinity or a NaN is in each)
+__device__ __forceinline__ int h_copy(uint32_t max_bits) {
+  return max_bits >= __float_as_uint(0x1p-5f) ? 0 : max_bits >= __float_as_uint(0x1p-25f) ? 1 : 2;
 }
 // the exponent of a non-negative float
 __device__ __forceinline__ int exp_of(float v) { return (int)(__float_as_uint(v) >> 23) - 127; }
@@ -283,7 +296,12 @@ struct Smem {
   bool last;                                // this CTA's sums of a tile were the last to come
   float wt[8 * NT * DSCA_MAX_TOPK];         // routing weights by assignment
   float sg[8 * NT];                         // shared-expert gate
-  float xinv[8 * NT], hscale[8 * NT];       // fp8: 1 / scale of a token's row, scale of its intermediate
+  float xinv[8 * NT];                       // fp8: 1 / scale of a token's row
+  int xexp[8 * NT];                         // and the exponent of the sum of its magnitudes
+  // fp8: which copy of a row of the intermediate is read, and 1 / its scale: routed rows, then from kShared on tokens
+  static constexpr int kShared = 8 * NT * DSCA_MAX_TOPK;
+  float undo[F::kHalf ? kShared + 8 * NT : 1];
+  uint8_t copy[F::kHalf ? kShared + 8 * NT : 1];
   uint32_t xmax[kCompute][8];               // fp8, up to eight tokens: a warp's share of a row
   float xsum[kCompute][8];
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
@@ -378,7 +396,7 @@ __device__ __forceinline__ void select_token(const Args& a, S& s, int t, int par
   const bool v0 = e0 < E, v1 = e1 < E, first = blockIdx.x == 0 && !dry;
   if (a.x16 != nullptr && lane == 0 && !dry) {
     s.xinv[t] = __ldcg(a.xmeta + 2 * t);
-    s.hscale[t] = pow2(h_scale_exp(exp_of(__ldcg(a.xmeta + 2 * t + 1)), a.w1_exp, a.glu));
+    s.xexp[t] = exp_of(__ldcg(a.xmeta + 2 * t + 1));
   }
   if (a.w_gate != nullptr && (e0 == E || e1 == E) && !dry) s.sg[t] = 1.0f / (1.0f + expf(-(e0 == E ? l0 : l1)));
   if (first) {
@@ -598,8 +616,8 @@ __device__ __forceinline__ float4 tile_sum(const float* all, int splits, int pit
   return r;
 }
 // A lane's sums of 16-row tile q and token tile nt of an output tile.
-template <typename W, typename S>
-__device__ __forceinline__ void store_out(const Args& a, S& s, float4 v, int tile, int nt, int q, int lane) {
+template <typename W>
+__device__ __forceinline__ void store_out(const Args& a, float4 v, int tile, int nt, int q, int lane) {
   using X = typename W::X;
   const int r0 = tile * a.rt, rows = min(a.rt, a.d - r0);
   X* out = reinterpret_cast<X*>(a.out);
@@ -607,7 +625,7 @@ __device__ __forceinline__ void store_out(const Args& a, S& s, float4 v, int til
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int tk = nt * 8 + 2 * (lane & 3) + (i & 1), rr = 16 * q + (lane >> 2) + (i >> 1) * 8;
-    if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(W::kSize == 1 ? c[i] / s.hscale[tk] : c[i]);
+    if (tk < a.T && rr < rows) out[(size_t)tk * a.d + r0 + rr] = X(c[i]);
   }
 }
 
@@ -627,6 +645,8 @@ __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, i
     const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, part, parts, lane);
     if (lane == 0) a.lg[(size_t)(t * kLgPitch + r) * parts + part] = v;
   }
+  if (a.hmax != nullptr && cta == 0)
+    for (int r = wi * 32 + lane; r < a.T * (a.k + 1); r += nw * 32) a.hmax[r] = 0u;
   // fp8 weights, more than eight tokens: the t-th last CTA (the first have one dot product
   // more) writes token t's row in f16 (eight or less: the compute warps convert what they keep of it)
   const int counted = a.x16 != nullptr ? G : min(nd, G);  // CTAs that have a part in this
@@ -726,6 +746,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(smem_u32(&s.part_empty[threadIdx.x]), 1);
   }
   if (threadIdx.x >= 128 && threadIdx.x < 128 + DSCA_MAX_EXPERTS) s.emask[threadIdx.x - 128] = 0u;
+  if constexpr (kHalf)
+    for (int i = threadIdx.x; i < (int)sizeof(s.copy); i += kThreads) s.copy[i] = 0;
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&s.routed), 1);
     s.abort = 0;
@@ -967,10 +989,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int e = x_scale_exp(m);
       xs = pow2(e);
-      if (warp == 0 && t4 == 0) {
+      if (t4 == 0) {  // the same in every warp, which reads its own in GEMM2
         s.xinv[g] = pow2(-e);
-        s.hscale[g] = pow2(h_scale_exp(exp_of(l1), a.w1_exp, a.glu));
+        s.xexp[g] = exp_of(l1);
       }
+      __syncwarp();
       if (keep) {
         halve(va);
         halve(vb);
@@ -1161,7 +1184,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
     auto h_at = [&](int i, int n, int k) {
-      return i < 0 ? a.hs + ((size_t)n * a.hsp + k) * (kF32 ? 4 : 2) : a.h + ((size_t)s.asg[i][n] * a.hp + k) * (kF32 ? 4 : 2);
+      int row = i < 0 ? n : s.asg[i][n];
+      if constexpr (kHalf) row += s.copy[(i < 0 ? S::kShared : 0) + row] * (i < 0 ? a.T : a.T * a.k);
+      return (i < 0 ? a.hs : a.h) + ((size_t)row * (i < 0 ? a.hsp : a.hp) + k) * (kF32 ? 4 : 2);
+    };
+    // fp8: for each row of the (complete) shared or routed intermediate, the copy to read and 1 / its scale.  Every
+    // warp writes the same values for itself.
+    auto choose_copies = [&](bool sh) {
+      for (int r = lane; r < (sh ? a.T : a.T * a.k); r += 32) {
+        const int c = h_copy(__ldcg(a.hmax + (sh ? a.T * a.k : 0) + r)), at = (sh ? S::kShared : 0) + r;
+        s.copy[at] = (uint8_t)c;
+        // r / k exactly, for r < 256 and k <= 8
+        s.undo[at] = pow2(-h_scale_exp(s.xexp[sh ? r : (r * a.inv_k) >> 16], a.w1_exp, a.glu) - kCopyExp * c);
+      }
+      __syncwarp();
     };
     auto load_h = [&](uint4 (&v)[kVals], int i, int n, int k) {
       const int kend = i < 0 ? a.k2s : a.k2, bk = i < 0 ? a.b2s : a.b2;
@@ -1200,15 +1236,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       seek(i, j, info);
       auto step = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const bool sh = i < 0;
-        if (sh ? !have_s : !have_r) {
+        const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
+        // fp8: a fresh intermediate's copies are looked up while the first box's values are on their way, from the
+        // first copies, which rows of weights of one magnitude mostly have; they are asked for anew where a lane's
+        // row has another one (false).  With few tokens both by one piece of code (one token 27.8 us, 28.9 with one
+        // for the first box).
+        auto first_copies = [&]() {
+          choose_copies(sh);
+          return (bool)__all_sync(0xffffffffu, s.copy[sh ? S::kShared + min(n0 + g, a.T - 1) : (int)s.asg[i][n0 + g]] == 0);
+        };
+        float un[2] = {1.0f, 1.0f};  // and 1 / scale of the rows of this lane's two columns
+        auto columns = [&]() {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int n = n0 + 2 * t4 + c;
+            un[c] = s.undo[sh ? S::kShared + min(n, a.T - 1) : (int)s.asg[i][n]];
+          }
+        };
+        const bool fresh = sh ? !have_s : !have_r;
+        if (fresh) {
           if (lane == 0) {
             if (sh) waits.counter(a.ctr + kCtrShared, (uint32_t)(a.ups * (SUB == 2 ? (a.T + 7) / 8 : 1)));
             else waits.counter(a.ctr + kCtrRouted, s.handed);
           }
           __syncwarp();
           if (sh) have_s = true; else have_r = true;
+          if constexpr (kHalf && !kDirect) {
+            load_h(v, i, n0, k);
+            ready = first_copies();
+          }
         }
-        const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
         const int n_tok = sh ? a.T : (int)(info >> 8 & 255u);
         uint32_t next = info;
         const bool last = kF32 || n0 + 8 >= n_tok;
@@ -1228,6 +1285,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             sc[q][1] = __ldg(f + min(16 * q + g + 8, rows - 1));
           }
         }
+        if constexpr (kHalf && !kDirect) columns();
+        auto scaled = [&](float v, int c) { return kHalf ? v * un[c] : v; };
         auto join = [&](const float (&acc)[kSub2][4], int n0) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -1237,8 +1296,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               float* o = p + ((tk >> 3) * kSub2 * 32 + g * 4 + ((tk & 7) >> 1)) * 4 + (tk & 1);
 #pragma unroll
               for (int q = 0; q < kSub2; ++q) {
-                o[q * 128] = fmaf(acc[q][c], sc[q][0], o[q * 128]);
-                o[q * 128 + 2] = fmaf(acc[q][2 + c], sc[q][1], o[q * 128 + 2]);
+                o[q * 128] = fmaf(scaled(acc[q][c], c), sc[q][0], o[q * 128]);
+                o[q * 128 + 2] = fmaf(scaled(acc[q][2 + c], c), sc[q][1], o[q * 128 + 2]);
               }
             }
           }
@@ -1252,6 +1311,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             join(acc, n0);
           }
         } else {
+          if constexpr (kHalf && kDirect) {
+            bool look = fresh;
+#pragma unroll 1
+            while (!ready) {
+              load_h(v, i, n0, k);
+              ready = !look || first_copies();
+              look = false;
+            }
+            columns();
+          }
           if (!ready) load_h(v, i, n0, k);
           ready = ni < n_act && (ni < 0 || have_r);
           if (ready) load_h(w, ni, nn, nj * (ni < 0 ? a.b2s : a.b2));
@@ -1267,12 +1336,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kDirect) {
             const uint32_t m = (sh ? 0xffu : s.mask[i]) >> (2 * t4);
             if (m & 1u) {
-              sum[0] = fmaf(acc[0][0], sc[0][0], sum[0]);
-              sum[2] = fmaf(acc[0][2], sc[0][1], sum[2]);
+              sum[0] = fmaf(scaled(acc[0][0], 0), sc[0][0], sum[0]);
+              sum[2] = fmaf(scaled(acc[0][2], 0), sc[0][1], sum[2]);
             }
             if (m & 2u) {
-              sum[1] = fmaf(acc[0][1], sc[0][0], sum[1]);
-              sum[3] = fmaf(acc[0][3], sc[0][1], sum[3]);
+              sum[1] = fmaf(scaled(acc[0][1], 1), sc[0][0], sum[1]);
+              sum[3] = fmaf(scaled(acc[0][3], 1), sc[0][1], sum[3]);
             }
           } else {
             join(acc, n0);
@@ -1302,7 +1371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int w = 0; w < kCompute; ++w) add(c, *reinterpret_cast<const float4*>(s.sums[w][q / kSub2][q % kSub2][lane]));
-          if (a.splits == 1) store_out<W>(a, s, c, tile, q / kSub2, q % kSub2, lane);
+          if (a.splits == 1) store_out<W>(a, c, tile, q / kSub2, q % kSub2, lane);
           else *reinterpret_cast<float4*>(all + (split * kTiles + q) * 128) = c;
         }
         if (a.splits > 1) {
@@ -1316,7 +1385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           compute_sync();
           if (s.last)
             for (int q = warp; q < kTiles; q += kCompute)
-              store_out<W>(a, s, tile_sum(all + q * 128, a.splits, kTiles * 128), tile, q / kSub2, q % kSub2, lane);
+              store_out<W>(a, tile_sum(all + q * 128, a.splits, kTiles * 128), tile, q / kSub2, q % kSub2, lane);
         }
         compute_sync();
       }
@@ -1381,7 +1450,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           float wt[2];
           size_t at[2];
           bool on[2];
-          int tok[2];
+          int tok[2], rows[2];
+          uint32_t top[2] = {0u, 0u};  // fp8: the largest magnitude of these columns
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int n = n0 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
@@ -1390,6 +1460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
             tok[i] = on[i] ? (sh || kDirect ? n : (int)s.tok[ai][n]) : 0;
             wt[i] = sh ? s.sg[row] : s.wt[row];
+            rows[i] = row;
             at[i] = (size_t)row * (sh ? a.hsp : a.hp);
           }
           if (!waited) wait_parts();
@@ -1409,12 +1480,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (!on[i]) continue;
-            const float xi = kHalf ? s.xinv[tok[i]] : 1.0f, f = kHalf ? wt[i] * s.hscale[tok[i]] : wt[i];
+            const float xi = kHalf ? s.xinv[tok[i]] : 1.0f;
+            const float f = kHalf ? wt[i] * pow2(h_scale_exp(s.xexp[tok[i]], a.w1_exp, a.glu)) : wt[i];
             auto put = [&](int ch, float val) {
               if constexpr (kF32) {
                 reinterpret_cast<float*>(base)[at[i] + ch] = val;
               } else if constexpr (kHalf) {
-                reinterpret_cast<__half*>(base)[at[i] + ch] = __float2half_rn(val);
+                __half* o = reinterpret_cast<__half*>(base) + at[i] + ch;
+#pragma unroll
+                for (int c = 0; c < kCopies; ++c) o[c * lo] = __float2half_rn(val * pow2(kCopyExp * c));
+                top[i] = max(top[i], __float_as_uint(fabsf(val)));
               } else {
                 const __nv_bfloat16 hi = __float2bfloat16_rn(val);
                 const float rest = val - __bfloat162float(hi);
@@ -1436,6 +1511,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
+          if constexpr (kHalf) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+              for (int off = 4; off <= 16; off <<= 1) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+              if (g == 0 && on[i]) atomicMax(a.hmax + (sh ? a.T * a.k : 0) + rows[i], top[i]);
+            }
+          }
         }
         free_parts();
         ++owed[sh ? 0 : 1];
@@ -1453,7 +1536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int w = 0; w < kCompute; ++w) add(c, *reinterpret_cast<const float4*>(s.part[seq % kParts][w][0][0][lane]));
         if (a.splits == 1) {
-          store_out<W>(a, s, c, tile, 0, 0, lane);
+          store_out<W>(a, c, tile, 0, 0, lane);
           free_parts();
         } else {
           float* all = a.partial + (size_t)tile * a.splits * 128 + lane * 4;
@@ -1466,7 +1549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           before = __shfl_sync(0xffffffffu, before, 0);
           if (before == (uint32_t)a.splits - 1u) {
             __threadfence();
-            store_out<W>(a, s, tile_sum(all, a.splits, 128), tile, 0, 0, lane);
+            store_out<W>(a, tile_sum(all, a.splits, 128), tile, 0, 0, lane);
             if (lane == 0) a.ctr[kCtrTiles + tile] = 0u;
           }
         }
@@ -1501,6 +1584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+constexpr int kHBytes = 2 * kCopies;  // of a value of the intermediate, at most
 constexpr int kMaxItems = 256;  // items whose sums the workspace holds, 32 rows x 32 tokens each
 constexpr size_t kPartialBytes = (size_t)kMaxItems * 4 * 2 * 512;
 
@@ -1643,8 +1727,8 @@ int launch_t(const Args& a, const dsca_few_args* p, int sms, cudaStream_t stream
 size_t few_workspace_bytes(int T, int d, int k, int inter, int shared_inter) {
   const size_t hp = few::round_up(inter, 64), hsp = few::round_up(shared_inter, 64);
   const size_t x16 = T > 8 ? (size_t)T * (d * 2 + 8) : 0;  // fp8 weights
-  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * few::kDotParts * 8 + (size_t)T * k * hp * 4 + (size_t)T * hsp * 4 +
-         (x16 + 255) / 256 * 256 + few::kPartialBytes;
+  return DSCA_FEW_ZERO_BYTES + (size_t)T * few::kLgPitch * few::kDotParts * 8 + (size_t)T * (k * hp + hsp) * few::kHBytes +
+         few::round_up(T * (k + 1) * 4, 256) + (x16 + 255) / 256 * 256 + few::kPartialBytes;
 }
 
 int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
@@ -1658,6 +1742,7 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.wait_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
   a.T = p->T; a.d = p->d; a.E = p->E; a.mode = p->mode; a.norm_topk = p->norm_topk;
   a.k = p->mode == DSCA_ROUTE_SWITCH_TOP1 ? 1 : p->top_k;
+  a.inv_k = (1 << 16) / a.k + 1;
   a.glu = p->act == DSCA_ACT_SWIGLU;
   a.n1p = p->n1p; a.ip = p->ip; a.dp = p->dp; a.s_ip = p->shared_ip;
   const int shared = p->w_shared_gate != nullptr ? p->shared_inter : 0;
@@ -1667,11 +1752,12 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.ctr = (uint32_t*)w;
   a.lg = (double*)(w + DSCA_FEW_ZERO_BYTES);
   a.h = w + DSCA_FEW_ZERO_BYTES + (size_t)a.T * few::kLgPitch * few::kDotParts * 8;
-  a.hs = a.h + (size_t)a.T * a.k * a.hp * 4;
+  a.hs = a.h + (size_t)a.T * a.k * a.hp * few::kHBytes;
   a.partial = (float*)(w + few_workspace_bytes(a.T, a.d, a.k, p->inter, shared) - few::kPartialBytes);
   if (p->weights == DSCA_F8E4M3) {
+    a.hmax = (uint32_t*)(a.hs + (size_t)a.T * a.hsp * few::kHBytes);
     if (a.T > 8) {
-      a.x16 = a.hs + (size_t)a.T * a.hsp * 4;
+      a.x16 = (uint8_t*)a.hmax + few::round_up(a.T * (a.k + 1) * 4, 256);
       a.xmeta = (float*)(a.x16 + (size_t)a.T * a.d * 2);
     }
     int e = 0;
