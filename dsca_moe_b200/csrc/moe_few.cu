@@ -55,15 +55,17 @@
 // that takes its largest value to [2^14, 2^15) is exact in f16 down to 2^-29 of that value.  The
 // intermediate (one f16 term: it is off by 2^-11 at most where the output's bf16 is by 2^-8 and the weights'
 // own rounding by 2^-4; with a second one, twice the loads and products of
-// GEMM2, 32 tokens took 183 us instead of 153 and one took 31 instead of 27) needs a scale before it is known: |h| <= B^2 (SwiGLU; B with ReLU), B =
-// max|w1| sum|x|, so 2^14 / B^2 rounded down to a power of two cannot overflow.  How far below the bound a row's
-// values are depends on the weights (some 2^20 where all are alike, 2^30 and more where a few rows or one expert
-// are much larger than the rest), so the intermediate is stored three times, each copy 2^20 times the one before
-// (infinite where it overflows), and the largest magnitude of each row is kept along: GEMM2 reads the first copy in
-// which that is at least 2^-5, where every value has 11 significant bits or is off by 2^-20 of the row's largest,
-// as long as that largest value is not below 2^-59 of the bound.
-#include <math.h>
-
+// GEMM2, 32 tokens took 183 us instead of 153 and one took 31 instead of 27) needs a scale before it is known.  An
+// e4m3 weight is 448 times its row's scale at most, so |h| <= B = max(s_gate s_up) (448 sum|x|)^2 (SwiGLU; max(s) 448
+// sum|x| with ReLU), the maximum over the expert's channels, and 2^14 / B rounded down to a power of two cannot
+// overflow.  The maxima are taken anew in every call, while the router runs: they go with whatever the scales hold
+// then.  How far below the bound a row's values are depends on the weights (some 2^15 to 2^20 where all rows are
+// alike, 2^40 and more where a few are much larger, or are all zeros and have the scale 1), so the intermediate is
+// stored three times, each copy 2^20 times the one before (infinite where it overflows), and it is noted for each row
+// whether its largest magnitude reaches 2^-9 in the first copy or in the second: GEMM2 reads the first copy in which
+// it does, where every value has 11 significant bits or is off by 2^-16 of the row's largest, as long as that is at
+// least 2^-58 of B (2^-63, and the exponents' rounding up takes some 2^4).  Mostly that is the first copy for all rows,
+// as the values of an expert's first unit show already, and then nothing has to be looked up.
 #include <type_traits>
 
 #include "common.cuh"
@@ -88,7 +90,11 @@ constexpr int kCopies = 3;                // of the intermediate, fp8 weights
 constexpr int kCopyExp = 20;              // each is 2^20 times the one before
 
 // words of the counter block
-enum { kCtrLogits = 0, kCtrShared = 1, kCtrRouted = 2, kCtrExit = 3, kCtrTiles = 8 };
+// kCtrBound + e: fp8 weights, 1 + the largest exponent (GLU: sum of the exponents) of the scales of expert e's channels,
+// as they are stored (biased); e = E: the shared expert
+// behind kCtrShared and kCtrRouted: fp8 weights, how many rows of that intermediate reach kReaches0 in their first unit
+enum { kCtrLogits = 0, kCtrExit = 1, kCtrShared = 2, kCtrRouted = 4, kCtrTiles = 8, kCtrBound = 128 };
+static_assert(kCtrBound + DSCA_MAX_EXPERTS <= DSCA_FEW_ZERO_BYTES / 4, "counters are within the zeroed bytes");
 
 struct Args {
   const void* x;
@@ -104,15 +110,14 @@ struct Args {
   double* lg;       // [T][64][4] parts of the logits, column E = shared gate
   uint8_t* x16;     // fp8 weights, more than eight tokens: [T][d] token rows in f16
   float* xmeta;     // and [T][2]: 1 / their scale, the largest power of two below sum|x|
-  uint32_t* hmax;   // fp8 weights: [T * k], then [T]: largest magnitude of a row of h / hs (float bits of the first copy)
+  uint32_t* reach;  // fp8 weights: [T * k], then [T]: the sizes (h_reach) that values of a row of h / hs have
   uint8_t* h;       // [T * k][hp] intermediate: high terms, then the low terms; or fp32; or the f16 copies
   uint8_t* hs;      // [T][hsp] the shared expert's
   uint32_t* ctr;
   int32_t* err;
   int T, d, E, k, mode, norm_topk, glu;
   int n1p, ip, dp, s_ip;
-  int w1_exp;             // fp8: max|w1| < 2^w1_exp
-  int inv_k;              // 2^16 / k + 1
+  int inter, s_inter;     // channels of a routed expert / of the shared one
   int hp, hsp;            // row pitch of h / hs in values
   int upe, ups;           // units (16 or 32 weight rows of GEMM1) per routed expert / of the shared expert
   int k2, k2s;            // values of a row of w2 / ws2 that are read
@@ -180,16 +185,18 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // Exponent of the scale that takes a row whose largest magnitude has these bf16 bits to [2^14, 2^15),
 // within what fp32 holds together with its inverse.
 __device__ __forceinline__ int x_scale_exp(uint32_t max_bits) { return 141 - max(15, min(254, (int)(max_bits >> 7))); }
-// Exponent of the scale of the intermediate's first copy (see the top): sum|x| < 2^(e + 1), max|w1| < 2^w.  At most
-// 80, so that the last copy's inverse is a normal float.
-__device__ __forceinline__ int h_scale_exp(int e, int w, bool glu) {
-  const int b = e + 1 + w;
-  return max(-126, min(80, 14 - (glu ? 2 * b : b)));
+// Exponent of the scale of the intermediate's first copy (see the top): sum|x| < 2^(e + 1), bound: the expert's word
+// at kCtrBound (a stored exponent x stands for less than 2^(x - 126), and 448 < 2^9).  At most 80, so that the
+// last copy's inverse is a normal float.
+__device__ __forceinline__ int h_scale_exp(int e, int bound, bool glu) {
+  const int b = glu ? bound - 1 - 2 * 126 + 18 + 2 * (e + 1) : bound - 1 - 126 + 9 + e + 1;
+  return max(-126, min(80, 14 - b));
 }
-// the copy to read of a row whose largest magnitude has these bits (an infinity or a NaN is in each)
-__device__ __forceinline__ int h_copy(uint32_t max_bits) {
-  return max_bits >= __float_as_uint(0x1p-5f) ? 0 : max_bits >= __float_as_uint(0x1p-25f) ? 1 : 2;
-}
+// The sizes that a value of the first copy brings to its row (an infinity or a NaN brings both), and the copy to read
+// of a row with these.
+constexpr uint32_t kReaches0 = 1, kReaches1 = 2;
+__device__ __forceinline__ uint32_t h_reach(float v) { return fabsf(v) < 0x1p-29f ? 0u : fabsf(v) < 0x1p-9f ? kReaches1 : kReaches0 | kReaches1; }
+__device__ __forceinline__ int h_copy(uint32_t reach) { return reach & kReaches0 ? 0 : reach & kReaches1 ? 1 : 2; }
 // the exponent of a non-negative float
 __device__ __forceinline__ int exp_of(float v) { return (int)(__float_as_uint(v) >> 23) - 127; }
 // eight bf16 values times s -> f16
@@ -222,9 +229,9 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+__device__ __forceinline__ uint64_t ld_acquire(const uint32_t* p) {
+  uint64_t v;
+  asm volatile("ld.acquire.gpu.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
 // The kernel's waits, every one bounded.  One that has run out records the error and raises the CTA's flag,
@@ -250,20 +257,24 @@ struct Waits {
       if ((it & 15u) == 0u && over(t0)) return false;
     }
   }
-  // until *p has reached `target` (one thread; the counters only grow during a call).  As a signed distance:
-  // a workspace whose counter starts too low makes the wait run out.
-  __device__ __forceinline__ bool counter(const uint32_t* p, uint32_t target) const {
-    if ((int32_t)(ld_acquire(p) - target) >= 0) return true;
+  // until *p has reached `target` (one thread; the counters only grow during a call); the word behind it at that
+  // moment, 0 if the wait was given up.  As a signed distance: a workspace whose counter starts too low makes the
+  // wait run out.
+  __device__ __forceinline__ uint32_t counter(const uint32_t* p, uint32_t target) const {
+    uint64_t v = ld_acquire(p);
+    if ((int32_t)((uint32_t)v - target) >= 0) return (uint32_t)(v >> 32);
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
-      if ((int32_t)(ld_acquire(p) - target) >= 0) return true;
-      if ((it & 15u) == 0u && (*abort || over(t0))) return false;
+      v = ld_acquire(p);
+      if ((int32_t)((uint32_t)v - target) >= 0) return (uint32_t)(v >> 32);
+      if ((it & 15u) == 0u && (*abort || over(t0))) return 0u;
     }
   }
 };
-__device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n) {
+// n to *p, and `behind` to the word behind it
+__device__ __forceinline__ void ctr_add(uint32_t* p, uint32_t n, uint32_t behind = 0u) {
   __threadfence();
-  atomicAdd(p, n);
+  atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)behind << 32 | n);
 }
 
 // ---------------------------------------------------------------- shared memory
@@ -298,10 +309,11 @@ struct Smem {
   float sg[8 * NT];                         // shared-expert gate
   float xinv[8 * NT];                       // fp8: 1 / scale of a token's row
   int xexp[8 * NT];                         // and the exponent of the sum of its magnitudes
-  // fp8: which copy of a row of the intermediate is read, and 1 / its scale: routed rows, then from kShared on tokens
+  // fp8: which copy of a row of the intermediate is read: routed rows, then from kShared on tokens
   static constexpr int kShared = 8 * NT * DSCA_MAX_TOPK;
-  float undo[F::kHalf ? kShared + 8 * NT : 1];
   uint8_t copy[F::kHalf ? kShared + 8 * NT : 1];
+  float undo[F::kHalf && !F::kDirect ? kShared + 8 * NT : 1];  // and 1 / scale of its first copy
+  uint32_t bound[F::kHalf ? DSCA_MAX_EXPERTS : 1];  // the words at kCtrBound
   uint32_t xmax[kCompute][8];               // fp8, up to eight tokens: a warp's share of a row
   float xsum[kCompute][8];
   uint32_t emask[DSCA_MAX_EXPERTS];         // tokens of an expert
@@ -605,6 +617,34 @@ __device__ __forceinline__ void group_sync(int threads) { asm volatile("bar.sync
 
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kCompute * 32) : "memory"); }
 
+// Where the compute warps do not route: one of the routing warps announces their share of the bounds.
+__device__ __forceinline__ void bounds_arrive() { asm volatile("bar.arrive 3, %0;" ::"n"((kCompute + 1) * 32) : "memory"); }
+__device__ __forceinline__ void bounds_sync() { asm volatile("bar.sync 3, %0;" ::"n"((kCompute + 1) * 32) : "memory"); }
+
+// fp8: this warp's share of the bounds of all experts (see kCtrBound), 256 rows of w1 at a time.  Scales that are not
+// finite are left out: their channels' values are not finite whatever the scale.
+__device__ __forceinline__ void find_bounds(const Args& a, int warp, int lane) {
+  const int per = a.glu ? 128 : 256, ce = (a.inter + per - 1) / per, cs = (a.s_inter + per - 1) / per;
+  auto exponent = [](float s) { return __float_as_uint(s) >> 23 & 255u; };
+#pragma unroll 1
+  for (int q = warp * gridDim.x + blockIdx.x; q < a.E * ce + cs; q += kCompute * gridDim.x) {
+    const bool sh = q >= a.E * ce;
+    const int e = sh ? a.E : q / ce, c = sh ? q - a.E * ce : q % ce, left = (sh ? a.s_inter : a.inter) - c * per;
+    const float* sc = (sh ? a.ws1s : a.w1s + (size_t)e * a.n1p) + c * 256 + lane;
+    uint32_t m = 0u;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __ldg(sc + 32 * i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = exponent(v[i]), y = a.glu ? exponent(v[(i + 4) & 7]) : 0u;
+      if ((!a.glu || i < 4) && lane + 32 * i < left && x != 255u && y != 255u) m = max(m, x + y + 1u);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) atomicMax(a.ctr + kCtrBound + e, m);
+  }
+}
+
 __device__ __forceinline__ void add(float4& c, float4 o) {
   c.x += o.x; c.y += o.y; c.z += o.z; c.w += o.w;
 }
@@ -631,7 +671,7 @@ __device__ __forceinline__ void store_out(const Args& a, float4 v, int tile, int
 
 // Router: fp64 dot products spread over the grid, then softmax, selection and the expert lists in every
 // CTA for itself.  Warp wi of the nw warps that take part (they share named barrier 1).
-template <typename X, int SUB, int kTokens, bool kDirect, typename S>
+template <typename X, int SUB, int kTokens, bool kDirect, bool kHalf, typename S>
 __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, int wi, int nw, int lane) {
   const int G = gridDim.x, cta = blockIdx.x;
   // a logit's product in four parts while that leaves a warp one (one token of the Qwen block 32.7 us, whole
@@ -645,11 +685,11 @@ __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, i
     const double v = dot64(reinterpret_cast<const X*>(a.x) + (size_t)t * a.d, w, a.d, part, parts, lane);
     if (lane == 0) a.lg[(size_t)(t * kLgPitch + r) * parts + part] = v;
   }
-  if (a.hmax != nullptr && cta == 0)
-    for (int r = wi * 32 + lane; r < a.T * (a.k + 1); r += nw * 32) a.hmax[r] = 0u;
+  if (kHalf && cta == 0)
+    for (int r = wi * 32 + lane; r < a.T * (a.k + 1); r += nw * 32) a.reach[r] = 0u;
   // fp8 weights, more than eight tokens: the t-th last CTA (the first have one dot product
   // more) writes token t's row in f16 (eight or less: the compute warps convert what they keep of it)
-  const int counted = a.x16 != nullptr ? G : min(nd, G);  // CTAs that have a part in this
+  const int counted = kHalf ? G : min(nd, G);  // CTAs that have a part in this
   for (int tc = G - 1 - cta; a.x16 != nullptr && wi == nw - 1 && tc < a.T; tc += G) {
     const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const X*>(a.x) + (size_t)tc * a.d);
     uint4* dst = reinterpret_cast<uint4*>(a.x16) + (size_t)tc * (a.d / 8);
@@ -669,6 +709,7 @@ __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, i
     }
   }
   group_sync(nw * 32);
+  if (kHalf && wi == 0 && nw == kServices) bounds_sync();
   if (wi == 0 && lane == 0 && cta < counted) ctr_add(a.ctr + kCtrLogits, 1u);
   __syncwarp();
   for (int t = wi - nw; t < a.T; t += nw) {
@@ -683,6 +724,12 @@ __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, i
     group_sync(nw * 32);
   }
   group_sync(nw * 32);
+  if constexpr (kHalf) {
+    if (wi == nw - 1) {
+      s.bound[lane] = __ldcg(a.ctr + kCtrBound + lane);
+      s.bound[lane + 32] = __ldcg(a.ctr + kCtrBound + lane + 32);
+    }
+  }
   if (wi == 0) {
     const uint32_t m0 = s.emask[lane], m1 = s.emask[lane + 32];
     const uint32_t b0 = __ballot_sync(0xffffffffu, m0 != 0u), b1 = __ballot_sync(0xffffffffu, m1 != 0u);
@@ -699,6 +746,9 @@ __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, i
     }
   }
   group_sync(nw * 32);
+  if constexpr (kHalf && !kDirect)
+    if (wi == 0 && lane < a.T && a.w_gate != nullptr)
+      s.undo[S::kShared + lane] = pow2(-h_scale_exp(s.xexp[lane], (int)s.bound[a.E], a.glu));
   for (int i = wi; i < s.n_act; i += nw) {
     const int e = s.act[i];
     const uint32_t m = s.emask[e];
@@ -713,6 +763,8 @@ __device__ __forceinline__ void route(const Args& a, S& s, const Waits& waits, i
     if (n < kTokens) {
       s.tok[i][n] = (uint8_t)t;
       s.asg[i][n] = (uint8_t)(t * a.k + s.slot[e][t]);
+      if constexpr (kHalf && !kDirect)
+        if (on) s.undo[s.asg[i][n]] = pow2(-h_scale_exp(s.xexp[t], (int)s.bound[e], a.glu));
     }
   }
   group_sync(nw * 32);
@@ -886,7 +938,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (on) s.left[w] = (uint32_t)st | phase << 8 | (uint32_t)wrapped << 9;
   } else if (warp < kCompute) {
     // ================================================================ compute
-    if (all_route) route<X, SUB, 8 * NT, kDirect>(a, s, waits, kServices + warp, route_warps, lane);
+    if (kHalf && all_route) find_bounds(a, warp, lane);
+    if (all_route) route<X, SUB, 8 * NT, kDirect, kHalf>(a, s, waits, kServices + warp, route_warps, lane);
     const uint32_t base = ring + (uint32_t)(warp * a.stages * a.stage);
     int st = 0, given = 0;  // next stage, sums handed over
     uint32_t phase = 0u;    // parity of the next stage's copy
@@ -944,6 +997,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (keep) {
         if (warp < a.n1) load_x(va, -1, a.T, 0, warp * a.b1);
         if (warp + kCompute < a.n1) load_x(vb, -1, a.T, 0, (warp + kCompute) * a.b1);
+      }
+    }
+    // behind the loads of x, which take as long
+    if constexpr (kHalf) {
+      if (!all_route) {
+        find_bounds(a, warp, lane);
+        bounds_arrive();
       }
     }
     float xs = 1.0f;  // the scale of token g's row
@@ -1183,20 +1243,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // join the warp's sums of all tokens in shared memory (a lane's values have places of their own).
     const size_t h_lo = (size_t)a.T * a.k * a.hp * 2, hs_lo = (size_t)a.T * a.hsp * 2;
     bool have_s = false, have_r = false;  // the intermediates, which come from every CTA's service warps
+    bool mixed = false;                   // fp8: not all rows of them are read from their first copy
     auto h_at = [&](int i, int n, int k) {
       int row = i < 0 ? n : s.asg[i][n];
-      if constexpr (kHalf) row += s.copy[(i < 0 ? S::kShared : 0) + row] * (i < 0 ? a.T : a.T * a.k);
+      if constexpr (kHalf)
+        if (mixed) row += s.copy[(i < 0 ? S::kShared : 0) + row] * (i < 0 ? a.T : a.T * a.k);
       return (i < 0 ? a.hs : a.h) + ((size_t)row * (i < 0 ? a.hsp : a.hp) + k) * (kF32 ? 4 : 2);
     };
-    // fp8: for each row of the (complete) shared or routed intermediate, the copy to read and 1 / its scale.  Every
-    // warp writes the same values for itself.
+    // fp8: the copy to read of each row of the (complete) shared or routed intermediate, where not all are known to be the
+    // first.  Every warp writes the same for itself.
     auto choose_copies = [&](bool sh) {
-      for (int r = lane; r < (sh ? a.T : a.T * a.k); r += 32) {
-        const int c = h_copy(__ldcg(a.hmax + (sh ? a.T * a.k : 0) + r)), at = (sh ? S::kShared : 0) + r;
-        s.copy[at] = (uint8_t)c;
-        // r / k exactly, for r < 256 and k <= 8
-        s.undo[at] = pow2(-h_scale_exp(s.xexp[sh ? r : (r * a.inv_k) >> 16], a.w1_exp, a.glu) - kCopyExp * c);
-      }
+#pragma unroll 1
+      for (int r = lane; r < (sh ? a.T : a.T * a.k); r += 32)
+        s.copy[(sh ? S::kShared : 0) + r] = (uint8_t)h_copy(__ldcg(a.reach + (sh ? a.T * a.k : 0) + r));
       __syncwarp();
     };
     auto load_h = [&](uint4 (&v)[kVals], int i, int n, int k) {
@@ -1237,33 +1296,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto step = [&](uint4 (&v)[kVals], uint4 (&w)[kVals]) {
         const bool sh = i < 0;
         const int bk = sh ? a.b2s : a.b2, pitch = bk * W::kSize, blk = sh ? blk2s : blk2, k = j * bk;
-        // fp8: a fresh intermediate's copies are looked up while the first box's values are on their way, from the
-        // first copies, which rows of weights of one magnitude mostly have; they are asked for anew where a lane's
-        // row has another one (false).  With few tokens both by one piece of code (one token 27.8 us, 28.9 with one
-        // for the first box).
-        auto first_copies = [&]() {
-          choose_copies(sh);
-          return (bool)__all_sync(0xffffffffu, s.copy[sh ? S::kShared + min(n0 + g, a.T - 1) : (int)s.asg[i][n0 + g]] == 0);
-        };
-        float un[2] = {1.0f, 1.0f};  // and 1 / scale of the rows of this lane's two columns
-        auto columns = [&]() {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int n = n0 + 2 * t4 + c;
-            un[c] = s.undo[sh ? S::kShared + min(n, a.T - 1) : (int)s.asg[i][n]];
-          }
-        };
-        const bool fresh = sh ? !have_s : !have_r;
-        if (fresh) {
-          if (lane == 0) {
-            if (sh) waits.counter(a.ctr + kCtrShared, (uint32_t)(a.ups * (SUB == 2 ? (a.T + 7) / 8 : 1)));
-            else waits.counter(a.ctr + kCtrRouted, s.handed);
-          }
+        if (sh ? !have_s : !have_r) {
+          uint32_t reached = 0u;
+          if (lane == 0)
+            reached = sh ? waits.counter(a.ctr + kCtrShared, (uint32_t)(a.ups * (SUB == 2 ? (a.T + 7) / 8 : 1)))
+                         : waits.counter(a.ctr + kCtrRouted, s.handed);
           __syncwarp();
           if (sh) have_s = true; else have_r = true;
-          if constexpr (kHalf && !kDirect) {
-            load_h(v, i, n0, k);
-            ready = first_copies();
+          if constexpr (kHalf) {
+            if (__shfl_sync(0xffffffffu, reached, 0) != (uint32_t)(sh ? a.T : a.T * a.k)) {
+              mixed = true;
+              choose_copies(sh);
+            }
           }
         }
         const int n_tok = sh ? a.T : (int)(info >> 8 & 255u);
@@ -1285,7 +1329,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             sc[q][1] = __ldg(f + min(16 * q + g + 8, rows - 1));
           }
         }
-        if constexpr (kHalf && !kDirect) columns();
+        float un[2] = {1.0f, 1.0f};  // fp8: 1 / scale of the rows of this lane's two columns
+        if constexpr (kHalf) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int n = n0 + 2 * t4 + c, row = sh ? S::kShared + min(n, a.T - 1) : (int)s.asg[i][n];
+            if constexpr (kDirect) un[c] = pow2(-h_scale_exp(s.xexp[n], (int)s.bound[sh ? a.E : (int)(info & 255u)], a.glu));
+            else un[c] = s.undo[row];
+            if (mixed) un[c] *= pow2(-kCopyExp * s.copy[row]);
+          }
+        }
         auto scaled = [&](float v, int c) { return kHalf ? v * un[c] : v; };
         auto join = [&](const float (&acc)[kSub2][4], int n0) {
 #pragma unroll
@@ -1311,16 +1364,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             join(acc, n0);
           }
         } else {
-          if constexpr (kHalf && kDirect) {
-            bool look = fresh;
-#pragma unroll 1
-            while (!ready) {
-              load_h(v, i, n0, k);
-              ready = !look || first_copies();
-              look = false;
-            }
-            columns();
-          }
           if (!ready) load_h(v, i, n0, k);
           ready = ni < n_act && (ni < 0 || have_r);
           if (ready) load_h(w, ni, nn, nj * (ni < 0 ? a.b2s : a.b2));
@@ -1393,16 +1436,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================================================ service
     const int sw = warp - kService;
-    route<X, SUB, 8 * NT, kDirect>(a, s, waits, sw, route_warps, lane);
+    route<X, SUB, 8 * NT, kDirect, kHalf>(a, s, waits, sw, route_warps, lane);
     const int2 ru = routed_units(wait_routed());
     const int nu = nu_s + ru.y;
     const size_t h_lo = (size_t)a.T * a.k * a.hp, hs_lo = (size_t)a.T * a.hsp;
     uint32_t owed[2] = {0u, 0u};  // handings over of the shared expert / the routed experts stored, not announced
+    uint32_t reached = 0u;        // fp8: rows that reach kReaches0 in these, if they are of first units
     auto announce = [&](int which, uint32_t* ctr) {
       if (owed[which] == 0u) return;
       __syncwarp();
-      if (lane == 0) ctr_add(ctr, owed[which]);
-      owed[which] = 0u;
+      if (lane == 0) ctr_add(ctr, owed[which], reached);
+      owed[which] = reached = 0u;
     };
     // Every second handing over is this warp's.
     int seq = 0;
@@ -1413,6 +1457,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[seq % kParts]));
     };
     int ai = 0, first = 0;  // active expert of the present routed unit, and that expert's first one
+    // fp8: the sizes that this warp has noted for the tokens from seen_n0 on of active expert seen_by (-1: shared)
+    uint32_t seen = 0u;
+    int seen_n0 = -1, seen_by = -1;
     for (int un = 0; un < nu; ++un) {
       const bool sh = un < nu_s;
       if (un == nu_s) announce(0, a.ctr + kCtrShared);
@@ -1450,8 +1497,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           float wt[2];
           size_t at[2];
           bool on[2];
-          int tok[2], rows[2];
-          uint32_t top[2] = {0u, 0u};  // fp8: the largest magnitude of these columns
+          int tok[2];
+          uint32_t reach[2] = {0u, 0u};  // fp8: sizes of these columns' values
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int n = n0 + 2 * t4 + i;  // column: the n-th token of the expert, or token n
@@ -1460,7 +1507,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int row = on[i] ? (sh ? n : (int)s.asg[ai][n]) : 0;
             tok[i] = on[i] ? (sh || kDirect ? n : (int)s.tok[ai][n]) : 0;
             wt[i] = sh ? s.sg[row] : s.wt[row];
-            rows[i] = row;
             at[i] = (size_t)row * (sh ? a.hsp : a.hp);
           }
           if (!waited) wait_parts();
@@ -1481,7 +1527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 2; ++i) {
             if (!on[i]) continue;
             const float xi = kHalf ? s.xinv[tok[i]] : 1.0f;
-            const float f = kHalf ? wt[i] * pow2(h_scale_exp(s.xexp[tok[i]], a.w1_exp, a.glu)) : wt[i];
+            const float f = kHalf ? wt[i] * pow2(h_scale_exp(s.xexp[tok[i]], (int)s.bound[sh ? a.E : e], a.glu)) : wt[i];
             auto put = [&](int ch, float val) {
               if constexpr (kF32) {
                 reinterpret_cast<float*>(base)[at[i] + ch] = val;
@@ -1489,7 +1535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __half* o = reinterpret_cast<__half*>(base) + at[i] + ch;
 #pragma unroll
                 for (int c = 0; c < kCopies; ++c) o[c * lo] = __float2half_rn(val * pow2(kCopyExp * c));
-                top[i] = max(top[i], __float_as_uint(fabsf(val)));
+                reach[i] |= h_reach(val);
               } else {
                 const __nv_bfloat16 hi = __float2bfloat16_rn(val);
                 const float rest = val - __bfloat162float(hi);
@@ -1512,12 +1558,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if constexpr (kHalf) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-              for (int off = 4; off <= 16; off <<= 1) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
-              if (g == 0 && on[i]) atomicMax(a.hmax + (sh ? a.T * a.k : 0) + rows[i], top[i]);
-            }
+            // the eight tokens' sizes side by side; what an expert's units before this one have brought is there already
+            if (n0 != seen_n0 || (sh ? -1 : ai) != seen_by) seen = 0u;
+            seen_n0 = n0;
+            seen_by = sh ? -1 : ai;
+            const uint32_t all = __reduce_or_sync(0xffffffffu, reach[0] << (4 * t4) | reach[1] << (4 * t4 + 2));
+            const uint32_t fresh = all & ~seen;
+            seen |= all;
+            if (u == 0) reached += __popc(all & kReaches0 * 0x5555u);
+            if (lane < 8 && (fresh >> (2 * lane) & 3u))
+              atomicOr(a.reach + (sh ? a.T * a.k + n0 + lane : (int)s.asg[ai][n0 + lane]), fresh >> (2 * lane) & 3u);
           }
         }
         free_parts();
@@ -1575,10 +1625,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   // ---- the last CTA to leave zeroes the counters for the next call
-  if (threadIdx.x == 0) {
-    __threadfence();
-    if (atomicAdd(a.ctr + kCtrExit, 1u) == (uint32_t)G - 1u) {
-      a.ctr[kCtrLogits] = a.ctr[kCtrShared] = a.ctr[kCtrRouted] = a.ctr[kCtrExit] = 0u;
+  if (warp == 0) {
+    uint32_t before = 0u;
+    if (lane == 0) {
+      __threadfence();
+      before = atomicAdd(a.ctr + kCtrExit, 1u);
+    }
+    if (__shfl_sync(0xffffffffu, before, 0) == (uint32_t)G - 1u) {
+      if (kHalf) a.ctr[kCtrBound + lane] = a.ctr[kCtrBound + 32 + lane] = 0u;
+      if (lane < kCtrTiles) a.ctr[lane] = 0u;
       __threadfence();
     }
   }
@@ -1669,7 +1724,7 @@ int launch(Args a, const dsca_few_args* p, int sms, cudaStream_t stream) {
   a.k2 = a.upe * unit;
   a.k2s = a.ups * unit;
   plan_tiles(a.d, sms, 16 * F::kSub2, &a.rt, &a.tiles, &a.splits);
-  if (a.splits > 1 && (kCtrTiles + a.tiles > DSCA_FEW_ZERO_BYTES / 4 || a.tiles * a.splits > kMaxItems)) return DSCA_ERR_CAPACITY;
+  if (a.splits > 1 && (kCtrTiles + a.tiles > kCtrBound || a.tiles * a.splits > kMaxItems)) return DSCA_ERR_CAPACITY;
   // a stage holds whole 16-row tiles: the rows behind a tile's last are read, and dropped
   const int rows = 16 * max(SUB, F::kSub2), most = min(kMaxBox, (kSmem - kFixed) / (2 * kCompute * rows) / 64 * 64);
   a.b1 = box_of<W, 1>(a.d * W::kSize, kCompute, most) / W::kSize;
@@ -1742,10 +1797,11 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.wait_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
   a.T = p->T; a.d = p->d; a.E = p->E; a.mode = p->mode; a.norm_topk = p->norm_topk;
   a.k = p->mode == DSCA_ROUTE_SWITCH_TOP1 ? 1 : p->top_k;
-  a.inv_k = (1 << 16) / a.k + 1;
   a.glu = p->act == DSCA_ACT_SWIGLU;
   a.n1p = p->n1p; a.ip = p->ip; a.dp = p->dp; a.s_ip = p->shared_ip;
   const int shared = p->w_shared_gate != nullptr ? p->shared_inter : 0;
+  a.inter = p->inter;
+  a.s_inter = shared;
   a.hp = few::round_up(p->inter, 64);
   a.hsp = few::round_up(shared, 64);
   uint8_t* w = (uint8_t*)p->workspace;
@@ -1755,14 +1811,11 @@ int launch_moe_few(const dsca_few_args* p, int num_sms, cudaStream_t stream) {
   a.hs = a.h + (size_t)a.T * a.k * a.hp * few::kHBytes;
   a.partial = (float*)(w + few_workspace_bytes(a.T, a.d, a.k, p->inter, shared) - few::kPartialBytes);
   if (p->weights == DSCA_F8E4M3) {
-    a.hmax = (uint32_t*)(a.hs + (size_t)a.T * a.hsp * few::kHBytes);
+    a.reach = (uint32_t*)(a.hs + (size_t)a.T * a.hsp * few::kHBytes);
     if (a.T > 8) {
-      a.x16 = (uint8_t*)a.hmax + few::round_up(a.T * (a.k + 1) * 4, 256);
+      a.x16 = (uint8_t*)a.reach + few::round_up(a.T * (a.k + 1) * 4, 256);
       a.xmeta = (float*)(a.x16 + (size_t)a.T * a.d * 2);
     }
-    int e = 0;
-    frexpf(p->w1_max, &e);  // w1_max < 2^e
-    a.w1_exp = max(-200, min(200, e));
   }
   if (p->weights == DSCA_BF16) return few::launch_t<few::Bf16>(a, p, num_sms, stream);
   if (p->weights == DSCA_F32) return few::launch_t<few::F32>(a, p, num_sms, stream);

@@ -143,14 +143,6 @@ def dequantize_fp8(pe: PackedExperts) -> PackedExperts:
     return f
 
 
-def _max_fp8(q: torch.Tensor | None, scale: torch.Tensor | None) -> float:
-    """Largest |q * scale| of e4m3 rows (0 without any)."""
-    if q is None:
-        return 0.0
-    top = (q.view(torch.uint8) & 0x7F).amax(-1).view(torch.float8_e4m3fn).float()  # magnitudes order like their bytes
-    return float((top * scale).max())
-
-
 def unpack_swiglu(pe: PackedExperts):
     """Inverse of pack_swiglu on float weights: (gate [E,I,d], up [E,I,d], down [E,d,I], shared)."""
     E, I, d, ip = pe.E, pe.inter, pe.d, pe.ip
@@ -438,10 +430,6 @@ class MoEEngine:
         self.few_tokens = 0
         self._few_ws = {}
         self._few_args, self._few_like = None, {}
-        # fp8: the largest magnitude of the first GEMMs' weights, from which forward_few scales its f16
-        # intermediates
-        self._w1_max = max(_max_fp8(experts.w1, experts.w1_scale), _max_fp8(experts.ws1, experts.ws1_scale)) \
-            if experts.fp8 else 0.0
         self.last_plan = None
         self.last_layout = None
         # when a list, forward() appends (name, cuda.Event) markers between its kernel launches
@@ -755,7 +743,7 @@ class MoEEngine:
             a.w1, a.w2, a.ws1, a.ws2 = _ptr(pe.w1), _ptr(pe.w2), _ptr(pe.ws1), _ptr(pe.ws2)
             a.w1_scale, a.w2_scale = _ptr(pe.w1_scale), _ptr(pe.w2_scale)
             a.ws1_scale, a.ws2_scale = _ptr(pe.ws1_scale), _ptr(pe.ws2_scale)
-            a.w1_max, a.err, a.wait_limit_ns = self._w1_max, _ptr(self.err), self.wait_limit_ns
+            a.err, a.wait_limit_ns = _ptr(self.err), self.wait_limit_ns
             self._few_bytes = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.d, self.top_k, pe.inter,
                                                                    pe.s_inter)
             self._few_args = a

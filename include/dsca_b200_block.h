@@ -61,8 +61,10 @@ DSCA_API int dsca_rms_norm(const dsca_rms_norm_args* a, dsca_stream_t stream);
  * dsca_grouped_ffn and dsca_combine in one, for a call whose time is the reading of the weights).
  *   logits = round(x W_r^T), summed in 64 bits and rounded to fp32, then to the type; probabilities, ties and weights as dsca_router_topk
  *   out    = round(sum_j w_j down(act(up x)) + sigmoid(round(x . g)) shared(x)), summed in fp32;
- *            the activated intermediate is held to 16 significant bits (DSCA_F32: fp32; DSCA_F8E4M3: 11 bits, or 2^-20
- *            of the largest value of its token's row in that expert where that is more)
+ *            the activated intermediate is held to 16 significant bits (DSCA_F32: fp32; DSCA_F8E4M3: 11 bits, or 2^-16
+ *            of the largest value of its token's row in that expert where that is more, for rows whose largest
+ *            value is at least 2^-58 of what the scales allow: max(s_gate s_up) (448 sum|x|)^2 with SwiGLU,
+ *            max(s) 448 sum|x| with ReLU)
  * Weights in the packing of dsca_ffn_args.  weights: DSCA_BF16 or DSCA_F32 (x, router and out in the
  * same type), or DSCA_F8E4M3 with the four scale arrays (x, router and out bf16).
  * d * (bytes of a weight) must be a multiple of 16 and every weight matrix 16-byte aligned.
@@ -92,10 +94,7 @@ typedef struct {
   const float* w2_scale;
   const float* ws1_scale;
   const float* ws2_scale;
-  float w1_max;               /* DSCA_F8E4M3: the largest magnitude among the (scaled) weights of w1 and ws1, or more: it
-                                 bounds the intermediate by b = w1_max * sum|x| (SwiGLU: b^2), from which its f16
-                                 scales come.  The accuracy above holds for rows whose largest value is at
-                                 least 2^-59 of the bound */
+  float w1_max;               /* DSCA_F8E4M3: not read (0, or any finite value that is not negative) */
   void* out;                  /* [T, d] */
   void* logits;               /* [T, E] */
   int32_t* topk_ids;          /* [T, top_k] */

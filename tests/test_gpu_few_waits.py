@@ -10,7 +10,7 @@ from test_gpu_few import _check, _engine, _run
 
 pytestmark = pytest.mark.gpu
 
-COUNTERS = {"logits": 0, "shared": 1, "routed": 2}
+COUNTERS = {"logits": 0, "shared": 2, "routed": 4}
 
 
 # up to four tokens two warps route beside the others' products, above all warps do; nine tokens and more are
