@@ -428,8 +428,8 @@ class MoEEngine:
         # its roundings (the intermediates and expert outputs are not rounded to bf16 here) and hold no
         # counts, token_row or other views of the scratch
         self.few_tokens = 0
-        self._few_ws = {}
-        self._few_args, self._few_like = None, {}
+        self._few_ws, self._few_like = {}, {}
+        self._few_now = self._few_experts = self._few_args = None
         self.last_plan = None
         self.last_layout = None
         # when a list, forward() appends (name, cuda.Event) markers between its kernel launches
@@ -716,38 +716,49 @@ class MoEEngine:
             return f"a weight row of {self.d} values is not a multiple of 16 bytes"
         return None
 
+    def _few_struct(self):
+        """dsca_few_args with everything that does not come from the call's tokens, as it is now: weights and
+        settings may have been replaced since the last call.  Filled anew only where something has changed
+        (comparing takes a microsecond, filling three)."""
+        pe, gate, addr = self.experts, self.shared_gate_weight, torch.Tensor.data_ptr
+        now = [self.top_k, self.route_mode, self.norm_topk, self.wait_limit_ns, addr(self.err), addr(self.router_weight),
+               addr(pe.w1), addr(pe.w2)]
+        if gate is not None:
+            now += addr(gate), addr(pe.ws1), addr(pe.ws2)
+        if pe.w1_scale is not None:
+            now += addr(pe.w1_scale), addr(pe.w2_scale)
+            if gate is not None:
+                now += addr(pe.ws1_scale), addr(pe.ws2_scale)
+        if now != self._few_now or pe is not self._few_experts:
+            a = L.FewArgs()
+            a.top_k, a.mode, a.norm_topk, a.wait_limit_ns, a.err, a.w_router, a.w1, a.w2 = now[:8]
+            a.d, a.E, a.weights = self.d, self.E, L.F8E4M3 if pe.fp8 else _dt(self.dtype)
+            a.act, a.inter, a.n1p, a.ip, a.dp = pe.act, pe.inter, pe.n1p, pe.ip, pe.dp
+            if gate is not None:
+                a.w_shared_gate, a.ws1, a.ws2 = now[8:11]
+                a.shared_inter, a.shared_n1p, a.shared_ip = pe.s_inter, pe.s_n1p, pe.s_ip
+            if pe.w1_scale is not None:
+                a.w1_scale, a.w2_scale = addr(pe.w1_scale), addr(pe.w2_scale)
+                if gate is not None:
+                    a.ws1_scale, a.ws2_scale = now[-2:]
+            a.workspace_bytes = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.d, self.top_k, pe.inter, pe.s_inter)
+            self._few_now, self._few_experts, self._few_args = now, pe, a
+        return L.FewArgs.from_buffer_copy(self._few_args)
+
     def _few_workspace(self):
-        """Scratch of dsca_moe_few (the current device is the engine's): one per stream, because calls
-        that may overlap must not share it.  A call that is being captured gets one of its own from the
+        """Scratch of dsca_moe_few (the current device is the engine's, _few_args are the call's): one per stream,
+        because calls that may overlap must not share it.  A call that is being captured gets one of its own from the
         graph's memory, with the part that must be zero zeroed by the graph."""
+        n = self._few_args.workspace_bytes
         if torch.cuda.is_current_stream_capturing():
-            ws = torch.empty(self._few_bytes, dtype=torch.uint8, device=self.device)
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device)
             ws[:L.FEW_ZERO_BYTES].zero_()
             return ws
         key = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
         ws = self._few_ws.get(key)
-        if ws is None:
-            ws = self._few_ws[key] = torch.zeros(self._few_bytes, dtype=torch.uint8, device=self.device)
+        if ws is None or ws.numel() < n:
+            ws = self._few_ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
         return ws
-
-    def _few_struct(self):
-        """dsca_few_args with everything that does not change from call to call."""
-        if self._few_args is None:
-            pe, a = self.experts, L.FewArgs()
-            a.w_router, a.w_shared_gate = _ptr(self.router_weight), _ptr(self.shared_gate_weight)
-            a.d, a.E, a.top_k = self.d, self.E, self.top_k
-            a.weights = L.F8E4M3 if pe.fp8 else _dt(self.dtype)
-            a.mode, a.norm_topk, a.act = self.route_mode, int(self.norm_topk), pe.act
-            a.inter, a.n1p, a.ip, a.dp = pe.inter, pe.n1p, pe.ip, pe.dp
-            a.shared_inter, a.shared_n1p, a.shared_ip = pe.s_inter, pe.s_n1p, pe.s_ip
-            a.w1, a.w2, a.ws1, a.ws2 = _ptr(pe.w1), _ptr(pe.w2), _ptr(pe.ws1), _ptr(pe.ws2)
-            a.w1_scale, a.w2_scale = _ptr(pe.w1_scale), _ptr(pe.w2_scale)
-            a.ws1_scale, a.ws2_scale = _ptr(pe.ws1_scale), _ptr(pe.ws2_scale)
-            a.err, a.wait_limit_ns = _ptr(self.err), self.wait_limit_ns
-            self._few_bytes = L.load().dsca_few_workspace_bytes(L.FEW_TOKENS, self.d, self.top_k, pe.inter,
-                                                                   pe.s_inter)
-            self._few_args = a
-        return L.FewArgs.from_buffer_copy(self._few_args)
 
     def forward_few(self, x: torch.Tensor) -> dict:
         """The whole block for at most 32 tokens in one kernel (dsca_moe_few): x [T, d] on this
@@ -768,23 +779,22 @@ class MoEEngine:
             x = x.to(dtype=self.dtype).contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-        like = self._few_like.get(T)
+        like = self._few_like.get((T, k))
         if like is None:  # an empty_like costs a third less host time than a tensor from sizes and a type
-            like = self._few_like[T] = (x.new_empty((T, self.E)), x.new_empty((T, k), dtype=torch.int32),
-                                        x.new_empty((T, k), dtype=torch.float32), x.new_empty(T, dtype=torch.int64))
+            like = self._few_like[T, k] = (x.new_empty((T, self.E)), x.new_empty((T, k), dtype=torch.int32),
+                                           x.new_empty((T, k), dtype=torch.float32), x.new_empty(T, dtype=torch.int64))
         new = torch.empty_like
         r = dict(out=new(x), logits=new(like[0]), topk_ids=new(like[1]), topk_w=new(like[2]), expert_index=new(like[3]))
         if T == 0:
             return r
-        a = self._few_struct()
+        a, addr = self._few_struct(), torch.Tensor.data_ptr
         if dev.index == torch._C._cuda_getDevice():
             ws = self._few_workspace()
         else:
             with torch.cuda.device(dev):
                 ws = self._few_workspace()
-        a.T, a.x, a.out, a.logits = T, x.data_ptr(), r["out"].data_ptr(), r["logits"].data_ptr()
-        a.topk_ids, a.topk_w = r["topk_ids"].data_ptr(), r["topk_w"].data_ptr()
-        a.expert_index, a.workspace, a.workspace_bytes = r["expert_index"].data_ptr(), ws.data_ptr(), self._few_bytes
+        a.T, a.x, a.out, a.logits, a.topk_ids = T, addr(x), addr(r["out"]), addr(r["logits"]), addr(r["topk_ids"])
+        a.topk_w, a.expert_index, a.workspace = addr(r["topk_w"]), addr(r["expert_index"]), addr(ws)
         L.call_on(dev, "dsca_moe_few", ctypes.byref(a))
         return r
 

@@ -24,7 +24,7 @@ def test_a_wait_that_runs_out(cuda, counter, kind, T):
     eng, w, router, gate, n = _engine(cuda, 512, 60, 4, 384, 768, kind=kind, seed=31)
     x = n(T, 512, std=1.0)
     want = {key: v.clone() for key, v in _run(eng, x).items()}
-    eng.wait_limit_ns, eng._few_args = 20_000_000, None
+    eng.wait_limit_ns = 20_000_000
     (ws,) = eng._few_ws.values()
     assert not ws[:L.FEW_ZERO_BYTES].any()
     ws.view(torch.int32)[COUNTERS[counter]] = -(1 << 20)
@@ -33,7 +33,7 @@ def test_a_wait_that_runs_out(cuda, counter, kind, T):
         eng.check()
     assert e.value.code == L.ERR_WAIT_TIMEOUT
     assert eng._few_ws == {}
-    eng.wait_limit_ns, eng._few_args = 2_000_000_000, None
+    eng.wait_limit_ns = 2_000_000_000
     r = _run(eng, x)
     assert all(torch.equal(r[key], want[key]) for key in want)
     _check(r, x, w, router, gate, 4)
@@ -47,7 +47,7 @@ def test_a_block_without_a_shared_expert(cuda, T):
     x = n(T, 256, std=1.0)
     want = _run(eng, x)["out"].clone()
     for counter in ("logits", "routed"):
-        eng.wait_limit_ns, eng._few_args = 20_000_000, None
+        eng.wait_limit_ns = 20_000_000
         (ws,) = eng._few_ws.values()
         ws.view(torch.int32)[COUNTERS[counter]] = -(1 << 20)
         eng.forward_few(x)
