@@ -257,22 +257,26 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
     mx = row_reduce<TPR, true>(mx, sm);
     const float s = (mx > 0.0f || mx != mx) ? __fdiv_rn(mx, 448.0f) : 1.0f;
     if (live && tid == 0) a.scale[row] = s;
-    // y / s as y times the rounded 1 / s, an fp32 rounding more than the quotient (a division an element
-    // took twice the kernel's time); rows so small that 1 / s leaves fp32's normal range do divide
-    const bool tiny = s < 1e-37f;
-    const float rs = tiny ? 0.0f : __frcp_rn(s);
+    // y / s rounded to fp32, from the rounded 1 / s and the remainder that it leaves (Markstein's correction; a
+    // division an element took twice the kernel's time).  Rows so small or large that 1 / s or the remainder
+    // leaves fp32's normal range do divide.
+    const bool divide = !(s >= 1e-30f && s <= 1e30f);
+    const float rs = divide ? 0.0f : __frcp_rn(s);
     uint8_t* q = a.q + row * a.d;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float v[8];
       normed(i, v);
       uint32_t b[4];
-      if (tiny) {
+      if (divide) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(v[j], s);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= rs;
+        for (int j = 0; j < 8; ++j) {
+          const float t = v[j] * rs;
+          v[j] = fmaf(fmaf(-t, s, v[j]), rs, t);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) b[j] = f8s::e4m3x2_rn(v[2 * j], v[2 * j + 1]);
