@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
   }
   if constexpr (QUANT == DSCA_NORM_Q_E4M3) {
     mx = row_reduce<TPR, true>(mx, sm);
-    const float s = (mx > 0.0f || mx != mx) ? __fdiv_rn(mx, 448.0f) : 1.0f;
+    float s = (mx > 0.0f || mx != mx) ? __fdiv_rn(mx, 448.0f) : 1.0f;
+    if (s == 0.0f) s = __uint_as_float(1u);  // a row below 2^-141: not divided by zero
     if (live && tid == 0) a.scale[row] = s;
     // y / s rounded to fp32, from the rounded 1 / s and the remainder that it leaves (Markstein's correction; a
     // division an element took twice the kernel's time).  Rows so small or large that 1 / s or the remainder

@@ -25,7 +25,7 @@ enum { DSCA_NORM_Q_NONE = 0, DSCA_NORM_Q_E4M3 = 1, DSCA_NORM_Q_SPLIT = 2 };
  * h is rounded to dtype before it is squared; the sum and y are fp32, y rounded once when stored.
  * quant:
  *   DSCA_NORM_Q_E4M3   q [rows, d] e4m3 = RN(y / s) of the unrounded y, scale[row] = s = max|y| / 448
- *                      (1 for a row of zeros; NaN for a row with a NaN);
+ *                      (1 for a row of zeros; 2^-149 at least; NaN for a row with a NaN);
  *   DSCA_NORM_Q_SPLIT  q [rows, 2 * Kd] (Kd = d rounded up to 128) and scale[row] = 1 / s exactly as
  *                      dsca_split_rows writes them from the rounded y.  dtype DSCA_BF16, d % 8 == 0,
  *                      q 8-byte aligned and the rows of y and residual_out 16-byte aligned.

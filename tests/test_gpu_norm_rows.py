@@ -48,3 +48,16 @@ def test_e4m3_codes_at_the_borders(cuda, dtype):
         assert torch.equal(out.scale, s.expand(2))
         want = ((w * x.float()).double() / s.double()).float().to(torch.float8_e4m3fn)
         assert torch.equal(out.q.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("top", [3e-45, 1e-43, 6e-43, 1e-38, 1e-31, 1e32, 3e38])
+def test_e4m3_rows_of_extreme_sizes(cuda, top):
+    """Scales down to fp32's smallest number (not below it, where they would be zero) and up to its largest."""
+    from dsca_moe_b200 import add_rms_norm
+
+    w = torch.tensor([top, 0.0, top * 0.5, top * 0.3, 0.0, top * 0.25, 0.0, -top], dtype=torch.float32, device=cuda)
+    out = add_rms_norm(torch.ones(3, 8, dtype=torch.bfloat16, device=cuda), w, 0.0, quant="e4m3")
+    s = (w.double().abs().max() / 448).float().clamp_min(2.0 ** -149)
+    assert torch.equal(out.scale, s.expand(3))
+    want = (w.double() / s.double()).float().to(torch.float8_e4m3fn)
+    assert torch.equal(out.q.view(torch.uint8), want.view(torch.uint8).expand(3, 8))
