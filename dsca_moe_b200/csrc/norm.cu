@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float t = v[j] * rs;
-          v[j] = fmaf(fmaf(-t, s, v[j]), rs, t);
+          v[j] = fmaf(fmaf(t, s, -v[j]), -rs, t);  // in this order a zero keeps its sign
         }
       }
 #pragma unroll
