@@ -1,8 +1,10 @@
-"""add_rms_norm's 8-bit rows where their codes are known bit for bit."""
+"""add_rms_norm's 8-bit rows where their codes are known bit for bit, and its kernels for many rows.
+
+Tolerances are those of test_gpu_norm."""
 import pytest
 import torch
 
-from test_gpu_norm import _inputs
+from test_gpu_norm import F32, _close, _exact, _inputs, _split
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +61,71 @@ def test_e4m3_rows_of_extreme_sizes(cuda, top):
     assert torch.equal(out.scale, s.expand(3))
     want = (w.double() / s.double()).float().to(torch.float8_e4m3fn)
     assert torch.equal(out.q.view(torch.uint8), want.view(torch.uint8).expand(3, 8))
+
+
+# With more than four rows an SM a row has 32 to 128 threads: widths on both sides of every border between these
+# kernels, and odd ones (single values instead of vectors)
+WIDTHS = [8, 250, 256, 257, 264, 511, 512, 520, 768, 761, 776, 1024, 1021, 1032, 2041, 2048, 2056]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [601, 1777])
+@pytest.mark.parametrize("d", WIDTHS)
+def test_many_rows(cuda, d, rows, dtype):
+    """Every form of the output, the last rows of a CTA's among them, and rows behind the last one left alone."""
+    from dsca_moe_b200 import add_rms_norm
+
+    for residual, gap in ((True, 0), (False, 5)):
+        x, r, w = _inputs(cuda, rows, d, dtype, rows + d, residual, gap)
+        x[5] = 0
+        h, ref = _exact(x, r, w)
+        out = add_rms_norm(x, w, residual=r)
+        _close(out.y, ref)
+        assert torch.equal(out.residual, h)
+        q = add_rms_norm(x, w, residual=r, quant="e4m3")
+        assert torch.equal(q.y, out.y) and torch.equal(q.residual, h)
+        if dtype == torch.float32:
+            s = out.y.abs().amax(-1).double() / 448
+            s = torch.where(s > 0, s, torch.ones_like(s)).float()
+            want = (out.y.double() / s.double()[:, None]).float().to(torch.float8_e4m3fn)
+            assert torch.equal(q.scale, s) and torch.equal(q.q.view(torch.uint8), want.view(torch.uint8))
+        else:
+            s = ref.abs().amax(-1) / 448
+            s = torch.where(s > 0, s, torch.ones_like(s))
+            assert ((q.scale.double() - s).abs() <= 2 * F32 * s).all()
+            got = q.q.float().double() * q.scale.double()[:, None]
+            tol = (2.0 ** -4 + 4 * F32) * ref.abs() + 2.0 ** -10 * s[:, None]
+            assert ((got - ref).abs() <= tol).all()
+        if dtype == torch.bfloat16 and d % 8 == 0:
+            q = add_rms_norm(x, w, residual=r, quant="split")
+            assert torch.equal(q.y, out.y) and torch.equal(q.residual, h)
+            want, inv = _split(out.y)
+            assert torch.equal(q.q.view(torch.uint8), want) and torch.equal(q.scale, inv)
+            only = add_rms_norm(x, w, residual=r, quant="split", write_y=False)
+            assert only.y is None and torch.equal(only.q.view(torch.uint8), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [256, 768, 1021, 2048])
+def test_rows_behind_the_last_are_left_alone(cuda, d, dtype):
+    """A last CTA that is only partly filled, with the outputs laid in larger buffers."""
+    import ctypes
+
+    from dsca_moe_b200 import _lib as L
+
+    rows, kp = 603, (d + 127) // 128 * 128
+    x, r, w = _inputs(cuda, rows, d, dtype, 7, True)
+    dt = L.BF16 if dtype == torch.bfloat16 else L.F32
+    for quant in (L.NORM_Q_NONE, L.NORM_Q_E4M3, L.NORM_Q_SPLIT):
+        if quant == L.NORM_Q_SPLIT and (dtype != torch.bfloat16 or d % 8):
+            continue
+        width = 2 * kp if quant == L.NORM_Q_SPLIT else d
+        y, h = (torch.full((rows + 9, d), 7.0, dtype=dtype, device=cuda) for _ in range(2))
+        q = torch.full((rows + 9, width), 0x5A, dtype=torch.uint8, device=cuda)
+        scale = torch.full((rows + 9,), 7.0, device=cuda)
+        a = L.RmsNormArgs(x.data_ptr(), r.data_ptr(), w.data_ptr(), rows, d, dt, dt, d, d, d, d, 1e-6, quant, y.data_ptr(),
+                          h.data_ptr(), q.data_ptr(), scale.data_ptr())
+        L.call("dsca_rms_norm", ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        _close(y[:rows], _exact(x, r, w)[1])
+        assert (y[rows:] == 7).all() and (h[rows:] == 7).all() and (q[rows:] == 0x5A).all() and (scale[rows:] == 7).all()
+        assert (scale[:rows] != 7).all() or quant == L.NORM_Q_NONE
