@@ -55,6 +55,7 @@ int device_info(int* num_sms, int* major) {
   return DSCA_OK;
 }
 
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
@@ -311,7 +312,11 @@ int dsca_moe_few(const dsca_few_args* a, dsca_stream_t stream) {
               (shared && (a->ws1_scale == nullptr || a->ws2_scale == nullptr))))
     return DSCA_ERR_BAD_ARG;
   if (fp8 && !(a->w1_max >= 0.0f && a->w1_max < 3.0e38f)) return DSCA_ERR_BAD_ARG;
-  if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return DSCA_ERR_BAD_ARG;
+  // what is read and written value by value
+  const void* words[] = {a->topk_ids, a->topk_w, a->w1_scale, a->w2_scale, a->ws1_scale, a->ws2_scale, a->err};
+  for (const void* p : words)
+    if (!aligned(p, 4)) return DSCA_ERR_BAD_ARG;
+  if (!aligned(a->logits, xsz) || !aligned(a->expert_index, 8) || !aligned(a->workspace, 256)) return DSCA_ERR_BAD_ARG;
   if (a->workspace_bytes < dsca::few_workspace_bytes(a->T, a->d, k, a->inter, shared ? a->shared_inter : 0))
     return DSCA_ERR_CAPACITY;
   int num_sms = 0, major = 0;
