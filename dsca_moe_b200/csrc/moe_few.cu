@@ -93,7 +93,8 @@ constexpr int kCopyExp = 20;              // each is 2^20 times the one before
 // kCtrBound + e: fp8 weights, 1 + the largest exponent (GLU: sum of the exponents) of the scales of expert e's channels,
 // as they are stored (biased); e = E: the shared expert
 // behind kCtrShared and kCtrRouted: fp8 weights, how many rows of that intermediate reach kReaches0 in their first unit
-enum { kCtrLogits = 0, kCtrExit = 1, kCtrShared = 2, kCtrRouted = 4, kCtrTiles = 8, kCtrBound = 128 };
+// (the first three are added to as pairs of words: nothing else lies in them)
+enum { kCtrLogits = 0, kCtrShared = 2, kCtrRouted = 4, kCtrExit = 6, kCtrTiles = 8, kCtrBound = 128 };
 static_assert(kCtrBound + DSCA_MAX_EXPERTS <= DSCA_FEW_ZERO_BYTES / 4, "counters are within the zeroed bytes");
 
 struct Args {

@@ -188,3 +188,17 @@ def test_an_engine_makes_no_copy_of_its_weights(cuda):
     assert torch.cuda.max_memory_allocated() - before < pe.w1.numel() // 8
     eng.forward_few(n(2, 1024))
     eng.check()
+
+
+@pytest.mark.parametrize("T", [1, 5, 12, 32])
+def test_tokens_of_zeros(cuda, T):
+    """Rows that no value of the intermediate ever reaches any size in, alone and between others (a padded batch)."""
+    eng, w, router, gate, n = block(cuda, 512, 12, 3, 200, 136, seed=48)
+    x = n(T, 512, std=1.0)
+    want = _run(eng, x)["out"].clone()
+    x[T // 2:] = 0
+    r = _run(eng, x)
+    lg, ids, p = _route(x, router, 3, False, False)
+    assert torch.equal(r["topk_ids"].long(), ids) and torch.equal(r["topk_w"], p)
+    assert torch.equal(r["out"][:T // 2], want[:T // 2])
+    assert (r["out"][T // 2:] == 0).all()
