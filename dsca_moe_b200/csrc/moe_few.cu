@@ -28,14 +28,18 @@
 //    sums in order.
 //
 // Measured, against the weights' bytes at the 6.5 TB/s of a copy: the Qwen block (d 2048, 60 experts of 1408, 4
-// a token, a shared one of 5632) 1 token in bf16 31.3 us (4.4 TB/s, 68%), with fp8 weights 26.0 us (41%),
-// 8 tokens in bf16 92-96 us (84%), 20 tokens 177 us, 32 tokens with fp8 weights 131 us (58%); a Switch block (d 768, 64
-// experts of 2048) 16 tokens 35.4 us (39%); fp32 (d 712, 13 experts of 333) 5 tokens 27.3 us where the bytes
+// a token, a shared one of 5632) 1 token in bf16 31.3 us (4.4 TB/s, 68%), with fp8 weights 28 us (38%),
+// 8 tokens in bf16 92-96 us (84%), 20 tokens 178 us, 32 tokens with fp8 weights 138 us (55%); a Switch block (d 768, 64
+// experts of 2048) 16 tokens 35.5 us (39%); fp32 (d 712, 13 experts of 333) 5 tokens 27.7 us where the bytes
 // take 5.3.  At one token some 13 us are not the stream's: launch (3), router (7, half of it under the
-// shared expert's weights), the two GEMMs' border (3), the last rows (2).
+// shared expert's weights), the two GEMMs' border (3), the last rows (2).  (The pairs of times beside the rules below
+// are those of the builds that the rules were chosen with; with fp8 weights those took 2 us less at one token and
+// 6 us at 32, before the intermediate's copies and bounds described below.)
 //
 // A warp spends 150 to 400 instructions on a box, at one in eight clocks (three or four warps a scheduler,
-// each waiting for its own last result); this, not the products, is what keeps it from DRAM speed.  So the boxes are as large as the shares allow; up to eight tokens, whose rows every
+// each waiting for its own last result); this, not the products, is what keeps it from DRAM speed.  Every form of the
+// kernel takes the 128 registers a thread that 16 warps leave, and spills 28 to 114 bytes a thread beyond them
+// (68 to 260 bytes read back).  So the boxes are as large as the shares allow; up to eight tokens, whose rows every
 // unit multiplies in full, x stays in registers through GEMM1 and the sums through GEMM2; with more,
 // an expert's few tokens are gathered for it, and units and tiles are 32 rows high where the rows are
 // short enough, so that 32 rows share one gathering.
@@ -53,7 +57,7 @@
 // fp8 weights go through f16: e4m3 converts to it exactly with one instruction a pair (to bf16 it
 // takes four, which alone cost more than the weights' DRAM time).  A token row times a power of two
 // that takes its largest value to [2^14, 2^15) is exact in f16 down to 2^-29 of that value.  The
-// intermediate (one f16 term: it is off by 2^-11 at most where the output's bf16 is by 2^-8 and the weights'
+// intermediate (one f16 term: it is off by 2^-11 at most where the output's bf16 is by 2^-9 and the weights'
 // own rounding by 2^-4; with a second one, twice the loads and products of
 // GEMM2, 32 tokens took 183 us instead of 153 and one took 31 instead of 27) needs a scale before it is known.  An
 // e4m3 weight is 448 times its row's scale at most, so |h| <= B = max(s_gate s_up) (448 sum|x|)^2 (SwiGLU; max(s) 448

@@ -9,12 +9,12 @@
 //
 // 8-bit rows: "e4m3" scales the unrounded y by s = max|y| / 448 (1 for a zero row), the row format
 // of the fp8 expert weights; "split" writes the rounded y as two e4m3 terms with a power-of-two
-// scale (fp8_split.cuh), the token operand of the fp8-weight GEMMs.
+// scale (fp8_split.cuh), the layout of the token operand of the fp8-weight GEMMs.
 //
 // One pass over the data: a row lives in the registers of its TPR threads (up to 64 values each)
 // between the sum and the stores, so DRAM sees every input and output once: it is bound by DRAM from a few
 // thousand rows on (with residual 16384 x 2048 bf16 41.5 us, 99% of a copy's 6.5 TB/s; 20000 x 768 with split
-// rows 26.7 us, 88%; 4096 x 2048 with e4m3 rows 14.2 us, 82%), below that by the launch and two trips to
+// rows 26.5 us, 89%; 4096 x 2048 with e4m3 rows 14.3 us, 81%), below that by the launch and two trips to
 // memory (1 x 2048 2.1 us).
 #include "common.cuh"
 #include "dsca_b200_block.h"

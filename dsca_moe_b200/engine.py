@@ -425,8 +425,14 @@ class MoEEngine:
         self._ws = {}
         # forward() runs calls of at most this many tokens through the one-kernel form where that
         # supports the block (forward_few); 0 = never.  Results then differ from the other path's by
-        # its roundings (the intermediates and expert outputs are not rounded to bf16 here) and hold no
-        # counts, token_row or other views of the scratch
+        # its roundings (the intermediates and expert outputs are not rounded to bf16 here; with fp8
+        # weights the intermediate has 11 significant bits) and hold no counts, token_row or other views of
+        # the scratch.  Its logits are summed in fp64, the other path's are not, so a token whose logits lie on
+        # a rounding border may get other experts or weights in a call of more tokens than this.
+        # Device us a call, one kernel | launch chain (Qwen block: d 2048, 60 experts of 1408, 4 a token, a shared
+        # one of 5632): bf16 1 token 33 | 98, 8 97 | 152, 16 154 | 171, 24 189 | 197, 32 209 | 203; fp8 weights
+        # 1 30 | 95, 8 73 | 140, 16 97 | 153, 32 138 | 177.  So 32 with fp8 weights and for smaller blocks, 24 for a
+        # bf16 block of this size
         self.few_tokens = 0
         self._few_ws, self._few_like = {}, {}
         self._few_now = self._few_experts = self._few_args = None
@@ -764,7 +770,8 @@ class MoEEngine:
         """The whole block for at most 32 tokens in one kernel (dsca_moe_few): x [T, d] on this
         engine's device -> fresh out [T, d], logits [T, E], topk_ids [T, k], topk_w [T, k] and
         expert_index [T], with forward()'s meaning.  One GPU, resident experts, any of the engine's
-        weight types; ValueError otherwise.  Runs on the current stream; can be captured."""
+        weight types, at most 64 logits (the shared expert's gate is one); ValueError otherwise.  Every wait
+        inside ends after wait_limit_ns (check() reports it).  Runs on the current stream; can be captured."""
         w = self.router_weight
         dev, k = w.device, self.top_k
         if x.dim() != 2 or x.shape[1] != self.d:

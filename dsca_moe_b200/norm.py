@@ -56,8 +56,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     x [..., d] bf16 or fp32 (rows may lie in a wider buffer), residual the same shape and type,
     weight [d] of x's type or fp32.  quant "e4m3": q [rows, d] with scale = max|y| / 448 a row, from
     the unrounded y (the row format of the fp8 expert weights); "split" (bf16, d % 8 == 0): q
-    [rows, 2 * ceil(d / 128) * 128], the two-term rows of dsca_split_rows with scale = 1 / s, the token
-    operand of the fp8-weight experts.  write_y=False leaves y out when only the 8-bit rows are
+    [rows, 2 * ceil(d / 128) * 128], the two-term rows of dsca_split_rows with scale = 1 / s, the layout in
+    which the fp8-weight experts multiply tokens (MoEEngine takes y and splits it itself).  write_y=False leaves y out when only the 8-bit rows are
     wanted.  Runs on x's device, on its current stream.  Inference only: the results carry no
     gradient."""
     dtype, dev, shape = x.dtype, x.device, x.shape
