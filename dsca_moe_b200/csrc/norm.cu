@@ -14,7 +14,7 @@
 // One pass over the data: a row lives in the registers of its TPR threads (up to 64 values each)
 // between the sum and the stores, so DRAM sees every input and output once: it is bound by DRAM from a few
 // thousand rows on (with residual 16384 x 2048 bf16 41.5 us, 99% of a copy's 6.5 TB/s; 20000 x 768 with split
-// rows 26.5 us, 89%; 4096 x 2048 with e4m3 rows 14.3 us, 81%), below that by the launch and two trips to
+// rows 26.5 us, 89%; 4096 x 2048 with e4m3 rows 14.5 us, 80%), below that by the launch and two trips to
 // memory (1 x 2048 2.1 us).
 #include "common.cuh"
 #include "dsca_b200_block.h"
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_kernel(const Args a) {
       c[0].get(f);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * f[j];
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * f[j] * inv;  // of bf16 values the first product is exact
   };
   T* ho = a.h ? reinterpret_cast<T*>(a.h) + row * a.ld_h : nullptr;
   T* yo = a.y ? reinterpret_cast<T*>(a.y) + row * a.ld_y : nullptr;

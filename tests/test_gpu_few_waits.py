@@ -53,4 +53,5 @@ def test_a_block_without_a_shared_expert(cuda, T):
         eng.forward_few(x)
         with pytest.raises(L.DscaError):
             eng.check()
+        eng.wait_limit_ns = 2_000_000_000
         assert torch.equal(_run(eng, x)["out"], want)

@@ -63,6 +63,21 @@ def test_e4m3_rows_of_extreme_sizes(cuda, top):
     assert torch.equal(out.q.view(torch.uint8), want.view(torch.uint8).expand(3, 8))
 
 
+@pytest.mark.parametrize("rows,d", [(40, 2048), (2000, 2048), (3000, 768), (8, 8192)])
+def test_bf16_rows_are_rounded_twice_at_most(cuda, rows, d):
+    """h w is exact in fp32, so y is its product with the rounded 1 / sqrt, once in fp32 and once in bf16.  Rows of small
+    integers have exact sums of squares, and with them a 1 / sqrt that is known bit for bit."""
+    from dsca_moe_b200 import add_rms_norm
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(rows + d)
+    x = torch.randint(-8, 9, (rows, d), generator=g, device=cuda).bfloat16()
+    w = (1 + 0.2 * torch.randn(d, generator=g, device=cuda)).bfloat16()
+    mean = ((x.double() ** 2).sum(-1, keepdim=True) / d).float()
+    inv = (1 / mean.double().sqrt()).float()
+    assert torch.equal(add_rms_norm(x, w, 0.0).y, (x.float() * w.float() * inv).bfloat16())
+
+
 # With more than four rows an SM a row has 32 to 128 threads: widths on both sides of every border between these
 # kernels, and odd ones (single values instead of vectors)
 WIDTHS = [8, 250, 256, 257, 264, 511, 512, 520, 768, 761, 776, 1024, 1021, 1032, 2041, 2048, 2056]
