@@ -6,6 +6,8 @@ Public surface (mirrors the reference's plugin):
   MoEEngine, pack_swiglu, pack_relu, plan_harmony, plan_layout   (engine level)
   build_exec_plan, QoSInputs, ExpertCache        (expert cache / QoS planner path)
   add_rms_norm                                   (the norm in front of a block, with 8-bit rows)
+  gated_ffn, GatedFFN, replace_dense_ffn         (dense gated layers of the same models, with gradients)
+  pack_int8, quantize_rows, int8_linear, gated_ffn_int8   (8-bit integer weights)
   write_run_outputs, TokenTrace                  (the reference's run output files)
 The compute runs in libdsca_b200.so (include/dsca_b200.h); build it with
 ``python -m dsca_moe_b200.build``.
@@ -19,7 +21,7 @@ def __getattr__(name):
     if name in ("QoSMoELayer", "ShardedQwenMoE", "patch", "placement_to_expert_to_gpu"):
         from . import layers
         return getattr(layers, name)
-    if name in ("replace_qosmoe_layer", "get_qosmoe_layers", "get_tensor_by_path"):
+    if name in ("replace_qosmoe_layer", "replace_dense_ffn", "get_qosmoe_layers", "get_tensor_by_path"):
         from . import plugin
         return getattr(plugin, name)
     if name in ("MoEEngine", "pack_swiglu", "pack_relu", "plan_harmony", "plan_layout", "PackedExperts",
@@ -29,6 +31,10 @@ def __getattr__(name):
     if name in ("add_rms_norm", "RmsNormOutput"):
         from . import norm
         return getattr(norm, name)
+    if name in ("gated_ffn", "gated_ffn_int8", "int8_linear", "quantize_rows", "pack_int8", "Int8Weight", "GatedFFN",
+                "check_dense"):
+        from . import dense
+        return getattr(dense, name)
     if name in ("write_run_outputs", "TokenTrace"):
         from . import reporting
         return getattr(reporting, name)

@@ -1,4 +1,4 @@
-"""ctypes binding of libdsca_b200.so (include/dsca_b200.h).
+"""ctypes binding of libdsca_b200.so (include/dsca_b200.h, dsca_b200_block.h, dsca_b200_dense.h).
 
 The library is the only compute path: if it is missing or the device is not an sm_100 part,
 every call raises; there is no CPU or eager-PyTorch fallback.
@@ -121,6 +121,46 @@ class FewArgs(ctypes.Structure):
                 ("wait_limit_ns", ctypes.c_uint64)]
 
 
+# ---- include/dsca_b200_dense.h
+GATE_SILU, GATE_GELU, GATE_RELU = range(3)
+DENSE_MAX_DIM = 1048576
+DENSE_MAX_ROWS = 16777216
+
+
+class GatedFfnArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("y", _vp), ("g", _vp), ("u", _vp),
+                ("h", _vp), ("rows", _i), ("d", _i), ("inter", _i), ("dtype", _i), ("act", _i), ("ld_x", _i64),
+                ("ld_gate", _i64), ("ld_up", _i64), ("ld_down", _i64), ("ld_y", _i64), ("ld_h", _i64),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
+
+
+class GatedFfnBackwardArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("dy", _vp), ("g", _vp), ("u", _vp),
+                ("h", _vp), ("dx", _vp), ("d_gate", _vp), ("d_up", _vp), ("d_down", _vp), ("dg", _vp), ("du", _vp),
+                ("rows", _i), ("d", _i), ("inter", _i), ("dtype", _i), ("act", _i), ("ld_x", _i64), ("ld_gate", _i64),
+                ("ld_up", _i64), ("ld_down", _i64), ("ld_dy", _i64), ("ld_h", _i64), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
+
+
+class QuantizeRowsArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("rows", _i), ("k", _i), ("dtype", _i), ("ld_x", _i64), ("q", _vp), ("ld_q", _i64),
+                ("scale", _vp)]
+
+
+class Int8LinearArgs(ctypes.Structure):
+    _fields_ = [("x", _vp), ("q", _vp), ("scale", _vp), ("w", _vp), ("w_scale", _vp), ("bias", _vp), ("y", _vp),
+                ("rows", _i), ("k", _i), ("n", _i), ("dtype", _i), ("ld_x", _i64), ("ld_q", _i64), ("ld_w", _i64),
+                ("ld_y", _i64), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
+
+
+class GatedFfnInt8Args(ctypes.Structure):
+    _fields_ = [("x", _vp), ("q", _vp), ("scale", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp),
+                ("gate_scale", _vp), ("up_scale", _vp), ("down_scale", _vp), ("h", _vp), ("hq", _vp), ("h_scale", _vp),
+                ("y", _vp), ("rows", _i), ("d", _i), ("inter", _i), ("dtype", _i), ("act", _i), ("ld_x", _i64),
+                ("ld_q", _i64), ("ld_gate", _i64), ("ld_up", _i64), ("ld_down", _i64), ("ld_h", _i64), ("ld_hq", _i64),
+                ("ld_y", _i64), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
+
+
 # every symbol include/dsca_b200.h declares
 EXPORTED = ["dsca_version", "dsca_status_string", "dsca_device_info", "dsca_router_topk",
             "dsca_dispatch_scan", "dsca_permute", "dsca_grouped_ffn", "dsca_combine",
@@ -131,6 +171,10 @@ EXPORTED = ["dsca_version", "dsca_status_string", "dsca_device_info", "dsca_rout
             "dsca_ep_region_free", "dsca_ep_return", "dsca_qos_priority", "dsca_router_pack_i8", "dsca_split_rows"]
 # every symbol include/dsca_b200_block.h declares
 EXPORTED_BLOCK = ["dsca_rms_norm", "dsca_few_workspace_bytes", "dsca_moe_few"]
+# every symbol include/dsca_b200_dense.h declares
+EXPORTED_DENSE = ["dsca_gated_ffn", "dsca_gated_ffn_backward", "dsca_quantize_rows", "dsca_int8_linear",
+                  "dsca_gated_ffn_int8", "dsca_gated_ffn_workspace", "dsca_gated_ffn_backward_workspace",
+                  "dsca_int8_linear_workspace", "dsca_gated_ffn_int8_workspace"]
 STATIC_SCRATCH_BYTES = 16 << 20
 
 _LIB = None
@@ -194,7 +238,13 @@ def load():
     lib.dsca_few_workspace_bytes.restype = ctypes.c_size_t
     lib.dsca_few_workspace_bytes.argtypes = [_i, _i, _i, _i, _i]
     lib.dsca_moe_few.argtypes = [p(FewArgs), _vp]
-    for name in EXPORTED + EXPORTED_BLOCK:
+    for name, args in (("dsca_gated_ffn", GatedFfnArgs), ("dsca_gated_ffn_backward", GatedFfnBackwardArgs),
+                       ("dsca_int8_linear", Int8LinearArgs), ("dsca_gated_ffn_int8", GatedFfnInt8Args)):
+        getattr(lib, name).argtypes = [p(args), _vp]
+        getattr(lib, name + "_workspace").argtypes = [p(args)]
+        getattr(lib, name + "_workspace").restype = ctypes.c_size_t
+    lib.dsca_quantize_rows.argtypes = [p(QuantizeRowsArgs), _vp]
+    for name in EXPORTED + EXPORTED_BLOCK + EXPORTED_DENSE:
         getattr(lib, name).restype = getattr(lib, name).restype or _i
     lib.dsca_version.restype = ctypes.c_char_p
     lib.dsca_status_string.restype = ctypes.c_char_p

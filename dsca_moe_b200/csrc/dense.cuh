@@ -1,0 +1,95 @@
+// Shared by the dense gated feed-forward block and the 8-bit integer products (dsca_b200_dense.h).
+//
+// Every product is written as out[n][m] = sum_k A[m][k] B[n][k], m the contiguous index of the
+// output's rows: for a forward product A is the weight and B the tokens, for a weight's gradient both
+// are activations and k the tokens.  An operand is K-major (element [r][k] at p[r * ld + k], a
+// weight as a Linear layer holds it) or MN-major (p[k * ld + r], the same matrix read the other way), so
+// no product transposes a matrix in memory.
+#pragma once
+#include "common.cuh"
+#include "dsca_b200_dense.h"
+
+namespace dsca {
+namespace dense {
+
+struct Operand {
+  const void* p;
+  int64_t ld;  // elements
+  int mn;      // 0 K-major, 1 MN-major
+};
+
+// Up to two segments whose sums are added: out = sum_s A_s B_s^T (dx = dg Wg + du Wu).
+struct Problem {
+  Operand a[2], b[2];
+  int nseg, M, N, K;
+  void* out;  // [N, M]
+  int64_t ldo;
+};
+
+// kStore: out = the product (8-bit: times row_scale[n] col_scale[0][m], plus bias[m]).
+// kGlu:   a[0] gate, a[1] up rows: out = act(g) * u; g and u as well where save_g is given.
+// kDGlu:  the product is dh; with g and u read: out = dh u act'(g), out2 = dh act(g).
+enum Epi { kStore = 0, kGlu = 1, kDGlu = 2 };
+constexpr int kMaxProblems = 4;
+
+struct Job {
+  int epi, act, nprob;
+  int i8;         // operands are 8-bit integers, the sum int32
+  int dtype;      // of the operands (unless i8) and of out
+  Problem prob[kMaxProblems];
+  void* save_g;   // kGlu: written; kDGlu: read (same for u); rows of prob[0].ldo
+  void* save_u;
+  void* out2;     // kDGlu: du
+  const float* row_scale;
+  const float* col_scale[2];
+  const void* bias;
+};
+
+// ---------------------------------------------------------------- gates
+// kFast (16-bit outputs): the hardware's exponential and division, good to 2^-21 here; otherwise the
+// full-precision ones.
+template <bool kFast>
+__device__ __forceinline__ float expf_(float x) { return kFast ? __expf(x) : expf(x); }
+template <bool kFast>
+__device__ __forceinline__ float div_(float a, float b) { return kFast ? __fdividef(a, b) : a / b; }
+
+// 0.5 (1 + tanh z) = 1 / (1 + e^-2z) for the gelu gate, z = sqrt(2 / pi) (g + 0.044715 g^3)
+template <bool kFast>
+__device__ __forceinline__ float gelu_p(float g) {
+  const float z2 = -1.5957691216057308f * (g + 0.044715f * g * g * g);
+  return div_<kFast>(1.0f, 1.0f + expf_<kFast>(z2));
+}
+
+template <bool kFast>
+__device__ __forceinline__ float gate(float g, int act) {
+  if (act == DSCA_GATE_SILU) return div_<kFast>(g, 1.0f + expf_<kFast>(-g));
+  if (act == DSCA_GATE_RELU) return g <= 0.0f ? 0.0f : g;  // NaN stays
+  return g * gelu_p<kFast>(g);
+}
+
+// act(g) and act'(g)
+template <bool kFast>
+__device__ __forceinline__ void gate_grad(float g, int act, float* a, float* da) {
+  if (act == DSCA_GATE_SILU) {
+    const float s = div_<kFast>(1.0f, 1.0f + expf_<kFast>(-g));
+    *a = g * s;
+    // the second term is 0 where 1 - s is, also for an infinite g
+    *da = s + (s < 1.0f && s > 0.0f ? g * s * (1.0f - s) : 0.0f);
+    if (g != g) *da = g;
+  } else if (act == DSCA_GATE_RELU) {
+    *a = g <= 0.0f ? 0.0f : g;
+    *da = g <= 0.0f ? 0.0f : (g != g ? g : 1.0f);
+  } else {
+    const float p = gelu_p<kFast>(g);
+    *a = g * p;
+    const float q = p * (1.0f - p);
+    *da = p + (q > 0.0f ? 2.0f * g * q * 0.7978845608028654f * (1.0f + 0.134145f * g * g) : 0.0f);
+    if (g != g) *da = g;
+  }
+}
+
+int launch_simt(const Job& j, cudaStream_t stream);
+int launch_quantize_rows(const dsca_quantize_rows_args* a, cudaStream_t stream);
+
+}  // namespace dense
+}  // namespace dsca

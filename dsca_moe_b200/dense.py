@@ -1,0 +1,391 @@
+"""Dense gated feed-forward blocks and 8-bit integer products (include/dsca_b200_dense.h).
+
+The dense layers between MoE blocks (Qwen2MoeMLP of `mlp_only_layers` and `decoder_sparse_step`, or a
+shared expert on its own) are y = (act(x Wg^T) * (x Wu^T)) Wd^T:
+
+  gated_ffn        the block in bf16 or fp32 on weights as Linear layers hold them, with its gradients
+  gated_ffn_int8   the block on 8-bit integer weights (inference)
+  int8_linear      one product with 8-bit integer weights, scales for each token and channel
+  quantize_rows, pack_int8   rows and weights in 8-bit integers
+  GatedFFN         the module that replace_dense_ffn and patch(dense_ffn=...) put into a model
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from .norm import _DTYPES, _stride
+
+__all__ = ["GatedFFN", "Int8Weight", "check_dense", "gated_ffn", "gated_ffn_int8", "int8_linear", "pack_int8",
+           "quantize_rows"]
+
+_ACTS = {"silu": L.GATE_SILU, "gelu": L.GATE_GELU, "relu": L.GATE_RELU}
+_ERR: dict = {}
+
+
+def _err(dev) -> int:
+    """Address of the device's error word (a wait inside a kernel that ran out records there)."""
+    t = _ERR.get(dev.index)
+    if t is None:
+        t = _ERR[dev.index] = torch.zeros(64, dtype=torch.int32, device=dev)
+    return t.data_ptr()
+
+
+def check_dense(device=None):
+    """Raise if a dense block or 8-bit product on `device` recorded an error since the last check, which
+    it clears (synchronises the current stream)."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    t = _ERR.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    if t is not None:
+        L.call_on(t.device, "dsca_check_error", t.data_ptr())
+
+
+def _act(act: str) -> int:
+    code = _ACTS.get(act)
+    if code is None:
+        raise ValueError(f"act must be 'silu', 'gelu' (tanh form) or 'relu', not {act!r}")
+    return code
+
+
+def _rows(x, name: str, width: int | None = None):
+    """(rows, row stride) of x [..., width] on a GPU."""
+    if x.device.type != "cuda":
+        raise ValueError(f"{name} must be on a GPU")
+    if x.dim() == 0 or x.shape[-1] == 0 or (width is not None and x.shape[-1] != width):
+        raise ValueError(f"{name}: expected [..., {'d' if width is None else width}] rows, got {tuple(x.shape)}")
+    d = x.shape[-1]
+    if d > L.DENSE_MAX_DIM:
+        raise ValueError(f"{name}: rows of {d} values exceed {L.DENSE_MAX_DIM}")
+    rows = x.numel() // d
+    if rows > L.DENSE_MAX_ROWS:
+        raise ValueError(f"{name}: {rows} rows exceed {L.DENSE_MAX_ROWS}")
+    return rows, (d if x.is_contiguous() or rows == 0 else _stride(x, name, d))
+
+
+def _weight(w, name: str, out: int, inp: int, x) -> int:
+    if w.dim() != 2 or w.shape[0] != out or w.shape[1] != inp:
+        raise ValueError(f"{name}: expected [{out}, {inp}], got {tuple(w.shape)}")
+    if w.dtype != x.dtype or w.device != x.device:
+        raise ValueError(f"{name} must have x's type and device")
+    return inp if w.is_contiguous() else _stride(w, name, inp)
+
+
+def _workspace(name: str, args, dev):
+    """The call's workspace, allocated on the current stream, in args."""
+    n = getattr(L.load(), name)(ctypes.byref(args))
+    if n == 0:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), n
+    return ws
+
+
+def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
+    dev, dtype = x.device, x.dtype
+    rows, d, inter, ld_x, ld_g, ld_u, ld_d = shapes
+    y = torch.empty(x.shape, dtype=dtype, device=dev)
+    if rows == 0:
+        return y, None
+    ld_h = (inter + 7) // 8 * 8
+    buf = torch.empty((3 if save else 1, rows, ld_h), dtype=dtype, device=dev)
+    step = rows * ld_h * buf.element_size()
+    h = buf.data_ptr()
+    g, u = (h + step, h + 2 * step) if save else (None, None)
+    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, h, rows, d, inter,
+                       _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
+    with torch.cuda.device(dev):
+        ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
+    L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
+    return y, buf
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd, act, shapes):
+        y, buf = _forward(x, wg, wu, wd, act, shapes, True)
+        ctx.act, ctx.shapes = act, shapes
+        ctx.save_for_backward(x, wg, wu, wd, buf)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, wg, wu, wd, buf = ctx.saved_tensors
+        rows, d, inter, ld_x, ld_g, ld_u, ld_d = ctx.shapes
+        dev, dtype = x.device, x.dtype
+        need = ctx.needs_input_grad
+        dx = torch.empty(x.shape, dtype=dtype, device=dev) if need[0] else None
+        dwg = torch.empty((inter, d), dtype=dtype, device=dev) if need[1] else None
+        dwu = torch.empty((inter, d), dtype=dtype, device=dev) if need[2] else None
+        dwd = torch.empty((d, inter), dtype=dtype, device=dev) if need[3] else None
+        ptr = [None if t is None else t.data_ptr() for t in (dx, dwg, dwu, dwd)]
+        a = L.GatedFfnBackwardArgs()
+        a.dx, a.d_gate, a.d_up, a.d_down = ptr
+        a.rows, a.d, a.inter, a.dtype, a.act = rows, d, inter, _DTYPES[dtype], ctx.act
+        keep = ()
+        if rows:
+            try:
+                ld_dy = d if dy.is_contiguous() else _stride(dy, "dy", d)
+            except ValueError:  # a gradient may come in any strides (expanded, transposed)
+                dy, ld_dy = dy.contiguous(), d
+            ld_h = buf.shape[2]
+            step = rows * ld_h * buf.element_size()
+            grads = torch.empty((2, rows, ld_h), dtype=dtype, device=dev)
+            a.x, a.w_gate, a.w_up, a.w_down, a.dy = (t.data_ptr() for t in (x, wg, wu, wd, dy))
+            h = buf.data_ptr()
+            a.h, a.g, a.u = h, h + step, h + 2 * step
+            a.dg, a.du = grads.data_ptr(), grads.data_ptr() + step
+            a.ld_x, a.ld_gate, a.ld_up, a.ld_down, a.ld_dy, a.ld_h = ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h
+            a.err = _err(dev)
+            with torch.cuda.device(dev):
+                keep = (grads, _workspace("dsca_gated_ffn_backward_workspace", a, dev))
+        L.call_on(dev, "dsca_gated_ffn_backward", ctypes.byref(a))
+        del keep
+        return dx, dwg, dwu, dwd, None, None
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              act: str = "silu") -> torch.Tensor:
+    """y = (act(x w_gate^T) * (x w_up^T)) w_down^T, with gradients for x and the three weights.
+
+    x [..., d] bf16 or fp32 (rows may lie in a wider buffer), w_gate and w_up [inter, d], w_down
+    [d, inter] of x's type, as Linear layers hold them.  act: "silu", "gelu" (tanh form) or "relu".
+    Products are summed in fp32; for bf16 the gate, up and intermediate values are rounded to bf16 once
+    each (the intermediate from the unrounded ones).  Under autograd the call keeps the three [rows,
+    inter] intermediates for the backward pass; second derivatives are not offered.  Runs on x's
+    device, on its current stream; check_dense() reports a wait that ran out."""
+    code = _act(act)
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    rows, ld_x = _rows(x, "x")
+    d = x.shape[-1]
+    if w_gate.dim() != 2 or w_gate.shape[0] == 0:
+        raise ValueError(f"w_gate: expected [inter, {d}], got {tuple(w_gate.shape)}")
+    inter = w_gate.shape[0]
+    if inter > L.DENSE_MAX_DIM:
+        raise ValueError(f"w_gate: {inter} rows exceed {L.DENSE_MAX_DIM}")
+    shapes = (rows, d, inter, ld_x, _weight(w_gate, "w_gate", inter, d, x), _weight(w_up, "w_up", inter, d, x),
+              _weight(w_down, "w_down", d, inter, x))
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
+        return _GatedFFN.apply(x, w_gate, w_up, w_down, code, shapes)
+    return _forward(x, w_gate, w_up, w_down, code, shapes, False)[0]
+
+
+# ----------------------------------------------------------------------------- 8-bit integers
+class Int8Weight(NamedTuple):
+    """q [out, in] int8 codes (a view of rows padded with zeros to a multiple of 16), scale [out] fp32:
+    the weight is q * scale[:, None]."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        return (self.q.float() * self.scale[:, None]).to(dtype)
+
+
+def _quantize(x):
+    """(codes [rows, k rounded up to 16], scales) of x's rows."""
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    rows, ld_x = _rows(x, "x")
+    k = x.shape[-1]
+    ld_q = (k + 15) // 16 * 16
+    q = torch.empty((rows, ld_q), dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if rows:
+        a = L.QuantizeRowsArgs(x.data_ptr(), rows, k, dt, ld_x, q.data_ptr(), ld_q, scale.data_ptr())
+        L.call_on(x.device, "dsca_quantize_rows", ctypes.byref(a))
+    return q, scale
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q [..., k] int8, scale [...] fp32) of x [..., k] bf16 or fp32: scale = max|x| / 127 a row (1 for a
+    row of zeros), q the quotient 127 x / max|x| rounded to the nearest integer, ties to even,
+    exactly.  q's rows lie a multiple of 16 bytes apart, the bytes between them zero.  A row with an
+    infinity or a NaN has that as its scale.  Inference only."""
+    q, scale = _quantize(x)
+    k = x.shape[-1]
+    return q[:, :k] if x.dim() == 2 else q[:, :k].unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0, :k], scale
+
+
+def pack_int8(weight: torch.Tensor) -> Int8Weight:
+    """A Linear layer's weight [out, in] (bf16 or fp32, on a GPU) in 8-bit integers, one scale an output
+    channel."""
+    if weight.dim() != 2 or weight.shape[0] == 0:
+        raise ValueError(f"weight: expected [out, in], got {tuple(weight.shape)}")
+    return Int8Weight(*quantize_rows(weight.detach()))
+
+
+def _int8_weight(w, name: str, dev, inp: int, out: int | None = None) -> int:
+    """Row stride of an Int8Weight."""
+    q, s = w
+    if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] != inp or (out is not None and q.shape[0] != out):
+        raise ValueError(f"{name}: expected an Int8Weight [{'out' if out is None else out}, {inp}], got "
+                         f"{q.dtype} {tuple(q.shape)}")
+    if q.device != dev or s.device != dev:
+        raise ValueError(f"{name} must be on x's device")
+    if s.dtype != torch.float32 or s.shape != (q.shape[0],) or not s.is_contiguous():
+        raise ValueError(f"{name}: scale must be a contiguous float32 [{q.shape[0]}] tensor")
+    ld = q.stride(0) if q.shape[0] > 1 else (inp + 15) // 16 * 16
+    if (inp > 1 and q.stride(1) != 1) or ld % 16 or ld < inp or q.data_ptr() % 16:
+        raise ValueError(f"{name}: rows of codes must lie a multiple of 16 bytes apart (pack_int8 lays them out)")
+    return ld
+
+
+_INT8_MAX_K = 131072
+
+
+def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None = None,
+                x_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y = x W^T (+ bias) with W in 8-bit integers (pack_int8) and x's rows quantised in the call.
+
+    x [..., k] bf16 or fp32; or int8 codes of quantize_rows with their x_scale [...], out_dtype then
+    chooses y's type (bf16 by default, otherwise x's type).  Codes lie in [-127, 127].  The products' sum
+    is exact; it is scaled in fp32 and rounded once.  bias [n] of y's type.  Inference only."""
+    given = x.dtype == torch.int8
+    if given:
+        if x_scale is None:
+            raise ValueError("int8 codes need x_scale")
+        dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    else:
+        if x_scale is not None:
+            raise ValueError("x_scale goes with int8 codes")
+        dtype = x.dtype
+        if out_dtype not in (None, dtype):
+            raise ValueError("out_dtype goes with int8 codes (y has x's type otherwise)")
+    dt = _DTYPES.get(dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {dtype}")
+    rows, ld_x = _rows(x, "x")
+    k, dev = x.shape[-1], x.device
+    if k > _INT8_MAX_K:
+        raise ValueError(f"sums of {k} products exceed {_INT8_MAX_K}")
+    ld_w = _int8_weight(weight, "weight", dev, k)
+    n = weight.q.shape[0]
+    if bias is not None and (bias.dtype != dtype or bias.device != dev or tuple(bias.shape) != (n,)
+                             or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous [{n}] tensor of y's type on x's device")
+    if given:
+        if x_scale.shape != x.shape[:-1] or x_scale.dtype != torch.float32 or x_scale.device != dev \
+                or not x_scale.is_contiguous():
+            raise ValueError("x_scale must be a contiguous float32 tensor, one value a row of x")
+        if rows == 1:
+            ld_x = (k + 15) // 16 * 16
+        if rows and (ld_x % 16 or x.data_ptr() % 16):
+            raise ValueError("rows of codes must lie a multiple of 16 bytes apart (quantize_rows lays them out)")
+    y = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
+    if rows == 0:
+        return y
+    a = L.Int8LinearArgs()
+    if given:
+        a.q, a.scale, a.ld_q = x.data_ptr(), x_scale.data_ptr(), ld_x
+    else:
+        ld_q = (k + 15) // 16 * 16
+        buf = torch.empty(rows * (ld_q + 4), dtype=torch.uint8, device=dev)
+        a.x, a.ld_x, a.ld_q = x.data_ptr(), ld_x, ld_q
+        a.q, a.scale = buf.data_ptr(), buf.data_ptr() + rows * ld_q
+    a.w, a.w_scale, a.ld_w = weight.q.data_ptr(), weight.scale.data_ptr(), ld_w
+    a.bias = None if bias is None else bias.data_ptr()
+    a.y, a.ld_y = y.data_ptr(), n
+    a.rows, a.k, a.n, a.dtype, a.err = rows, k, n, dt, _err(dev)
+    with torch.cuda.device(dev):
+        ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
+    L.call_on(dev, "dsca_int8_linear", ctypes.byref(a))
+    return y
+
+
+def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down: Int8Weight,
+                   act: str = "silu") -> torch.Tensor:
+    """gated_ffn with its weights in 8-bit integers (pack_int8): x's rows are quantised, the gated
+    intermediate is formed in fp32 and its rows quantised in turn.  x [..., d] bf16 or fp32; y has its
+    shape and type.  Inference only."""
+    code = _act(act)
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    rows, ld_x = _rows(x, "x")
+    d, dev = x.shape[-1], x.device
+    inter = w_gate[0].shape[0]
+    if max(d, inter) > _INT8_MAX_K:
+        raise ValueError(f"sums of {max(d, inter)} products exceed {_INT8_MAX_K}")
+    a = L.GatedFfnInt8Args()
+    a.ld_gate = _int8_weight(w_gate, "w_gate", dev, d)
+    a.ld_up = _int8_weight(w_up, "w_up", dev, d, inter)
+    a.ld_down = _int8_weight(w_down, "w_down", dev, inter, d)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if rows == 0:
+        return y
+    ld_q, ld_hq = (d + 15) // 16 * 16, (inter + 15) // 16 * 16
+    # one buffer: h, the two sets of codes, the two sets of scales
+    buf = torch.empty(rows * (5 * ld_hq + ld_q + 8), dtype=torch.uint8, device=dev)
+    p = buf.data_ptr()
+    a.h, a.hq, a.q = p, p + rows * 4 * ld_hq, p + rows * 5 * ld_hq
+    a.scale = a.q + rows * ld_q
+    a.h_scale = a.scale + 4 * rows
+    a.x, a.y = x.data_ptr(), y.data_ptr()
+    a.w_gate, a.w_up, a.w_down = w_gate[0].data_ptr(), w_up[0].data_ptr(), w_down[0].data_ptr()
+    a.gate_scale, a.up_scale, a.down_scale = w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr()
+    a.rows, a.d, a.inter, a.dtype, a.act, a.err = rows, d, inter, dt, code, _err(dev)
+    a.ld_x, a.ld_q, a.ld_h, a.ld_hq, a.ld_y = ld_x, ld_q, ld_hq, ld_hq, d
+    with torch.cuda.device(dev):
+        ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
+    L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
+    return y
+
+
+# ----------------------------------------------------------------------------- module
+_NAMES = (("gate_proj", "up_proj", "down_proj"), ("wi_0", "wi_1", "wo"))
+
+
+def _act_name(mod) -> str:
+    """The gate's name of a transformers MLP (its act_fn / act module)."""
+    fn = getattr(mod, "act_fn", None)
+    fn = getattr(mod, "act", None) if fn is None else fn
+    name = type(fn).__name__
+    if isinstance(fn, nn.SiLU) or name in ("SiLUActivation", "SiLU"):
+        return "silu"
+    if isinstance(fn, nn.ReLU):
+        return "relu"
+    if name in ("NewGELUActivation", "GELUTanh", "PytorchGELUTanh", "FastGELUActivation") \
+            or (isinstance(fn, nn.GELU) and fn.approximate == "tanh"):
+        return "gelu"
+    raise ValueError(f"gate activation {name} is not offered (silu, tanh gelu, relu)")
+
+
+class GatedFFN(nn.Module):
+    """A dense gated MLP (Qwen2MoeMLP's gate_proj / up_proj / down_proj, or wi_0 / wi_1 / wo) on gated_ffn.
+
+    Keeps the old module's Linear layers under their names, so that its parameters, their gradients and
+    state_dict stay what they were.  int8=True packs the weights in 8-bit integers instead (buffers;
+    inference only) and lets the Linear layers go."""
+
+    def __init__(self, old: nn.Module, int8: bool = False):
+        super().__init__()
+        names = next((n for n in _NAMES if all(hasattr(old, m) for m in n)), None)
+        if names is None:
+            raise ValueError(f"{type(old).__name__} has neither gate_proj / up_proj / down_proj nor wi_0 / wi_1 / wo")
+        linears = [getattr(old, n) for n in names]
+        if any(getattr(m, "bias", None) is not None for m in linears):
+            raise ValueError("gated blocks with biases are not offered")
+        self.names, self.act, self.int8 = names, _act_name(old), bool(int8)
+        if not int8:
+            for n, m in zip(names, linears):
+                setattr(self, n, m)
+            return
+        self.widths = tuple(m.weight.shape[1] for m in linears)
+        for n, m in zip(names, linears):
+            q, scale = _quantize(m.weight.detach())
+            self.register_buffer(n + "_q", q)  # whole padded rows, so that a copy keeps their layout
+            self.register_buffer(n + "_scale", scale)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.int8:
+            return gated_ffn_int8(x, *(Int8Weight(getattr(self, n + "_q")[:, :k], getattr(self, n + "_scale"))
+                                       for n, k in zip(self.names, self.widths)), act=self.act)
+        return gated_ffn(x, *(getattr(self, n).weight for n in self.names), act=self.act)

@@ -273,9 +273,14 @@ class ShardedQwenMoE(nn.Module):
         return r["out"].view(b, s, d), r["logits"]
 
 
-def patch(model, rank, world, policy="fifo", few_tokens=0):
+def patch(model, rank, world, policy="fifo", few_tokens=0, dense_ffn=None):
     """qwen_ep_adapter/qwen_ep.py:100-109: swap every Qwen2MoeSparseMoeBlock of model.model.layers.
-    The swapped blocks return what the installed transformers' Qwen2MoeDecoderLayer expects."""
+    The swapped blocks return what the installed transformers' Qwen2MoeDecoderLayer expects.
+    `dense_ffn`: None leaves the dense layers between them (Qwen2MoeMLP of mlp_only_layers and
+    decoder_sparse_step) as they are, "same" swaps them for GatedFFN on their parameters, "int8" for
+    GatedFFN on 8-bit integer weights."""
+    if dense_ffn not in (None, "same", "int8"):
+        raise ValueError(f"dense_ffn must be None, 'same' or 'int8', not {dense_ffn!r}")
     changed = 0
     tuple_out = hf_callers_unpack_tuples()
     for layer in model.model.layers:
@@ -285,4 +290,8 @@ def patch(model, rank, world, policy="fifo", few_tokens=0):
             changed += 1
     if not changed:
         raise RuntimeError("No Qwen2MoeSparseMoeBlock found: wrong checkpoint/model version")
+    if dense_ffn is not None:
+        from .plugin import replace_dense_ffn
+
+        replace_dense_ffn(model, "Qwen2MoeDecoderLayer", "Qwen2MoeMLP", int8=dense_ffn == "int8")
     return changed
