@@ -11,8 +11,8 @@ bool at(const void* p, uintptr_t n) { return p != nullptr && reinterpret_cast<ui
 bool at_or_null(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 int64_t esize(int dtype) { return dtype == DSCA_BF16 ? 2 : 4; }
 bool dim_ok(int64_t v) { return v >= 1 && v <= DSCA_DENSE_MAX_DIM; }
-// a row stride no larger than 2^40 elements keeps every offset of 2^24 rows inside 64 bits
-bool ld_ok(int64_t ld, int64_t width) { return ld >= width && ld < (int64_t(1) << 40); }
+// a row stride below 2^37 elements: TMA's 2^40 bytes, and every offset of 2^24 rows inside 64 bits
+bool ld_ok(int64_t ld, int64_t width) { return ld >= width && ld < (int64_t(1) << 37); }
 bool type_ok(int dtype) { return dtype == DSCA_BF16 || dtype == DSCA_F32; }
 bool act_ok(int act) { return act == DSCA_GATE_SILU || act == DSCA_GATE_GELU || act == DSCA_GATE_RELU; }
 
@@ -102,74 +102,170 @@ int check(const dsca_gated_ffn_int8_args* a) {
   return DSCA_OK;
 }
 
-int run(const dsca_gated_ffn_args* a, cudaStream_t s) {
-  Job j = {};
-  j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = a->dtype;
-  j.prob[0] = problem({a->w_gate, a->ld_gate, 0}, {a->x, a->ld_x, 0}, a->inter, a->rows, a->d, a->h, a->ld_h);
-  j.prob[0].a[1] = {a->w_up, a->ld_up, 0};
-  j.save_g = a->g; j.save_u = a->u;
-  if (int rc = launch_simt(j, s)) return rc;
-  Job k = {};
-  k.epi = kStore; k.nprob = 1; k.dtype = a->dtype;
-  k.prob[0] = problem({a->w_down, a->ld_down, 0}, {a->h, a->ld_h, 0}, a->d, a->rows, a->inter, a->y, a->ld_y);
-  return launch_simt(k, s);
-}
+// ---------------------------------------------------------------- calls as lists of launches
+//
+// Each entry point is written once, as a function that lays out its workspace and issues its launches; `dry`, it
+// only adds up the workspace's bytes.
+struct Call {
+  bool dry;
+  uint8_t* base;
+  cudaStream_t stream;
+  int32_t* err;
+  size_t used = 0;
+  RelayList relays = {};
 
-int run(const dsca_gated_ffn_backward_args* a, cudaStream_t s) {
-  const int T = a->rows, d = a->d, I = a->inter;
-  Job j = {};
-  j.epi = kDGlu; j.act = a->act; j.nprob = 1; j.dtype = a->dtype;
-  j.prob[0] = problem({a->w_down, a->ld_down, 1}, {a->dy, a->ld_dy, 0}, I, T, d, a->dg, a->ld_h);
-  j.save_g = const_cast<void*>(a->g); j.save_u = const_cast<void*>(a->u); j.out2 = a->du;
-  if (a->dx != nullptr || a->d_gate != nullptr || a->d_up != nullptr)
-    if (int rc = launch_simt(j, s)) return rc;
-  Job k = {};
-  k.epi = kStore; k.dtype = a->dtype;
-  if (a->dx != nullptr) {
-    Problem p = problem({a->w_gate, a->ld_gate, 1}, {a->dg, a->ld_h, 0}, d, T, I, a->dx, d);
-    p.nseg = 2;
-    p.a[1] = {a->w_up, a->ld_up, 1};
-    p.b[1] = {a->du, a->ld_h, 0};
-    k.prob[k.nprob++] = p;
+  void* take(size_t bytes) {
+    const size_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    return dry ? nullptr : base + at;
   }
-  const Operand x = {a->x, a->ld_x, 1};
-  if (a->d_gate != nullptr) k.prob[k.nprob++] = problem(x, {a->dg, a->ld_h, 1}, d, I, T, a->d_gate, d);
-  if (a->d_up != nullptr) k.prob[k.nprob++] = problem(x, {a->du, a->ld_h, 1}, d, I, T, a->d_up, d);
+  // A matrix as an operand: as it lies where TMA can load it, otherwise laid out anew (by relay()).
+  Operand operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype, int mn) {
+    if (dtype == DSCA_BF16 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0) return {p, ld, mn, 0};
+    const bool f32 = dtype == DSCA_F32;
+    const int64_t ldd = (cols + 7) / 8 * 8, rows_p = f32 ? (rows + 15) / 16 * 16 : rows;
+    void* dst = take((size_t)(rows_p * ldd) * (f32 ? 6 : 2));
+    relays.item[relays.n++] = {p, dst, rows, rows_p, cols, ld, ldd, dtype, 0, 0};
+    return {dst, ldd, mn, rows_p};
+  }
+  // The launch that lays out what operand() collected; false in *none when there was something.
+  int relay(bool* none) {
+    *none = relays.n == 0;
+    const int rc = dry || relays.n == 0 ? DSCA_OK : launch_relay(relays, stream);
+    relays.n = 0;
+    return rc;
+  }
+  // A job's own workspace (partial tiles), its counters zeroed: before the first launch, so that nothing lies
+  // between products that follow one another.
+  int reserve(const Job& j, void** ws) {
+    const size_t bytes = tc_workspace(j), zero = tc_zero_bytes(j);
+    *ws = bytes != 0 ? take(bytes) : nullptr;
+    if (!dry && zero != 0 && cudaMemsetAsync(*ws, 0, zero, stream) != cudaSuccess) return DSCA_ERR_CUDA;
+    return DSCA_OK;
+  }
+  int product(const Job& j, void* ws, bool pdl) { return dry ? DSCA_OK : launch_tc(j, ws, err, pdl, stream); }
+  int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale) {
+    dsca_quantize_rows_args a = {x, rows, k, dtype, ld_x, q, ld_q, scale};
+    return dry ? DSCA_OK : launch_quantize_rows(&a, stream);
+  }
+};
+
+Operand as(Operand o, int mn) {
+  o.mn = mn;
+  return o;
+}
+
+#define TRY(call) \
+  if (int rc_ = (call)) return rc_
+
+int run(Call& c, const dsca_gated_ffn_args* a) {
+  const int dt = a->dtype, T = a->rows, d = a->d, I = a->inter;
+  Job j = {}, k = {};
+  j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
+  j.prob[0] = problem(c.operand(a->w_gate, I, d, a->ld_gate, dt, 0), c.operand(a->x, T, d, a->ld_x, dt, 0), I, T, d,
+                      a->h, a->ld_h);
+  j.prob[0].a[1] = c.operand(a->w_up, I, d, a->ld_up, dt, 0);
+  j.save_g = a->g; j.save_u = a->u;
+  k.epi = kStore; k.nprob = 1; k.dtype = dt;
+  k.prob[0] = problem(c.operand(a->w_down, d, I, a->ld_down, dt, 0), {}, d, T, I, a->y, a->ld_y);
+  void *wj, *wk;
+  bool none;
+  TRY(c.reserve(j, &wj));
+  TRY(c.reserve(k, &wk));
+  TRY(c.relay(&none));
+  TRY(c.product(j, wj, false));
+  k.prob[0].b[0] = c.operand(a->h, T, I, a->ld_h, dt, 0);
+  TRY(c.relay(&none));
+  return c.product(k, wk, none);
+}
+
+int run(Call& c, const dsca_gated_ffn_backward_args* a) {
+  const int dt = a->dtype, T = a->rows, d = a->d, I = a->inter;
+  const bool weights = a->d_gate != nullptr || a->d_up != nullptr;
+  const bool inner = a->dx != nullptr || weights;
+  Job j = {}, k = {};
+  void *wj = nullptr, *wk = nullptr;
+  bool none;
+  const Operand dy = c.operand(a->dy, T, d, a->ld_dy, dt, 0);
+  if (inner) {
+    j.epi = kDGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
+    j.prob[0] = problem(c.operand(a->w_down, d, I, a->ld_down, dt, 1), dy, I, T, d, a->dg, a->ld_h);
+    j.save_g = const_cast<float*>(a->g); j.save_u = const_cast<float*>(a->u); j.out2 = a->du;
+    TRY(c.reserve(j, &wj));
+    TRY(c.relay(&none));
+    TRY(c.product(j, wj, false));
+  }
+  k.epi = kStore; k.dtype = dt;
+  Operand dg = {}, du = {};
+  if (a->dx != nullptr || a->d_gate != nullptr) dg = c.operand(a->dg, T, I, a->ld_h, dt, 0);
+  if (a->dx != nullptr || a->d_up != nullptr) du = c.operand(a->du, T, I, a->ld_h, dt, 0);
+  if (a->dx != nullptr) {
+    Problem& p = k.prob[k.nprob++];
+    p = problem(c.operand(a->w_gate, I, d, a->ld_gate, dt, 1), dg, d, T, I, a->dx, d);
+    p.nseg = 2;
+    p.a[1] = c.operand(a->w_up, I, d, a->ld_up, dt, 1);
+    p.b[1] = du;
+  }
+  if (weights) {
+    const Operand x = c.operand(a->x, T, d, a->ld_x, dt, 1);
+    if (a->d_gate != nullptr) k.prob[k.nprob++] = problem(x, as(dg, 1), d, I, T, a->d_gate, d);
+    if (a->d_up != nullptr) k.prob[k.nprob++] = problem(x, as(du, 1), d, I, T, a->d_up, d);
+  }
   if (a->d_down != nullptr)
-    k.prob[k.nprob++] = problem({a->h, a->ld_h, 1}, {a->dy, a->ld_dy, 1}, I, d, T, a->d_down, I);
-  return k.nprob ? launch_simt(k, s) : DSCA_OK;
+    k.prob[k.nprob++] = problem(c.operand(a->h, T, I, a->ld_h, dt, 1), as(dy, 1), I, d, T, a->d_down, I);
+  if (k.nprob == 0) return DSCA_OK;
+  TRY(c.reserve(k, &wk));
+  TRY(c.relay(&none));
+  // a memset of counters lies between the two as well where one of the products is split
+  return c.product(k, wk, inner && none && wk == nullptr);
 }
 
-int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale,
-             cudaStream_t s) {
-  dsca_quantize_rows_args a = {x, rows, k, dtype, ld_x, q, ld_q, scale};
-  return launch_quantize_rows(&a, s);
-}
-
-int run(const dsca_int8_linear_args* a, cudaStream_t s) {
-  if (a->x != nullptr)
-    if (int rc = quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, s)) return rc;
+int run(Call& c, const dsca_int8_linear_args* a) {
   Job j = {};
   j.epi = kStore; j.nprob = 1; j.dtype = a->dtype; j.i8 = 1;
-  j.prob[0] = problem({a->w, a->ld_w, 0}, {a->q, a->ld_q, 0}, a->n, a->rows, a->k, a->y, a->ld_y);
+  j.prob[0] = problem({a->w, a->ld_w, 0, 0}, {a->q, a->ld_q, 0, 0}, a->n, a->rows, a->k, a->y, a->ld_y);
   j.row_scale = a->scale; j.col_scale[0] = a->w_scale; j.bias = a->bias;
-  return launch_simt(j, s);
+  void* wj;
+  TRY(c.reserve(j, &wj));
+  if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale));
+  return c.product(j, wj, a->x != nullptr);
 }
 
-int run(const dsca_gated_ffn_int8_args* a, cudaStream_t s) {
-  if (int rc = quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, s)) return rc;
-  Job j = {};
+int run(Call& c, const dsca_gated_ffn_int8_args* a) {
+  Job j = {}, k = {};
   j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = DSCA_F32; j.i8 = 1;
-  j.prob[0] = problem({a->w_gate, a->ld_gate, 0}, {a->q, a->ld_q, 0}, a->inter, a->rows, a->d, a->h, a->ld_h);
-  j.prob[0].a[1] = {a->w_up, a->ld_up, 0};
+  j.prob[0] = problem({a->w_gate, a->ld_gate, 0, 0}, {a->q, a->ld_q, 0, 0}, a->inter, a->rows, a->d, a->h, a->ld_h);
+  j.prob[0].a[1] = {a->w_up, a->ld_up, 0, 0};
   j.row_scale = a->scale; j.col_scale[0] = a->gate_scale; j.col_scale[1] = a->up_scale;
-  if (int rc = launch_simt(j, s)) return rc;
-  if (int rc = quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale, s)) return rc;
-  Job k = {};
   k.epi = kStore; k.nprob = 1; k.dtype = a->dtype; k.i8 = 1;
-  k.prob[0] = problem({a->w_down, a->ld_down, 0}, {a->hq, a->ld_hq, 0}, a->d, a->rows, a->inter, a->y, a->ld_y);
+  k.prob[0] = problem({a->w_down, a->ld_down, 0, 0}, {a->hq, a->ld_hq, 0, 0}, a->d, a->rows, a->inter, a->y, a->ld_y);
   k.row_scale = a->h_scale; k.col_scale[0] = a->down_scale;
-  return launch_simt(k, s);
+  void *wj, *wk;
+  TRY(c.reserve(j, &wj));
+  TRY(c.reserve(k, &wk));
+  TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale));
+  TRY(c.product(j, wj, true));
+  TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale));
+  return c.product(k, wk, true);
+}
+
+#undef TRY
+
+template <typename Args>
+int call(const Args* a, cudaStream_t stream) {
+  Call size = {true, nullptr, nullptr, nullptr};
+  if (int rc = run(size, a)) return rc;
+  if (size.used > a->workspace_bytes) return DSCA_ERR_CAPACITY;
+  if (size.used != 0 && !at(a->workspace, 256)) return DSCA_ERR_BAD_ARG;
+  Call c = {false, reinterpret_cast<uint8_t*>(a->workspace), stream, a->err};
+  return run(c, a);
+}
+
+template <typename Args>
+size_t workspace(const Args* a) {
+  if (check(a) != DSCA_OK || a->rows == 0) return 0;
+  Call size = {true, nullptr, nullptr, nullptr};
+  return run(size, a) == DSCA_OK ? size.used : 0;
 }
 
 }  // namespace
@@ -182,7 +278,7 @@ extern "C" {
 
 int dsca_gated_ffn(const dsca_gated_ffn_args* a, dsca_stream_t stream) {
   if (int rc = dense::check(a)) return rc;
-  return a->rows == 0 ? DSCA_OK : dense::run(a, stream);
+  return a->rows == 0 ? DSCA_OK : dense::call(a, stream);
 }
 
 int dsca_gated_ffn_backward(const dsca_gated_ffn_backward_args* a, dsca_stream_t stream) {
@@ -193,7 +289,7 @@ int dsca_gated_ffn_backward(const dsca_gated_ffn_backward_args* a, dsca_stream_t
       if (p != nullptr && cudaMemsetAsync(p, 0, bytes, stream) != cudaSuccess) return DSCA_ERR_CUDA;
     return DSCA_OK;
   }
-  return dense::run(a, stream);
+  return dense::call(a, stream);
 }
 
 int dsca_quantize_rows(const dsca_quantize_rows_args* a, dsca_stream_t stream) {
@@ -203,17 +299,17 @@ int dsca_quantize_rows(const dsca_quantize_rows_args* a, dsca_stream_t stream) {
 
 int dsca_int8_linear(const dsca_int8_linear_args* a, dsca_stream_t stream) {
   if (int rc = dense::check(a)) return rc;
-  return a->rows == 0 ? DSCA_OK : dense::run(a, stream);
+  return a->rows == 0 ? DSCA_OK : dense::call(a, stream);
 }
 
 int dsca_gated_ffn_int8(const dsca_gated_ffn_int8_args* a, dsca_stream_t stream) {
   if (int rc = dense::check(a)) return rc;
-  return a->rows == 0 ? DSCA_OK : dense::run(a, stream);
+  return a->rows == 0 ? DSCA_OK : dense::call(a, stream);
 }
 
-size_t dsca_gated_ffn_workspace(const dsca_gated_ffn_args* a) { return dense::check(a) ? 0 : 0; }
-size_t dsca_gated_ffn_backward_workspace(const dsca_gated_ffn_backward_args* a) { return dense::check(a) ? 0 : 0; }
-size_t dsca_int8_linear_workspace(const dsca_int8_linear_args* a) { return dense::check(a) ? 0 : 0; }
-size_t dsca_gated_ffn_int8_workspace(const dsca_gated_ffn_int8_args* a) { return dense::check(a) ? 0 : 0; }
+size_t dsca_gated_ffn_workspace(const dsca_gated_ffn_args* a) { return dense::workspace(a); }
+size_t dsca_gated_ffn_backward_workspace(const dsca_gated_ffn_backward_args* a) { return dense::workspace(a); }
+size_t dsca_int8_linear_workspace(const dsca_int8_linear_args* a) { return dense::workspace(a); }
+size_t dsca_gated_ffn_int8_workspace(const dsca_gated_ffn_int8_args* a) { return dense::workspace(a); }
 
 }  // extern "C"

@@ -14,8 +14,9 @@ namespace dense {
 
 struct Operand {
   const void* p;
-  int64_t ld;  // elements
-  int mn;      // 0 K-major, 1 MN-major
+  int64_t ld;     // elements
+  int mn;         // 0 K-major, 1 MN-major
+  int64_t plane;  // fp32 products: rows from one plane of bf16 terms to the next
 };
 
 // Up to two segments whose sums are added: out = sum_s A_s B_s^T (dx = dg Wg + du Wu).
@@ -37,8 +38,8 @@ struct Job {
   int i8;         // operands are 8-bit integers, the sum int32
   int dtype;      // of the operands (unless i8) and of out
   Problem prob[kMaxProblems];
-  void* save_g;   // kGlu: written; kDGlu: read (same for u); rows of prob[0].ldo
-  void* save_u;
+  float* save_g;  // kGlu: written; kDGlu: read (same for u); rows of prob[0].ldo
+  float* save_u;
   void* out2;     // kDGlu: du
   const float* row_scale;
   const float* col_scale[2];
@@ -88,7 +89,25 @@ __device__ __forceinline__ void gate_grad(float g, int act, float* a, float* da)
   }
 }
 
-int launch_simt(const Job& j, cudaStream_t stream);
+// A matrix to lay out anew (dense_split.cu).
+struct Relay {
+  const void* src;
+  void* dst;
+  int64_t rows, rows_p, cols, lds, ldd;  // ldd a multiple of 8
+  int dtype, vec;
+  uint32_t first;
+};
+constexpr int kMaxRelays = 8;
+struct RelayList {
+  Relay item[kMaxRelays];
+  int n;
+};
+int launch_relay(RelayList& list, cudaStream_t stream);
+
+// Tensor-core products (dense_tc.cu).  ws: tc_workspace() bytes, of which the first tc_zero_bytes() are zero.
+size_t tc_workspace(const Job& j);
+size_t tc_zero_bytes(const Job& j);
+int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t stream);
 int launch_quantize_rows(const dsca_quantize_rows_args* a, cudaStream_t stream);
 
 }  // namespace dense

@@ -90,32 +90,33 @@ def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
     rows, d, inter, ld_x, ld_g, ld_u, ld_d = shapes
     y = torch.empty(x.shape, dtype=dtype, device=dev)
     if rows == 0:
-        return y, None
+        return y, (None, None)
     ld_h = (inter + 7) // 8 * 8
-    buf = torch.empty((3 if save else 1, rows, ld_h), dtype=dtype, device=dev)
-    step = rows * ld_h * buf.element_size()
-    h = buf.data_ptr()
-    g, u = (h + step, h + 2 * step) if save else (None, None)
-    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, h, rows, d, inter,
-                       _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
+    h = torch.empty((rows, ld_h), dtype=dtype, device=dev)
+    # g and u in fp32: the backward pass then rounds nothing but its products' operands
+    gu = torch.empty((2, rows, ld_h), dtype=torch.float32, device=dev) if save else None
+    g = gu.data_ptr() if save else None
+    u = g + 4 * rows * ld_h if save else None
+    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, h.data_ptr(), rows, d,
+                       inter, _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
     with torch.cuda.device(dev):
         ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
-    return y, buf
+    return y, (h, gu)
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, wd, act, shapes):
-        y, buf = _forward(x, wg, wu, wd, act, shapes, True)
+        y, (h, gu) = _forward(x, wg, wu, wd, act, shapes, True)
         ctx.act, ctx.shapes = act, shapes
-        ctx.save_for_backward(x, wg, wu, wd, buf)
+        ctx.save_for_backward(x, wg, wu, wd, h, gu)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, buf = ctx.saved_tensors
+        x, wg, wu, wd, h, gu = ctx.saved_tensors
         rows, d, inter, ld_x, ld_g, ld_u, ld_d = ctx.shapes
         dev, dtype = x.device, x.dtype
         need = ctx.needs_input_grad
@@ -133,13 +134,11 @@ class _GatedFFN(torch.autograd.Function):
                 ld_dy = d if dy.is_contiguous() else _stride(dy, "dy", d)
             except ValueError:  # a gradient may come in any strides (expanded, transposed)
                 dy, ld_dy = dy.contiguous(), d
-            ld_h = buf.shape[2]
-            step = rows * ld_h * buf.element_size()
+            ld_h = h.shape[1]
             grads = torch.empty((2, rows, ld_h), dtype=dtype, device=dev)
             a.x, a.w_gate, a.w_up, a.w_down, a.dy = (t.data_ptr() for t in (x, wg, wu, wd, dy))
-            h = buf.data_ptr()
-            a.h, a.g, a.u = h, h + step, h + 2 * step
-            a.dg, a.du = grads.data_ptr(), grads.data_ptr() + step
+            a.h, a.g, a.u = h.data_ptr(), gu.data_ptr(), gu.data_ptr() + 4 * rows * ld_h
+            a.dg, a.du = grads.data_ptr(), grads.data_ptr() + rows * ld_h * grads.element_size()
             a.ld_x, a.ld_gate, a.ld_up, a.ld_down, a.ld_dy, a.ld_h = ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h
             a.err = _err(dev)
             with torch.cuda.device(dev):
@@ -155,9 +154,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     x [..., d] bf16 or fp32 (rows may lie in a wider buffer), w_gate and w_up [inter, d], w_down
     [d, inter] of x's type, as Linear layers hold them.  act: "silu", "gelu" (tanh form) or "relu".
-    Products are summed in fp32; for bf16 the gate, up and intermediate values are rounded to bf16 once
-    each (the intermediate from the unrounded ones).  Under autograd the call keeps the three [rows,
-    inter] intermediates for the backward pass; second derivatives are not offered.  Runs on x's
+    Products are summed in fp32; the gated intermediate is rounded to x's type, and so are its two
+    gradients in the backward pass.  Under autograd the call keeps the intermediate and, in fp32, the gate
+    and up values, each [rows, inter], for the backward pass; second derivatives are not offered.  Runs on x's
     device, on its current stream; check_dense() reports a wait that ran out."""
     code = _act(act)
     if x.dtype not in _DTYPES:

@@ -29,9 +29,8 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 #define DSCA_DENSE_MAX_ROWS 16777216
 
 /*
- * g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T; sums in fp32, g, u, h and y rounded to dtype
- * (h from the unrounded g and u).  g and u are written when given (both or neither): the backward
- * pass reads them.  h is a work area [rows, ld_h] that the backward pass reads as well.
+ * g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T; sums in fp32, h and y rounded to dtype.  g and u
+ * are written in fp32 when given (both or neither): the backward pass reads them.  h is a work area [rows, ld_h] that the backward pass reads as well.
  */
 typedef struct {
   const void* x;        /* [rows, d], dtype */
@@ -39,14 +38,14 @@ typedef struct {
   const void* w_up;     /* [inter, d] */
   const void* w_down;   /* [d, inter] */
   void* y;              /* [rows, d] */
-  void* g;              /* [rows, ld_h] or NULL */
-  void* u;
+  float* g;             /* [rows, ld_h] or NULL */
+  float* u;
   void* h;              /* [rows, ld_h] */
   int rows, d, inter;
   int dtype;            /* DSCA_BF16, DSCA_F32 */
   int act;              /* DSCA_GATE_* */
   int64_t ld_x, ld_gate, ld_up, ld_down, ld_y;
-  int64_t ld_h;         /* of g, u, h: a multiple of 16 bytes, at least inter; g, u, h 16-byte aligned */
+  int64_t ld_h;         /* of g, u, h, in elements: rows of h a multiple of 16 bytes apart, at least inter; g, u, h 16-byte aligned */
   void* workspace;      /* dsca_dense_workspace_bytes(), 256-byte aligned; may be NULL when that is 0 */
   size_t workspace_bytes;
   int32_t* err;
@@ -64,8 +63,8 @@ typedef struct {
   const void* w_up;
   const void* w_down;
   const void* dy;       /* [rows, d] */
-  const void* g;        /* as dsca_gated_ffn wrote them */
-  const void* u;
+  const float* g;       /* as dsca_gated_ffn wrote them */
+  const float* u;
   const void* h;
   void* dx;             /* [rows, d] contiguous, or NULL */
   void* d_gate;         /* [inter, d] contiguous, or NULL */
