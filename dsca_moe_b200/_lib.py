@@ -129,14 +129,14 @@ DENSE_MAX_ROWS = 16777216
 
 class GatedFfnArgs(ctypes.Structure):
     _fields_ = [("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("y", _vp), ("g", _vp), ("u", _vp),
-                ("h", _vp), ("rows", _i), ("d", _i), ("inter", _i), ("dtype", _i), ("act", _i), ("ld_x", _i64),
+                ("gu_exp", _vp), ("h", _vp), ("rows", _i), ("d", _i), ("inter", _i), ("dtype", _i), ("act", _i), ("ld_x", _i64),
                 ("ld_gate", _i64), ("ld_up", _i64), ("ld_down", _i64), ("ld_y", _i64), ("ld_h", _i64),
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]
 
 
 class GatedFfnBackwardArgs(ctypes.Structure):
     _fields_ = [("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("dy", _vp), ("g", _vp), ("u", _vp),
-                ("h", _vp), ("dx", _vp), ("d_gate", _vp), ("d_up", _vp), ("d_down", _vp), ("dg", _vp), ("du", _vp),
+                ("gu_exp", _vp), ("h", _vp), ("dx", _vp), ("d_gate", _vp), ("d_up", _vp), ("d_down", _vp), ("dg", _vp), ("du", _vp),
                 ("rows", _i), ("d", _i), ("inter", _i), ("dtype", _i), ("act", _i), ("ld_x", _i64), ("ld_gate", _i64),
                 ("ld_up", _i64), ("ld_down", _i64), ("ld_dy", _i64), ("ld_h", _i64), ("workspace", _vp),
                 ("workspace_bytes", ctypes.c_size_t), ("err", _vp)]

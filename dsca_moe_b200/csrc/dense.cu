@@ -34,7 +34,8 @@ int check(const dsca_gated_ffn_args* a) {
   if (a->rows == 0) return DSCA_OK;
   const int64_t e = esize(a->dtype);
   if (!at(a->x, e) || !at(a->w_gate, e) || !at(a->w_up, e) || !at(a->w_down, e) || !at(a->y, e) || !at(a->h, 16) ||
-      !at_or_null(a->g, 16) || !at_or_null(a->u, 16) || (a->g == nullptr) != (a->u == nullptr))
+      !at_or_null(a->g, 16) || !at_or_null(a->u, 16) || (a->g == nullptr) != (a->u == nullptr) ||
+      (a->g != nullptr && a->dtype == DSCA_BF16 && a->gu_exp == nullptr))
     return DSCA_ERR_BAD_ARG;
   if (!ld_ok(a->ld_x, a->d) || !ld_ok(a->ld_gate, a->d) || !ld_ok(a->ld_up, a->d) || !ld_ok(a->ld_down, a->inter) ||
       !ld_ok(a->ld_y, a->d) || !ld_ok(a->ld_h, a->inter) || a->ld_h * e % 16 != 0)
@@ -51,7 +52,8 @@ int check(const dsca_gated_ffn_backward_args* a) {
     return DSCA_ERR_BAD_ARG;
   if (a->rows == 0) return DSCA_OK;
   if (!at(a->x, e) || !at(a->w_gate, e) || !at(a->w_up, e) || !at(a->w_down, e) || !at(a->dy, e) || !at(a->g, 16) ||
-      !at(a->u, 16) || !at(a->h, 16) || !at(a->dg, 16) || !at(a->du, 16))
+      !at(a->u, 16) || !at(a->h, 16) || !at(a->dg, 16) || !at(a->du, 16) ||
+      (a->dtype == DSCA_BF16 && a->gu_exp == nullptr))
     return DSCA_ERR_BAD_ARG;
   if (!ld_ok(a->ld_x, a->d) || !ld_ok(a->ld_gate, a->d) || !ld_ok(a->ld_up, a->d) || !ld_ok(a->ld_down, a->inter) ||
       !ld_ok(a->ld_dy, a->d) || !ld_ok(a->ld_h, a->inter) || a->ld_h * e % 16 != 0)
@@ -165,7 +167,7 @@ int run(Call& c, const dsca_gated_ffn_args* a) {
   j.prob[0] = problem(c.operand(a->w_gate, I, d, a->ld_gate, dt, 0), c.operand(a->x, T, d, a->ld_x, dt, 0), I, T, d,
                       a->h, a->ld_h);
   j.prob[0].a[1] = c.operand(a->w_up, I, d, a->ld_up, dt, 0);
-  j.save_g = a->g; j.save_u = a->u;
+  j.save_g = a->g; j.save_u = a->u; j.save_e = a->gu_exp;
   k.epi = kStore; k.nprob = 1; k.dtype = dt;
   k.prob[0] = problem(c.operand(a->w_down, d, I, a->ld_down, dt, 0), {}, d, T, I, a->y, a->ld_y);
   void *wj, *wk;
@@ -190,7 +192,8 @@ int run(Call& c, const dsca_gated_ffn_backward_args* a) {
   if (inner) {
     j.epi = kDGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
     j.prob[0] = problem(c.operand(a->w_down, d, I, a->ld_down, dt, 1), dy, I, T, d, a->dg, a->ld_h);
-    j.save_g = const_cast<float*>(a->g); j.save_u = const_cast<float*>(a->u); j.out2 = a->du;
+    j.save_g = const_cast<void*>(a->g); j.save_u = const_cast<void*>(a->u); j.out2 = a->du;
+    j.save_e = const_cast<uint8_t*>(a->gu_exp);
     TRY(c.reserve(j, &wj));
     TRY(c.relay(&none));
     TRY(c.product(j, wj, false));

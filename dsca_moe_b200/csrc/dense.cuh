@@ -38,8 +38,9 @@ struct Job {
   int i8;         // operands are 8-bit integers, the sum int32
   int dtype;      // of the operands (unless i8) and of out
   Problem prob[kMaxProblems];
-  float* save_g;  // kGlu: written; kDGlu: read (same for u); rows of prob[0].ldo
-  float* save_u;
+  void* save_g;   // kGlu: written; kDGlu: read (same for u); rows of prob[0].ldo
+  void* save_u;
+  uint8_t* save_e;
   void* out2;     // kDGlu: du
   const float* row_scale;
   const float* col_scale[2];

@@ -11,9 +11,15 @@
 // rows of k by 64 values of m or n, which the MMA reads transposed, so that the gradients' products take
 // weights and activations as they lie.
 //
-// Gated products (kGlu): a CTA's 128 rows of A are eight boxes of 16 rows, alternately gate and up rows of
-// the same 16 channels.  The gate and up values of a channel then lie 16 lanes apart in the same TMEM
-// quarter, and one shuffle in a warp brings them together.
+// Gated products (kGlu): a CTA's 128 rows of A are 64 gate rows and the up rows of the same channels, so the
+// epilogue warps of lane quarters q and q + 2 hold the gate and up values of the same 32 channels.  For each
+// chunk of 32 columns the gate warp forms the products of the first 16 and the up warp those of the last,
+// after handing each other the other half through shared memory.  (Alternating boxes of 16 gate and 16 up
+// rows would bring both into one warp, but eight small boxes instead of two cost more than the exchange:
+// 4096 x 2048 x 5632 188 us against 152.)
+// Saved for the backward pass in 16 bits: g and u as fp16 with one power of two for a channel's 32 tokens
+// (11 bits of significand for every value within 2^29 of the largest), half of fp32's bytes, which the
+// backward pass reads against the clock of its first product.
 //
 // 32-bit inputs (kF32): every value is split into three bf16 terms (8 + 8 + 8 bits, dense_split.cu) and the
 // product is six MMA passes over k: hi.hi into one accumulator, hi.mid, mid.hi, hi.lo, mid.mid and lo.hi into
@@ -34,9 +40,13 @@ namespace dsca {
 namespace dense {
 namespace tc {
 
-constexpr int kStages = 3;
+#ifndef KSUB
+#define KSUB 2
+#endif
+constexpr int kSub = KSUB;                       // k boxes of a stage
+constexpr int kStages = 6 / kSub;
 constexpr int kBoxBytes = 128 * 128;             // an operand's part of one k box
-constexpr int kStageBytes = 4 * kBoxBytes;       // A and B, two boxes
+constexpr int kStageBytes = 2 * kSub * kBoxBytes;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kStgBytes = 2 * 32 * 32 * 2;       // per epilogue warp: two 32 x 32 blocks of bf16
@@ -65,8 +75,9 @@ struct Params {
   CUtensorMap a[kMaxProblems][2], b[kMaxProblems][2];
   Prob prob[kMaxProblems];
   int nprob, total, act;
-  float* save_g;
-  float* save_u;
+  void* save_g;   // fp16 codes (16-bit inputs) or fp32
+  void* save_u;
+  uint8_t* save_e;  // fp16: the exponents, [2][ceil(N / 32)][ldo]
   void* out2;
   const float* row_scale;
   const float* col_scale[2];
@@ -80,6 +91,7 @@ struct Ctl {
   uint64_t full[kStages], empty[kStages], tmem_full[2], tmem_empty[2], mma_done;
   uint32_t tmem_base;
   int abort_flag;
+  int pair_ok[kEpiWarps], pair_old[kEpiWarps];
 };
 
 struct Tile {
@@ -135,23 +147,86 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, ui
       : "memory");
 }
 
-// box b of a problem: segment, term and slice of k
+// Where box b of a problem lies: slice k of a segment and, for 32-bit inputs, one of the six terms, which follow
+// one another within a slice.  Divisions once a tile, then counted on.
 template <int IN>
-__device__ __forceinline__ void box_at(const Prob& q, int b, int& seg, int& term, int& k) {
-  if constexpr (IN == kF32) {  // a slice's six terms follow one another
-    const int s = b / 6;
-    term = b - 6 * s;
-    seg = s / q.kb;
-    k = s - seg * q.kb;
-  } else {
-    seg = b / q.kb;
-    k = b - seg * q.kb;
+struct BoxAt {
+  int seg, term, k;
+  __device__ __forceinline__ BoxAt(const Prob& q, int b) {
+    int s = b;
     term = 0;
+    if constexpr (IN == kF32) {
+      s = b / 6;
+      term = b - 6 * s;
+    }
+    seg = s >= q.kb ? 1 : 0;
+    k = s - seg * q.kb;
   }
-}
+  __device__ __forceinline__ void next(int kb) {
+    if constexpr (IN == kF32) {
+      if (++term < 6) return;
+      term = 0;
+    }
+    if (++k == kb) {
+      k = 0;
+      ++seg;
+    }
+  }
+};
 // the planes (hi 0, mid 1, lo 2) that term t multiplies
 __device__ __forceinline__ int plane_a(int t) { return t == 2 || t == 4 ? 1 : t == 5 ? 2 : 0; }
 __device__ __forceinline__ int plane_b(int t) { return t == 1 || t == 4 ? 1 : t == 3 ? 2 : 0; }
+
+// The two warps (64 threads) that exchange gate and up values.
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// 32 tokens of one channel as fp16 times a power of two that brings the largest finite one to [2^14, 2^15); the
+// exponent byte is the largest's, at least 14 so that the factor is a normal number.
+__device__ __forceinline__ void save_f16(const Params& P, const Prob& q, int up, int ch, int n, int ntok, const float (&v)[32]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float a = fabsf(v[j]);
+    if (j < ntok && a <= 3.4028234663852886e38f) m = fmaxf(m, a);
+  }
+  const uint32_t e = max(14u, __float_as_uint(m) >> 23);
+  const float s = __uint_as_float((268u - e) << 23);  // 2^(141 - e)
+  if (ch >= q.M) return;
+  __half* at = reinterpret_cast<__half*>(up ? P.save_u : P.save_g) + (int64_t)n * q.ldo + ch;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < ntok) at[j * q.ldo] = __float2half_rn(v[j] * s);
+  P.save_e[((int64_t)up * ((q.N + 31) / 32) + n / 32) * q.ldo + ch] = (uint8_t)e;
+}
+
+// g and u of the chunk after the one in work (kDGlu, 16 bits): 32 tokens x 32 channels each, 16 bytes a load.
+struct Ahead {
+  uint4 v[8];
+  uint32_t e[2];
+  __device__ __forceinline__ void load(const Params& P, const Prob& q, const Tile& t, uint32_t rank, int q4, int lane, int c) {
+    const int m0 = t.m * 256 + 128 * (int)rank + 32 * q4, ch = m0 + 8 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int tok = c + (i & 3) * 8 + (lane >> 2);
+      const __half* p = reinterpret_cast<const __half*>(i < 4 ? P.save_g : P.save_u);
+      v[i] = ch < q.M && tok < t.ntok ? __ldg(reinterpret_cast<const uint4*>(p + (int64_t)(t.n0 + tok) * q.ldo + ch))
+                                      : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      e[i] = m0 + lane < q.M && c < t.ntok
+                 ? P.save_e[((int64_t)i * ((q.N + 31) / 32) + (t.n0 + c) / 32) * q.ldo + m0 + lane] : 141u;
+  }
+  __device__ __forceinline__ void store(uint8_t* stg, int lane) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<uint4*>(stg + (i >> 2) * 2048 + ((i & 3) * 8 + (lane >> 2)) * 64 + 16 * (lane & 3)) = v[i];
+  }
+  __device__ __forceinline__ float scale(int i) const {  // 2^(e - 141)
+    const int x = (int)e[i] - 14;  // its biased exponent; 0 and 1 from e = 14, 15 on
+    return x > 0 ? __uint_as_float((uint32_t)x << 23) : 5.877471754111438e-39f;
+  }
+};
 
 template <int EPI, int IN, typename O>
 __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params P) {
@@ -162,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + 2 * kBoxBytes;  // of stage 0
+  const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + kSub * kBoxBytes;  // of stage 0
   const int warp = warp_id(), lane = lane_id();
   volatile int* abort_flag = &ctl.abort_flag;
   const uint32_t rank = cluster_ctarank();
@@ -212,36 +287,35 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         const int half = mma_n(q, t.ntok) / 2;
         const int b_row = t.n0 + half * (int)rank;
         const uint32_t b_bytes = (uint32_t)(q.tn / 2) * 128u;  // a whole box lands; rows past the tile are not used
-        for (int b = t.box0; b < t.box1; b += 2) {
+        const int kb = q.kb, a_mn = q.a_mn, b_atoms = q.b_mn ? q.tn / 128 : 0;
+        const CUtensorMap *ma = P.a[t.p], *mb = P.b[t.p];
+        BoxAt<IN> at(q, t.box0);
+        for (int b = t.box0; b < t.box1; b += kSub) {
           if (!mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, P.err)) { ok = false; break; }
           const uint32_t fb0 = mapa_shared(smem_u32(&ctl.full[s]), 0);
-          const int nb = min(2, t.box1 - b);
+          const int nb = min(kSub, t.box1 - b);
           if (rank == 0)
             mbar_arrive_expect_tx(smem_u32(&ctl.full[s]), 2u * (uint32_t)nb * ((uint32_t)kBoxBytes + b_bytes));
-          for (int h = 0; h < nb; ++h) {
-            int seg, term, k;
-            box_at<IN>(q, b + h, seg, term, k);
+          for (int h = 0; h < nb; ++h, at.next(kb)) {
             const uint32_t da = smem_a + s * kStageBytes + h * kBoxBytes, db = smem_b + s * kStageBytes + h * kBoxBytes;
-            const int pa = IN == kF32 ? plane_a(term) * q.a_plane : 0, pb = IN == kF32 ? plane_b(term) * q.b_plane : 0;
+            const int pa = IN == kF32 ? plane_a(at.term) * q.a_plane : 0, pb = IN == kF32 ? plane_b(at.term) * q.b_plane : 0;
+            const int kx = at.k * KE;
             if constexpr (kGluE) {
               const int r0 = t.m * 128 + 64 * (int)rank + pa;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                tma_load_2d_pair(da + i * 4096, &P.a[t.p][0], fb0, k * KE, r0 + 16 * i);
-                tma_load_2d_pair(da + i * 4096 + 2048, &P.a[t.p][1], fb0, k * KE, r0 + 16 * i);
-              }
-            } else if (q.a_mn) {
+              tma_load_2d_pair(da, ma, fb0, kx, r0);
+              tma_load_2d_pair(da + 8192, ma + 1, fb0, kx, r0);
+            } else if (a_mn) {
               const int r0 = t.m * 256 + 128 * (int)rank;
-              tma_load_2d_pair(da, &P.a[t.p][seg], fb0, r0, k * KE + pa);
-              tma_load_2d_pair(da + 8192, &P.a[t.p][seg], fb0, r0 + 64, k * KE + pa);
+              tma_load_2d_pair(da, ma + at.seg, fb0, r0, kx + pa);
+              tma_load_2d_pair(da + 8192, ma + at.seg, fb0, r0 + 64, kx + pa);
             } else {
-              tma_load_2d_pair(da, &P.a[t.p][seg], fb0, k * KE, t.m * 256 + 128 * (int)rank + pa);
+              tma_load_2d_pair(da, ma + at.seg, fb0, kx, t.m * 256 + 128 * (int)rank + pa);
             }
-            if (q.b_mn) {
-              for (int i = 0; i < q.tn / 128; ++i)
-                tma_load_2d_pair(db + i * 8192, &P.b[t.p][seg], fb0, b_row + 64 * i, k * KE + pb);
+            if (b_atoms) {
+              tma_load_2d_pair(db, mb + at.seg, fb0, b_row, kx + pb);
+              if (b_atoms > 1) tma_load_2d_pair(db + 8192, mb + at.seg, fb0, b_row + 64, kx + pb);
             } else {
-              tma_load_2d_pair(db, &P.b[t.p][seg], fb0, k * KE, b_row + pb);
+              tma_load_2d_pair(db, mb + at.seg, fb0, kx, b_row + pb);
             }
           }
           pending[s] = (int)ph;
@@ -271,26 +345,36 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         }
         tc_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(acc * 256);
-        const uint64_t astep = q.a_mn ? 128u : 2u, bstep = q.b_mn ? 128u : 2u;  // 16 bytes each: 2 KB or 32 bytes
-        uint32_t used[2] = {0u, 0u};
-        for (int b = t.box0; b < t.box1; b += 2) {
+        // descriptors but for the stage, and their steps of one MMA (in 16 bytes: 2 KB or 32 bytes)
+        const uint64_t ad0 = q.a_mn ? sw128_mnmajor_desc(smem_a) : sw128_kmajor_desc(smem_a);
+        const uint64_t bd0 = q.b_mn ? sw128_mnmajor_desc(smem_b) : sw128_kmajor_desc(smem_b);
+        const uint64_t astep = q.a_mn ? 128u : 2u, bstep = q.b_mn ? 128u : 2u;
+        const int kb = q.kb, last_steps = (q.K - (kb - 1) * KE + KS - 1) / KS;
+        uint32_t used0 = 0u, used1 = 0u;
+        BoxAt<IN> at(q, t.box0);
+        for (int b = t.box0; b < t.box1; b += kSub) {
           if (!mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, P.err)) { ok = false; break; }
           tc_fence_after();
-          const int nb = min(2, t.box1 - b);
-          for (int h = 0; h < nb; ++h) {
-            int seg, term, k;
-            box_at<IN>(q, b + h, seg, term, k);
-            const uint32_t da = smem_a + s * kStageBytes + h * kBoxBytes, db = smem_b + s * kStageBytes + h * kBoxBytes;
-            const uint64_t ad = q.a_mn ? sw128_mnmajor_desc(da) : sw128_kmajor_desc(da);
-            const uint64_t bd = q.b_mn ? sw128_mnmajor_desc(db) : sw128_kmajor_desc(db);
-            const int steps = (min(KE, q.K - k * KE) + KS - 1) / KS;
-            const int which = IN == kF32 && term != 0 ? 1 : 0;
-            for (int i = 0; i < steps; ++i) {
-              if constexpr (IN == kI8)
-                umma_i8_pair(d, ad + astep * i, bd + bstep * i, idesc, used[0]);
-              else
-                umma_f16_pair(d + (uint32_t)(which * 128), ad + astep * i, bd + bstep * i, idesc, used[which]);
-              used[which] = 1u;
+          const int nb = min(kSub, t.box1 - b);
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) {
+            if (h < nb) {
+              const uint64_t off = (uint64_t)((s * kStageBytes + h * kBoxBytes) >> 4);
+              const uint64_t ad = ad0 + off, bd = bd0 + off;
+              const int steps = at.k == kb - 1 ? last_steps : 4;
+              const bool corr = IN == kF32 && at.term != 0;
+              const uint32_t dd = corr ? d + 128u : d;
+              uint32_t used = corr ? used1 : used0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (i < steps) {
+                  if constexpr (IN == kI8) umma_i8_pair(dd, ad + astep * i, bd + bstep * i, idesc, used);
+                  else umma_f16_pair(dd, ad + astep * i, bd + bstep * i, idesc, used);
+                  used = 1u;
+                }
+              if (corr) used1 = 1u;
+              else used0 = 1u;
+              at.next(kb);
             }
           }
           umma_commit_pair_both(smem_u32(&ctl.empty[s]));
@@ -309,14 +393,22 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     const int q4 = warp & 3, ew = warp - 2, eh = ew >> 2;
     uint8_t* stg = smem + kStages * kStageBytes + ew * kStgBytes;
     __nv_bfloat16* stg16 = reinterpret_cast<__nv_bfloat16*>(stg);
-    int it = 0;
+    int it = 0, xb = 0;
+    Ahead ahead;
     for (int unit = unit0; unit < P.total; unit += units, ++it) {
       const Tile t = decode(P, unit);
       const Prob& q = P.prob[t.p];
       const int acc = it & 1;
+      if constexpr (EPI == kDGlu && IN == kBf16) ahead.load(P, q, t, rank, q4, lane, 32 * eh);
       int w_ok = 1;
       if (lane == 0) w_ok = mbar_wait(smem_u32(&ctl.tmem_full[acc]), (uint32_t)((it >> 1) & 1), abort_flag, P.err) ? 1 : 0;
       w_ok = __shfl_sync(0xffffffffu, w_ok, 0);
+      if constexpr (kGluE) {
+        // the two warps of an exchange go on or leave together
+        if (lane == 0) ctl.pair_ok[ew] = w_ok;
+        pair_barrier(1 + (ew & 1) + 2 * eh);
+        w_ok = *reinterpret_cast<volatile int*>(&ctl.pair_ok[ew ^ 2]) & w_ok;
+      }
       if (!w_ok) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * 256);
@@ -353,15 +445,26 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         __syncwarp();
         uint32_t old = 0;
         uint32_t* counter = P.counters + q.counter + (t.tile * 2 + rank) * kEpiWarps + ew;
-        if (lane == 0) old = atomicAdd(counter, 1u);
-        old = __shfl_sync(0xffffffffu, old, 0);
+        if constexpr (kGluE) {
+          // one count for the two warps of an exchange, which finish a tile together
+          pair_barrier(1 + (ew & 1) + 2 * eh);
+          if (!(q4 >> 1) && lane == 0) {
+            __threadfence();
+            ctl.pair_old[ew] = (int)atomicAdd(counter, 1u);
+          }
+          pair_barrier(1 + (ew & 1) + 2 * eh);
+          old = (uint32_t)*reinterpret_cast<volatile int*>(&ctl.pair_old[ew | 2]);  // the gate warps are 2, 3, 6, 7
+        } else {
+          if (lane == 0) old = atomicAdd(counter, 1u);
+          old = __shfl_sync(0xffffffffu, old, 0);
+        }
         mine = old == (uint32_t)q.splits - 1u;
         if (mine) __threadfence();
       }
       if (mine) {
         const int mrow = t.m * 256 + 128 * (int)rank + 32 * q4 + lane;  // this lane's m (not kGlu)
-        const int gch = t.m * 128 + 64 * (int)rank + 16 * q4 + (lane & 15);  // kGlu: its channel
-        const int up = lane >> 4;                                             // ... of gate (0) or up (1)
+        const int gch = t.m * 128 + 64 * (int)rank + 32 * (q4 & 1) + lane;  // kGlu: its channel
+        const int up = q4 >> 1;                                              // ... of gate (0) or up (1)
         float cs = 1.0f, bias = 0.0f;
         if constexpr (IN == kI8) {
           if constexpr (kGluE) cs = gch < q.M ? __ldg((up ? P.col_scale[1] : P.col_scale[0]) + gch) : 0.0f;
@@ -377,13 +480,28 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         for (int c = 32 * eh; c < ncol; c += 64) {
           if (c >= t.ntok) break;
           float gv[32], uv[32];
-          if constexpr (EPI == kDGlu) {  // on their way before the accumulator is read
+          if constexpr (EPI == kDGlu && IN == kBf16) {
+            // the chunk's g and u go through shared memory to the lane of their channel; the next chunk's
+            // are on their way meanwhile
+            const float sg = ahead.scale(0), su = ahead.scale(1);
+            ahead.store(stg, lane);
+            __syncwarp();
+            if (c + 64 < ncol) ahead.load(P, q, t, rank, q4, lane, c + 64);
+            const __half* sh = reinterpret_cast<const __half*>(stg);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              gv[j] = __half2float(sh[j * 32 + lane]) * sg;
+              uv[j] = __half2float(sh[1024 + j * 32 + lane]) * su;
+            }
+            __syncwarp();
+          } else if constexpr (EPI == kDGlu) {  // on their way before the accumulator is read
             const int64_t at = (int64_t)(t.n0 + c) * q.ldo + mrow;
+            const float *pg = reinterpret_cast<const float*>(P.save_g), *pu = reinterpret_cast<const float*>(P.save_u);
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const bool in = mrow < q.M && c + j < t.ntok;
-              gv[j] = in ? __ldg(P.save_g + at + j * q.ldo) : 0.0f;
-              uv[j] = in ? __ldg(P.save_u + at + j * q.ldo) : 0.0f;
+              gv[j] = in ? __ldg(pg + at + j * q.ldo) : 0.0f;
+              uv[j] = in ? __ldg(pu + at + j * q.ldo) : 0.0f;
             }
           }
           float v[32];
@@ -416,35 +534,47 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             }
           }
           if constexpr (kGluE) {
-            if (P.save_g != nullptr && gch < q.M) {
-              float* at = (up ? P.save_u : P.save_g) + (int64_t)(t.n0 + c) * q.ldo + gch;
+            if (P.save_g != nullptr) {
+              if constexpr (IN == kBf16) save_f16(P, q, up, gch, t.n0 + c, t.ntok - c, v);
+              else if (gch < q.M) {
+                float* at = reinterpret_cast<float*>(up ? P.save_u : P.save_g) + (int64_t)(t.n0 + c) * q.ldo + gch;
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (c + j < t.ntok) at[j * q.ldo] = v[j];
+                for (int j = 0; j < 32; ++j)
+                  if (c + j < t.ntok) at[j * q.ldo] = v[j];
+              }
             }
-            // the gate lanes form tokens 0-15 of the chunk, the up lanes 16-31
+            // the gate warp forms columns 0-15 of the chunk, the up warp 16-31; two buffers, so that one
+            // barrier a chunk is enough
+            float* mine_x = reinterpret_cast<float*>(stg) + xb * 512;
+            float* other_x = reinterpret_cast<float*>(smem + kStages * kStageBytes + (ew ^ 2) * kStgBytes) + xb * 512;
+            xb ^= 1;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mine_x[j * 32 + lane] = up ? v[j] : v[16 + j];
+            pair_barrier(1 + (ew & 1) + 2 * eh);
             float o[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[16 + j], 16);
+              const float got = other_x[j * 32 + lane];
               const float g = up ? got : v[j], u = up ? v[16 + j] : got;
               o[j] = gate<kFast>(g, P.act) * u;
             }
             const int tok0 = c + 16 * up;
             O* out = reinterpret_cast<O*>(q.out);
-            if (sizeof(O) == 2 && q.vec && t.m * 128 + 64 * (int)rank + 16 * q4 + 16 <= q.M) {
+            if (sizeof(O) == 2 && q.vec && (gch & ~31) + 32 <= q.M) {
               if constexpr (sizeof(O) == 2) {
+                // staged where the other warp's values lay, which this warp alone reads
+                __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(other_x);
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) stg16[(16 * up + j) * 16 + (lane & 15)] = __float2bfloat16_rn(o[j]);
+                for (int j = 0; j < 16; ++j) st[j * 32 + lane] = __float2bfloat16_rn(o[j]);
                 __syncwarp();
 #pragma unroll
                 for (int rr = 0; rr < 2; ++rr) {
-                  const int tok = rr * 16 + (lane >> 1);
-                  if (c + tok < t.ntok)
-                    *reinterpret_cast<uint4*>(out + (int64_t)(t.n0 + c + tok) * q.ldo + (gch & ~15) + 8 * (lane & 1)) =
-                        *reinterpret_cast<const uint4*>(stg16 + tok * 16 + 8 * (lane & 1));
+                  const int tok = rr * 8 + (lane >> 2);
+                  if (tok0 + tok < t.ntok)
+                    *reinterpret_cast<uint4*>(out + (int64_t)(t.n0 + tok0 + tok) * q.ldo + (gch & ~31) + 8 * (lane & 3)) =
+                        *reinterpret_cast<const uint4*>(st + tok * 32 + 8 * (lane & 3));
                 }
-                __syncwarp();
               }
             } else if (gch < q.M) {
 #pragma unroll
@@ -641,17 +771,18 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     q.boxes = q.nseg * (f32 ? 6 : 1) * q.kb;
     q.a_mn = s.a[0].mn; q.b_mn = s.b[0].mn;
     q.tiles_m = ceil_div(s.M, j.epi == kGlu ? 128 : 256);
-    // rows of n a tile: as few waves of tiles as possible, and among those the smallest tiles (one problem
-    // alone; 4096 tokens by 2048: 18 tiles of 240 rows, 1.95 waves, instead of 16 of 256, 1.73)
+    // rows of n a tile: the waves of tiles by a tile's time, which is mostly the 256 rows of A (2048 x 5632, us a
+    // stage of two boxes: 1.15 at 256 rows of n, 0.95 at 192, 0.86 at 128)
     q.tn = most;
     if (q.b_mn) {
       if (s.N <= 128) q.tn = 128;
     } else {
       double best = 0;
+      const int unit = j.epi == kStore ? 16 : 32;  // g and u are saved by whole 32 tokens
       for (int nt = ceil_div(s.N, most), e = nt + 4; nt <= e; ++nt) {
-        const int tn = std::max(16, (ceil_div(s.N, nt) + 15) / 16 * 16);
+        const int tn = std::max(unit, (ceil_div(s.N, nt) + unit - 1) / unit * unit);
         const int64_t tiles = (int64_t)q.tiles_m * ceil_div(s.N, tn);
-        const double cost = (j.nprob == 1 ? (double)ceil_div(tiles, pairs) : (double)tiles / pairs) * (tn + 16);
+        const double cost = (j.nprob == 1 ? (double)ceil_div(tiles, pairs) : (double)tiles / pairs) * (tn + 280);
         if (best == 0 || cost < best * 0.99) {
           best = cost;
           q.tn = tn;
@@ -721,7 +852,7 @@ int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t strea
       auto rows = [&](const Operand& o, int r) { return f32 ? planes * o.plane : (int64_t)(o.mn ? s.K : r); };
       if (has_a)
         if (int rc = tc::make_map(&P.a[i][g], a.p, rows(a, s.M), a.mn ? s.M : s.K, a.ld, es,
-                                  a.mn ? 64 : j.epi == kGlu ? 16 : 128))
+                                  a.mn || j.epi == kGlu ? 64 : 128))
           return rc;
       if (has_b)
         if (int rc = tc::make_map(&P.b[i][g], b.p, rows(b, s.N), b.mn ? s.N : s.K, b.ld, es, b.mn ? 64 : q.tn / 2))
@@ -729,7 +860,7 @@ int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t strea
     }
   }
   P.act = j.act;
-  P.save_g = j.save_g; P.save_u = j.save_u; P.out2 = j.out2;
+  P.save_g = j.save_g; P.save_u = j.save_u; P.save_e = j.save_e; P.out2 = j.out2;
   P.row_scale = j.row_scale; P.col_scale[0] = j.col_scale[0]; P.col_scale[1] = j.col_scale[1]; P.bias = j.bias;
   P.counters = reinterpret_cast<uint32_t*>(ws);
   P.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + (counters * 4 + 255) / 256 * 256);

@@ -93,11 +93,14 @@ def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
         return y, (None, None)
     ld_h = (inter + 7) // 8 * 8
     h = torch.empty((rows, ld_h), dtype=dtype, device=dev)
-    # g and u in fp32: the backward pass then rounds nothing but its products' operands
-    gu = torch.empty((2, rows, ld_h), dtype=torch.float32, device=dev) if save else None
-    g = gu.data_ptr() if save else None
-    u = g + 4 * rows * ld_h if save else None
-    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, h.data_ptr(), rows, d,
+    gu, g, u, e = None, None, None, None
+    if save:
+        size = 2 if dtype == torch.bfloat16 else 4
+        step = rows * ld_h * size
+        gu = torch.empty(2 * step + (0 if size == 4 else (rows + 31) // 32 * 2 * ld_h), dtype=torch.uint8, device=dev)
+        g = gu.data_ptr()
+        u, e = g + step, (g + 2 * step if size == 2 else None)
+    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h.data_ptr(), rows, d,
                        inter, _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
     with torch.cuda.device(dev):
         ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
@@ -137,7 +140,9 @@ class _GatedFFN(torch.autograd.Function):
             ld_h = h.shape[1]
             grads = torch.empty((2, rows, ld_h), dtype=dtype, device=dev)
             a.x, a.w_gate, a.w_up, a.w_down, a.dy = (t.data_ptr() for t in (x, wg, wu, wd, dy))
-            a.h, a.g, a.u = h.data_ptr(), gu.data_ptr(), gu.data_ptr() + 4 * rows * ld_h
+            step = rows * ld_h * (2 if dtype == torch.bfloat16 else 4)
+            a.h, a.g, a.u = h.data_ptr(), gu.data_ptr(), gu.data_ptr() + step
+            a.gu_exp = gu.data_ptr() + 2 * step
             a.dg, a.du = grads.data_ptr(), grads.data_ptr() + rows * ld_h * grads.element_size()
             a.ld_x, a.ld_gate, a.ld_up, a.ld_down, a.ld_dy, a.ld_h = ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h
             a.err = _err(dev)
@@ -155,8 +160,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     x [..., d] bf16 or fp32 (rows may lie in a wider buffer), w_gate and w_up [inter, d], w_down
     [d, inter] of x's type, as Linear layers hold them.  act: "silu", "gelu" (tanh form) or "relu".
     Products are summed in fp32; the gated intermediate is rounded to x's type, and so are its two
-    gradients in the backward pass.  Under autograd the call keeps the intermediate and, in fp32, the gate
-    and up values, each [rows, inter], for the backward pass; second derivatives are not offered.  Runs on x's
+    gradients in the backward pass.  Under autograd the call keeps the intermediate, the gate and the up
+    values, each [rows, inter] (the latter two to 11 bits for bf16), for the backward pass; second derivatives are not offered.  Runs on x's
     device, on its current stream; check_dense() reports a wait that ran out."""
     code = _act(act)
     if x.dtype not in _DTYPES:

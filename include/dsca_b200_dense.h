@@ -30,7 +30,8 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 
 /*
  * g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T; sums in fp32, h and y rounded to dtype.  g and u
- * are written in fp32 when given (both or neither): the backward pass reads them.  h is a work area [rows, ld_h] that the backward pass reads as well.
+ * are written when given (both or neither), for the backward pass: in fp32 for DSCA_F32; for DSCA_BF16 as
+ * fp16 times a power of two for each channel of 32 tokens, whose exponents gu_exp takes.  h is a work area [rows, ld_h] that the backward pass reads as well.
  */
 typedef struct {
   const void* x;        /* [rows, d], dtype */
@@ -38,8 +39,9 @@ typedef struct {
   const void* w_up;     /* [inter, d] */
   const void* w_down;   /* [d, inter] */
   void* y;              /* [rows, d] */
-  float* g;             /* [rows, ld_h] or NULL */
-  float* u;
+  void* g;              /* [rows, ld_h] fp32 or fp16, or NULL */
+  void* u;
+  uint8_t* gu_exp;      /* [2, ceil(rows / 32), ld_h]; with DSCA_BF16 and g */
   void* h;              /* [rows, ld_h] */
   int rows, d, inter;
   int dtype;            /* DSCA_BF16, DSCA_F32 */
@@ -63,8 +65,9 @@ typedef struct {
   const void* w_up;
   const void* w_down;
   const void* dy;       /* [rows, d] */
-  const float* g;       /* as dsca_gated_ffn wrote them */
-  const float* u;
+  const void* g;        /* as dsca_gated_ffn wrote them */
+  const void* u;
+  const uint8_t* gu_exp;
   const void* h;
   void* dx;             /* [rows, d] contiguous, or NULL */
   void* d_gate;         /* [inter, d] contiguous, or NULL */

@@ -76,10 +76,10 @@ def _args(name):
 _COMMON = [dict(rows=-1), dict(dtype=2), dict(dtype=-1)]
 _BAD = {
     "dsca_gated_ffn": _COMMON + [dict(x=None), dict(w_gate=None), dict(w_up=None), dict(w_down=None), dict(y=None),
-                                 dict(h=None), dict(g=None), dict(u=None), dict(h=4104), dict(x=4097), dict(d=0), dict(inter=0),
+                                 dict(h=None), dict(g=None), dict(u=None), dict(gu_exp=None), dict(h=4104), dict(x=4097), dict(d=0), dict(inter=0),
                                  dict(act=3), dict(ld_x=63), dict(ld_gate=63), dict(ld_up=0), dict(ld_down=95), dict(ld_y=1),
                                  dict(ld_h=95), dict(ld_h=97), dict(d=1 << 21), dict(ld_x=1 << 41)],
-    "dsca_gated_ffn_backward": _COMMON + [dict(x=None), dict(dy=None), dict(g=None), dict(u=None), dict(h=None), dict(dg=None),
+    "dsca_gated_ffn_backward": _COMMON + [dict(x=None), dict(dy=None), dict(g=None), dict(u=None), dict(gu_exp=None), dict(h=None), dict(dg=None),
                                           dict(du=None), dict(dx=4097), dict(d_gate=4097), dict(d=0), dict(inter=-2), dict(act=-1),
                                           dict(ld_dy=63), dict(ld_down=95), dict(ld_h=100)],
     "dsca_quantize_rows": _COMMON + [dict(x=None), dict(q=None), dict(scale=None), dict(q=4104), dict(scale=4098), dict(k=0),
