@@ -111,16 +111,18 @@ int check(const dsca_gated_ffn_int8_args* a) {
 struct Call {
   bool dry;
   uint8_t* base;
+  size_t bytes;
   cudaStream_t stream;
   int32_t* err;
   size_t used = 0;
   RelayList relays = {};
 
-  void* take(size_t bytes) {
+  void* take(size_t n) {
     const size_t at = used;
-    used += (bytes + 255) / 256 * 256;
+    used += (n + 255) / 256 * 256;
     return dry ? nullptr : base + at;
   }
+  bool fits() const { return dry || used <= bytes; }
   // A matrix as an operand: as it lies where TMA can load it, otherwise laid out anew (by relay()).
   Operand operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype, int mn) {
     if (dtype == DSCA_BF16 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0) return {p, ld, mn, 0};
@@ -130,22 +132,37 @@ struct Call {
     relays.item[relays.n++] = {p, dst, rows, rows_p, cols, ld, ldd, dtype, 0, 0};
     return {dst, ldd, mn, rows_p};
   }
-  // The launch that lays out what operand() collected; false in *none when there was something.
+  // The launch that lays out what operand() collected; *none when there was nothing.
   int relay(bool* none) {
     *none = relays.n == 0;
     const int rc = dry || relays.n == 0 ? DSCA_OK : launch_relay(relays, stream);
     relays.n = 0;
     return rc;
   }
-  // A job's own workspace (partial tiles), its counters zeroed: before the first launch, so that nothing lies
-  // between products that follow one another.
-  int reserve(const Job& j, void** ws) {
-    const size_t bytes = tc_workspace(j), zero = tc_zero_bytes(j);
-    *ws = bytes != 0 ? take(bytes) : nullptr;
-    if (!dry && zero != 0 && cudaMemsetAsync(*ws, 0, zero, stream) != cudaSuccess) return DSCA_ERR_CUDA;
-    return DSCA_OK;
+  // The jobs' own workspaces, counters zeroed: before the products, so that nothing lies between those that follow
+  // one another.
+  struct Own {
+    void *parts = nullptr, *counters = nullptr;
+  };
+  int reserve(const Job* const* jobs, Own* own, int n) {
+    size_t parts[2], counters[2], zero = 0;
+    for (int i = 0; i < n; ++i) {
+      if (int rc = tc_workspace(*jobs[i], &parts[i], &counters[i])) return rc;
+      zero += counters[i];
+    }
+    if (zero == 0) return fits() ? DSCA_OK : DSCA_ERR_CAPACITY;
+    uint8_t* at = reinterpret_cast<uint8_t*>(take(zero));
+    for (int i = 0; i < n; ++i) {
+      if (parts[i] != 0) own[i].parts = take(parts[i]);
+      if (!dry) own[i].counters = at;
+      at += counters[i];
+    }
+    if (!fits()) return DSCA_ERR_CAPACITY;
+    return dry || cudaMemsetAsync(own[0].counters, 0, zero, stream) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
   }
-  int product(const Job& j, void* ws, bool pdl) { return dry ? DSCA_OK : launch_tc(j, ws, err, pdl, stream); }
+  int product(const Job& j, const Own& o, bool pdl) {
+    return dry ? DSCA_OK : launch_tc(j, o.parts, o.counters, err, pdl, stream);
+  }
   int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale) {
     dsca_quantize_rows_args a = {x, rows, k, dtype, ld_x, q, ld_q, scale};
     return dry ? DSCA_OK : launch_quantize_rows(&a, stream);
@@ -170,15 +187,17 @@ int run(Call& c, const dsca_gated_ffn_args* a) {
   j.save_g = a->g; j.save_u = a->u; j.save_e = a->gu_exp;
   k.epi = kStore; k.nprob = 1; k.dtype = dt;
   k.prob[0] = problem(c.operand(a->w_down, d, I, a->ld_down, dt, 0), {}, d, T, I, a->y, a->ld_y);
-  void *wj, *wk;
+  const Job* jobs[] = {&j, &k};
+  Call::Own own[2];
   bool none;
-  TRY(c.reserve(j, &wj));
-  TRY(c.reserve(k, &wk));
+  TRY(c.reserve(jobs, own, 2));
   TRY(c.relay(&none));
-  TRY(c.product(j, wj, false));
-  k.prob[0].b[0] = c.operand(a->h, T, I, a->ld_h, dt, 0);
+  const Operand h = c.operand(a->h, T, I, a->ld_h, dt, 0);
+  if (!c.fits()) return DSCA_ERR_CAPACITY;
+  TRY(c.product(j, own[0], false));
+  k.prob[0].b[0] = h;
   TRY(c.relay(&none));
-  return c.product(k, wk, none);
+  return c.product(k, own[1], none);
 }
 
 int run(Call& c, const dsca_gated_ffn_backward_args* a) {
@@ -186,41 +205,46 @@ int run(Call& c, const dsca_gated_ffn_backward_args* a) {
   const bool weights = a->d_gate != nullptr || a->d_up != nullptr;
   const bool inner = a->dx != nullptr || weights;
   Job j = {}, k = {};
-  void *wj = nullptr, *wk = nullptr;
   bool none;
+  // the first product's operands and those of the second that are there already
   const Operand dy = c.operand(a->dy, T, d, a->ld_dy, dt, 0);
   if (inner) {
     j.epi = kDGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
     j.prob[0] = problem(c.operand(a->w_down, d, I, a->ld_down, dt, 1), dy, I, T, d, a->dg, a->ld_h);
     j.save_g = const_cast<void*>(a->g); j.save_u = const_cast<void*>(a->u); j.out2 = a->du;
     j.save_e = const_cast<uint8_t*>(a->gu_exp);
-    TRY(c.reserve(j, &wj));
-    TRY(c.relay(&none));
-    TRY(c.product(j, wj, false));
   }
   k.epi = kStore; k.dtype = dt;
+  Operand wg = {}, wu = {}, x = {}, h = {};
+  if (a->dx != nullptr) {
+    wg = c.operand(a->w_gate, I, d, a->ld_gate, dt, 1);
+    wu = c.operand(a->w_up, I, d, a->ld_up, dt, 1);
+  }
+  if (weights) x = c.operand(a->x, T, d, a->ld_x, dt, 1);
+  if (a->d_down != nullptr) h = c.operand(a->h, T, I, a->ld_h, dt, 1);
+  if (!c.fits()) return DSCA_ERR_CAPACITY;
+  TRY(c.relay(&none));
+  // ... and those that the first product makes
   Operand dg = {}, du = {};
   if (a->dx != nullptr || a->d_gate != nullptr) dg = c.operand(a->dg, T, I, a->ld_h, dt, 0);
   if (a->dx != nullptr || a->d_up != nullptr) du = c.operand(a->du, T, I, a->ld_h, dt, 0);
   if (a->dx != nullptr) {
     Problem& p = k.prob[k.nprob++];
-    p = problem(c.operand(a->w_gate, I, d, a->ld_gate, dt, 1), dg, d, T, I, a->dx, d);
+    p = problem(wg, dg, d, T, I, a->dx, d);
     p.nseg = 2;
-    p.a[1] = c.operand(a->w_up, I, d, a->ld_up, dt, 1);
+    p.a[1] = wu;
     p.b[1] = du;
   }
-  if (weights) {
-    const Operand x = c.operand(a->x, T, d, a->ld_x, dt, 1);
-    if (a->d_gate != nullptr) k.prob[k.nprob++] = problem(x, as(dg, 1), d, I, T, a->d_gate, d);
-    if (a->d_up != nullptr) k.prob[k.nprob++] = problem(x, as(du, 1), d, I, T, a->d_up, d);
-  }
-  if (a->d_down != nullptr)
-    k.prob[k.nprob++] = problem(c.operand(a->h, T, I, a->ld_h, dt, 1), as(dy, 1), I, d, T, a->d_down, I);
+  if (a->d_gate != nullptr) k.prob[k.nprob++] = problem(x, as(dg, 1), d, I, T, a->d_gate, d);
+  if (a->d_up != nullptr) k.prob[k.nprob++] = problem(x, as(du, 1), d, I, T, a->d_up, d);
+  if (a->d_down != nullptr) k.prob[k.nprob++] = problem(h, as(dy, 1), I, d, T, a->d_down, I);
   if (k.nprob == 0) return DSCA_OK;
-  TRY(c.reserve(k, &wk));
+  const Job* jobs[] = {&k, &j};
+  Call::Own own[2];
+  TRY(c.reserve(jobs, own, inner ? 2 : 1));
+  if (inner) TRY(c.product(j, own[1], false));
   TRY(c.relay(&none));
-  // a memset of counters lies between the two as well where one of the products is split
-  return c.product(k, wk, inner && none && wk == nullptr);
+  return c.product(k, own[0], inner && none);
 }
 
 int run(Call& c, const dsca_int8_linear_args* a) {
@@ -228,10 +252,11 @@ int run(Call& c, const dsca_int8_linear_args* a) {
   j.epi = kStore; j.nprob = 1; j.dtype = a->dtype; j.i8 = 1;
   j.prob[0] = problem({a->w, a->ld_w, 0, 0}, {a->q, a->ld_q, 0, 0}, a->n, a->rows, a->k, a->y, a->ld_y);
   j.row_scale = a->scale; j.col_scale[0] = a->w_scale; j.bias = a->bias;
-  void* wj;
-  TRY(c.reserve(j, &wj));
+  const Job* jobs[] = {&j};
+  Call::Own own[1];
+  TRY(c.reserve(jobs, own, 1));
   if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale));
-  return c.product(j, wj, a->x != nullptr);
+  return c.product(j, own[0], a->x != nullptr);
 }
 
 int run(Call& c, const dsca_gated_ffn_int8_args* a) {
@@ -243,31 +268,28 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   k.epi = kStore; k.nprob = 1; k.dtype = a->dtype; k.i8 = 1;
   k.prob[0] = problem({a->w_down, a->ld_down, 0, 0}, {a->hq, a->ld_hq, 0, 0}, a->d, a->rows, a->inter, a->y, a->ld_y);
   k.row_scale = a->h_scale; k.col_scale[0] = a->down_scale;
-  void *wj, *wk;
-  TRY(c.reserve(j, &wj));
-  TRY(c.reserve(k, &wk));
+  const Job* jobs[] = {&j, &k};
+  Call::Own own[2];
+  TRY(c.reserve(jobs, own, 2));
   TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale));
-  TRY(c.product(j, wj, true));
+  TRY(c.product(j, own[0], true));
   TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale));
-  return c.product(k, wk, true);
+  return c.product(k, own[1], true);
 }
 
 #undef TRY
 
 template <typename Args>
 int call(const Args* a, cudaStream_t stream) {
-  Call size = {true, nullptr, nullptr, nullptr};
-  if (int rc = run(size, a)) return rc;
-  if (size.used > a->workspace_bytes) return DSCA_ERR_CAPACITY;
-  if (size.used != 0 && !at(a->workspace, 256)) return DSCA_ERR_BAD_ARG;
-  Call c = {false, reinterpret_cast<uint8_t*>(a->workspace), stream, a->err};
+  if (a->workspace_bytes != 0 && !at(a->workspace, 256)) return DSCA_ERR_BAD_ARG;
+  Call c = {false, reinterpret_cast<uint8_t*>(a->workspace), a->workspace_bytes, stream, a->err};
   return run(c, a);
 }
 
 template <typename Args>
 size_t workspace(const Args* a) {
   if (check(a) != DSCA_OK || a->rows == 0) return 0;
-  Call size = {true, nullptr, nullptr, nullptr};
+  Call size = {true, nullptr, 0, nullptr, nullptr};
   return run(size, a) == DSCA_OK ? size.used : 0;
 }
 

@@ -75,9 +75,7 @@ __device__ __forceinline__ void gate_grad(float g, int act, float* a, float* da)
   if (act == DSCA_GATE_SILU) {
     const float s = div_<kFast>(1.0f, 1.0f + expf_<kFast>(-g));
     *a = g * s;
-    // the second term is 0 where 1 - s is, also for an infinite g
-    *da = s + (s < 1.0f && s > 0.0f ? g * s * (1.0f - s) : 0.0f);
-    if (g != g) *da = g;
+    *da = s + *a * (1.0f - s);
   } else if (act == DSCA_GATE_RELU) {
     *a = g <= 0.0f ? 0.0f : g;
     *da = g <= 0.0f ? 0.0f : (g != g ? g : 1.0f);
@@ -105,10 +103,10 @@ struct RelayList {
 };
 int launch_relay(RelayList& list, cudaStream_t stream);
 
-// Tensor-core products (dense_tc.cu).  ws: tc_workspace() bytes, of which the first tc_zero_bytes() are zero.
-size_t tc_workspace(const Job& j);
-size_t tc_zero_bytes(const Job& j);
-int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t stream);
+// Tensor-core products (dense_tc.cu), with tc_workspace()'s bytes of partial tiles and of counters, which are zero
+// at the launch.
+int tc_workspace(const Job& j, size_t* parts, size_t* counters);
+int launch_tc(const Job& j, void* parts, void* counters, int32_t* err, bool pdl, cudaStream_t stream);
 int launch_quantize_rows(const dsca_quantize_rows_args* a, cudaStream_t stream);
 
 }  // namespace dense

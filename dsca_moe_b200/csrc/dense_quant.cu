@@ -2,9 +2,10 @@
 // nearest integer, ties to even, exactly.
 //
 // Why the exact quotient and not x / scale: the scale is rounded, so values half way between two
-// codes (x = max|x| / 2 is 63.5) would fall to either side by the row.  127 x is exact in fp32 for a
-// bf16 x and IEEE division rounds the exact quotient, which is never within 2^-9 of a tie without
-// being one; for an fp32 x the quotient is taken again in 64 bits where it lies close to a tie.
+// codes (x = max|x| / 2 is 63.5) would fall to either side by the row.  A product with 127 / max|x| finds the code of
+// all values but those close to a tie, which take the quotient: 127 x is exact in fp32 for a bf16 x and IEEE
+// division rounds the exact quotient, which is never within 2^-9 of a tie without being one; for an fp32 x it is
+// taken in 64 bits.
 //
 // Bound by DRAM from a few thousand rows on: a row is read once into registers (up to 8192 values;
 // longer rows are read a second time from L2).
@@ -28,19 +29,27 @@ __device__ __forceinline__ float value(const T* p, int64_t i) {
   else return p[i];
 }
 
-// the code of x in a row whose largest magnitude is amax (> 0)
+// The exact code of x in a row whose largest magnitude is amax (> 0).
 template <typename T>
-__device__ __forceinline__ int code(float x, float amax) {
-  const float q = __fdiv_rn(__fmul_rn(127.0f, x), amax);
-  float r = rintf(q);
-  if constexpr (sizeof(T) == 4) {
-    // 127 x overflows or loses bits at the ends of fp32's range: 64 bits there and near a tie
-    if (fabsf(fabsf(q - r) - 0.5f) < 1e-4f || amax > 1e36f || amax < 1e-30f)
-      r = (float)rint(127.0 * (double)x / (double)amax);
-  } else if (amax > 1e36f || amax < 1e-30f) {
-    r = (float)rint(127.0 * (double)x / (double)amax);
+__device__ __noinline__ float exact_code(float x, float amax) {
+  if (sizeof(T) == 2 && amax < 1e36f && amax > 1e-30f) return rintf(__fdiv_rn(__fmul_rn(127.0f, x), amax));
+  return (float)rint(127.0 * (double)x / (double)amax);
+}
+
+// Four codes in a word.  inv is 127 / amax to 2^-23: a product with it is off by less than 2^-16, so only values
+// that close to a tie need the exact quotient.  Adding 1.5 * 2^23 rounds to an integer, whose low byte is the code.
+template <typename T>
+__device__ __forceinline__ uint32_t codes4(const float* x, float amax, float inv) {
+  constexpr float kRound = 12582912.0f;
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = x[i] * inv;
+    float r = v + kRound;
+    if (fabsf(v - (r - kRound)) > 0.49996f) r = exact_code<T>(x[i], amax) + kRound;
+    b[i] = __float_as_uint(r);
   }
-  return (int)r;
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
 // TPR threads a row, CH chunks of eight values a thread in registers (CH = 0: longer rows).
@@ -107,14 +116,26 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
   }
   if (!live) return;
   if (tid == 0) a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
-  const bool usable = m > 0.0f && m < INFINITY;  // codes mean nothing otherwise: zeros
-  auto store = [&](int c, const float (&o)[8]) {
-    uint32_t w[2] = {0u, 0u};
+  // codes mean nothing in a row that is not finite: zeros
+  const bool usable = m > 0.0f && m < INFINITY;
+  const bool ends = m < 1e-30f || m > 1e36f;  // 127 / m or 127 x leaves fp32's normal numbers
+  const float inv = usable && !ends ? __fdiv_rn(127.0f, m) : 0.0f;
+  auto store = [&](int c, float (&o)[8]) {
+    uint2 w = make_uint2(0u, 0u);
     if (usable) {
+      if (ends) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e / 4] |= (uint32_t)(code<T>(o[e], m) & 255) << (8 * (e % 4));
+        for (int e = 0; e < 8; ++e) {
+          const float r = exact_code<T>(o[e], m);
+          const uint32_t byte = (uint32_t)((int)r & 255) << (8 * (e % 4));
+          if (e < 4) w.x |= byte;
+          else w.y |= byte;
+        }
+      } else {
+        w = make_uint2(codes4<T>(o, m, inv), codes4<T>(o + 4, m, inv));
+      }
     }
-    *reinterpret_cast<uint2*>(a.q + row * a.ld_q + c * 8) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(a.q + row * a.ld_q + c * 8) = w;
   };
   if constexpr (CH > 0) {
 #pragma unroll
@@ -150,6 +171,7 @@ int run(const dsca_quantize_rows_args& a, cudaStream_t stream) {
   }
   if (chunks <= 256) return launch<T, 256, 1>(a, stream);
   if (chunks <= 512) return launch<T, 256, 2>(a, stream);
+  if (chunks <= 768) return launch<T, 256, 3>(a, stream);
   if (chunks <= 1024) return launch<T, 256, 4>(a, stream);
   return launch<T, 256, 0>(a, stream);
 }

@@ -1,25 +1,27 @@
 // The products of dense.cuh on the tensor cores: CTA pairs, tcgen05 cta_group::2, TMA-fed.
 //
-// A tile is 256 m x up to 256 n: each CTA of a pair loads its 128 rows of A and half of the tile's rows of
-// B, so an SM streams 32 KB for every 64-wide slice of k in 16 bits (128-wide in 8), and the even CTA issues
-// the MMAs (M256 N<=256) into both CTAs' tensor memory.  TMEM lane = m, the output's contiguous index, column
-// = n: a token tile of 20 rows costs 32 columns, not 256.
+// A tile is 256 rows of one operand (the MMA's A, 128 a CTA) by up to 256 of the other (its B, half a CTA), so an
+// SM streams 32 KB for every 64-wide slice of k in 16 bits (128-wide in 8); the even CTA issues the MMAs into both
+// CTAs' tensor memory.  Two orientations:
+//   rows      A is the operand of the output's rows (tokens; rows of a weight's gradient): TMEM lane = row,
+//             columns = consecutive values of that row, which a thread stores as they lie.
+//   columns   A is the weight, B the tokens: a tile of 20 tokens costs 32 columns, not 256 rows; the epilogue turns
+//             32 x 32 blocks in shared memory.  For up to 128 rows of output.
 //   warp 0      TMA producer (one thread), 128-byte swizzle, three stages of two 128-byte k boxes
 //   warp 1      TMEM (512 columns: two accumulators); in the even CTA the MMA issuer
-//   warps 2-9   epilogue: two warps to a lane quarter, alternate chunks of 32 columns
+//   warps 2-9   epilogue: two warps to a lane quarter, alternate chunks of 32 TMEM columns
 // Operands: a K-major one is loaded as boxes of 128 bytes of k by its rows; an MN-major one as boxes of 64
 // rows of k by 64 values of m or n, which the MMA reads transposed, so that the gradients' products take
 // weights and activations as they lie.
 //
-// Gated products (kGlu): a CTA's 128 rows of A are 64 gate rows and the up rows of the same channels, so the
-// epilogue warps of lane quarters q and q + 2 hold the gate and up values of the same 32 channels.  For each
-// chunk of 32 columns the gate warp forms the products of the first 16 and the up warp those of the last,
-// after handing each other the other half through shared memory.  (Alternating boxes of 16 gate and 16 up
-// rows would bring both into one warp, but eight small boxes instead of two cost more than the exchange:
-// 4096 x 2048 x 5632 188 us against 152.)
-// Saved for the backward pass in 16 bits: g and u as fp16 with one power of two for a channel's 32 tokens
-// (11 bits of significand for every value within 2^29 of the largest), half of fp32's bytes, which the
-// backward pass reads against the clock of its first product.
+// Gated products (kGlu).  Rows: the even CTA loads the gate rows of B and the odd one the up rows of the same
+// channels, so that each thread finds a token's gate and up values in its own lane, half a tile apart.  Columns: a
+// CTA's 128 rows of A are 64 gate rows and the up rows of the same channels; the warps of lane quarters q and
+// q + 2 hold the two, and for each chunk of 32 tokens the gate warp forms the products of the first 16 and the up
+// warp those of the last, after handing each other the other half through shared memory.
+// Saved for the backward pass in 16 bits: g and u as fp16 with one power of two for a token's 32 channels (11 bits
+// of significand for every value within 2^29 of the largest), half of fp32's bytes, which the backward pass reads
+// against the clock of its first product.
 //
 // 32-bit inputs (kF32): every value is split into three bf16 terms (8 + 8 + 8 bits, dense_split.cu) and the
 // product is six MMA passes over k: hi.hi into one accumulator, hi.mid, mid.hi, hi.lo, mid.mid and lo.hi into
@@ -56,15 +58,16 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
 enum In { kBf16 = 0, kI8 = 1, kF32 = 2 };
 
 struct Prob {
-  int M, N, K;
+  int rows, cols, K;     // of the output [rows, cols]
+  int row;               // orientation: rows (1) or columns (0)
   int nseg, kb;          // segments; k boxes of each
   int boxes;             // nseg * terms * kb
-  int a_mn, b_mn;
+  int a_mn, b_mn;        // majors of the MMA's A and B
   int tiles_m, tiles_n, tn;
   int splits, per;       // k splits and boxes of each (even)
   int first;             // the problem's first unit of work
   int a_plane, b_plane;  // kF32: rows between the planes of three terms
-  int vec;               // out rows start on 16-byte boundaries
+  int vec;               // output rows start on 16-byte (1) or 32-byte (2) boundaries
   int64_t part;          // splits > 1: offset of the partial tiles in floats
   int counter;           // ... and of the arrival counters
   void* out;
@@ -77,11 +80,12 @@ struct Params {
   int nprob, total, act;
   void* save_g;   // fp16 codes (16-bit inputs) or fp32
   void* save_u;
-  uint8_t* save_e;  // fp16: the exponents, [2][ceil(N / 32)][ldo]
+  uint8_t* save_e;  // fp16: the exponents, [2][rows][ceil(cols / 32)]
   void* out2;
   const float* row_scale;
   const float* col_scale[2];
   const void* bias;
+  int vec_cols;  // col_scale on 16-byte boundaries
   float* parts;
   uint32_t* counters;
   int32_t* err;
@@ -95,11 +99,11 @@ struct Ctl {
 };
 
 struct Tile {
-  int p, m, n0, ntok, box0, box1, split;
-  int64_t tile;  // within the problem
+  int p, m0, n0, nval, box0, box1, split;  // first row of A, of B and how many of B (kGlu rows: of channels)
+  int64_t tile;                            // within the problem
 };
 
-__device__ __forceinline__ Tile decode(const Params& P, int unit) {
+__device__ __forceinline__ Tile decode(const Params& P, int unit, int am, int bn) {
   Tile t;
   t.p = 0;
   while (t.p + 1 < P.nprob && unit >= P.prob[t.p + 1].first) ++t.p;
@@ -111,17 +115,20 @@ __device__ __forceinline__ Tile decode(const Params& P, int unit) {
   // groups of eight m tiles, n by n inside: the pairs that run at one time share both operands' rows in L2
   const int g = l / (8 * q.tiles_n), r = l - g * 8 * q.tiles_n;
   const int gm = min(8, q.tiles_m - 8 * g);
-  t.m = 8 * g + r % gm;
-  t.n0 = (r / gm) * q.tn;
-  t.ntok = min(q.tn, q.N - t.n0);
+  t.m0 = (8 * g + r % gm) * (q.row ? 256 : am);
+  const int step = q.row ? q.tn / bn : q.tn;
+  t.n0 = (r / gm) * step;
+  t.nval = min(step, (q.row ? q.cols : q.rows) - t.n0);
   t.box0 = t.split * q.per;
   t.box1 = min(q.boxes, t.box0 + q.per);
   return t;
 }
 
-// MMA N of a tile with ntok rows of B: each CTA holds half, whole 8-row groups (64 rows if MN-major)
-__device__ __forceinline__ int mma_n(const Prob& q, int ntok) {
-  return q.b_mn ? (ntok + 127) & ~127 : max(16, (ntok + 15) & ~15);
+// MMA N of a tile: each CTA holds half of B's rows, whole 8-row groups (64 rows if MN-major); the rows form of a
+// gated product always takes the whole tile
+__device__ __forceinline__ int mma_n(const Prob& q, const Tile& t, bool glu) {
+  if (glu && q.row) return q.tn;
+  return q.b_mn ? (t.nval + 127) & ~127 : max(16, (t.nval + 15) & ~15);
 }
 
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
@@ -180,60 +187,161 @@ __device__ __forceinline__ int plane_b(int t) { return t == 1 || t == 4 ? 1 : t 
 // The two warps (64 threads) that exchange gate and up values.
 __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
-// 32 tokens of one channel as fp16 times a power of two that brings the largest finite one to [2^14, 2^15); the
-// exponent byte is the largest's, at least 14 so that the factor is a normal number.
-__device__ __forceinline__ void save_f16(const Params& P, const Prob& q, int up, int ch, int n, int ntok, const float (&v)[32]) {
-  float m = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float a = fabsf(v[j]);
-    if (j < ntok && a <= 3.4028234663852886e38f) m = fmaxf(m, a);
-  }
-  const uint32_t e = max(14u, __float_as_uint(m) >> 23);
-  const float s = __uint_as_float((268u - e) << 23);  // 2^(141 - e)
-  if (ch >= q.M) return;
-  __half* at = reinterpret_cast<__half*>(up ? P.save_u : P.save_g) + (int64_t)n * q.ldo + ch;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j < ntok) at[j * q.ldo] = __float2half_rn(v[j] * s);
-  P.save_e[((int64_t)up * ((q.N + 31) / 32) + n / 32) * q.ldo + ch] = (uint8_t)e;
+// ---- g and u in 16 bits: fp16 times a power of two that brings the largest finite one of a token's 32 channels
+// to [2^14, 2^15).  The exponent byte is the largest's, at least 14 so that the factor is a normal number.
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= 3.4028234663852886e38f ? a : 0.0f;
+}
+__device__ __forceinline__ uint32_t f16_exp(float largest) { return max(14u, __float_as_uint(largest) >> 23); }
+__device__ __forceinline__ float f16_factor(uint32_t e) { return __uint_as_float((268u - e) << 23); }  // 2^(141 - e)
+__device__ __forceinline__ float f16_back(uint32_t e) {                                               // 2^(e - 141)
+  return e > 14u ? __uint_as_float((e - 14u) << 23) : 5.877471754111438e-39f;
 }
 
-// g and u of the chunk after the one in work (kDGlu, 16 bits): 32 tokens x 32 channels each, 16 bytes a load.
+// h = act(g) u, in place of g; dg = dh u act'(g) and du = dh act(g), in place of g and u.  One loop for each gate, so
+// that the choice is made once.
+template <bool kFast, int N>
+__device__ __forceinline__ void gate_all(float (&g)[N], const float (&u)[N], int act) {
+  if (act == DSCA_GATE_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = gate<kFast>(g[j], DSCA_GATE_SILU) * u[j];
+  } else if (act == DSCA_GATE_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = gate<kFast>(g[j], DSCA_GATE_RELU) * u[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = gate<kFast>(g[j], DSCA_GATE_GELU) * u[j];
+  }
+}
+template <bool kFast, int ACT, int N>
+__device__ __forceinline__ void gate_grad_loop(const float (&dh)[N], float (&g)[N], float (&u)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float a, da;
+    gate_grad<kFast>(g[j], ACT, &a, &da);
+    g[j] = dh[j] * u[j] * da;
+    u[j] = dh[j] * a;
+  }
+}
+template <bool kFast, int N>
+__device__ __forceinline__ void gate_grad_all(const float (&dh)[N], float (&g)[N], float (&u)[N], int act) {
+  if (act == DSCA_GATE_SILU) gate_grad_loop<kFast, DSCA_GATE_SILU>(dh, g, u);
+  else if (act == DSCA_GATE_RELU) gate_grad_loop<kFast, DSCA_GATE_RELU>(dh, g, u);
+  else gate_grad_loop<kFast, DSCA_GATE_GELU>(dh, g, u);
+}
+
+// ---- rows form: 32 consecutive values of one output row from column n on.  vec: rows start on 16-byte (1) or
+// 32-byte (2) boundaries; a whole 32-byte sector a store where they do, half a sector costs L2 twice the writes.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+template <typename O>
+__device__ __forceinline__ void store_row(O* row, int n, int cols, int vec, const float (&v)[32]) {
+  constexpr int PER = 32 / sizeof(O);  // values of 32 bytes
+#pragma unroll
+  for (int i = 0; i < 32 / PER; ++i) {
+    const int at = n + i * PER;
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (sizeof(O) == 2) w[k] = pack_bf16x2(v[i * PER + 2 * k], v[i * PER + 2 * k + 1]);
+      else w[k] = __float_as_uint(v[i * PER + k]);
+    }
+    if (vec == 2 && at + PER <= cols) {
+      store32(row + at, w);
+    } else if (vec && at + PER <= cols) {
+      *reinterpret_cast<uint4*>(row + at) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + at + PER / 2) = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (at + k < cols) {
+          if constexpr (sizeof(O) == 2) row[at + k] = __float2bfloat16_rn(v[i * PER + k]);
+          else row[at + k] = v[i * PER + k];
+        }
+    }
+  }
+}
+// 32 floats from column n on (zeros past cols); the same for every lane or a row of its own
+__device__ __forceinline__ void load_row(const float* row, int n, int cols, bool vec, float (&v)[32]) {
+  if (vec && n + 32 <= cols) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(row + n + 4 * i));
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = n + j < cols ? __ldg(row + n + j) : 0.0f;
+}
+// Saved rows start on 16-byte boundaries and hold a multiple of eight values (ld_h), so pieces of eight are whole.
+__device__ __forceinline__ void save_row_f16(const Params& P, const Prob& q, int up, int64_t row, int n, const float (&v)[32]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) m = fmaxf(m, finite_abs(v[j]));
+  const uint32_t e = f16_exp(m);
+  const float s = f16_factor(e);
+  __half* at = reinterpret_cast<__half*>(up ? P.save_u : P.save_g) + row * q.ldo + n;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const __half2 h2 = __floats2half2_rn(v[16 * i + 2 * k] * s, v[16 * i + 2 * k + 1] * s);
+      w[k] = *reinterpret_cast<const uint32_t*>(&h2);
+    }
+    if (q.vec == 2 && n + 16 * i + 16 <= q.cols) {
+      store32(at + 16 * i, w);
+    } else {
+      if (n + 16 * i < q.cols) *reinterpret_cast<uint4*>(at + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (n + 16 * i + 8 < q.cols) *reinterpret_cast<uint4*>(at + 16 * i + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  P.save_e[((int64_t)up * q.rows + row) * ((q.cols + 31) / 32) + n / 32] = (uint8_t)e;
+}
+// g and u of a chunk, loaded while the one before it is in work
 struct Ahead {
   uint4 v[8];
   uint32_t e[2];
-  __device__ __forceinline__ void load(const Params& P, const Prob& q, const Tile& t, uint32_t rank, int q4, int lane, int c) {
-    const int m0 = t.m * 256 + 128 * (int)rank + 32 * q4, ch = m0 + 8 * (lane & 3);
+  __device__ __forceinline__ void load(const Params& P, const Prob& q, int64_t row, int n, int nend) {
+    const bool live = row < q.rows && n < nend;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int tok = c + (i & 3) * 8 + (lane >> 2);
       const __half* p = reinterpret_cast<const __half*>(i < 4 ? P.save_g : P.save_u);
-      v[i] = ch < q.M && tok < t.ntok ? __ldg(reinterpret_cast<const uint4*>(p + (int64_t)(t.n0 + tok) * q.ldo + ch))
-                                      : make_uint4(0u, 0u, 0u, 0u);
+      const int c = n + 8 * (i & 3);
+      v[i] = live && c < q.cols ? __ldg(reinterpret_cast<const uint4*>(p + row * q.ldo + c)) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      e[i] = m0 + lane < q.M && c < t.ntok
-                 ? P.save_e[((int64_t)i * ((q.N + 31) / 32) + (t.n0 + c) / 32) * q.ldo + m0 + lane] : 141u;
+      e[i] = live ? P.save_e[((int64_t)i * q.rows + row) * ((q.cols + 31) / 32) + n / 32] : 141u;
   }
-  __device__ __forceinline__ void store(uint8_t* stg, int lane) const {
+  __device__ __forceinline__ void get(int i, float (&o)[32]) const {
+    const float s = f16_back(e[i]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      *reinterpret_cast<uint4*>(stg + (i >> 2) * 2048 + ((i & 3) * 8 + (lane >> 2)) * 64 + 16 * (lane & 3)) = v[i];
-  }
-  __device__ __forceinline__ float scale(int i) const {  // 2^(e - 141)
-    const int x = (int)e[i] - 14;  // its biased exponent; 0 and 1 from e = 14, 15 on
-    return x > 0 ? __uint_as_float((uint32_t)x << 23) : 5.877471754111438e-39f;
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w[4] = {v[4 * i + k].x, v[4 * i + k].y, v[4 * i + k].z, v[4 * i + k].w};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[h]));
+        o[8 * k + 2 * h] = f.x * s;
+        o[8 * k + 2 * h + 1] = f.y * s;
+      }
+    }
   }
 };
 
 template <int EPI, int IN, typename O>
 __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params P) {
   constexpr bool kGluE = EPI == kGlu;
+  constexpr int kAM = kGluE ? 128 : 256;     // channels or columns of a tile in the columns form
+  constexpr int kBN = kGluE ? 2 : 1;         // rows of B to a channel in the rows form
   constexpr int KE = IN == kI8 ? 128 : 64;   // k elements of a box
   constexpr int KS = IN == kI8 ? 32 : 16;    // ... and of one MMA
-  constexpr bool kFast = sizeof(O) == 2 && IN != kI8;
+  constexpr bool kFast = IN != kF32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -282,13 +390,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       for (int i = 0; i < kStages; ++i) pending[i] = -1;
       bool ok = true;
       for (int unit = unit0; ok && unit < P.total; unit += units) {
-        const Tile t = decode(P, unit);
+        const Tile t = decode(P, unit, kAM, kBN);
         const Prob& q = P.prob[t.p];
-        const int half = mma_n(q, t.ntok) / 2;
-        const int b_row = t.n0 + half * (int)rank;
+        const bool glu_rows = kGluE && q.row;
+        const int b_row = glu_rows ? t.n0 : t.n0 + mma_n(q, t, kGluE) / 2 * (int)rank;
+        const int a_row = kGluE && !q.row ? t.m0 + 64 * (int)rank : t.m0 + 128 * (int)rank;
         const uint32_t b_bytes = (uint32_t)(q.tn / 2) * 128u;  // a whole box lands; rows past the tile are not used
         const int kb = q.kb, a_mn = q.a_mn, b_atoms = q.b_mn ? q.tn / 128 : 0;
-        const CUtensorMap *ma = P.a[t.p], *mb = P.b[t.p];
+        const CUtensorMap *ma = P.a[t.p], *mb = glu_rows ? P.b[t.p] + rank : P.b[t.p];
         BoxAt<IN> at(q, t.box0);
         for (int b = t.box0; b < t.box1; b += kSub) {
           if (!mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, P.err)) { ok = false; break; }
@@ -300,16 +409,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             const uint32_t da = smem_a + s * kStageBytes + h * kBoxBytes, db = smem_b + s * kStageBytes + h * kBoxBytes;
             const int pa = IN == kF32 ? plane_a(at.term) * q.a_plane : 0, pb = IN == kF32 ? plane_b(at.term) * q.b_plane : 0;
             const int kx = at.k * KE;
-            if constexpr (kGluE) {
-              const int r0 = t.m * 128 + 64 * (int)rank + pa;
-              tma_load_2d_pair(da, ma, fb0, kx, r0);
-              tma_load_2d_pair(da + 8192, ma + 1, fb0, kx, r0);
+            if (kGluE && !glu_rows) {
+              tma_load_2d_pair(da, ma, fb0, kx, a_row + pa);
+              tma_load_2d_pair(da + 8192, ma + 1, fb0, kx, a_row + pa);
             } else if (a_mn) {
-              const int r0 = t.m * 256 + 128 * (int)rank;
-              tma_load_2d_pair(da, ma + at.seg, fb0, r0, kx + pa);
-              tma_load_2d_pair(da + 8192, ma + at.seg, fb0, r0 + 64, kx + pa);
+              tma_load_2d_pair(da, ma + at.seg, fb0, a_row, kx + pa);
+              tma_load_2d_pair(da + 8192, ma + at.seg, fb0, a_row + 64, kx + pa);
             } else {
-              tma_load_2d_pair(da, ma + at.seg, fb0, kx, t.m * 256 + 128 * (int)rank + pa);
+              tma_load_2d_pair(da, ma + at.seg, fb0, kx, a_row + pa);
             }
             if (b_atoms) {
               tma_load_2d_pair(db, mb + at.seg, fb0, b_row, kx + pb);
@@ -333,12 +440,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       uint32_t ph = 0;
       bool ok = true;
       for (int unit = unit0; ok && unit < P.total; unit += units, ++it) {
-        const Tile t = decode(P, unit);
+        const Tile t = decode(P, unit, kAM, kBN);
         const Prob& q = P.prob[t.p];
         const int acc = it & 1;
         // D f32 (1) or s32 (2); A, B bf16 (1) or signed 8-bit (1); majors; N; M = 256
         const uint32_t idesc = ((IN == kI8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)q.a_mn << 15) |
-                               ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n(q, t.ntok) >> 3) << 17) | (16u << 24);
+                               ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n(q, t, kGluE) >> 3) << 17) | (16u << 24);
         if (!mbar_wait(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
           ok = false;
           break;
@@ -392,28 +499,30 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     // ---------------- epilogue
     const int q4 = warp & 3, ew = warp - 2, eh = ew >> 2;
     uint8_t* stg = smem + kStages * kStageBytes + ew * kStgBytes;
-    __nv_bfloat16* stg16 = reinterpret_cast<__nv_bfloat16*>(stg);
+    const int pair_id = 1 + (ew & 1) + 2 * eh;  // barrier of an exchange
     int it = 0, xb = 0;
     Ahead ahead;
     for (int unit = unit0; unit < P.total; unit += units, ++it) {
-      const Tile t = decode(P, unit);
+      const Tile t = decode(P, unit, kAM, kBN);
       const Prob& q = P.prob[t.p];
       const int acc = it & 1;
-      if constexpr (EPI == kDGlu && IN == kBf16) ahead.load(P, q, t, rank, q4, lane, 32 * eh);
+      const int64_t lrow = t.m0 + 128 * (int)rank + 32 * q4 + lane;  // rows form: this lane's output row
+      if constexpr (EPI == kDGlu && IN == kBf16)
+        if (q.row) ahead.load(P, q, lrow, t.n0 + 32 * eh, t.n0 + t.nval);
       int w_ok = 1;
       if (lane == 0) w_ok = mbar_wait(smem_u32(&ctl.tmem_full[acc]), (uint32_t)((it >> 1) & 1), abort_flag, P.err) ? 1 : 0;
       w_ok = __shfl_sync(0xffffffffu, w_ok, 0);
       if constexpr (kGluE) {
         // the two warps of an exchange go on or leave together
         if (lane == 0) ctl.pair_ok[ew] = w_ok;
-        pair_barrier(1 + (ew & 1) + 2 * eh);
+        pair_barrier(pair_id);
         w_ok = *reinterpret_cast<volatile int*>(&ctl.pair_ok[ew ^ 2]) & w_ok;
       }
       if (!w_ok) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * 256);
-      const int ncol = mma_n(q, t.ntok);
-      // a chunk of the accumulator: lane's m, 32 columns from c on
+      const int ncol = mma_n(q, t, kGluE);
+      // 32 columns of the accumulator from c on
       auto chunk = [&](int c, uint32_t (&v)[32]) {
         tmem_ld32(taddr + c, v);
         if constexpr (IN == kF32) {
@@ -427,19 +536,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         }
       };
       bool mine = true;
-      float* part = nullptr;
-      int64_t part_step = 0;
+      float* part = nullptr;  // [split][rank][column / 4][lane][4]
+      const int tnp = (q.tn + 31) & ~31;  // whole chunks
+      const int64_t part_step = (int64_t)2 * tnp * 128;
       if (q.splits > 1) {
-        // this warp's part of the tile: [split][column][lane]
-        part_step = (int64_t)2 * q.tn * 128;
-        part = P.parts + q.part + t.tile * q.splits * part_step + (int64_t)rank * q.tn * 128 + q4 * 32 + lane;
+        part = P.parts + q.part + t.tile * q.splits * part_step + (int64_t)rank * tnp * 128 + (q4 * 32 + lane) * 4;
         for (int c = 32 * eh; c < ncol; c += 64) {
           uint32_t v[32];
           chunk(c, v);
           float* at = part + t.split * part_step + (int64_t)c * 128;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < t.ntok) at[(int64_t)j * 128] = __uint_as_float(v[j]);
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(at + j * 512) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
         }
         __threadfence();
         __syncwarp();
@@ -447,12 +555,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         uint32_t* counter = P.counters + q.counter + (t.tile * 2 + rank) * kEpiWarps + ew;
         if constexpr (kGluE) {
           // one count for the two warps of an exchange, which finish a tile together
-          pair_barrier(1 + (ew & 1) + 2 * eh);
+          pair_barrier(pair_id);
           if (!(q4 >> 1) && lane == 0) {
             __threadfence();
             ctl.pair_old[ew] = (int)atomicAdd(counter, 1u);
           }
-          pair_barrier(1 + (ew & 1) + 2 * eh);
+          pair_barrier(pair_id);
           old = (uint32_t)*reinterpret_cast<volatile int*>(&ctl.pair_old[ew | 2]);  // the gate warps are 2, 3, 6, 7
         } else {
           if (lane == 0) old = atomicAdd(counter, 1u);
@@ -461,71 +569,163 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         mine = old == (uint32_t)q.splits - 1u;
         if (mine) __threadfence();
       }
-      if (mine) {
-        const int mrow = t.m * 256 + 128 * (int)rank + 32 * q4 + lane;  // this lane's m (not kGlu)
-        const int gch = t.m * 128 + 64 * (int)rank + 32 * (q4 & 1) + lane;  // kGlu: its channel
-        const int up = q4 >> 1;                                              // ... of gate (0) or up (1)
-        float cs = 1.0f, bias = 0.0f;
-        if constexpr (IN == kI8) {
-          if constexpr (kGluE) cs = gch < q.M ? __ldg((up ? P.col_scale[1] : P.col_scale[0]) + gch) : 0.0f;
-          else cs = mrow < q.M ? __ldg(P.col_scale[0] + mrow) : 0.0f;
+      // the finished product's 32 columns from c on: parts in the order of k (8-bit: int32 sums)
+      auto finished = [&](int c, uint32_t (&r)[32]) {
+        if (q.splits == 1) {
+          chunk(c, r);
+          return;
         }
-        if constexpr (EPI == kStore && IN == kI8) {
-          if (P.bias != nullptr && mrow < q.M) {
-            if constexpr (sizeof(O) == 2) bias = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(P.bias)[mrow]);
-            else bias = reinterpret_cast<const float*>(P.bias)[mrow];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = 0u;
+#pragma unroll 2
+        for (int s = 0; s < q.splits; ++s) {
+          const float* at = part + s * part_step + (int64_t)c * 128;
+          uint4 x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = __ldcg(reinterpret_cast<const uint4*>(at + j * 512));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (IN == kI8) r[4 * j + k] += w[k];
+              else r[4 * j + k] = __float_as_uint(__uint_as_float(r[4 * j + k]) + __uint_as_float(w[k]));
+            }
           }
         }
+      };
+      if (mine && q.row) {
+        // ------------ rows: this lane's row, 32 of its values at a time
+        const bool live = lrow < q.rows;
+        O* out = reinterpret_cast<O*>(q.out) + lrow * q.ldo;
+        float rs = 1.0f;
+        if constexpr (IN == kI8) rs = live ? __ldg(P.row_scale + lrow) : 0.0f;
+        const int span = kGluE ? q.tn / 2 : ncol;  // columns of the tile's output
 #pragma unroll 1
-        for (int c = 32 * eh; c < ncol; c += 64) {
-          if (c >= t.ntok) break;
-          float gv[32], uv[32];
-          if constexpr (EPI == kDGlu && IN == kBf16) {
-            // the chunk's g and u go through shared memory to the lane of their channel; the next chunk's
-            // are on their way meanwhile
-            const float sg = ahead.scale(0), su = ahead.scale(1);
-            ahead.store(stg, lane);
-            __syncwarp();
-            if (c + 64 < ncol) ahead.load(P, q, t, rank, q4, lane, c + 64);
-            const __half* sh = reinterpret_cast<const __half*>(stg);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              gv[j] = __half2float(sh[j * 32 + lane]) * sg;
-              uv[j] = __half2float(sh[1024 + j * 32 + lane]) * su;
-            }
-            __syncwarp();
-          } else if constexpr (EPI == kDGlu) {  // on their way before the accumulator is read
-            const int64_t at = (int64_t)(t.n0 + c) * q.ldo + mrow;
-            const float *pg = reinterpret_cast<const float*>(P.save_g), *pu = reinterpret_cast<const float*>(P.save_u);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const bool in = mrow < q.M && c + j < t.ntok;
-              gv[j] = in ? __ldg(pg + at + j * q.ldo) : 0.0f;
-              uv[j] = in ? __ldg(pu + at + j * q.ldo) : 0.0f;
-            }
-          }
+        for (int c = 32 * eh; c < span; c += 64) {
+          if (c >= t.nval) break;
+          const int n = t.n0 + c;
           float v[32];
           {
             uint32_t r[32];
-            if (q.splits > 1) {
-              // the parts in the order of k (8-bit: int32 sums)
+            finished(c, r);
+            if constexpr (IN == kI8) {
+              float cs[32];
+              load_row(P.col_scale[0], n, q.cols, P.vec_cols, cs);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = 0u;
-              for (int s = 0; s < q.splits; ++s) {
-                const float* at = part + s * part_step + (int64_t)c * 128;
+              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * (cs[j] * rs);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+            }
+          }
+          if constexpr (kGluE) {
+            float u[32];
+            {
+              uint32_t r[32];
+              finished(c + q.tn / 2, r);
+              if constexpr (IN == kI8) {
+                float cs[32];
+                load_row(P.col_scale[1], n, q.cols, P.vec_cols, cs);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) u[j] = (float)(int)r[j] * (cs[j] * rs);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(r[j]);
+              }
+            }
+            if (P.save_g != nullptr && live) {
+              if constexpr (IN == kBf16) {
+                save_row_f16(P, q, 0, lrow, n, v);
+                save_row_f16(P, q, 1, lrow, n, u);
+              } else {
+                store_row(reinterpret_cast<float*>(P.save_g) + lrow * q.ldo, n, q.cols, 1, v);
+                store_row(reinterpret_cast<float*>(P.save_u) + lrow * q.ldo, n, q.cols, 1, u);
+              }
+            }
+            gate_all<kFast>(v, u, P.act);
+            if (live) store_row(out, n, q.cols, q.vec, v);
+          } else if constexpr (EPI == kDGlu) {
+            float g[32], u[32];
+            if constexpr (IN == kBf16) {
+              ahead.get(0, g);
+              ahead.get(1, u);
+              ahead.load(P, q, lrow, n + 64, t.n0 + t.nval);
+            } else if (live) {
+              load_row(reinterpret_cast<const float*>(P.save_g) + lrow * q.ldo, n, q.cols, true, g);
+              load_row(reinterpret_cast<const float*>(P.save_u) + lrow * q.ldo, n, q.cols, true, u);
+            }
+            if (live) {
+              gate_grad_all<kFast>(v, g, u, P.act);
+              store_row(out, n, q.cols, q.vec, g);
+              store_row(reinterpret_cast<O*>(P.out2) + lrow * q.ldo, n, q.cols, q.vec, u);
+            }
+          } else {
+            if constexpr (IN == kI8) {
+              if (P.bias != nullptr) {
+                const O* b = reinterpret_cast<const O*>(P.bias);
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                  if (c + j < t.ntok) {
-                    const float x = __ldcg(at + (int64_t)j * 128);
-                    if constexpr (IN == kI8) r[j] += __float_as_uint(x);
-                    else r[j] = __float_as_uint(__uint_as_float(r[j]) + x);
+                  if (n + j < q.cols) {
+                    if constexpr (sizeof(O) == 2) v[j] += __bfloat162float(b[n + j]);
+                    else v[j] += b[n + j];
                   }
               }
-            } else {
-              chunk(c, r);
             }
+            if (live) store_row(out, n, q.cols, q.vec, v);
+          }
+        }
+      } else if (mine) {
+        // ------------ columns: this lane's output column, 32 tokens at a time
+        const int ch = kGluE ? t.m0 + 64 * (int)rank + 32 * (q4 & 1) + lane : (int)lrow;
+        const int up = kGluE ? q4 >> 1 : 0;  // kGlu: a warp of gate or up values
+        const bool whole = q.vec && (ch & ~31) + 32 <= q.cols;
+        float cs = 1.0f, bias = 0.0f;
+        if constexpr (IN == kI8) cs = ch < q.cols ? __ldg((up ? P.col_scale[1] : P.col_scale[0]) + ch) : 0.0f;
+        if constexpr (EPI == kStore && IN == kI8) {
+          if (P.bias != nullptr && ch < q.cols) {
+            if constexpr (sizeof(O) == 2) bias = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(P.bias)[ch]);
+            else bias = reinterpret_cast<const float*>(P.bias)[ch];
+          }
+        }
+        // n tokens of the block o (32 or 16 of them, lane = column), tokens tok0 + j of the tile, through `st`
+        auto put = [&](O* base, const auto& o, int tok0, __nv_bfloat16* st) {
+          constexpr int N = sizeof(o) / sizeof(o[0]);
+          if constexpr (sizeof(O) == 2) {
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < N; ++j) st[j * 32 + lane] = __float2bfloat16_rn(o[j]);
+              __syncwarp();
+#pragma unroll
+              for (int rr = 0; rr < N / 8; ++rr) {
+                const int tok = rr * 8 + (lane >> 2);
+                if (tok0 + tok < t.nval)
+                  *reinterpret_cast<uint4*>(base + (int64_t)(t.n0 + tok0 + tok) * q.ldo + (ch & ~31) + 8 * (lane & 3)) =
+                      *reinterpret_cast<const uint4*>(st + tok * 32 + 8 * (lane & 3));
+              }
+              __syncwarp();
+              return;
+            }
+          }
+          if (ch < q.cols) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (tok0 + j < t.nval) {
+                O* at = base + (int64_t)(t.n0 + tok0 + j) * q.ldo + ch;
+                if constexpr (sizeof(O) == 2) *at = __float2bfloat16_rn(o[j]);
+                else *at = o[j];
+              }
+          }
+        };
+#pragma unroll 1
+        for (int c = 32 * eh; c < ncol; c += 64) {
+          if (c >= t.nval) break;
+          float v[32];
+          {
+            uint32_t r[32];
+            finished(c, r);
             if constexpr (IN == kI8) {
-              const float rs = c + lane < t.ntok ? __ldg(P.row_scale + t.n0 + c + lane) : 0.0f;
+              const float rs = c + lane < t.nval ? __ldg(P.row_scale + t.n0 + c + lane) : 0.0f;
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * (cs * __shfl_sync(0xffffffffu, rs, j));
             } else {
@@ -533,107 +733,89 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
             }
           }
+          const int64_t tok = t.n0 + c;
           if constexpr (kGluE) {
             if (P.save_g != nullptr) {
-              if constexpr (IN == kBf16) save_f16(P, q, up, gch, t.n0 + c, t.ntok - c, v);
-              else if (gch < q.M) {
-                float* at = reinterpret_cast<float*>(up ? P.save_u : P.save_g) + (int64_t)(t.n0 + c) * q.ldo + gch;
+              if constexpr (IN == kBf16) {
+                const int groups = (q.cols + 31) / 32;
+                uint32_t el = 0;  // lane j's: the exponent of token j
+                __half* at = reinterpret_cast<__half*>(up ? P.save_u : P.save_g) + tok * q.ldo + ch;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  const float a = ch < q.cols ? finite_abs(v[j]) : 0.0f;
+                  const uint32_t e = f16_exp(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a))));
+                  if (lane == j) el = e;
+                  if (ch < q.cols && c + j < t.nval) at[j * q.ldo] = __float2half_rn(v[j] * f16_factor(e));
+                }
+                if (c + lane < t.nval && (ch & ~31) < q.cols)
+                  P.save_e[((int64_t)up * q.rows + tok + lane) * groups + ch / 32] = (uint8_t)el;
+              } else if (ch < q.cols) {
+                float* at = reinterpret_cast<float*>(up ? P.save_u : P.save_g) + tok * q.ldo + ch;
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                  if (c + j < t.ntok) at[j * q.ldo] = v[j];
+                  if (c + j < t.nval) at[j * q.ldo] = v[j];
               }
             }
-            // the gate warp forms columns 0-15 of the chunk, the up warp 16-31; two buffers, so that one
-            // barrier a chunk is enough
+            // two buffers, so that one barrier a chunk is enough
             float* mine_x = reinterpret_cast<float*>(stg) + xb * 512;
             float* other_x = reinterpret_cast<float*>(smem + kStages * kStageBytes + (ew ^ 2) * kStgBytes) + xb * 512;
             xb ^= 1;
 #pragma unroll
             for (int j = 0; j < 16; ++j) mine_x[j * 32 + lane] = up ? v[j] : v[16 + j];
-            pair_barrier(1 + (ew & 1) + 2 * eh);
-            float o[16];
+            pair_barrier(pair_id);
+            float g[16], u[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float got = other_x[j * 32 + lane];
-              const float g = up ? got : v[j], u = up ? v[16 + j] : got;
-              o[j] = gate<kFast>(g, P.act) * u;
+              g[j] = up ? got : v[j];
+              u[j] = up ? v[16 + j] : got;
             }
-            const int tok0 = c + 16 * up;
-            O* out = reinterpret_cast<O*>(q.out);
-            if (sizeof(O) == 2 && q.vec && (gch & ~31) + 32 <= q.M) {
-              if constexpr (sizeof(O) == 2) {
-                // staged where the other warp's values lay, which this warp alone reads
-                __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(other_x);
-                __syncwarp();
+            gate_all<kFast>(g, u, P.act);
+            // staged where the other warp's values lay, which this warp alone reads
+            __syncwarp();
+            put(reinterpret_cast<O*>(q.out), g, c + 16 * up, reinterpret_cast<__nv_bfloat16*>(other_x));
+          } else if constexpr (EPI == kDGlu) {
+            float g[32], u[32];
+            if constexpr (IN == kBf16) {
+              const int groups = (q.cols + 31) / 32;
+              float sc[2] = {0.0f, 0.0f};  // lane j's: the factors of token j
+              if (c + lane < t.nval && (ch & ~31) < q.cols) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) st[j * 32 + lane] = __float2bfloat16_rn(o[j]);
-                __syncwarp();
-#pragma unroll
-                for (int rr = 0; rr < 2; ++rr) {
-                  const int tok = rr * 8 + (lane >> 2);
-                  if (tok0 + tok < t.ntok)
-                    *reinterpret_cast<uint4*>(out + (int64_t)(t.n0 + tok0 + tok) * q.ldo + (gch & ~31) + 8 * (lane & 3)) =
-                        *reinterpret_cast<const uint4*>(st + tok * 32 + 8 * (lane & 3));
-                }
+                for (int i = 0; i < 2; ++i)
+                  sc[i] = f16_back(P.save_e[((int64_t)i * q.rows + tok + lane) * groups + ch / 32]);
               }
-            } else if (gch < q.M) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (tok0 + j < t.ntok) {
-                  O* at = out + (int64_t)(t.n0 + tok0 + j) * q.ldo + gch;
-                  if constexpr (sizeof(O) == 2) *at = __float2bfloat16_rn(o[j]);
-                  else *at = o[j];
-                }
-            }
-          } else {
-            constexpr int NO = EPI == kDGlu ? 2 : 1;
-            if constexpr (EPI == kDGlu) {
+              const __half *pg = reinterpret_cast<const __half*>(P.save_g), *pu = reinterpret_cast<const __half*>(P.save_u);
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                float a, da;
-                gate_grad<kFast>(gv[j], P.act, &a, &da);
-                const float dh = v[j];
-                v[j] = dh * uv[j] * da;
-                uv[j] = dh * a;
+                const bool in = ch < q.cols && c + j < t.nval;
+                const int64_t at = (tok + j) * q.ldo + ch;
+                g[j] = in ? __half2float(pg[at]) : 0.0f;
+                u[j] = in ? __half2float(pu[at]) : 0.0f;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                g[j] *= __shfl_sync(0xffffffffu, sc[0], j);
+                u[j] *= __shfl_sync(0xffffffffu, sc[1], j);
+              }
+            } else {
+              const float *pg = reinterpret_cast<const float*>(P.save_g), *pu = reinterpret_cast<const float*>(P.save_u);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const bool in = ch < q.cols && c + j < t.nval;
+                const int64_t at = (tok + j) * q.ldo + ch;
+                g[j] = in ? __ldg(pg + at) : 0.0f;
+                u[j] = in ? __ldg(pu + at) : 0.0f;
               }
             }
-            if constexpr (EPI == kStore && IN == kI8) {
+            gate_grad_all<kFast>(v, g, u, P.act);
+            put(reinterpret_cast<O*>(q.out), g, c, reinterpret_cast<__nv_bfloat16*>(stg));
+            put(reinterpret_cast<O*>(P.out2), u, c, reinterpret_cast<__nv_bfloat16*>(stg));
+          } else {
+            if constexpr (IN == kI8) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] += bias;
             }
-            O* outs[2] = {reinterpret_cast<O*>(q.out), reinterpret_cast<O*>(P.out2)};
-            if (sizeof(O) == 2 && q.vec && t.m * 256 + 128 * (int)rank + 32 * q4 + 32 <= q.M) {
-              if constexpr (sizeof(O) == 2) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  stg16[j * 32 + lane] = __float2bfloat16_rn(v[j]);
-                  if constexpr (NO == 2) stg16[1024 + j * 32 + lane] = __float2bfloat16_rn(uv[j]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int o = 0; o < NO; ++o)
-#pragma unroll
-                  for (int rr = 0; rr < 4; ++rr) {
-                    const int tok = rr * 8 + (lane >> 2);
-                    if (c + tok < t.ntok)
-                      *reinterpret_cast<uint4*>(outs[o] + (int64_t)(t.n0 + c + tok) * q.ldo + (mrow & ~31) + 8 * (lane & 3)) =
-                          *reinterpret_cast<const uint4*>(stg16 + o * 1024 + tok * 32 + 8 * (lane & 3));
-                  }
-                __syncwarp();
-              }
-            } else if (mrow < q.M) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (c + j < t.ntok) {
-                  const int64_t at = (int64_t)(t.n0 + c + j) * q.ldo + mrow;
-                  if constexpr (sizeof(O) == 2) outs[0][at] = __float2bfloat16_rn(v[j]);
-                  else outs[0][at] = v[j];
-                  if constexpr (NO == 2) {
-                    if constexpr (sizeof(O) == 2) outs[1][at] = __float2bfloat16_rn(uv[j]);
-                    else outs[1][at] = uv[j];
-                  }
-                }
-            }
+            put(reinterpret_cast<O*>(q.out), v, c, reinterpret_cast<__nv_bfloat16*>(stg));
           }
         }
       }
@@ -765,47 +947,78 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     const Problem& s = j.prob[i];
     Prob& q = P.prob[i];
     q = Prob{};
-    q.M = s.M; q.N = s.N; q.K = s.K;
-    q.nseg = j.epi == kGlu ? 1 : s.nseg;
+    const bool glu = j.epi == kGlu;
+    q.rows = s.N; q.cols = s.M; q.K = s.K;
+    const int oes = j.dtype == DSCA_BF16 ? 2 : 4;
+    auto on = [&](const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+    auto rows_on = [&](int64_t n) {
+      return s.ldo * oes % n == 0 && on(s.out, n) && on(j.out2, n) && on(j.save_g, n) && on(j.save_u, n);
+    };
+    q.vec = rows_on(32) ? 2 : rows_on(16) ? 1 : 0;
+    // Rows need wide stores: a thread's single values would lie a row apart (2-byte stores of 901-wide rows, training
+    // 333 x 1021 x 901: 53 us against 21 for the last product)
+    q.row = s.N > 128 && q.vec;
+    q.nseg = glu ? 1 : s.nseg;
     q.kb = ceil_div(s.K, ke);
-    q.boxes = q.nseg * (f32 ? 6 : 1) * q.kb;
-    q.a_mn = s.a[0].mn; q.b_mn = s.b[0].mn;
-    q.tiles_m = ceil_div(s.M, j.epi == kGlu ? 128 : 256);
-    // rows of n a tile: the waves of tiles by a tile's time, which is mostly the 256 rows of A (2048 x 5632, us a
-    // stage of two boxes: 1.15 at 256 rows of n, 0.95 at 192, 0.86 at 128)
-    q.tn = most;
-    if (q.b_mn) {
-      if (s.N <= 128) q.tn = 128;
-    } else {
-      double best = 0;
-      const int unit = j.epi == kStore ? 16 : 32;  // g and u are saved by whole 32 tokens
-      for (int nt = ceil_div(s.N, most), e = nt + 4; nt <= e; ++nt) {
-        const int tn = std::max(unit, (ceil_div(s.N, nt) + unit - 1) / unit * unit);
-        const int64_t tiles = (int64_t)q.tiles_m * ceil_div(s.N, tn);
-        const double cost = (j.nprob == 1 ? (double)ceil_div(tiles, pairs) : (double)tiles / pairs) * (tn + 280);
-        if (best == 0 || cost < best * 0.99) {
-          best = cost;
-          q.tn = tn;
-        }
+    const int terms = f32 ? 6 : 1;
+    q.boxes = q.nseg * terms * q.kb;
+    q.a_mn = q.row ? s.b[0].mn : s.a[0].mn;
+    q.b_mn = q.row ? s.a[0].mn : s.b[0].mn;
+    // Tile width and k splits by an estimate of the time: waves of tiles, each its boxes' time and a fixed part.  A box
+    // costs mostly its 256 rows of A: 256 rows of B 1, 192 0.83, 128 0.75 of the time (2048 x 5632).
+    const int whole = f32 ? 6 : 2;  // boxes that stay together: all terms of a slice, whole stages
+    double best = -1;
+    auto consider = [&](int tn, int splits) {
+      const int per_tile = q.row && glu ? tn / 2 : tn;
+      const int tm = q.row ? ceil_div(q.rows, 256) : ceil_div(q.cols, glu ? 128 : 256);
+      const int tiles_n = ceil_div(q.row ? q.cols : q.rows, per_tile);
+      const int64_t tiles = (int64_t)tm * tiles_n;
+      const int per = ceil_div(ceil_div(q.boxes, splits), whole) * whole;
+      splits = ceil_div(q.boxes, per);
+      if (splits > 1 && tiles * splits > 2 * pairs) return;  // bounds the partial tiles
+      const double box = 0.2 + 0.1 * tn / 128.0;                     // us
+      const double fixed = 1.0 + (splits > 1 ? 1.5 + 0.5 * splits * tn / 64.0 : 0.0);
+      const double waves = j.nprob == 1 ? (double)ceil_div(tiles * splits, pairs) : std::max(1.0, (double)(tiles * splits) / pairs);
+      const double cost = waves * (box * per + fixed) + 0.02 * tn / 256.0 * per;
+      if (best < 0 || cost < best * 0.98) {
+        best = cost;
+        q.tn = tn; q.tiles_m = tm; q.tiles_n = tiles_n;
+        q.splits = splits; q.per = per;
+      }
+    };
+    for (int splits = 1; splits <= (j.nprob == 1 ? 8 : 1) && (splits == 1 || q.boxes >= 4 * whole * splits); ++splits) {
+      if (q.row || q.b_mn) {
+        // a gated tile's gate and up chunks of 32 belong to one warp only from 64 channels on
+        for (int tn = most; tn >= (q.b_mn || glu ? 128 : 64); tn /= 2) consider(tn, splits);
+      } else {
+        for (int nt = ceil_div(q.rows, most), e = nt + 2; nt <= e; ++nt)  // tokens in equal tiles
+          consider(std::max(32, ceil_div(ceil_div(q.rows, nt), 32) * 32), splits);
       }
     }
-    q.tiles_n = ceil_div(s.N, q.tn);
-    q.splits = 1;
-    q.per = (q.boxes + 1) / 2 * 2;
+  }
+  // Several problems: one whose tiles take long against the whole launch's share of a pair is split (training
+  // 640 x 768 x 2048: dx has nine tiles of 64 boxes beside 72 of ten)
+  if (j.nprob > 1) {
+    double work = 0;
+    auto time = [](const Prob& q) { return (0.2 + 0.1 * q.tn / 128.0) * q.boxes; };
+    for (int i = 0; i < j.nprob; ++i) work += time(P.prob[i]) * P.prob[i].tiles_m * P.prob[i].tiles_n;
+    for (int i = 0; i < j.nprob; ++i) {
+      Prob& q = P.prob[i];
+      const int whole = f32 ? 6 : 2;
+      int want = (int)std::min(8.0, time(q) / (0.6 * work / pairs));
+      want = std::min(want, q.boxes / (4 * whole));
+      if (want < 2 || (int64_t)q.tiles_m * q.tiles_n * want > 2 * pairs) continue;
+      q.per = ceil_div(ceil_div(q.boxes, want), whole) * whole;
+      q.splits = ceil_div(q.boxes, q.per);
+    }
+  }
+  for (int i = 0; i < j.nprob; ++i) {
+    Prob& q = P.prob[i];
     const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
-    if (j.nprob == 1 && tiles * 2 <= pairs) {
-      // at least four stages (eight boxes) a split
-      const int want = (int)std::min<int64_t>(pairs / tiles, q.boxes / 8);
-      if (want > 1) {
-        const int whole = f32 ? 6 : 2;  // all terms of a slice, whole stages
-        q.per = ceil_div(ceil_div(q.boxes, want), whole) * whole;
-        q.splits = ceil_div(q.boxes, q.per);
-      }
-    }
     if (q.splits > 1) {
       q.part = (int64_t)*floats;
       q.counter = (int)*counters;
-      *floats += (size_t)tiles * q.splits * 2 * q.tn * 128;
+      *floats += (size_t)tiles * q.splits * 2 * ((q.tn + 31) / 32 * 32) * 128;
       *counters += (size_t)tiles * 2 * kEpiWarps;
     }
     q.first = (int)total;
@@ -818,15 +1031,16 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
 
 }  // namespace tc
 
-size_t tc_workspace(const Job& j) {
+int tc_workspace(const Job& j, size_t* parts, size_t* counters) {
   tc::Params P;
-  size_t floats, counters;
-  if (tc::plan(j, P, tc::resident_pairs(), &floats, &counters) < 0) return 0;
-  return (counters * 4 + 255) / 256 * 256 + floats * 4;
+  size_t floats, n;
+  if (tc::plan(j, P, tc::resident_pairs(), &floats, &n) < 0) return DSCA_ERR_CAPACITY;
+  *parts = floats * 4;
+  *counters = n * 4;
+  return DSCA_OK;
 }
 
-// The counters lie at the start of ws (zeroed by the caller), the partial tiles behind them.
-int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t stream) {
+int launch_tc(const Job& j, void* parts, void* counts, int32_t* err, bool pdl, cudaStream_t stream) {
   tc::Params P = {};
   const int pairs = tc::resident_pairs();
   size_t floats, counters;
@@ -839,31 +1053,29 @@ int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t strea
     tc::Prob& q = P.prob[i];
     q.out = s.out;
     q.ldo = s.ldo;
-    const int oes = j.dtype == DSCA_BF16 ? 2 : 4;
-    q.vec = reinterpret_cast<uintptr_t>(s.out) % 16 == 0 && s.ldo * oes % 16 == 0 &&
-            reinterpret_cast<uintptr_t>(j.out2) % 16 == 0;
     const int planes = f32 ? 3 : 1;
-    q.a_plane = (int)s.a[0].plane;
-    q.b_plane = (int)s.b[0].plane;
-    for (int g = 0; g < 2; ++g) {
-      const Operand &a = s.a[g], &b = s.b[g];
-      const bool has_a = g == 0 || j.epi == kGlu || s.nseg > 1, has_b = g == 0 || (j.epi != kGlu && s.nseg > 1);
-      // fp32: three planes of rows (an MN-major plane ends on a whole MMA step of zeros)
-      auto rows = [&](const Operand& o, int r) { return f32 ? planes * o.plane : (int64_t)(o.mn ? s.K : r); };
-      if (has_a)
-        if (int rc = tc::make_map(&P.a[i][g], a.p, rows(a, s.M), a.mn ? s.M : s.K, a.ld, es,
-                                  a.mn || j.epi == kGlu ? 64 : 128))
-          return rc;
-      if (has_b)
-        if (int rc = tc::make_map(&P.b[i][g], b.p, rows(b, s.N), b.mn ? s.N : s.K, b.ld, es, b.mn ? 64 : q.tn / 2))
-          return rc;
-    }
+    const Operand *A = q.row ? s.b : s.a, *B = q.row ? s.a : s.b;  // the MMA's operands
+    const int a_ext = q.row ? s.N : s.M, b_ext = q.row ? s.M : s.N;
+    q.a_plane = (int)A[0].plane;
+    q.b_plane = (int)B[0].plane;
+    const bool glu = j.epi == kGlu;
+    const int na = glu ? (q.row ? 1 : 2) : s.nseg, nb = glu ? (q.row ? 2 : 1) : s.nseg;
+    // fp32: three planes of rows (an MN-major plane ends on a whole MMA step of zeros)
+    auto map = [&](CUtensorMap* m, const Operand& o, int ext, int box) {
+      const int64_t rows = f32 ? planes * o.plane : (int64_t)(o.mn ? s.K : ext);
+      return tc::make_map(m, o.p, rows, o.mn ? ext : s.K, o.ld, es, o.mn ? 64 : box);
+    };
+    for (int g = 0; g < na; ++g)
+      if (int rc = map(&P.a[i][g], A[g], a_ext, glu && !q.row ? 64 : 128)) return rc;
+    for (int g = 0; g < nb; ++g)
+      if (int rc = map(&P.b[i][g], B[g], b_ext, q.tn / 2)) return rc;
   }
   P.act = j.act;
   P.save_g = j.save_g; P.save_u = j.save_u; P.save_e = j.save_e; P.out2 = j.out2;
   P.row_scale = j.row_scale; P.col_scale[0] = j.col_scale[0]; P.col_scale[1] = j.col_scale[1]; P.bias = j.bias;
-  P.counters = reinterpret_cast<uint32_t*>(ws);
-  P.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + (counters * 4 + 255) / 256 * 256);
+  P.vec_cols = (reinterpret_cast<uintptr_t>(j.col_scale[0]) | reinterpret_cast<uintptr_t>(j.col_scale[1])) % 16 == 0;
+  P.counters = reinterpret_cast<uint32_t*>(counts);
+  P.parts = reinterpret_cast<float*>(parts);
   P.err = err;
   using B = __nv_bfloat16;
   if (j.i8) {
@@ -879,14 +1091,6 @@ int launch_tc(const Job& j, void* ws, int32_t* err, bool pdl, cudaStream_t strea
   if (j.epi == kGlu) return tc::launch<kGlu, tc::kBf16, B>(P, pairs, pdl, stream);
   if (j.epi == kDGlu) return tc::launch<kDGlu, tc::kBf16, B>(P, pairs, pdl, stream);
   return tc::launch<kStore, tc::kBf16, B>(P, pairs, pdl, stream);
-}
-
-// Bytes of counters at the start of the workspace that have to be zero at the launch.
-size_t tc_zero_bytes(const Job& j) {
-  tc::Params P;
-  size_t floats, counters;
-  if (tc::plan(j, P, tc::resident_pairs(), &floats, &counters) < 0) return 0;
-  return counters * 4;
 }
 
 }  // namespace dense

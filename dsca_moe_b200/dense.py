@@ -77,7 +77,12 @@ def _weight(w, name: str, out: int, inp: int, x) -> int:
 
 def _workspace(name: str, args, dev):
     """The call's workspace, allocated on the current stream, in args."""
-    n = getattr(L.load(), name)(ctypes.byref(args))
+    fn = getattr(L._LIB or L.load(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        n = fn(ctypes.byref(args))
+    else:
+        with torch.cuda.device(dev):
+            n = fn(ctypes.byref(args))
     if n == 0:
         return None
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -91,19 +96,18 @@ def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
     y = torch.empty(x.shape, dtype=dtype, device=dev)
     if rows == 0:
         return y, (None, None)
-    ld_h = (inter + 7) // 8 * 8
+    ld_h = (inter + 15) // 16 * 16  # rows on 32-byte sectors
     h = torch.empty((rows, ld_h), dtype=dtype, device=dev)
     gu, g, u, e = None, None, None, None
     if save:
         size = 2 if dtype == torch.bfloat16 else 4
         step = rows * ld_h * size
-        gu = torch.empty(2 * step + (0 if size == 4 else (rows + 31) // 32 * 2 * ld_h), dtype=torch.uint8, device=dev)
+        gu = torch.empty(2 * step + (0 if size == 4 else 2 * rows * ((inter + 31) // 32)), dtype=torch.uint8, device=dev)
         g = gu.data_ptr()
         u, e = g + step, (g + 2 * step if size == 2 else None)
     a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h.data_ptr(), rows, d,
                        inter, _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
-    with torch.cuda.device(dev):
-        ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
+    ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
     return y, (h, gu)
 
@@ -146,8 +150,7 @@ class _GatedFFN(torch.autograd.Function):
             a.dg, a.du = grads.data_ptr(), grads.data_ptr() + rows * ld_h * grads.element_size()
             a.ld_x, a.ld_gate, a.ld_up, a.ld_down, a.ld_dy, a.ld_h = ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h
             a.err = _err(dev)
-            with torch.cuda.device(dev):
-                keep = (grads, _workspace("dsca_gated_ffn_backward_workspace", a, dev))
+            keep = (grads, _workspace("dsca_gated_ffn_backward_workspace", a, dev))
         L.call_on(dev, "dsca_gated_ffn_backward", ctypes.byref(a))
         del keep
         return dx, dwg, dwu, dwd, None, None
@@ -298,8 +301,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     a.bias = None if bias is None else bias.data_ptr()
     a.y, a.ld_y = y.data_ptr(), n
     a.rows, a.k, a.n, a.dtype, a.err = rows, k, n, dt, _err(dev)
-    with torch.cuda.device(dev):
-        ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
+    ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_int8_linear", ctypes.byref(a))
     return y
 
@@ -337,8 +339,7 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     a.gate_scale, a.up_scale, a.down_scale = w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr()
     a.rows, a.d, a.inter, a.dtype, a.act, a.err = rows, d, inter, dt, code, _err(dev)
     a.ld_x, a.ld_q, a.ld_h, a.ld_hq, a.ld_y = ld_x, ld_q, ld_hq, ld_hq, d
-    with torch.cuda.device(dev):
-        ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
+    ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
     return y
 

@@ -31,7 +31,7 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 /*
  * g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T; sums in fp32, h and y rounded to dtype.  g and u
  * are written when given (both or neither), for the backward pass: in fp32 for DSCA_F32; for DSCA_BF16 as
- * fp16 times a power of two for each channel of 32 tokens, whose exponents gu_exp takes.  h is a work area [rows, ld_h] that the backward pass reads as well.
+ * fp16 times a power of two for every 32 channels of a token, whose exponents gu_exp takes.  h is a work area [rows, ld_h] that the backward pass reads as well.
  */
 typedef struct {
   const void* x;        /* [rows, d], dtype */
@@ -41,7 +41,7 @@ typedef struct {
   void* y;              /* [rows, d] */
   void* g;              /* [rows, ld_h] fp32 or fp16, or NULL */
   void* u;
-  uint8_t* gu_exp;      /* [2, ceil(rows / 32), ld_h]; with DSCA_BF16 and g */
+  uint8_t* gu_exp;      /* [2, rows, ceil(inter / 32)]; with DSCA_BF16 and g */
   void* h;              /* [rows, ld_h] */
   int rows, d, inter;
   int dtype;            /* DSCA_BF16, DSCA_F32 */

@@ -3,7 +3,8 @@
 Bounds.  A sum of k products in fp32, in any order and with truncating additions, is off by at most
 (k + 8) 2^-23 of the sum of the products' magnitudes (`acc`).  Each rounding to the type is off by
 half a step, eps / 2 (`half`).  The gates' exponentials and divisions are good to 2^-18 of their value
-in 16 bits, 2^-21 in 32 (`fast`).  |act'| <= 1.13 for all gates, |act''| <= 0.8 (relu: act' may be
+for 16-bit and 8-bit operands (the hardware's exponential: 2^-22, and 2^-24 |g| / ln 2 from its argument; where that
+passes 2^-18, |g| > 45, the value is below e^-45), 2^-21 for 32-bit ones (`fast`).  |act'| <= 1.13 for all gates, |act''| <= 0.8 (relu: act' may be
 anything in [0, 1] where g's own error reaches 0).  Errors of factors are carried through each
 product at first order with both factors' magnitudes enlarged by their errors."""
 import math
@@ -54,10 +55,11 @@ def ffn(x, wg, wu, wd, name, dtype, dy=None):
         return out
     dy = dy.double()
     if dtype == torch.bfloat16:
-        # the backward pass reads g and u in 11 bits, or 2^-25 of 2^-14 of a channel's largest of 32 tokens
+        # the backward pass reads g and u in 11 bits, or half of 2^-24 of the scaled range (2^-38 of the largest of a
+        # token's 32 channels)
         def held(v, e):
-            big = torch.nn.functional.pad(v.abs() + e, (0, 0, 0, -T % 32)).view(-1, 32, I).amax(1)
-            return e + 2.0 ** -12 * (v.abs() + e) + 2.0 ** -38 * big.repeat_interleave(32, 0)[:T]
+            big = torch.nn.functional.pad(v.abs() + e, (0, -I % 32)).view(T, -1, 32).amax(2)
+            return e + 2.0 ** -12 * (v.abs() + e) + 2.0 ** -38 * big.repeat_interleave(32, 1)[:, :I]
         eg, eu = held(g, eg), held(u, eu)
     ea = 1.13 * eg + fast * (a.abs() + 1.13 * eg)
     eda = (g.abs() <= eg).double() if name == "relu" else 0.8 * eg + fast * (da.abs() + g.abs() * 0.5)
@@ -110,7 +112,7 @@ def ffn_int8(x, wg, wu, wd, name, dtype):
         return v, 4 * 2.0 ** -24 * v.abs()
     (g, eg), (u, eu) = prod(wg), prod(wu)
     a, _ = act(g, name)
-    ea = 1.13 * eg + 2.0 ** -21 * a.abs()
+    ea = 1.13 * eg + 2.0 ** -18 * a.abs()
     h = a * u
     eh = _mul(a, ea, u, eu) * 1.01 + 2.0 ** -24 * h.abs()
     m = h.abs().amax(-1, keepdim=True)
