@@ -17,7 +17,14 @@ from .runtime import QoSRuntimeContext, RequestStateTable  # noqa: F401
 
 
 def __getattr__(name):
-    # torch-dependent pieces load lazily so that `import dsca_moe_b200` stays cheap
+    # torch-dependent pieces load lazily so that `import dsca_moe_b200` stays cheap, and are found
+    # without this function from then on
+    value = _load(name)
+    globals()[name] = value
+    return value
+
+
+def _load(name):
     if name in ("QoSMoELayer", "ShardedQwenMoE", "patch", "placement_to_expert_to_gpu"):
         from . import layers
         return getattr(layers, name)

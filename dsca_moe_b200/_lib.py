@@ -125,6 +125,7 @@ class FewArgs(ctypes.Structure):
 GATE_SILU, GATE_GELU, GATE_RELU = range(3)
 DENSE_MAX_DIM = 1048576
 DENSE_MAX_ROWS = 16777216
+DENSE_FEW_TOKENS = 16
 
 
 class GatedFfnArgs(ctypes.Structure):

@@ -26,7 +26,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
               "--expt-relaxed-constexpr", "-I" + INCLUDE] + ARCH
 CU_SOURCES = ["router.cu", "router_tc.cu", "dispatch.cu", "gemm_sm100.cu", "gemm_sm100_pair.cu", "gemm_sm100_fp8.cu", "gemm_sm100_fp8t.cu", "gemm_simt.cu", "abi.cu",
-              "ffn_static_scratch.cu", "ep.cu", "qos.cu", "norm.cu", "moe_few.cu", "dense.cu", "dense_tc.cu", "dense_split.cu", "dense_quant.cu"]
+              "ffn_static_scratch.cu", "ep.cu", "qos.cu", "norm.cu", "moe_few.cu", "dense.cu", "dense_tc.cu", "dense_split.cu", "dense_few.cu", "dense_quant.cu"]
 CXX_SOURCES = ["plan.cpp"]
 
 

@@ -35,7 +35,7 @@ int check(const dsca_gated_ffn_args* a) {
   const int64_t e = esize(a->dtype);
   if (!at(a->x, e) || !at(a->w_gate, e) || !at(a->w_up, e) || !at(a->w_down, e) || !at(a->y, e) || !at(a->h, 16) ||
       !at_or_null(a->g, 16) || !at_or_null(a->u, 16) || (a->g == nullptr) != (a->u == nullptr) ||
-      (a->g != nullptr && a->dtype == DSCA_BF16 && a->gu_exp == nullptr))
+      (a->g != nullptr && a->dtype == DSCA_BF16 && !at(a->gu_exp, 4)))
     return DSCA_ERR_BAD_ARG;
   if (!ld_ok(a->ld_x, a->d) || !ld_ok(a->ld_gate, a->d) || !ld_ok(a->ld_up, a->d) || !ld_ok(a->ld_down, a->inter) ||
       !ld_ok(a->ld_y, a->d) || !ld_ok(a->ld_h, a->inter) || a->ld_h * e % 16 != 0)
@@ -53,7 +53,7 @@ int check(const dsca_gated_ffn_backward_args* a) {
   if (a->rows == 0) return DSCA_OK;
   if (!at(a->x, e) || !at(a->w_gate, e) || !at(a->w_up, e) || !at(a->w_down, e) || !at(a->dy, e) || !at(a->g, 16) ||
       !at(a->u, 16) || !at(a->h, 16) || !at(a->dg, 16) || !at(a->du, 16) ||
-      (a->dtype == DSCA_BF16 && a->gu_exp == nullptr))
+      (a->dtype == DSCA_BF16 && !at(a->gu_exp, 4)))
     return DSCA_ERR_BAD_ARG;
   if (!ld_ok(a->ld_x, a->d) || !ld_ok(a->ld_gate, a->d) || !ld_ok(a->ld_up, a->d) || !ld_ok(a->ld_down, a->inter) ||
       !ld_ok(a->ld_dy, a->d) || !ld_ok(a->ld_h, a->inter) || a->ld_h * e % 16 != 0)
@@ -163,9 +163,9 @@ struct Call {
   int product(const Job& j, const Own& o, bool pdl) {
     return dry ? DSCA_OK : launch_tc(j, o.parts, o.counters, err, pdl, stream);
   }
-  int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale) {
+  int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, bool pdl) {
     dsca_quantize_rows_args a = {x, rows, k, dtype, ld_x, q, ld_q, scale};
-    return dry ? DSCA_OK : launch_quantize_rows(&a, stream);
+    return dry ? DSCA_OK : launch_quantize_rows(&a, pdl, stream);
   }
 };
 
@@ -180,6 +180,21 @@ Operand as(Operand o, int mn) {
 int run(Call& c, const dsca_gated_ffn_args* a) {
   const int dt = a->dtype, T = a->rows, d = a->d, I = a->inter;
   Job j = {}, k = {};
+  if (T <= DSCA_DENSE_FEW_TOKENS) {
+    j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
+    j.prob[0] = problem({a->w_gate, a->ld_gate, 0, 0}, {a->x, a->ld_x, 0, 0}, I, T, d, a->h, a->ld_h);
+    j.prob[0].a[1] = {a->w_up, a->ld_up, 0, 0};
+    j.save_g = a->g; j.save_u = a->u; j.save_e = a->gu_exp;
+    k.epi = kStore; k.nprob = 1; k.dtype = dt;
+    k.prob[0] = problem({a->w_down, a->ld_down, 0, 0}, {a->h, a->ld_h, 0, 0}, d, T, I, a->y, a->ld_y);
+    if (few_fits(j) && few_fits(k)) {
+      if (c.dry) return DSCA_OK;
+      TRY(launch_few(j, false, c.stream));
+      return launch_few(k, true, c.stream);
+    }
+    j = {};
+    k = {};
+  }
   j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
   j.prob[0] = problem(c.operand(a->w_gate, I, d, a->ld_gate, dt, 0), c.operand(a->x, T, d, a->ld_x, dt, 0), I, T, d,
                       a->h, a->ld_h);
@@ -254,8 +269,10 @@ int run(Call& c, const dsca_int8_linear_args* a) {
   j.row_scale = a->scale; j.col_scale[0] = a->w_scale; j.bias = a->bias;
   const Job* jobs[] = {&j};
   Call::Own own[1];
-  TRY(c.reserve(jobs, own, 1));
-  if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale));
+  const bool few = few_fits(j);
+  if (!few) TRY(c.reserve(jobs, own, 1));
+  if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false));
+  if (few) return c.dry ? DSCA_OK : launch_few(j, a->x != nullptr, c.stream);
   return c.product(j, own[0], a->x != nullptr);
 }
 
@@ -270,10 +287,13 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   k.row_scale = a->h_scale; k.col_scale[0] = a->down_scale;
   const Job* jobs[] = {&j, &k};
   Call::Own own[2];
-  TRY(c.reserve(jobs, own, 2));
-  TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale));
-  TRY(c.product(j, own[0], true));
-  TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale));
+  const bool few = few_fits(j) && few_fits(k);
+  if (!few) TRY(c.reserve(jobs, own, 2));
+  TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false));
+  if (few && !c.dry) TRY(launch_few(j, true, c.stream));
+  if (!few) TRY(c.product(j, own[0], true));
+  TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale, true));
+  if (few) return c.dry ? DSCA_OK : launch_few(k, true, c.stream);
   return c.product(k, own[1], true);
 }
 
@@ -319,7 +339,7 @@ int dsca_gated_ffn_backward(const dsca_gated_ffn_backward_args* a, dsca_stream_t
 
 int dsca_quantize_rows(const dsca_quantize_rows_args* a, dsca_stream_t stream) {
   if (int rc = dense::check(a)) return rc;
-  return a->rows == 0 ? DSCA_OK : dense::launch_quantize_rows(a, stream);
+  return a->rows == 0 ? DSCA_OK : dense::launch_quantize_rows(a, false, stream);
 }
 
 int dsca_int8_linear(const dsca_int8_linear_args* a, dsca_stream_t stream) {

@@ -88,6 +88,20 @@ __device__ __forceinline__ void gate_grad(float g, int act, float* a, float* da)
   }
 }
 
+// ---- g and u of 16-bit products for the backward pass: fp16 times a power of two that brings the largest finite one
+// of its group of a token's channels to [2^14, 2^15).  The exponent byte is the largest's, at least 14 so that the
+// factor is a normal number; a row has one for every eight channels (groups of 32 write four equal ones).
+__host__ __device__ __forceinline__ int exp_groups(int cols) { return (cols + 31) / 32 * 4; }
+__device__ __forceinline__ uint32_t f16_exp(float largest) { return max(14u, __float_as_uint(largest) >> 23); }
+__device__ __forceinline__ float f16_factor(uint32_t e) { return __uint_as_float((268u - e) << 23); }  // 2^(141 - e)
+__device__ __forceinline__ float f16_back(uint32_t e) {                                               // 2^(e - 141)
+  return e > 14u ? __uint_as_float((e - 14u) << 23) : 5.877471754111438e-39f;
+}
+
+// Products for few tokens (dense_few.cu); no workspace, any alignment.
+bool few_fits(const Job& j);
+int launch_few(const Job& j, bool pdl, cudaStream_t stream);
+
 // A matrix to lay out anew (dense_split.cu).
 struct Relay {
   const void* src;
@@ -107,7 +121,7 @@ int launch_relay(RelayList& list, cudaStream_t stream);
 // at the launch.
 int tc_workspace(const Job& j, size_t* parts, size_t* counters);
 int launch_tc(const Job& j, void* parts, void* counters, int32_t* err, bool pdl, cudaStream_t stream);
-int launch_quantize_rows(const dsca_quantize_rows_args* a, cudaStream_t stream);
+int launch_quantize_rows(const dsca_quantize_rows_args* a, bool pdl, cudaStream_t stream);
 
 }  // namespace dense
 }  // namespace dsca

@@ -60,6 +60,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
   const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;
   const bool live = row < a.rows;
+  pdl_launch_dependents();  // a product that follows asks for its first weights meanwhile
+  pdl_wait();
   const T* x = reinterpret_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x;
   float v[CH > 0 ? CH : 1][8];
   float m = 0.0f;
@@ -152,34 +154,42 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
 }
 
 template <typename T, int TPR, int CH>
-int launch(const dsca_quantize_rows_args& a, cudaStream_t stream) {
+int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
   const unsigned grid = (unsigned)(((int64_t)a.rows * TPR + 255) / 256);
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ld_x * (int64_t)sizeof(T)) % 16 == 0;
-  if (vec) quantize_kernel<T, TPR, CH, true><<<grid, 256, 0, stream>>>(a);
-  else quantize_kernel<T, TPR, CH, false><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  auto kern = vec ? quantize_kernel<T, TPR, CH, true> : quantize_kernel<T, TPR, CH, false>;
+  return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
 template <typename T>
-int run(const dsca_quantize_rows_args& a, cudaStream_t stream) {
+int run(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
   const int chunks = (int)(a.ld_q / 8);
   if (a.rows > 4 * current_device_sms()) {  // a warp a row while a warp holds it
-    if (chunks <= 32) return launch<T, 32, 1>(a, stream);
-    if (chunks <= 64) return launch<T, 32, 2>(a, stream);
-    if (chunks <= 128) return launch<T, 64, 2>(a, stream);
-    if (chunks <= 256) return launch<T, 128, 2>(a, stream);
+    if (chunks <= 32) return launch<T, 32, 1>(a, pdl, stream);
+    if (chunks <= 64) return launch<T, 32, 2>(a, pdl, stream);
+    if (chunks <= 128) return launch<T, 64, 2>(a, pdl, stream);
+    if (chunks <= 256) return launch<T, 128, 2>(a, pdl, stream);
   }
-  if (chunks <= 256) return launch<T, 256, 1>(a, stream);
-  if (chunks <= 512) return launch<T, 256, 2>(a, stream);
-  if (chunks <= 768) return launch<T, 256, 3>(a, stream);
-  if (chunks <= 1024) return launch<T, 256, 4>(a, stream);
-  return launch<T, 256, 0>(a, stream);
+  if (chunks <= 256) return launch<T, 256, 1>(a, pdl, stream);
+  if (chunks <= 512) return launch<T, 256, 2>(a, pdl, stream);
+  if (chunks <= 768) return launch<T, 256, 3>(a, pdl, stream);
+  if (chunks <= 1024) return launch<T, 256, 4>(a, pdl, stream);
+  return launch<T, 256, 0>(a, pdl, stream);
 }
 
 }  // namespace quant
 
-int launch_quantize_rows(const dsca_quantize_rows_args* a, cudaStream_t stream) {
-  return a->dtype == DSCA_BF16 ? quant::run<__nv_bfloat16>(*a, stream) : quant::run<float>(*a, stream);
+int launch_quantize_rows(const dsca_quantize_rows_args* a, bool pdl, cudaStream_t stream) {
+  return a->dtype == DSCA_BF16 ? quant::run<__nv_bfloat16>(*a, pdl, stream) : quant::run<float>(*a, pdl, stream);
 }
 
 }  // namespace dense

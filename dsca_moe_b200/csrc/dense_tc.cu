@@ -19,13 +19,16 @@
 // CTA's 128 rows of A are 64 gate rows and the up rows of the same channels; the warps of lane quarters q and
 // q + 2 hold the two, and for each chunk of 32 tokens the gate warp forms the products of the first 16 and the up
 // warp those of the last, after handing each other the other half through shared memory.
-// Saved for the backward pass in 16 bits: g and u as fp16 with one power of two for a token's 32 channels (11 bits
-// of significand for every value within 2^29 of the largest), half of fp32's bytes, which the backward pass reads
+// Saved for the backward pass in 16 bits: g and u as fp16 with one power of two for a token's 32 channels (11 bits of
+// significand for every value within 2^29 of the largest), half of fp32's bytes, which the backward pass reads
 // against the clock of its first product.
 //
-// 32-bit inputs (kF32): every value is split into three bf16 terms (8 + 8 + 8 bits, dense_split.cu) and the
-// product is six MMA passes over k: hi.hi into one accumulator, hi.mid, mid.hi, hi.lo, mid.mid and lo.hi into
-// another, which the epilogue adds.  What is left out is 2^-24 of the product's terms.
+// 32-bit inputs (kF32): every value is split into three bf16 terms (8 + 8 + 8 bits, dense_split.cu); a stage holds the
+// three planes of both operands' slice of k (72 KB, two stages), and six products are taken of them: hi.hi into one
+// accumulator, hi.mid, mid.hi, hi.lo, mid.mid and lo.hi into another.  What is left out is 2^-24 of the product's
+// terms.  The tensor cores' fp32 additions truncate, half a step of the running sum each, always towards zero: chains
+// over all of k = 1408 were off by 4e-6.  So every 256 of k the epilogue warps take the sums into registers and
+// add them there, rounding to nearest.
 //
 // Long k with few tiles: the k boxes are split over several pairs, each stores its fp32 tile to the workspace,
 // and for every warp's part the last one to arrive adds the parts in the order of k: the result does not
@@ -42,29 +45,40 @@ namespace dsca {
 namespace dense {
 namespace tc {
 
-#ifndef KSUB
-#define KSUB 2
-#endif
-constexpr int kSub = KSUB;                       // k boxes of a stage
-constexpr int kStages = 6 / kSub;
-constexpr int kBoxBytes = 128 * 128;             // an operand's part of one k box
-constexpr int kStageBytes = 2 * kSub * kBoxBytes;
+constexpr int kMaxStages = 3;
+constexpr int kBoxBytes = 128 * 128;             // A's part of one k box (slice of k); B's, but for kF32
+constexpr int kRingBytes = 12 * kBoxBytes;       // all stages
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kStgBytes = 2 * 32 * 32 * 2;       // per epilogue warp: two 32 x 32 blocks of bf16
-constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kStgBytes + 1024;
+constexpr int kSmemBytes = kRingBytes + kEpiWarps * kStgBytes + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
 
 enum In { kBf16 = 0, kI8 = 1, kF32 = 2 };
+
+// A stage's layout by the inputs: two boxes of A and two of B; kF32: one slice, three planes of A and of B (whose
+// tiles have at most 128 rows, half a box).
+template <int IN>
+struct Ring {
+  static constexpr bool F = IN == kF32;
+  static constexpr int kSub = F ? 1 : 2;     // slices of a stage
+  static constexpr int kPlanes = F ? 3 : 1;
+  static constexpr int kStages = F ? 2 : 3;
+  static constexpr int kBBytes = F ? kBoxBytes / 2 : kBoxBytes;
+  static constexpr int kB = kSub * kPlanes * kBoxBytes;                  // offset of B in a stage
+  static constexpr int kStageBytes = kB + kSub * kPlanes * kBBytes;
+  static constexpr int kChunk = 4;           // kF32: slices between two takings of the sums
+  static_assert(kStages * kStageBytes <= kRingBytes && kStages <= kMaxStages, "ring");
+};
 
 struct Prob {
   int rows, cols, K;     // of the output [rows, cols]
   int row;               // orientation: rows (1) or columns (0)
   int nseg, kb;          // segments; k boxes of each
-  int boxes;             // nseg * terms * kb
+  int boxes;             // nseg * kb
   int a_mn, b_mn;        // majors of the MMA's A and B
   int tiles_m, tiles_n, tn;
-  int splits, per;       // k splits and boxes of each (even)
+  int splits, per;       // k splits and boxes of each
   int first;             // the problem's first unit of work
   int a_plane, b_plane;  // kF32: rows between the planes of three terms
   int vec;               // output rows start on 16-byte (1) or 32-byte (2) boundaries
@@ -80,7 +94,7 @@ struct Params {
   int nprob, total, act;
   void* save_g;   // fp16 codes (16-bit inputs) or fp32
   void* save_u;
-  uint8_t* save_e;  // fp16: the exponents, [2][rows][ceil(cols / 32)]
+  uint8_t* save_e;  // fp16: the exponents, [2][rows][exp_groups(cols)]
   void* out2;
   const float* row_scale;
   const float* col_scale[2];
@@ -92,7 +106,7 @@ struct Params {
 };
 
 struct Ctl {
-  uint64_t full[kStages], empty[kStages], tmem_full[2], tmem_empty[2], mma_done;
+  uint64_t full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2], mma_done;
   uint32_t tmem_base;
   int abort_flag;
   int pair_ok[kEpiWarps], pair_old[kEpiWarps];
@@ -154,49 +168,24 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, ui
       : "memory");
 }
 
-// Where box b of a problem lies: slice k of a segment and, for 32-bit inputs, one of the six terms, which follow
-// one another within a slice.  Divisions once a tile, then counted on.
-template <int IN>
+// Where box b of a problem lies: slice k of a segment.
 struct BoxAt {
-  int seg, term, k;
-  __device__ __forceinline__ BoxAt(const Prob& q, int b) {
-    int s = b;
-    term = 0;
-    if constexpr (IN == kF32) {
-      s = b / 6;
-      term = b - 6 * s;
-    }
-    seg = s >= q.kb ? 1 : 0;
-    k = s - seg * q.kb;
-  }
+  int seg, k;
+  __device__ __forceinline__ BoxAt(const Prob& q, int b) : seg(b >= q.kb ? 1 : 0), k(b - seg * q.kb) {}
   __device__ __forceinline__ void next(int kb) {
-    if constexpr (IN == kF32) {
-      if (++term < 6) return;
-      term = 0;
-    }
     if (++k == kb) {
       k = 0;
       ++seg;
     }
   }
 };
-// the planes (hi 0, mid 1, lo 2) that term t multiplies
-__device__ __forceinline__ int plane_a(int t) { return t == 2 || t == 4 ? 1 : t == 5 ? 2 : 0; }
-__device__ __forceinline__ int plane_b(int t) { return t == 1 || t == 4 ? 1 : t == 3 ? 2 : 0; }
 
 // The two warps (64 threads) that exchange gate and up values.
 __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
-// ---- g and u in 16 bits: fp16 times a power of two that brings the largest finite one of a token's 32 channels
-// to [2^14, 2^15).  The exponent byte is the largest's, at least 14 so that the factor is a normal number.
 __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);
   return a <= 3.4028234663852886e38f ? a : 0.0f;
-}
-__device__ __forceinline__ uint32_t f16_exp(float largest) { return max(14u, __float_as_uint(largest) >> 23); }
-__device__ __forceinline__ float f16_factor(uint32_t e) { return __uint_as_float((268u - e) << 23); }  // 2^(141 - e)
-__device__ __forceinline__ float f16_back(uint32_t e) {                                               // 2^(e - 141)
-  return e > 14u ? __uint_as_float((e - 14u) << 23) : 5.877471754111438e-39f;
 }
 
 // h = act(g) u, in place of g; dg = dh u act'(g) and du = dh act(g), in place of g and u.  One loop for each gate, so
@@ -301,7 +290,7 @@ __device__ __forceinline__ void save_row_f16(const Params& P, const Prob& q, int
       if (n + 16 * i + 8 < q.cols) *reinterpret_cast<uint4*>(at + 16 * i + 8) = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
-  P.save_e[((int64_t)up * q.rows + row) * ((q.cols + 31) / 32) + n / 32] = (uint8_t)e;
+  *reinterpret_cast<uint32_t*>(P.save_e + ((int64_t)up * q.rows + row) * exp_groups(q.cols) + n / 8) = e * 0x01010101u;
 }
 // g and u of a chunk, loaded while the one before it is in work
 struct Ahead {
@@ -317,12 +306,12 @@ struct Ahead {
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      e[i] = live ? P.save_e[((int64_t)i * q.rows + row) * ((q.cols + 31) / 32) + n / 32] : 141u;
+      e[i] = live ? *reinterpret_cast<const uint32_t*>(P.save_e + ((int64_t)i * q.rows + row) * exp_groups(q.cols) + n / 8) : 0u;
   }
   __device__ __forceinline__ void get(int i, float (&o)[32]) const {
-    const float s = f16_back(e[i]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      const float s = f16_back(e[i] >> (8 * k) & 255u);
       const uint32_t w[4] = {v[4 * i + k].x, v[4 * i + k].y, v[4 * i + k].z, v[4 * i + k].w};
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
@@ -337,6 +326,8 @@ struct Ahead {
 template <int EPI, int IN, typename O>
 __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params P) {
   constexpr bool kGluE = EPI == kGlu;
+  using R = Ring<IN>;
+  constexpr int kSub = R::kSub, kStages = R::kStages, kStageBytes = R::kStageBytes;
   constexpr int kAM = kGluE ? 128 : 256;     // channels or columns of a tile in the columns form
   constexpr int kBN = kGluE ? 2 : 1;         // rows of B to a channel in the rows form
   constexpr int KE = IN == kI8 ? 128 : 64;   // k elements of a box
@@ -345,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + kSub * kBoxBytes;  // of stage 0
+  const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + R::kB;  // of stage 0
   const int warp = warp_id(), lane = lane_id();
   volatile int* abort_flag = &ctl.abort_flag;
   const uint32_t rank = cluster_ctarank();
@@ -396,33 +387,36 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         const int b_row = glu_rows ? t.n0 : t.n0 + mma_n(q, t, kGluE) / 2 * (int)rank;
         const int a_row = kGluE && !q.row ? t.m0 + 64 * (int)rank : t.m0 + 128 * (int)rank;
         const uint32_t b_bytes = (uint32_t)(q.tn / 2) * 128u;  // a whole box lands; rows past the tile are not used
-        const int kb = q.kb, a_mn = q.a_mn, b_atoms = q.b_mn ? q.tn / 128 : 0;
+        const int kb = q.kb, a_mn = q.a_mn, b_atoms = q.b_mn ? q.tn / 128 : 0, a_plane = q.a_plane, b_plane = q.b_plane;
         const CUtensorMap *ma = P.a[t.p], *mb = glu_rows ? P.b[t.p] + rank : P.b[t.p];
-        BoxAt<IN> at(q, t.box0);
+        BoxAt at(q, t.box0);
         for (int b = t.box0; b < t.box1; b += kSub) {
           if (!mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, P.err)) { ok = false; break; }
           const uint32_t fb0 = mapa_shared(smem_u32(&ctl.full[s]), 0);
           const int nb = min(kSub, t.box1 - b);
           if (rank == 0)
-            mbar_arrive_expect_tx(smem_u32(&ctl.full[s]), 2u * (uint32_t)nb * ((uint32_t)kBoxBytes + b_bytes));
+            mbar_arrive_expect_tx(smem_u32(&ctl.full[s]), 2u * (uint32_t)(nb * R::kPlanes) * ((uint32_t)kBoxBytes + b_bytes));
           for (int h = 0; h < nb; ++h, at.next(kb)) {
-            const uint32_t da = smem_a + s * kStageBytes + h * kBoxBytes, db = smem_b + s * kStageBytes + h * kBoxBytes;
-            const int pa = IN == kF32 ? plane_a(at.term) * q.a_plane : 0, pb = IN == kF32 ? plane_b(at.term) * q.b_plane : 0;
             const int kx = at.k * KE;
-            if (kGluE && !glu_rows) {
-              tma_load_2d_pair(da, ma, fb0, kx, a_row + pa);
-              tma_load_2d_pair(da + 8192, ma + 1, fb0, kx, a_row + pa);
-            } else if (a_mn) {
-              tma_load_2d_pair(da, ma + at.seg, fb0, a_row, kx + pa);
-              tma_load_2d_pair(da + 8192, ma + at.seg, fb0, a_row + 64, kx + pa);
-            } else {
-              tma_load_2d_pair(da, ma + at.seg, fb0, kx, a_row + pa);
-            }
-            if (b_atoms) {
-              tma_load_2d_pair(db, mb + at.seg, fb0, b_row, kx + pb);
-              if (b_atoms > 1) tma_load_2d_pair(db + 8192, mb + at.seg, fb0, b_row + 64, kx + pb);
-            } else {
-              tma_load_2d_pair(db, mb + at.seg, fb0, kx, b_row + pb);
+#pragma unroll
+            for (int pl = 0; pl < R::kPlanes; ++pl) {
+              const uint32_t da = smem_a + s * kStageBytes + (h + pl) * kBoxBytes, db = smem_b + s * kStageBytes + (h + pl) * R::kBBytes;
+              const int pa = pl * a_plane, pb = pl * b_plane;
+              if (kGluE && !glu_rows) {
+                tma_load_2d_pair(da, ma, fb0, kx, a_row + pa);
+                tma_load_2d_pair(da + 8192, ma + 1, fb0, kx, a_row + pa);
+              } else if (a_mn) {
+                tma_load_2d_pair(da, ma + at.seg, fb0, a_row, kx + pa);
+                tma_load_2d_pair(da + 8192, ma + at.seg, fb0, a_row + 64, kx + pa);
+              } else {
+                tma_load_2d_pair(da, ma + at.seg, fb0, kx, a_row + pa);
+              }
+              if (b_atoms) {
+                tma_load_2d_pair(db, mb + at.seg, fb0, b_row, kx + pb);
+                if (b_atoms > 1) tma_load_2d_pair(db + 8192, mb + at.seg, fb0, b_row + 64, kx + pb);
+              } else {
+                tma_load_2d_pair(db, mb + at.seg, fb0, kx, b_row + pb);
+              }
             }
           }
           pending[s] = (int)ph;
@@ -439,56 +433,68 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       int s = 0, it = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int unit = unit0; ok && unit < P.total; unit += units, ++it) {
+      for (int unit = unit0; ok && unit < P.total; unit += units) {
         const Tile t = decode(P, unit, kAM, kBN);
         const Prob& q = P.prob[t.p];
-        const int acc = it & 1;
         // D f32 (1) or s32 (2); A, B bf16 (1) or signed 8-bit (1); majors; N; M = 256
         const uint32_t idesc = ((IN == kI8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)q.a_mn << 15) |
                                ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n(q, t, kGluE) >> 3) << 17) | (16u << 24);
-        if (!mbar_wait(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem_base + (uint32_t)(acc * 256);
         // descriptors but for the stage, and their steps of one MMA (in 16 bytes: 2 KB or 32 bytes)
         const uint64_t ad0 = q.a_mn ? sw128_mnmajor_desc(smem_a) : sw128_kmajor_desc(smem_a);
         const uint64_t bd0 = q.b_mn ? sw128_mnmajor_desc(smem_b) : sw128_kmajor_desc(smem_b);
         const uint64_t astep = q.a_mn ? 128u : 2u, bstep = q.b_mn ? 128u : 2u;
         const int kb = q.kb, last_steps = (q.K - (kb - 1) * KE + KS - 1) / KS;
-        uint32_t used0 = 0u, used1 = 0u;
-        BoxAt<IN> at(q, t.box0);
-        for (int b = t.box0; b < t.box1; b += kSub) {
-          if (!mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, P.err)) { ok = false; break; }
-          tc_fence_after();
-          const int nb = min(kSub, t.box1 - b);
-#pragma unroll
-          for (int h = 0; h < kSub; ++h) {
-            if (h < nb) {
-              const uint64_t off = (uint64_t)((s * kStageBytes + h * kBoxBytes) >> 4);
-              const uint64_t ad = ad0 + off, bd = bd0 + off;
-              const int steps = at.k == kb - 1 ? last_steps : 4;
-              const bool corr = IN == kF32 && at.term != 0;
-              const uint32_t dd = corr ? d + 128u : d;
-              uint32_t used = corr ? used1 : used0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (i < steps) {
-                  if constexpr (IN == kI8) umma_i8_pair(dd, ad + astep * i, bd + bstep * i, idesc, used);
-                  else umma_f16_pair(dd, ad + astep * i, bd + bstep * i, idesc, used);
-                  used = 1u;
-                }
-              if (corr) used1 = 1u;
-              else used0 = 1u;
-              at.next(kb);
-            }
+        BoxAt at(q, t.box0);
+        // an accumulator takes the whole tile, kF32: a chunk of it
+        for (int c0 = t.box0; ok && c0 < t.box1; ++it) {
+          const int c1 = IN == kF32 ? min(t.box1, c0 + R::kChunk) : t.box1;
+          const int acc = it & 1;
+          if (!mbar_wait(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
+            ok = false;
+            break;
           }
-          umma_commit_pair_both(smem_u32(&ctl.empty[s]));
-          if (++s == kStages) { s = 0; ph ^= 1u; }
+          tc_fence_after();
+          const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+          uint32_t used = 0u;
+          for (int b = c0; b < c1; b += kSub) {
+            if (!mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, P.err)) { ok = false; break; }
+            tc_fence_after();
+            const int nb = min(kSub, c1 - b);
+#pragma unroll
+            for (int h = 0; h < kSub; ++h) {
+              if (h < nb) {
+                const uint64_t ad = ad0 + (uint64_t)((s * kStageBytes + h * kBoxBytes) >> 4);
+                const uint64_t bd = bd0 + (uint64_t)((s * kStageBytes + h * R::kBBytes) >> 4);
+                const int steps = at.k == kb - 1 ? last_steps : 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (i < steps) {
+                    const uint64_t ai = ad + astep * i, bi = bd + bstep * i;
+                    if constexpr (IN == kI8) {
+                      umma_i8_pair(d, ai, bi, idesc, used);
+                    } else {
+                      umma_f16_pair(d, ai, bi, idesc, used);
+                      if constexpr (IN == kF32) {
+                        constexpr uint64_t PA = kBoxBytes >> 4, PB = R::kBBytes >> 4;
+                        umma_f16_pair(d + 128u, ai, bi + PB, idesc, used);
+                        umma_f16_pair(d + 128u, ai + PA, bi, idesc, 1u);
+                        umma_f16_pair(d + 128u, ai, bi + 2 * PB, idesc, 1u);
+                        umma_f16_pair(d + 128u, ai + PA, bi + PB, idesc, 1u);
+                        umma_f16_pair(d + 128u, ai + 2 * PA, bi, idesc, 1u);
+                      }
+                    }
+                    used = 1u;
+                  }
+                at.next(kb);
+              }
+            }
+            umma_commit_pair_both(smem_u32(&ctl.empty[s]));
+            if (++s == kStages) { s = 0; ph ^= 1u; }
+          }
+          if (!ok) break;
+          umma_commit_pair_both(smem_u32(&ctl.tmem_full[acc]));
+          c0 = c1;
         }
-        if (!ok) break;
-        umma_commit_pair_both(smem_u32(&ctl.tmem_full[acc]));
       }
       if (!ok) {  // every MMA issued has completed before TMEM is freed
         umma_commit_pair(mapa_shared(smem_u32(&ctl.mma_done), 0));
@@ -498,20 +504,49 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   } else {
     // ---------------- epilogue
     const int q4 = warp & 3, ew = warp - 2, eh = ew >> 2;
-    uint8_t* stg = smem + kStages * kStageBytes + ew * kStgBytes;
+    uint8_t* stg = smem + kRingBytes + ew * kStgBytes;
     const int pair_id = 1 + (ew & 1) + 2 * eh;  // barrier of an exchange
     int it = 0, xb = 0;
     Ahead ahead;
-    for (int unit = unit0; unit < P.total; unit += units, ++it) {
+    for (int unit = unit0; unit < P.total; unit += units) {
       const Tile t = decode(P, unit, kAM, kBN);
       const Prob& q = P.prob[t.p];
-      const int acc = it & 1;
       const int64_t lrow = t.m0 + 128 * (int)rank + 32 * q4 + lane;  // rows form: this lane's output row
       if constexpr (EPI == kDGlu && IN == kBf16)
         if (q.row) ahead.load(P, q, lrow, t.n0 + 32 * eh, t.n0 + t.nval);
+      const int ncol = mma_n(q, t, kGluE);
+      uint32_t taddr = 0;
+      float fs[2][32];  // kF32: the sums of this warp's two chunks of columns
+      if constexpr (IN == kF32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) fs[0][j] = fs[1][j] = 0.0f;
+      }
       int w_ok = 1;
-      if (lane == 0) w_ok = mbar_wait(smem_u32(&ctl.tmem_full[acc]), (uint32_t)((it >> 1) & 1), abort_flag, P.err) ? 1 : 0;
-      w_ok = __shfl_sync(0xffffffffu, w_ok, 0);
+      for (int c0 = t.box0; c0 < t.box1; c0 += IN == kF32 ? R::kChunk : t.box1 - t.box0) {
+        const int acc = it & 1;
+        w_ok = 1;
+        if (lane == 0) w_ok = mbar_wait(smem_u32(&ctl.tmem_full[acc]), (uint32_t)((it >> 1) & 1), abort_flag, P.err) ? 1 : 0;
+        w_ok = __shfl_sync(0xffffffffu, w_ok, 0);
+        if (!w_ok) break;
+        tc_fence_after();
+        taddr = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * 256);
+        if constexpr (IN == kF32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (32 * eh + 64 * h < ncol) {
+              uint32_t v[32], w[32];
+              tmem_ld32(taddr + 32 * eh + 64 * h, v);
+              tmem_ld32(taddr + 128 + 32 * eh + 64 * h, w);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) fs[h][j] += __uint_as_float(v[j]) + __uint_as_float(w[j]);
+            }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&ctl.tmem_empty[acc]), 0));
+          ++it;
+        }
+      }
       if constexpr (kGluE) {
         // the two warps of an exchange go on or leave together
         if (lane == 0) ctl.pair_ok[ew] = w_ok;
@@ -519,19 +554,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         w_ok = *reinterpret_cast<volatile int*>(&ctl.pair_ok[ew ^ 2]) & w_ok;
       }
       if (!w_ok) break;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * 256);
-      const int ncol = mma_n(q, t, kGluE);
       // 32 columns of the accumulator from c on
       auto chunk = [&](int c, uint32_t (&v)[32]) {
-        tmem_ld32(taddr + c, v);
         if constexpr (IN == kF32) {
-          uint32_t w[32];
-          tmem_ld32(taddr + 128 + c, w);
-          tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(c >= 64 ? fs[1][j] : fs[0][j]);
         } else {
+          tmem_ld32(taddr + c, v);
           tmem_wait_ld();
         }
       };
@@ -737,7 +766,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           if constexpr (kGluE) {
             if (P.save_g != nullptr) {
               if constexpr (IN == kBf16) {
-                const int groups = (q.cols + 31) / 32;
                 uint32_t el = 0;  // lane j's: the exponent of token j
                 __half* at = reinterpret_cast<__half*>(up ? P.save_u : P.save_g) + tok * q.ldo + ch;
 #pragma unroll
@@ -748,7 +776,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
                   if (ch < q.cols && c + j < t.nval) at[j * q.ldo] = __float2half_rn(v[j] * f16_factor(e));
                 }
                 if (c + lane < t.nval && (ch & ~31) < q.cols)
-                  P.save_e[((int64_t)up * q.rows + tok + lane) * groups + ch / 32] = (uint8_t)el;
+                  *reinterpret_cast<uint32_t*>(P.save_e + ((int64_t)up * q.rows + tok + lane) * exp_groups(q.cols) +
+                                               (ch & ~31) / 8) = el * 0x01010101u;
               } else if (ch < q.cols) {
                 float* at = reinterpret_cast<float*>(up ? P.save_u : P.save_g) + tok * q.ldo + ch;
 #pragma unroll
@@ -758,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             }
             // two buffers, so that one barrier a chunk is enough
             float* mine_x = reinterpret_cast<float*>(stg) + xb * 512;
-            float* other_x = reinterpret_cast<float*>(smem + kStages * kStageBytes + (ew ^ 2) * kStgBytes) + xb * 512;
+            float* other_x = reinterpret_cast<float*>(smem + kRingBytes + (ew ^ 2) * kStgBytes) + xb * 512;
             xb ^= 1;
 #pragma unroll
             for (int j = 0; j < 16; ++j) mine_x[j * 32 + lane] = up ? v[j] : v[16 + j];
@@ -777,12 +806,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           } else if constexpr (EPI == kDGlu) {
             float g[32], u[32];
             if constexpr (IN == kBf16) {
-              const int groups = (q.cols + 31) / 32;
-              float sc[2] = {0.0f, 0.0f};  // lane j's: the factors of token j
+              uint32_t ex[2] = {0u, 0u};  // lane j's: the exponents of token j
               if (c + lane < t.nval && (ch & ~31) < q.cols) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                  sc[i] = f16_back(P.save_e[((int64_t)i * q.rows + tok + lane) * groups + ch / 32]);
+                  ex[i] = *reinterpret_cast<const uint32_t*>(P.save_e + ((int64_t)i * q.rows + tok + lane) * exp_groups(q.cols) +
+                                                             (ch & ~31) / 8);
               }
               const __half *pg = reinterpret_cast<const __half*>(P.save_g), *pu = reinterpret_cast<const __half*>(P.save_u);
 #pragma unroll
@@ -794,8 +823,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               }
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                g[j] *= __shfl_sync(0xffffffffu, sc[0], j);
-                u[j] *= __shfl_sync(0xffffffffu, sc[1], j);
+                // of this lane's eight channels
+                g[j] *= f16_back(__shfl_sync(0xffffffffu, ex[0], j) >> (lane & 24) & 255u);
+                u[j] *= f16_back(__shfl_sync(0xffffffffu, ex[1], j) >> (lane & 24) & 255u);
               }
             } else {
               const float *pg = reinterpret_cast<const float*>(P.save_g), *pu = reinterpret_cast<const float*>(P.save_u);
@@ -819,9 +849,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&ctl.tmem_empty[acc]), 0));
+      if constexpr (IN != kF32) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&ctl.tmem_empty[it & 1]), 0));
+        ++it;
+      }
     }
   }
 
@@ -960,13 +993,13 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     q.row = s.N > 128 && q.vec;
     q.nseg = glu ? 1 : s.nseg;
     q.kb = ceil_div(s.K, ke);
-    const int terms = f32 ? 6 : 1;
-    q.boxes = q.nseg * terms * q.kb;
+    q.boxes = q.nseg * q.kb;
     q.a_mn = q.row ? s.b[0].mn : s.a[0].mn;
     q.b_mn = q.row ? s.a[0].mn : s.b[0].mn;
     // Tile width and k splits by an estimate of the time: waves of tiles, each its boxes' time and a fixed part.  A box
     // costs mostly its 256 rows of A: 256 rows of B 1, 192 0.83, 128 0.75 of the time (2048 x 5632).
-    const int whole = f32 ? 6 : 2;  // boxes that stay together: all terms of a slice, whole stages
+    const int whole = f32 ? 1 : 2;  // boxes of a stage
+    const double slice = f32 ? 3.0 : 1.0;  // a box's time against 16 bits'
     double best = -1;
     auto consider = [&](int tn, int splits) {
       const int per_tile = q.row && glu ? tn / 2 : tn;
@@ -976,7 +1009,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
       const int per = ceil_div(ceil_div(q.boxes, splits), whole) * whole;
       splits = ceil_div(q.boxes, per);
       if (splits > 1 && tiles * splits > 2 * pairs) return;  // bounds the partial tiles
-      const double box = 0.2 + 0.1 * tn / 128.0;                     // us
+      const double box = slice * (0.2 + 0.1 * tn / 128.0);           // us
       const double fixed = 1.0 + (splits > 1 ? 1.5 + 0.5 * splits * tn / 64.0 : 0.0);
       const double waves = j.nprob == 1 ? (double)ceil_div(tiles * splits, pairs) : std::max(1.0, (double)(tiles * splits) / pairs);
       const double cost = waves * (box * per + fixed) + 0.02 * tn / 256.0 * per;
@@ -986,7 +1019,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
         q.splits = splits; q.per = per;
       }
     };
-    for (int splits = 1; splits <= (j.nprob == 1 ? 8 : 1) && (splits == 1 || q.boxes >= 4 * whole * splits); ++splits) {
+    for (int splits = 1; splits <= (j.nprob == 1 ? 8 : 1) && (splits == 1 || q.boxes >= (f32 ? 2 : 8) * splits); ++splits) {
       if (q.row || q.b_mn) {
         // a gated tile's gate and up chunks of 32 belong to one warp only from 64 channels on
         for (int tn = most; tn >= (q.b_mn || glu ? 128 : 64); tn /= 2) consider(tn, splits);
@@ -1004,9 +1037,9 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     for (int i = 0; i < j.nprob; ++i) work += time(P.prob[i]) * P.prob[i].tiles_m * P.prob[i].tiles_n;
     for (int i = 0; i < j.nprob; ++i) {
       Prob& q = P.prob[i];
-      const int whole = f32 ? 6 : 2;
+      const int whole = f32 ? 1 : 2;
       int want = (int)std::min(8.0, time(q) / (0.6 * work / pairs));
-      want = std::min(want, q.boxes / (4 * whole));
+      want = std::min(want, q.boxes / (f32 ? 2 : 8));
       if (want < 2 || (int64_t)q.tiles_m * q.tiles_n * want > 2 * pairs) continue;
       q.per = ceil_div(ceil_div(q.boxes, want), whole) * whole;
       q.splits = ceil_div(q.boxes, q.per);

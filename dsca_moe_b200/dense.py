@@ -26,23 +26,25 @@ __all__ = ["GatedFFN", "Int8Weight", "check_dense", "gated_ffn", "gated_ffn_int8
 
 _ACTS = {"silu": L.GATE_SILU, "gelu": L.GATE_GELU, "relu": L.GATE_RELU}
 _ERR: dict = {}
+_BF16 = torch.bfloat16
 
 
 def _err(dev) -> int:
     """Address of the device's error word (a wait inside a kernel that ran out records there)."""
-    t = _ERR.get(dev.index)
-    if t is None:
-        t = _ERR[dev.index] = torch.zeros(64, dtype=torch.int32, device=dev)
-    return t.data_ptr()
+    e = _ERR.get(dev.index)
+    if e is None:
+        t = torch.zeros(64, dtype=torch.int32, device=dev)
+        e = _ERR[dev.index] = (t.data_ptr(), t)
+    return e[0]
 
 
 def check_dense(device=None):
     """Raise if a dense block or 8-bit product on `device` recorded an error since the last check, which
     it clears (synchronises the current stream)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    t = _ERR.get(dev.index if dev.index is not None else torch.cuda.current_device())
-    if t is not None:
-        L.call_on(t.device, "dsca_check_error", t.data_ptr())
+    e = _ERR.get(dev.index if dev.index is not None else torch.cuda.current_device())
+    if e is not None:
+        L.call_on(e[1].device, "dsca_check_error", e[0])
 
 
 def _act(act: str) -> int:
@@ -68,6 +70,9 @@ def _rows(x, name: str, width: int | None = None):
 
 
 def _weight(w, name: str, out: int, inp: int, x) -> int:
+    """Row stride of a weight [out, inp] of x's type on x's device."""
+    if w.shape == (out, inp) and w.dtype is x.dtype and w.device == x.device and w.is_contiguous():
+        return inp
     if w.dim() != 2 or w.shape[0] != out or w.shape[1] != inp:
         raise ValueError(f"{name}: expected [{out}, {inp}], got {tuple(w.shape)}")
     if w.dtype != x.dtype or w.device != x.device:
@@ -91,39 +96,44 @@ def _workspace(name: str, args, dev):
 
 
 def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
+    """(y, the buffer with h and, with `save`, g and u)."""
     dev, dtype = x.device, x.dtype
     rows, d, inter, ld_x, ld_g, ld_u, ld_d = shapes
     y = torch.empty(x.shape, dtype=dtype, device=dev)
     if rows == 0:
-        return y, (None, None)
-    ld_h = (inter + 15) // 16 * 16  # rows on 32-byte sectors
-    h = torch.empty((rows, ld_h), dtype=dtype, device=dev)
-    gu, g, u, e = None, None, None, None
-    if save:
-        size = 2 if dtype == torch.bfloat16 else 4
-        step = rows * ld_h * size
-        gu = torch.empty(2 * step + (0 if size == 4 else 2 * rows * ((inter + 31) // 32)), dtype=torch.uint8, device=dev)
-        g = gu.data_ptr()
-        u, e = g + step, (g + 2 * step if size == 2 else None)
-    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h.data_ptr(), rows, d,
-                       inter, _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
-    ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
+        return y, None
+    ld_h, step, size = _saved(rows, inter, dtype)
+    buf = torch.empty(size if save else step, dtype=torch.uint8, device=dev)
+    h = buf.data_ptr()
+    g, u, e = (h + step, h + 2 * step, h + 3 * step) if save else (None, None, None)
+    a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h, rows, d, inter,
+                       _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
+    if rows > L.DENSE_FEW_TOKENS or dtype is not _BF16:
+        ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
-    return y, (h, gu)
+    return y, buf
+
+
+def _saved(rows: int, inter: int, dtype):
+    """(row stride, bytes of each of h, g and u, bytes in all with g's and u's exponents): rows on 32-byte sectors; g and u
+    take what h takes (fp16 codes beside bf16, fp32 beside fp32)."""
+    ld_h = (inter + 15) // 16 * 16
+    step = rows * ld_h * (2 if dtype is _BF16 else 4)
+    return ld_h, step, 3 * step + (8 * rows * ((inter + 31) // 32) if dtype is _BF16 else 0)
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, wd, act, shapes):
-        y, (h, gu) = _forward(x, wg, wu, wd, act, shapes, True)
+        y, buf = _forward(x, wg, wu, wd, act, shapes, True)
         ctx.act, ctx.shapes = act, shapes
-        ctx.save_for_backward(x, wg, wu, wd, h, gu)
+        ctx.save_for_backward(x, wg, wu, wd, buf)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, h, gu = ctx.saved_tensors
+        x, wg, wu, wd, buf = ctx.saved_tensors
         rows, d, inter, ld_x, ld_g, ld_u, ld_d = ctx.shapes
         dev, dtype = x.device, x.dtype
         need = ctx.needs_input_grad
@@ -131,28 +141,27 @@ class _GatedFFN(torch.autograd.Function):
         dwg = torch.empty((inter, d), dtype=dtype, device=dev) if need[1] else None
         dwu = torch.empty((inter, d), dtype=dtype, device=dev) if need[2] else None
         dwd = torch.empty((d, inter), dtype=dtype, device=dev) if need[3] else None
-        ptr = [None if t is None else t.data_ptr() for t in (dx, dwg, dwu, dwd)]
-        a = L.GatedFfnBackwardArgs()
-        a.dx, a.d_gate, a.d_up, a.d_down = ptr
-        a.rows, a.d, a.inter, a.dtype, a.act = rows, d, inter, _DTYPES[dtype], ctx.act
-        keep = ()
+        dx_p, dwg_p, dwu_p, dwd_p = [None if t is None else t.data_ptr() for t in (dx, dwg, dwu, dwd)]
         if rows:
-            try:
-                ld_dy = d if dy.is_contiguous() else _stride(dy, "dy", d)
-            except ValueError:  # a gradient may come in any strides (expanded, transposed)
-                dy, ld_dy = dy.contiguous(), d
-            ld_h = h.shape[1]
-            grads = torch.empty((2, rows, ld_h), dtype=dtype, device=dev)
-            a.x, a.w_gate, a.w_up, a.w_down, a.dy = (t.data_ptr() for t in (x, wg, wu, wd, dy))
-            step = rows * ld_h * (2 if dtype == torch.bfloat16 else 4)
-            a.h, a.g, a.u = h.data_ptr(), gu.data_ptr(), gu.data_ptr() + step
-            a.gu_exp = gu.data_ptr() + 2 * step
-            a.dg, a.du = grads.data_ptr(), grads.data_ptr() + rows * ld_h * grads.element_size()
-            a.ld_x, a.ld_gate, a.ld_up, a.ld_down, a.ld_dy, a.ld_h = ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h
-            a.err = _err(dev)
-            keep = (grads, _workspace("dsca_gated_ffn_backward_workspace", a, dev))
+            ld_dy = d
+            if not dy.is_contiguous():
+                try:
+                    ld_dy = _stride(dy, "dy", d)
+                except ValueError:  # a gradient may come in any strides (expanded, transposed)
+                    dy = dy.contiguous()
+            ld_h, step, _ = _saved(rows, inter, dtype)
+            grads = torch.empty(2 * step, dtype=torch.uint8, device=dev)
+            h, dg = buf.data_ptr(), grads.data_ptr()
+            a = L.GatedFfnBackwardArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), dy.data_ptr(), h + step,
+                                       h + 2 * step, h + 3 * step, h, dx_p, dwg_p, dwu_p, dwd_p, dg, dg + step, rows, d,
+                                       inter, _DTYPES[dtype], ctx.act, ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h, None, 0,
+                                       _err(dev))
+            ws = _workspace("dsca_gated_ffn_backward_workspace", a, dev)  # noqa: F841 - alive until the launch
+        else:
+            a = L.GatedFfnBackwardArgs()
+            a.dx, a.d_gate, a.d_up, a.d_down = dx_p, dwg_p, dwu_p, dwd_p
+            a.d, a.inter, a.dtype, a.act = d, inter, _DTYPES[dtype], ctx.act
         L.call_on(dev, "dsca_gated_ffn_backward", ctypes.byref(a))
-        del keep
         return dx, dwg, dwu, dwd, None, None
 
 
@@ -232,6 +241,13 @@ def pack_int8(weight: torch.Tensor) -> Int8Weight:
 def _int8_weight(w, name: str, dev, inp: int, out: int | None = None) -> int:
     """Row stride of an Int8Weight."""
     q, s = w
+    shape = q.shape
+    if q.dtype is torch.int8 and len(shape) == 2 and shape[1] == inp and (out is None or shape[0] == out) \
+            and q.device == dev and s.device == dev and s.dtype is torch.float32 and s.shape == shape[:1] \
+            and s.is_contiguous() and shape[0] > 1:
+        ld, last = q.stride()
+        if (last == 1 or inp == 1) and ld >= inp and ld % 16 == 0 and q.data_ptr() % 16 == 0:
+            return ld
     if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] != inp or (out is not None and q.shape[0] != out):
         raise ValueError(f"{name}: expected an Int8Weight [{'out' if out is None else out}, {inp}], got "
                          f"{q.dtype} {tuple(q.shape)}")
@@ -274,7 +290,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     if k > _INT8_MAX_K:
         raise ValueError(f"sums of {k} products exceed {_INT8_MAX_K}")
     ld_w = _int8_weight(weight, "weight", dev, k)
-    n = weight.q.shape[0]
+    n = weight[0].shape[0]
     if bias is not None and (bias.dtype != dtype or bias.device != dev or tuple(bias.shape) != (n,)
                              or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous [{n}] tensor of y's type on x's device")
@@ -289,19 +305,18 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     y = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
     if rows == 0:
         return y
-    a = L.Int8LinearArgs()
     if given:
-        a.q, a.scale, a.ld_q = x.data_ptr(), x_scale.data_ptr(), ld_x
+        x_p, q_p, s_p, ld_q = None, x.data_ptr(), x_scale.data_ptr(), ld_x
     else:
         ld_q = (k + 15) // 16 * 16
         buf = torch.empty(rows * (ld_q + 4), dtype=torch.uint8, device=dev)
-        a.x, a.ld_x, a.ld_q = x.data_ptr(), ld_x, ld_q
-        a.q, a.scale = buf.data_ptr(), buf.data_ptr() + rows * ld_q
-    a.w, a.w_scale, a.ld_w = weight.q.data_ptr(), weight.scale.data_ptr(), ld_w
-    a.bias = None if bias is None else bias.data_ptr()
-    a.y, a.ld_y = y.data_ptr(), n
-    a.rows, a.k, a.n, a.dtype, a.err = rows, k, n, dt, _err(dev)
-    ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
+        x_p, q_p = x.data_ptr(), buf.data_ptr()
+        s_p = q_p + rows * ld_q
+    a = L.Int8LinearArgs(x_p, q_p, s_p, weight[0].data_ptr(), weight[1].data_ptr(),
+                         None if bias is None else bias.data_ptr(), y.data_ptr(), rows, k, n, dt, ld_x, ld_q, ld_w, n,
+                         None, 0, _err(dev))
+    if rows > L.DENSE_FEW_TOKENS:
+        ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_int8_linear", ctypes.byref(a))
     return y
 
@@ -320,26 +335,25 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     inter = w_gate[0].shape[0]
     if max(d, inter) > _INT8_MAX_K:
         raise ValueError(f"sums of {max(d, inter)} products exceed {_INT8_MAX_K}")
-    a = L.GatedFfnInt8Args()
-    a.ld_gate = _int8_weight(w_gate, "w_gate", dev, d)
-    a.ld_up = _int8_weight(w_up, "w_up", dev, d, inter)
-    a.ld_down = _int8_weight(w_down, "w_down", dev, inter, d)
+    ld_gate = _int8_weight(w_gate, "w_gate", dev, d)
+    ld_up = _int8_weight(w_up, "w_up", dev, d, inter)
+    ld_down = _int8_weight(w_down, "w_down", dev, inter, d)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     if rows == 0:
         return y
     ld_q, ld_hq = (d + 15) // 16 * 16, (inter + 15) // 16 * 16
     # one buffer: h, the two sets of codes, the two sets of scales
     buf = torch.empty(rows * (5 * ld_hq + ld_q + 8), dtype=torch.uint8, device=dev)
-    p = buf.data_ptr()
-    a.h, a.hq, a.q = p, p + rows * 4 * ld_hq, p + rows * 5 * ld_hq
-    a.scale = a.q + rows * ld_q
-    a.h_scale = a.scale + 4 * rows
-    a.x, a.y = x.data_ptr(), y.data_ptr()
-    a.w_gate, a.w_up, a.w_down = w_gate[0].data_ptr(), w_up[0].data_ptr(), w_down[0].data_ptr()
-    a.gate_scale, a.up_scale, a.down_scale = w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr()
-    a.rows, a.d, a.inter, a.dtype, a.act, a.err = rows, d, inter, dt, code, _err(dev)
-    a.ld_x, a.ld_q, a.ld_h, a.ld_hq, a.ld_y = ld_x, ld_q, ld_hq, ld_hq, d
-    ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
+    h = buf.data_ptr()
+    hq = h + rows * 4 * ld_hq
+    q = hq + rows * ld_hq
+    scale = q + rows * ld_q
+    a = L.GatedFfnInt8Args(x.data_ptr(), q, scale, w_gate[0].data_ptr(), w_up[0].data_ptr(), w_down[0].data_ptr(),
+                           w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr(), h, hq, scale + 4 * rows,
+                           y.data_ptr(), rows, d, inter, dt, code, ld_x, ld_q, ld_gate, ld_up, ld_down, ld_hq, ld_hq, d,
+                           None, 0, _err(dev))
+    if rows > L.DENSE_FEW_TOKENS:
+        ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
     return y
 

@@ -27,11 +27,13 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 /* Largest width (d, inter, k, n) and number of rows of these entry points. */
 #define DSCA_DENSE_MAX_DIM 1048576
 #define DSCA_DENSE_MAX_ROWS 16777216
+/* Forward calls in bf16 or 8-bit integers need no workspace for at most this many rows. */
+#define DSCA_DENSE_FEW_TOKENS 16
 
 /*
  * g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T; sums in fp32, h and y rounded to dtype.  g and u
  * are written when given (both or neither), for the backward pass: in fp32 for DSCA_F32; for DSCA_BF16 as
- * fp16 times a power of two for every 32 channels of a token, whose exponents gu_exp takes.  h is a work area [rows, ld_h] that the backward pass reads as well.
+ * fp16 times a power of two for a few channels of a token, whose exponents gu_exp takes.  h is a work area [rows, ld_h] that the backward pass reads as well.
  */
 typedef struct {
   const void* x;        /* [rows, d], dtype */
@@ -41,7 +43,7 @@ typedef struct {
   void* y;              /* [rows, d] */
   void* g;              /* [rows, ld_h] fp32 or fp16, or NULL */
   void* u;
-  uint8_t* gu_exp;      /* [2, rows, ceil(inter / 32)]; with DSCA_BF16 and g */
+  uint8_t* gu_exp;      /* [2, rows, 4 * ceil(inter / 32)], 4-byte aligned; with DSCA_BF16 and g */
   void* h;              /* [rows, ld_h] */
   int rows, d, inter;
   int dtype;            /* DSCA_BF16, DSCA_F32 */

@@ -28,7 +28,8 @@ def test_symbols_and_constants(lib):
     assert set(re.findall(r"\b(dsca_[a-z0-9_]+)\s*\(", src)) == set(L.EXPORTED_DENSE)
     for name in L.EXPORTED_DENSE:
         assert hasattr(lib, name), name
-    for c, v in (("DSCA_DENSE_MAX_DIM", L.DENSE_MAX_DIM), ("DSCA_DENSE_MAX_ROWS", L.DENSE_MAX_ROWS)):
+    for c, v in (("DSCA_DENSE_MAX_DIM", L.DENSE_MAX_DIM), ("DSCA_DENSE_MAX_ROWS", L.DENSE_MAX_ROWS),
+                 ("DSCA_DENSE_FEW_TOKENS", L.DENSE_FEW_TOKENS)):
         assert int(re.search(rf"#define {c} (\d+)", src).group(1)) == v
     assert set(re.findall(r"\}\s*(dsca_[a-z0-9_]+)\s*;", src)) == set(STRUCTS)
 
