@@ -3,9 +3,7 @@
 //
 // Why the exact quotient and not x / scale: the scale is rounded, so values half way between two
 // codes (x = max|x| / 2 is 63.5) would fall to either side by the row.  A product with 127 / max|x| finds the code of
-// all values but those close to a tie, which take the quotient: 127 x is exact in fp32 for a bf16 x and IEEE
-// division rounds the exact quotient, which is never within 2^-9 of a tie without being one; for an fp32 x it is
-// taken in 64 bits.
+// all values but those close to a tie, which compare 127 x with the border times max|x|, exactly.
 //
 // Bound by DRAM from a few thousand rows on: a row is read once into registers (up to 8192 values;
 // longer rows are read a second time from L2).
@@ -23,139 +21,183 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// The code of x in a row whose largest magnitude is amax, by division in 64 bits.
+__device__ __forceinline__ float divided_code(float x, float amax) { return (float)rint(127.0 * (double)x / (double)amax); }
+
+// The code next to r that x has, r being one of the two integers around 127 x / amax: the sign of 127 x - h amax at the
+// border h half way towards the other one decides.  Both products are exact: in fp32 for bf16 values (15 and 16 bits), in
+// 64 bits for fp32 ones.
 template <typename T>
-__device__ __forceinline__ float value(const T* p, int64_t i) {
-  if constexpr (sizeof(T) == 2) return __bfloat162float(p[i]);
-  else return p[i];
+__device__ __forceinline__ float settled(float r, float toward, float x, float amax) {
+  const float s = copysignf(1.0f, toward), h = r + 0.5f * s;
+  float over;  // beyond the border (> 0) or on it
+  if constexpr (sizeof(T) == 2) {
+    over = fmaf(-h, amax, 127.0f * x) * s;
+  } else {
+    const double e = fma(-(double)h, (double)amax, 127.0 * (double)x);
+    over = e > 0.0 ? s : e < 0.0 ? -s : 0.0f;
+  }
+  const bool odd = (int)r & 1;
+  return over > 0.0f || (over == 0.0f && odd) ? r + s : r;
 }
 
-// The exact code of x in a row whose largest magnitude is amax (> 0).
+// Eight codes.  inv is 127 / amax to 2^-23: a product with it is off by less than 2^-16, so only values that close to
+// a tie need the exact comparison (where one of the eight does, all take it: ties are common among bf16 values,
+// whose quotients have few bits).  Adding 1.5 * 2^23 rounds to an integer, whose low byte is the code.
 template <typename T>
-__device__ __noinline__ float exact_code(float x, float amax) {
-  if (sizeof(T) == 2 && amax < 1e36f && amax > 1e-30f) return rintf(__fdiv_rn(__fmul_rn(127.0f, x), amax));
-  return (float)rint(127.0 * (double)x / (double)amax);
-}
-
-// Four codes in a word.  inv is 127 / amax to 2^-23: a product with it is off by less than 2^-16, so only values
-// that close to a tie need the exact quotient.  Adding 1.5 * 2^23 rounds to an integer, whose low byte is the code.
-template <typename T>
-__device__ __forceinline__ uint32_t codes4(const float* x, float amax, float inv) {
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float amax, float inv) {
   constexpr float kRound = 12582912.0f;
-  uint32_t b[4];
+  uint32_t b[8];
+  float far = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float v = x[i] * inv;
-    float r = v + kRound;
-    if (fabsf(v - (r - kRound)) > 0.49996f) r = exact_code<T>(x[i], amax) + kRound;
+  for (int i = 0; i < 8; ++i) {
+    const float v = x[i] * inv, r = v + kRound;
+    far = fmaxf(far, fabsf(v - (r - kRound)));
     b[i] = __float_as_uint(r);
   }
-  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  if (far > 0.49996f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float r = __uint_as_float(b[i]) - kRound;
+      b[i] = __float_as_uint(settled<T>(r, x[i] * inv - r, x[i], amax) + kRound);
+    }
+  }
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
-// TPR threads a row, CH chunks of eight values a thread in registers (CH = 0: longer rows).
-template <typename T, int TPR, int CH, bool kVec>
-__global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a) {
-  __shared__ float red[8];
-  constexpr int kRows = 256 / TPR;
-  const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * kRows + sub;
-  const bool live = row < a.rows;
-  pdl_launch_dependents();  // a product that follows asks for its first weights meanwhile
-  pdl_wait();
-  const T* x = reinterpret_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x;
-  float v[CH > 0 ? CH : 1][8];
-  float m = 0.0f;
-  auto load = [&](int c, float (&o)[8]) {
-    if (kVec && c * 8 + 8 <= a.k) {
-      if constexpr (sizeof(T) == 2) {
-        const uint4 u = *reinterpret_cast<const uint4*>(x + c * 8);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight consecutive values as they lie in memory.
+template <typename T>
+struct Raw {
+  static constexpr int W = sizeof(T) * 2;  // words
+  uint32_t w[W];
+  template <bool kVec>
+  __device__ __forceinline__ void load(const T* x, int c, int k) {
+    if (kVec && c * 8 + 8 <= k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[2 * i] = __uint_as_float(w[i] << 16);
-          o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 f = *reinterpret_cast<const float4*>(x + c * 8 + 4 * i);
-          o[4 * i] = f.x; o[4 * i + 1] = f.y; o[4 * i + 2] = f.z; o[4 * i + 3] = f.w;
-        }
+      for (int i = 0; i < W / 4; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(x + c * 8) + 4 * i);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = c * 8 + i < a.k ? value(x, c * 8 + i) : 0.0f;
+      for (int i = 0; i < W; ++i) w[i] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c * 8 + i < k) {
+          if constexpr (sizeof(T) == 2) w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[c * 8 + i] << (16 * (i % 2));
+          else w[i] = __float_as_uint(x[c * 8 + i]);
+        }
     }
-  };
-  const int chunks = (int)((a.ld_q) / 8);  // those past k are zeros
-  if (live) {
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 2) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return __uint_as_float(w[i]);
+  }
+};
+
+// TPR threads a row, CH chunks of eight values a thread in registers (CH = 0: longer rows, read twice).  A CTA goes
+// through rows with the next one's values on their way while one is turned into codes: with a CTA a row and no
+// such overlap, 16384 x 5632 bf16 took 107 us.
+template <typename T, int TPR, int CH, bool kVec>
+__global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a) {
+  __shared__ float red[2][8];
+  constexpr int kRows = 256 / TPR, N = CH > 0 ? CH : 1;
+  const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
+  const int chunks = (int)(a.ld_q / 8);  // those past k are zeros
+  const T* base = reinterpret_cast<const T*>(a.x);
+  pdl_launch_dependents();  // a product that follows asks for its first weights meanwhile
+  pdl_wait();
+  Raw<T> next[N];
+  auto fetch = [&](int64_t row) {
     if constexpr (CH > 0) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int c = i * TPR + tid;
-        if (c < chunks) {
-          load(c, v[i]);
+        if (row < a.rows && c < chunks) next[i].template load<kVec>(base + row * a.ld_x, c, a.k);
+      }
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + sub;
+  fetch(row);
+  // whole CTAs go round together (the reduction's barrier)
+  for (int64_t first = (int64_t)blockIdx.x * kRows, it = 0; first < a.rows; first += step, row += step, ++it) {
+    const bool live = row < a.rows;
+    const T* x = base + (live ? row : 0) * a.ld_x;
+    Raw<T> v[N];
+    float m = 0.0f;
+    if constexpr (CH > 0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[i][e]));
+      for (int i = 0; i < N; ++i) {
+        v[i] = next[i];
+        if (live && i * TPR + tid < chunks) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[i].get(e)));
         }
+      }
+      fetch(row + step);
+    } else if (live) {
+      for (int c = tid; c < chunks; c += TPR) {
+        v[0].template load<kVec>(x, c, a.k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[0].get(e)));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if constexpr (TPR > 32) {
+      float* r = red[it & 1];  // two, so that one barrier a row is enough
+      if (threadIdx.x % 32 == 0) r[threadIdx.x / 32] = m;
+      __syncthreads();
+      m = r[sub * (TPR / 32)];
+#pragma unroll
+      for (int i = 1; i < TPR / 32; ++i) m = max_nan(m, r[sub * (TPR / 32) + i]);
+    }
+    if (!live) continue;
+    if (tid == 0) a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
+    // codes mean nothing in a row that is not finite: zeros
+    const bool usable = m > 0.0f && m < INFINITY;
+    const bool ends = m < 1e-30f || m > 1e36f;  // 127 / m or 127 x leaves fp32's normal numbers
+    const float inv = usable && !ends ? __fdiv_rn(127.0f, m) : 0.0f;
+    auto store = [&](int c, const Raw<T>& raw) {
+      uint2 w = make_uint2(0u, 0u);
+      if (usable) {
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = raw.get(e);
+        if (!ends) {
+          w = codes8<T>(o, m, inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t byte = (uint32_t)((int)divided_code(o[e], m) & 255) << (8 * (e % 4));
+            if (e < 4) w.x |= byte;
+            else w.y |= byte;
+          }
+        }
+      }
+      *reinterpret_cast<uint2*>(a.q + row * a.ld_q + c * 8) = w;
+    };
+    if constexpr (CH > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = i * TPR + tid;
+        if (c < chunks) store(c, v[i]);
       }
     } else {
       for (int c = tid; c < chunks; c += TPR) {
-        load(c, v[0]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[0][e]));
+        v[0].template load<kVec>(x, c, a.k);
+        store(c, v[0]);
       }
-    }
-  }
-#pragma unroll
-  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if constexpr (TPR > 32) {
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
-    __syncthreads();
-    m = red[sub * (TPR / 32)];
-#pragma unroll
-    for (int i = 1; i < TPR / 32; ++i) m = max_nan(m, red[sub * (TPR / 32) + i]);
-  }
-  if (!live) return;
-  if (tid == 0) a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
-  // codes mean nothing in a row that is not finite: zeros
-  const bool usable = m > 0.0f && m < INFINITY;
-  const bool ends = m < 1e-30f || m > 1e36f;  // 127 / m or 127 x leaves fp32's normal numbers
-  const float inv = usable && !ends ? __fdiv_rn(127.0f, m) : 0.0f;
-  auto store = [&](int c, float (&o)[8]) {
-    uint2 w = make_uint2(0u, 0u);
-    if (usable) {
-      if (ends) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float r = exact_code<T>(o[e], m);
-          const uint32_t byte = (uint32_t)((int)r & 255) << (8 * (e % 4));
-          if (e < 4) w.x |= byte;
-          else w.y |= byte;
-        }
-      } else {
-        w = make_uint2(codes4<T>(o, m, inv), codes4<T>(o + 4, m, inv));
-      }
-    }
-    *reinterpret_cast<uint2*>(a.q + row * a.ld_q + c * 8) = w;
-  };
-  if constexpr (CH > 0) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int c = i * TPR + tid;
-      if (c < chunks) store(c, v[i]);
-    }
-  } else {
-    for (int c = tid; c < chunks; c += TPR) {
-      load(c, v[0]);
-      store(c, v[0]);
     }
   }
 }
 
 template <typename T, int TPR, int CH>
 int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(((int64_t)a.rows * TPR + 255) / 256);
+  // as many CTAs as the SMs hold (registers: six of 256 threads)
+  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, 6ll * current_device_sms());
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ld_x * (int64_t)sizeof(T)) % 16 == 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
