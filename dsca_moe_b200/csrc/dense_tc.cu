@@ -717,33 +717,41 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             else bias = reinterpret_cast<const float*>(P.bias)[ch];
           }
         }
-        // n tokens of the block o (32 or 16 of them, lane = column), tokens tok0 + j of the tile, through `st`
+        // 32 or 16 tokens of the block o (lane = column) from token tok0 of the tile on, through `st`
+        const int64_t ldo = q.ldo;
+        const int cols = q.cols;
         auto put = [&](O* base, const auto& o, int tok0, __nv_bfloat16* st) {
           constexpr int N = sizeof(o) / sizeof(o[0]);
+          const int left = t.nval - tok0;  // tokens
           if constexpr (sizeof(O) == 2) {
             if (whole) {
 #pragma unroll
               for (int j = 0; j < N; ++j) st[j * 32 + lane] = __float2bfloat16_rn(o[j]);
               __syncwarp();
+              O* at = base + (int64_t)(t.n0 + tok0 + (lane >> 2)) * ldo + (ch & ~31) + 8 * (lane & 3);
 #pragma unroll
-              for (int rr = 0; rr < N / 8; ++rr) {
-                const int tok = rr * 8 + (lane >> 2);
-                if (tok0 + tok < t.nval)
-                  *reinterpret_cast<uint4*>(base + (int64_t)(t.n0 + tok0 + tok) * q.ldo + (ch & ~31) + 8 * (lane & 3)) =
-                      *reinterpret_cast<const uint4*>(st + tok * 32 + 8 * (lane & 3));
-              }
+              for (int rr = 0; rr < N / 8; ++rr, at += 8 * ldo)
+                if (rr * 8 + (lane >> 2) < left)
+                  *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(st + (rr * 8 + (lane >> 2)) * 32 + 8 * (lane & 3));
               __syncwarp();
               return;
             }
           }
-          if (ch < q.cols) {
+          if (ch < cols) {
+            O* at = base + (int64_t)(t.n0 + tok0) * ldo + ch;
+            auto one = [&](float x) {
+              if constexpr (sizeof(O) == 2) *at = __float2bfloat16_rn(x);
+              else *at = x;
+              at += ldo;
+            };
+            if (left >= N) {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-              if (tok0 + j < t.nval) {
-                O* at = base + (int64_t)(t.n0 + tok0 + j) * q.ldo + ch;
-                if constexpr (sizeof(O) == 2) *at = __float2bfloat16_rn(o[j]);
-                else *at = o[j];
-              }
+              for (int j = 0; j < N; ++j) one(o[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < N; ++j)
+                if (j < left) one(o[j]);
+            }
           }
         };
 #pragma unroll 1
@@ -997,9 +1005,9 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     q.a_mn = q.row ? s.b[0].mn : s.a[0].mn;
     q.b_mn = q.row ? s.a[0].mn : s.b[0].mn;
     // Tile width and k splits by an estimate of the time: waves of tiles, each its boxes' time and a fixed part.  A box
-    // costs mostly its 256 rows of A: 256 rows of B 1, 192 0.83, 128 0.75 of the time (2048 x 5632).
+    // costs mostly its 256 rows of A: 0.50 us at 256 rows of B, 0.43 at 128, 0.38 at 32 (2048 x 5632).
     const int whole = f32 ? 1 : 2;  // boxes of a stage
-    const double slice = f32 ? 3.0 : 1.0;  // a box's time against 16 bits'
+    const double slice = f32 ? 2.0 : 1.0;  // a box's time against 16 bits'
     double best = -1;
     auto consider = [&](int tn, int splits) {
       const int per_tile = q.row && glu ? tn / 2 : tn;
@@ -1009,10 +1017,13 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
       const int per = ceil_div(ceil_div(q.boxes, splits), whole) * whole;
       splits = ceil_div(q.boxes, per);
       if (splits > 1 && tiles * splits > 2 * pairs) return;  // bounds the partial tiles
-      const double box = slice * (0.2 + 0.1 * tn / 128.0);           // us
-      const double fixed = 1.0 + (splits > 1 ? 1.5 + 0.5 * splits * tn / 64.0 : 0.0);
+      const double box = slice * (0.36 + 0.07 * tn / 128.0);         // us
+      // the last tile's epilogue is not hidden: its chunks of 32 columns, two warps a lane quarter, and the pieces'
+      // sums if the tile is split
+      const double chunks = (tn + 63) / 64;
+      const double last = chunks + (splits > 1 ? 2.0 + 0.4 * splits * chunks : 0.0);
       const double waves = j.nprob == 1 ? (double)ceil_div(tiles * splits, pairs) : std::max(1.0, (double)(tiles * splits) / pairs);
-      const double cost = waves * (box * per + fixed) + 0.02 * tn / 256.0 * per;
+      const double cost = waves * (box * per + 0.5) + last;
       if (best < 0 || cost < best * 0.98) {
         best = cost;
         q.tn = tn; q.tiles_m = tm; q.tiles_n = tiles_n;
@@ -1024,7 +1035,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
         // a gated tile's gate and up chunks of 32 belong to one warp only from 64 channels on
         for (int tn = most; tn >= (q.b_mn || glu ? 128 : 64); tn /= 2) consider(tn, splits);
       } else {
-        for (int nt = ceil_div(q.rows, most), e = nt + 2; nt <= e; ++nt)  // tokens in equal tiles
+        for (int nt = ceil_div(q.rows, most), e = 2 * nt + 4; nt <= e; ++nt)  // tokens in equal tiles
           consider(std::max(32, ceil_div(ceil_div(q.rows, nt), 32) * 32), splits);
       }
     }
@@ -1033,7 +1044,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
   // 640 x 768 x 2048: dx has nine tiles of 64 boxes beside 72 of ten)
   if (j.nprob > 1) {
     double work = 0;
-    auto time = [](const Prob& q) { return (0.2 + 0.1 * q.tn / 128.0) * q.boxes; };
+    auto time = [](const Prob& q) { return (0.36 + 0.07 * q.tn / 128.0) * q.boxes; };
     for (int i = 0; i < j.nprob; ++i) work += time(P.prob[i]) * P.prob[i].tiles_m * P.prob[i].tiles_n;
     for (int i = 0; i < j.nprob; ++i) {
       Prob& q = P.prob[i];
