@@ -189,8 +189,8 @@ int run(Call& c, const dsca_gated_ffn_args* a) {
     k.prob[0] = problem({a->w_down, a->ld_down, 0, 0}, {a->h, a->ld_h, 0, 0}, d, T, I, a->y, a->ld_y);
     if (few_fits(j) && few_fits(k)) {
       if (c.dry) return DSCA_OK;
-      TRY(launch_few(j, false, c.stream));
-      return launch_few(k, true, c.stream);
+      TRY(launch_few(j, &k, false, c.stream));
+      return launch_few(k, nullptr, true, c.stream);
     }
     j = {};
     k = {};
@@ -272,7 +272,7 @@ int run(Call& c, const dsca_int8_linear_args* a) {
   const bool few = few_fits(j);
   if (!few) TRY(c.reserve(jobs, own, 1));
   if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false));
-  if (few) return c.dry ? DSCA_OK : launch_few(j, a->x != nullptr, c.stream);
+  if (few) return c.dry ? DSCA_OK : launch_few(j, nullptr, a->x != nullptr, c.stream);
   return c.product(j, own[0], a->x != nullptr);
 }
 
@@ -290,10 +290,10 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   const bool few = few_fits(j) && few_fits(k);
   if (!few) TRY(c.reserve(jobs, own, 2));
   TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false));
-  if (few && !c.dry) TRY(launch_few(j, true, c.stream));
+  if (few && !c.dry) TRY(launch_few(j, &k, true, c.stream));
   if (!few) TRY(c.product(j, own[0], true));
   TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale, true));
-  if (few) return c.dry ? DSCA_OK : launch_few(k, true, c.stream);
+  if (few) return c.dry ? DSCA_OK : launch_few(k, nullptr, true, c.stream);
   return c.product(k, own[1], true);
 }
 

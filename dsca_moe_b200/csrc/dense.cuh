@@ -100,7 +100,8 @@ __device__ __forceinline__ float f16_back(uint32_t e) {                         
 
 // Products for few tokens (dense_few.cu); no workspace, any alignment.
 bool few_fits(const Job& j);
-int launch_few(const Job& j, bool pdl, cudaStream_t stream);
+// next: the product behind it, whose weights it asks into L2.
+int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream);
 
 // A matrix to lay out anew (dense_split.cu).
 struct Relay {

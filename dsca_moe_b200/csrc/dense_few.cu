@@ -44,6 +44,9 @@ struct Params {
   const float* row_scale;
   const float* col_scale[2];
   const void* bias;
+  const uint8_t* ahead;  // the next product's weights: asked into L2 by this one's CTAs, `ahead_step` bytes each
+  int64_t ahead_bytes;
+  int ahead_step;
 };
 
 template <typename T>
@@ -189,6 +192,14 @@ __global__ void __launch_bounds__(32 * kWarps) few_kernel(const __grid_constant_
     }
   }
 
+  // this CTA's weights have all been asked for: a share of the next product's, so that DRAM does not rest while the
+  // sums are joined and the next launch starts
+  if (p.ahead != nullptr && threadIdx.x == 0) {
+    const int64_t from = (int64_t)blockIdx.x * p.ahead_step;
+    const int64_t n = min((int64_t)p.ahead_step, p.ahead_bytes - from);
+    if (n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.ahead + from), "r"((uint32_t)n) : "memory");
+  }
+
   // ---- the warps' parts, added in their order
   if constexpr (kF) {
 #pragma unroll
@@ -274,6 +285,8 @@ int launch(Params& p, bool pdl, cudaStream_t stream) {
   int splits = 1;
   while (splits < 8 && p.tiles * splits * 2 <= 4 * sms && steps >= splits * 2 * kU * kWarps) splits *= 2;
   p.per = (steps + splits - 1) / splits;
+  const int ctas = splits * p.tiles;
+  p.ahead_step = (int)(((p.ahead_bytes + ctas - 1) / ctas + 127) / 128 * 128);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(splits * p.tiles));
   cfg.blockDim = dim3(32 * kWarps);
@@ -316,7 +329,7 @@ bool few_fits(const Job& j) {
   return j.nprob == 1 && j.prob[0].nseg == 1 && j.prob[0].N <= most && j.epi != kDGlu && !j.prob[0].a[0].mn;
 }
 
-int launch_few(const Job& j, bool pdl, cudaStream_t stream) {
+int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   const Problem& s = j.prob[0];
   few::Params p = {};
   const int es = j.i8 ? 1 : j.dtype == DSCA_BF16 ? 2 : 4;
@@ -331,6 +344,15 @@ int launch_few(const Job& j, bool pdl, cudaStream_t stream) {
   p.out = s.out; p.ldo = s.ldo;
   p.save_g = j.save_g; p.save_u = j.save_u; p.save_e = j.save_e; p.groups = exp_groups(s.M);
   p.row_scale = j.row_scale; p.col_scale[0] = j.col_scale[0]; p.col_scale[1] = j.col_scale[1]; p.bias = j.bias;
+  if (next != nullptr) {
+    const Operand& w = next->prob[0].a[0];
+    const int64_t bytes = (int64_t)next->prob[0].M * w.ld * es;
+    // rows that follow one another, and no more than a part of L2 keeps
+    if (reinterpret_cast<uintptr_t>(w.p) % 16 == 0 && (w.ld == next->prob[0].K || j.i8) && bytes % 16 == 0 && bytes <= (48 << 20)) {
+      p.ahead = reinterpret_cast<const uint8_t*>(w.p);
+      p.ahead_bytes = bytes;
+    }
+  }
   using B = __nv_bfloat16;
   if (j.i8) {
     if (j.epi == kGlu) return few::by_tokens<int8_t, float, kGlu>(p, true, true, pdl, stream);
