@@ -132,15 +132,21 @@ struct Call {
     relays.item[relays.n++] = {p, dst, rows, rows_p, cols, ld, ldd, dtype, 0, 0};
     return {dst, ldd, mn, rows_p};
   }
-  // The launch that lays out what operand() collected; *none when there was nothing.
+  // The launch that lays out what operand() collected, and zeroes the counters that reserve() left to it; *none when
+  // there was nothing to launch.
   int relay(bool* none) {
     *none = relays.n == 0;
-    const int rc = dry || relays.n == 0 ? DSCA_OK : launch_relay(relays, stream);
+    int rc = DSCA_OK;
+    if (!dry) {
+      if (relays.n != 0) rc = launch_relay(relays, stream);
+      else if (relays.zero != nullptr && cudaMemsetAsync(relays.zero, 0, relays.zero_bytes, stream) != cudaSuccess) rc = DSCA_ERR_CUDA;
+    }
     relays.n = 0;
+    relays.zero = nullptr;
     return rc;
   }
-  // The jobs' own workspaces, counters zeroed: before the products, so that nothing lies between those that follow
-  // one another.
+  // The jobs' own workspaces; their counters are zeroed by the relay() that has to come next, before the products, so
+  // that nothing lies between those that follow one another.
   struct Own {
     void *parts = nullptr, *counters = nullptr;
   };
@@ -158,7 +164,9 @@ struct Call {
       at += counters[i];
     }
     if (!fits()) return DSCA_ERR_CAPACITY;
-    return dry || cudaMemsetAsync(own[0].counters, 0, zero, stream) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+    relays.zero = own[0].counters;
+    relays.zero_bytes = zero;
+    return DSCA_OK;
   }
   int product(const Job& j, const Own& o, bool pdl) {
     return dry ? DSCA_OK : launch_tc(j, o.parts, o.counters, err, pdl, stream);
@@ -237,27 +245,32 @@ int run(Call& c, const dsca_gated_ffn_backward_args* a) {
   }
   if (weights) x = c.operand(a->x, T, d, a->ld_x, dt, 1);
   if (a->d_down != nullptr) h = c.operand(a->h, T, I, a->ld_h, dt, 1);
-  if (!c.fits()) return DSCA_ERR_CAPACITY;
-  TRY(c.relay(&none));
   // ... and those that the first product makes
-  Operand dg = {}, du = {};
-  if (a->dx != nullptr || a->d_gate != nullptr) dg = c.operand(a->dg, T, I, a->ld_h, dt, 0);
-  if (a->dx != nullptr || a->d_up != nullptr) du = c.operand(a->du, T, I, a->ld_h, dt, 0);
-  if (a->dx != nullptr) {
-    Problem& p = k.prob[k.nprob++];
-    p = problem(wg, dg, d, T, I, a->dx, d);
-    p.nseg = 2;
-    p.a[1] = wu;
-    p.b[1] = du;
-  }
-  if (a->d_gate != nullptr) k.prob[k.nprob++] = problem(x, as(dg, 1), d, I, T, a->d_gate, d);
-  if (a->d_up != nullptr) k.prob[k.nprob++] = problem(x, as(du, 1), d, I, T, a->d_up, d);
-  if (a->d_down != nullptr) k.prob[k.nprob++] = problem(h, as(dy, 1), I, d, T, a->d_down, I);
+  auto second = [&](Operand dg, Operand du) {
+    k.nprob = 0;
+    if (a->dx != nullptr) {
+      Problem& p = k.prob[k.nprob++];
+      p = problem(wg, as(dg, 0), d, T, I, a->dx, d);
+      p.nseg = 2;
+      p.a[1] = wu;
+      p.b[1] = as(du, 0);
+    }
+    if (a->d_gate != nullptr) k.prob[k.nprob++] = problem(x, as(dg, 1), d, I, T, a->d_gate, d);
+    if (a->d_up != nullptr) k.prob[k.nprob++] = problem(x, as(du, 1), d, I, T, a->d_up, d);
+    if (a->d_down != nullptr) k.prob[k.nprob++] = problem(h, as(dy, 1), I, d, T, a->d_down, I);
+  };
+  second({}, {});
   if (k.nprob == 0) return DSCA_OK;
   const Job* jobs[] = {&k, &j};
   Call::Own own[2];
   TRY(c.reserve(jobs, own, inner ? 2 : 1));
+  TRY(c.relay(&none));
+  Operand dg = {}, du = {};
+  if (a->dx != nullptr || a->d_gate != nullptr) dg = c.operand(a->dg, T, I, a->ld_h, dt, 0);
+  if (a->dx != nullptr || a->d_up != nullptr) du = c.operand(a->du, T, I, a->ld_h, dt, 0);
+  if (!c.fits()) return DSCA_ERR_CAPACITY;
   if (inner) TRY(c.product(j, own[1], false));
+  second(dg, du);
   TRY(c.relay(&none));
   return c.product(k, own[0], inner && none);
 }
@@ -270,7 +283,9 @@ int run(Call& c, const dsca_int8_linear_args* a) {
   const Job* jobs[] = {&j};
   Call::Own own[1];
   const bool few = few_fits(j);
+  bool none;
   if (!few) TRY(c.reserve(jobs, own, 1));
+  TRY(c.relay(&none));
   if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false));
   if (few) return c.dry ? DSCA_OK : launch_few(j, nullptr, a->x != nullptr, c.stream);
   return c.product(j, own[0], a->x != nullptr);
@@ -288,7 +303,9 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   const Job* jobs[] = {&j, &k};
   Call::Own own[2];
   const bool few = few_fits(j) && few_fits(k);
+  bool none;
   if (!few) TRY(c.reserve(jobs, own, 2));
+  TRY(c.relay(&none));
   TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false));
   if (few && !c.dry) TRY(launch_few(j, &k, true, c.stream));
   if (!few) TRY(c.product(j, own[0], true));

@@ -115,6 +115,8 @@ constexpr int kMaxRelays = 8;
 struct RelayList {
   Relay item[kMaxRelays];
   int n;
+  void* zero;         // words to zero as well, or NULL
+  size_t zero_bytes;
 };
 int launch_relay(RelayList& list, cudaStream_t stream);
 

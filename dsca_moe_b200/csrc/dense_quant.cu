@@ -49,11 +49,15 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float amax, float i
   constexpr float kRound = 12582912.0f;
   uint32_t b[8];
   float far = 0.0f;
+  const float2 inv2 = make_float2(inv, inv), up = make_float2(kRound, kRound);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = x[i] * inv, r = v + kRound;
-    far = fmaxf(far, fabsf(v - (r - kRound)));
-    b[i] = __float_as_uint(r);
+  for (int i = 0; i < 8; i += 2) {  // two values an instruction
+    const float2 v = make_float2(x[i], x[i + 1]), r = __ffma2_rn(v, inv2, up);
+    const float2 c = __ffma2_rn(r, make_float2(-1.0f, -1.0f), up);  // minus the code
+    const float2 d = __ffma2_rn(v, inv2, c);
+    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+    b[i] = __float_as_uint(r.x);
+    b[i + 1] = __float_as_uint(r.y);
   }
   if (far > 0.49996f) {
 #pragma unroll
@@ -89,6 +93,20 @@ struct Raw {
           else w[i] = __float_as_uint(x[c * 8 + i]);
         }
     }
+  }
+  // the larger of m and the eight magnitudes, as bit patterns (NaN's are above infinity's): all of 32-bit values; for
+  // bf16 two 16-bit ones side by side
+  __device__ __forceinline__ uint32_t largest(uint32_t m) const {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 2) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      else m = max(m, w[i] & 0x7fffffffu);
+    }
+    return m;
+  }
+  static __device__ __forceinline__ float as_float(uint32_t m) {
+    if constexpr (sizeof(T) == 2) return __uint_as_float(max(m << 16, m & 0xffff0000u));
+    else return __uint_as_float(m);
   }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 2) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
@@ -126,26 +144,22 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
     const bool live = row < a.rows;
     const T* x = base + (live ? row : 0) * a.ld_x;
     Raw<T> v[N];
-    float m = 0.0f;
+    uint32_t bits = 0u;
     if constexpr (CH > 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         v[i] = next[i];
-        if (live && i * TPR + tid < chunks) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[i].get(e)));
-        }
+        if (live && i * TPR + tid < chunks) bits = v[i].largest(bits);
       }
       fetch(row + step);
     } else if (live) {
       for (int c = tid; c < chunks; c += TPR) {
         v[0].template load<kVec>(x, c, a.k);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(v[0].get(e)));
+        bits = v[0].largest(bits);
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // a row's largest magnitude, NaN if there is one
+    float m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(Raw<T>::as_float(bits))));
     if constexpr (TPR > 32) {
       float* r = red[it & 1];  // two, so that one barrier a row is enough
       if (threadIdx.x % 32 == 0) r[threadIdx.x / 32] = m;
@@ -196,8 +210,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
 
 template <typename T, int TPR, int CH>
 int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
-  // as many CTAs as the SMs hold (registers: six of 256 threads)
-  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, 6ll * current_device_sms());
+  // up to eight CTAs an SM, which go round
+  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, 8ll * current_device_sms());
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ld_x * (int64_t)sizeof(T)) % 16 == 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);

@@ -21,6 +21,9 @@ __device__ __forceinline__ void split3(float x, float* hi, float* mid, float* lo
 }
 
 __global__ void __launch_bounds__(256) relay_kernel(const __grid_constant__ RelayList L) {
+  if (L.zero != nullptr)
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < L.zero_bytes / 4; i += (size_t)gridDim.x * 256)
+      reinterpret_cast<uint32_t*>(L.zero)[i] = 0u;
   int e = 0;
   while (e + 1 < L.n && blockIdx.x >= L.item[e + 1].first) ++e;
   const Relay& m = L.item[e];

@@ -21,9 +21,10 @@ def act(g, name):
     if name == "silu":
         s = torch.sigmoid(g)
         return g * s, s * (1 + g * (1 - s))
+    # (1 + tanh z) / 2 = sigmoid(2 z), which does not cancel where tanh z is near -1
     c = math.sqrt(2 / math.pi)
-    t = torch.tanh(c * (g + 0.044715 * g ** 3))
-    return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 0.134145 * g * g)
+    p = torch.sigmoid(2 * c * (g + 0.044715 * g ** 3))
+    return g * p, p + 2 * g * p * (1 - p) * c * (1 + 0.134145 * g * g)
 
 
 def _acc(k):
@@ -55,11 +56,11 @@ def ffn(x, wg, wu, wd, name, dtype, dy=None):
         return out
     dy = dy.double()
     if dtype == torch.bfloat16:
-        # the backward pass reads g and u in 11 bits, or half of 2^-24 of the scaled range (2^-38 of the largest of a
-        # token's 32 channels)
+        # the backward pass reads g and u as fp16: off by 2^-11 (half a step of 11 bits), or by half of 2^-24 of the
+        # scaled range (2^-38 of the largest of a token's 32 channels)
         def held(v, e):
             big = torch.nn.functional.pad(v.abs() + e, (0, -I % 32)).view(T, -1, 32).amax(2)
-            return e + 2.0 ** -12 * (v.abs() + e) + 2.0 ** -38 * big.repeat_interleave(32, 1)[:, :I]
+            return e + 2.0 ** -11 * (v.abs() + e) + 2.0 ** -38 * big.repeat_interleave(32, 1)[:, :I]
         eg, eu = held(g, eg), held(u, eu)
     ea = 1.13 * eg + fast * (a.abs() + 1.13 * eg)
     eda = (g.abs() <= eg).double() if name == "relu" else 0.8 * eg + fast * (da.abs() + g.abs() * 0.5)
