@@ -255,7 +255,7 @@ def _int8_weight(w, name: str, dev, inp: int, out: int | None = None) -> int:
         raise ValueError(f"{name} must be on x's device")
     if s.dtype != torch.float32 or s.shape != (q.shape[0],) or not s.is_contiguous():
         raise ValueError(f"{name}: scale must be a contiguous float32 [{q.shape[0]}] tensor")
-    ld = q.stride(0) if q.shape[0] > 1 else (inp + 15) // 16 * 16
+    ld = q.stride(0)
     if (inp > 1 and q.stride(1) != 1) or ld % 16 or ld < inp or q.data_ptr() % 16:
         raise ValueError(f"{name}: rows of codes must lie a multiple of 16 bytes apart (pack_int8 lays them out)")
     return ld

@@ -110,6 +110,50 @@ def test_gradients_asked_for(cuda, T):
         assert not gated_ffn(xt, wg, wu, wd).requires_grad
 
 
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 values of x and y: the first and the last rows."""
+    from dsca_moe_b200 import gated_ffn, gated_ffn_int8, int8_linear, pack_int8, quantize_rows
+
+    T, d, I = 270001, 8192, 40
+    g = torch.Generator(device=cuda)
+    g.manual_seed(1)
+    x = torch.randn(T, d, generator=g, device=cuda, dtype=BF16)
+    wg, wu, wd = (torch.randn(*s, generator=g, device=cuda).mul_(s[1] ** -0.5).to(BF16) for s in ((I, d), (I, d), (d, I)))
+    dy = torch.randn(T, d, generator=g, device=cuda, dtype=BF16)
+    last = slice(T - 33, T)
+    p = [x.requires_grad_()] + [t.clone().requires_grad_() for t in (wg, wu, wd)]
+    y = gated_ffn(*p)
+    (dx,) = torch.autograd.grad(y, p[0], dy)
+    for rows in (slice(0, 33), last):
+        ref = R.ffn(x[rows].detach(), wg, wu, wd, "silu", BF16, dy[rows])
+        R.close(y[rows].detach(), ref["y"])
+        R.close(dx[rows], ref["dx"])
+    del y, dx
+    x = x.detach()
+    q, s = quantize_rows(x)
+    assert torch.equal(q[last].double(), R.codes(x[last].double())[0])
+    pw = [pack_int8(w) for w in (wg, wu, wd)]
+    wide = pack_int8(torch.randn(d, 64, generator=g, device=cuda, dtype=BF16))
+    R.close(int8_linear(q[:, :64], wide, x_scale=s)[last], R.int8_linear(q[last, :64], s[last], wide.q, wide.scale, BF16))
+    R.close(gated_ffn_int8(x, *pw)[last], R.ffn_int8(x[last], *pw, "silu", BF16))
+
+
+@pytest.mark.parametrize("T,d,I,dtype", [(2600, 520, 1544, BF16), (4100, 256, 300, BF16), (3000, 264, 200, F32), (20000, 64, 72, BF16)])
+def test_many_tiles(cuda, T, d, I, dtype):
+    """More tiles than CTA pairs, ragged ones among them."""
+    from dsca_moe_b200 import gated_ffn, gated_ffn_int8, pack_int8
+
+    x, wg, wu, wd, dy = _inputs(cuda, T, d, I, dtype, 31)
+    ref = R.ffn(x, wg, wu, wd, "silu", dtype, dy)
+    p = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    y = gated_ffn(*p)
+    R.close(y.detach(), ref["y"], "y")
+    for got, k in zip(torch.autograd.grad(y, p, dy), ("dx", "d_gate", "d_up", "d_down")):
+        R.close(got, ref[k], k)
+    q = [pack_int8(w) for w in (wg, wu, wd)]
+    R.close(gated_ffn_int8(x, *q), R.ffn_int8(x, *q, "silu", dtype))
+
+
 def test_gradient_against_differences(cuda):
     from dsca_moe_b200 import gated_ffn
 
@@ -354,6 +398,9 @@ def test_refusals_on_the_gpu(cuda):
         int8_linear(x[:, :63], odd)
     with pytest.raises(ValueError, match="16 bytes"):
         int8_linear(odd.q, Int8Weight(pack_int8(wg[:, :63]).q, q.scale), x_scale=q.scale)
+    # a single row of codes has to lie in whole 16 bytes too: what follows it is multiplied
+    with pytest.raises(ValueError, match="16 bytes"):
+        int8_linear(x[:, :63], Int8Weight(torch.zeros(1, 63, dtype=torch.int8, device=cuda), q.scale[:1]))
     with pytest.raises(ValueError, match="w_down"):
         gated_ffn_int8(x, q, q, q)
     xr = x.clone().requires_grad_()
