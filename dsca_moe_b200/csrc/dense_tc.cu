@@ -158,14 +158,59 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr) {
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+// The producer and the MMA issuer are whole warps, of which one lane (`one`, a predicate in the instruction and no
+// branch) issues: their loops stay uniform over the warp, so that addresses, coordinates and descriptors are computed
+// in uniform registers, where these instructions take them.  Loops of a single lane moved every operand there by
+// itself, an MMA took 160 to 190 cycles to issue and 128 to run.
+__device__ __forceinline__ void umma_pair(uint32_t one, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t one, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                              uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
       : "memory");
+}
+__device__ __forceinline__ void commit_both(uint32_t one, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+      "h"((unsigned short)3), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void load_pair(uint32_t one, uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int32_t c0,
+                                          int32_t c1) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t one, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(one)
+      : "memory");
+}
+// mbar_wait() with one verdict for the warp
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
 }
 
 // Where box b of a problem lies: slice k of a segment.
@@ -337,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t smem_a = smem_u32(smem), smem_b = smem_a + R::kB;  // of stage 0
-  const int warp = warp_id(), lane = lane_id();
+  const int warp = __shfl_sync(0xffffffffu, warp_id(), 0), lane = lane_id();  // uniform for the compiler too
+  const uint32_t one = lane == 0;
   volatile int* abort_flag = &ctl.abort_flag;
   const uint32_t rank = cluster_ctarank();
   const int unit0 = (int)(blockIdx.x >> 1), units = (int)(gridDim.x >> 1);
@@ -374,11 +420,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
 
   if (warp == 0) {
     // ---------------- TMA producer
-    if (lane == 0) {
+    {
+      const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]), full0_even = mapa_shared(full0, 0);
+      const uint32_t even = rank == 0;
       int s = 0;
       uint32_t ph = 0;
-      int pending[kStages];
-      for (int i = 0; i < kStages; ++i) pending[i] = -1;
+      uint32_t armed = 0, parity = 0;  // stages with copies under way since, and the phase of each
       bool ok = true;
       for (int unit = unit0; ok && unit < P.total; unit += units) {
         const Tile t = decode(P, unit, kAM, kBN);
@@ -391,11 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         const CUtensorMap *ma = P.a[t.p], *mb = glu_rows ? P.b[t.p] + rank : P.b[t.p];
         BoxAt at(q, t.box0);
         for (int b = t.box0; b < t.box1; b += kSub) {
-          if (!mbar_wait(smem_u32(&ctl.empty[s]), ph ^ 1u, abort_flag, P.err)) { ok = false; break; }
-          const uint32_t fb0 = mapa_shared(smem_u32(&ctl.full[s]), 0);
+          if (!wait_warp(empty0 + 8 * s, ph ^ 1u, abort_flag, P.err)) { ok = false; break; }
+          const uint32_t fb0 = full0_even + 8 * s;
           const int nb = min(kSub, t.box1 - b);
-          if (rank == 0)
-            mbar_arrive_expect_tx(smem_u32(&ctl.full[s]), 2u * (uint32_t)(nb * R::kPlanes) * ((uint32_t)kBoxBytes + b_bytes));
+          expect_tx(one & even, full0 + 8 * s, 2u * (uint32_t)(nb * R::kPlanes) * ((uint32_t)kBoxBytes + b_bytes));
           for (int h = 0; h < nb; ++h, at.next(kb)) {
             const int kx = at.k * KE;
 #pragma unroll
@@ -403,33 +449,36 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               const uint32_t da = smem_a + s * kStageBytes + (h + pl) * kBoxBytes, db = smem_b + s * kStageBytes + (h + pl) * R::kBBytes;
               const int pa = pl * a_plane, pb = pl * b_plane;
               if (kGluE && !glu_rows) {
-                tma_load_2d_pair(da, ma, fb0, kx, a_row + pa);
-                tma_load_2d_pair(da + 8192, ma + 1, fb0, kx, a_row + pa);
+                load_pair(one, da, ma, fb0, kx, a_row + pa);
+                load_pair(one, da + 8192, ma + 1, fb0, kx, a_row + pa);
               } else if (a_mn) {
-                tma_load_2d_pair(da, ma + at.seg, fb0, a_row, kx + pa);
-                tma_load_2d_pair(da + 8192, ma + at.seg, fb0, a_row + 64, kx + pa);
+                load_pair(one, da, ma + at.seg, fb0, a_row, kx + pa);
+                load_pair(one, da + 8192, ma + at.seg, fb0, a_row + 64, kx + pa);
               } else {
-                tma_load_2d_pair(da, ma + at.seg, fb0, kx, a_row + pa);
+                load_pair(one, da, ma + at.seg, fb0, kx, a_row + pa);
               }
               if (b_atoms) {
-                tma_load_2d_pair(db, mb + at.seg, fb0, b_row, kx + pb);
-                if (b_atoms > 1) tma_load_2d_pair(db + 8192, mb + at.seg, fb0, b_row + 64, kx + pb);
+                load_pair(one, db, mb + at.seg, fb0, b_row, kx + pb);
+                if (b_atoms > 1) load_pair(one, db + 8192, mb + at.seg, fb0, b_row + 64, kx + pb);
               } else {
-                tma_load_2d_pair(db, mb + at.seg, fb0, kx, b_row + pb);
+                load_pair(one, db, mb + at.seg, fb0, kx, b_row + pb);
               }
             }
           }
-          pending[s] = (int)ph;
+          armed |= 1u << s;
+          parity = (parity & ~(1u << s)) | ph << s;
           if (++s == kStages) { s = 0; ph ^= 1u; }
         }
       }
       if (!ok && rank == 0)
         for (int i = 0; i < kStages; ++i)
-          if (pending[i] >= 0) drain(smem_u32(&ctl.full[i]), (uint32_t)pending[i]);
+          if (armed >> i & 1u) drain(full0 + 8 * i, parity >> i & 1u);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]);
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
       int s = 0, it = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -449,15 +498,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         for (int c0 = t.box0; ok && c0 < t.box1; ++it) {
           const int c1 = IN == kF32 ? min(t.box1, c0 + R::kChunk) : t.box1;
           const int acc = it & 1;
-          if (!mbar_wait(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
+          if (!wait_warp(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+          const uint32_t d = tmem + (uint32_t)(acc * 256);
           uint32_t used = 0u;
           for (int b = c0; b < c1; b += kSub) {
-            if (!mbar_wait(smem_u32(&ctl.full[s]), ph, abort_flag, P.err)) { ok = false; break; }
+            if (!wait_warp(full0 + 8 * s, ph, abort_flag, P.err)) { ok = false; break; }
             tc_fence_after();
             const int nb = min(kSub, c1 - b);
 #pragma unroll
@@ -471,16 +520,16 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
                   if (i < steps) {
                     const uint64_t ai = ad + astep * i, bi = bd + bstep * i;
                     if constexpr (IN == kI8) {
-                      umma_i8_pair(d, ai, bi, idesc, used);
+                      umma_i8_pair(one, d, ai, bi, idesc, used);
                     } else {
-                      umma_f16_pair(d, ai, bi, idesc, used);
+                      umma_pair(one, d, ai, bi, idesc, used);
                       if constexpr (IN == kF32) {
                         constexpr uint64_t PA = kBoxBytes >> 4, PB = R::kBBytes >> 4;
-                        umma_f16_pair(d + 128u, ai, bi + PB, idesc, used);
-                        umma_f16_pair(d + 128u, ai + PA, bi, idesc, 1u);
-                        umma_f16_pair(d + 128u, ai, bi + 2 * PB, idesc, 1u);
-                        umma_f16_pair(d + 128u, ai + PA, bi + PB, idesc, 1u);
-                        umma_f16_pair(d + 128u, ai + 2 * PA, bi, idesc, 1u);
+                        umma_pair(one, d + 128u, ai, bi + PB, idesc, used);
+                        umma_pair(one, d + 128u, ai + PA, bi, idesc, 1u);
+                        umma_pair(one, d + 128u, ai, bi + 2 * PB, idesc, 1u);
+                        umma_pair(one, d + 128u, ai + PA, bi + PB, idesc, 1u);
+                        umma_pair(one, d + 128u, ai + 2 * PA, bi, idesc, 1u);
                       }
                     }
                     used = 1u;
@@ -488,16 +537,16 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
                 at.next(kb);
               }
             }
-            umma_commit_pair_both(smem_u32(&ctl.empty[s]));
+            commit_both(one, empty0 + 8 * s);
             if (++s == kStages) { s = 0; ph ^= 1u; }
           }
           if (!ok) break;
-          umma_commit_pair_both(smem_u32(&ctl.tmem_full[acc]));
+          commit_both(one, smem_u32(&ctl.tmem_full[acc]));
           c0 = c1;
         }
       }
       if (!ok) {  // every MMA issued has completed before TMEM is freed
-        umma_commit_pair(mapa_shared(smem_u32(&ctl.mma_done), 0));
+        if (lane == 0) umma_commit_pair(mapa_shared(smem_u32(&ctl.mma_done), 0));
         drain(smem_u32(&ctl.mma_done), 0);
       }
     }
