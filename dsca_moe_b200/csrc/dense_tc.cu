@@ -9,7 +9,7 @@
 //             32 x 32 blocks in shared memory.  For up to 128 rows of output.
 //   warp 0      TMA producer (one thread), 128-byte swizzle, three stages of two 128-byte k boxes
 //   warp 1      TMEM (512 columns: two accumulators); in the even CTA the MMA issuer
-//   warps 2-9   epilogue: two warps to a lane quarter, alternate chunks of 32 TMEM columns
+//   warps 4-11  epilogue: two warps to a lane quarter, alternate chunks of 32 TMEM columns
 // Operands: a K-major one is loaded as boxes of 128 bytes of k by its rows; an MN-major one as boxes of 64
 // rows of k by 64 values of m or n, which the MMA reads transposed, so that the gradients' products take
 // weights and activations as they lie.
@@ -49,7 +49,12 @@ constexpr int kMaxStages = 3;
 constexpr int kBoxBytes = 128 * 128;             // A's part of one k box (slice of k); B's, but for kF32
 constexpr int kRingBytes = 12 * kBoxBytes;       // all stages
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kFirstEpi = 4;                       // warps 0 producer, 1 MMA issuer, 2 and 3 idle
+constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
+// Registers a thread after the set-up: the launch's 168 x 384 are dealt out anew (168 would spill what an epilogue has
+// on its way from memory, which waits for it there).
+constexpr int kRegsFew = 56, kRegsEpi = 224;
+static_assert(128 * kRegsFew + 32 * kEpiWarps * kRegsEpi <= 168 * kThreads, "registers of the launch");
 constexpr int kStgBytes = 2 * 32 * 32 * 2;       // per epilogue warp: two 32 x 32 blocks of bf16
 constexpr int kSmemBytes = kRingBytes + kEpiWarps * kStgBytes + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
@@ -337,33 +342,49 @@ __device__ __forceinline__ void save_row_f16(const Params& P, const Prob& q, int
   }
   *reinterpret_cast<uint32_t*>(P.save_e + ((int64_t)up * q.rows + row) * exp_groups(q.cols) + n / 8) = e * 0x01010101u;
 }
-// g and u of a chunk, loaded while the one before it is in work
+// g and u of a chunk, loaded while the one before it is in work; 32 bytes a load where rows start on such boundaries
+// (every lane reads a row of its own, and a request takes a cycle for each row: with 16 bytes a load they, not the
+// MMAs, set the time of 8192 x 2048 x 5632's first backward product)
+__device__ __forceinline__ void load32(const void* p, uint32_t* w) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
 struct Ahead {
-  uint4 v[8];
+  uint32_t v[2][16];
   uint32_t e[2];
   __device__ __forceinline__ void load(const Params& P, const Prob& q, int64_t row, int n, int nend) {
     const bool live = row < q.rows && n < nend;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __half* p = reinterpret_cast<const __half*>(i < 4 ? P.save_g : P.save_u);
-      const int c = n + 8 * (i & 3);
-      v[i] = live && c < q.cols ? __ldg(reinterpret_cast<const uint4*>(p + row * q.ldo + c)) : make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int i = 0; i < 2; ++i) {
+      const __half* p = reinterpret_cast<const __half*>(i == 0 ? P.save_g : P.save_u) + row * q.ldo + n;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int h = 0; h < 2; ++h) {
+        if (!live || n + 16 * h >= q.cols) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[i][8 * h + k] = 0u;
+        } else if (q.vec == 2) {
+          load32(p + 16 * h, v[i] + 8 * h);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint4 x = n + 16 * h + 8 * k < q.cols ? __ldg(reinterpret_cast<const uint4*>(p + 16 * h + 8 * k))
+                                                        : make_uint4(0u, 0u, 0u, 0u);
+            v[i][8 * h + 4 * k] = x.x; v[i][8 * h + 4 * k + 1] = x.y;
+            v[i][8 * h + 4 * k + 2] = x.z; v[i][8 * h + 4 * k + 3] = x.w;
+          }
+        }
+      }
       e[i] = live ? *reinterpret_cast<const uint32_t*>(P.save_e + ((int64_t)i * q.rows + row) * exp_groups(q.cols) + n / 8) : 0u;
+    }
   }
   __device__ __forceinline__ void get(int i, float (&o)[32]) const {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float s = f16_back(e[i] >> (8 * k) & 255u);
-      const uint32_t w[4] = {v[4 * i + k].x, v[4 * i + k].y, v[4 * i + k].z, v[4 * i + k].w};
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[h]));
-        o[8 * k + 2 * h] = f.x * s;
-        o[8 * k + 2 * h + 1] = f.y * s;
-      }
+    for (int k = 0; k < 16; ++k) {
+      const float s = f16_back(e[i] >> (8 * (k / 4)) & 255u);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i][k]));
+      o[2 * k] = f.x * s;
+      o[2 * k + 1] = f.y * s;
     }
   }
 };
@@ -418,9 +439,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   pdl_launch_dependents();
   pdl_wait();  // the launch before this one (when it is its programmatic dependent) has written its results
 
-  if (warp == 0) {
+  if (warp < kFirstEpi) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+    if (warp == 0) {
     // ---------------- TMA producer
-    {
       const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]), full0_even = mapa_shared(full0, 0);
       const uint32_t even = rank == 0;
       int s = 0;
@@ -473,8 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       if (!ok && rank == 0)
         for (int i = 0; i < kStages; ++i)
           if (armed >> i & 1u) drain(full0 + 8 * i, parity >> i & 1u);
-    }
-  } else if (warp == 1) {
+    } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA)
     if (rank == 0) {
       const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]);
@@ -550,9 +571,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         drain(smem_u32(&ctl.mma_done), 0);
       }
     }
+    }
   } else {
     // ---------------- epilogue
-    const int q4 = warp & 3, ew = warp - 2, eh = ew >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    const int q4 = warp & 3, ew = warp - kFirstEpi, eh = ew >> 2;
     uint8_t* stg = smem + kRingBytes + ew * kStgBytes;
     const int pair_id = 1 + (ew & 1) + 2 * eh;  // barrier of an exchange
     int it = 0, xb = 0;
@@ -639,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             ctl.pair_old[ew] = (int)atomicAdd(counter, 1u);
           }
           pair_barrier(pair_id);
-          old = (uint32_t)*reinterpret_cast<volatile int*>(&ctl.pair_old[ew | 2]);  // the gate warps are 2, 3, 6, 7
+          old = (uint32_t)*reinterpret_cast<volatile int*>(&ctl.pair_old[ew & ~2]);  // the gate warps are 0, 1, 4, 5
         } else {
           if (lane == 0) old = atomicAdd(counter, 1u);
           old = __shfl_sync(0xffffffffu, old, 0);
