@@ -48,23 +48,30 @@ struct Job {
 };
 
 // ---------------------------------------------------------------- gates
-// kFast (16-bit outputs): the hardware's exponential and division, good to 2^-21 here; otherwise the
-// full-precision ones.
+// kFast (16-bit and 8-bit operands): the hardware's exponential and reciprocal without the steps that keep subnormal
+// numbers, good to 2^-18 here (where they flush to zero, 1 + e^-x is 1 or its reciprocal below 2^-126); otherwise
+// the full-precision ones.
 template <bool kFast>
-__device__ __forceinline__ float expf_(float x) { return kFast ? __expf(x) : expf(x); }
-template <bool kFast>
-__device__ __forceinline__ float div_(float a, float b) { return kFast ? __fdividef(a, b) : a / b; }
+__device__ __forceinline__ float sigmoid(float x) {
+  if constexpr (kFast) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+  } else {
+    return 1.0f / (1.0f + expf(-x));
+  }
+}
 
-// 0.5 (1 + tanh z) = 1 / (1 + e^-2z) for the gelu gate, z = sqrt(2 / pi) (g + 0.044715 g^3)
+// the gelu gate: 0.5 (1 + tanh z) = sigmoid(2 z), z = sqrt(2 / pi) (g + 0.044715 g^3)
 template <bool kFast>
 __device__ __forceinline__ float gelu_p(float g) {
-  const float z2 = -1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return div_<kFast>(1.0f, 1.0f + expf_<kFast>(z2));
+  return sigmoid<kFast>(1.5957691216057308f * (g + 0.044715f * g * g * g));
 }
 
 template <bool kFast>
 __device__ __forceinline__ float gate(float g, int act) {
-  if (act == DSCA_GATE_SILU) return div_<kFast>(g, 1.0f + expf_<kFast>(-g));
+  if (act == DSCA_GATE_SILU) return kFast ? g * sigmoid<true>(g) : g / (1.0f + expf(-g));
   if (act == DSCA_GATE_RELU) return g <= 0.0f ? 0.0f : g;  // NaN stays
   return g * gelu_p<kFast>(g);
 }
@@ -73,7 +80,7 @@ __device__ __forceinline__ float gate(float g, int act) {
 template <bool kFast>
 __device__ __forceinline__ void gate_grad(float g, int act, float* a, float* da) {
   if (act == DSCA_GATE_SILU) {
-    const float s = div_<kFast>(1.0f, 1.0f + expf_<kFast>(-g));
+    const float s = sigmoid<kFast>(g);
     *a = g * s;
     *da = s + *a * (1.0f - s);
   } else if (act == DSCA_GATE_RELU) {

@@ -273,7 +273,7 @@ __device__ __forceinline__ void gate_grad_all(const float (&dh)[N], float (&g)[N
 // ---- rows form: 32 consecutive values of one output row from column n on.  vec: rows start on 16-byte (1) or
 // 32-byte (2) boundaries; a whole 32-byte sector a store where they do, half a sector costs L2 twice the writes.
 __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+  asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
                "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
@@ -342,11 +342,11 @@ __device__ __forceinline__ void save_row_f16(const Params& P, const Prob& q, int
   }
   *reinterpret_cast<uint32_t*>(P.save_e + ((int64_t)up * q.rows + row) * exp_groups(q.cols) + n / 8) = e * 0x01010101u;
 }
-// g and u of a chunk, loaded while the one before it is in work; 32 bytes a load where rows start on such boundaries
-// (every lane reads a row of its own, and a request takes a cycle for each row: with 16 bytes a load they, not the
-// MMAs, set the time of 8192 x 2048 x 5632's first backward product)
+// g and u of a chunk, loaded while the one before it is in work: 32 bytes a load where rows start on such boundaries.
+// Every lane has a row of its own, and what these loads and the stores leave in L1 only pushes one another out: without
+// it 4096 x 2048 x 5632's first backward product takes 86 us instead of 103.
 __device__ __forceinline__ void load32(const void* p, uint32_t* w) {
-  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                : "l"(p));
 }
