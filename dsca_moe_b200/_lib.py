@@ -125,7 +125,8 @@ class FewArgs(ctypes.Structure):
 GATE_SILU, GATE_GELU, GATE_RELU = range(3)
 DENSE_MAX_DIM = 1048576
 DENSE_MAX_ROWS = 16777216
-DENSE_FEW_TOKENS = 16
+DENSE_FEW_TOKENS = 8
+DENSE_FEW_BYTES = 50331648
 
 
 class GatedFfnArgs(ctypes.Structure):

@@ -1,4 +1,4 @@
-// The products of dense.cuh for at most 16 tokens (fp32: 8): the weights' stream through the warps' registers.
+// The products of dense.cuh for at most 16 tokens (fp32: 6): the weights' stream through the warps' registers.
 //
 // Such a call reads every weight once and has nothing else to wait for, so the weights go from memory straight into
 // mma.sync fragments: a lane's 16 bytes of a weight row are eight bf16 (16 codes) in a row, and since a sum over k may
@@ -322,11 +322,16 @@ int by_tokens(Params& p, bool vw, bool vx, bool pdl, cudaStream_t stream) {
 }  // namespace few
 
 bool few_fits(const Job& j) {
-  // Against the tensor-memory products, us (2048 x 5632 blocks of weights larger than L2): bf16 16 tokens 29 | 37, 24
-  // tokens 37 | 39; 8-bit 16 tokens 23 | 35, 24 tokens 29 | 35, but 24 x 2048 x 151936 100 | 67; fp32 4 tokens 83 | 151,
-  // 8 tokens 130 | 151, 12 tokens 193 | 151
-  const int most = !j.i8 && j.dtype == DSCA_F32 ? 8 : DSCA_DENSE_FEW_TOKENS;
-  return j.nprob == 1 && j.prob[0].nseg == 1 && j.prob[0].N <= most && j.epi != kDGlu && !j.prob[0].a[0].mn;
+  // Against the tensor-memory products, us (sets of weights larger than L2, 2048 wide): bf16 block of 5632 16 tokens
+  // 28 | 31, 24 tokens 37 | 31; of 22528 (92 MB a product at least) 8 tokens 60 | 66, 16 tokens 74 | 66; 8-bit product of
+  // 5632 16 tokens 7 | 10, of 22528 19 | 17, of 151936 (311 MB) 1 token 65 | 58, 16 tokens 84 | 59; fp32 block of 5632 4
+  // tokens 85 | 121, 8 tokens 133 | 121
+  const Problem& s = j.prob[0];
+  const int es = j.i8 ? 1 : j.dtype == DSCA_BF16 ? 2 : 4;
+  const int64_t bytes = (int64_t)s.M * s.K * es * (j.epi == kGlu ? 2 : 1);
+  if (j.nprob != 1 || s.nseg != 1 || j.epi == kDGlu || s.a[0].mn) return false;
+  if (!j.i8 && j.dtype == DSCA_F32) return s.N <= 6;
+  return s.N <= 8 ? bytes <= (256ll << 20) : s.N <= 16 && bytes <= DSCA_DENSE_FEW_BYTES;
 }
 
 int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {

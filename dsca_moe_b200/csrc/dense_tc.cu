@@ -1077,9 +1077,9 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     q.a_mn = q.row ? s.b[0].mn : s.a[0].mn;
     q.b_mn = q.row ? s.a[0].mn : s.b[0].mn;
     // Tile width and k splits by an estimate of the time: waves of tiles, each its boxes' time and a fixed part.  A box
-    // costs mostly its 256 rows of A: 0.50 us at 256 rows of B, 0.43 at 128, 0.38 at 32 (2048 x 5632).
+    // costs 0.38 us at 256 rows of B, 0.28 at 128 (4096 x 2048 x 5632); an fp32 slice three times that.
     const int whole = f32 ? 1 : 2;  // boxes of a stage
-    const double slice = f32 ? 2.0 : 1.0;  // a box's time against 16 bits'
+    const double slice = f32 ? 3.0 : 1.0;  // a box's time against 16 bits'
     double best = -1;
     auto consider = [&](int tn, int splits) {
       const int per_tile = q.row && glu ? tn / 2 : tn;
@@ -1089,7 +1089,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
       const int per = ceil_div(ceil_div(q.boxes, splits), whole) * whole;
       splits = ceil_div(q.boxes, per);
       if (splits > 1 && tiles * splits > 2 * pairs) return;  // bounds the partial tiles
-      const double box = slice * (0.36 + 0.07 * tn / 128.0);         // us
+      const double box = slice * (0.2 + 0.09 * tn / 128.0);          // us
       // the last tile's epilogue is not hidden: its chunks of 32 columns, two warps a lane quarter, and the pieces'
       // sums if the tile is split
       const double chunks = (tn + 63) / 64;
@@ -1116,7 +1116,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
   // 640 x 768 x 2048: dx has nine tiles of 64 boxes beside 72 of ten)
   if (j.nprob > 1) {
     double work = 0;
-    auto time = [](const Prob& q) { return (0.36 + 0.07 * q.tn / 128.0) * q.boxes; };
+    auto time = [](const Prob& q) { return (0.2 + 0.09 * q.tn / 128.0) * q.boxes; };
     for (int i = 0; i < j.nprob; ++i) work += time(P.prob[i]) * P.prob[i].tiles_m * P.prob[i].tiles_n;
     for (int i = 0; i < j.nprob; ++i) {
       Prob& q = P.prob[i];

@@ -80,6 +80,11 @@ def _weight(w, name: str, out: int, inp: int, x) -> int:
     return inp if w.is_contiguous() else _stride(w, name, inp)
 
 
+def _few(rows: int, weight_bytes: int) -> bool:
+    """Whether a call needs no workspace whatever its alignment (include/dsca_b200_dense.h)."""
+    return rows <= L.DENSE_FEW_TOKENS and weight_bytes <= L.DENSE_FEW_BYTES
+
+
 def _workspace(name: str, args, dev):
     """The call's workspace, allocated on the current stream, in args."""
     fn = getattr(L._LIB or L.load(), name)
@@ -108,7 +113,7 @@ def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
     g, u, e = (h + step, h + 2 * step, h + 3 * step) if save else (None, None, None)
     a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h, rows, d, inter,
                        _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
-    if rows > L.DENSE_FEW_TOKENS or dtype is not _BF16:
+    if dtype is not _BF16 or not _few(rows, 4 * inter * d):
         ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
     return y, buf
@@ -315,7 +320,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     a = L.Int8LinearArgs(x_p, q_p, s_p, weight[0].data_ptr(), weight[1].data_ptr(),
                          None if bias is None else bias.data_ptr(), y.data_ptr(), rows, k, n, dt, ld_x, ld_q, ld_w, n,
                          None, 0, _err(dev))
-    if rows > L.DENSE_FEW_TOKENS:
+    if not _few(rows, n * ld_w):
         ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_int8_linear", ctypes.byref(a))
     return y
@@ -352,7 +357,7 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
                            w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr(), h, hq, scale + 4 * rows,
                            y.data_ptr(), rows, d, inter, dt, code, ld_x, ld_q, ld_gate, ld_up, ld_down, ld_hq, ld_hq, d,
                            None, 0, _err(dev))
-    if rows > L.DENSE_FEW_TOKENS:
+    if not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
         ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
     return y

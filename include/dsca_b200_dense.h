@@ -27,8 +27,10 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 /* Largest width (d, inter, k, n) and number of rows of these entry points. */
 #define DSCA_DENSE_MAX_DIM 1048576
 #define DSCA_DENSE_MAX_ROWS 16777216
-/* Forward calls in bf16 or 8-bit integers need no workspace for at most this many rows. */
-#define DSCA_DENSE_FEW_TOKENS 16
+/* Forward calls in bf16 or 8-bit integers need no workspace for at most this many rows, where the weights of each
+ * of their products (gate and up together) have at most that many bytes. */
+#define DSCA_DENSE_FEW_TOKENS 8
+#define DSCA_DENSE_FEW_BYTES 50331648
 
 /*
  * g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T; sums in fp32, h and y rounded to dtype.  g and u

@@ -29,7 +29,7 @@ def test_symbols_and_constants(lib):
     for name in L.EXPORTED_DENSE:
         assert hasattr(lib, name), name
     for c, v in (("DSCA_DENSE_MAX_DIM", L.DENSE_MAX_DIM), ("DSCA_DENSE_MAX_ROWS", L.DENSE_MAX_ROWS),
-                 ("DSCA_DENSE_FEW_TOKENS", L.DENSE_FEW_TOKENS)):
+                 ("DSCA_DENSE_FEW_TOKENS", L.DENSE_FEW_TOKENS), ("DSCA_DENSE_FEW_BYTES", L.DENSE_FEW_BYTES)):
         assert int(re.search(rf"#define {c} (\d+)", src).group(1)) == v
     assert set(re.findall(r"\}\s*(dsca_[a-z0-9_]+)\s*;", src)) == set(STRUCTS)
 
