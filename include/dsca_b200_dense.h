@@ -9,6 +9,9 @@
  * dsca_int8_linear          y = x W^T with both in 8-bit integers, scales for each token and channel
  * dsca_gated_ffn_int8       the gated block with 8-bit integer weights
  *
+ * DSCA_F32 products hold every value as three bf16 terms, 24 bits in all; magnitudes below 2^-100 keep fewer (the third
+ * term becomes subnormal), which is below 2^-116 in absolute terms.
+ *
  * Matrices are row-major with row strides in elements (ld_*, at least the width) and a contiguous
  * last dimension; weights lie as a Linear layer holds them, [out, in].  Any sizes; rows on 16-byte
  * boundaries are taken as they lie, others are copied into the workspace first.
@@ -87,7 +90,7 @@ typedef struct {
 } dsca_gated_ffn_backward_args;
 
 /*
- * scale[row] = max|x| / 127 (1 for a row of zeros), q = the quotient 127 x / max|x| rounded to the
+ * Codes lie in [-127, 127].  scale[row] = max|x| / 127 (1 for a row of zeros), q = the quotient 127 x / max|x| rounded to the
  * nearest integer, ties to even, exactly.  A row with an infinity or a NaN has that as its scale and
  * codes of no meaning.  Columns [k, ld_q) of q are written as zeros.
  */
