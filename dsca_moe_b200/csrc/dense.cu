@@ -316,8 +316,21 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
 
 #undef TRY
 
+// The kernels are sm_100a code.
+int device_ok() {
+  static volatile int known[kMaxDevices];  // 1 yes, 2 no
+  int dev = 0, major = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return DSCA_ERR_CUDA;
+  const int k = dev < kMaxDevices ? __atomic_load_n(&known[dev], __ATOMIC_ACQUIRE) : 0;
+  if (k == 1) return DSCA_OK;
+  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return DSCA_ERR_CUDA;
+  if (dev < kMaxDevices) __atomic_store_n(&known[dev], major == 10 ? 1 : 2, __ATOMIC_RELEASE);
+  return major == 10 ? DSCA_OK : DSCA_ERR_UNSUPPORTED;
+}
+
 template <typename Args>
 int call(const Args* a, cudaStream_t stream) {
+  if (int rc = device_ok()) return rc;
   if (a->workspace_bytes != 0 && !at(a->workspace, 256)) return DSCA_ERR_BAD_ARG;
   Call c = {false, reinterpret_cast<uint8_t*>(a->workspace), a->workspace_bytes, stream, a->err};
   return run(c, a);
@@ -356,7 +369,9 @@ int dsca_gated_ffn_backward(const dsca_gated_ffn_backward_args* a, dsca_stream_t
 
 int dsca_quantize_rows(const dsca_quantize_rows_args* a, dsca_stream_t stream) {
   if (int rc = dense::check(a)) return rc;
-  return a->rows == 0 ? DSCA_OK : dense::launch_quantize_rows(a, false, stream);
+  if (a->rows == 0) return DSCA_OK;
+  if (int rc = dense::device_ok()) return rc;
+  return dense::launch_quantize_rows(a, false, stream);
 }
 
 int dsca_int8_linear(const dsca_int8_linear_args* a, dsca_stream_t stream) {

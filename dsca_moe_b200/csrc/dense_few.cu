@@ -354,9 +354,9 @@ int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   p.row_scale = j.row_scale; p.col_scale[0] = j.col_scale[0]; p.col_scale[1] = j.col_scale[1]; p.bias = j.bias;
   if (next != nullptr) {
     const Operand& w = next->prob[0].a[0];
-    const int64_t bytes = (int64_t)next->prob[0].M * w.ld * es;
-    // rows that follow one another, and no more than a part of L2 keeps
-    if (reinterpret_cast<uintptr_t>(w.p) % 16 == 0 && (w.ld == next->prob[0].K || j.i8) && bytes % 16 == 0 && bytes <= (48 << 20)) {
+    const int64_t bytes = ((next->prob[0].M - 1) * w.ld + next->prob[0].K) * es & ~15ll;  // up to the last row's end
+    // rows that (nearly) follow one another, and no more than a part of L2 keeps
+    if (reinterpret_cast<uintptr_t>(w.p) % 16 == 0 && w.ld < next->prob[0].K + 16 && bytes <= (48 << 20)) {
       p.ahead = reinterpret_cast<const uint8_t*>(w.p);
       p.ahead_bytes = bytes;
     }

@@ -121,7 +121,7 @@ struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2], mma_done;
   uint32_t tmem_base;
   int abort_flag;
-  int pair_ok[kEpiWarps], pair_old[kEpiWarps];
+  int pair_ok[2][kEpiWarps], pair_old[kEpiWarps];
 };
 
 struct Tile {
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     const int q4 = warp & 3, ew = warp - kFirstEpi, eh = ew >> 2;
     uint8_t* stg = smem + kRingBytes + ew * kStgBytes;
     const int pair_id = 1 + (ew & 1) + 2 * eh;  // barrier of an exchange
-    int it = 0, xb = 0;
+    int it = 0, xb = 0, round = 0;
     Ahead ahead;
     for (int unit = unit0; unit < P.total; unit += units) {
       const Tile t = decode(P, unit, kAM, kBN);
@@ -627,10 +627,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         }
       }
       if constexpr (kGluE) {
-        // the two warps of an exchange go on or leave together
-        if (lane == 0) ctl.pair_ok[ew] = w_ok;
+        // the two warps of an exchange go on or leave together (two verdicts in turn: a warp may give its next one
+        // before the other has read this one)
+        if (lane == 0) ctl.pair_ok[round & 1][ew] = w_ok;
         pair_barrier(pair_id);
-        w_ok = *reinterpret_cast<volatile int*>(&ctl.pair_ok[ew ^ 2]) & w_ok;
+        w_ok = *reinterpret_cast<volatile int*>(&ctl.pair_ok[round & 1][ew ^ 2]) & w_ok;
+        ++round;
       }
       if (!w_ok) break;
       // 32 columns of the accumulator from c on
@@ -1114,7 +1116,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
         // a gated tile's gate and up chunks of 32 belong to one warp only from 64 channels on
         for (int tn = most; tn >= (q.b_mn || glu ? 128 : 64); tn /= 2) consider(tn, splits);
       } else {
-        for (int nt = ceil_div(q.rows, most), e = 2 * nt + 4; nt <= e; ++nt)  // tokens in equal tiles
+        for (int nt = ceil_div(q.rows, most), e = nt + std::min(nt + 4, 12); nt <= e; ++nt)  // tokens in equal tiles
           consider(std::max(32, ceil_div(ceil_div(q.rows, nt), 32) * 32), splits);
       }
     }

@@ -29,10 +29,13 @@ _ERR: dict = {}
 _BF16 = torch.bfloat16
 
 
-def _err(dev) -> int:
-    """Address of the device's error word (a wait inside a kernel that ran out records there)."""
+def _err(dev):
+    """Address of the device's error word (a wait inside a kernel that ran out records there); None for calls captured
+    before the first other call, whose graph's memory must not hold it."""
     e = _ERR.get(dev.index)
     if e is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
         t = torch.zeros(64, dtype=torch.int32, device=dev)
         e = _ERR[dev.index] = (t.data_ptr(), t)
     return e[0]
