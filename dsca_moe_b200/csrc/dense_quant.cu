@@ -2,12 +2,14 @@
 // nearest integer, ties to even, exactly.
 //
 // Why the exact quotient and not x / scale: the scale is rounded, so values half way between two
-// codes (x = max|x| / 2 is 63.5) would fall to either side by the row.  A product with 127 / max|x| finds the code of
-// all values but those close to a tie, which compare 127 x with the border times max|x|, exactly.
+// codes (x = max|x| / 2 is 63.5) would fall to either side by the row.  A product with 127 / max|x| is off by 2^-23
+// of itself.  bf16 quotients are a tie or 2^-16 of themselves away from one, so the product rounded to 19 bits lies on
+// the right side of each tie and on the tie where the quotient does; fp32 values close to a tie compare 127 x with the
+// border times max|x|, exactly.  (The comparison for bf16 too: its ties are so common that a third of the warps took
+// it, 16384 x 5632 57 us, now 43.)
 //
-// A row is read once into registers (up to 8192 values; longer rows are read a second time from L2).  16384 x 5632 bf16
-// 60 us (4.6 TB/s, 71 % of a copy; its instructions, 69 % of the issue slots, bound it as much as DRAM does), 4096 x 5632
-// fp32 20 us (5.7 TB/s), one row 2.5 us.
+// A row is read once (up to 8192 values; longer rows are read a second time from L2).  16384 x 5632 bf16 43 us (6.4
+// TB/s, a copy's rate), 4096 x 5632 fp32 20.5 us (5.6 TB/s), one row 2.5 us.
 #include "dense.cuh"
 
 #include <algorithm>
@@ -20,45 +22,53 @@ namespace quant {
 __device__ __forceinline__ float divided_code(float x, float amax) { return (float)rint(127.0 * (double)x / (double)amax); }
 
 // The code next to r that x has, r being one of the two integers around 127 x / amax: the sign of 127 x - h amax at the
-// border h half way towards the other one decides.  Both products are exact: in fp32 for bf16 values (15 and 16 bits), in
-// 64 bits for fp32 ones.
-template <typename T>
+// border h half way towards the other one decides, both products exact in 64 bits.
 __device__ __forceinline__ float settled(float r, float toward, float x, float amax) {
   const float s = copysignf(1.0f, toward), h = r + 0.5f * s;
-  float over;  // beyond the border (> 0) or on it
-  if constexpr (sizeof(T) == 2) {
-    over = fmaf(-h, amax, 127.0f * x) * s;
-  } else {
-    const double e = fma(-(double)h, (double)amax, 127.0 * (double)x);
-    over = e > 0.0 ? s : e < 0.0 ? -s : 0.0f;
-  }
+  const double over = fma(-(double)h, (double)amax, 127.0 * (double)x) * (double)s;  // beyond the border (> 0) or on it
   const bool odd = (int)r & 1;
-  return over > 0.0f || (over == 0.0f && odd) ? r + s : r;
+  return over > 0.0 || (over == 0.0 && odd) ? r + s : r;
 }
 
-// Eight codes.  inv is 127 / amax to 2^-23: a product with it is off by less than 2^-16, so only values that close to
-// a tie need the exact comparison (where one of the eight does, all take it: ties are common among bf16 values,
-// whose quotients have few bits).  Adding 1.5 * 2^23 rounds to an integer, whose low byte is the code.
+// Eight codes.  inv is 127 / amax to 2^-24, a product with it off by less than 2^-23 of itself.  Adding 1.5 * 2^23 rounds to
+// an integer, ties to even, whose low byte is the code.
+//
+// bf16: x = X 2^a and amax = M 2^b with X and M from 128 to 255 (the quotient 127 X 2^e / M with e = a - b <= 0), so a
+// border (2 j + 1) / 2 that is not the quotient is at least 2^e / (2 M) away from it, 1 / (254 X) > 2^-16 of it.  The product
+// rounded to 19 bits, off by 2^-19 more, lies on the same side; and borders below 128, with their 8 bits, are among
+// the 19-bit numbers, the nearest to products 2^-23 off.  (p - (33 p - 32 p), each step rounded: 24 - 5 bits.)
+//
+// fp32: only values within 2^-16 of a tie need the exact comparison; where one of the eight does, all take it.
 template <typename T>
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float amax, float inv) {
   constexpr float kRound = 12582912.0f;
   uint32_t b[8];
-  float far = 0.0f;
-  const float2 inv2 = make_float2(inv, inv), up = make_float2(kRound, kRound);
+  const float2 inv2 = make_float2(inv, inv), up = make_float2(kRound, kRound), minus = make_float2(-1.0f, -1.0f);
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {  // two values an instruction
-    const float2 v = make_float2(x[i], x[i + 1]), r = __ffma2_rn(v, inv2, up);
-    const float2 c = __ffma2_rn(r, make_float2(-1.0f, -1.0f), up);  // minus the code
-    const float2 d = __ffma2_rn(v, inv2, c);
-    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
-    b[i] = __float_as_uint(r.x);
-    b[i + 1] = __float_as_uint(r.y);
-  }
-  if (far > 0.49996f) {
+    for (int i = 0; i < 8; i += 2) {  // two values an instruction
+      const float2 p = __fmul2_rn(make_float2(x[i], x[i + 1]), inv2), c = __ffma2_rn(p, make_float2(32.0f, 32.0f), p);
+      const float2 low = __ffma2_rn(p, minus, c), r = __fadd2_rn(__ffma2_rn(low, minus, c), up);
+      b[i] = __float_as_uint(r.x);
+      b[i + 1] = __float_as_uint(r.y);
+    }
+  } else {
+    float far = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float r = __uint_as_float(b[i]) - kRound;
-      b[i] = __float_as_uint(settled<T>(r, x[i] * inv - r, x[i], amax) + kRound);
+    for (int i = 0; i < 8; i += 2) {
+      const float2 v = make_float2(x[i], x[i + 1]), r = __ffma2_rn(v, inv2, up);
+      const float2 c = __ffma2_rn(r, minus, up);  // minus the code
+      const float2 d = __ffma2_rn(v, inv2, c);
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+      b[i] = __float_as_uint(r.x);
+      b[i + 1] = __float_as_uint(r.y);
+    }
+    if (far > 0.49996f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float r = __uint_as_float(b[i]) - kRound;
+        b[i] = __float_as_uint(settled(r, x[i] * inv - r, x[i], amax) + kRound);
+      }
     }
   }
   return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
@@ -89,13 +99,18 @@ struct Raw {
         }
     }
   }
-  // the larger of m and the eight magnitudes, as bit patterns (NaN's are above infinity's): all of 32-bit values; for
-  // bf16 two 16-bit ones side by side
+  // the larger of m and the eight magnitudes, as bit patterns: of 32-bit values (NaN's are above infinity's); for bf16 two
+  // 16-bit ones side by side, NaN where there is one
   __device__ __forceinline__ uint32_t largest(uint32_t m) const {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      if constexpr (sizeof(T) == 2) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-      else m = max(m, w[i] & 0x7fffffffu);
+      if constexpr (sizeof(T) == 2) {
+        __nv_bfloat162 x, y;
+        memcpy(&x, &m, 4);
+        memcpy(&y, &w[i], 4);
+        x = __hmax2_nan(x, __habs2(y));
+        memcpy(&m, &x, 4);
+      } else m = max(m, w[i] & 0x7fffffffu);
     }
     return m;
   }
@@ -111,29 +126,49 @@ struct Raw {
 
 // TPR threads a row, CH chunks of eight values a thread in registers (CH = 0: longer rows, read twice).  A CTA goes
 // through rows with the next one's values on their way while one is turned into codes: with a CTA a row and no
-// such overlap, 16384 x 5632 bf16 took 107 us.
+// such overlap, 16384 x 5632 bf16 took 107 us.  bf16 rows of more than two chunks a thread come through a ring of two
+// rows in shared memory, by copies that hold no registers (54 us with the next row in registers, 47 with a ring of
+// one); shorter rows do not gain (4096 x 2048 7.0 | 6.5 us), nor does fp32 (22 us either way).
+template <typename T, int CH, bool kVec>
+constexpr bool in_ring() { return kVec && CH > 2 && sizeof(T) == 2; }
+constexpr int kDepth = 2;
+
 template <typename T, int TPR, int CH, bool kVec>
 __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a) {
   __shared__ uint32_t red[2][8];
+  extern __shared__ uint4 ring[];  // [kDepth][CH][256], each thread's own chunks
   constexpr int kRows = 256 / TPR, N = CH > 0 ? CH : 1;
+  constexpr bool kRing = in_ring<T, CH, kVec>();
   const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
   const int chunks = (int)(a.ld_q / 8);  // those past k are zeros
   const T* base = reinterpret_cast<const T*>(a.x);
   pdl_launch_dependents();  // a product that follows asks for its first weights meanwhile
   pdl_wait();
   Raw<T> next[N];
-  auto fetch = [&](int64_t row) {
+  auto fetch = [&](int64_t row, int slot) {
     if constexpr (CH > 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int c = i * TPR + tid;
-        if (row < a.rows && c < chunks) next[i].template load<kVec>(base + row * a.ld_x, c, a.k);
+        if (row < a.rows && c < chunks) {
+          if constexpr (kRing) {
+            const int n = min(max(a.k - c * 8, 0), 8);  // the rest of the 16 bytes are zeros
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&ring[(slot * N + i) * 256 + threadIdx.x])),
+                         "l"(base + row * a.ld_x + (n > 0 ? c * 8 : 0)), "r"(2 * n)
+                         : "memory");
+          } else {
+            next[i].template load<kVec>(base + row * a.ld_x, c, a.k);
+          }
+        }
       }
     }
+    if constexpr (kRing) asm volatile("cp.async.commit_group;" ::: "memory");
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + sub;
-  fetch(row);
+  int slot = 0;
+  fetch(row, 0);
+  if constexpr (kRing) fetch(row + step, 1);
   // whole CTAs go round together (the reduction's barrier)
   for (int64_t first = (int64_t)blockIdx.x * kRows, it = 0; first < a.rows; first += step, row += step, ++it) {
     const bool live = row < a.rows;
@@ -141,12 +176,14 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
     Raw<T> v[N];
     uint32_t bits = 0u;
     if constexpr (CH > 0) {
+      if constexpr (kRing) asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        v[i] = next[i];
+        if constexpr (kRing) *reinterpret_cast<uint4*>(v[i].w) = ring[(slot * N + i) * 256 + threadIdx.x];
+        else v[i] = next[i];
         if (live && i * TPR + tid < chunks) bits = v[i].largest(bits);
       }
-      fetch(row + step);
+      if constexpr (!kRing) fetch(row + step, 0);
     } else if (live) {
       for (int c = tid; c < chunks; c += TPR) {
         v[0].template load<kVec>(x, c, a.k);
@@ -164,6 +201,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
       for (int i = 1; i < TPR / 32; ++i) bits = max(bits, r[sub * (TPR / 32) + i]);
     }
     const float m = __uint_as_float(bits);
+    if constexpr (kRing) {  // m is known, so this thread's chunks have left the slot
+      fetch(row + kDepth * step, slot);
+      slot ^= 1;
+    }
     if (!live) continue;
     if (tid == 0) a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
     // codes mean nothing in a row that is not finite: zeros
@@ -206,8 +247,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
 
 template <typename T, int TPR, int CH>
 int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
-  // up to eight CTAs an SM, which go round
-  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, 8ll * current_device_sms());
+  // CTAs go round, two for each that an SM holds at a time or nearly so (long fp32 rows: 80 registers a thread, three)
+  constexpr int kCtas = sizeof(T) == 4 && CH > 2 ? 6 : 8;
+  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, (int64_t)kCtas * current_device_sms());
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ld_x * (int64_t)sizeof(T)) % 16 == 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -218,6 +260,7 @@ int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
+  if (vec && in_ring<T, CH, true>()) cfg.dynamicSmemBytes = (size_t)kDepth * CH * 256 * 16;  // 24 or 32 KB
   auto kern = vec ? quantize_kernel<T, TPR, CH, true> : quantize_kernel<T, TPR, CH, false>;
   return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }

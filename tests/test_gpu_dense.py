@@ -231,6 +231,51 @@ def test_quantize_rows(cuda, rows, k, gap, dtype):
     assert ((s.double() - sr).abs() <= 2.0 ** -24 * sr + 1.5e-45).all()
 
 
+@pytest.mark.parametrize("k,powers", [(2560, 10), (5632, 22)])
+def test_quantize_rows_every_quotient(cuda, k, powers):
+    """bf16: every pair of eight-bit significands and every power of two between them that leaves a code."""
+    from dsca_moe_b200 import quantize_rows
+
+    sig = torch.arange(128, 256, device=cuda, dtype=torch.float64)
+    x = torch.cat([s * 2.0 ** -e * sig for e in range(powers) for s in (1, -1)]).repeat(128, 1)
+    x = torch.where(x.abs() <= sig[:, None], x, torch.zeros_like(x))  # a row's largest magnitude is its significand
+    assert x.shape == (128, k) and torch.equal(x.abs().amax(1), sig)
+    x = torch.cat([x * 2.0 ** b for b in (-99, -50, -7, 0, 1, 60, 112)])
+    v = x.bfloat16()
+    assert torch.equal(v.double(), x)
+    q, s = quantize_rows(v)
+    qr, sr = R.codes(x)
+    assert torch.equal(q.double(), qr) and torch.equal(s, sr.float())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,k,gap", [(1, 4097, 7), (3, 4104, 0), (1300, 4104, 16), (2500, 5632, 0), (900, 6145, 7), (1500, 8192, 0),
+                                        (1200, 8185, 7)])
+def test_quantize_long_rows(cuda, rows, k, gap, dtype):
+    """Rows of more than 4096 values: several for each CTA, the last chunk cut short, a row that is not finite."""
+    from dsca_moe_b200 import quantize_rows
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(rows + k)
+    x = (torch.randn(rows, k + gap, generator=g, device=cuda) * torch.exp(torch.randn(rows, 1, generator=g, device=cuda))).to(dtype)
+    x[:, k:] = float("nan")  # of no row
+    x = x[:, :k]
+    x[rows // 2] = 0
+    x[rows // 3, k - 1] = 1000
+    q, s = quantize_rows(x)
+    qr, sr = R.codes(x.double())
+    assert torch.equal(q.double(), qr) and torch.equal(s, sr.float())
+    if q.stride(0) > k:
+        assert not torch.as_strided(q, (rows, q.stride(0) - k), (q.stride(0), 1), k).any()
+    for bad in (float("nan"), float("inf")):
+        y = x.clone()
+        y[rows // 2, 5] = bad
+        q2, s2 = quantize_rows(y)
+        keep = torch.arange(rows, device=cuda) != rows // 2
+        assert torch.equal(q2[keep], q[keep]) and torch.equal(s2[keep], s[keep])
+        assert not q2[rows // 2].any() and not torch.isfinite(s2[rows // 2])
+
+
 INT8_SHAPES = [(1, 16, 1), (1, 2048, 5632), (1, 33, 77), (4, 1021, 130), (8, 5632, 2048), (9, 256, 1000), (16, 128, 64),
                (20, 2048, 901), (32, 4100, 300), (33, 100, 257), (64, 512, 512), (100, 1021, 1363), (129, 144, 2000),
                (257, 2048, 264), (777, 1021, 1363), (1030, 640, 768)]
