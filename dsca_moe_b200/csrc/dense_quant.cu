@@ -126,11 +126,11 @@ struct Raw {
 
 // TPR threads a row, CH chunks of eight values a thread in registers (CH = 0: longer rows, read twice).  A CTA goes
 // through rows with the next one's values on their way while one is turned into codes: with a CTA a row and no
-// such overlap, 16384 x 5632 bf16 took 107 us.  bf16 rows of more than two chunks a thread come through a ring of two
+// such overlap, 16384 x 5632 bf16 took 107 us.  bf16 rows of more than 2048 values come through a ring of two
 // rows in shared memory, by copies that hold no registers (54 us with the next row in registers, 47 with a ring of
-// one); shorter rows do not gain (4096 x 2048 7.0 | 6.5 us), nor does fp32 (22 us either way).
-template <typename T, int CH, bool kVec>
-constexpr bool in_ring() { return kVec && CH > 2 && sizeof(T) == 2; }
+// one; 16384 x 4096 33 | 37); shorter rows do not gain (4096 x 2048 7.0 | 6.5 us), nor does fp32 (22 us either way).
+template <typename T, int TPR, int CH, bool kVec>
+constexpr bool in_ring() { return kVec && TPR * CH > 256 && sizeof(T) == 2; }
 constexpr int kDepth = 2;
 
 template <typename T, int TPR, int CH, bool kVec>
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
   __shared__ uint32_t red[2][8];
   extern __shared__ uint4 ring[];  // [kDepth][CH][256], each thread's own chunks
   constexpr int kRows = 256 / TPR, N = CH > 0 ? CH : 1;
-  constexpr bool kRing = in_ring<T, CH, kVec>();
+  constexpr bool kRing = in_ring<T, TPR, CH, kVec>();
   const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
   const int chunks = (int)(a.ld_q / 8);  // those past k are zeros
   const T* base = reinterpret_cast<const T*>(a.x);
@@ -260,7 +260,7 @@ int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  if (vec && in_ring<T, CH, true>()) cfg.dynamicSmemBytes = (size_t)kDepth * CH * 256 * 16;  // 24 or 32 KB
+  if (vec && in_ring<T, TPR, CH, true>()) cfg.dynamicSmemBytes = (size_t)kDepth * CH * 256 * 16;  // 24 or 32 KB
   auto kern = vec ? quantize_kernel<T, TPR, CH, true> : quantize_kernel<T, TPR, CH, false>;
   return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
