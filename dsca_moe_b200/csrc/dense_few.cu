@@ -107,6 +107,24 @@ __device__ __forceinline__ uint4 load16(const T* row, int k, int K, bool live) {
   }
 }
 
+// Four fp32 values in a row as three bf16 terms, which hold them exactly: the upper 8 bits of significand cut off (never
+// beyond the largest bf16), the next 8 rounded, what is left.  In each term's two words the values' own order.
+struct Terms {
+  uint32_t t[3][2];
+  __device__ __forceinline__ explicit Terms(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t p = w[2 * i], q = w[2 * i + 1];
+      const float rp = __uint_as_float(p) - __uint_as_float(p & 0xffff0000u), rq = __uint_as_float(q) - __uint_as_float(q & 0xffff0000u);
+      const uint32_t m = pack_bf16x2(rp, rq);
+      t[0][i] = __byte_perm(p, q, 0x7632);
+      t[1][i] = m;
+      t[2][i] = __byte_perm(__float_as_uint(rp - __uint_as_float(m << 16)), __float_as_uint(rq - __uint_as_float(m & 0xffff0000u)), 0x7632);
+    }
+  }
+};
+
 __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
@@ -136,7 +154,8 @@ __global__ void __launch_bounds__(32 * kWarps) few_kernel(const __grid_constant_
   int s = split * p.per + warp;
   pdl_launch_dependents();
 
-  uint4 a[kU], b[kU];
+  const T* x = reinterpret_cast<const T*>(p.x);
+  uint4 a[kU], b[kU], u[kU][NT];
   auto fetch = [&](int s0, uint4 (&ra)[kU], uint4 (&rb)[kU]) {
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
@@ -145,53 +164,68 @@ __global__ void __launch_bounds__(32 * kWarps) few_kernel(const __grid_constant_
       rb[i] = load16<T, kVecW, true>(w1, k, p.K, l1 && at < s_end);
     }
   };
+  auto fetch_x = [&](int s0, uint4 (&ru)[kU][NT]) {
+#pragma unroll
+    for (int i = 0; i < kU; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int at = s0 + i * kWarps, tok = 8 * n + g;
+        ru[i][n] = load16<T, kVecX, false>(x + (int64_t)tok * p.ldx, at * STEP + t4 * V, p.K, tok < p.T && at < s_end);
+      }
+  };
   fetch(s, a, b);
   pdl_wait();
+  fetch_x(s, u);
 
-  constexpr int NA = kF ? 8 * NT : 4;  // fp32: every token's sum for both rows, this lane's quarter of k
-  Acc acc[kF ? 2 : NT][NA];
+  Acc acc[NT][4];
 #pragma unroll
-  for (int i = 0; i < (kF ? 2 : NT); ++i)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int j = 0; j < NA; ++j) acc[i][j] = 0;
-  const T* x = reinterpret_cast<const T*>(p.x);
+    for (int e = 0; e < 4; ++e) acc[n][e] = 0;
   for (; s < s_end; s += kU * kWarps) {
-    uint4 na[kU], nb[kU];
+    uint4 na[kU], nb[kU], nu[kU][NT];
     fetch(s + kU * kWarps, na, nb);
+    fetch_x(s + kU * kWarps, nu);
+    if constexpr (kF) {
+      // a batch's sums, the six products of terms down to 2^-16 of the largest; the smaller five apart, and both
+      // added in fp32, since MMAs cut their sums off
+      float big[NT][4], small[NT][4];
 #pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      const int at = s + i * kWarps, k = at * STEP + t4 * V;
-      if (at < s_end) {
-        if constexpr (kF) {
-          const float wa[4] = {__uint_as_float(a[i].x), __uint_as_float(a[i].y), __uint_as_float(a[i].z), __uint_as_float(a[i].w)};
-          const float wb[4] = {__uint_as_float(b[i].x), __uint_as_float(b[i].y), __uint_as_float(b[i].z), __uint_as_float(b[i].w)};
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < 8 * NT; ++n) {
-            if (n < p.T) {
-              const uint4 u = load16<T, kVecX, false>(x + n * p.ldx, k, p.K, true);
-              const float xv[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
+        for (int e = 0; e < 4; ++e) big[n][e] = small[n][e] = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                acc[0][n] = fmaf(wa[e], xv[e], acc[0][n]);
-                acc[1][n] = fmaf(wb[e], xv[e], acc[1][n]);
-              }
-            }
-          }
-        } else {
+      for (int i = 0; i < kU; ++i) {
+        const Terms A(a[i]), B(b[i]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int tok = 8 * n + g;
-            const uint4 u = load16<T, kVecX, false>(x + (int64_t)tok * p.ldx, k, p.K, tok < p.T);
-            mma(acc[n], a[i].x, b[i].x, a[i].y, b[i].y, u.x, u.y);
-            mma(acc[n], a[i].z, b[i].z, a[i].w, b[i].w, u.z, u.w);
-          }
+        for (int n = 0; n < NT; ++n) {
+          const Terms X(u[i][n]);
+#pragma unroll
+          for (int o = 2; o >= 0; --o)
+#pragma unroll
+            for (int w = 0; w <= o; ++w)
+              mma(o == 0 ? big[n] : small[n], A.t[w][0], B.t[w][0], A.t[w][1], B.t[w][1], X.t[o - w][0], X.t[o - w][1]);
         }
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] += big[n][e] + small[n][e];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kU; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma(acc[n], a[i].x, b[i].x, a[i].y, b[i].y, u[i][n].x, u[i][n].y);
+          mma(acc[n], a[i].z, b[i].z, a[i].w, b[i].w, u[i][n].z, u[i][n].w);
+        }
     }
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
       a[i] = na[i];
       b[i] = nb[i];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) u[i][n] = nu[i][n];
     }
   }
 
@@ -204,22 +238,10 @@ __global__ void __launch_bounds__(32 * kWarps) few_kernel(const __grid_constant_
   }
 
   // ---- the warps' parts, added in their order
-  if constexpr (kF) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < 8 * NT; ++n) {
-        float v = acc[r][n];
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        if (t4 == (n & 3)) red[warp][g + 8 * r][n] = v;
-      }
-  } else {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][g + 8 * (e >> 1)][8 * n + 2 * t4 + (e & 1)] = acc[n][e];
-  }
+    for (int e = 0; e < 4; ++e) red[warp][g + 8 * (e >> 1)][8 * n + 2 * t4 + (e & 1)] = acc[n][e];
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * 8 * NT; i += 32 * kWarps) {
     const int r = i / (8 * NT), n = i % (8 * NT);
@@ -318,8 +340,7 @@ int by_vec(Params& p, bool vw, bool vx, bool pdl, cudaStream_t stream) {
 template <typename T, typename O, int EPI>
 int by_tokens(Params& p, bool vw, bool vx, bool pdl, cudaStream_t stream) {
   if (p.T <= 8) return by_vec<T, O, EPI, 1>(p, vw, vx, pdl, stream);
-  if constexpr (!std::is_same<T, float>::value) return by_vec<T, O, EPI, 2>(p, vw, vx, pdl, stream);
-  return DSCA_ERR_BAD_ARG;
+  return by_vec<T, O, EPI, 2>(p, vw, vx, pdl, stream);
 }
 
 }  // namespace few
@@ -333,7 +354,7 @@ bool few_fits(const Job& j) {
   const int es = j.i8 ? 1 : j.dtype == DSCA_BF16 ? 2 : 4;
   const int64_t bytes = (int64_t)s.M * s.K * es * (j.epi == kGlu ? 2 : 1);
   if (j.nprob != 1 || s.nseg != 1 || j.epi == kDGlu || s.a[0].mn) return false;
-  if (!j.i8 && j.dtype == DSCA_F32) return s.N <= 6;
+  if (!j.i8 && j.dtype == DSCA_F32) return s.N <= 16;
   return s.N <= 8 ? bytes <= (256ll << 20) : s.N <= 16 && bytes <= DSCA_DENSE_FEW_BYTES;
 }
 
