@@ -195,7 +195,7 @@ int run(Call& c, const dsca_gated_ffn_args* a) {
     j.save_g = a->g; j.save_u = a->u; j.save_e = a->gu_exp;
     k.epi = kStore; k.nprob = 1; k.dtype = dt;
     k.prob[0] = problem({a->w_down, a->ld_down, 0, 0}, {a->h, a->ld_h, 0, 0}, d, T, I, a->y, a->ld_y);
-    if (few_fits(j) && few_fits(k)) {
+    if (few_fits(j, false) && few_fits(k, false)) {
       if (c.dry) return DSCA_OK;
       TRY(launch_few(j, &k, false, c.stream));
       return launch_few(k, nullptr, true, c.stream);
@@ -282,7 +282,7 @@ int run(Call& c, const dsca_int8_linear_args* a) {
   j.row_scale = a->scale; j.col_scale[0] = a->w_scale; j.bias = a->bias;
   const Job* jobs[] = {&j};
   Call::Own own[1];
-  const bool few = few_fits(j);
+  const bool few = few_fits(j, true);
   bool none;
   if (!few) TRY(c.reserve(jobs, own, 1));
   TRY(c.relay(&none));
@@ -302,7 +302,7 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   k.row_scale = a->h_scale; k.col_scale[0] = a->down_scale;
   const Job* jobs[] = {&j, &k};
   Call::Own own[2];
-  const bool few = few_fits(j) && few_fits(k);
+  const bool few = few_fits(j, false) && few_fits(k, false);
   bool none;
   if (!few) TRY(c.reserve(jobs, own, 2));
   TRY(c.relay(&none));

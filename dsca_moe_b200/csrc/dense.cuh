@@ -105,8 +105,8 @@ __device__ __forceinline__ float f16_back(uint32_t e) {                         
   return e > 14u ? __uint_as_float((e - 14u) << 23) : 5.877471754111438e-39f;
 }
 
-// Products for few tokens (dense_few.cu); no workspace, any alignment.
-bool few_fits(const Job& j);
+// Products for few tokens (dense_few.cu); no workspace, any alignment.  alone: a single product, not one of a block's two.
+bool few_fits(const Job& j, bool alone);
 // next: the product behind it, whose weights it asks into L2.
 int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream);
 

@@ -1,4 +1,4 @@
-// The products of dense.cuh for at most 16 tokens (fp32: 6): the weights' stream through the warps' registers.
+// The products of dense.cuh for at most 16 tokens: the weights' stream through the warps' registers.
 //
 // Such a call reads every weight once and has nothing else to wait for, so the weights go from memory straight into
 // mma.sync fragments: a lane's 16 bytes of a weight row are eight bf16 (16 codes) in a row, and since a sum over k may
@@ -13,10 +13,13 @@
 // A launch that follows another of the call (programmatic dependent) asks for its first weights before it waits for the
 // tokens that the other one makes.
 //
-// Bound by DRAM while it streams (92 MB a product and more: 5 TB/s), by launch, first and last loads and the joining of
-// sums in small products: one token through a 2048 x 5632 block 21 us in bf16 (69 MB; 10.6 at the copy rate), 17 us with
-// 8-bit weights (four launches); 16 tokens 28 us.  fp32 weights are multiplied on the CUDA cores (1 token 48 us, 4
-// tokens 85 us: the tokens' loads).
+// fp32: both sides as three bf16 terms each, made in registers; the six products of terms down to 2^-16 of the largest
+// (what is left out is below 2^-22 of it), since the CUDA cores took 8 tokens' loads of x for each weight (133 us, now 41).
+//
+// Bound by DRAM while it streams (92 MB a product and more: 5 to 6 TB/s), by launch, first and last loads and the joining of
+// sums in small products: one token through a 2048 x 5632 block 18.4 us in bf16 (69 MB; 10.6 at the copy rate), 15.8 us with
+// 8-bit weights (four launches); 16 tokens 23.4 us.  fp32 40 us for up to 8 tokens (138 MB; 28 with one product of terms, 33
+// with three: the MMAs and the splitting), 16 tokens 53 us.
 #include "dense.cuh"
 
 #include <cooperative_groups.h>
@@ -130,9 +133,10 @@ __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162floa
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// NT groups of eight tokens.
+// NT groups of eight tokens.  (Two: four CTAs an SM, 16 tokens through a 2048 x 5632 bf16 block 23.3 us, 25.5 with the three
+// that 70 registers a thread let in; one group loses by any such bound.)
 template <typename T, typename O, int EPI, int NT, bool kVecW, bool kVecX>
-__global__ void __launch_bounds__(32 * kWarps) few_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 4 : 0) few_kernel(const __grid_constant__ Params p) {
   using Acc = typename Traits<T>::Acc;
   constexpr int V = Traits<T>::kVals;
   constexpr int STEP = 4 * V;  // k of a step: 64 bytes of a row
@@ -345,17 +349,17 @@ int by_tokens(Params& p, bool vw, bool vx, bool pdl, cudaStream_t stream) {
 
 }  // namespace few
 
-bool few_fits(const Job& j) {
-  // Against the tensor-memory products, us (sets of weights larger than L2, 2048 wide): bf16 block of 5632 16 tokens
-  // 28 | 31, 24 tokens 37 | 31; of 22528 (92 MB a product at least) 8 tokens 60 | 66, 16 tokens 74 | 66; 8-bit product of
-  // 5632 16 tokens 7 | 10, of 22528 19 | 17, of 151936 (311 MB) 1 token 65 | 58, 16 tokens 84 | 59; fp32 block of 5632 4
-  // tokens 85 | 121, 8 tokens 133 | 121
+bool few_fits(const Job& j, bool alone) {
+  // Against the tensor-memory products, us (sets of weights larger than L2, 2048 wide).  Up to 8 tokens: bf16 block of 5632
+  // 19 | 31, of 45056 99 | 106; 8-bit product of 5632 6 | 10, of 151936 59.5 | 59.  9 to 16 tokens: bf16 block of 5632
+  // 23 | 31, of 22528 (185 MB of gate and up) 66 | 66, of 45056 121 | 107; 8-bit block of 22528 50 | 60; but 8-bit product of
+  // 5632 (12 MB) 7.6 | 9.7, of 11264 11.9 | 11.5, of 45056 29 | 24, whose other form has no operands to lay out.  fp32,
+  // whose other form splits the weights in memory first: block of 5632 1 token 40 | 122, 16 tokens 53 | 122
   const Problem& s = j.prob[0];
-  const int es = j.i8 ? 1 : j.dtype == DSCA_BF16 ? 2 : 4;
-  const int64_t bytes = (int64_t)s.M * s.K * es * (j.epi == kGlu ? 2 : 1);
   if (j.nprob != 1 || s.nseg != 1 || j.epi == kDGlu || s.a[0].mn) return false;
-  if (!j.i8 && j.dtype == DSCA_F32) return s.N <= 16;
-  return s.N <= 8 ? bytes <= (256ll << 20) : s.N <= 16 && bytes <= DSCA_DENSE_FEW_BYTES;
+  if (s.N <= 8 || (!j.i8 && j.dtype == DSCA_F32)) return s.N <= 16;
+  const int64_t bytes = (int64_t)s.M * s.K * (j.i8 ? 1 : 2) * (j.epi == kGlu ? 2 : 1);
+  return s.N <= 16 && bytes <= (alone ? 16ll << 20 : 128ll << 20);
 }
 
 int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {

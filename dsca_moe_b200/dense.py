@@ -116,7 +116,7 @@ def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
     g, u, e = (h + step, h + 2 * step, h + 3 * step) if save else (None, None, None)
     a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h, rows, d, inter,
                        _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
-    if dtype is not _BF16 or not _few(rows, 4 * inter * d):
+    if not _few(rows, 2 * inter * d * x.element_size()):
         ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
     return y, buf

@@ -30,8 +30,8 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 /* Largest width (d, inter, k, n) and number of rows of these entry points. */
 #define DSCA_DENSE_MAX_DIM 1048576
 #define DSCA_DENSE_MAX_ROWS 16777216
-/* Forward calls in bf16 or 8-bit integers need no workspace for at most this many rows, where the weights of each
- * of their products (gate and up together) have at most that many bytes. */
+/* Forward calls need no workspace for at most this many rows, where the weights of each of their products (gate and up
+ * together) have at most that many bytes. */
 #define DSCA_DENSE_FEW_TOKENS 8
 #define DSCA_DENSE_FEW_BYTES 50331648
 
@@ -55,7 +55,7 @@ typedef struct {
   int act;              /* DSCA_GATE_* */
   int64_t ld_x, ld_gate, ld_up, ld_down, ld_y;
   int64_t ld_h;         /* of g, u, h, in elements: rows of h a multiple of 16 bytes apart, at least inter; g, u, h 16-byte aligned */
-  void* workspace;      /* dsca_dense_workspace_bytes(), 256-byte aligned; may be NULL when that is 0 */
+  void* workspace;      /* dsca_gated_ffn_workspace(), 256-byte aligned; may be NULL when that is 0 */
   size_t workspace_bytes;
   int32_t* err;
 } dsca_gated_ffn_args;
