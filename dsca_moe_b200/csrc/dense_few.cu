@@ -14,7 +14,7 @@
 // tokens that the other one makes.
 //
 // fp32: both sides as three bf16 terms each, made in registers; the six products of terms down to 2^-16 of the largest
-// (what is left out is below 2^-22 of it), since the CUDA cores took 8 tokens' loads of x for each weight (133 us, now 41).
+// (what is left out is below 2^-21 of it), since the CUDA cores took 8 tokens' loads of x for each weight (133 us, now 41).
 //
 // Bound by DRAM while it streams (92 MB a product and more: 5 to 6 TB/s), by launch, first and last loads and the joining of
 // sums in small products: one token through a 2048 x 5632 block 18.4 us in bf16 (69 MB; 10.6 at the copy rate), 15.8 us with
