@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   if (warp < kFirstEpi) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
     if (warp == 0) {
-    // ---------------- TMA producer
+      // ---------------- TMA producer
       const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]), full0_even = mapa_shared(full0, 0);
       const uint32_t even = rank == 0;
       int s = 0;
@@ -503,81 +503,81 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         for (int i = 0; i < kStages; ++i)
           if (armed >> i & 1u) drain(full0 + 8 * i, parity >> i & 1u);
     } else if (warp == 1) {
-    // ---------------- MMA issuer (even CTA)
-    if (rank == 0) {
-      const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]);
-      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-      int s = 0, it = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int unit = unit0; ok && unit < P.total; unit += units) {
-        const Tile t = decode(P, unit, kAM, kBN);
-        const Prob& q = P.prob[t.p];
-        // D f32 (1) or s32 (2); A, B bf16 (1) or signed 8-bit (1); majors; N; M = 256
-        const uint32_t idesc = ((IN == kI8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)q.a_mn << 15) |
-                               ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n(q, t, kGluE) >> 3) << 17) | (16u << 24);
-        // descriptors but for the stage, and their steps of one MMA (in 16 bytes: 2 KB or 32 bytes)
-        const uint64_t ad0 = q.a_mn ? sw128_mnmajor_desc(smem_a) : sw128_kmajor_desc(smem_a);
-        const uint64_t bd0 = q.b_mn ? sw128_mnmajor_desc(smem_b) : sw128_kmajor_desc(smem_b);
-        const uint64_t astep = q.a_mn ? 128u : 2u, bstep = q.b_mn ? 128u : 2u;
-        const int kb = q.kb, last_steps = (q.K - (kb - 1) * KE + KS - 1) / KS;
-        BoxAt at(q, t.box0);
-        // an accumulator takes the whole tile, kF32: a chunk of it
-        for (int c0 = t.box0; ok && c0 < t.box1; ++it) {
-          const int c1 = IN == kF32 ? min(t.box1, c0 + R::kChunk) : t.box1;
-          const int acc = it & 1;
-          if (!wait_warp(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(acc * 256);
-          uint32_t used = 0u;
-          for (int b = c0; b < c1; b += kSub) {
-            if (!wait_warp(full0 + 8 * s, ph, abort_flag, P.err)) { ok = false; break; }
-            tc_fence_after();
-            const int nb = min(kSub, c1 - b);
-#pragma unroll
-            for (int h = 0; h < kSub; ++h) {
-              if (h < nb) {
-                const uint64_t ad = ad0 + (uint64_t)((s * kStageBytes + h * kBoxBytes) >> 4);
-                const uint64_t bd = bd0 + (uint64_t)((s * kStageBytes + h * R::kBBytes) >> 4);
-                const int steps = at.k == kb - 1 ? last_steps : 4;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (i < steps) {
-                    const uint64_t ai = ad + astep * i, bi = bd + bstep * i;
-                    if constexpr (IN == kI8) {
-                      umma_i8_pair(one, d, ai, bi, idesc, used);
-                    } else {
-                      umma_pair(one, d, ai, bi, idesc, used);
-                      if constexpr (IN == kF32) {
-                        constexpr uint64_t PA = kBoxBytes >> 4, PB = R::kBBytes >> 4;
-                        umma_pair(one, d + 128u, ai, bi + PB, idesc, used);
-                        umma_pair(one, d + 128u, ai + PA, bi, idesc, 1u);
-                        umma_pair(one, d + 128u, ai, bi + 2 * PB, idesc, 1u);
-                        umma_pair(one, d + 128u, ai + PA, bi + PB, idesc, 1u);
-                        umma_pair(one, d + 128u, ai + 2 * PA, bi, idesc, 1u);
-                      }
-                    }
-                    used = 1u;
-                  }
-                at.next(kb);
-              }
+      // ---------------- MMA issuer (even CTA)
+      if (rank == 0) {
+        const uint32_t full0 = smem_u32(&ctl.full[0]), empty0 = smem_u32(&ctl.empty[0]);
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+        int s = 0, it = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int unit = unit0; ok && unit < P.total; unit += units) {
+          const Tile t = decode(P, unit, kAM, kBN);
+          const Prob& q = P.prob[t.p];
+          // D f32 (1) or s32 (2); A, B bf16 (1) or signed 8-bit (1); majors; N; M = 256
+          const uint32_t idesc = ((IN == kI8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)q.a_mn << 15) |
+                                 ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n(q, t, kGluE) >> 3) << 17) | (16u << 24);
+          // descriptors but for the stage, and their steps of one MMA (in 16 bytes: 2 KB or 32 bytes)
+          const uint64_t ad0 = q.a_mn ? sw128_mnmajor_desc(smem_a) : sw128_kmajor_desc(smem_a);
+          const uint64_t bd0 = q.b_mn ? sw128_mnmajor_desc(smem_b) : sw128_kmajor_desc(smem_b);
+          const uint64_t astep = q.a_mn ? 128u : 2u, bstep = q.b_mn ? 128u : 2u;
+          const int kb = q.kb, last_steps = (q.K - (kb - 1) * KE + KS - 1) / KS;
+          BoxAt at(q, t.box0);
+          // an accumulator takes the whole tile, kF32: a chunk of it
+          for (int c0 = t.box0; ok && c0 < t.box1; ++it) {
+            const int c1 = IN == kF32 ? min(t.box1, c0 + R::kChunk) : t.box1;
+            const int acc = it & 1;
+            if (!wait_warp(smem_u32(&ctl.tmem_empty[acc]), (uint32_t)(((it >> 1) & 1) ^ 1), abort_flag, P.err)) {
+              ok = false;
+              break;
             }
-            commit_both(one, empty0 + 8 * s);
-            if (++s == kStages) { s = 0; ph ^= 1u; }
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(acc * 256);
+            uint32_t used = 0u;
+            for (int b = c0; b < c1; b += kSub) {
+              if (!wait_warp(full0 + 8 * s, ph, abort_flag, P.err)) { ok = false; break; }
+              tc_fence_after();
+              const int nb = min(kSub, c1 - b);
+#pragma unroll
+              for (int h = 0; h < kSub; ++h) {
+                if (h < nb) {
+                  const uint64_t ad = ad0 + (uint64_t)((s * kStageBytes + h * kBoxBytes) >> 4);
+                  const uint64_t bd = bd0 + (uint64_t)((s * kStageBytes + h * R::kBBytes) >> 4);
+                  const int steps = at.k == kb - 1 ? last_steps : 4;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (i < steps) {
+                      const uint64_t ai = ad + astep * i, bi = bd + bstep * i;
+                      if constexpr (IN == kI8) {
+                        umma_i8_pair(one, d, ai, bi, idesc, used);
+                      } else {
+                        umma_pair(one, d, ai, bi, idesc, used);
+                        if constexpr (IN == kF32) {
+                          constexpr uint64_t PA = kBoxBytes >> 4, PB = R::kBBytes >> 4;
+                          umma_pair(one, d + 128u, ai, bi + PB, idesc, used);
+                          umma_pair(one, d + 128u, ai + PA, bi, idesc, 1u);
+                          umma_pair(one, d + 128u, ai, bi + 2 * PB, idesc, 1u);
+                          umma_pair(one, d + 128u, ai + PA, bi + PB, idesc, 1u);
+                          umma_pair(one, d + 128u, ai + 2 * PA, bi, idesc, 1u);
+                        }
+                      }
+                      used = 1u;
+                    }
+                  at.next(kb);
+                }
+              }
+              commit_both(one, empty0 + 8 * s);
+              if (++s == kStages) { s = 0; ph ^= 1u; }
+            }
+            if (!ok) break;
+            commit_both(one, smem_u32(&ctl.tmem_full[acc]));
+            c0 = c1;
           }
-          if (!ok) break;
-          commit_both(one, smem_u32(&ctl.tmem_full[acc]));
-          c0 = c1;
+        }
+        if (!ok) {  // every MMA issued has completed before TMEM is freed
+          if (lane == 0) umma_commit_pair(mapa_shared(smem_u32(&ctl.mma_done), 0));
+          drain(smem_u32(&ctl.mma_done), 0);
         }
       }
-      if (!ok) {  // every MMA issued has completed before TMEM is freed
-        if (lane == 0) umma_commit_pair(mapa_shared(smem_u32(&ctl.mma_done), 0));
-        drain(smem_u32(&ctl.mma_done), 0);
-      }
-    }
     }
   } else {
     // ---------------- epilogue
