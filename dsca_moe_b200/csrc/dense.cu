@@ -188,7 +188,7 @@ Operand as(Operand o, int mn) {
 int run(Call& c, const dsca_gated_ffn_args* a) {
   const int dt = a->dtype, T = a->rows, d = a->d, I = a->inter;
   Job j = {}, k = {};
-  if (T <= 16) {
+  if (T <= 32) {
     j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = dt;
     j.prob[0] = problem({a->w_gate, a->ld_gate, 0, 0}, {a->x, a->ld_x, 0, 0}, I, T, d, a->h, a->ld_h);
     j.prob[0].a[1] = {a->w_up, a->ld_up, 0, 0};

@@ -1,4 +1,4 @@
-// The products of dense.cuh for at most 16 tokens: the weights' stream through the warps' registers.
+// The products of dense.cuh for at most 16 tokens (fp32: 32): the weights' stream through the warps' registers.
 //
 // Such a call reads every weight once and has nothing else to wait for, so the weights go from memory straight into
 // mma.sync fragments: a lane's 16 bytes of a weight row are eight bf16 (16 codes) in a row, and since a sum over k may
@@ -19,7 +19,7 @@
 // Bound by DRAM while it streams (92 MB a product and more: 5 to 6 TB/s), by launch, first and last loads and the joining of
 // sums in small products: one token through a 2048 x 5632 block 18.4 us in bf16 (69 MB; 10.6 at the copy rate), 15.8 us with
 // 8-bit weights (four launches); 16 tokens 23.4 us.  fp32 40 us for up to 8 tokens (138 MB; 28 with one product of terms, 33
-// with three: the MMAs and the splitting), 16 tokens 53 us.
+// with three: the MMAs and the splitting), 16 tokens 53 us, 24 67 us, 32 82 us.
 #include "dense.cuh"
 
 #include <cooperative_groups.h>
@@ -134,9 +134,10 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // NT groups of eight tokens.  (Two: four CTAs an SM, 16 tokens through a 2048 x 5632 bf16 block 23.3 us, 25.5 with the three
-// that 70 registers a thread let in; one group loses by any such bound.)
+// that 70 registers a thread let in; three and four, fp32: two CTAs, 32 tokens 82 us, 103 without, for all that two values
+// a thread are spilled; one group loses by any such bound.)
 template <typename T, typename O, int EPI, int NT, bool kVecW, bool kVecX>
-__global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 4 : 0) few_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 0 : NT == 2 ? 4 : 2) few_kernel(const __grid_constant__ Params p) {
   using Acc = typename Traits<T>::Acc;
   constexpr int V = Traits<T>::kVals;
   constexpr int STEP = 4 * V;  // k of a step: 64 bytes of a row
@@ -344,6 +345,10 @@ int by_vec(Params& p, bool vw, bool vx, bool pdl, cudaStream_t stream) {
 template <typename T, typename O, int EPI>
 int by_tokens(Params& p, bool vw, bool vx, bool pdl, cudaStream_t stream) {
   if (p.T <= 8) return by_vec<T, O, EPI, 1>(p, vw, vx, pdl, stream);
+  if constexpr (std::is_same<T, float>::value) {
+    if (p.T > 24) return by_vec<T, O, EPI, 4>(p, vw, vx, pdl, stream);
+    if (p.T > 16) return by_vec<T, O, EPI, 3>(p, vw, vx, pdl, stream);
+  }
   return by_vec<T, O, EPI, 2>(p, vw, vx, pdl, stream);
 }
 
@@ -354,10 +359,11 @@ bool few_fits(const Job& j, bool alone) {
   // 19 | 31, of 45056 99 | 106; 8-bit product of 5632 6 | 10, of 151936 59.5 | 59.  9 to 16 tokens: bf16 block of 5632
   // 23 | 31, of 22528 (185 MB of gate and up) 66 | 66, of 45056 121 | 107; 8-bit block of 22528 50 | 60; but 8-bit product of
   // 5632 (12 MB) 7.6 | 9.7, of 11264 11.9 | 11.5, of 45056 29 | 24, whose other form has no operands to lay out.  fp32,
-  // whose other form splits the weights in memory first: block of 5632 1 token 40 | 122, 16 tokens 53 | 122
+  // whose other form splits the weights in memory first: block of 5632 1 token 40 | 122, 16 tokens 53 | 122,
+  // 24 67 | 122, 32 82 | 122; of 11008 (4096 wide) 32 271 | 417; 712 x 1021 32 18 | 33
   const Problem& s = j.prob[0];
   if (j.nprob != 1 || s.nseg != 1 || j.epi == kDGlu || s.a[0].mn) return false;
-  if (s.N <= 8 || (!j.i8 && j.dtype == DSCA_F32)) return s.N <= 16;
+  if (s.N <= 8 || (!j.i8 && j.dtype == DSCA_F32)) return s.N <= 32;
   const int64_t bytes = (int64_t)s.M * s.K * (j.i8 ? 1 : 2) * (j.epi == kGlu ? 2 : 1);
   return s.N <= 16 && bytes <= (alone ? 16ll << 20 : 128ll << 20);
 }
