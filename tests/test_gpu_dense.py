@@ -276,6 +276,28 @@ def test_quantize_long_rows(cuda, rows, k, gap, dtype):
         assert not q2[rows // 2].any() and not torch.isfinite(s2[rows // 2])
 
 
+@pytest.mark.parametrize("T", [1, 8, 11, 24, 32, 33])
+@pytest.mark.parametrize("d,I", [(256, 320), (101, 67)])
+def test_f32_few_tokens_range(cuda, T, d, I):
+    """fp32 values of every size, the largest among them, and rows that are not finite beside rows that are."""
+    from dsca_moe_b200 import gated_ffn
+
+    x, wg, wu, wd, _ = _inputs(cuda, T, d, I, F32)
+    for sx, sw in ((2.0 ** 40, 1.0), (2.0 ** -30, 1.0), (2.0 ** -60, 2.0 ** 60)):
+        args = (x * sx, wg * sw, wu * sw, wd)
+        R.close(gated_ffn(*args, act="relu"), R.ffn(*args, "relu", F32)["y"], (sx, sw))
+    big = wg.clone()
+    big[I // 2, d // 3] = torch.finfo(F32).max  # no bf16 is as large
+    args = (x * 2.0 ** -100, big, wu, wd)
+    R.close(gated_ffn(*args, act="relu"), R.ffn(*args, "relu", F32)["y"], "largest")
+    want = gated_ffn(x, wg, wu, wd)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        y = x.clone()
+        y[T // 2, d // 2] = bad
+        got, keep = gated_ffn(y, wg, wu, wd), torch.arange(T, device=cuda) != T // 2
+        assert not torch.isfinite(got[T // 2]).any() and torch.equal(got[keep], want[keep])
+
+
 INT8_SHAPES = [(1, 16, 1), (1, 2048, 5632), (1, 33, 77), (4, 1021, 130), (8, 5632, 2048), (9, 256, 1000), (16, 128, 64),
                (20, 2048, 901), (32, 4100, 300), (33, 100, 257), (64, 512, 512), (100, 1021, 1363), (129, 144, 2000),
                (257, 2048, 264), (777, 1021, 1363), (1030, 640, 768)]
