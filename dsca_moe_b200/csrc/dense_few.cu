@@ -358,7 +358,8 @@ bool few_fits(const Job& j, bool alone) {
   // Against the tensor-memory products, us (sets of weights larger than L2, 2048 wide).  Up to 8 tokens: bf16 block of 5632
   // 19 | 31, of 45056 99 | 106; 8-bit product of 5632 6 | 10, of 151936 59.5 | 59.  9 to 16 tokens: bf16 block of 5632
   // 23 | 31, of 22528 (185 MB of gate and up) 66 | 66, of 45056 121 | 107; 8-bit block of 22528 50 | 60; but 8-bit product of
-  // 5632 (12 MB) 7.6 | 9.7, of 11264 11.9 | 11.5, of 45056 29 | 24, whose other form has no operands to lay out.  fp32,
+  // 5632 (12 MB) 7.6 | 9.7, of 11264 11.9 | 11.5, of 45056 29 | 24, whose other form has no operands to lay out.  17 to 24
+  // tokens: bf16 block of 5632 33 | 31, 8-bit 28 | 29, 8-bit product 10.8 | 9.8.  fp32,
   // whose other form splits the weights in memory first: block of 5632 1 token 40 | 122, 16 tokens 53 | 122,
   // 24 67 | 122, 32 82 | 122; of 11008 (4096 wide) 32 271 | 417; 712 x 1021 32 18 | 33
   const Problem& s = j.prob[0];
