@@ -151,10 +151,13 @@ __device__ __forceinline__ Tile decode(const Params& P, int unit, int am, int bn
 }
 
 // MMA N of a tile: each CTA holds half of B's rows, whole 8-row groups (64 rows if MN-major); the rows form of a
-// gated product always takes the whole tile
-__device__ __forceinline__ int mma_n(const Prob& q, const Tile& t, bool glu) {
+// gated product always takes the whole tile.  A pair's 8-bit MMAs of 256 rows have N in steps of 32, its 16-bit ones of
+// 16; every tile's width (and with it the boxes that land) is a multiple of 32, so the rounded N stays inside it.
+template <int IN>
+__host__ __device__ __forceinline__ int mma_n(const Prob& q, int nval, bool glu) {
+  constexpr int kStep = IN == kI8 ? 32 : 16;
   if (glu && q.row) return q.tn;
-  return q.b_mn ? (t.nval + 127) & ~127 : max(16, (t.nval + 15) & ~15);
+  return q.b_mn ? (nval + 127) & ~127 : (nval + kStep - 1) & ~(kStep - 1);
 }
 
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         const Tile t = decode(P, unit, kAM, kBN);
         const Prob& q = P.prob[t.p];
         const bool glu_rows = kGluE && q.row;
-        const int b_row = glu_rows ? t.n0 : t.n0 + mma_n(q, t, kGluE) / 2 * (int)rank;
+        const int b_row = glu_rows ? t.n0 : t.n0 + mma_n<IN>(q, t.nval, kGluE) / 2 * (int)rank;
         const int a_row = kGluE && !q.row ? t.m0 + 64 * (int)rank : t.m0 + 128 * (int)rank;
         const uint32_t b_bytes = (uint32_t)(q.tn / 2) * 128u;  // a whole box lands; rows past the tile are not used
         const int kb = q.kb, a_mn = q.a_mn, b_atoms = q.b_mn ? q.tn / 128 : 0, a_plane = q.a_plane, b_plane = q.b_plane;
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           const Prob& q = P.prob[t.p];
           // D f32 (1) or s32 (2); A, B bf16 (1) or signed 8-bit (1); majors; N; M = 256
           const uint32_t idesc = ((IN == kI8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)q.a_mn << 15) |
-                                 ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n(q, t, kGluE) >> 3) << 17) | (16u << 24);
+                                 ((uint32_t)q.b_mn << 16) | ((uint32_t)(mma_n<IN>(q, t.nval, kGluE) >> 3) << 17) | (16u << 24);
           // descriptors but for the stage, and their steps of one MMA (in 16 bytes: 2 KB or 32 bytes)
           const uint64_t ad0 = q.a_mn ? sw128_mnmajor_desc(smem_a) : sw128_kmajor_desc(smem_a);
           const uint64_t bd0 = q.b_mn ? sw128_mnmajor_desc(smem_b) : sw128_kmajor_desc(smem_b);
@@ -593,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       const int64_t lrow = t.m0 + 128 * (int)rank + 32 * q4 + lane;  // rows form: this lane's output row
       if constexpr (EPI == kDGlu && IN == kBf16)
         if (q.row) ahead.load(P, q, lrow, t.n0 + 32 * eh, t.n0 + t.nval);
-      const int ncol = mma_n(q, t, kGluE);
+      const int ncol = mma_n<IN>(q, t.nval, kGluE);
       uint32_t taddr = 0;
       float fs[2][32];  // kF32: the sums of this warp's two chunks of columns
       if constexpr (IN == kF32) {
