@@ -43,6 +43,7 @@ struct Job {
   uint8_t* save_e;
   void* out2;     // kDGlu: du
   const float* row_scale;
+  const float* row_max;  // kGlu of 8-bit operands, instead of row_scale: the rows' largest magnitudes; out is held in 64 bits
   const float* col_scale[2];
   const void* bias;
 };
@@ -74,6 +75,19 @@ __device__ __forceinline__ float gate(float g, int act) {
   if (act == DSCA_GATE_SILU) return kFast ? g * sigmoid<true>(g) : g / (1.0f + expf(-g));
   if (act == DSCA_GATE_RELU) return g <= 0.0f ? 0.0f : g;  // NaN stays
   return g * gelu_p<kFast>(g);
+}
+
+// The gate in 64 bits.
+__device__ __forceinline__ double gate64(double g, int act) {
+  if (act == DSCA_GATE_RELU) return g <= 0.0 ? 0.0 : g;
+  const double z = act == DSCA_GATE_SILU ? g : 2.0 * 0.7978845608028654 * (g + 0.044715 * g * g * g);
+  const double e = exp(-fabs(z));  // sigmoid(z), which does not cancel on either side
+  return g * ((z >= 0.0 ? 1.0 : e) / (1.0 + e));
+}
+
+// h = act(g) u of two exact sums of codes in 64 bits; xs: the token's scale, max|x| / 127.
+__device__ __forceinline__ double h64(int sum_g, int sum_u, double xs, double gs, double us, int act) {
+  return gate64((double)sum_g * xs * gs, act) * ((double)sum_u * xs * us);
 }
 
 // act(g) and act'(g)
@@ -131,7 +145,11 @@ int launch_relay(RelayList& list, cudaStream_t stream);
 // at the launch.
 int tc_workspace(const Job& j, size_t* parts, size_t* counters);
 int launch_tc(const Job& j, void* parts, void* counters, int32_t* err, bool pdl, cudaStream_t stream);
-int launch_quantize_rows(const dsca_quantize_rows_args* a, bool pdl, cudaStream_t stream);
+// row_max (or NULL): the rows' largest magnitudes as well.
+int launch_quantize_rows(const dsca_quantize_rows_args* a, float* row_max, bool pdl, cudaStream_t stream);
+// Rows of 64-bit values (as kGlu with row_max leaves them), ld a multiple of 16.
+int launch_quantize_rows64(const double* x, int rows, int k, int64_t ld, int8_t* q, int64_t ld_q, float* scale, bool pdl,
+                           cudaStream_t stream);
 
 }  // namespace dense
 }  // namespace dsca

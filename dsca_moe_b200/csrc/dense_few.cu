@@ -47,7 +47,7 @@ struct Params {
   void* save_u;
   uint8_t* save_e;
   int groups;  // exponents of a saved row
-  const float* row_scale;
+  const float* row_scale;  // O = double: row_max
   const float* col_scale[2];
   const void* bias;
   const uint8_t* ahead;  // the next product's weights: asked into L2 by this one's CTAs, `ahead_step` bytes each
@@ -132,6 +132,7 @@ __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(double* p, float v) { *p = v; }
 
 // NT groups of eight tokens.  (Two: four CTAs an SM, 16 tokens through a 2048 x 5632 bf16 block 23.3 us, 25.5 with the three
 // that 70 registers a thread let in; three and four, fp32: two CTAs, 32 tokens 82 us, 103 without, for all that two values
@@ -270,8 +271,15 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 0 : NT == 2 ? 4 : 2) fe
       va += part[c][n];
       if constexpr (kGluE) vb += part[c + 8][n];
     }
-    float v = (float)va, u = (float)vb;
     const bool in = m < p.M;
+    if constexpr (std::is_same<O, double>::value) {
+      if (in) {
+        const double xs = (double)p.row_scale[n] / 127.0;
+        reinterpret_cast<double*>(p.out)[(int64_t)n * p.ldo + m] = h64(va, vb, xs, p.col_scale[0][m], p.col_scale[1][m], p.act);
+      }
+      continue;
+    }
+    float v = (float)va, u = (float)vb;
     if constexpr (std::is_same<T, int8_t>::value) {
       const float rs = p.row_scale[n];
       v *= in ? p.col_scale[0][m] * rs : 0.0f;
@@ -383,7 +391,7 @@ int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   p.act = j.act;
   p.out = s.out; p.ldo = s.ldo;
   p.save_g = j.save_g; p.save_u = j.save_u; p.save_e = j.save_e; p.groups = exp_groups(s.M);
-  p.row_scale = j.row_scale; p.col_scale[0] = j.col_scale[0]; p.col_scale[1] = j.col_scale[1]; p.bias = j.bias;
+  p.row_scale = j.row_max != nullptr ? j.row_max : j.row_scale; p.col_scale[0] = j.col_scale[0]; p.col_scale[1] = j.col_scale[1]; p.bias = j.bias;
   if (next != nullptr) {
     const Operand& w = next->prob[0].a[0];
     const int64_t bytes = ((next->prob[0].M - 1) * w.ld + next->prob[0].K) * es & ~15ll;  // up to the last row's end
@@ -395,7 +403,9 @@ int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   }
   using B = __nv_bfloat16;
   if (j.i8) {
-    if (j.epi == kGlu) return few::by_tokens<int8_t, float, kGlu>(p, true, true, pdl, stream);
+    if (j.epi == kGlu)
+      return j.row_max != nullptr ? few::by_tokens<int8_t, double, kGlu>(p, true, true, pdl, stream)
+                                  : few::by_tokens<int8_t, float, kGlu>(p, true, true, pdl, stream);
     return j.dtype == DSCA_BF16 ? few::by_tokens<int8_t, B, kStore>(p, true, true, pdl, stream)
                                 : few::by_tokens<int8_t, float, kStore>(p, true, true, pdl, stream);
   }

@@ -134,7 +134,7 @@ constexpr bool in_ring() { return kVec && TPR * CH > 256 && sizeof(T) == 2; }
 constexpr int kDepth = 2;
 
 template <typename T, int TPR, int CH, bool kVec>
-__global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a) {
+__global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a, float* row_max) {
   __shared__ uint32_t red[2][8];
   extern __shared__ uint4 ring[];  // [kDepth][CH][256], each thread's own chunks
   constexpr int kRows = 256 / TPR, N = CH > 0 ? CH : 1;
@@ -206,7 +206,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
       slot ^= 1;
     }
     if (!live) continue;
-    if (tid == 0) a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
+    if (tid == 0) {
+      a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
+      if (row_max != nullptr) row_max[row] = m;
+    }
     // codes mean nothing in a row that is not finite: zeros
     const bool usable = m > 0.0f && m < INFINITY;
     const bool ends = m < 1e-30f || m > 1e36f;  // 127 / m or 127 x leaves fp32's normal numbers
@@ -246,7 +249,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
 }
 
 template <typename T, int TPR, int CH>
-int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
+int launch(const dsca_quantize_rows_args& a, float* row_max, bool pdl, cudaStream_t stream) {
   // CTAs go round, two for each that an SM holds at a time or nearly so (long fp32 rows: 80 registers a thread, three)
   constexpr int kCtas = sizeof(T) == 4 && CH > 2 ? 6 : 8;
   const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, (int64_t)kCtas * current_device_sms());
@@ -262,29 +265,119 @@ int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
   cfg.numAttrs = pdl ? 1 : 0;
   if (vec && in_ring<T, TPR, CH, true>()) cfg.dynamicSmemBytes = (size_t)kDepth * CH * 256 * 16;  // 24 or 32 KB
   auto kern = vec ? quantize_kernel<T, TPR, CH, true> : quantize_kernel<T, TPR, CH, false>;
-  return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kern, a, row_max) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+}
+
+// Rows of 64-bit values: the quotient in 64 bits, divided where the product with 127 / max is next to a tie.  TPR threads a
+// row, four values each at a time; the row is read a second time from L1 or L2.
+template <int TPR>
+__global__ void __launch_bounds__(256) quantize64_kernel(const double* __restrict__ x, int rows, int k, int64_t ld, int8_t* q,
+                                                         int64_t ld_q, float* scale) {
+  __shared__ unsigned long long red[2][8];
+  constexpr int kRows = 256 / TPR;
+  const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
+  const int pieces = (int)(ld_q / 4);
+  pdl_launch_dependents();
+  pdl_wait();
+  int it = 0;
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += (int64_t)gridDim.x * kRows, it ^= 1) {
+    const int64_t row = first + sub;
+    const bool live = row < rows;
+    const double* r = x + (live ? row : 0) * ld;
+    // rows lie on 32-byte boundaries and hold a multiple of 16 values, of which those past k are not written
+    auto load = [&](int c, double (&v)[4]) {
+      const double2 a = c * 4 < k ? *reinterpret_cast<const double2*>(r + c * 4) : make_double2(0.0, 0.0);
+      const double2 b = c * 4 + 2 < k ? *reinterpret_cast<const double2*>(r + c * 4 + 2) : make_double2(0.0, 0.0);
+      v[0] = a.x;
+      v[1] = c * 4 + 1 < k ? a.y : 0.0;
+      v[2] = b.x;
+      v[3] = c * 4 + 3 < k ? b.y : 0.0;
+    };
+    unsigned long long bits = 0;  // of the largest magnitude, a NaN's being the largest
+    if (live) {
+#pragma unroll 4
+      for (int c = tid; c < pieces; c += TPR) {
+        double v[4];
+        load(c, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bits = max(bits, (unsigned long long)__double_as_longlong(fabs(v[e])));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    if constexpr (TPR > 32) {
+      if (threadIdx.x % 32 == 0) red[it][threadIdx.x / 32] = bits;
+      __syncthreads();  // one a row: the next one writes the other half
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) bits = max(bits, red[it][sub * (TPR / 32) + i]);
+    }
+    if (!live) continue;
+    const double m = __longlong_as_double((long long)bits);
+    const float s = (float)(m / 127.0);
+    if (tid == 0) scale[row] = m == 0.0 ? 1.0f : s;
+    const bool usable = m > 0.0 && s < INFINITY;  // codes of other rows mean nothing
+    const double inv = usable ? 127.0 / m : 0.0;
+#pragma unroll 4
+    for (int c = tid; c < pieces; c += TPR) {
+      char4 w = make_char4(0, 0, 0, 0);
+      if (usable) {
+        double v[4];
+        int o[4];
+        load(c, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double p = v[e] * inv;
+          o[e] = __double2int_rn(p);
+          if (fabs(p - (double)o[e]) > 0.5 - 1e-9) o[e] = __double2int_rn(127.0 * v[e] / m);  // p is good to 1e-13
+        }
+        w = make_char4((signed char)o[0], (signed char)o[1], (signed char)o[2], (signed char)o[3]);
+      }
+      *reinterpret_cast<char4*>(q + row * ld_q + c * 4) = w;
+    }
+  }
+}
+
+template <int TPR>
+int launch64(const double* x, int rows, int k, int64_t ld, int8_t* q, int64_t ld_q, float* scale, bool pdl, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(((int64_t)rows * TPR + 255) / 256, (int64_t)8 * current_device_sms()));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, quantize64_kernel<TPR>, x, rows, k, ld, q, ld_q, scale) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
 template <typename T>
-int run(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
+int run(const dsca_quantize_rows_args& a, float* row_max, bool pdl, cudaStream_t stream) {
   const int chunks = (int)(a.ld_q / 8);
   if (a.rows > 4 * current_device_sms()) {  // a warp a row while a warp holds it
-    if (chunks <= 32) return launch<T, 32, 1>(a, pdl, stream);
-    if (chunks <= 64) return launch<T, 32, 2>(a, pdl, stream);
-    if (chunks <= 128) return launch<T, 64, 2>(a, pdl, stream);
-    if (chunks <= 256) return launch<T, 128, 2>(a, pdl, stream);
+    if (chunks <= 32) return launch<T, 32, 1>(a, row_max, pdl, stream);
+    if (chunks <= 64) return launch<T, 32, 2>(a, row_max, pdl, stream);
+    if (chunks <= 128) return launch<T, 64, 2>(a, row_max, pdl, stream);
+    if (chunks <= 256) return launch<T, 128, 2>(a, row_max, pdl, stream);
   }
-  if (chunks <= 256) return launch<T, 256, 1>(a, pdl, stream);
-  if (chunks <= 512) return launch<T, 256, 2>(a, pdl, stream);
-  if (chunks <= 768) return launch<T, 256, 3>(a, pdl, stream);
-  if (chunks <= 1024) return launch<T, 256, 4>(a, pdl, stream);
-  return launch<T, 256, 0>(a, pdl, stream);
+  if (chunks <= 256) return launch<T, 256, 1>(a, row_max, pdl, stream);
+  if (chunks <= 512) return launch<T, 256, 2>(a, row_max, pdl, stream);
+  if (chunks <= 768) return launch<T, 256, 3>(a, row_max, pdl, stream);
+  if (chunks <= 1024) return launch<T, 256, 4>(a, row_max, pdl, stream);
+  return launch<T, 256, 0>(a, row_max, pdl, stream);
 }
 
 }  // namespace quant
 
-int launch_quantize_rows(const dsca_quantize_rows_args* a, bool pdl, cudaStream_t stream) {
-  return a->dtype == DSCA_BF16 ? quant::run<__nv_bfloat16>(*a, pdl, stream) : quant::run<float>(*a, pdl, stream);
+int launch_quantize_rows(const dsca_quantize_rows_args* a, float* row_max, bool pdl, cudaStream_t stream) {
+  return a->dtype == DSCA_BF16 ? quant::run<__nv_bfloat16>(*a, row_max, pdl, stream) : quant::run<float>(*a, row_max, pdl, stream);
+}
+
+int launch_quantize_rows64(const double* x, int rows, int k, int64_t ld, int8_t* q, int64_t ld_q, float* scale, bool pdl,
+                           cudaStream_t stream) {
+  // a warp a row where there are rows for all of them and the rows are short
+  return k <= 1024 && rows > 4 * current_device_sms() ? quant::launch64<32>(x, rows, k, ld, q, ld_q, scale, pdl, stream)
+                                                      : quant::launch64<256>(x, rows, k, ld, q, ld_q, scale, pdl, stream);
 }
 
 }  // namespace dense

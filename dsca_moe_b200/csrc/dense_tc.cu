@@ -108,7 +108,7 @@ struct Params {
   void* save_u;
   uint8_t* save_e;  // fp16: the exponents, [2][rows][exp_groups(cols)]
   void* out2;
-  const float* row_scale;
+  const float* row_scale;  // O = double: row_max
   const float* col_scale[2];
   const void* bias;
   int vec_cols;  // col_scale on 16-byte boundaries
@@ -399,6 +399,12 @@ struct Ahead {
   }
 };
 
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
 template <int EPI, int IN, typename O>
 __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params P) {
   constexpr bool kGluE = EPI == kGlu;
@@ -409,6 +415,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   constexpr int KE = IN == kI8 ? 128 : 64;   // k elements of a box
   constexpr int KS = IN == kI8 ? 32 : 16;    // ... and of one MMA
   constexpr bool kFast = IN != kF32;
+  constexpr bool kWide = sizeof(O) == 8;     // h of 8-bit products in 64 bits
+  static_assert(!kWide || (kGluE && IN == kI8), "64-bit results");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -707,7 +715,77 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           }
         }
       };
-      if (mine && q.row) {
+      // eight columns, of 8-bit operands
+      auto finished8 = [&](int c, uint32_t (&r)[8]) {
+        if (q.splits == 1) {
+          tmem_ld8(taddr + c, r);
+          tmem_wait_ld();
+          return;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = 0u;
+        for (int s = 0; s < q.splits; ++s) {
+          const float* at = part + s * part_step + (int64_t)c * 128;
+          const uint4 a = __ldcg(reinterpret_cast<const uint4*>(at)), b = __ldcg(reinterpret_cast<const uint4*>(at + 512));
+          r[0] += a.x; r[1] += a.y; r[2] += a.z; r[3] += a.w;
+          r[4] += b.x; r[5] += b.y; r[6] += b.z; r[7] += b.w;
+        }
+      };
+      if constexpr (kWide) {
+        // ------------ h in 64 bits, eight values of a row (rows) or of a column (columns) at a time
+        if (mine && q.row) {
+          const bool live = lrow < q.rows;
+          const double xs = live ? (double)__ldg(P.row_scale + lrow) / 127.0 : 0.0;
+          double* out = reinterpret_cast<double*>(q.out) + lrow * q.ldo;
+#pragma unroll 1
+          for (int c = 32 * eh; c < min(q.tn / 2, t.nval); c += c % 32 == 24 ? 40 : 8) {  // alternate chunks of 32
+            uint32_t g[8], u[8];
+            finished8(c, g);
+            finished8(c + q.tn / 2, u);
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 8; i += 4) {
+                const int n = t.n0 + c + i;
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int at = min(n + j, q.cols - 1);
+                  const double h = h64((int)g[i + j], (int)u[i + j], xs, __ldg(P.col_scale[0] + at), __ldg(P.col_scale[1] + at), P.act);
+                  w[2 * j] = (uint32_t)__double2loint(h);
+                  w[2 * j + 1] = (uint32_t)__double2hiint(h);
+                }
+                // (rows hold a multiple of 16 values and start on 32-byte boundaries)
+                if (n < q.cols) store32(out + n, w);
+              }
+            }
+          }
+        } else if (mine) {
+          const int ch = t.m0 + 64 * (int)rank + 32 * (q4 & 1) + lane, up = q4 >> 1;
+          const bool in = ch < q.cols;
+          const double gs = in ? __ldg(P.col_scale[0] + ch) : 0.0f, us = in ? __ldg(P.col_scale[1] + ch) : 0.0f;
+#pragma unroll 1
+          for (int c = 32 * eh; c < t.nval; c += c % 32 == 24 ? 40 : 8) {
+            uint32_t r[8];
+            finished8(c, r);
+            // the gate warp forms the first four tokens, the up warp the others (two buffers: one barrier a step)
+            uint32_t* mine_x = reinterpret_cast<uint32_t*>(stg) + xb * 512;
+            const uint32_t* other_x = reinterpret_cast<const uint32_t*>(smem + kRingBytes + (ew ^ 2) * kStgBytes) + xb * 512;
+            xb ^= 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mine_x[j * 32 + lane] = up ? r[j] : r[4 + j];
+            pair_barrier(pair_id);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t got = other_x[j * 32 + lane];
+              const int tok = c + 4 * up + j;
+              if (in && tok < t.nval)
+                reinterpret_cast<double*>(q.out)[(int64_t)(t.n0 + tok) * q.ldo + ch] =
+                    h64((int)(up ? got : r[j]), (int)(up ? r[4 + j] : got), (double)__ldg(P.row_scale + t.n0 + tok) / 127.0, gs, us,
+                        P.act);
+            }
+          }
+        }
+      } else if (mine && q.row) {
         // ------------ rows: this lane's row, 32 of its values at a time
         const bool live = lrow < q.rows;
         O* out = reinterpret_cast<O*>(q.out) + lrow * q.ldo;
@@ -1074,7 +1152,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     q = Prob{};
     const bool glu = j.epi == kGlu;
     q.rows = s.N; q.cols = s.M; q.K = s.K;
-    const int oes = j.dtype == DSCA_BF16 ? 2 : 4;
+    const int oes = j.row_max != nullptr ? 8 : j.dtype == DSCA_BF16 ? 2 : 4;
     auto on = [&](const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
     auto rows_on = [&](int64_t n) {
       return s.ldo * oes % n == 0 && on(s.out, n) && on(j.out2, n) && on(j.save_g, n) && on(j.save_u, n);
@@ -1200,14 +1278,16 @@ int launch_tc(const Job& j, void* parts, void* counts, int32_t* err, bool pdl, c
   }
   P.act = j.act;
   P.save_g = j.save_g; P.save_u = j.save_u; P.save_e = j.save_e; P.out2 = j.out2;
-  P.row_scale = j.row_scale; P.col_scale[0] = j.col_scale[0]; P.col_scale[1] = j.col_scale[1]; P.bias = j.bias;
+  P.row_scale = j.row_max != nullptr ? j.row_max : j.row_scale; P.col_scale[0] = j.col_scale[0]; P.col_scale[1] = j.col_scale[1]; P.bias = j.bias;
   P.vec_cols = (reinterpret_cast<uintptr_t>(j.col_scale[0]) | reinterpret_cast<uintptr_t>(j.col_scale[1])) % 16 == 0;
   P.counters = reinterpret_cast<uint32_t*>(counts);
   P.parts = reinterpret_cast<float*>(parts);
   P.err = err;
   using B = __nv_bfloat16;
   if (j.i8) {
-    if (j.epi == kGlu) return tc::launch<kGlu, tc::kI8, float>(P, pairs, pdl, stream);
+    if (j.epi == kGlu)
+      return j.row_max != nullptr ? tc::launch<kGlu, tc::kI8, double>(P, pairs, pdl, stream)
+                                  : tc::launch<kGlu, tc::kI8, float>(P, pairs, pdl, stream);
     return j.dtype == DSCA_BF16 ? tc::launch<kStore, tc::kI8, B>(P, pairs, pdl, stream)
                                 : tc::launch<kStore, tc::kI8, float>(P, pairs, pdl, stream);
   }

@@ -332,8 +332,10 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
 def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down: Int8Weight,
                    act: str = "silu") -> torch.Tensor:
     """gated_ffn with its weights in 8-bit integers (pack_int8): x's rows are quantised, the gated
-    intermediate is formed in fp32 and its rows quantised in turn.  x [..., d] bf16 or fp32; y has its
-    shape and type.  Inference only."""
+    intermediate is formed and its rows quantised in turn.  x [..., d] bf16 or fp32; y has its shape and
+    type.  fp32 tokens: the intermediate is formed in 64 bits, so that its codes are those of the
+    definition.  bf16 tokens: it is formed in fp32, with gates good to 2^-18 of their value, and a code next
+    to a border may lie on its other side, which moves y by about one of its roundings.  Inference only."""
     code = _act(act)
     dt = _DTYPES.get(x.dtype)
     if dt is None:
@@ -350,17 +352,18 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     if rows == 0:
         return y
     ld_q, ld_hq = (d + 15) // 16 * 16, (inter + 15) // 16 * 16
-    # one buffer: h, the two sets of codes, the two sets of scales
-    buf = torch.empty(rows * (5 * ld_hq + ld_q + 8), dtype=torch.uint8, device=dev)
+    # one buffer: h (fp32 tokens': in 64 bits, in the workspace), the two sets of codes, the two sets of scales
+    h_bytes = 0 if dt == L.F32 else 4 * ld_hq
+    buf = torch.empty(rows * (h_bytes + ld_hq + ld_q + 8), dtype=torch.uint8, device=dev)
     h = buf.data_ptr()
-    hq = h + rows * 4 * ld_hq
+    hq = h + rows * h_bytes
     q = hq + rows * ld_hq
     scale = q + rows * ld_q
     a = L.GatedFfnInt8Args(x.data_ptr(), q, scale, w_gate[0].data_ptr(), w_up[0].data_ptr(), w_down[0].data_ptr(),
                            w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr(), h, hq, scale + 4 * rows,
                            y.data_ptr(), rows, d, inter, dt, code, ld_x, ld_q, ld_gate, ld_up, ld_down, ld_hq, ld_hq, d,
                            None, 0, _err(dev))
-    if not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
+    if dt == L.F32 or not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
         ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
     return y

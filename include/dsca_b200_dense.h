@@ -31,7 +31,7 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 #define DSCA_DENSE_MAX_DIM 1048576
 #define DSCA_DENSE_MAX_ROWS 16777216
 /* Forward calls need no workspace for at most this many rows, where the weights of each of their products (gate and up
- * together) have at most that many bytes. */
+ * together) have at most that many bytes; but dsca_gated_ffn_int8 with DSCA_F32 always takes one. */
 #define DSCA_DENSE_FEW_TOKENS 8
 #define DSCA_DENSE_FEW_BYTES 50331648
 
@@ -123,8 +123,9 @@ typedef struct {
 } dsca_int8_linear_args;
 
 /*
- * dsca_gated_ffn with its weights in 8-bit integers: x quantised by rows, h = act(g) * u in fp32
- * (a work area), quantised by rows, then the down product.
+ * dsca_gated_ffn with its weights in 8-bit integers: x quantised by rows, h = act(g) * u, quantised by rows, then the down
+ * product.  DSCA_F32: h in 64 bits (in the workspace), from the exact sums and the scale max|x| / 127 unrounded.  DSCA_BF16: h in
+ * fp32 (a work area), its gate good to 2^-18, so that a code next to a border may lie on its other side.
  */
 typedef struct {
   const void* x;        /* [rows, d], dtype */
@@ -136,7 +137,7 @@ typedef struct {
   const float* gate_scale; /* [inter] */
   const float* up_scale;
   const float* down_scale; /* [d] */
-  float* h;             /* work area [rows, ld_h] */
+  float* h;             /* work area [rows, ld_h], DSCA_F32: not touched */
   int8_t* hq;           /* work area [rows, ld_hq] */
   float* h_scale;       /* work area [rows] */
   void* y;              /* [rows, d], dtype */

@@ -27,3 +27,67 @@ def test_int8_partial_tiles(cuda, T, k, n):
     q, s = quantize_rows(x)
     R.close(int8_linear(x, w), R.int8_linear(q, s, w.q, w.scale, BF16))
     check_dense()
+
+
+def _ffn_int8_defined(x, wg, wu, wd, name):
+    """(value, bound) of the block on fp32 tokens with the codes of the intermediate in 64 bits and no allowance at their borders.
+    The row's scale, the sum's conversion and two products round once each, 2^-24 of the value."""
+    q, s = R.codes(x.double())
+    g, u = ((q @ w.q.double().T) * s[:, None] * w.scale.double() for w in (wg, wu))
+    hq, hs = R.codes(R.act(g, name)[0] * u)
+    y = (hq @ wd.q.double().T) * hs[:, None] * wd.scale.double()
+    return y, 4.1 * 2.0 ** -24 * y.abs()
+
+
+@pytest.mark.parametrize("name", R.ACTS)
+@pytest.mark.parametrize("T,d,I", [(1, 2048, 5632), (1, 8, 3), (7, 264, 1021), (12, 768, 2048), (16, 1000, 520), (24, 2048, 1408), (40, 512, 2050),
+                                   (128, 320, 264), (300, 777, 1000), (2800, 2000, 843), (1500, 256, 2056), (5000, 64, 520)])
+def test_int8_block_codes_of_f32_tokens(cuda, T, d, I, name):
+    """fp32 tokens: every code of the intermediate is that of the 64-bit definition (a single one on the other side of its
+    border moves that token's y by hundreds of the bounds)."""
+    from dsca_moe_b200 import check_dense, gated_ffn_int8, pack_int8
+
+    randn = _randn(cuda, T + d + I)
+    x = randn(T, d) * torch.exp(0.3 * randn(T, 1))
+    wg, wu, wd = (pack_int8(randn(*s) * s[1] ** -0.5) for s in ((I, d), (I, d), (d, I)))
+    R.close(gated_ffn_int8(x, wg, wu, wd, act=name), _ffn_int8_defined(x, wg, wu, wd, name))
+    check_dense()
+
+
+@pytest.mark.parametrize("T", [2, 30, 300])
+def test_int8_block_of_f32_tokens_range(cuda, T):
+    """Gates far from zero, rows of every size, a row of zeros, rows that are not finite beside rows that are; the same call
+    again gives the same bits."""
+    from dsca_moe_b200 import gated_ffn_int8, pack_int8
+
+    randn = _randn(cuda, T)
+    wg, wu, wd = (pack_int8(randn(*s)) for s in ((200, 136), (200, 136), (136, 200)))
+    x = randn(T, 136) * 10 ** torch.linspace(-9, 6, T, device=cuda)[:, None]
+    x[T // 2] = 0
+    for name in R.ACTS:
+        y = gated_ffn_int8(x, wg, wu, wd, act=name)
+        R.close(y, _ffn_int8_defined(x, wg, wu, wd, name), name)
+        assert not y[T // 2].any() and torch.equal(y, gated_ffn_int8(x, wg, wu, wd, act=name))
+        for bad in (float("nan"), float("inf")):
+            xb = x.clone()
+            xb[T // 2, 3] = bad
+            got, keep = gated_ffn_int8(xb, wg, wu, wd, act=name), torch.arange(T, device=cuda) != T // 2
+            assert not torch.isfinite(got[T // 2]).any() and torch.equal(got[keep], y[keep])
+
+
+def test_int8_block_of_f32_tokens_captured(cuda):
+    """Captured, with new tokens in the buffers at each replay; and a batch in front, rows of a wider buffer."""
+    from dsca_moe_b200 import gated_ffn_int8, pack_int8
+
+    randn = _randn(cuda, 0)
+    w = [pack_int8(randn(*s) * s[1] ** -0.5) for s in ((264, 128), (264, 128), (128, 264))]
+    x = randn(2, 20, 133)[..., :128]
+    gated_ffn_int8(x, *w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = gated_ffn_int8(x, *w)
+    for _ in range(3):
+        x.copy_(randn(2, 20, 128))
+        graph.replay()
+        R.close(y.view(40, 128), _ffn_int8_defined(x.reshape(40, 128), *w, "silu"))
