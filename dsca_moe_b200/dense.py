@@ -130,11 +130,25 @@ def _saved(rows: int, inter: int, dtype):
     return ld_h, step, 3 * step + (8 * rows * ((inter + 31) // 32) if dtype is _BF16 else 0)
 
 
+def _as_saved(t, name: str, shape, like):
+    """(t, its row stride) of a tensor that the backward pass reads.  Saved-tensor hooks (offloading, for one) may return it
+    in other strides than it was saved with, and a gradient comes in any (expanded, transposed)."""
+    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"{name} came back as {t.dtype} {tuple(t.shape)} on {t.device}, not {like.dtype} {tuple(shape)} on "
+                           f"{like.device}")
+    if t.is_contiguous():
+        return t, shape[-1]
+    try:
+        return t, _stride(t, name, shape[-1])
+    except ValueError:
+        return t.contiguous(), shape[-1]
+
+
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, wd, act, shapes):
         y, buf = _forward(x, wg, wu, wd, act, shapes, True)
-        ctx.act, ctx.shapes = act, shapes
+        ctx.act, ctx.sizes, ctx.x_shape, ctx.saved_bytes = act, shapes[:3], x.shape, 0 if buf is None else buf.numel()
         ctx.save_for_backward(x, wg, wu, wd, buf)
         return y
 
@@ -142,21 +156,22 @@ class _GatedFFN(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, wg, wu, wd, buf = ctx.saved_tensors
-        rows, d, inter, ld_x, ld_g, ld_u, ld_d = ctx.shapes
-        dev, dtype = x.device, x.dtype
+        rows, d, inter = ctx.sizes
+        dev, dtype = dy.device, dy.dtype
         need = ctx.needs_input_grad
-        dx = torch.empty(x.shape, dtype=dtype, device=dev) if need[0] else None
+        dx = torch.empty(ctx.x_shape, dtype=dtype, device=dev) if need[0] else None
         dwg = torch.empty((inter, d), dtype=dtype, device=dev) if need[1] else None
         dwu = torch.empty((inter, d), dtype=dtype, device=dev) if need[2] else None
         dwd = torch.empty((d, inter), dtype=dtype, device=dev) if need[3] else None
         dx_p, dwg_p, dwu_p, dwd_p = [None if t is None else t.data_ptr() for t in (dx, dwg, dwu, dwd)]
         if rows:
-            ld_dy = d
-            if not dy.is_contiguous():
-                try:
-                    ld_dy = _stride(dy, "dy", d)
-                except ValueError:  # a gradient may come in any strides (expanded, transposed)
-                    dy = dy.contiguous()
+            dy, ld_dy = _as_saved(dy, "dy", ctx.x_shape, dy)
+            x, ld_x = _as_saved(x, "x", ctx.x_shape, dy)
+            (wg, ld_g), (wu, ld_u), (wd, ld_d) = (_as_saved(w, n, torch.Size(s), dy) for w, n, s in (
+                (wg, "w_gate", (inter, d)), (wu, "w_up", (inter, d)), (wd, "w_down", (d, inter))))
+            if buf.dtype != torch.uint8 or buf.device != dev or buf.numel() != ctx.saved_bytes or not buf.is_contiguous() \
+                    or buf.data_ptr() % 16:
+                raise RuntimeError("the saved intermediates came back otherwise than they were saved")
             ld_h, step, _ = _saved(rows, inter, dtype)
             grads = torch.empty(2 * step, dtype=torch.uint8, device=dev)
             h, dg = buf.data_ptr(), grads.data_ptr()

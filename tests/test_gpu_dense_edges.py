@@ -91,3 +91,33 @@ def test_int8_block_of_f32_tokens_captured(cuda):
         x.copy_(randn(2, 20, 128))
         graph.replay()
         R.close(y.view(40, 128), _ffn_int8_defined(x.reshape(40, 128), *w, "silu"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,d,I,gap", [(3, 40, 24, 8), (40, 96, 136, 16), (150, 136, 264, 8), (300, 130, 66, 3)])
+def test_saved_tensor_hooks(cuda, T, d, I, gap, dtype):
+    """Hooks that return what was saved in other strides (offloading to the host lays it out densely): rows of wider buffers
+    keep their gradients."""
+    from dsca_moe_b200 import gated_ffn
+
+    randn = _randn(cuda, T)
+    x, wg, wu, wd = ((randn(r, c + gap) * c ** -0.5).to(dtype)[:, :c] for r, c in ((T, d), (I, d), (I, d), (d, I)))
+    dy = randn(T, d).to(dtype)
+    ref = R.ffn(x, wg, wu, wd, "silu", dtype, dy)
+
+    def transposed(t):
+        return t.t().contiguous().t() if t.dim() == 2 else t
+
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t),
+                  torch.autograd.graph.saved_tensors_hooks(lambda t: t, transposed)):
+        p = [t.detach().requires_grad_() for t in (x, wg, wu, wd)]
+        with hooks:
+            y = gated_ffn(*p)
+        for got, k in zip(torch.autograd.grad(y, p, dy), ("dx", "d_gate", "d_up", "d_down")):
+            R.close(got, ref[k], k)
+    for change in (lambda t: t[..., :-1], lambda t: t.double() if t.is_floating_point() else t):
+        p = [t.detach().requires_grad_() for t in (x, wg, wu, wd)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            y = gated_ffn(*p)
+        with pytest.raises(RuntimeError, match="came back"):
+            y.backward(dy)
