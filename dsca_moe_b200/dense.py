@@ -403,22 +403,49 @@ def _act_name(mod) -> str:
     raise ValueError(f"gate activation {name} is not offered (silu, tanh gelu, relu)")
 
 
+def _bare(m: nn.Module) -> bool:
+    """Whether nothing hangs on a module: no hook and no forward of its own."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or "forward" in m.__dict__)
+
+
+def _plain(m: nn.Module) -> bool:
+    """Whether a layer is its weight's product and nothing else: a Linear (adapters and parametrisations have types of their
+    own) without bias and hooks, on an ordinary tensor."""
+    return type(m) is nn.Linear and m.bias is None and type(m.weight) in (nn.Parameter, torch.Tensor) and _bare(m)
+
+
 class GatedFFN(nn.Module):
     """A dense gated MLP (Qwen2MoeMLP's gate_proj / up_proj / down_proj, or wi_0 / wi_1 / wo) on gated_ffn.
 
     Keeps the old module's Linear layers under their names, so that its parameters, their gradients and
-    state_dict stay what they were.  int8=True packs the weights in 8-bit integers instead (buffers;
-    inference only) and lets the Linear layers go."""
+    state_dict stay what they were.  The layers run one by one, as in the old module, where the block is not the whole
+    of it: with a dropout in training mode, with an adapter or a hook that was put on a layer since, with weights of another type than x
+    (a `wo` kept in fp32), under fp16 autocast.  bf16 autocast runs the block in bf16.  Modules that already have hooks, adapters or other
+    parts are refused.  int8=True packs the weights in 8-bit integers instead (buffers; inference only) and
+    lets the Linear layers go."""
 
     def __init__(self, old: nn.Module, int8: bool = False):
         super().__init__()
+        kind = type(old).__name__
         names = next((n for n in _NAMES if all(hasattr(old, m) for m in n)), None)
         if names is None:
-            raise ValueError(f"{type(old).__name__} has neither gate_proj / up_proj / down_proj nor wi_0 / wi_1 / wo")
+            raise ValueError(f"{kind} has neither gate_proj / up_proj / down_proj nor wi_0 / wi_1 / wo")
         linears = [getattr(old, n) for n in names]
         if any(getattr(m, "bias", None) is not None for m in linears):
             raise ValueError("gated blocks with biases are not offered")
-        self.names, self.act, self.int8 = names, _act_name(old), bool(int8)
+        act = _act_name(old)
+        if not _bare(old) or not all(_plain(m) for m in linears):
+            raise ValueError(f"{kind} has hooks, adapters or layers other than nn.Linear, which the block would leave out "
+                             "(replace it first, then put them on)")
+        dropout = getattr(old, "dropout", None)
+        rest = sorted(set(dict(old.named_children())) - {*names, "act_fn", "act", "dropout"})
+        if rest or not (dropout is None or type(dropout) is nn.Dropout):
+            raise ValueError(f"{kind} has {', '.join(rest) or 'a dropout of its own'}, which the block would leave out")
+        self.names, self.act, self.int8 = names, act, bool(int8)
+        self.act_fn = old.act_fn if getattr(old, "act_fn", None) is not None else old.act
+        self.dropout = dropout
+        self.training = old.training
         if not int8:
             for n, m in zip(names, linears):
                 setattr(self, n, m)
@@ -429,8 +456,35 @@ class GatedFFN(nn.Module):
             self.register_buffer(n + "_q", q)  # whole padded rows, so that a copy keeps their layout
             self.register_buffer(n + "_scale", scale)
 
+    def _layers(self, x: torch.Tensor) -> torch.Tensor:
+        """The old module's forward."""
+        gate, up, down = (getattr(self, n) for n in self.names)
+        h = self.act_fn(gate(x)) * up(x)
+        if self.dropout is not None:
+            h = self.dropout(h)
+        w = getattr(down, "weight", None)
+        if self.names[2] == "wo" and isinstance(w, torch.Tensor) and w.is_floating_point() and h.dtype != w.dtype:
+            h = h.to(w.dtype)
+        return down(h)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        drop = self.dropout is not None and (type(self.dropout) is not nn.Dropout or not _bare(self.dropout)
+                                             or (self.dropout.training and self.dropout.p > 0))
+        amp = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
+        if amp is not None and not (amp in _DTYPES and x.is_floating_point() and x.dtype != torch.float64):
+            amp = None if self.int8 else False
         if self.int8:
-            return gated_ffn_int8(x, *(Int8Weight(getattr(self, n + "_q")[:, :k], getattr(self, n + "_scale"))
-                                       for n, k in zip(self.names, self.widths)), act=self.act)
-        return gated_ffn(x, *(getattr(self, n).weight for n in self.names), act=self.act)
+            if drop:
+                raise RuntimeError("a dropout is not offered on 8-bit weights (call eval())")
+            return gated_ffn_int8(x if amp is None else x.to(amp),
+                                  *(Int8Weight(getattr(self, n + "_q")[:, :k], getattr(self, n + "_scale"))
+                                    for n, k in zip(self.names, self.widths)), act=self.act)
+        linears = [getattr(self, n) for n in self.names]
+        if drop or amp is False or not all(_plain(m) for m in linears):
+            return self._layers(x)
+        weights = [m.weight for m in linears]
+        if amp is not None:  # what autocast does at each layer
+            x, weights = x.to(amp), [w.to(amp) for w in weights]
+        if any(w.dtype is not x.dtype for w in weights):
+            return self._layers(x)
+        return gated_ffn(x, *weights, act=self.act)

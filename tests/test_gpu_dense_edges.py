@@ -121,3 +121,59 @@ def test_saved_tensor_hooks(cuda, T, d, I, gap, dtype):
             y = gated_ffn(*p)
         with pytest.raises(RuntimeError, match="came back"):
             y.backward(dy)
+
+
+def _mlp(dev, dtype, d=64, inter=200):
+    class M(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate_proj, self.up_proj = torch.nn.Linear(d, inter, bias=False), torch.nn.Linear(d, inter, bias=False)
+            self.down_proj, self.act_fn = torch.nn.Linear(inter, d, bias=False), torch.nn.SiLU()
+
+    torch.manual_seed(3)
+    return M().to(dev, dtype)
+
+
+def test_module_under_autocast(cuda):
+    """fp32 parameters under bf16 autocast: the block on bf16 values, gradients in the parameters' type; fp16 autocast runs the
+    layers."""
+    from dsca_moe_b200 import GatedFFN, pack_int8
+
+    m = GatedFFN(_mlp(cuda, F32))
+    randn = _randn(cuda, 5)
+    w = [m.gate_proj.weight, m.up_proj.weight, m.down_proj.weight]
+    for dtype in (BF16, F32):
+        x, dy = randn(70, 64).to(dtype).requires_grad_(), randn(70, 64).to(BF16)
+        ref = R.ffn(x.detach().to(BF16), *(t.detach().to(BF16) for t in w), "silu", BF16, dy)
+        with torch.autocast("cuda", torch.bfloat16):
+            y = m(x)
+        assert y.dtype == BF16
+        R.close(y.detach(), ref["y"])
+        for got, p, k in zip(torch.autograd.grad(y, [x] + w, dy), [x] + w, ("dx", "d_gate", "d_up", "d_down")):
+            assert got.dtype == p.dtype
+            R.close(got, ref[k], k)
+    with torch.autocast("cuda", torch.float16):
+        assert m(x).dtype == torch.float16
+    q = GatedFFN(_mlp(cuda, F32), int8=True)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = q(x.detach())
+    R.close(y, R.ffn_int8(x.detach().to(BF16), *(pack_int8(t) for t in w), "silu", BF16))
+
+
+def test_t5_block_in_eval_mode(cuda):
+    """T5's gated MLP with its dropout off runs as the block; on 8-bit weights a dropout that is on is refused."""
+    from transformers import T5Config
+    from transformers.models.t5.modeling_t5 import T5DenseGatedActDense
+
+    from dsca_moe_b200 import GatedFFN
+
+    torch.manual_seed(2)
+    old = T5DenseGatedActDense(T5Config(d_model=64, d_ff=200, feed_forward_proj="gated-gelu")).to(cuda, BF16)
+    x = _randn(cuda, 8)(40, 64).to(BF16)
+    m = GatedFFN(old.eval())
+    ref = R.ffn(x, old.wi_0.weight.detach(), old.wi_1.weight.detach(), old.wo.weight.detach(), "gelu", BF16)
+    R.close(m(x).detach(), ref["y"])
+    q = GatedFFN(old, int8=True)
+    q(x)
+    with pytest.raises(RuntimeError, match="dropout"):
+        q.train()(x)
