@@ -20,8 +20,11 @@ import torch.nn as nn
 
 from . import _lib as L
 from .engine import MoEEngine, default_expert_to_gpu, pack_relu, pack_swiglu
+from .gradients import refuse_tangents, without_gradient
 from .qos import QoSInputs
 from .reporting import TRACE
+
+_BLOCK = "an MoE block"
 
 
 def hf_callers_unpack_tuples() -> bool:
@@ -182,10 +185,19 @@ class QoSMoELayer(nn.Module):
         self.num_prefetch_launched.append(len(launched))
         return launched
 
-    @torch.no_grad()
     def forward(self, hidden_states):
+        """The block has no backward pass: one that reaches it raises (gradients.py)."""
         if self.runtime_context is None:
             raise RuntimeError("QoSMoELayer requires runtime_context before forward")
+        refuse_tangents(_BLOCK, hidden_states)
+        r = self._forward(hidden_states)
+        if not isinstance(r, tuple):
+            return without_gradient(_BLOCK, r, hidden_states)
+        out, (logits, index) = r
+        return without_gradient(_BLOCK, out, hidden_states), (without_gradient(_BLOCK, logits, hidden_states), index)
+
+    @torch.no_grad()
+    def _forward(self, hidden_states):
         stats = bool(getattr(self.config, "collect_stats", False))
         if stats:
             ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -263,8 +275,16 @@ class ShardedQwenMoE(nn.Module):
         self.engine.few_tokens = int(few_tokens)
         self.route_calls = 0
 
-    @torch.no_grad()
     def forward(self, hidden_states):
+        """The block has no backward pass: one that reaches it raises (gradients.py)."""
+        refuse_tangents(_BLOCK, hidden_states)
+        r = self._forward(hidden_states)
+        if not isinstance(r, tuple):
+            return without_gradient(_BLOCK, r, hidden_states)
+        return tuple(without_gradient(_BLOCK, t, hidden_states) for t in r)
+
+    @torch.no_grad()
+    def _forward(self, hidden_states):
         b, s, d = hidden_states.shape
         r = self.engine.forward(hidden_states.reshape(-1, d))
         self.route_calls += 1
@@ -278,7 +298,8 @@ def patch(model, rank, world, policy="fifo", few_tokens=0, dense_ffn=None):
     The swapped blocks return what the installed transformers' Qwen2MoeDecoderLayer expects.
     `dense_ffn`: None leaves the dense layers between them (Qwen2MoeMLP of mlp_only_layers and
     decoder_sparse_step) as they are, "same" swaps them for GatedFFN on their parameters, "int8" for
-    GatedFFN on 8-bit integer weights."""
+    GatedFFN on 8-bit integer weights.  The MoE blocks have no backward pass, so of a patched model what lies behind the
+    last of them can be trained, with the rest frozen; a backward pass that reaches a block raises."""
     if dense_ffn not in (None, "same", "int8"):
         raise ValueError(f"dense_ffn must be None, 'same' or 'int8', not {dense_ffn!r}")
     changed = 0

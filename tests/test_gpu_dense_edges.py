@@ -177,3 +177,26 @@ def test_t5_block_in_eval_mode(cuda):
     q(x)
     with pytest.raises(RuntimeError, match="dropout"):
         q.train()(x)
+
+
+def test_patched_model_refuses_gradients_through_moe_blocks(cuda):
+    """A model whose MoE blocks are swapped: logits with autograd on are those without it, a loss that would reach a layer
+    through a block raises, and what lies behind the last block trains."""
+    from test_gpu_dense import _tiny_qwen
+
+    from dsca_moe_b200 import patch
+
+    m = _tiny_qwen()
+    patch(m, 0, 1, dense_ffn="same")
+    ids = torch.randint(0, 97, (2, 11), device=cuda)
+    with torch.no_grad():
+        want = m(ids).logits
+    y = m(ids).logits
+    assert torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="MoE block"):
+        y.float().square().mean().backward()
+    m.requires_grad_(False)
+    m.lm_head.weight.requires_grad_()
+    y = m(ids).logits
+    (grad,) = torch.autograd.grad(y.float().square().mean(), m.lm_head.weight)
+    assert grad.abs().sum() > 0
