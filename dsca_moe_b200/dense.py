@@ -19,6 +19,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
+from .gradients import refuse_tangents, without_gradient
 from .norm import _DTYPES, _stride
 
 __all__ = ["GatedFFN", "Int8Weight", "check_dense", "gated_ffn", "gated_ffn_int8", "int8_linear", "pack_int8",
@@ -196,8 +197,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     [d, inter] of x's type, as Linear layers hold them.  act: "silu", "gelu" (tanh form) or "relu".
     Products are summed in fp32; the gated intermediate is rounded to x's type, and so are its two
     gradients in the backward pass.  Under autograd the call keeps the intermediate, the gate and the up
-    values, each [rows, inter] (the latter two to 11 bits for bf16), for the backward pass; second derivatives are not offered.  Runs on x's
-    device, on its current stream; check_dense() reports a wait that ran out."""
+    values, each [rows, inter] (the latter two to 11 bits for bf16), for the backward pass; second derivatives and forward-mode
+    ones are not offered.  Runs on x's device, on its current stream; check_dense() reports a wait that ran out."""
     code = _act(act)
     if x.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {x.dtype}")
@@ -210,6 +211,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         raise ValueError(f"w_gate: {inter} rows exceed {L.DENSE_MAX_DIM}")
     shapes = (rows, d, inter, ld_x, _weight(w_gate, "w_gate", inter, d, x), _weight(w_up, "w_up", inter, d, x),
               _weight(w_down, "w_down", d, inter, x))
+    refuse_tangents("gated_ffn", x, w_gate, w_up, w_down)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
                                     or w_down.requires_grad):
         return _GatedFFN.apply(x, w_gate, w_up, w_down, code, shapes)
@@ -229,6 +231,7 @@ class Int8Weight(NamedTuple):
 
 def _quantize(x):
     """(codes [rows, k rounded up to 16], scales) of x's rows."""
+    refuse_tangents("quantize_rows", x)
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise ValueError(f"unsupported dtype {x.dtype}")
@@ -240,14 +243,14 @@ def _quantize(x):
     if rows:
         a = L.QuantizeRowsArgs(x.data_ptr(), rows, k, dt, ld_x, q.data_ptr(), ld_q, scale.data_ptr())
         L.call_on(x.device, "dsca_quantize_rows", ctypes.byref(a))
-    return q, scale
+    return q, without_gradient("quantize_rows", scale, x)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q [..., k] int8, scale [...] fp32) of x [..., k] bf16 or fp32: scale = max|x| / 127 a row (1 for a
     row of zeros), q the quotient 127 x / max|x| rounded to the nearest integer, ties to even,
     exactly.  q's rows lie a multiple of 16 bytes apart, the bytes between them zero.  A row with an
-    infinity or a NaN has that as its scale.  Inference only."""
+    infinity or a NaN has that as its scale.  Inference only: a backward pass that reaches the scale raises."""
     q, scale = _quantize(x)
     k = x.shape[-1]
     return q[:, :k] if x.dim() == 2 else q[:, :k].unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0, :k], scale
@@ -293,7 +296,9 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
 
     x [..., k] bf16 or fp32; or int8 codes of quantize_rows with their x_scale [...], out_dtype then
     chooses y's type (bf16 by default, otherwise x's type).  Codes lie in [-127, 127].  The products' sum
-    is exact; it is scaled in fp32 and rounded once.  bias [n] of y's type.  Inference only."""
+    is exact; it is scaled in fp32 and rounded once.  bias [n] of y's type.  Inference only: a backward pass
+    that reaches y raises."""
+    refuse_tangents("int8_linear", x, bias, x_scale)
     given = x.dtype == torch.int8
     if given:
         if x_scale is None:
@@ -341,7 +346,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     if not _few(rows, n * ld_w):
         ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_int8_linear", ctypes.byref(a))
-    return y
+    return without_gradient("int8_linear", y, x, bias, x_scale, weight[1])
 
 
 def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down: Int8Weight,
@@ -350,7 +355,9 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     intermediate is formed and its rows quantised in turn.  x [..., d] bf16 or fp32; y has its shape and
     type.  fp32 tokens: the intermediate is formed in 64 bits, so that its codes are those of the
     definition.  bf16 tokens: it is formed in fp32, with gates good to 2^-18 of their value, and a code next
-    to a border may lie on its other side, which moves y by about one of its roundings.  Inference only."""
+    to a border may lie on its other side, which moves y by about one of its roundings.  Inference only: a
+    backward pass that reaches y raises."""
+    refuse_tangents("gated_ffn_int8", x)
     code = _act(act)
     dt = _DTYPES.get(x.dtype)
     if dt is None:
@@ -381,7 +388,7 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     if dt == L.F32 or not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
         ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
-    return y
+    return without_gradient("gated_ffn_int8", y, x, w_gate[1], w_up[1], w_down[1])
 
 
 # ----------------------------------------------------------------------------- module

@@ -200,3 +200,37 @@ def test_patched_model_refuses_gradients_through_moe_blocks(cuda):
     y = m(ids).logits
     (grad,) = torch.autograd.grad(y.float().square().mean(), m.lm_head.weight)
     assert grad.abs().sum() > 0
+
+
+def test_calls_without_gradients(cuda):
+    """8-bit calls on what wants a gradient: the values of a call without autograd, and an error from the backward pass that
+    reaches them; forward-mode tangents are refused by every call."""
+    import torch.autograd.forward_ad as fwad
+
+    from dsca_moe_b200 import GatedFFN, gated_ffn, gated_ffn_int8, int8_linear, pack_int8, quantize_rows
+
+    m = GatedFFN(_mlp(cuda, BF16), int8=True)
+    randn = _randn(cuda, 6)
+    lin = torch.nn.Linear(64, 64, bias=False).to(cuda, BF16)
+    x, w = randn(5, 64).to(BF16), [pack_int8(randn(*s).to(BF16)) for s in ((200, 64), (200, 64), (64, 200))]
+    bias = randn(200).to(BF16).requires_grad_()
+    q, s = quantize_rows(x)
+    for name, call in (("gated_ffn_int8", lambda t: t + m(t)), ("gated_ffn_int8", lambda t: gated_ffn_int8(t, *w)),
+                       ("int8_linear", lambda t: int8_linear(t, w[0])), ("quantize_rows", lambda t: quantize_rows(t)[1]),
+                       ("int8_linear", lambda t: int8_linear(q, w[0], bias=bias, x_scale=s)),
+                       ("int8_linear", lambda t: int8_linear(q, w[0], x_scale=quantize_rows(t)[1]))):
+        y = call(lin(x))
+        with torch.no_grad():
+            assert torch.equal(call(lin(x)), y)
+        with pytest.raises(RuntimeError, match=name + " has no backward"):
+            y.float().sum().backward()
+        call(lin(x).detach())
+    assert not pack_int8(lin.weight).scale.requires_grad
+    wg, wd = randn(200, 64).to(BF16), randn(64, 200).to(BF16)
+    with fwad.dual_level():
+        t = fwad.make_dual(x, x)
+        for call in (lambda: gated_ffn(t, wg, wg, wd), lambda: gated_ffn(x, wg, fwad.make_dual(wg, wg), wd), lambda: quantize_rows(t),
+                     lambda: int8_linear(t, w[0]), lambda: gated_ffn_int8(t, *w)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        gated_ffn(x, wg, wg, wd)
