@@ -463,6 +463,15 @@ class GatedFFN(nn.Module):
             self.register_buffer(n + "_q", q)  # whole padded rows, so that a copy keeps their layout
             self.register_buffer(n + "_scale", scale)
 
+    def _apply(self, fn, recurse=True):
+        """The scales of 8-bit weights stay fp32 when the model changes its type."""
+        scales = {n: b for n, b in self._buffers.items() if n.endswith("_scale")}
+        super()._apply(fn, recurse)
+        for n, b in scales.items():
+            if self._buffers[n].dtype != b.dtype:
+                self._buffers[n] = b.to(self._buffers[n].device)
+        return self
+
     def _layers(self, x: torch.Tensor) -> torch.Tensor:
         """The old module's forward."""
         gate, up, down = (getattr(self, n) for n in self.names)

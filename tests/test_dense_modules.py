@@ -139,3 +139,24 @@ def test_plain_layers_take_the_block():
               GatedFFN(_t5().eval())):
         with pytest.raises(ValueError, match="GPU"):
             m(torch.randn(2, 8))
+
+
+def test_int8_scales_stay_fp32(monkeypatch):
+    """A model that changes its type leaves the 8-bit weights what they were."""
+    import dsca_moe_b200.dense as D
+
+    def quantize(w):  # (the kernel's, on the host)
+        s = w.abs().amax(1) / 127
+        return torch.round(w / s[:, None]).to(torch.int8), s
+
+    monkeypatch.setattr(D, "_quantize", quantize)
+    model = nn.Sequential(nn.Linear(8, 8), D.GatedFFN(Gated(), int8=True))
+    was = {k: v.clone() for k, v in model[1].state_dict().items()}
+    assert len(was) == 6
+    for change in (lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.bfloat16)):
+        change(model)
+        now = model[1].state_dict()
+        assert now.keys() == was.keys() and all(now[k].dtype == was[k].dtype and torch.equal(now[k], was[k]) for k in was)
+    assert model[0].weight.dtype == torch.bfloat16
+    model.to("meta")
+    assert all(b.device.type == "meta" and b.dtype == was[n].dtype for n, b in model[1].named_buffers())
