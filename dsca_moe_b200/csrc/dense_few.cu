@@ -40,6 +40,7 @@ struct Params {
   const void* x;
   int64_t ldx;
   int T, M, K, tiles, act;
+  int tail;  // codes behind the last whole 16 (K does not count them)
   int per;  // steps of one CTA of the cluster
   void* out;
   int64_t ldo;
@@ -108,6 +109,20 @@ __device__ __forceinline__ uint4 load16(const T* row, int k, int K, bool live) {
       }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+
+// The products of the first n < 16 of 16 codes; what lies behind them is read and does not count.
+__device__ __forceinline__ int tail_sum(const int8_t* x, const int8_t* w, int n) {
+  const uint4 a = *reinterpret_cast<const uint4*>(x), b = *reinterpret_cast<const uint4*>(w);
+  const uint32_t xs[4] = {a.x, a.y, a.z, a.w}, ws[4] = {b.x, b.y, b.z, b.w};
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int keep = n - 4 * i;
+    const uint32_t v = keep >= 4 ? xs[i] : keep > 0 ? xs[i] & ((1u << (8 * keep)) - 1u) : 0u;
+    sum = __dp4a((int)v, (int)ws[i], sum);
+  }
+  return sum;
 }
 
 // Four fp32 values in a row as three bf16 terms, which hold them exactly: the upper 8 bits of significand cut off (never
@@ -272,6 +287,13 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 0 : NT == 2 ? 4 : 2) fe
       if constexpr (kGluE) vb += part[c + 8][n];
     }
     const bool in = m < p.M;
+    if constexpr (std::is_same<T, int8_t>::value) {
+      if (p.tail != 0 && in) {
+        const int8_t* xt = reinterpret_cast<const int8_t*>(p.x) + (int64_t)n * p.ldx + p.K;
+        va += tail_sum(xt, reinterpret_cast<const int8_t*>(p.w[0]) + (int64_t)m * p.ldw[0] + p.K, p.tail);
+        if constexpr (kGluE) vb += tail_sum(xt, reinterpret_cast<const int8_t*>(p.w[1]) + (int64_t)m * p.ldw[1] + p.K, p.tail);
+      }
+    }
     if constexpr (std::is_same<O, double>::value) {
       if (in) {
         const double xs = (double)p.row_scale[n] / 127.0;
@@ -318,7 +340,7 @@ template <typename T, typename O, int EPI, int NT, bool kVecW, bool kVecX>
 int launch(Params& p, bool pdl, cudaStream_t stream) {
   constexpr int STEP = 4 * Traits<T>::kVals;
   p.tiles = (p.M + (EPI == kGlu ? 8 : 16) - 1) / (EPI == kGlu ? 8 : 16);
-  const int steps = (p.K + STEP - 1) / STEP, sms = current_device_sms();
+  const int steps = std::max(1, (p.K + STEP - 1) / STEP), sms = current_device_sms();
   // CTAs to a tile: up to some three CTAs an SM, and a whole batch of steps for each warp
   int splits = 1;
   while (splits < 8 && p.tiles * splits * 2 <= 4 * sms && steps >= splits * 2 * kU * kWarps) splits *= 2;
@@ -387,7 +409,8 @@ int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   p.x = s.b[0].p; p.ldx = s.b[0].ld;
   const bool vw = whole(s.a[0]) && (j.epi != kGlu || whole(s.a[1])), vx = whole(s.b[0]);
   p.T = s.N; p.M = s.M;
-  p.K = j.i8 ? (s.K + 15) / 16 * 16 : s.K;  // the weights' padding is zeros
+  p.tail = j.i8 ? s.K % 16 : 0;
+  p.K = s.K - p.tail;
   p.act = j.act;
   p.out = s.out; p.ldo = s.ldo;
   p.save_g = j.save_g; p.save_u = j.save_u; p.save_e = j.save_e; p.groups = exp_groups(s.M);

@@ -111,7 +111,7 @@ typedef struct {
   const void* x;        /* [rows, k], dtype, or NULL: q and scale are given */
   int8_t* q;            /* [rows, ld_q] */
   float* scale;         /* [rows] */
-  const int8_t* w;      /* [n, ld_w], 16-byte aligned, columns [k, ld_w) zero */
+  const int8_t* w;      /* [n, ld_w], 16-byte aligned; columns [k, ld_w) of w and q do not count, up to whole 16 bytes they are read */
   const float* w_scale; /* [n] */
   const void* bias;     /* [n], dtype, or NULL */
   void* y;              /* [rows, n], dtype */
@@ -131,7 +131,7 @@ typedef struct {
   const void* x;        /* [rows, d], dtype */
   int8_t* q;            /* work area [rows, ld_q] */
   float* scale;         /* work area [rows] */
-  const int8_t* w_gate; /* [inter, ld_gate], 16-byte aligned, columns past d zero */
+  const int8_t* w_gate; /* [inter, ld_gate], 16-byte aligned; columns past d do not count */
   const int8_t* w_up;
   const int8_t* w_down; /* [d, ld_down] */
   const float* gate_scale; /* [inter] */

@@ -234,3 +234,26 @@ def test_calls_without_gradients(cuda):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
         gated_ffn(x, wg, wg, wd)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 8, 12, 16, 17, 40, 200])
+@pytest.mark.parametrize("k", [1, 15, 50, 63, 64, 113, 1000])
+def test_codes_and_weights_of_wider_ones(cuda, rows, k):
+    """Codes and weights that are both views of wider ones: what lies behind the k-th column counts for no number of rows."""
+    from dsca_moe_b200 import Int8Weight, gated_ffn_int8, int8_linear, pack_int8, quantize_rows
+
+    randn = _randn(cuda, rows + k)
+    q, s = quantize_rows(randn(rows, 1040).to(BF16))
+    w = pack_int8(randn(96, 1040).to(BF16))
+    part = Int8Weight(w.q[:, :k], w.scale)
+    for n in (0, rows - 1):  # one row alone as well
+        R.close(int8_linear(q[n:n + 1, :k], part, x_scale=s[n:n + 1]), R.int8_linear(q[n:n + 1, :k], s[n:n + 1], part.q, w.scale, BF16))
+    R.close(int8_linear(q[:, :k], part, x_scale=s), R.int8_linear(q[:, :k], s, part.q, w.scale, BF16))
+    R.close(int8_linear(q[0, :k], part, x_scale=s[0])[None], R.int8_linear(q[:1, :k], s[:1], part.q, w.scale, BF16))
+    x = randn(rows, k)
+    down = pack_int8(randn(k, 96))
+    R.close(gated_ffn_int8(x, part, part, down), _ffn_int8_defined(x, part, part, down, "silu"))
+    wide = pack_int8(randn(96, k + 200))
+    x = randn(rows, 96)
+    up, down = pack_int8(randn(k, 96)), Int8Weight(wide.q[:, :k], wide.scale)
+    R.close(gated_ffn_int8(x, up, up, down), _ffn_int8_defined(x, up, up, down, "silu"))
