@@ -304,8 +304,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 0 : NT == 2 ? 4 : 2) fe
     float v = (float)va, u = (float)vb;
     if constexpr (std::is_same<T, int8_t>::value) {
       const float rs = p.row_scale[n];
-      v *= in ? p.col_scale[0][m] * rs : 0.0f;
-      if constexpr (kGluE) u *= in ? p.col_scale[1][m] * rs : 0.0f;
+      // (the scales' own product may leave fp32's normal numbers where the result does not)
+      v = in ? v * p.col_scale[0][m] * rs : 0.0f;
+      if constexpr (kGluE) u = in ? u * p.col_scale[1][m] * rs : 0.0f;
     }
     if constexpr (kGluE) {
       if (p.save_g != nullptr) {

@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               float cs[32];
               load_row(P.col_scale[0], n, q.cols, P.vec_cols, cs);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * (cs[j] * rs);
+              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * cs[j] * rs;
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
                 float cs[32];
                 load_row(P.col_scale[1], n, q.cols, P.vec_cols, cs);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) u[j] = (float)(int)r[j] * (cs[j] * rs);
+                for (int j = 0; j < 32; ++j) u[j] = (float)(int)r[j] * cs[j] * rs;
               } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(r[j]);
@@ -926,7 +926,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             if constexpr (IN == kI8) {
               const float rs = c + lane < t.nval ? __ldg(P.row_scale + t.n0 + c + lane) : 0.0f;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * (cs * __shfl_sync(0xffffffffu, rs, j));
+              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * cs * __shfl_sync(0xffffffffu, rs, j);
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);

@@ -296,7 +296,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
 
     x [..., k] bf16 or fp32; or int8 codes of quantize_rows with their x_scale [...], out_dtype then
     chooses y's type (bf16 by default, otherwise x's type).  Codes lie in [-127, 127].  The products' sum
-    is exact; it is scaled in fp32 and rounded once.  bias [n] of y's type.  Inference only: a backward pass
+    is exact; its conversion to fp32, the products with the channel's and the token's scale and the addition of
+    the bias round to fp32, the result to y's type.  bias [n] of y's type.  Inference only: a backward pass
     that reaches y raises."""
     refuse_tangents("int8_linear", x, bias, x_scale)
     given = x.dtype == torch.int8

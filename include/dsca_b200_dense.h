@@ -104,8 +104,8 @@ typedef struct {
 } dsca_quantize_rows_args;
 
 /*
- * y = (q w^T) * scale[row] * w_scale[column] (+ bias): the sum exact in 32-bit integers, the rest in
- * fp32, rounded once.  With x, q and scale are work areas that dsca_quantize_rows of x fills first.
+ * y = (q w^T) * w_scale[column] * scale[row] (+ bias): the sum exact in 32-bit integers, its conversion and the products and
+ * the addition, in this order, in fp32, the result rounded to dtype.  With x, q and scale are work areas that dsca_quantize_rows of x fills first.
  */
 typedef struct {
   const void* x;        /* [rows, k], dtype, or NULL: q and scale are given */

@@ -257,3 +257,20 @@ def test_codes_and_weights_of_wider_ones(cuda, rows, k):
     x = randn(rows, 96)
     up, down = pack_int8(randn(k, 96)), Int8Weight(wide.q[:, :k], wide.scale)
     R.close(gated_ffn_int8(x, up, up, down), _ffn_int8_defined(x, up, up, down, "silu"))
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_int8_scales_of_every_size(cuda, T, dtype):
+    """Rows and weights so small or large that the product of their two scales is no normal number while the result is."""
+    from dsca_moe_b200 import gated_ffn_int8, int8_linear, pack_int8, quantize_rows
+
+    randn = _randn(cuda, T)
+    for sx, sw in ((2.0 ** -112, 2.0 ** -10), (2.0 ** -90, 2.0 ** -30), (2.0 ** 100, 2.0 ** 20), (2.0 ** 120, 2.0 ** -60), (2.0 ** -100, 2.0 ** 80)):
+        x, w = (randn(T, 264) * sx).to(dtype), pack_int8((randn(136, 264) * sw).to(dtype))
+        q, s = quantize_rows(x)
+        R.close(int8_linear(x, w), R.int8_linear(q, s, w.q, w.scale, dtype), (sx, sw))
+        # gate and up of some 2^-20 to 2^0 each: their sums stay normal numbers while the scales' products do not
+        up, down = pack_int8((randn(136, 264) * 2.0 ** -8 / sx).to(dtype)), pack_int8(randn(264, 136).to(dtype))
+        if 2.0 ** -8 / sx < 2.0 ** 90:
+            R.close(gated_ffn_int8(x, up, up, down, act="relu"), R.ffn_int8(x, up, up, down, "relu", dtype), sx)
