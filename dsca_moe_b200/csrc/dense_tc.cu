@@ -1137,6 +1137,11 @@ int resident_pairs() {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// Boxes of 16-bit operands that one accumulator takes, 65536 of k: the tensor cores' additions truncate, always towards
+// zero, and a sum of one sign loses 3e-4 to 5e-4 of itself over these (12 million tokens in 8 accumulators: a weight's gradient
+// off by 9.5e-3, now 5e-4).  Longer sums are split, their parts added in rounded fp32.
+constexpr int kMaxChain = 1024;
+
 // The tiling of a job: fills everything of P but the maps and pointers.  Returns the units of work, or -1 when they
 // pass 2^31.
 int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counters) {
@@ -1221,7 +1226,12 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
   for (int i = 0; i < j.nprob; ++i) {
     Prob& q = P.prob[i];
     const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
+    if (!j.i8 && !f32 && q.per > kMaxChain) {
+      q.per = kMaxChain;
+      q.splits = ceil_div(q.boxes, q.per);
+    }
     if (q.splits > 1) {
+      if ((int64_t)*counters + tiles * 2 * kEpiWarps > 0x7fffffff) return -1;
       q.part = (int64_t)*floats;
       q.counter = (int)*counters;
       *floats += (size_t)tiles * q.splits * 2 * ((q.tn + 31) / 32 * 32) * 128;

@@ -274,3 +274,44 @@ def test_int8_scales_of_every_size(cuda, T, dtype):
         up, down = pack_int8((randn(136, 264) * 2.0 ** -8 / sx).to(dtype)), pack_int8(randn(264, 136).to(dtype))
         if 2.0 ** -8 / sx < 2.0 ** 90:
             R.close(gated_ffn_int8(x, up, up, down, act="relu"), R.ffn_int8(x, up, up, down, "relu", dtype), sx)
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_int8_products_of_subnormal_scales(cuda, T, dtype):
+    """Scales whose product, near 1e-42, has some ten bits left; the results are normal numbers (all terms of one sign)."""
+    from dsca_moe_b200 import int8_linear, pack_int8, quantize_rows
+
+    randn = _randn(cuda, T)
+    for sx, sw in ((2.0 ** -115, 2.0 ** -10), (2.0 ** -105, 2.0 ** -20), (2.0 ** -60, 2.0 ** -65), (2.0 ** -5, 2.0 ** -120)):
+        x, w = (randn(T, 264).abs() * sx).to(dtype), pack_int8((randn(136, 264).abs() * sw).to(dtype))
+        q, s = quantize_rows(x)
+        v, e = R.int8_linear(q, s, w.q, w.scale, dtype)
+        assert v.min() > 2.0 ** -126 and (s[0].double() * w.scale[0].double()) < 2.0 ** -130
+        assert ((int8_linear(x, w).double() - v).abs() <= e + 2.0 ** -149).all(), (sx, sw)
+
+
+@pytest.mark.parametrize("T", [65536, 65536 * 2 + 1, 900000, 3000001])
+def test_weight_gradients_of_many_tokens(cuda, T):
+    """Sums of one sign over many tokens, whose terms are exact, so that only the sum's own additions and the final rounding
+    count.  An accumulator takes 65536 tokens in steps of 16 at most: 4096 additions cut off at 2^-23 of the running sum, which is
+    half the final one on average, 2^-12 of the sum; twice that for what is cut off inside a step."""
+    from dsca_moe_b200 import check_dense, gated_ffn
+
+    d = I = 64
+    g = torch.Generator(device=cuda)
+    g.manual_seed(1)
+    top = torch.linspace(2, 64, 32, device=cuda).round()  # columns of different means
+    a = 1 + (torch.rand(T, 32, generator=g, device=cuda) * (top + 1)).floor().clamp_max(64) / 64
+    x = torch.cat([a, 4 - a], 1).to(BF16)  # a row's sum is 128: with weights of 1 / 128 g = u = 1
+    c = (1 + torch.randint(0, 128, (T, 1), generator=g, device=cuda) / 128).to(BF16)
+    wg, wu = (torch.full((I, d), 1 / 128, dtype=BF16, device=cuda, requires_grad=True) for _ in range(2))
+    wd = torch.full((d, I), 1 / I, dtype=BF16, device=cuda, requires_grad=True)
+    y = gated_ffn(x, wg, wu, wd, act="relu")
+    assert (y == 1).all()
+    got = torch.autograd.grad(y, (wg, wu, wd), c.expand(T, d).contiguous())
+    ref = sum((x[i:i + 500000].double() * c[i:i + 500000].double()).sum(0) for i in range(0, T, 500000))  # dh = dg = du = c, h = 1
+    for v, r in zip(got, (ref.expand(I, d), ref.expand(I, d), c.double().sum().expand(d, I))):
+        half = 2.0 ** (torch.floor(torch.log2(r)) - 8)
+        assert ((v.double() - r).abs() <= half + 2.0 ** -11 * r).all(), float(((v.double() - r) / r).abs().max())
+    check_dense()
