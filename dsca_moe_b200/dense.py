@@ -423,6 +423,26 @@ def _plain(m: nn.Module) -> bool:
     return type(m) is nn.Linear and m.bias is None and type(m.weight) in (nn.Parameter, torch.Tensor) and _bare(m)
 
 
+def _parts(old: nn.Module):
+    """(names, Linear layers, gate, dropout or None) of a gated MLP; raises for one that is more than the block."""
+    kind = type(old).__name__
+    names = next((n for n in _NAMES if all(hasattr(old, m) for m in n)), None)
+    if names is None:
+        raise ValueError(f"{kind} has neither gate_proj / up_proj / down_proj nor wi_0 / wi_1 / wo")
+    linears = [getattr(old, n) for n in names]
+    if any(getattr(m, "bias", None) is not None for m in linears):
+        raise ValueError("gated blocks with biases are not offered")
+    act = _act_name(old)
+    if not _bare(old) or not all(_plain(m) for m in linears):
+        raise ValueError(f"{kind} has hooks, adapters or layers other than nn.Linear, which the block would leave out "
+                         "(replace it first, then put them on)")
+    dropout = getattr(old, "dropout", None)
+    rest = sorted(set(dict(old.named_children())) - {*names, "act_fn", "act", "dropout"})
+    if rest or not (dropout is None or type(dropout) is nn.Dropout):
+        raise ValueError(f"{kind} has {', '.join(rest) or 'a dropout of its own'}, which the block would leave out")
+    return names, linears, act, dropout
+
+
 class GatedFFN(nn.Module):
     """A dense gated MLP (Qwen2MoeMLP's gate_proj / up_proj / down_proj, or wi_0 / wi_1 / wo) on gated_ffn.
 
@@ -435,21 +455,7 @@ class GatedFFN(nn.Module):
 
     def __init__(self, old: nn.Module, int8: bool = False):
         super().__init__()
-        kind = type(old).__name__
-        names = next((n for n in _NAMES if all(hasattr(old, m) for m in n)), None)
-        if names is None:
-            raise ValueError(f"{kind} has neither gate_proj / up_proj / down_proj nor wi_0 / wi_1 / wo")
-        linears = [getattr(old, n) for n in names]
-        if any(getattr(m, "bias", None) is not None for m in linears):
-            raise ValueError("gated blocks with biases are not offered")
-        act = _act_name(old)
-        if not _bare(old) or not all(_plain(m) for m in linears):
-            raise ValueError(f"{kind} has hooks, adapters or layers other than nn.Linear, which the block would leave out "
-                             "(replace it first, then put them on)")
-        dropout = getattr(old, "dropout", None)
-        rest = sorted(set(dict(old.named_children())) - {*names, "act_fn", "act", "dropout"})
-        if rest or not (dropout is None or type(dropout) is nn.Dropout):
-            raise ValueError(f"{kind} has {', '.join(rest) or 'a dropout of its own'}, which the block would leave out")
+        names, linears, act, dropout = _parts(old)
         self.names, self.act, self.int8 = names, act, bool(int8)
         self.act_fn = old.act_fn if getattr(old, "act_fn", None) is not None else old.act
         self.dropout = dropout

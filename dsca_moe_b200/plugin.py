@@ -75,17 +75,18 @@ def _replace(model, parent_t, moe_t, layer_idx, name_experts, router_path, confi
 def replace_dense_ffn(model, mlp_parent_type, mlp_type, int8=False):
     """Inside every module whose class name is `mlp_parent_type`, replace each child whose class name is
     `mlp_type` (a gated MLP: gate_proj / up_proj / down_proj or wi_0 / wi_1 / wo) by a GatedFFN, on the same
-    parameters or, with int8=True, on 8-bit integer weights.  Returns the number replaced."""
-    from .dense import GatedFFN
+    parameters or, with int8=True, on 8-bit integer weights.  Returns the number replaced; raises, with the model as it
+    was, where GatedFFN refuses one."""
+    from .dense import GatedFFN, _parts
 
-    changed = 0
-    for parent in list(model.modules()):
-        if type(parent).__name__ != mlp_parent_type:
-            continue
-        for name, child in list(parent.named_children()):
-            if type(child).__name__ == mlp_type:
-                setattr(parent, name, GatedFFN(child, int8=int8))
-                changed += 1
+    found = [(parent, name, child) for parent in model.modules() if type(parent).__name__ == mlp_parent_type
+             for name, child in parent.named_children() if type(child).__name__ == mlp_type]
+    for _, _, child in found:  # before the first is replaced
+        _parts(child)
+    changed = len(found)
+    while found:  # 8-bit weights: one old module at a time stays beside its packed one
+        parent, name, child = found.pop(0)
+        setattr(parent, name, GatedFFN(child, int8=int8))
     return changed
 
 

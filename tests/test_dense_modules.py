@@ -160,3 +160,21 @@ def test_int8_scales_stay_fp32(monkeypatch):
     assert model[0].weight.dtype == torch.bfloat16
     model.to("meta")
     assert all(b.device.type == "meta" and b.dtype == was[n].dtype for n, b in model[1].named_buffers())
+
+
+def test_a_refused_layer_leaves_the_model_as_it_was():
+    from dsca_moe_b200 import GatedFFN, replace_dense_ffn
+
+    class Layer(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.mlp = Gated()
+
+    model = nn.Sequential(Layer(), Layer())
+    model[1].mlp.act_fn = nn.GELU()
+    with pytest.raises(ValueError, match="not offered"):
+        replace_dense_ffn(model, "Layer", "Gated")
+    assert type(model[0].mlp) is Gated
+    model[1].mlp.act_fn = nn.ReLU()
+    assert replace_dense_ffn(model, "Layer", "Gated") == 2
+    assert [type(m.mlp) for m in model] == [GatedFFN, GatedFFN] and model[1].mlp.act == "relu"
