@@ -16,7 +16,7 @@ class _WithoutGradient(torch.autograd.Function):
     @staticmethod
     def forward(ctx, what, out, *inputs):
         ctx.what = what
-        return out.view_as(out)
+        return out.detach()  # no view: callers may add to it in place
 
     @staticmethod
     def backward(ctx, dy):

@@ -83,3 +83,17 @@ def test_helpers():
         refuse_tangents("it", x, w, None)
         with pytest.raises(NotImplementedError, match="it has no forward-mode"):
             refuse_tangents("it", x, fwad.make_dual(x, x))
+
+
+@pytest.mark.parametrize("make", [_qwen, _switch])
+def test_results_in_place(make):
+    """A decoder that adds to the block's result in place."""
+    block, first, x = make(False), nn.Linear(8, 8), torch.randn(2, 3, 8)
+    with torch.no_grad():
+        want = (block(first(x)) * 3).add_(first(x))
+    out = block(first(x))
+    out.mul_(3)
+    out += first(x)
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="MoE block"):
+        out.sum().backward()
