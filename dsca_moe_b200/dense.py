@@ -38,6 +38,7 @@ def _err(dev):
         if torch.cuda.is_current_stream_capturing():
             return None
         t = torch.zeros(64, dtype=torch.int32, device=dev)
+        torch.cuda.current_stream(dev).synchronize()  # once: a call on another stream may record before this one's zeros land
         e = _ERR[dev.index] = (t.data_ptr(), t)
     return e[0]
 

@@ -315,3 +315,17 @@ def test_weight_gradients_of_many_tokens(cuda, T):
         half = 2.0 ** (torch.floor(torch.log2(r)) - 8)
         assert ((v.double() - r).abs() <= half + 2.0 ** -11 * r).all(), float(((v.double() - r) / r).abs().max())
     check_dense()
+
+
+def test_error_word_is_there_before_its_address_is(cuda, monkeypatch):
+    """The word's zeros have landed when the first call gets its address, whatever its stream was busy with: a call on another
+    stream may record an error at once."""
+    import dsca_moe_b200.dense as D
+
+    monkeypatch.setattr(D, "_ERR", {})
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.zeros(64, dtype=torch.int32, device=cuda)  # its memory is at hand: no allocation that waits by itself
+        torch.cuda._sleep(400_000_000)
+        D._err(torch.device("cuda", torch.cuda.current_device()))
+        assert stream.query()
