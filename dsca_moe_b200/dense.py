@@ -132,12 +132,11 @@ def _saved(rows: int, inter: int, dtype):
     return ld_h, step, 3 * step + (8 * rows * ((inter + 31) // 32) if dtype is _BF16 else 0)
 
 
-def _as_saved(t, name: str, shape, like):
+def _as_saved(t, name: str, shape, dtype, index: int):
     """(t, its row stride) of a tensor that the backward pass reads.  Saved-tensor hooks (offloading, for one) may return it
     in other strides than it was saved with, and a gradient comes in any (expanded, transposed)."""
-    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"{name} came back as {t.dtype} {tuple(t.shape)} on {t.device}, not {like.dtype} {tuple(shape)} on "
-                           f"{like.device}")
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
+        raise RuntimeError(f"{name} came back as {t.dtype} {tuple(t.shape)} on {t.device}, not {dtype} {tuple(shape)} on GPU {index}")
     if t.is_contiguous():
         return t, shape[-1]
     try:
@@ -150,7 +149,7 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, wd, act, shapes):
         y, buf = _forward(x, wg, wu, wd, act, shapes, True)
-        ctx.act, ctx.sizes, ctx.x_shape, ctx.saved_bytes = act, shapes[:3], x.shape, 0 if buf is None else buf.numel()
+        ctx.act, ctx.sizes, ctx.x_shape = act, shapes[:3], x.shape
         ctx.save_for_backward(x, wg, wu, wd, buf)
         return y
 
@@ -167,16 +166,17 @@ class _GatedFFN(torch.autograd.Function):
         dwd = torch.empty((d, inter), dtype=dtype, device=dev) if need[3] else None
         dx_p, dwg_p, dwu_p, dwd_p = [None if t is None else t.data_ptr() for t in (dx, dwg, dwu, dwd)]
         if rows:
-            dy, ld_dy = _as_saved(dy, "dy", ctx.x_shape, dy)
-            x, ld_x = _as_saved(x, "x", ctx.x_shape, dy)
-            (wg, ld_g), (wu, ld_u), (wd, ld_d) = (_as_saved(w, n, torch.Size(s), dy) for w, n, s in (
-                (wg, "w_gate", (inter, d)), (wu, "w_up", (inter, d)), (wd, "w_down", (d, inter))))
-            if buf.dtype != torch.uint8 or buf.device != dev or buf.numel() != ctx.saved_bytes or not buf.is_contiguous() \
-                    or buf.data_ptr() % 16:
-                raise RuntimeError("the saved intermediates came back otherwise than they were saved")
-            ld_h, step, _ = _saved(rows, inter, dtype)
+            i, x_shape = dy.get_device(), ctx.x_shape
+            dy, ld_dy = _as_saved(dy, "dy", x_shape, dtype, i)
+            x, ld_x = _as_saved(x, "x", x_shape, dtype, i)
+            wg, ld_g = _as_saved(wg, "w_gate", (inter, d), dtype, i)
+            wu, ld_u = _as_saved(wu, "w_up", (inter, d), dtype, i)
+            wd, ld_d = _as_saved(wd, "w_down", (d, inter), dtype, i)
+            ld_h, step, size = _saved(rows, inter, dtype)
             grads = torch.empty(2 * step, dtype=torch.uint8, device=dev)
             h, dg = buf.data_ptr(), grads.data_ptr()
+            if buf.dtype is not torch.uint8 or buf.get_device() != i or buf.numel() != size or not buf.is_contiguous() or h % 16:
+                raise RuntimeError("the saved intermediates came back otherwise than they were saved")
             a = L.GatedFfnBackwardArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), dy.data_ptr(), h + step,
                                        h + 2 * step, h + 3 * step, h, dx_p, dwg_p, dwu_p, dwd_p, dg, dg + step, rows, d,
                                        inter, _DTYPES[dtype], ctx.act, ld_x, ld_g, ld_u, ld_d, ld_dy, ld_h, None, 0,

@@ -32,6 +32,7 @@ def refuse_tangents(what: str, *inputs) -> None:
 
 def without_gradient(what: str, out: torch.Tensor, *inputs) -> torch.Tensor:
     """`out`; a backward pass through it raises where one of `inputs` wants a gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return _WithoutGradient.apply(what, out, *inputs)
+    for t in inputs:
+        if t is not None and t.requires_grad:
+            return _WithoutGradient.apply(what, out, *inputs) if torch.is_grad_enabled() else out
     return out
