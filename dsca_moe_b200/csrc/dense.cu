@@ -171,10 +171,10 @@ struct Call {
   int product(const Job& j, const Own& o, bool pdl) {
     return dry ? DSCA_OK : launch_tc(j, o.parts, o.counters, err, pdl, stream);
   }
-  int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, float* row_max,
+  int quantize(const void* x, int rows, int k, int dtype, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, bool max_alone,
                bool pdl) {
     dsca_quantize_rows_args a = {x, rows, k, dtype, ld_x, q, ld_q, scale};
-    return dry ? DSCA_OK : launch_quantize_rows(&a, row_max, pdl, stream);
+    return dry ? DSCA_OK : launch_quantize_rows(&a, max_alone, pdl, stream);
   }
 };
 
@@ -287,27 +287,18 @@ int run(Call& c, const dsca_int8_linear_args* a) {
   bool none;
   if (!few) TRY(c.reserve(jobs, own, 1));
   TRY(c.relay(&none));
-  if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, nullptr, false));
+  if (a->x != nullptr) TRY(c.quantize(a->x, a->rows, a->k, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, false, false));
   if (few) return c.dry ? DSCA_OK : launch_few(j, nullptr, a->x != nullptr, c.stream);
   return c.product(j, own[0], a->x != nullptr);
 }
 
 int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   Job j = {}, k = {};
-  // fp32 tokens: h in 64 bits, from the exact sums on.  One code on the other side of its border moves a token's y by
-  // 1e-3 of its size, and an h off by fp32's roundings has one in every 10^6 there.  (bf16 tokens' y is rounded by as much.)
-  const bool wide = a->dtype == DSCA_F32;
-  const int64_t ld_w = ((int64_t)a->inter + 15) / 16 * 16;
-  double* hw = nullptr;
-  if (wide) {
-    hw = reinterpret_cast<double*>(c.take((size_t)a->rows * ld_w * sizeof(double)));
-    j.row_max = reinterpret_cast<float*>(c.take((size_t)a->rows * sizeof(float)));
-    if (!c.fits()) return DSCA_ERR_CAPACITY;
-  }
   j.epi = kGlu; j.act = a->act; j.nprob = 1; j.dtype = DSCA_F32; j.i8 = 1;
-  j.prob[0] = problem({a->w_gate, a->ld_gate, 0, 0}, {a->q, a->ld_q, 0, 0}, a->inter, a->rows, a->d,
-                      wide ? static_cast<void*>(hw) : a->h, wide ? ld_w : a->ld_h);
+  j.prob[0] = problem({a->w_gate, a->ld_gate, 0, 0}, {a->q, a->ld_q, 0, 0}, a->inter, a->rows, a->d, a->h, a->ld_h);
   j.prob[0].a[1] = {a->w_up, a->ld_up, 0, 0};
+  const bool wide = a->dtype == DSCA_F32;
+  if (wide) j.row_max = a->scale;
   j.row_scale = a->scale; j.col_scale[0] = a->gate_scale; j.col_scale[1] = a->up_scale;
   k.epi = kStore; k.nprob = 1; k.dtype = a->dtype; k.i8 = 1;
   k.prob[0] = problem({a->w_down, a->ld_down, 0, 0}, {a->hq, a->ld_hq, 0, 0}, a->d, a->rows, a->inter, a->y, a->ld_y);
@@ -318,11 +309,13 @@ int run(Call& c, const dsca_gated_ffn_int8_args* a) {
   bool none;
   if (!few) TRY(c.reserve(jobs, own, 2));
   TRY(c.relay(&none));
-  TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, const_cast<float*>(j.row_max), false));
+  TRY(c.quantize(a->x, a->rows, a->d, a->dtype, a->ld_x, a->q, a->ld_q, a->scale, wide, false));
   if (few && !c.dry) TRY(launch_few(j, &k, true, c.stream));
   if (!few) TRY(c.product(j, own[0], true));
-  if (!wide) TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale, nullptr, true));
-  if (wide && !c.dry) TRY(launch_quantize_rows64(hw, a->rows, a->inter, ld_w, a->hq, a->ld_hq, a->h_scale, true, c.stream));
+  // fp32 tokens: one code on the other side of its border moves a token's y by 1e-3 of its size, and an h in fp32 has such
+  // codes in every call.  (bf16 tokens' y is rounded by as much.)
+  if (!wide) TRY(c.quantize(a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale, false, true));
+  if (wide && !c.dry) TRY(launch_quantize_h(a, true, c.stream));
   if (few) return c.dry ? DSCA_OK : launch_few(k, nullptr, true, c.stream);
   return c.product(k, own[1], true);
 }
@@ -384,7 +377,7 @@ int dsca_quantize_rows(const dsca_quantize_rows_args* a, dsca_stream_t stream) {
   if (int rc = dense::check(a)) return rc;
   if (a->rows == 0) return DSCA_OK;
   if (int rc = dense::device_ok()) return rc;
-  return dense::launch_quantize_rows(a, nullptr, false, stream);
+  return dense::launch_quantize_rows(a, false, false, stream);
 }
 
 int dsca_int8_linear(const dsca_int8_linear_args* a, dsca_stream_t stream) {

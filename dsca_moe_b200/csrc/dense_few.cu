@@ -48,7 +48,8 @@ struct Params {
   void* save_u;
   uint8_t* save_e;
   int groups;  // exponents of a saved row
-  const float* row_scale;  // O = double: row_max
+  const float* row_scale;  // close: row_max
+  int close;
   const float* col_scale[2];
   const void* bias;
   const uint8_t* ahead;  // the next product's weights: asked into L2 by this one's CTAs, `ahead_step` bytes each
@@ -147,7 +148,6 @@ __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(double* p, float v) { *p = v; }
 
 // NT groups of eight tokens.  (Two: four CTAs an SM, 16 tokens through a 2048 x 5632 bf16 block 23.3 us, 25.5 with the three
 // that 70 registers a thread let in; three and four, fp32: two CTAs, 32 tokens 82 us, 103 without, for all that two values
@@ -294,19 +294,24 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 0 : NT == 2 ? 4 : 2) fe
         if constexpr (kGluE) vb += tail_sum(xt, reinterpret_cast<const int8_t*>(p.w[1]) + (int64_t)m * p.ldw[1] + p.K, p.tail);
       }
     }
-    if constexpr (std::is_same<O, double>::value) {
-      if (in) {
-        const double xs = (double)p.row_scale[n] / 127.0;
-        reinterpret_cast<double*>(p.out)[(int64_t)n * p.ldo + m] = h64(va, vb, xs, p.col_scale[0][m], p.col_scale[1][m], p.act);
+    if constexpr (kGluE && std::is_same<T, int8_t>::value) {
+      if (p.close) {
+        if (in) {
+          const int g[1] = {va}, u[1] = {vb};
+          const float gs[1] = {p.col_scale[0][m]}, us[1] = {p.col_scale[1][m]};
+          const Two xs[1] = {scale_two(p.row_scale[n])};
+          float h[1];
+          close_all(h, g, u, gs, us, xs, p.act);
+          reinterpret_cast<float*>(p.out)[(int64_t)n * p.ldo + m] = h[0];
+        }
+        continue;
       }
-      continue;
     }
     float v = (float)va, u = (float)vb;
     if constexpr (std::is_same<T, int8_t>::value) {
       const float rs = p.row_scale[n];
-      // (the scales' own product may leave fp32's normal numbers where the result does not)
-      v = in ? v * p.col_scale[0][m] * rs : 0.0f;
-      if constexpr (kGluE) u = in ? u * p.col_scale[1][m] * rs : 0.0f;
+      v = in ? scaled<true>(va, p.col_scale[0][m], rs) : 0.0f;
+      if constexpr (kGluE) u = in ? scaled<true>(vb, p.col_scale[1][m], rs) : 0.0f;
     }
     if constexpr (kGluE) {
       if (p.save_g != nullptr) {
@@ -415,7 +420,8 @@ int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   p.act = j.act;
   p.out = s.out; p.ldo = s.ldo;
   p.save_g = j.save_g; p.save_u = j.save_u; p.save_e = j.save_e; p.groups = exp_groups(s.M);
-  p.row_scale = j.row_max != nullptr ? j.row_max : j.row_scale; p.col_scale[0] = j.col_scale[0]; p.col_scale[1] = j.col_scale[1]; p.bias = j.bias;
+  p.close = j.row_max != nullptr;
+  p.row_scale = p.close ? j.row_max : j.row_scale; p.col_scale[0] = j.col_scale[0]; p.col_scale[1] = j.col_scale[1]; p.bias = j.bias;
   if (next != nullptr) {
     const Operand& w = next->prob[0].a[0];
     const int64_t bytes = ((next->prob[0].M - 1) * w.ld + next->prob[0].K) * es & ~15ll;  // up to the last row's end
@@ -427,9 +433,7 @@ int launch_few(const Job& j, const Job* next, bool pdl, cudaStream_t stream) {
   }
   using B = __nv_bfloat16;
   if (j.i8) {
-    if (j.epi == kGlu)
-      return j.row_max != nullptr ? few::by_tokens<int8_t, double, kGlu>(p, true, true, pdl, stream)
-                                  : few::by_tokens<int8_t, float, kGlu>(p, true, true, pdl, stream);
+    if (j.epi == kGlu) return few::by_tokens<int8_t, float, kGlu>(p, true, true, pdl, stream);
     return j.dtype == DSCA_BF16 ? few::by_tokens<int8_t, B, kStore>(p, true, true, pdl, stream)
                                 : few::by_tokens<int8_t, float, kStore>(p, true, true, pdl, stream);
   }

@@ -13,6 +13,7 @@
 #include "dense.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace dsca {
 namespace dense {
@@ -75,6 +76,32 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float amax, float i
                     __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
+// Rows of h (below): the largest value under which all codes are formed again, and the error of 127 h / max relative to itself:
+// the bounds of h and of the largest, the rounded 127 / max and its product.
+constexpr float kTiny = 1e-25f;
+constexpr float kOpen = 2.1f * kCloseH + 2.4e-7f;
+
+// Eight codes of h, and whether one of them is open.
+__device__ __forceinline__ uint2 codes8_h(const float (&x)[8], float inv, bool& open) {
+  constexpr float kRound = 12582912.0f;
+  uint32_t b[8];
+  const float2 inv2 = make_float2(inv, inv), up = make_float2(kRound, kRound), minus = make_float2(-1.0f, -1.0f);
+  const float own = inv * kOpen;
+  float far = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 v = make_float2(x[i], x[i + 1]), r = __ffma2_rn(v, inv2, up);
+    const float2 c = __ffma2_rn(r, minus, up);  // minus the code
+    const float2 d = __ffma2_rn(v, inv2, c);
+    far = fmaxf(far, fmaxf(fmaf(fabsf(v.x), own, fabsf(d.x)), fmaf(fabsf(v.y), own, fabsf(d.y))));
+    b[i] = __float_as_uint(r.x);
+    b[i + 1] = __float_as_uint(r.y);
+  }
+  open |= far > 0.499999f;
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
 // Eight consecutive values as they lie in memory.
 template <typename T>
 struct Raw {
@@ -124,6 +151,31 @@ struct Raw {
   }
 };
 
+// ---- The intermediate of an 8-bit block, by the codes of its 64-bit value (kH)
+//
+// h = act(g) u was formed within kCloseH of itself, and so was the row's largest.  Where that leaves open on which side of a border
+// 127 h / max|h| lies (one value in 30000), warps form the h of that channel, and of those that may be the row's largest, again
+// from the codes: two exact sums of d products, scales and gate in 64 bits.  Other rows' scale is off by kCloseH.
+//
+// A gate that is 0 in fp32 instead of 1e-36 and products below fp32's normal numbers matter only in rows whose largest value is
+// tiny (kTiny): there all values are formed again.
+
+// h of a row and channel in 64 bits, by a whole warp.  Codes of x past d are zeros, those of the weights do not count.
+__device__ __noinline__ double warp_h(const dsca_gated_ffn_int8_args& a, int64_t row, int c, double xs) {
+  const int8_t *x = a.q + row * a.ld_q, *g = a.w_gate + (int64_t)c * a.ld_gate, *u = a.w_up + (int64_t)c * a.ld_up;
+  int sg = 0, su = 0;
+#pragma unroll 4
+  for (int i = 16 * (int)(threadIdx.x % 32); i < a.d; i += 512) {
+    const int4 p = *reinterpret_cast<const int4*>(x + i), q = __ldg(reinterpret_cast<const int4*>(g + i)),
+               r = __ldg(reinterpret_cast<const int4*>(u + i));
+    sg = __dp4a(p.x, q.x, __dp4a(p.y, q.y, __dp4a(p.z, q.z, __dp4a(p.w, q.w, sg))));
+    su = __dp4a(p.x, r.x, __dp4a(p.y, r.y, __dp4a(p.z, r.z, __dp4a(p.w, r.w, su))));
+  }
+  sg = __reduce_add_sync(0xffffffffu, sg);
+  su = __reduce_add_sync(0xffffffffu, su);
+  return gate64((double)sg * xs * (double)a.gate_scale[c], a.act) * ((double)su * xs * (double)a.up_scale[c]);
+}
+
 // TPR threads a row, CH chunks of eight values a thread in registers (CH = 0: longer rows, read twice).  A CTA goes
 // through rows with the next one's values on their way while one is turned into codes: with a CTA a row and no
 // such overlap, 16384 x 5632 bf16 took 107 us.  bf16 rows of more than 2048 values come through a ring of two
@@ -133,8 +185,13 @@ template <typename T, int TPR, int CH, bool kVec>
 constexpr bool in_ring() { return kVec && TPR * CH > 256 && sizeof(T) == 2; }
 constexpr int kDepth = 2;
 
-template <typename T, int TPR, int CH, bool kVec>
-__global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a, float* row_max) {
+// What the scales take: max / 127; the largest magnitude itself; max / 127 with the sign set where a code of the row (or of one
+// that shares its CTA) is open.
+enum Form { kScale = 0, kMax = 1, kH = 2 };
+
+template <typename T, int TPR, int CH, bool kVec, int FORM>
+__global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_args a) {
+  static_assert(FORM == kScale || sizeof(T) == 4, "fp32 tokens");
   __shared__ uint32_t red[2][8];
   extern __shared__ uint4 ring[];  // [kDepth][CH][256], each thread's own chunks
   constexpr int kRows = 256 / TPR, N = CH > 0 ? CH : 1;
@@ -205,14 +262,13 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
       fetch(row + kDepth * step, slot);
       slot ^= 1;
     }
-    if (!live) continue;
-    if (tid == 0) {
-      a.scale[row] = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
-      if (row_max != nullptr) row_max[row] = m;
-    }
+    if (FORM != kH && !live) continue;
+    const float scale = FORM == kMax ? m : m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
+    if (FORM != kH && tid == 0) a.scale[row] = scale;
     // codes mean nothing in a row that is not finite: zeros
     const bool usable = m > 0.0f && m < INFINITY;
-    const bool ends = m < 1e-30f || m > 1e36f;  // 127 / m or 127 x leaves fp32's normal numbers
+    const bool ends = FORM == kH ? m < kTiny : m < 1e-30f || m > 1e36f;  // 127 / m or 127 x leaves fp32's normal numbers
+    bool open = FORM == kH && live && usable && ends;  // a code of this thread's
     const float inv = usable && !ends ? __fdiv_rn(127.0f, m) : 0.0f;
     auto store = [&](int c, const Raw<T>& raw) {
       uint2 w = make_uint2(0u, 0u);
@@ -220,7 +276,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
         float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = raw.get(e);
-        if (!ends) {
+        if constexpr (FORM == kH) {
+          if (!ends) w = codes8_h(o, inv, open);
+        } else if (!ends) {
           w = codes8<T>(o, m, inv);
         } else {
 #pragma unroll
@@ -237,19 +295,25 @@ __global__ void __launch_bounds__(256) quantize_kernel(const dsca_quantize_rows_
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int c = i * TPR + tid;
-        if (c < chunks) store(c, v[i]);
+        if (live && c < chunks) store(c, v[i]);
       }
-    } else {
+    } else if (live) {
       for (int c = tid; c < chunks; c += TPR) {
         v[0].template load<kVec>(x, c, a.k);
         store(c, v[0]);
       }
     }
+    if constexpr (FORM == kH) {
+      bool any;
+      if constexpr (TPR > 32) any = __syncthreads_or(open) != 0;
+      else any = __any_sync(0xffffffffu, open) != 0;
+      if (live && tid == 0) a.scale[row] = any && usable ? -scale : scale;
+    }
   }
 }
 
-template <typename T, int TPR, int CH>
-int launch(const dsca_quantize_rows_args& a, float* row_max, bool pdl, cudaStream_t stream) {
+template <typename T, int TPR, int CH, int FORM>
+int launch(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
   // CTAs go round, two for each that an SM holds at a time or nearly so (long fp32 rows: 80 registers a thread, three)
   constexpr int kCtas = sizeof(T) == 4 && CH > 2 ? 6 : 8;
   const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * TPR + 255) / 256, (int64_t)kCtas * current_device_sms());
@@ -264,120 +328,135 @@ int launch(const dsca_quantize_rows_args& a, float* row_max, bool pdl, cudaStrea
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
   if (vec && in_ring<T, TPR, CH, true>()) cfg.dynamicSmemBytes = (size_t)kDepth * CH * 256 * 16;  // 24 or 32 KB
-  auto kern = vec ? quantize_kernel<T, TPR, CH, true> : quantize_kernel<T, TPR, CH, false>;
-  return cudaLaunchKernelEx(&cfg, kern, a, row_max) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
+  // (rows of h are on 16-byte boundaries)
+  auto kern = FORM == kH || vec ? quantize_kernel<T, TPR, CH, true, FORM> : quantize_kernel<T, TPR, CH, FORM == kH, FORM>;
+  return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
-// Rows of 64-bit values: the quotient in 64 bits, divided where the product with 127 / max is next to a tie.  TPR threads a
-// row, four values each at a time; the row is read a second time from L1 or L2.
-template <int TPR>
-__global__ void __launch_bounds__(256) quantize64_kernel(const double* __restrict__ x, int rows, int k, int64_t ld, int8_t* q,
-                                                         int64_t ld_q, float* scale) {
-  __shared__ unsigned long long red[2][8];
-  constexpr int kRows = 256 / TPR;
-  const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
-  const int pieces = (int)(ld_q / 4);
+template <typename T, int FORM>
+int run(const dsca_quantize_rows_args& a, bool pdl, cudaStream_t stream) {
+  const int chunks = (int)(a.ld_q / 8);
+  if (a.rows > 4 * current_device_sms()) {  // a warp a row while a warp holds it
+    if (chunks <= 32) return launch<T, 32, 1, FORM>(a, pdl, stream);
+    if (chunks <= 64) return launch<T, 32, 2, FORM>(a, pdl, stream);
+    if (chunks <= 128) return launch<T, 64, 2, FORM>(a, pdl, stream);
+    if (chunks <= 256) return launch<T, 128, 2, FORM>(a, pdl, stream);
+  }
+  if (chunks <= 256) return launch<T, 256, 1, FORM>(a, pdl, stream);
+  if (chunks <= 512) return launch<T, 256, 2, FORM>(a, pdl, stream);
+  if (chunks <= 768) return launch<T, 256, 3, FORM>(a, pdl, stream);
+  if (chunks <= 1024) return launch<T, 256, 4, FORM>(a, pdl, stream);
+  return launch<T, 256, 0, FORM>(a, pdl, stream);
+}
+
+// Rows with open codes (their scale's sign is set): their largest value and those codes from 64 bits, a CTA a row.  The first open
+// value of each lane is formed before the largest is known and held, so that most rows wait for one such sum.  A launch of its
+// own: in the one above it took that kernel's registers and with them its speed (4096 x 5632 77 us, the two of them 42: 19 and 23).
+__global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ dsca_gated_ffn_int8_args a) {
+  __shared__ double red[2][8];
+  const int lane = threadIdx.x % 32, k = a.inter;
   pdl_launch_dependents();
   pdl_wait();
   int it = 0;
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += (int64_t)gridDim.x * kRows, it ^= 1) {
-    const int64_t row = first + sub;
-    const bool live = row < rows;
-    const double* r = x + (live ? row : 0) * ld;
-    // rows lie on 32-byte boundaries and hold a multiple of 16 values, of which those past k are not written
-    auto load = [&](int c, double (&v)[4]) {
-      const double2 a = c * 4 < k ? *reinterpret_cast<const double2*>(r + c * 4) : make_double2(0.0, 0.0);
-      const double2 b = c * 4 + 2 < k ? *reinterpret_cast<const double2*>(r + c * 4 + 2) : make_double2(0.0, 0.0);
-      v[0] = a.x;
-      v[1] = c * 4 + 1 < k ? a.y : 0.0;
-      v[2] = b.x;
-      v[3] = c * 4 + 3 < k ? b.y : 0.0;
-    };
-    unsigned long long bits = 0;  // of the largest magnitude, a NaN's being the largest
-    if (live) {
-#pragma unroll 4
-      for (int c = tid; c < pieces; c += TPR) {
-        double v[4];
-        load(c, v);
+  auto settle = [&](int64_t row, float s) {  // s: max / 127, rounded
+    const float m = 127.0f * s;
+    const bool all = m < 1.001f * kTiny;
+    const float inv = all ? 0.0f : __fdiv_rn(1.0f, s), least = all ? 0.0f : m * (1.0f - kOpen - 2.4e-7f);
+    const float* h = a.h + row * a.ld_h;
+    const double xs = (double)a.scale[row] / 127.0;
+    // f(channel, its lane, whether it may be the largest, whether its code is open) for each such value of the warp in turn
+    auto scan = [&](auto f) {
+      for (int c0 = 0; c0 < k; c0 += 8192) {  // 32 values a thread at a time
+        float4 v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bits = max(bits, (unsigned long long)__double_as_longlong(fabs(v[e])));
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-    if constexpr (TPR > 32) {
-      if (threadIdx.x % 32 == 0) red[it][threadIdx.x / 32] = bits;
-      __syncthreads();  // one a row: the next one writes the other half
-#pragma unroll
-      for (int i = 0; i < TPR / 32; ++i) bits = max(bits, red[it][sub * (TPR / 32) + i]);
-    }
-    if (!live) continue;
-    const double m = __longlong_as_double((long long)bits);
-    const float s = (float)(m / 127.0);
-    if (tid == 0) scale[row] = m == 0.0 ? 1.0f : s;
-    const bool usable = m > 0.0 && s < INFINITY;  // codes of other rows mean nothing
-    const double inv = usable ? 127.0 / m : 0.0;
-#pragma unroll 4
-    for (int c = tid; c < pieces; c += TPR) {
-      char4 w = make_char4(0, 0, 0, 0);
-      if (usable) {
-        double v[4];
-        int o[4];
-        load(c, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double p = v[e] * inv;
-          o[e] = __double2int_rn(p);
-          if (fabs(p - (double)o[e]) > 0.5 - 1e-9) o[e] = __double2int_rn(127.0 * v[e] / m);  // p is good to 1e-13
+        for (int i = 0; i < 8; ++i) {
+          const int at = c0 + 1024 * i + 4 * (int)threadIdx.x;  // rows hold a multiple of four values
+          v[i] = at < k ? *reinterpret_cast<const float4*>(h + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        w = make_char4((signed char)o[0], (signed char)o[1], (signed char)o[2], (signed char)o[3]);
+        uint32_t top = 0, open = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float h4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = h4[e] * inv;
+            if (c0 + 1024 * i + 4 * (int)threadIdx.x + e < k) {
+              top |= (uint32_t)(fabsf(h4[e]) >= least) << (4 * i + e);
+              open |= (uint32_t)(all || fabsf(p - rintf(p)) > 0.499999f - fabsf(p) * (kOpen + 2.4e-7f)) << (4 * i + e);
+            }
+          }
+        }
+        uint32_t marks = top | open;
+        for (unsigned any; (any = __ballot_sync(0xffffffffu, marks != 0u)) != 0u;) {
+          const int src = __ffs(any) - 1, e = __ffs(__shfl_sync(0xffffffffu, marks, src)) - 1;
+          const int c = c0 + 1024 * (e / 4) + 4 * ((int)(threadIdx.x & ~31u) + src) + e % 4;
+          f(c, src, (__shfl_sync(0xffffffffu, top, src) >> e & 1u) != 0u, (__shfl_sync(0xffffffffu, open, src) >> e & 1u) != 0u);
+          if (lane == src) marks &= marks - 1u;
+        }
       }
-      *reinterpret_cast<char4*>(q + row * ld_q + c * 4) = w;
+    };
+    double m64 = 0.0, held = 0.0;
+    int held_c = -1;
+    bool more = false;
+    scan([&](int c, int src, bool top, bool open) {
+      const bool hold = open && lane == src && held_c < 0;
+      const double w = top || __any_sync(0xffffffffu, hold) ? warp_h(a, row, c, xs) : 0.0;
+      if (top) m64 = fmax(m64, fabs(w));
+      if (hold) {
+        held = w;
+        held_c = c;
+      } else if (open && lane == src) {
+        more = true;
+      }
+    });
+    if (lane == 0) red[it][threadIdx.x / 32] = m64;  // the same in all lanes
+    __syncthreads();                                 // one a row: the next one writes the other half
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m64 = fmax(m64, red[it][i]);
+    it ^= 1;
+    int8_t* q = a.hq + row * a.ld_hq;
+    auto put = [&](int c, double w) { q[c] = (int8_t)(m64 > 0.0 ? (int)rint(127.0 * w / m64) : 0); };
+    if (held_c >= 0) put(held_c, held);
+    if (__any_sync(0xffffffffu, more))
+      scan([&](int c, int src, bool, bool open) {
+        if (!__any_sync(0xffffffffu, open && lane == src && c != held_c)) return;
+        const double w = warp_h(a, row, c, xs);
+        if (lane == src) put(c, w);
+      });
+    if (threadIdx.x == 0) a.h_scale[row] = m64 == 0.0 ? 1.0f : (float)(m64 / 127.0);
+  };
+  // 32 rows' signs at a time
+  for (int64_t first = blockIdx.x; first < a.rows; first += 32ll * gridDim.x) {
+    const int64_t mine = first + (int64_t)lane * gridDim.x;
+    const float s = mine < a.rows ? *const_cast<const volatile float*>(a.h_scale + mine) : 0.0f;
+    __syncthreads();  // every warp has read them before a row is settled
+    for (unsigned rows = __ballot_sync(0xffffffffu, __float_as_int(s) < 0 && s == s); rows != 0u; rows &= rows - 1u) {
+      const int i = __ffs(rows) - 1;
+      settle(first + (int64_t)i * gridDim.x, fabsf(__shfl_sync(0xffffffffu, s, i)));
     }
   }
 }
 
-template <int TPR>
-int launch64(const double* x, int rows, int k, int64_t ld, int8_t* q, int64_t ld_q, float* scale, bool pdl, cudaStream_t stream) {
+}  // namespace quant
+
+int launch_quantize_rows(const dsca_quantize_rows_args* a, bool max_alone, bool pdl, cudaStream_t stream) {
+  if (a->dtype == DSCA_BF16) return quant::run<__nv_bfloat16, quant::kScale>(*a, pdl, stream);
+  return max_alone ? quant::run<float, quant::kMax>(*a, pdl, stream) : quant::run<float, quant::kScale>(*a, pdl, stream);
+}
+
+int launch_quantize_h(const dsca_gated_ffn_int8_args* a, bool pdl, cudaStream_t stream) {
+  const dsca_quantize_rows_args rows = {a->h, a->rows, a->inter, DSCA_F32, a->ld_h, a->hq, a->ld_hq, a->h_scale};
+  if (int rc = quant::run<float, quant::kH>(rows, pdl, stream)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(((int64_t)rows * TPR + 255) / 256, (int64_t)8 * current_device_sms()));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(a->rows, (int64_t)32 * current_device_sms()));  // more than fit: rows differ
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, quantize64_kernel<TPR>, x, rows, k, ld, q, ld_q, scale) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
-}
-
-template <typename T>
-int run(const dsca_quantize_rows_args& a, float* row_max, bool pdl, cudaStream_t stream) {
-  const int chunks = (int)(a.ld_q / 8);
-  if (a.rows > 4 * current_device_sms()) {  // a warp a row while a warp holds it
-    if (chunks <= 32) return launch<T, 32, 1>(a, row_max, pdl, stream);
-    if (chunks <= 64) return launch<T, 32, 2>(a, row_max, pdl, stream);
-    if (chunks <= 128) return launch<T, 64, 2>(a, row_max, pdl, stream);
-    if (chunks <= 256) return launch<T, 128, 2>(a, row_max, pdl, stream);
-  }
-  if (chunks <= 256) return launch<T, 256, 1>(a, row_max, pdl, stream);
-  if (chunks <= 512) return launch<T, 256, 2>(a, row_max, pdl, stream);
-  if (chunks <= 768) return launch<T, 256, 3>(a, row_max, pdl, stream);
-  if (chunks <= 1024) return launch<T, 256, 4>(a, row_max, pdl, stream);
-  return launch<T, 256, 0>(a, row_max, pdl, stream);
-}
-
-}  // namespace quant
-
-int launch_quantize_rows(const dsca_quantize_rows_args* a, float* row_max, bool pdl, cudaStream_t stream) {
-  return a->dtype == DSCA_BF16 ? quant::run<__nv_bfloat16>(*a, row_max, pdl, stream) : quant::run<float>(*a, row_max, pdl, stream);
-}
-
-int launch_quantize_rows64(const double* x, int rows, int k, int64_t ld, int8_t* q, int64_t ld_q, float* scale, bool pdl,
-                           cudaStream_t stream) {
-  // a warp a row where there are rows for all of them and the rows are short
-  return k <= 1024 && rows > 4 * current_device_sms() ? quant::launch64<32>(x, rows, k, ld, q, ld_q, scale, pdl, stream)
-                                                      : quant::launch64<256>(x, rows, k, ld, q, ld_q, scale, pdl, stream);
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, quant::settle_kernel, *a) == cudaSuccess ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
 }  // namespace dense

@@ -108,7 +108,7 @@ struct Params {
   void* save_u;
   uint8_t* save_e;  // fp16: the exponents, [2][rows][exp_groups(cols)]
   void* out2;
-  const float* row_scale;  // O = double: row_max
+  const float* row_scale;  // CLOSE: row_max
   const float* col_scale[2];
   const void* bias;
   int vec_cols;  // col_scale on 16-byte boundaries
@@ -399,13 +399,15 @@ struct Ahead {
   }
 };
 
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(taddr));
 }
 
-template <int EPI, int IN, typename O>
+// CLOSE: gated 8-bit products by close_h.
+template <int EPI, int IN, typename O, bool CLOSE = false>
 __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params P) {
   constexpr bool kGluE = EPI == kGlu;
   using R = Ring<IN>;
@@ -415,8 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   constexpr int KE = IN == kI8 ? 128 : 64;   // k elements of a box
   constexpr int KS = IN == kI8 ? 32 : 16;    // ... and of one MMA
   constexpr bool kFast = IN != kF32;
-  constexpr bool kWide = sizeof(O) == 8;     // h of 8-bit products in 64 bits
-  static_assert(!kWide || (kGluE && IN == kI8), "64-bit results");
+  constexpr bool kBigI8 = EPI == kStore && sizeof(O) == 4;  // order of an 8-bit sum's scales
+  static_assert(!CLOSE || (kGluE && IN == kI8), "gated 8-bit products");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -715,74 +717,106 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           }
         }
       };
-      // eight columns, of 8-bit operands
-      auto finished8 = [&](int c, uint32_t (&r)[8]) {
+      // sixteen columns, of 8-bit operands
+      auto finished16 = [&](int c, uint32_t (&r)[16]) {
         if (q.splits == 1) {
-          tmem_ld8(taddr + c, r);
-          tmem_wait_ld();
+          tmem_ld16(taddr + c, r);
           return;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = 0u;
+        for (int j = 0; j < 16; ++j) r[j] = 0u;
         for (int s = 0; s < q.splits; ++s) {
           const float* at = part + s * part_step + (int64_t)c * 128;
-          const uint4 a = __ldcg(reinterpret_cast<const uint4*>(at)), b = __ldcg(reinterpret_cast<const uint4*>(at + 512));
-          r[0] += a.x; r[1] += a.y; r[2] += a.z; r[3] += a.w;
-          r[4] += b.x; r[5] += b.y; r[6] += b.z; r[7] += b.w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 x = __ldcg(reinterpret_cast<const uint4*>(at + j * 512));
+            r[4 * j] += x.x; r[4 * j + 1] += x.y; r[4 * j + 2] += x.z; r[4 * j + 3] += x.w;
+          }
         }
       };
-      if constexpr (kWide) {
-        // ------------ h in 64 bits, eight values of a row (rows) or of a column (columns) at a time
+      if constexpr (CLOSE) {
+        // ------------ 16 values of a row (rows) or of a column (columns) at a time, which keeps the code short
         if (mine && q.row) {
           const bool live = lrow < q.rows;
-          const double xs = live ? (double)__ldg(P.row_scale + lrow) / 127.0 : 0.0;
-          double* out = reinterpret_cast<double*>(q.out) + lrow * q.ldo;
+          const Two xs = scale_two(live ? __ldg(P.row_scale + lrow) : 0.0f);
+          float* out = reinterpret_cast<float*>(q.out) + lrow * q.ldo;
 #pragma unroll 1
-          for (int c = 32 * eh; c < min(q.tn / 2, t.nval); c += c % 32 == 24 ? 40 : 8) {  // alternate chunks of 32
-            uint32_t g[8], u[8];
-            finished8(c, g);
-            finished8(c + q.tn / 2, u);
-            if (live) {
+          for (int c = 32 * eh; c < t.nval; c += c % 32 == 16 ? 48 : 16) {  // alternate chunks of 32
+            const int n = t.n0 + c;
+            uint32_t g[16], u[16];
+            finished16(c, g);
+            finished16(c + q.tn / 2, u);
+            float gs[16], us[16], h[16];
+            Two x16[16];
+            if (P.vec_cols && n + 16 <= q.cols) {
 #pragma unroll
-              for (int i = 0; i < 8; i += 4) {
-                const int n = t.n0 + c + i;
+              for (int j = 0; j < 16; j += 4) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(P.col_scale[0] + n + j));
+                const float4 b = __ldg(reinterpret_cast<const float4*>(P.col_scale[1] + n + j));
+                gs[j] = a.x; gs[j + 1] = a.y; gs[j + 2] = a.z; gs[j + 3] = a.w;
+                us[j] = b.x; us[j + 1] = b.y; us[j + 2] = b.z; us[j + 3] = b.w;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const int at = min(n + j, q.cols - 1);
+                gs[j] = __ldg(P.col_scale[0] + at);
+                us[j] = __ldg(P.col_scale[1] + at);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x16[j] = xs;
+            tmem_wait_ld();
+            close_all(h, reinterpret_cast<const int(&)[16]>(g), reinterpret_cast<const int(&)[16]>(u), gs, us, x16, P.act);
+            if (!live) continue;
+#pragma unroll
+            for (int i = 0; i < 16; i += 8) {
+              if (q.vec == 2 && n + i + 8 <= q.cols) {
                 uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int at = min(n + j, q.cols - 1);
-                  const double h = h64((int)g[i + j], (int)u[i + j], xs, __ldg(P.col_scale[0] + at), __ldg(P.col_scale[1] + at), P.act);
-                  w[2 * j] = (uint32_t)__double2loint(h);
-                  w[2 * j + 1] = (uint32_t)__double2hiint(h);
-                }
-                // (rows hold a multiple of 16 values and start on 32-byte boundaries)
-                if (n < q.cols) store32(out + n, w);
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(h[i + j]);
+                store32(out + n + i, w);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (n + i + j < q.cols) out[n + i + j] = h[i + j];
               }
             }
           }
         } else if (mine) {
           const int ch = t.m0 + 64 * (int)rank + 32 * (q4 & 1) + lane, up = q4 >> 1;
           const bool in = ch < q.cols;
-          const double gs = in ? __ldg(P.col_scale[0] + ch) : 0.0f, us = in ? __ldg(P.col_scale[1] + ch) : 0.0f;
+          const float gs = in ? __ldg(P.col_scale[0] + ch) : 0.0f, us = in ? __ldg(P.col_scale[1] + ch) : 0.0f;
+          float gs16[16], us16[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) gs16[j] = gs, us16[j] = us;
 #pragma unroll 1
-          for (int c = 32 * eh; c < t.nval; c += c % 32 == 24 ? 40 : 8) {
-            uint32_t r[8];
-            finished8(c, r);
-            // the gate warp forms the first four tokens, the up warp the others (two buffers: one barrier a step)
+          for (int c = 32 * eh; c < t.nval; c += 64) {
+            uint32_t r[32];
+            finished(c, r);
+            const Two mine2 = scale_two(c + lane < t.nval ? __ldg(P.row_scale + t.n0 + c + lane) : 0.0f);  // of token c + lane
+            // the gate warp forms the first 16 tokens, the up warp the others (two buffers: one barrier a chunk)
             uint32_t* mine_x = reinterpret_cast<uint32_t*>(stg) + xb * 512;
             const uint32_t* other_x = reinterpret_cast<const uint32_t*>(smem + kRingBytes + (ew ^ 2) * kStgBytes) + xb * 512;
             xb ^= 1;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mine_x[j * 32 + lane] = up ? r[j] : r[4 + j];
+            for (int j = 0; j < 16; ++j) mine_x[j * 32 + lane] = up ? r[j] : r[16 + j];
             pair_barrier(pair_id);
+            int g[16], u[16];
+            float h[16];
+            Two xs[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 16; ++j) {
               const uint32_t got = other_x[j * 32 + lane];
-              const int tok = c + 4 * up + j;
-              if (in && tok < t.nval)
-                reinterpret_cast<double*>(q.out)[(int64_t)(t.n0 + tok) * q.ldo + ch] =
-                    h64((int)(up ? got : r[j]), (int)(up ? r[4 + j] : got), (double)__ldg(P.row_scale + t.n0 + tok) / 127.0, gs, us,
-                        P.act);
+              g[j] = (int)(up ? got : r[j]);
+              u[j] = (int)(up ? r[16 + j] : got);
+              xs[j] = {__shfl_sync(0xffffffffu, mine2.hi, 16 * up + j), __shfl_sync(0xffffffffu, mine2.lo, 16 * up + j)};
             }
+            close_all(h, g, u, gs16, us16, xs, P.act);
+            float* out = reinterpret_cast<float*>(q.out) + (int64_t)(t.n0 + c + 16 * up) * q.ldo + ch;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (in && c + 16 * up + j < t.nval) out[j * q.ldo] = h[j];
           }
         }
       } else if (mine && q.row) {
@@ -804,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               float cs[32];
               load_row(P.col_scale[0], n, q.cols, P.vec_cols, cs);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * cs[j] * rs;
+              for (int j = 0; j < 32; ++j) v[j] = scaled<kBigI8>((int)r[j], cs[j], rs);
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -819,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
                 float cs[32];
                 load_row(P.col_scale[1], n, q.cols, P.vec_cols, cs);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) u[j] = (float)(int)r[j] * cs[j] * rs;
+                for (int j = 0; j < 32; ++j) u[j] = scaled<kBigI8>((int)r[j], cs[j], rs);
               } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(r[j]);
@@ -926,7 +960,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             if constexpr (IN == kI8) {
               const float rs = c + lane < t.nval ? __ldg(P.row_scale + t.n0 + c + lane) : 0.0f;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * cs * __shfl_sync(0xffffffffu, rs, j);
+              for (int j = 0; j < 32; ++j) v[j] = scaled<kBigI8>((int)r[j], cs, __shfl_sync(0xffffffffu, rs, j));
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -1084,10 +1118,10 @@ int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64
   return r == CUDA_SUCCESS ? DSCA_OK : DSCA_ERR_CUDA;
 }
 
-template <int EPI, int IN, typename O>
+template <int EPI, int IN, typename O, bool CLOSE = false>
 int launch(const Params& P, int pairs, bool pdl, cudaStream_t stream) {
   static PerDeviceOnce once;
-  auto kern = dense_kernel<EPI, IN, O>;
+  auto kern = dense_kernel<EPI, IN, O, CLOSE>;
   if (once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); }) !=
       cudaSuccess)
     return DSCA_ERR_CUDA;
@@ -1157,7 +1191,7 @@ int64_t plan(const Job& j, Params& P, int pairs, size_t* floats, size_t* counter
     q = Prob{};
     const bool glu = j.epi == kGlu;
     q.rows = s.N; q.cols = s.M; q.K = s.K;
-    const int oes = j.row_max != nullptr ? 8 : j.dtype == DSCA_BF16 ? 2 : 4;
+    const int oes = j.dtype == DSCA_BF16 ? 2 : 4;
     auto on = [&](const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
     auto rows_on = [&](int64_t n) {
       return s.ldo * oes % n == 0 && on(s.out, n) && on(j.out2, n) && on(j.save_g, n) && on(j.save_u, n);
@@ -1296,7 +1330,7 @@ int launch_tc(const Job& j, void* parts, void* counts, int32_t* err, bool pdl, c
   using B = __nv_bfloat16;
   if (j.i8) {
     if (j.epi == kGlu)
-      return j.row_max != nullptr ? tc::launch<kGlu, tc::kI8, double>(P, pairs, pdl, stream)
+      return j.row_max != nullptr ? tc::launch<kGlu, tc::kI8, float, true>(P, pairs, pdl, stream)
                                   : tc::launch<kGlu, tc::kI8, float>(P, pairs, pdl, stream);
     return j.dtype == DSCA_BF16 ? tc::launch<kStore, tc::kI8, B>(P, pairs, pdl, stream)
                                 : tc::launch<kStore, tc::kI8, float>(P, pairs, pdl, stream);

@@ -297,8 +297,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
 
     x [..., k] bf16 or fp32; or int8 codes of quantize_rows with their x_scale [...], out_dtype then
     chooses y's type (bf16 by default, otherwise x's type).  Codes lie in [-127, 127].  The products' sum
-    is exact; its conversion to fp32, the products with the channel's and the token's scale and the addition of
-    the bias round to fp32, the result to y's type.  bias [n] of y's type.  Inference only: a backward pass
+    is exact; its conversion to fp32, the products with the two scales and the addition of the bias round to
+    fp32, the result to y's type.  bias [n] of y's type.  Inference only: a backward pass
     that reaches y raises."""
     refuse_tangents("int8_linear", x, bias, x_scale)
     given = x.dtype == torch.int8
@@ -355,9 +355,9 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
                    act: str = "silu") -> torch.Tensor:
     """gated_ffn with its weights in 8-bit integers (pack_int8): x's rows are quantised, the gated
     intermediate is formed and its rows quantised in turn.  x [..., d] bf16 or fp32; y has its shape and
-    type.  fp32 tokens: the intermediate is formed in 64 bits, so that its codes are those of the
-    definition.  bf16 tokens: it is formed in fp32, with gates good to 2^-18 of their value, and a code next
-    to a border may lie on its other side, which moves y by about one of its roundings.  Inference only: a
+    type.  The intermediate is formed in fp32.  fp32 tokens: where that leaves a code open it is formed
+    again in 64 bits, so that all codes are those of the definition.  bf16 tokens: a code next to a border may
+    lie on its other side, which moves y by about one of its roundings.  Inference only: a
     backward pass that reaches y raises."""
     refuse_tangents("gated_ffn_int8", x)
     code = _act(act)
@@ -376,18 +376,17 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     if rows == 0:
         return y
     ld_q, ld_hq = (d + 15) // 16 * 16, (inter + 15) // 16 * 16
-    # one buffer: h (fp32 tokens': in 64 bits, in the workspace), the two sets of codes, the two sets of scales
-    h_bytes = 0 if dt == L.F32 else 4 * ld_hq
-    buf = torch.empty(rows * (h_bytes + ld_hq + ld_q + 8), dtype=torch.uint8, device=dev)
+    # one buffer: h, the two sets of codes, the two sets of scales
+    buf = torch.empty(rows * (5 * ld_hq + ld_q + 8), dtype=torch.uint8, device=dev)
     h = buf.data_ptr()
-    hq = h + rows * h_bytes
+    hq = h + rows * 4 * ld_hq
     q = hq + rows * ld_hq
     scale = q + rows * ld_q
     a = L.GatedFfnInt8Args(x.data_ptr(), q, scale, w_gate[0].data_ptr(), w_up[0].data_ptr(), w_down[0].data_ptr(),
                            w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr(), h, hq, scale + 4 * rows,
                            y.data_ptr(), rows, d, inter, dt, code, ld_x, ld_q, ld_gate, ld_up, ld_down, ld_hq, ld_hq, d,
                            None, 0, _err(dev))
-    if dt == L.F32 or not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
+    if not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
         ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
     return without_gradient("gated_ffn_int8", y, x, w_gate[1], w_up[1], w_down[1])

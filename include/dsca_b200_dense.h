@@ -31,7 +31,7 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 #define DSCA_DENSE_MAX_DIM 1048576
 #define DSCA_DENSE_MAX_ROWS 16777216
 /* Forward calls need no workspace for at most this many rows, where the weights of each of their products (gate and up
- * together) have at most that many bytes; but dsca_gated_ffn_int8 with DSCA_F32 always takes one. */
+ * together) have at most that many bytes. */
 #define DSCA_DENSE_FEW_TOKENS 8
 #define DSCA_DENSE_FEW_BYTES 50331648
 
@@ -104,8 +104,8 @@ typedef struct {
 } dsca_quantize_rows_args;
 
 /*
- * y = (q w^T) * w_scale[column] * scale[row] (+ bias): the sum exact in 32-bit integers, its conversion and the products and
- * the addition, in this order, in fp32, the result rounded to dtype.  With x, q and scale are work areas that dsca_quantize_rows of x fills first.
+ * y = (q w^T) * w_scale[column] * scale[row] (+ bias): the sum exact in 32-bit integers, its conversion, the products with the
+ * smaller and the larger scale and the addition, in this order, in fp32, the result rounded to dtype.  With x, q and scale are work areas that dsca_quantize_rows of x fills first.
  */
 typedef struct {
   const void* x;        /* [rows, k], dtype, or NULL: q and scale are given */
@@ -123,21 +123,22 @@ typedef struct {
 } dsca_int8_linear_args;
 
 /*
- * dsca_gated_ffn with its weights in 8-bit integers: x quantised by rows, h = act(g) * u, quantised by rows, then the down
- * product.  DSCA_F32: h in 64 bits (in the workspace), from the exact sums and the scale max|x| / 127 unrounded.  DSCA_BF16: h in
- * fp32 (a work area), its gate good to 2^-18, so that a code next to a border may lie on its other side.
+ * dsca_gated_ffn with its weights in 8-bit integers: x quantised by rows, h = act(g) * u in fp32 (a work area), quantised by
+ * rows, then the down product.  DSCA_F32: the codes of h are those of its 64-bit value (from the exact sums and the scale
+ * max|x| / 127 unrounded).  DSCA_BF16: they are those of the fp32 value, whose gate is good to 2^-18, so that a code next to a border
+ * may lie on its other side.
  */
 typedef struct {
   const void* x;        /* [rows, d], dtype */
   int8_t* q;            /* work area [rows, ld_q] */
-  float* scale;         /* work area [rows] */
+  float* scale;         /* work area [rows] (DSCA_BF16: the rows' scales, DSCA_F32: their largest magnitudes) */
   const int8_t* w_gate; /* [inter, ld_gate], 16-byte aligned; columns past d do not count */
   const int8_t* w_up;
   const int8_t* w_down; /* [d, ld_down] */
   const float* gate_scale; /* [inter] */
   const float* up_scale;
   const float* down_scale; /* [d] */
-  float* h;             /* work area [rows, ld_h], DSCA_F32: not touched */
+  float* h;             /* work area [rows, ld_h] */
   int8_t* hq;           /* work area [rows, ld_hq] */
   float* h_scale;       /* work area [rows] */
   void* y;              /* [rows, d], dtype */

@@ -31,20 +31,22 @@ def test_int8_partial_tiles(cuda, T, k, n):
 
 def _ffn_int8_defined(x, wg, wu, wd, name):
     """(value, bound) of the block on fp32 tokens with the codes of the intermediate in 64 bits and no allowance at their borders.
-    The row's scale, the sum's conversion and two products round once each, 2^-24 of the value."""
+    The row's largest is off by 16 units of 2^-24 at most (the gate's exponential 5, 1 + e 1, its reciprocal 2, their product 1, the
+    product with g 2, u 4, h 1) where no code hangs on it, its scale rounds once; the sum's conversion and two products 3."""
     q, s = R.codes(x.double())
     g, u = ((q @ w.q.double().T) * s[:, None] * w.scale.double() for w in (wg, wu))
     hq, hs = R.codes(R.act(g, name)[0] * u)
     y = (hq @ wd.q.double().T) * hs[:, None] * wd.scale.double()
-    return y, 4.1 * 2.0 ** -24 * y.abs()
+    return y, 20.1 * 2.0 ** -24 * y.abs()
 
 
 @pytest.mark.parametrize("name", R.ACTS)
 @pytest.mark.parametrize("T,d,I", [(1, 2048, 5632), (1, 8, 3), (7, 264, 1021), (12, 768, 2048), (16, 1000, 520), (24, 2048, 1408), (40, 512, 2050),
-                                   (128, 320, 264), (300, 777, 1000), (2800, 2000, 843), (1500, 256, 2056), (5000, 64, 520)])
+                                   (128, 320, 264), (300, 777, 1000), (2800, 2000, 843), (1500, 256, 2056), (5000, 64, 520),
+                                   (3, 64, 9001), (700, 40, 8300), (1300, 2048, 5632), (900, 520, 1000)])
 def test_int8_block_codes_of_f32_tokens(cuda, T, d, I, name):
     """fp32 tokens: every code of the intermediate is that of the 64-bit definition (a single one on the other side of its
-    border moves that token's y by hundreds of the bounds)."""
+    border moves some of that token's y by many of the bounds)."""
     from dsca_moe_b200 import check_dense, gated_ffn_int8, pack_int8
 
     randn = _randn(cuda, T + d + I)
@@ -329,3 +331,34 @@ def test_error_word_is_there_before_its_address_is(cuda, monkeypatch):
         torch.cuda._sleep(400_000_000)
         D._err(torch.device("cuda", torch.cuda.current_device()))
         assert stream.query()
+
+
+@pytest.mark.parametrize("T,inter", [(3, 40), (5, 1300), (700, 40)])
+def test_int8_block_of_f32_tokens_equal_and_tiny_values(cuda, T, inter):
+    """Rows whose values are all the largest, or all on a border of two codes, or all below fp32's normal numbers in between."""
+    from dsca_moe_b200 import Int8Weight, gated_ffn_int8, pack_int8
+
+    randn = _randn(cuda, T)
+    down = pack_int8(randn(64, inter))
+    x = randn(T, 64)
+    same = pack_int8(torch.ones(inter, 64, device=cuda))
+    R.close(gated_ffn_int8(x, same, same, down), _ffn_int8_defined(x, same, same, down, "silu"))
+    # u = 1 and g from 1 to 127 half steps of the largest: 127 h / max|h| = n + 1 / 2 for odd ones
+    q = torch.zeros(inter, 64, dtype=torch.int8, device=cuda)
+    q[:, 0] = torch.arange(inter, device=cuda) % 127 + 1
+    ones = torch.ones(inter, device=cuda)
+    x = torch.zeros(T, 64, device=cuda)
+    x[:, 0] = 1
+    q2 = q.clone()
+    q2[:, 0] = 1
+    q[0, 0] = 127
+    half = torch.where(torch.arange(inter, device=cuda) > 0, 0.5, 1.0).float()
+    gate, up = Int8Weight(q, half), Int8Weight(q2, ones)
+    R.close(gated_ffn_int8(x, gate, up, down, act="relu"), _ffn_int8_defined(x, gate, up, down, "relu"))
+    for scale in (1e-18, 1e-12):  # h near 1e-36 and 1e-24 beside a gate and up of 1e-18 and 1e-12
+        wide = Int8Weight(down.q, down.scale / scale / scale)
+        w = [pack_int8(randn(inter, 64)) for _ in range(2)]
+        for name in R.ACTS:
+            x = randn(T, 64) * scale
+            y, ref = gated_ffn_int8(x, *w, wide, act=name), _ffn_int8_defined(x, *w, wide, name)
+            R.close(y, (ref[0], ref[1] * (1 if scale > 1e-15 else 2 ** 6)), (scale, name))
