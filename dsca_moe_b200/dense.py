@@ -61,11 +61,12 @@ def _act(act: str) -> int:
 
 def _rows(x, name: str, width: int | None = None):
     """(rows, row stride) of x [..., width] on a GPU."""
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"{name} must be on a GPU")
-    if x.dim() == 0 or x.shape[-1] == 0 or (width is not None and x.shape[-1] != width):
-        raise ValueError(f"{name}: expected [..., {'d' if width is None else width}] rows, got {tuple(x.shape)}")
-    d = x.shape[-1]
+    shape = x.shape
+    if not shape or shape[-1] == 0 or (width is not None and shape[-1] != width):
+        raise ValueError(f"{name}: expected [..., {'d' if width is None else width}] rows, got {tuple(shape)}")
+    d = shape[-1]
     if d > L.DENSE_MAX_DIM:
         raise ValueError(f"{name}: rows of {d} values exceed {L.DENSE_MAX_DIM}")
     rows = x.numel() // d
@@ -74,9 +75,9 @@ def _rows(x, name: str, width: int | None = None):
     return rows, (d if x.is_contiguous() or rows == 0 else _stride(x, name, d))
 
 
-def _weight(w, name: str, out: int, inp: int, x) -> int:
+def _weight(w, name: str, out: int, inp: int, x, dtype, index: int) -> int:
     """Row stride of a weight [out, inp] of x's type on x's device."""
-    if w.shape == (out, inp) and w.dtype is x.dtype and w.device == x.device and w.is_contiguous():
+    if w.is_contiguous() and w.shape == (out, inp) and w.dtype is dtype and w.get_device() == index:
         return inp
     if w.dim() != 2 or w.shape[0] != out or w.shape[1] != inp:
         raise ValueError(f"{name}: expected [{out}, {inp}], got {tuple(w.shape)}")
@@ -137,8 +138,6 @@ def _as_saved(t, name: str, shape, dtype, index: int):
     in other strides than it was saved with, and a gradient comes in any (expanded, transposed)."""
     if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
         raise RuntimeError(f"{name} came back as {t.dtype} {tuple(t.shape)} on {t.device}, not {dtype} {tuple(shape)} on GPU {index}")
-    if t.is_contiguous():
-        return t, shape[-1]
     try:
         return t, _stride(t, name, shape[-1])
     except ValueError:
@@ -167,11 +166,20 @@ class _GatedFFN(torch.autograd.Function):
         dx_p, dwg_p, dwu_p, dwd_p = [None if t is None else t.data_ptr() for t in (dx, dwg, dwu, dwd)]
         if rows:
             i, x_shape = dy.get_device(), ctx.x_shape
-            dy, ld_dy = _as_saved(dy, "dy", x_shape, dtype, i)
-            x, ld_x = _as_saved(x, "x", x_shape, dtype, i)
-            wg, ld_g = _as_saved(wg, "w_gate", (inter, d), dtype, i)
-            wu, ld_u = _as_saved(wu, "w_up", (inter, d), dtype, i)
-            wd, ld_d = _as_saved(wd, "w_down", (d, inter), dtype, i)
+            ld_dy = d
+            if not dy.is_contiguous():
+                dy, ld_dy = _as_saved(dy, "dy", x_shape, dtype, i)
+            # the usual case first: as they were saved
+            ld_x = ld_g = ld_u = d
+            ld_d, up = inter, (inter, d)
+            if not (x.is_contiguous() and x.shape == x_shape and x.dtype is dtype and x.get_device() == i):
+                x, ld_x = _as_saved(x, "x", x_shape, dtype, i)
+            if not (wg.is_contiguous() and wg.shape == up and wg.dtype is dtype and wg.get_device() == i):
+                wg, ld_g = _as_saved(wg, "w_gate", up, dtype, i)
+            if not (wu.is_contiguous() and wu.shape == up and wu.dtype is dtype and wu.get_device() == i):
+                wu, ld_u = _as_saved(wu, "w_up", up, dtype, i)
+            if not (wd.is_contiguous() and wd.shape == (d, inter) and wd.dtype is dtype and wd.get_device() == i):
+                wd, ld_d = _as_saved(wd, "w_down", (d, inter), dtype, i)
             ld_h, step, size = _saved(rows, inter, dtype)
             grads = torch.empty(2 * step, dtype=torch.uint8, device=dev)
             h, dg = buf.data_ptr(), grads.data_ptr()
@@ -200,18 +208,18 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     gradients in the backward pass.  Under autograd the call keeps the intermediate, the gate and the up
     values, each [rows, inter] (the latter two to 11 bits for bf16), for the backward pass; second derivatives and forward-mode
     ones are not offered.  Runs on x's device, on its current stream; check_dense() reports a wait that ran out."""
-    code = _act(act)
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"unsupported dtype {x.dtype}")
+    code, dtype = _act(act), x.dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {dtype}")
     rows, ld_x = _rows(x, "x")
-    d = x.shape[-1]
+    d, i = x.shape[-1], x.get_device()
     if w_gate.dim() != 2 or w_gate.shape[0] == 0:
         raise ValueError(f"w_gate: expected [inter, {d}], got {tuple(w_gate.shape)}")
     inter = w_gate.shape[0]
     if inter > L.DENSE_MAX_DIM:
         raise ValueError(f"w_gate: {inter} rows exceed {L.DENSE_MAX_DIM}")
-    shapes = (rows, d, inter, ld_x, _weight(w_gate, "w_gate", inter, d, x), _weight(w_up, "w_up", inter, d, x),
-              _weight(w_down, "w_down", d, inter, x))
+    shapes = (rows, d, inter, ld_x, _weight(w_gate, "w_gate", inter, d, x, dtype, i),
+              _weight(w_up, "w_up", inter, d, x, dtype, i), _weight(w_down, "w_down", d, inter, x, dtype, i))
     refuse_tangents("gated_ffn", x, w_gate, w_up, w_down)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
                                     or w_down.requires_grad):
@@ -269,8 +277,9 @@ def _int8_weight(w, name: str, dev, inp: int, out: int | None = None) -> int:
     """Row stride of an Int8Weight."""
     q, s = w
     shape = q.shape
+    index = dev.index
     if q.dtype is torch.int8 and len(shape) == 2 and shape[1] == inp and (out is None or shape[0] == out) \
-            and q.device == dev and s.device == dev and s.dtype is torch.float32 and s.shape == shape[:1] \
+            and q.get_device() == index and s.get_device() == index and s.dtype is torch.float32 and s.shape == shape[:1] \
             and s.is_contiguous() and shape[0] > 1:
         ld, last = q.stride()
         if (last == 1 or inp == 1) and ld >= inp and ld % 16 == 0 and q.data_ptr() % 16 == 0:
