@@ -10,6 +10,8 @@
 //
 // A row is read once (up to 8192 values; longer rows are read a second time from L2).  16384 x 5632 bf16 43 us (6.4
 // TB/s, a copy's rate), 4096 x 5632 fp32 20.5 us (5.6 TB/s), one row 2.5 us.
+//
+// The intermediate of an 8-bit block on fp32 tokens takes the codes of its 64-bit value, although it comes in fp32 (kH, settle_kernel).
 #include "dense.cuh"
 
 #include <algorithm>
@@ -37,7 +39,7 @@ __device__ __forceinline__ float settled(float r, float toward, float x, float a
 // bf16: x = X 2^a and amax = M 2^b with X and M from 128 to 255 (the quotient 127 X 2^e / M with e = a - b <= 0), so a
 // border (2 j + 1) / 2 that is not the quotient is at least 2^e / (2 M) away from it, 1 / (254 X) > 2^-16 of it.  The product
 // rounded to 19 bits, off by 2^-19 more, lies on the same side; and borders below 128, with their 8 bits, are among
-// the 19-bit numbers, the nearest to products 2^-23 off.  (p - (33 p - 32 p), each step rounded: 24 - 5 bits.)
+// the 19-bit numbers, the nearest to products 2^-23 off.  (Veltkamp's splitting: 33 p - (33 p - p), each step rounded, 24 - 5 bits.)
 //
 // fp32: only values within 2^-16 of a tie need the exact comparison; where one of the eight does, all take it.
 template <typename T>

@@ -86,11 +86,6 @@ def _weight(w, name: str, out: int, inp: int, x, dtype, index: int) -> int:
     return inp if w.is_contiguous() else _stride(w, name, inp)
 
 
-def _few(rows: int, weight_bytes: int) -> bool:
-    """Whether a call needs no workspace whatever its alignment (include/dsca_b200_dense.h)."""
-    return rows <= L.DENSE_FEW_TOKENS and weight_bytes <= L.DENSE_FEW_BYTES
-
-
 def _workspace(name: str, args, dev):
     """The call's workspace, allocated on the current stream, in args."""
     fn = getattr(L._LIB or L.load(), name)
@@ -119,7 +114,7 @@ def _forward(x, wg, wu, wd, act: int, shapes, save: bool):
     g, u, e = (h + step, h + 2 * step, h + 3 * step) if save else (None, None, None)
     a = L.GatedFfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr(), g, u, e, h, rows, d, inter,
                        _DTYPES[dtype], act, ld_x, ld_g, ld_u, ld_d, d, ld_h, None, 0, _err(dev))
-    if not _few(rows, 2 * inter * d * x.element_size()):
+    if rows > L.DENSE_FEW_TOKENS:  # others need none
         ws = _workspace("dsca_gated_ffn_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn", ctypes.byref(a))
     return y, buf
@@ -354,7 +349,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     a = L.Int8LinearArgs(x_p, q_p, s_p, weight[0].data_ptr(), weight[1].data_ptr(),
                          None if bias is None else bias.data_ptr(), y.data_ptr(), rows, k, n, dt, ld_x, ld_q, ld_w, n,
                          None, 0, _err(dev))
-    if not _few(rows, n * ld_w):
+    if rows > L.DENSE_FEW_TOKENS:
         ws = _workspace("dsca_int8_linear_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_int8_linear", ctypes.byref(a))
     return without_gradient("int8_linear", y, x, bias, x_scale, weight[1])
@@ -366,7 +361,7 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
     intermediate is formed and its rows quantised in turn.  x [..., d] bf16 or fp32; y has its shape and
     type.  The intermediate is formed in fp32.  fp32 tokens: where that leaves a code open it is formed
     again in 64 bits, so that all codes are those of the definition.  bf16 tokens: a code next to a border may
-    lie on its other side, which moves y by about one of its roundings.  Inference only: a
+    lie on its other side, which moves y by one code's worth of that channel.  Inference only: a
     backward pass that reaches y raises."""
     refuse_tangents("gated_ffn_int8", x)
     code = _act(act)
@@ -395,7 +390,7 @@ def gated_ffn_int8(x: torch.Tensor, w_gate: Int8Weight, w_up: Int8Weight, w_down
                            w_gate[1].data_ptr(), w_up[1].data_ptr(), w_down[1].data_ptr(), h, hq, scale + 4 * rows,
                            y.data_ptr(), rows, d, inter, dt, code, ld_x, ld_q, ld_gate, ld_up, ld_down, ld_hq, ld_hq, d,
                            None, 0, _err(dev))
-    if not _few(rows, max(2 * inter * ld_gate, d * ld_down)):
+    if rows > L.DENSE_FEW_TOKENS:
         ws = _workspace("dsca_gated_ffn_int8_workspace", a, dev)  # noqa: F841 - alive until the launch
     L.call_on(dev, "dsca_gated_ffn_int8", ctypes.byref(a))
     return without_gradient("gated_ffn_int8", y, x, w_gate[1], w_up[1], w_down[1])

@@ -10,7 +10,11 @@
  * dsca_gated_ffn_int8       the gated block with 8-bit integer weights
  *
  * DSCA_F32 products hold every value as three bf16 terms, 24 bits in all; magnitudes below 2^-100 keep fewer (the third
- * term becomes subnormal), which is below 2^-116 in absolute terms.
+ * term becomes subnormal), which is below 2^-116 in absolute terms.  An infinite value makes its sums NaN (a term of it meets
+ * zero terms of the other side).
+ *
+ * 16-bit sums of one sign are off by up to 2^-11 of themselves before they are rounded (the tensor cores' additions truncate;
+ * every 65536 of k they are added up in rounded fp32).
  *
  * Matrices are row-major with row strides in elements (ld_*, at least the width) and a contiguous
  * last dimension; weights lie as a Linear layer holds them, [out, in].  Any sizes; rows on 16-byte
@@ -30,8 +34,8 @@ enum { DSCA_GATE_SILU = 0, DSCA_GATE_GELU = 1 /* tanh form */, DSCA_GATE_RELU = 
 /* Largest width (d, inter, k, n) and number of rows of these entry points. */
 #define DSCA_DENSE_MAX_DIM 1048576
 #define DSCA_DENSE_MAX_ROWS 16777216
-/* Forward calls need no workspace for at most this many rows, where the weights of each of their products (gate and up
- * together) have at most that many bytes. */
+/* Forward calls need no workspace for at most this many rows, whatever the sizes of their weights.  (The bytes are those up to
+ * which the calls promised it before.) */
 #define DSCA_DENSE_FEW_TOKENS 8
 #define DSCA_DENSE_FEW_BYTES 50331648
 

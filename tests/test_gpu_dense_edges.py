@@ -362,3 +362,23 @@ def test_int8_block_of_f32_tokens_equal_and_tiny_values(cuda, T, inter):
             x = randn(T, 64) * scale
             y, ref = gated_ffn_int8(x, *w, wide, act=name), _ffn_int8_defined(x, *w, wide, name)
             R.close(y, (ref[0], ref[1] * (1 if scale > 1e-15 else 2 ** 6)), (scale, name))
+
+
+def test_eight_tokens_of_large_weights(cuda):
+    """Calls of at most eight rows take no workspace, whatever the weights' size."""
+    import ctypes
+
+    from dsca_moe_b200 import _lib as L
+    from dsca_moe_b200 import gated_ffn, int8_linear, pack_int8, quantize_rows
+
+    randn = _randn(cuda, 9)
+    x = randn(8, 2048).to(BF16)
+    wg, wu, wd = ((randn(*s) * s[1] ** -0.5).to(BF16) for s in ((13000, 2048), (13000, 2048), (2048, 13000)))
+    R.close(gated_ffn(x, wg, wu, wd), R.ffn(x, wg, wu, wd, "silu", BF16)["y"])
+    w = pack_int8(torch.cat([wg, wu, wg]))
+    q, s = quantize_rows(x)
+    R.close(int8_linear(x, w), R.int8_linear(q, s, w.q, w.scale, BF16))
+    y = torch.empty(8, 39000, dtype=BF16, device=cuda)
+    a = L.Int8LinearArgs(None, q.data_ptr(), s.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(), None, y.data_ptr(), 8, 2048, 39000,
+                         L.BF16, 2048, 2048, 2048, 39000, None, 0, None)
+    assert L.load().dsca_int8_linear_workspace(ctypes.byref(a)) == 0
