@@ -124,9 +124,12 @@ def prepare(case, seed):
             s["dy"] = n(T, d, std=0.1)
     if case["kind"] in ("int8", "ffn8"):
         if own:
-            from dsca_moe_b200 import pack_int8
+            from dsca_moe_b200 import Int8Weight, pack_int8
 
-            s["w"] = {key: pack_int8(v) for key, v in w.items()}  # a serving program's weights
+            # a serving program's weights, with the scales that the plain form has: _codes divides on the GPU, where torch
+            # multiplies by 1 / 127, so that they may be a step from pack_int8's, and a code of the intermediate
+            # next to a border hangs on it
+            s["w"] = {key: Int8Weight(pack_int8(v).q, _packed(v)[1]) for key, v in w.items()}
         else:
             s["w"] = {key: _packed(v) for key, v in w.items()}
         return s
