@@ -310,8 +310,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 0 : NT == 2 ? 4 : 2) fe
     float v = (float)va, u = (float)vb;
     if constexpr (std::is_same<T, int8_t>::value) {
       const float rs = p.row_scale[n];
-      v = in ? scaled<true>(va, p.col_scale[0][m], rs) : 0.0f;
-      if constexpr (kGluE) u = in ? scaled<true>(vb, p.col_scale[1][m], rs) : 0.0f;
+      constexpr bool kBigI8 = !kGluE && sizeof(O) == 4;  // as in the other kernel
+      v = in ? scaled<kBigI8>(va, p.col_scale[0][m], rs) : 0.0f;
+      if constexpr (kGluE) u = in ? scaled<kBigI8>(vb, p.col_scale[1][m], rs) : 0.0f;
     }
     if constexpr (kGluE) {
       if (p.save_g != nullptr) {

@@ -744,6 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           for (int c = 32 * eh; c < t.nval; c += c % 32 == 16 ? 48 : 16) {  // alternate chunks of 32
             const int n = t.n0 + c;
             uint32_t g[16], u[16];
+            __syncwarp();
             finished16(c, g);
             finished16(c + q.tn / 2, u);
             float gs[16], us[16], h[16];
@@ -768,18 +769,19 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             for (int j = 0; j < 16; ++j) x16[j] = xs;
             tmem_wait_ld();
             close_all(h, reinterpret_cast<const int(&)[16]>(g), reinterpret_cast<const int(&)[16]>(u), gs, us, x16, P.act);
-            if (!live) continue;
+            if (live) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 8) {
-              if (q.vec == 2 && n + i + 8 <= q.cols) {
-                uint32_t w[8];
+              for (int i = 0; i < 16; i += 8) {
+                if (q.vec == 2 && n + i + 8 <= q.cols) {
+                  uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(h[i + j]);
-                store32(out + n + i, w);
-              } else {
+                  for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(h[i + j]);
+                  store32(out + n + i, w);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (n + i + j < q.cols) out[n + i + j] = h[i + j];
+                  for (int j = 0; j < 8; ++j)
+                    if (n + i + j < q.cols) out[n + i + j] = h[i + j];
+                }
               }
             }
           }

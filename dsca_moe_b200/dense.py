@@ -202,7 +202,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     Products are summed in fp32; the gated intermediate is rounded to x's type, and so are its two
     gradients in the backward pass.  Under autograd the call keeps the intermediate, the gate and the up
     values, each [rows, inter] (the latter two to 11 bits for bf16), for the backward pass; second derivatives and forward-mode
-    ones are not offered.  Runs on x's device, on its current stream; check_dense() reports a wait that ran out."""
+    ones are not offered.  Autocast does not apply (GatedFFN follows it).  Runs on x's device, on its current stream; check_dense() reports a wait that ran out."""
     code, dtype = _act(act), x.dtype
     if dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {dtype}")

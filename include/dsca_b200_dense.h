@@ -108,8 +108,9 @@ typedef struct {
 } dsca_quantize_rows_args;
 
 /*
- * y = (q w^T) * w_scale[column] * scale[row] (+ bias): the sum exact in 32-bit integers, its conversion, the products with the
- * smaller and the larger scale and the addition, in this order, in fp32, the result rounded to dtype.  With x, q and scale are work areas that dsca_quantize_rows of x fills first.
+ * y = (q w^T) * w_scale[column] * scale[row] (+ bias): the sum exact in 32-bit integers, its conversion, the products with the two
+ * scales and the addition in fp32, the result rounded to dtype.  DSCA_F32: the smaller scale first; DSCA_BF16: the column's
+ * first, so that a column's scale above 2^97 may make y infinite where the row's would bring it back.  With x, q and scale are work areas that dsca_quantize_rows of x fills first.
  */
 typedef struct {
   const void* x;        /* [rows, k], dtype, or NULL: q and scale are given */
